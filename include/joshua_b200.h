@@ -339,6 +339,128 @@ int32_t jq_sample_greedy_dev(const float* logits, uint64_t rows, uint64_t vocab,
                              int32_t* window, int32_t* window_state, int32_t* token, int32_t* pos, void* scratch,
                              void* stream);
 
+/* ── serving many sequences: rotary positions, a paged cache in few bits, attention over it, sampling ──
+ * The steps around the quantized products when a batch of long sequences is
+ * served: they stand in for the rope, the `Tensor::cat` of the KV cache, the
+ * attention (src/quantized_qwen3_moe.rs:330-386) and the temperature branch of
+ * `sample_token` (src/engine.rs:2339-2378), with the cache in pages and in
+ * fewer bits than the reference keeps it in.  f32 activations, device buffers,
+ * a caller stream, no synchronisation, no allocation: all can be captured in a
+ * graph.  Rows are 16-byte aligned.
+ *
+ * Rotary positions come from a table of pairs, table[p][i] = m (cos, sin)(p f_i),
+ * i < rot_dim / 2, which jq_rope_table_dev builds (in 64 bits, rounded once):
+ *   f_i = theta^(-2 i / rot_dim) / freq_factors[i]   (host array, NULL: ones; a
+ *   GGUF file's `rope_freqs.weight`), then by `scaling`:
+ *   NONE    as it is; LINEAR  f_i / factor;
+ *   YARN    f_i (1 - r_i) / factor + f_i r_i, r_i = 1 below pair `low`, 0 above pair
+ *           `high`, linear between; low and high are where orig_ctx positions make
+ *           beta_fast and beta_slow turns, rounded outwards
+ *           (src/quantized_deepseek2.rs:243-300).
+ * `mscale` m scales both (0: 1; YaRN files that want 0.1 ln(factor) + 1 pass it).
+ * The first rot_dim <= 256 dimensions of a head turn, the others pass. */
+#define JQ_ROPE_NONE 0
+#define JQ_ROPE_LINEAR 1
+#define JQ_ROPE_YARN 2
+typedef struct {
+    double theta;
+    int32_t scaling; /* JQ_ROPE_* */
+    float factor;    /* > 0 with a scaling */
+    uint32_t orig_ctx;
+    float beta_fast, beta_slow; /* YARN: 32 and 1 in the reference */
+    float mscale;
+} jq_rope_config;
+int32_t jq_rope_table_dev(const jq_rope_config* cfg, const float* freq_factors, uint32_t rot_dim, uint32_t n_pos,
+                          float* table_dev, void* stream);
+
+typedef struct {
+    const float* table; /* device, [n_pos][rot_dim / 2][2] */
+    uint32_t n_pos;
+    uint32_t rot_dim;    /* even */
+    int32_t interleaved; /* 0: pairs (i, i + rot_dim / 2); 1: pairs (2 i, 2 i + 1) */
+} jq_rope;
+
+/* out = x with the `heads` heads of every row turned to its position: (a cos - b sin, a sin + b cos), each operation
+ * rounded by itself.  inverse != 0 turns back, which is also the gradient's way through (for m = 1).  Rows are x_stride and
+ * out_stride floats apart, heads of a row one after another; out may be x.  A row whose position is negative or >= n_pos
+ * is left as it was and *bad_pos_dev (may be NULL) set to 1. */
+int32_t jq_rope_dev(const jq_rope* rope, const float* x, uint64_t x_stride, const int32_t* pos, uint32_t rows, uint32_t heads,
+                    uint32_t head_dim, int32_t inverse, float* out, uint64_t out_stride, int32_t* bad_pos_dev, void* stream);
+
+/* A cache of pages of JQ_KV_PAGE positions (keys and values of all kv heads), jq_kv_page_bytes bytes each, one after another
+ * from a 16-byte boundary on.  The caller hands pages out: position p of sequence i is in page
+ * page_table[i * table_stride + p / JQ_KV_PAGE] (device int32), so table_stride * JQ_KV_PAGE positions at most.  Sequences
+ * may name the same page; whoever appends to it then writes for all.  Pages need no clearing before use.
+ *   type      JQ_KV_F16: halves (finite values past +-65504 saturate);
+ *             JQ_KV_Q8_0: blocks of 32 dimensions, d = f16(max |x| / 127), code = rint(x / d);
+ *             JQ_KV_Q4_0: d = f16(m / -8), m the block's value of largest magnitude (the negative one of two equal ones),
+ *             code = rint(x / d) in [-8, 7].
+ *             The GGUF block types' values in an order of their own.  A block (JQ_KV_F16: a value) that is not finite reads
+ *             back as NaN.
+ *   head_dim  64, 128 or 256 */
+#define JQ_KV_PAGE 64
+#define JQ_KV_F16 1u
+#define JQ_KV_Q4_0 2u
+#define JQ_KV_Q8_0 8u
+typedef struct {
+    uint32_t type;
+    uint32_t n_kv;
+    uint32_t head_dim;
+    uint32_t n_pages;
+    void* pages; /* device */
+} jq_kv_cache;
+uint64_t jq_kv_page_bytes(uint32_t type, uint32_t n_kv, uint32_t head_dim); /* 0: not supported */
+
+/* New positions: row i of qkv ([n_q + 2 n_kv, head_dim], rows qkv_stride floats apart) belongs to position pos[i] of sequence
+ * seq[i] (NULL: sequence i).  Queries and keys take the optional per-head RMS norm (both weights or none) and the rotation
+ * (rope NULL: none); queries go to q_out [rows, n_q, head_dim], keys and values into the cache.  A row without a place (a
+ * sequence outside [0, n_seq), a position outside the page table or the rope table, a page id outside the cache) stores
+ * nothing and sets *bad_pos_dev (may be NULL) to 1.  Two rows of one call must not name the same place. */
+int32_t jq_kv_append_dev(const jq_kv_cache* cache, const jq_rope* rope, const float* qkv, uint64_t qkv_stride, const int32_t* pos,
+                         const int32_t* seq, const int32_t* page_table, uint32_t n_seq, uint32_t table_stride, uint32_t rows,
+                         uint32_t n_q, const float* q_norm_w, const float* k_norm_w, float qk_eps, float* q_out,
+                         int32_t* bad_pos_dev, void* stream);
+
+/* Positions back as f32: row i (as above) of head h goes to k_out and v_out + h * head_stride + i * row_stride.  A row
+ * without a place is NaN and sets *bad_pos_dev.  With row_stride = head_dim this is the cache that
+ * jq_attention_prefill_dev reads. */
+int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32_t* seq, const int32_t* page_table, uint32_t n_seq,
+                       uint32_t table_stride, uint32_t rows, float* k_out, float* v_out, uint64_t row_stride, uint64_t head_stride,
+                       int32_t* bad_pos_dev, void* stream);
+
+/* Attention of one new token per sequence: out[b, h] = softmax(scale q[b, h] . K[0 .. len[b]) ^T) V, query head h on kv head
+ * h / (n_q / n_kv); scale 0: 1 / sqrt(head_dim).  q and out rows are q_stride and out_stride floats apart.  len[b] = 0: zeros.
+ *   shared_pages: the first so many pages are the same for the whole batch (a common prompt): read from the first sequence's
+ * table entries, once for all.  Every len is then 0 or at least shared_pages * JQ_KV_PAGE.
+ *   A len outside its range or a page id outside the cache makes the sequence's rows NaN and sets *bad_pos_dev.
+ *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, ZEROED once before the first
+ * call (it holds arrival counters that the kernels leave at zero); one call at a time. */
+uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t table_stride,
+                                          uint32_t shared_pages);
+int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* len,
+                               const int32_t* page_table, uint32_t batch, uint32_t table_stride, uint32_t n_q, float scale,
+                               uint32_t shared_pages, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos_dev,
+                               void* stream);
+
+/* One token of every row of logits, drawn with a given random number: `sample_token` at temperature > 0
+ * (src/engine.rs:2339-2378) with the usual rules, each row its own (device arrays of `rows`, each may be NULL).
+ *   weight of a token: w = rint(2^32 e), e = exp((l - max) / temperature), a whole number; NaN and -inf weigh nothing.
+ *   Tokens in order of logit, equal ones lower id first; kept is the shortest of the runs that
+ *   top_k (<= 0: off)   the first top_k,
+ *   top_p (>= 1: off)   those of the top_k run with less than max(1, trunc(top_p W)) in front of them, W the run's weight,
+ *   min_p (<= 0: off)   those with e >= min_p
+ *   keep.  token: the first id at which the kept weights, summed in order of ids, pass trunc(uniform W'), W' their sum;
+ *   prob (may be NULL): its weight / W'.  A row that keeps nothing (all -inf or NaN): token -1, prob 0.
+ *   temperature <= 0: the maximum, its lowest id.  NULL: 1.
+ * The sums are exact, so a row's token does not depend on the batch or the launch.  uniform: in [0, 1).
+ * repetition_penalty, window and window_state as for jq_sample_greedy_dev; pos (may be NULL) is advanced by one per row.
+ * logits: rows row_stride floats apart, read only; vocab <= JQ_SAMPLE_MAX_VOCAB. */
+#define JQ_SAMPLE_MAX_VOCAB 393216u
+int32_t jq_sample_dev(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float* uniform,
+                      const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                      float repetition_penalty, int32_t* window, int32_t* window_state, int32_t* token, float* prob, int32_t* pos,
+                      void* stream);
+
 /* ── MoE layer ───────────────────────────────────────────────────────────
  * Replaces `Moe::forward` of the three loaders: routing, per-expert gather,
  * SwiGLU MLP over quantized expert banks, weighted scatter-add, optional
