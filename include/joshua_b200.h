@@ -435,8 +435,8 @@ int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32
  *   A len outside its range or a page id outside the cache makes the sequence's rows NaN and sets *bad_pos_dev.
  *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, ZEROED once before the first
  * call (it holds arrival counters that the kernels leave at zero); one call at a time. */
-uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t table_stride,
-                                          uint32_t shared_pages);
+#define JQ_ATTENTION_MAX_BATCH 4096u
+uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t shared_pages);
 int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* len,
                                const int32_t* page_table, uint32_t batch, uint32_t table_stride, uint32_t n_q, float scale,
                                uint32_t shared_pages, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos_dev,

@@ -1,123 +1,826 @@
 // Attention of one new token per sequence over the pages of the quantised cache.
 //
-// out[b, head, :] = sum_t p_t V_t / sum_t p_t with p_t = exp(scale q . K_t - max), t = 0 .. len[b] - 1.  Pages are independent:
-// one CTA a page and query head gives the page's sum with its own maximum, a second kernel joins them in order.
+// out[b, head, :] = sum_t p_t V_t / sum_t p_t, p_t = 2^(s_t - max), s_t = scale log2(e) q . K_t, t = 0 .. len[b] - 1, in one
+// pass with a running maximum and sum.  A warp takes STEP positions of a kv head and all query rows that share it:
+//   scores   S^T = K Q^T as m16n8k16 products, keys (codes as they are: whole numbers or halves, exact in f16) the 16-row
+//            operand, query rows the 8 columns, in two f16 terms under a power of two of their row (22 bits).  The accumulator
+//            of a block of 32 dimensions is scaled by the block's factor and added in f32.
+//   output   O^T = V^T P^T, values the 16-row operand; probabilities times the value's scale of the block, under a power of two
+//            of the step's largest scale, in two f16 terms (22 bits below the largest).  Accumulators hold a step, not the
+//            sequence: the tensor core adds with truncation, the running output is added round-to-nearest.
+// Up to four query rows stand as four pairs of columns (term, term): one product does both terms.
 #include "kv_pages.cuh"
 
 namespace jq {
 
 namespace {
 
-// part[b, head, page]: HD sums, the maximum, the sum of exponentials
-template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(128) attention_page_kernel(KvPages c, const float* __restrict__ q, uint64_t q_stride,
-                                                             const int32_t* __restrict__ len, uint32_t n_q, float scale,
-                                                             uint32_t shared, float* __restrict__ part) {
-    constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);
-    __shared__ float s_q[HD], s_p[KV_PAGE], s_red[4];
-    pdl_trigger_all();
-    const uint32_t page = blockIdx.x, head = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int32_t n = len[b];
-    if (n <= 0 || (uint32_t)n > c.table_stride * (uint64_t)KV_PAGE || page * KV_PAGE >= (uint32_t)n) return;
-    float* dst = part + (((uint64_t)b * n_q + head) * c.table_stride + page) * (HD + 2);
-    const uint32_t cnt = min(KV_PAGE, (uint32_t)n - page * KV_PAGE);
-    const int32_t id = c.table[(uint64_t)(page < shared ? 0 : b) * c.table_stride + page];
-    if (id < 0 || (uint32_t)id >= c.n_pages) {
-        for (uint32_t i = threadIdx.x; i < HD + 2; i += 128) dst[i] = NAN;
-        return;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // read once: not kept in L1
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// the 8x8 transpose between the accumulator's layout (row = position) and the B operand's (row of lanes = column)
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t t;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+    return t;
+}
+__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// a and b, and what f16 leaves of them
+__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    *hi = half2_bits(h), *lo = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
+}
+__device__ __forceinline__ uint32_t split1(float a) {  // (term, term)
+    const float h = __half2float(__float2half_rn(a));
+    return half2_bits(__floats2half2_rn(h, a - h));
+}
+// bytes b, b + 1 of w (codes + 128) as halves
+template <int B>
+__device__ __forceinline__ uint32_t codes8(uint32_t w) {
+    return half2_bits(__hsub2(bits_half2(__byte_perm(w, 0x64646464u, B == 0 ? 0x4140 : 0x4342)), __float2half2_rn(1152.0f)));
+}
+// four-bit codes + 8 at bits 4 N .. and 16 + 4 N .. as halves
+template <int N>
+__device__ __forceinline__ uint32_t codes4(uint32_t w) {
+    if constexpr (N >= 2) w >>= 8;
+    if constexpr (N % 2 == 0)  // 1024 + n
+        return half2_bits(__hsub2(bits_half2((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f)));
+    // 1024 + 16 n
+    return half2_bits(__hfma2(bits_half2((w & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
+}
+
+template <uint32_t KIND_, uint32_t HD_>
+struct Step {
+    static constexpr uint32_t KIND = KIND_, HD = HD_, NB = HD / 32, BITS = KIND == KV_F16 ? 16 : KIND == KV_Q8_0 ? 8 : 4;
+    static constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);  // a head of a page
+    // positions at a time: 16 KB to 4 KB of codes, 16 to 64 registers a lane for keys and as many for values
+    static constexpr uint32_t WANT = 64 * 128 * 4 / (HD * BITS), POS = WANT < 16 ? 16 : WANT > 64 ? 64 : WANT;
+    static constexpr uint32_t GROUPS = POS / 16, VECS = POS * HD * BITS / 8 / 512;
+    static constexpr uint32_t SW = KIND == KV_F16 ? 1 : POS / 16;  // words of two scales a block
+};
+
+// One step's keys or values, a lane's share: codes, scales of positions lane / 4 + 8 i by block.
+template <class T>
+struct Rows {
+    uint4 c[T::VECS];
+    uint32_t s[T::NB][T::SW];
+
+    // KEEP: other warps of the SM read it too
+    template <bool KEEP = false>
+    __device__ __forceinline__ void load(const uint8_t* part, uint32_t at, uint32_t lane) {
+        const uint8_t* p = part + at * (T::HD * T::BITS / 8) + lane * 16;
+#pragma unroll
+        for (uint32_t i = 0; i < T::VECS; ++i) c[i] = KEEP ? __ldg(reinterpret_cast<const uint4*>(p + i * 512)) : ld_stream(p + i * 512);
+        if constexpr (T::KIND != KV_F16) {
+            const uint8_t* q = part + kv_code_bytes(T::KIND, T::HD) + ((at / 32 * 8 + lane / 4) * T::NB) * 8;
+            if constexpr (T::POS == 16) {
+#pragma unroll
+                for (uint32_t b = 0; b < T::NB; ++b) s[b][0] = __ldg(reinterpret_cast<const uint32_t*>(q + b * 8 + at % 32 / 4));
+            } else {
+#pragma unroll
+                for (uint32_t h = 0; h < T::POS / 32; ++h)
+#pragma unroll
+                    for (uint32_t b = 0; b < T::NB; b += 2) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(q + h * (64 * T::NB) + b * 8));
+                        s[b][2 * h] = v.x, s[b][2 * h + 1] = v.y, s[b + 1][2 * h] = v.z, s[b + 1][2 * h + 1] = v.w;
+                    }
+            }
+        }
     }
-    const uint8_t* tile = c.pages + ((uint64_t)id * c.n_kv + head / (n_q / c.n_kv)) * HEAD;
-    for (uint32_t i = threadIdx.x; i < HD; i += 128) s_q[i] = q[b * q_stride + head * HD + i];
-    __syncthreads();
-    float mx = -INFINITY;
-    for (uint32_t t = warp; t < cnt; t += 4) {
-        float acc = 0.0f;
-        for (uint32_t d = 4 * lane; d < HD; d += 128) {
-            const float4 k = kv_load<KIND, HD, false>(tile, t, d);
-            acc = fmaf(s_q[d], k.x, fmaf(s_q[d + 1], k.y, fmaf(s_q[d + 2], k.z, fmaf(s_q[d + 3], k.w, acc))));
+    __device__ __forceinline__ uint32_t word(uint32_t vec, uint32_t i) const {
+        return i == 0 ? c[vec].x : i == 1 ? c[vec].y : i == 2 ? c[vec].z : c[vec].w;
+    }
+    // scale of position lane / 4 + 8 i
+    __device__ __forceinline__ float scale(uint32_t b, uint32_t i) const {
+        const float2 f = __half22float2(bits_half2(s[b][i / 2]));
+        return i % 2 ? f.y : f.x;
+    }
+    // A operand of 16 keys (group a) and 16 dimensions (half h of block b)
+    __device__ __forceinline__ void key(uint32_t a, uint32_t b, uint32_t h, uint32_t (&r)[4]) const {
+        if constexpr (T::KIND == KV_F16) {
+            const uint32_t v = (a * T::NB + b) * 2 + h;
+            r[0] = word(v, 0), r[1] = word(v, 2), r[2] = word(v, 1), r[3] = word(v, 3);
+        } else if constexpr (T::KIND == KV_Q8_0) {
+            const uint32_t v = a * T::NB + b, x = word(v, h), y = word(v, 2 + h);
+            r[0] = codes8<0>(x), r[1] = codes8<0>(y), r[2] = codes8<2>(x), r[3] = codes8<2>(y);
+        } else {
+            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + h);
+            r[0] = codes4<0>(x), r[1] = codes4<2>(x), r[2] = codes4<1>(x), r[3] = codes4<3>(x);
+        }
+    }
+    // A operand of 16 dimensions (tile m of block b) and 16 positions (group a)
+    __device__ __forceinline__ void value(uint32_t a, uint32_t b, uint32_t m, uint32_t (&r)[4]) const {
+        if constexpr (T::KIND == KV_F16) {
+            const uint32_t v = (a * T::NB + b) * 2 + m;
+            r[0] = word(v, 0), r[1] = word(v, 1), r[2] = word(v, 2), r[3] = word(v, 3);
+        } else if constexpr (T::KIND == KV_Q8_0) {
+            const uint32_t v = a * T::NB + b, x = word(v, 2 * m), y = word(v, 2 * m + 1);
+            r[0] = codes8<0>(x), r[1] = codes8<2>(x), r[2] = codes8<0>(y), r[3] = codes8<2>(y);
+        } else {
+            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + m);
+            r[0] = codes4<0>(x), r[1] = codes4<1>(x), r[2] = codes4<2>(x), r[3] = codes4<3>(x);
+        }
+    }
+};
+
+// Query rows of a warp: NT tiles of eight columns.  PAIRS: four rows, (term, term) in neighbouring columns; else eight rows a
+// tile, the terms as two products.  A lane's rows are those of its accumulator columns: lane % 4, or 8 t + 2 (lane % 4) + {0, 1}.
+template <class T, uint32_t NT, bool PAIRS>
+struct Queries {
+    static constexpr uint32_t ROWS = PAIRS ? 4 : 8 * NT, MINE = PAIRS ? 1 : 2 * NT;
+    // words of the B operand in shared memory: [tile][block half][term][lane] pairs
+    static constexpr uint32_t WORDS = PAIRS ? 0 : NT * (T::HD / 16) * 2 * 64;
+};
+
+template <class T, uint32_t NT, bool PAIRS>
+struct Attend {
+    using Q = Queries<T, NT, PAIRS>;
+    static constexpr uint32_t HD = T::HD, NB = T::NB, GROUPS = T::GROUPS, MINE = Q::MINE, COLS = PAIRS ? 1 : 2;
+    uint32_t qf[PAIRS ? 2 * NB : 1][2];  // B operand of the query rows, in registers (PAIRS)
+    const uint32_t* q_shared;            // or in shared memory
+    float rf[MINE];                      // what a row's scores are multiplied by
+    float mx[MINE], sum[MINE];           // running maximum; sum of this lane's positions
+    float o[NB][2][NT][2 * COLS];        // dimensions 4 (lane / 4) + 2 m + {0, 1} of a block, by column
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; ++i) mx[i] = -INFINITY, sum[i] = 0.0f;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+            for (uint32_t m = 0; m < 2; ++m)
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                    for (uint32_t i = 0; i < 2 * COLS; ++i) o[b][m][t][i] = 0.0f;
+    }
+
+    // `row(i)`: query row i as a pointer to HD floats, NULL for none.  With shared memory: all lanes of the warp write, and
+    // other warps may read after a barrier.
+    template <class F>
+    __device__ __forceinline__ void load_queries(F row, float scale, uint32_t lane, uint32_t* shared) {
+        const uint32_t n = lane / 4, c = lane % 4;
+        q_shared = shared;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; ++t) {
+            const float* src = row(PAIRS ? n / 2 : 8 * t + n);
+            float x[NB][8], amax = 0.0f;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b) {
+                const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 u = src ? *reinterpret_cast<const float4*>(src + 32 * b + 8 * c) : zero;
+                const float4 v = src ? *reinterpret_cast<const float4*>(src + 32 * b + 8 * c + 4) : zero;
+                const float w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[b][i] = w[i], amax = fmaxf(amax, fabsf(w[i]));
+            }
+            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+            // a power of two that puts the row's largest value just below 2^15
+            const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
+            const float up = __uint_as_float(bits << 23);
+            const float down = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * scale * 1.44269504f;
+#pragma unroll
+            for (uint32_t b = 0; b < NB; ++b)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    uint32_t hi[2], lo[2];
+                    split2(x[b][4 * h] * up, x[b][4 * h + 1] * up, &hi[0], &lo[0]);
+                    split2(x[b][4 * h + 2] * up, x[b][4 * h + 3] * up, &hi[1], &lo[1]);
+                    if constexpr (PAIRS) {
+                        qf[2 * b + h][0] = n % 2 ? lo[0] : hi[0], qf[2 * b + h][1] = n % 2 ? lo[1] : hi[1];
+                    } else {
+                        uint2* to = reinterpret_cast<uint2*>(shared) + ((t * 2 * NB + 2 * b + h) * 2) * 32 + lane;
+                        to[0] = make_uint2(hi[0], hi[1]), to[32] = make_uint2(lo[0], lo[1]);
+                    }
+                }
+            if constexpr (PAIRS) {
+                rf[0] = __shfl_sync(0xFFFFFFFFu, down, 8 * c);
+            } else {
+                rf[2 * t] = __shfl_sync(0xFFFFFFFFu, down, 8 * c), rf[2 * t + 1] = __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);
+            }
+        }
+        if constexpr (!PAIRS) __syncwarp();
+    }
+
+    // s[group][tile][...]: position lane / 4 (+ 8 in the upper half) by column
+    __device__ __forceinline__ void scores(const Rows<T>& k, uint32_t lane, float (&s)[GROUPS][NT][2 * COLS]) const {
+#pragma unroll
+        for (uint32_t a = 0; a < GROUPS; ++a)
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                for (uint32_t i = 0; i < 2 * COLS; ++i) s[a][t][i] = 0.0f;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            uint2 q[2][NT][PAIRS ? 1 : 2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t) {
+                    if constexpr (PAIRS) {
+                        q[h][t][0] = make_uint2(qf[2 * b + h][0], qf[2 * b + h][1]);
+                    } else {
+                        const uint2* from = reinterpret_cast<const uint2*>(q_shared) + ((t * 2 * NB + 2 * b + h) * 2) * 32 + lane;
+                        q[h][t][0] = from[0], q[h][t][1] = from[32];
+                    }
+                }
+#pragma unroll
+            for (uint32_t a = 0; a < GROUPS; ++a) {
+                uint32_t r[2][4];
+                k.key(a, b, 0, r[0]), k.key(a, b, 1, r[1]);
+                float up = 1.0f, down = 1.0f;
+                if constexpr (T::KIND != KV_F16) up = k.scale(b, 2 * a), down = k.scale(b, 2 * a + 1);
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t) {
+                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int term = PAIRS ? 0 : 1; term >= 0; --term)
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) mma16816(d, r[h], q[h][t][term].x, q[h][t][term].y);
+                    if constexpr (PAIRS) {
+                        s[a][t][0] = fmaf(d[0] + d[1], up, s[a][t][0]), s[a][t][1] = fmaf(d[2] + d[3], down, s[a][t][1]);
+                    } else {
+                        s[a][t][0] = fmaf(d[0], up, s[a][t][0]), s[a][t][1] = fmaf(d[1], up, s[a][t][1]);
+                        s[a][t][2] = fmaf(d[2], down, s[a][t][2]), s[a][t][3] = fmaf(d[3], down, s[a][t][3]);
+                    }
+                }
+            }
+        }
+    }
+
+    // scores -> probabilities under the new maximum; positions from `valid` on are nothing.  alpha: of what was before.
+    __device__ __forceinline__ void softmax(float (&s)[GROUPS][NT][2 * COLS], uint32_t valid, uint32_t lane, float (&alpha)[MINE]) {
+        float nm[MINE];
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; ++i) nm[i] = mx[i];
+#pragma unroll
+        for (uint32_t a = 0; a < GROUPS; ++a)
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t c = 0; c < COLS; ++c) {
+                        const uint32_t i = COLS * t + c;
+                        float& x = s[a][t][COLS * h + c];
+                        x = 16 * a + 8 * h + lane / 4 < valid ? x * rf[i] : -INFINITY;
+                        nm[i] = fmaxf(nm[i], x);
+                    }
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; ++i) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) nm[i] = fmaxf(nm[i], __shfl_xor_sync(0xFFFFFFFFu, nm[i], o));
+            alpha[i] = ex2(mx[i] - nm[i]);
+            mx[i] = nm[i], sum[i] *= alpha[i];
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xFFFFFFFFu, acc, o);
-        if (lane == 0) s_p[t] = acc * scale;
-        mx = fmaxf(mx, acc * scale);
+        for (uint32_t a = 0; a < GROUPS; ++a)
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t c = 0; c < COLS; ++c) {
+                        const uint32_t i = COLS * t + c;
+                        float& x = s[a][t][COLS * h + c];
+                        x = ex2(x - nm[i]);
+                        sum[i] += x;
+                    }
     }
-    if (lane == 0) s_red[warp] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    for (uint32_t t = threadIdx.x; t < cnt; t += 128) s_p[t] = expf(s_p[t] - mx);
-    __syncthreads();
-    float sum = 0.0f;
-    for (uint32_t t = 0; t < cnt; ++t) sum += s_p[t];
-    for (uint32_t d = 4 * threadIdx.x; d < HD; d += 512) {
-        float4 o = make_float4(0, 0, 0, 0);
-        for (uint32_t t = 0; t < cnt; ++t) {
-            const float4 v = kv_load<KIND, HD, true>(tile + HEAD / 2, t, d);
-            const float p = s_p[t];
-            o.x = fmaf(p, v.x, o.x), o.y = fmaf(p, v.y, o.y), o.z = fmaf(p, v.z, o.z), o.w = fmaf(p, v.w, o.w);
+
+    // B operands of the probabilities times up[i], the factor of position lane / 4 + 8 i
+    struct Terms {
+        uint32_t b[GROUPS][NT][PAIRS ? 1 : 2][2];
+    };
+    __device__ __forceinline__ void terms(const float (&p)[GROUPS][NT][2 * COLS], const float (&up)[2 * GROUPS], Terms& w) const {
+#pragma unroll
+        for (uint32_t a = 0; a < GROUPS; ++a)
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    if constexpr (PAIRS) {
+                        w.b[a][t][0][h] = transpose8(split1(p[a][t][h] * up[2 * a + h]));
+                    } else {
+                        uint32_t hi, lo;
+                        split2(p[a][t][2 * h] * up[2 * a + h], p[a][t][2 * h + 1] * up[2 * a + h], &hi, &lo);
+                        w.b[a][t][0][h] = transpose8(hi), w.b[a][t][1][h] = transpose8(lo);
+                    }
+                }
+    }
+
+    __device__ __forceinline__ void output(const float (&p)[GROUPS][NT][2 * COLS], Rows<T>& v, uint32_t valid, uint32_t lane,
+                                           const float (&alpha)[MINE]) {
+        Terms w;
+        float up[2 * GROUPS], down = 1.0f / 16384.0f;
+        bool moved = false;
+#pragma unroll
+        for (uint32_t i = 0; i < MINE; ++i) moved |= alpha[i] != 1.0f;
+        moved = __any_sync(0xFFFFFFFFu, moved);
+        if constexpr (T::KIND == KV_F16) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * GROUPS; ++i) up[i] = 16384.0f;
+            terms(p, up, w);
+            if (valid < T::POS) {  // what stands behind the last position may be no number
+                const uint32_t c = lane % 4 * 2;
+#pragma unroll
+                for (uint32_t i = 0; i < T::VECS; ++i) {
+                    const uint32_t first = i / (2 * NB) * 16 + c;
+                    const uint32_t low = (first < valid ? 0xFFFFu : 0u) | (first + 1 < valid ? 0xFFFF0000u : 0u);
+                    const uint32_t high = (first + 8 < valid ? 0xFFFFu : 0u) | (first + 9 < valid ? 0xFFFF0000u : 0u);
+                    v.c[i].x &= low, v.c[i].y &= low, v.c[i].z &= high, v.c[i].w &= high;
+                }
+            }
+        } else if (valid < T::POS) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * GROUPS; i += 2) {
+                const uint32_t at = 8 * i + lane / 4, keep = (at < valid ? 0xFFFFu : 0u) | (at + 8 < valid ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b) v.s[b][i / 2] &= keep;
+            }
         }
-        dst[d] = o.x, dst[d + 1] = o.y, dst[d + 2] = o.z, dst[d + 3] = o.w;
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            if constexpr (T::KIND != KV_F16) {
+                uint32_t top = 0x04000400u;  // not below the smallest normal number
+#pragma unroll
+                for (uint32_t i = 0; i < T::SW; ++i) top = __vmaxu2(top, v.s[b][i] & 0x7FFF7FFFu);
+                const uint32_t e = __reduce_max_sync(0xFFFFFFFFu, max(top >> 16, top & 0xFFFFu)) >> 10;
+                const float f = __uint_as_float((156u - e) << 23);  // 2^(29 - e): the largest scale times f is below 2^15
+                down = __uint_as_float((98u + e) << 23);
+#pragma unroll
+                for (uint32_t i = 0; i < 2 * GROUPS; ++i) up[i] = v.scale(b, i) * f;
+                terms(p, up, w);
+            }
+#pragma unroll
+            for (uint32_t m = 0; m < 2; ++m) {
+                float d[NT][4];
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t) d[t][0] = d[t][1] = d[t][2] = d[t][3] = 0.0f;
+#pragma unroll
+                for (uint32_t a = 0; a < GROUPS; ++a) {
+                    uint32_t r[4];
+                    v.value(a, b, m, r);
+#pragma unroll
+                    for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int term = PAIRS ? 0 : 1; term >= 0; --term) mma16816(d[t], r, w.b[a][t][term][0], w.b[a][t][term][1]);
+                }
+#pragma unroll
+                for (uint32_t t = 0; t < NT; ++t) {
+                    float (&x)[2 * COLS] = o[b][m][t];
+                    if (moved) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 2 * COLS; ++i) x[i] *= alpha[PAIRS ? 0 : 2 * t + i % 2];
+                    }
+                    if constexpr (PAIRS) {
+                        x[0] = fmaf(d[t][0] + d[t][1], down, x[0]), x[1] = fmaf(d[t][2] + d[t][3], down, x[1]);
+                    } else {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) x[i] = fmaf(d[t][i], down, x[i]);
+                    }
+                }
+            }
+        }
     }
-    if (threadIdx.x == 0) dst[HD] = mx, dst[HD + 1] = sum;
-}
 
-__global__ void __launch_bounds__(128) attention_page_merge_kernel(const float* __restrict__ part, const int32_t* __restrict__ len,
-                                                                   uint32_t n_q, uint32_t hd, uint32_t stride, uint32_t shared,
-                                                                   float* __restrict__ out, uint64_t out_stride,
-                                                                   int32_t* __restrict__ bad_pos) {
-    pdl_trigger_all();
-    const uint32_t head = blockIdx.x, b = blockIdx.y;
-    const int32_t n = len[b];
-    float* dst = out + b * out_stride + (uint64_t)head * hd;
-    const bool bad = n < 0 || (uint32_t)n > stride * (uint64_t)KV_PAGE || (n > 0 && (uint32_t)n < shared * KV_PAGE);
-    const uint32_t pages = bad ? 0 : ((uint32_t)n + KV_PAGE - 1) / KV_PAGE;
-    if (bad && head == 0 && threadIdx.x == 0 && bad_pos) atomicExch(bad_pos, 1);
-    const float* src = part + ((uint64_t)b * n_q + head) * stride * (hd + 2);
-    float mx = -INFINITY, den = 0.0f;
-    bool lost = bad;
-    for (uint32_t i = 0; i < pages; ++i) {
-        const float m = src[(uint64_t)i * (hd + 2) + hd];
-        lost |= m != m;
-        mx = fmaxf(mx, m);
+    // [ROWS][HD] sums, then maxima and sums of exponentials of the rows
+    __device__ __forceinline__ void store(float* to, uint32_t lane) {
+        const uint32_t g = lane / 4, c = lane % 4;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; ++t)
+#pragma unroll
+            for (uint32_t i = 0; i < COLS; ++i) {
+                const uint32_t row = PAIRS ? c : 8 * t + 2 * c + i, mine = PAIRS ? 0 : 2 * t + i;
+#pragma unroll
+                for (uint32_t b = 0; b < NB; ++b)
+                    *reinterpret_cast<float4*>(to + row * HD + 32 * b + 4 * g) =
+                        make_float4(o[b][0][t][i], o[b][0][t][COLS + i], o[b][1][t][i], o[b][1][t][COLS + i]);
+                float l = sum[mine];
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+                if (g == 0) to[Q::ROWS * HD + row] = mx[mine], to[Q::ROWS * HD + Q::ROWS + row] = l;
+            }
     }
-    if (lost && !bad && head == 0 && threadIdx.x == 0 && bad_pos) atomicExch(bad_pos, 1);
-    for (uint32_t i = 0; i < pages; ++i) den += expf(src[(uint64_t)i * (hd + 2) + hd] - mx) * src[(uint64_t)i * (hd + 2) + hd + 1];
-    for (uint32_t d = threadIdx.x; d < hd; d += 128) {
-        float acc = 0.0f;
-        for (uint32_t i = 0; i < pages; ++i) acc = fmaf(expf(src[(uint64_t)i * (hd + 2) + hd] - mx), src[(uint64_t)i * (hd + 2) + d], acc);
-        dst[d] = lost ? NAN : pages ? acc / den : 0.0f;
-    }
-}
+};
 
-struct LaunchPages {
-    const KvPages& c;
+struct PagedArgs {
+    KvPages c;
     const float* q;
     uint64_t q_stride;
     const int32_t* len;
-    uint32_t n_q;
+    uint32_t n_q, group, split;  // query heads; heads a kv head; warps' worth of them (each up to ROWS rows)
     float scale;
-    uint32_t shared;
-    float* part;
+    uint32_t common, done;  // leading pages named by the first sequence; leading pages that the other kernel takes
+    float* out;
+    uint64_t out_stride;
+    uint32_t* arrived;  // [batch * n_kv * split], zero between calls
+    float* part;        // [grid][2][ROWS (HD + 2)]
+    const float* lead;  // done: [lead_splits][n_kv][batch * group][HD], then their maxima, then their sums
+    uint32_t lead_splits;
+    int32_t* bad_pos;
+};
+
+// Weight of a piece with maximum m under the joint maximum; equal ones are 1 (infinities too)
+__device__ __forceinline__ float piece_weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
+
+__device__ __forceinline__ const float* lead_row(const PagedArgs& a, uint32_t hd, uint32_t i, uint32_t kvh, uint32_t row, const float** m,
+                                                 const float** l) {
+    const uint64_t rows = (uint64_t)a.c.n_seq * a.group, all = a.lead_splits * (uint64_t)a.c.n_kv * rows;
+    const uint64_t at = ((uint64_t)i * a.c.n_kv + kvh) * rows + row;
+    *m = a.lead + all * hd + at, *l = a.lead + all * hd + all + at;
+    return a.lead + at * hd;
+}
+
+// out = the joined pieces (n of them, `piece(i)` points to [ROWS][HD] sums, maxima, sums) and those of the leading pages, by
+// `threads` threads.  A row of nothing is zero.
+template <uint32_t HD, uint32_t ROWS, class F>
+__device__ __forceinline__ void finish(const PagedArgs& a, uint32_t b, uint32_t head_group, uint32_t n, F piece, uint32_t tid,
+                                       uint32_t threads) {
+    const uint32_t kvh = head_group / a.split, first = head_group % a.split * ROWS, rows = min(ROWS, a.group - first);
+    for (uint32_t i = tid; i < rows * (HD / 4); i += threads) {
+        const uint32_t row = i / (HD / 4), d = i % (HD / 4) * 4, in_batch = b * a.group + first + row;
+        float top = -INFINITY;
+        for (uint32_t j = 0; j < n; ++j) top = fmaxf(top, piece(j)[ROWS * HD + row]);
+        for (uint32_t j = 0; j < a.lead_splits; ++j) {
+            const float *m, *l;
+            lead_row(a, HD, j, kvh, in_batch, &m, &l);
+            top = fmaxf(top, *m);
+        }
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float den = 0.0f;
+        auto add = [&](const float* o, float m, float l) {
+            const float w = piece_weight(m, top);
+            const float4 v = *reinterpret_cast<const float4*>(o + d);
+            x.x = fmaf(w, v.x, x.x), x.y = fmaf(w, v.y, x.y), x.z = fmaf(w, v.z, x.z), x.w = fmaf(w, v.w, x.w);
+            den = fmaf(w, l, den);
+        };
+        for (uint32_t j = 0; j < a.lead_splits; ++j) {
+            const float *m, *l, *o = lead_row(a, HD, j, kvh, in_batch, &m, &l);
+            add(o, *m, *l);
+        }
+        for (uint32_t j = 0; j < n; ++j) add(piece(j) + row * HD, piece(j)[ROWS * HD + row], piece(j)[ROWS * HD + ROWS + row]);
+        const float inv = n + a.lead_splits ? 1.0f / den : 0.0f;
+        *reinterpret_cast<float4*>(a.out + b * a.out_stride + (uint64_t)(kvh * a.group + first + row) * HD + d) =
+            make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    }
+}
+
+// Positions of a sequence's own (behind the leading pages), or -1 where its length is out of range.
+__device__ __forceinline__ int32_t own_positions(const PagedArgs& a, uint32_t b) {
+    const int32_t n = a.len[b];
+    if (n < 0 || (uint32_t)n > a.c.table_stride * KV_PAGE || (n > 0 && (uint32_t)n < a.common * KV_PAGE)) return -1;
+    return n == 0 ? 0 : n - (int32_t)(a.done * KV_PAGE);
+}
+
+// The sequences' steps stand in one row: sequence by sequence, head group by head group.  It is cut into equal pieces, one a
+// warp, whatever the lengths; a CTA's warps have neighbouring ones.  Pieces of one segment (sequence, head group) are joined
+// within the CTA, then, where a segment spans CTAs, by the last one of them to arrive, in order.
+template <class T, bool PAIRS, uint32_t WARPS, uint32_t MIN_CTAS>
+__global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(PagedArgs a) {
+    using At = Attend<T, 1, PAIRS>;
+    constexpr uint32_t HD = T::HD, ROWS = At::Q::ROWS, PIECE = ROWS * (HD + 2);
+    extern __shared__ __align__(16) uint32_t s_mem[];
+    __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_last;
+    uint32_t* s_cum = s_mem;                                                       // [batch + 1] steps in front of a sequence
+    float* s_piece = reinterpret_cast<float*>(s_mem + ((a.c.n_seq + 4) & ~3u));    // [WARPS][2][PIECE]
+    uint32_t* s_q = reinterpret_cast<uint32_t*>(s_piece + WARPS * 2 * PIECE);      // [WARPS] query operands
+    pdl_trigger_all();
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, batch = a.c.n_seq, groups = a.c.n_kv * a.split;
+    if (tid < 2 * WARPS) s_seg[tid] = 0xFFFFFFFFu;
+    // running sum of the sequences' steps, a run of sequences a thread
+    const uint32_t per = (batch + WARPS * 32 - 1) / (WARPS * 32), b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
+    uint32_t mine = 0;
+    for (uint32_t b = b0; b < b1; ++b) mine += (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
+    uint32_t run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, run, o);
+        run += lane >= o ? up : 0;
+    }
+    if (lane == 31) s_scan[warp] = run;
+    __syncthreads();
+    for (uint32_t w = 0; w < warp; ++w) run += s_scan[w];
+    run -= mine;
+    for (uint32_t b = b0; b < b1; ++b) {
+        s_cum[b] = run;
+        run += (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
+    }
+    if (b1 == batch && (b0 < b1 || tid == 0)) s_cum[batch] = run;
+    __syncthreads();
+
+    const uint64_t total = (uint64_t)s_cum[batch] * groups;
+    const uint64_t workers = min((uint64_t)gridDim.x * WARPS, total);
+    const uint64_t me = (uint64_t)blockIdx.x * WARPS + warp;
+    uint64_t at = me < workers ? me * total / workers : 0;
+    const uint64_t end = me < workers ? (me + 1) * total / workers : 0;
+    At w;
+    bool first_piece = true;
+    uint32_t b = 0;
+    if (at < end) {  // the last sequence that begins at or before it (and has steps)
+        uint32_t lo = 0, hi = batch;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            (uint64_t)s_cum[mid] * groups <= at ? lo = mid : hi = mid;
+        }
+        b = lo;
+    }
+    while (at < end) {
+        while (s_cum[b + 1] == s_cum[b] || (uint64_t)s_cum[b + 1] * groups <= at) ++b;
+        const uint32_t steps = s_cum[b + 1] - s_cum[b];
+        const uint64_t in_seq = at - (uint64_t)s_cum[b] * groups;
+        const uint32_t hg = (uint32_t)(in_seq / steps), u0 = (uint32_t)(in_seq % steps);
+        const uint32_t u1 = (uint32_t)min((uint64_t)steps, u0 + (end - at));
+        const uint32_t kvh = hg / a.split, first = hg % a.split * ROWS;
+        const uint32_t own = (uint32_t)own_positions(a, b);
+        // page ids of 32 pages at a time, a lane each
+        constexpr uint32_t PER_PAGE = KV_PAGE / T::POS;
+        const int32_t* table = a.c.table + (uint64_t)b * a.c.table_stride;
+        uint32_t have = u0 / PER_PAGE;
+        int32_t ids = 0;
+        auto fetch_ids = [&] {
+            const uint32_t p = a.done + have + lane;
+            ids = p < a.c.table_stride ? (p < a.common ? a.c.table[p] : table[p]) : -1;
+        };
+        bool lost = false;
+        auto tile_of = [&](uint32_t u) -> const uint8_t* {
+            const uint32_t p = u / PER_PAGE;
+            if (p - have >= 32) have = p, fetch_ids();
+            const int32_t id = __shfl_sync(0xFFFFFFFFu, ids, p - have);
+            const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
+            lost |= !fine;
+            return a.c.pages + ((uint64_t)(fine ? id : 0) * a.c.n_kv + kvh) * T::HEAD;
+        };
+        fetch_ids();
+        const uint8_t* tile = tile_of(u0);
+        Rows<T> k, v;
+        k.load(tile, u0 % PER_PAGE * T::POS, lane);
+        const float* q = a.q + b * a.q_stride + (uint64_t)(kvh * a.group + first) * HD;
+        w.load_queries([&](uint32_t i) -> const float* { return first + i < a.group ? q + i * HD : nullptr; }, a.scale, lane,
+                       s_q + warp * At::Q::WORDS);
+        w.reset();
+        for (uint32_t u = u0; u < u1; ++u) {
+            const uint32_t valid = min(own - u * T::POS, T::POS);
+            v.load(tile + T::HEAD / 2, u % PER_PAGE * T::POS, lane);
+            float s[T::GROUPS][1][2 * At::COLS], alpha[At::MINE];
+            w.scores(k, lane, s);
+            if (u + 1 < u1) {
+                tile = tile_of(u + 1);
+                k.load(tile, (u + 1) % PER_PAGE * T::POS, lane);
+            }
+            w.softmax(s, valid, lane, alpha);
+            w.output(s, v, valid, lane, alpha);
+        }
+        if (lost) {
+#pragma unroll
+            for (uint32_t i = 0; i < At::MINE; ++i) w.sum[i] = NAN;
+            if (lane == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+        }
+        const uint32_t slot = 2 * warp + (first_piece ? 0 : 1);
+        float* to = s_piece + slot * PIECE;
+        __syncwarp();
+        w.store(to, lane);
+        __syncwarp();
+        if (u0 == 0 && u1 == steps) {
+            finish<HD, ROWS>(a, b, hg, 1, [&](uint32_t) { return to; }, lane, 32);
+        } else {
+            if (lane == 0) s_seg[slot] = b * groups + hg, s_from[slot] = u0, s_to[slot] = u1;
+            first_piece = false;
+        }
+        at += u1 - u0;
+    }
+    __syncthreads();
+    // pieces of segments that no warp has whole, in order
+    for (uint32_t i = 0; i < 2 * WARPS;) {
+        const uint32_t seg = s_seg[i];
+        if (seg == 0xFFFFFFFFu) {
+            ++i;
+            continue;
+        }
+        static_assert(WARPS <= 8, "slot numbers in four bits");
+        uint64_t slots = 0;  // of the segment
+        uint32_t n = 0, last = i;
+        for (uint32_t j = i; j < 2 * WARPS; ++j)
+            if (s_seg[j] == seg) slots |= (uint64_t)j << (4 * n), ++n, last = j;
+        const uint32_t sb = seg / groups, hg = seg % groups, steps = s_cum[sb + 1] - s_cum[sb], from = s_from[i], to = s_to[last];
+        auto local = [&](uint32_t j) -> const float* { return s_piece + (uint32_t)(slots >> (4 * j) & 15) * PIECE; };
+        if (from == 0 && to == steps) {
+            finish<HD, ROWS>(a, sb, hg, n, local, tid, WARPS * 32);
+        } else {
+            float* dst = a.part + ((uint64_t)blockIdx.x * 2 + (from == 0)) * PIECE;
+            for (uint32_t x = tid; x < ROWS * (HD / 4); x += WARPS * 32) {
+                const uint32_t row = x / (HD / 4), d = x % (HD / 4) * 4;
+                float top = -INFINITY, den = 0.0f;
+                for (uint32_t j = 0; j < n; ++j) top = fmaxf(top, local(j)[ROWS * HD + row]);
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (uint32_t j = 0; j < n; ++j) {
+                    const float* p = local(j);
+                    const float f = piece_weight(p[ROWS * HD + row], top);
+                    const float4 y = *reinterpret_cast<const float4*>(p + row * HD + d);
+                    sum.x = fmaf(f, y.x, sum.x), sum.y = fmaf(f, y.y, sum.y), sum.z = fmaf(f, y.z, sum.z), sum.w = fmaf(f, y.w, sum.w);
+                    den = fmaf(f, p[ROWS * HD + ROWS + row], den);
+                }
+                __stcg(reinterpret_cast<float4*>(dst + row * HD + d), sum);
+                if (d == 0) __stcg(dst + ROWS * HD + row, top), __stcg(dst + ROWS * HD + ROWS + row, den);
+            }
+            // the CTAs that have a piece of it
+            const uint64_t u_first = (uint64_t)s_cum[sb] * groups + (uint64_t)hg * steps, u_last = u_first + steps - 1;
+            const uint32_t c0 = (uint32_t)(((u_first + 1) * workers - 1) / total / WARPS);
+            const uint32_t c1 = (uint32_t)(((u_last + 1) * workers - 1) / total / WARPS);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const uint32_t before = atomicAdd(a.arrived + seg, 1);
+                s_last = before == c1 - c0;
+                if (s_last) a.arrived[seg] = 0;
+            }
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                const float* part = a.part;
+                finish<HD, ROWS>(a, sb, hg, c1 - c0 + 1,
+                                 [&](uint32_t j) { return part + ((uint64_t)(c0 + j) * 2 + (j == 0)) * PIECE; }, tid, WARPS * 32);
+            }
+            __syncthreads();
+        }
+        i = last + 1;  // pieces of a segment follow one another
+    }
+    // sequences without steps of their own
+    for (uint32_t sb = blockIdx.x; sb < batch; sb += gridDim.x) {
+        if (s_cum[sb + 1] != s_cum[sb]) continue;
+        const int32_t own = own_positions(a, sb);
+        if (own < 0 && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+        if (own < 0 || a.len[sb] == 0) {
+            for (uint32_t i = tid; i < a.n_q * HD; i += WARPS * 32) a.out[sb * a.out_stride + i] = own < 0 ? NAN : 0.0f;
+        } else {
+            for (uint32_t hg = 0; hg < groups; ++hg) finish<HD, ROWS>(a, sb, hg, 0, [&](uint32_t) { return s_piece; }, tid, WARPS * 32);
+        }
+    }
+}
+
+// The leading pages, once for all sequences: query rows of the batch (of one kv head) are the columns, NT * 8 a warp.  A CTA's
+// warps take `sets` sets of rows and WARPS / sets parts of the CTA's share of the pages.
+template <class T, uint32_t NT, uint32_t WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) attention_lead_kernel(PagedArgs a, float* __restrict__ lead, uint32_t sets) {
+    using At = Attend<T, NT, false>;
+    constexpr uint32_t HD = T::HD, ROWS = At::Q::ROWS, PIECE = ROWS * (HD + 2), AREA = PIECE > At::Q::WORDS ? PIECE : At::Q::WORDS;
+    constexpr uint32_t PER_PAGE = KV_PAGE / T::POS;
+    extern __shared__ __align__(16) uint32_t s_mem[];  // [WARPS][AREA]: query operands, then the warps' sums
+    pdl_trigger_all();
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, set = warp % sets, part = warp / sets, parts = WARPS / sets;
+    const uint32_t split = blockIdx.x, kvh = blockIdx.z, rows = a.c.n_seq * a.group, first = (blockIdx.y * sets + set) * ROWS;
+    const uint32_t p0 = (uint32_t)((uint64_t)split * a.done / gridDim.x), p1 = (uint32_t)((uint64_t)(split + 1) * a.done / gridDim.x);
+    const uint32_t steps = (p1 - p0) * PER_PAGE, u0 = part * steps / parts, u1 = (part + 1) * steps / parts;
+    At w;
+    w.load_queries(
+        [&](uint32_t i) -> const float* {
+            const uint32_t row = first + i;
+            return row < rows ? a.q + row / a.group * a.q_stride + (uint64_t)(kvh * a.group + row % a.group) * HD : nullptr;
+        },
+        a.scale, lane, s_mem + warp * AREA);
+    w.reset();
+    bool lost = false;
+    auto tile_of = [&](uint32_t u) -> const uint8_t* {
+        const int32_t id = __ldg(a.c.table + p0 + u / PER_PAGE);
+        const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
+        lost |= !fine;
+        return a.c.pages + ((uint64_t)(fine ? id : 0) * a.c.n_kv + kvh) * T::HEAD;
+    };
+    if (u0 < u1) {
+        Rows<T> k, v;
+        const uint8_t* tile = tile_of(u0);
+        k.template load<true>(tile, u0 % PER_PAGE * T::POS, lane);
+        for (uint32_t u = u0; u < u1; ++u) {
+            v.template load<true>(tile + T::HEAD / 2, u % PER_PAGE * T::POS, lane);
+            float s[T::GROUPS][NT][2 * At::COLS], alpha[At::MINE];
+            w.scores(k, lane, s);
+            if (u + 1 < u1) {
+                tile = tile_of(u + 1);
+                k.template load<true>(tile, (u + 1) % PER_PAGE * T::POS, lane);
+            }
+            w.softmax(s, T::POS, lane, alpha);
+            w.output(s, v, T::POS, lane, alpha);
+        }
+    }
+    if (lost) {
+#pragma unroll
+        for (uint32_t i = 0; i < At::MINE; ++i) w.sum[i] = NAN;
+        if (lane == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+    }
+    __syncthreads();  // the query operands have been read
+    float* pieces = reinterpret_cast<float*>(s_mem);
+    w.store(pieces + warp * AREA, lane);
+    __syncthreads();
+    const uint64_t all = (uint64_t)gridDim.x * a.c.n_kv * rows, base = ((uint64_t)split * a.c.n_kv + kvh) * rows;
+    for (uint32_t i = tid; i < sets * ROWS * (HD / 4); i += WARPS * 32) {
+        const uint32_t d = i % (HD / 4) * 4, r = i / (HD / 4) % ROWS, st = i / (HD / 4) / ROWS;
+        const uint32_t row = (blockIdx.y * sets + st) * ROWS + r;
+        if (row >= rows) continue;
+        float top = -INFINITY, den = 0.0f;
+        for (uint32_t j = 0; j < parts; ++j) top = fmaxf(top, pieces[(j * sets + st) * AREA + ROWS * HD + r]);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t j = 0; j < parts; ++j) {
+            const float* p = pieces + (j * sets + st) * AREA;
+            const float f = piece_weight(p[ROWS * HD + r], top);
+            const float4 y = *reinterpret_cast<const float4*>(p + r * HD + d);
+            sum.x = fmaf(f, y.x, sum.x), sum.y = fmaf(f, y.y, sum.y), sum.z = fmaf(f, y.z, sum.z), sum.w = fmaf(f, y.w, sum.w);
+            den = fmaf(f, p[ROWS * HD + ROWS + r], den);
+        }
+        *reinterpret_cast<float4*>(lead + (base + row) * HD + d) = sum;
+        if (d == 0) lead[all * HD + base + row] = top, lead[all * HD + all + base + row] = den;
+    }
+}
+
+constexpr uint32_t AP_WARPS = 4, LEAD_WARPS = 8;
+constexpr uint32_t ap_ctas(uint32_t hd) { return hd == 256 ? 2 : 3; }  // a SM, by the registers that the kernel needs
+constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
+
+// How a call is cut up: the same for its scratch and its launches.
+struct PagedPlan {
+    uint32_t group, split, rows, grid;       // of the kernel over the sequences' own pages
+    uint32_t lead, sets, blocks, splits;     // of the leading pages' kernel: pages, row sets of a CTA, row blocks, page splits
+    size_t part_at, lead_at, bytes;
+};
+PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t shared) {
+    PagedPlan p{};
+    p.group = n_q / n_kv;
+    p.rows = p.group <= 4 ? 4 : 8;
+    p.split = (p.group + p.rows - 1) / p.rows;
+    p.grid = (uint32_t)num_sms() * ap_ctas(hd);
+    p.lead = batch > 1 ? shared : 0;
+    if (p.lead) {
+        const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
+        p.sets = 1;
+        while (p.sets < LEAD_WARPS && p.sets < tiles) p.sets *= 2;
+        p.blocks = (tiles + p.sets - 1) / p.sets;
+        p.splits = std::max(1u, std::min({p.lead, (uint32_t)num_sms() / std::max(1u, p.blocks * n_kv), 32u}));
+    }
+    p.part_at = ((size_t)batch * n_kv * p.split * 4 + 255) / 256 * 256;
+    p.lead_at = p.part_at + ((size_t)p.grid * 2 * p.rows * (hd + 2) * 4 + 255) / 256 * 256;
+    p.bytes = p.lead_at + (size_t)p.splits * n_q * batch * (hd + 2) * 4;
+    return p;
+}
+
+struct LaunchPaged {
+    PagedArgs a;
+    const PagedPlan& p;
+    float* lead;
     cudaStream_t s;
+
+    template <class T, bool PAIRS>
+    cudaError_t own() const {
+        using At = Attend<T, 1, PAIRS>;
+        constexpr uint32_t BYTES = AP_WARPS * (2 * At::Q::ROWS * (T::HD + 2) + At::Q::WORDS) * 4;
+        auto kern = attention_paged_kernel<T, PAIRS, AP_WARPS, ap_ctas(T::HD)>;
+        static bool configured[MAX_DEVICES] = {};
+        if (cudaError_t e = set_max_smem_once(kern, BYTES + (ATTENTION_MAX_BATCH + 4) * 4, configured); e != cudaSuccess) return e;
+        return launch_pdl(kern, dim3(p.grid), AP_WARPS * 32, BYTES + ((a.c.n_seq + 4) & ~3u) * 4, s, a);
+    }
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
-        return launch_pdl(attention_page_kernel<KIND, HD>, dim3(c.table_stride, n_q, c.n_seq), 128, 0, s, c, q, q_stride, len, n_q, scale,
-                          shared, part);
+        using T = Step<KIND, HD>;
+        if (p.lead) {
+            using At = Attend<T, lead_tiles(HD), false>;
+            constexpr uint32_t PIECE = At::Q::ROWS * (HD + 2), AREA = PIECE > At::Q::WORDS ? PIECE : At::Q::WORDS;
+            auto kern = attention_lead_kernel<T, lead_tiles(HD), LEAD_WARPS>;
+            static bool configured[MAX_DEVICES] = {};
+            if (cudaError_t e = set_max_smem_once(kern, LEAD_WARPS * AREA * 4, configured); e != cudaSuccess) return e;
+            cudaError_t e = launch_pdl(kern, dim3(p.splits, p.blocks, a.c.n_kv), LEAD_WARPS * 32, LEAD_WARPS * AREA * 4, s, a, lead, p.sets);
+            if (e != cudaSuccess) return e;
+        }
+        return p.rows == 4 ? own<T, true>() : own<T, false>();
     }
 };
 
 }  // namespace
 
-size_t attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t table_stride, uint32_t shared) {
-    return (size_t)batch * n_q * table_stride * (hd + 2) * 4;
+size_t attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t shared) {
+    return plan(batch, n_q, n_kv, hd, shared).bytes;
 }
 
 cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* len, uint32_t n_q, float scale,
                                    uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, cudaStream_t s) {
-    float* part = static_cast<float*>(scratch);
-    cudaError_t e = for_kind(c.kind, c.hd, LaunchPages{c, q, q_stride, len, n_q, scale, shared, part, s});
-    if (e != cudaSuccess) return e;
-    e = launch_pdl(attention_page_merge_kernel, dim3(n_q, c.n_seq), 128, 0, s, part, len, n_q, c.hd, c.table_stride, shared, out, out_stride,
-                   bad_pos);
+    const PagedPlan p = plan(c.n_seq, n_q, c.n_kv, c.hd, shared);
+    uint8_t* mem = static_cast<uint8_t*>(scratch);
+    float* lead = reinterpret_cast<float*>(mem + p.lead_at);
+    const PagedArgs a{c, q, q_stride, len, n_q, p.group, p.split, scale, shared, p.lead, out, out_stride,
+                      reinterpret_cast<uint32_t*>(mem), reinterpret_cast<float*>(mem + p.part_at), lead, p.splits, bad_pos};
+    cudaError_t e = for_kind(c.kind, c.hd, LaunchPaged{a, p, lead, s});
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

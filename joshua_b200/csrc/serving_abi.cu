@@ -149,9 +149,9 @@ int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32
     return jq::OK;
 }
 
-uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t table_stride,
-                                          uint32_t shared_pages) {
-    return jq::attention_paged_scratch_bytes(batch, n_q, n_kv, head_dim, table_stride, shared_pages);
+uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t shared_pages) {
+    if (batch == 0 || batch > JQ_ATTENTION_MAX_BATCH || n_kv == 0 || n_q == 0 || n_q % n_kv) return 0;
+    return jq::attention_paged_scratch_bytes(batch, n_q, n_kv, head_dim, shared_pages);
 }
 
 int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* len,
@@ -164,7 +164,9 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
     if (int32_t rc = check_cache(who, cache, page_table, batch, table_stride, &c)) return rc;
     if (int32_t rc = check_heads(who, cache, n_q)) return rc;
     if (!q || !len || !out || !scratch) return bad(who, "NULL buffer");
-    if (batch > 65535) return bad(who, "at most 65535 sequences");
+    static_assert(JQ_ATTENTION_MAX_BATCH == jq::ATTENTION_MAX_BATCH, "header");
+    if (batch > JQ_ATTENTION_MAX_BATCH) return jq_fail(jq::E_TOO_LARGE, "jq_attention_paged_dev: more than JQ_ATTENTION_MAX_BATCH sequences");
+    if ((uint64_t)batch * table_stride > 1u << 28) return bad(who, "a page table of more than 2^28 entries");
     if (shared_pages > table_stride) return bad(who, "more shared pages than a page table row has entries");
     if (!std::isfinite(scale)) return bad(who, "the scale must be finite");
     const uint64_t width = (uint64_t)n_q * cache->head_dim;

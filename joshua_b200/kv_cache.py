@@ -93,9 +93,9 @@ class PagedCache:
                          k.data_ptr(), v.data_ptr(), self.head_dim, max(k.shape[1], 1) * self.head_dim, self._bad, stream_of(pos)))
         return k, v
 
-    def scratch(self, batch: int, n_q: int, pages: int, shared_pages: int = 0) -> torch.Tensor:
+    def scratch(self, batch: int, n_q: int, shared_pages: int = 0) -> torch.Tensor:
         """Zeroed scratch for `attend` of such calls, one stream at a time."""
-        n = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, pages, shared_pages)
+        n = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages)
         return torch.zeros(n // 4 + 4, dtype=torch.float32, device=self.device)
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, scale: float = 0.0, shared_pages: int = 0,
@@ -111,10 +111,10 @@ class PagedCache:
             raise JoshuaB200Error(_lib.E_INVALID, f"{batch} query rows, {n} rows of out, {n_seq} of the page table")
         stream = stream_of(q)
         if scratch is None:
-            key = (stream, batch, n_q, per, shared_pages)
+            key = (stream, batch, n_q, shared_pages)
             scratch = self._scratch.get(key)
             if scratch is None:
-                scratch = self._scratch[key] = self.scratch(batch, n_q, per, shared_pages)
+                scratch = self._scratch[key] = self.scratch(batch, n_q, shared_pages)
         check(self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, self.device), pages, batch, per, n_q,
                            scale, shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream))
         return out

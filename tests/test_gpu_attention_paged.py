@@ -198,7 +198,7 @@ def test_strided_rows_another_stream_and_a_graph():
     cache.attend(wide[:, 128:128 + n_q * hd], n, table, n_q=n_q, out=into[:, 4:4 + n_q * hd])
     assert torch.equal(into[:, 4:4 + n_q * hd], want) and bool((into[:, :4] == 2).all()) and bool((into[:, 4 + n_q * hd:] == 2).all())
     torch.cuda.synchronize()
-    side, scratch = torch.cuda.Stream(), cache.scratch(4, n_q, 5)
+    side, scratch = torch.cuda.Stream(), cache.scratch(4, n_q)
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         assert torch.equal(cache.attend(q + 0, n, table, n_q=n_q, scratch=scratch), want)
