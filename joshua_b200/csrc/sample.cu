@@ -8,7 +8,10 @@
 //   min-p  those with exp((l - max) / T) >= min_p.
 // The token is the first id, in order of ids, at which the kept weights' running sum passes trunc(u W'), W' their sum.
 //
-// A cluster of CTAs takes a row, each a slice of it in shared memory: the logits are read once.
+// A cluster of CTAs takes a row, each a slice of it in shared memory: the logits are read once.  The border of top-k or top-p is
+// found from a histogram of the distance to the maximum (numbers or weights of tokens in 2048 equal bins), and within the bin
+// that holds it by comparing its tokens with one another; a bin with too many of them (equal logits) is halved by place instead.
+// With a top-k of up to 1024 all tokens down to its bin go to one CTA, which does the rest.
 #include <cooperative_groups.h>
 
 #include "serving.cuh"
@@ -19,7 +22,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t SM_THREADS = 512, SM_CTAS = 8, SM_WINDOW = 64;
+constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM_WINDOW = 64, SM_BINS = 2048, SM_FEW = 1024;
+
+using u64 = unsigned long long;
 
 // Logits as whole numbers of the same order; NaN and -inf come last, as 0.
 __device__ __forceinline__ uint32_t logit_key(float l) {
@@ -27,15 +32,237 @@ __device__ __forceinline__ uint32_t logit_key(float l) {
     return l > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
 
+struct Few {     // a token among few: its place in the order, its weight
+    u64 place, weight;
+};
 struct SampleShared {
-    float best;
-    unsigned long long sum[2], scan[SM_THREADS / 32];
-    uint32_t cnt[2], red_cnt[SM_THREADS / 32];
-    float red[SM_THREADS / 32];
+    union {
+        struct {
+            uint32_t number[SM_BINS], low[SM_BINS], high[SM_BINS];  // tokens, low and high halves of their weights
+        } bins;
+        Few few[SM_FEW];
+    };
+    float best, least;
+    float red[2][SM_WARPS];
+    uint32_t n_few, n_part, bin;
+    u64 part, border, before, sum, scan[SM_WARPS], scan2[SM_WARPS];
+    uint32_t number, red_number[SM_WARPS];
     int32_t window[SM_WINDOW];
 };
 
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(SampleArgs a) {
+template <class V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V warp_scan(V v, uint32_t lane) {  // sum of this lane's and those in front of it
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const V up = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        v += lane >= o ? up : V(0);
+    }
+    return v;
+}
+
+// trunc(u total), below total
+__device__ __forceinline__ u64 draw_of(float u, u64 total) {
+    const double at = (double)u * (double)total;
+    const u64 r = at >= 1.0 ? (u64)at : 0ull;
+    return total != 0 && r >= total ? total - 1 : r;
+}
+// the weight that top-p keeps of `total`
+__device__ __forceinline__ u64 most_of(float top_p, u64 total) {
+    const double p = (double)top_p * (double)total;
+    return p >= 1.0 ? (u64)p : 1ull;
+}
+
+// A row of logits spread over the cluster, and its rules.
+struct Row {
+    cg::cluster_group cluster;
+    SampleShared& sh;
+    float* l;  // this CTA's slice
+    uint32_t ctas, rank, lo, n, tid, warp, lane;
+    float best, temp, cutoff, to_bin;
+    bool greedy;
+
+    __device__ __forceinline__ float likeness(float x) const {  // exp((l - max) / T)
+        if (!(x > -INFINITY)) return 0.0f;
+        if (x == best) return 1.0f;
+        return !greedy ? expf(__fdiv_rn(__fsub_rn(x, best), temp)) : 0.0f;
+    }
+    __device__ __forceinline__ static u64 weight(float e) { return (u64)__float2ull_rn(e * 4294967296.0f); }
+    __device__ __forceinline__ u64 place(uint32_t i) const { return (u64)logit_key(l[i]) << 32 | (0xFFFFFFFFu - (lo + i)); }
+    // the bin of a logit, SM_BINS for those that weigh nothing: beyond 23 T from the maximum (exp(-23) < 2^-33)
+    __device__ __forceinline__ uint32_t bin(float x) const {
+        if (x == best) return 0;
+        const float d = best - x;
+        return d <= cutoff ? min(SM_BINS - 1, (uint32_t)(d * to_bin)) : SM_BINS;
+    }
+    template <class V>
+    __device__ __forceinline__ V& at(V& v, uint32_t r) const { return *cluster.map_shared_rank(&v, r); }
+
+    // sum over the block, to all of its threads
+    __device__ __forceinline__ u64 block_sum(u64 v) const {
+        v = warp_sum(v);
+        __syncthreads();
+        if (lane == 0) sh.scan[warp] = v;
+        __syncthreads();
+        u64 t = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < SM_WARPS; ++w) t += sh.scan[w];
+        return t;
+    }
+    // number and weight of the tokens at places >= t, over the cluster
+    __device__ void count(u64 t, uint32_t* number, u64* sum) const {
+        uint32_t c = 0;
+        u64 w = 0;
+        for (uint32_t i = tid; i < n; i += SM_THREADS) {
+            if (bin(l[i]) < SM_BINS && place(i) >= t) ++c, w += weight(likeness(l[i]));
+        }
+        const u64 c64 = block_sum(c), w64 = block_sum(w);
+        cluster.sync();  // what was there has been read
+        if (tid == 0) sh.number = (uint32_t)c64, sh.sum = w64;
+        cluster.sync();
+        *number = 0, *sum = 0;
+        for (uint32_t r = 0; r < ctas; ++r) *number += at(sh.number, r), *sum += at(sh.sum, r);
+    }
+
+    // The bin in which the running number of the tokens at places >= from reaches k, or (top_p < 1) their running weight what
+    // top-p keeps; what stands in front of the bin and how many tokens in it.  target: that number or weight.  False
+    // where there are fewer than k tokens; in_bin: how many.
+    __device__ bool border_bin(uint32_t k, float top_p, u64 from, uint32_t* border, u64* before, uint32_t* in_bin, u64* target_out) const {
+        const bool by_weight = top_p < 1.0f;
+        for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) sh.bins.number[i] = sh.bins.low[i] = sh.bins.high[i] = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += SM_THREADS) {
+            const uint32_t b = bin(l[i]);
+            if (b >= SM_BINS || (from != 0 && place(i) < from)) continue;
+            atomicAdd(&sh.bins.number[b], 1);
+            if (by_weight) {  // at most 49152 tokens: both halves' sums stay below 2^32
+                const u64 w = weight(likeness(l[i]));
+                atomicAdd(&sh.bins.low[b], (uint32_t)(w & 0xFFFF)), atomicAdd(&sh.bins.high[b], (uint32_t)(w >> 16));
+            }
+        }
+        cluster.sync();
+        // a run of bins a CTA
+        const uint32_t run = SM_BINS / ctas, b0 = rank * run;
+        constexpr uint32_t MOST = SM_BINS / SM_THREADS;
+        u64 value[MOST], mine = 0;
+        uint32_t number[MOST];
+#pragma unroll
+        for (uint32_t j = 0; j < MOST; ++j) {
+            const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1, b = tid * per + j;
+            value[j] = 0, number[j] = 0;
+            if (j < per && b < run) {
+                for (uint32_t r = 0; r < ctas; ++r) {
+                    number[j] += at(sh.bins.number[b0 + b], r);
+                    if (by_weight) value[j] += at(sh.bins.low[b0 + b], r) + ((u64)at(sh.bins.high[b0 + b], r) << 16);
+                }
+                if (!by_weight) value[j] = number[j];
+            }
+            mine += value[j];
+        }
+        u64 sum = warp_scan(mine, lane);
+        __syncthreads();
+        if (lane == 31) sh.scan[warp] = sum;
+        __syncthreads();
+        u64 all = 0, front = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < SM_WARPS; ++w) front += w < warp ? sh.scan[w] : 0, all += sh.scan[w];
+        sum += front;
+        if (tid == 0) sh.part = all, sh.n_part = 0xFFFFFFFFu;
+        cluster.sync();
+        u64 ahead = 0, whole = 0;
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const u64 x = at(sh.part, r);
+            ahead += r < rank ? x : 0, whole += x;
+        }
+        const u64 target = by_weight ? most_of(top_p, whole) : k;
+        *target_out = target;
+        if (whole < target) {  // the same everywhere
+            *in_bin = (uint32_t)whole;
+            cluster.sync();
+            return false;
+        }
+        u64 upto = ahead + sum - mine;
+#pragma unroll
+        for (uint32_t j = 0; j < MOST; ++j) {
+            if (upto < target && upto + value[j] >= target) {  // one thread of one CTA
+                const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1;
+                for (uint32_t r = 0; r < ctas; ++r) at(sh.bin, r) = b0 + tid * per + j, at(sh.before, r) = upto, at(sh.number, r) = number[j];
+            }
+            upto += value[j];
+        }
+        cluster.sync();
+        *border = sh.bin, *before = sh.before, *in_bin = sh.number;
+        return true;
+    }
+    // The tokens of bins first .. last at places >= from, into the few of CTA 0; there are `SM_FEW` at most.
+    __device__ void gather(uint32_t first, uint32_t last, u64 from) const {
+        cluster.sync();  // the histograms have been read
+        if (rank == 0 && tid == 0) sh.n_few = 0;
+        cluster.sync();
+        uint32_t* counter = cluster.map_shared_rank(&sh.n_few, 0);
+        Few* list = cluster.map_shared_rank(sh.few, 0);
+        for (uint32_t i = tid; i < n; i += SM_THREADS) {
+            const uint32_t b = bin(l[i]);
+            if (b < first || b > last || (from != 0 && place(i) < from)) continue;
+            const uint32_t to = atomicAdd(counter, 1);
+            if (to < SM_FEW) list[to] = Few{place(i), weight(likeness(l[i]))};
+        }
+        cluster.sync();
+    }
+    // The place of the last token that a rule keeps of those at places >= from: the first k, or (top_p < 1) top-p's.
+    __device__ u64 border_place(uint32_t k, float top_p, u64 from) const {
+        const bool by_weight = top_p < 1.0f;
+        uint32_t b, in_bin;
+        u64 before, target;
+        if (!border_bin(k, top_p, from, &b, &before, &in_bin, &target)) return from;
+        if (in_bin <= SM_FEW) {
+            gather(b, b, from);
+            if (rank == 0) {
+                const uint32_t m = sh.n_few;
+                for (uint32_t i = tid; i < m; i += SM_THREADS) {
+                    const Few me = sh.few[i];
+                    u64 ahead = before;
+                    for (uint32_t j = 0; j < m; ++j) {
+                        const Few f = sh.few[j];
+                        if (f.place > me.place) ahead += by_weight ? f.weight : 1;
+                    }
+                    if (ahead < target && ahead + (by_weight ? me.weight : 1) >= target)
+                        for (uint32_t r = 0; r < ctas; ++r) at(sh.border, r) = me.place;
+                }
+            }
+            cluster.sync();
+            return sh.border;
+        }
+        u64 t = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            uint32_t c;
+            u64 w;
+            count(max(from, t | 1ull << bit), &c, &w);
+            if ((by_weight ? w : c) >= target) t |= 1ull << bit;
+        }
+        return max(from, t);
+    }
+};
+
+__device__ __forceinline__ void give(const SampleArgs& a, uint32_t row, int32_t token, float prob) {
+    a.token[row] = token;
+    if (a.prob) a.prob[row] = prob;
+    if (a.pos) a.pos[row] += 1;
+    if (token < 0 || !a.window) return;
+    // the sampled id takes the oldest one's place
+    const int32_t have = a.window_state[2 * row], raw = a.window_state[2 * row + 1];
+    const int32_t next = raw < 0 || raw >= (int32_t)SM_WINDOW ? 0 : raw;
+    a.window[(uint64_t)row * SM_WINDOW + next] = token;
+    a.window_state[2 * row] = min(max(have, 0) + 1, (int32_t)SM_WINDOW);
+    a.window_state[2 * row + 1] = (next + 1) % (int32_t)SM_WINDOW;
+}
+
+__global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
     extern __shared__ float s_l[];  // this CTA's logits
     __shared__ SampleShared sh;
     pdl_trigger_all();
@@ -44,166 +271,180 @@ __global__ void __launch_bounds__(SM_THREADS) sample_kernel(SampleArgs a) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t per = (a.vocab + ctas - 1) / ctas, lo = min(a.vocab, rank * per), n = min(a.vocab, lo + per) - lo;
     const float* src = a.logits + row * a.stride + lo;
-    for (uint32_t i = tid; i < n; i += SM_THREADS) s_l[i] = src[i];
-    // the repetition penalty, on the copy: once for every occurrence in the recent window, by the thread of the first one
-    const uint32_t held = a.window ? min((uint32_t)max(a.window_state[2 * row], 0), SM_WINDOW) : 0;
-    if (tid < held) sh.window[tid] = a.window[(uint64_t)row * SM_WINDOW + tid];
-    __syncthreads();
-    if (tid < held && a.penalty != 1.0f) {
-        const int32_t tok = sh.window[tid];
-        bool first = tok >= (int32_t)lo && tok < (int32_t)(lo + n);
-        uint32_t times = 0;
-        for (uint32_t i = 0; i < held; ++i)
-            if (sh.window[i] == tok) first &= i >= tid, ++times;
-        if (first) {
-            float v = s_l[tok - lo];
-            for (uint32_t i = 0; i < times; ++i) v = v > 0.0f ? v / a.penalty : v * a.penalty;
-            s_l[tok - lo] = v;
-        }
-    }
-    __syncthreads();
-    float best = -INFINITY;
-    for (uint32_t i = tid; i < n; i += SM_THREADS) best = fmaxf(best, s_l[i]);  // NaN is passed over
+    float best = -INFINITY, least = INFINITY;
+    auto see = [&](float v) {  // NaN is passed over
+        best = fmaxf(best, v);
+        if (v > -INFINITY) least = fminf(least, v);
+    };
+    constexpr uint32_t AHEAD = 8;
+    uint32_t i = tid;
+    for (; i + (AHEAD - 1) * SM_THREADS < n; i += AHEAD * SM_THREADS) {
+        float v[AHEAD];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-    if (lane == 0) sh.red[warp] = best;
+        for (uint32_t j = 0; j < AHEAD; ++j) v[j] = __ldg(src + i + j * SM_THREADS);
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j) s_l[i + j * SM_THREADS] = v[j], see(v[j]);
+    }
+    for (; i < n; i += SM_THREADS) {
+        const float v = __ldg(src + i);
+        s_l[i] = v, see(v);
+    }
+    // the repetition penalty, on the copy: once for every occurrence in the recent window, by the thread of the first one
+    const uint32_t held = a.window && a.penalty != 1.0f ? min((uint32_t)max(a.window_state[2 * row], 0), SM_WINDOW) : 0;
+    if (held) {
+        if (tid < held) sh.window[tid] = a.window[(uint64_t)row * SM_WINDOW + tid];
+        __syncthreads();
+        if (tid < held) {
+            const int32_t tok = sh.window[tid];
+            bool first = tok >= (int32_t)lo && tok < (int32_t)(lo + n);
+            uint32_t times = 0;
+            for (uint32_t j = 0; j < held; ++j)
+                if (sh.window[j] == tok) first &= j >= tid, ++times;
+            if (first) {
+                float v = s_l[tok - lo];
+                for (uint32_t j = 0; j < times; ++j) v = v > 0.0f ? v / a.penalty : v * a.penalty;
+                s_l[tok - lo] = v;
+            }
+        }
+        __syncthreads();
+        best = -INFINITY, least = INFINITY;
+        for (uint32_t j = tid; j < n; j += SM_THREADS) see(s_l[j]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
+        least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+    }
+    if (lane == 0) sh.red[0][warp] = best, sh.red[1][warp] = least;
     __syncthreads();
     if (tid == 0) {
-        for (uint32_t w = 1; w < SM_THREADS / 32; ++w) best = fmaxf(best, sh.red[w]);
-        sh.best = best;
+        for (uint32_t w = 1; w < SM_WARPS; ++w) best = fmaxf(best, sh.red[0][w]), least = fminf(least, sh.red[1][w]);
+        sh.best = best, sh.least = least;
     }
     cluster.sync();
-    best = -INFINITY;
-    for (uint32_t r = 0; r < ctas; ++r) best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
-
-    const float temp = a.temperature ? a.temperature[row] : 1.0f, top_p = a.top_p ? a.top_p[row] : 1.0f;
-    const float min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
+    best = -INFINITY, least = INFINITY;
+    for (uint32_t r = 0; r < ctas; ++r) {
+        best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
+        least = fminf(least, *cluster.map_shared_rank(&sh.least, r));
+    }
+    if (!(best > -INFINITY)) {  // nothing to draw: the same in the whole cluster
+        if (rank == 0 && tid == 0) give(a, row, -1, 0.0f);
+        cluster.sync();
+        return;
+    }
+    const float given = a.temperature ? a.temperature[row] : 1.0f, temp = given > 3e38f ? 3e38f : given;  // NaN stays
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
+    const float min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f, u = a.uniform[row];
     const bool greedy = !(temp > 0.0f);
     const uint32_t top_k = greedy ? 1u : a.top_k ? (uint32_t)max(a.top_k[row], 0) : 0u;
-    auto likeness = [&](float l) {  // exp((l - max) / T)
-        if (!(l > -INFINITY)) return 0.0f;
-        if (l == best) return 1.0f;
-        return !greedy ? expf(__fdiv_rn(__fsub_rn(l, best), temp)) : 0.0f;
-    };
-    auto weight = [&](float e) { return (unsigned long long)__float2ull_rn(e * 4294967296.0f); };
-    auto place = [&](uint32_t i) { return (unsigned long long)logit_key(s_l[i]) << 32 | (0xFFFFFFFFu - (lo + i)); };
+    const float cutoff = greedy ? 0.0f : 23.0f * temp;
+    Row r{cluster, sh, s_l, ctas, rank, lo, n, tid, warp, lane, best, temp, cutoff, (float)SM_BINS / fminf(best - least, cutoff), greedy};
 
-    // number and weight of the tokens at places >= t, over the cluster
-    uint32_t turn = 0;
-    auto count = [&](unsigned long long t, uint32_t* number, unsigned long long* sum) {
-        uint32_t c = 0;
-        unsigned long long w = 0;
-        for (uint32_t i = tid; i < n; i += SM_THREADS) {
-            const float l = s_l[i], e = likeness(l);
-            if (place(i) >= t && e > 0.0f) ++c, w += weight(e);
-        }
+    u64 from = 0, total = 0;
+    uint32_t border, in_bin;
+    u64 before, target;
+    if (top_k != 0 && top_k <= SM_FEW) {
+        const bool cut = r.border_bin(top_k, 1.0f, 0, &border, &before, &in_bin, &target);
+        // all tokens down to the bin of the last one kept (or all there are)
+        if ((cut ? before : 0) + in_bin <= SM_FEW) {
+            r.gather(0, cut ? border : SM_BINS - 1, 0);
+            if (rank == 0) {
+                constexpr uint32_t PER = SM_FEW / SM_THREADS;
+                const uint32_t m = sh.n_few;
+                Few me[PER];
+                u64 ahead[PER];
+                bool in[PER];
+                u64 sum = 0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xFFFFFFFFu, c, o), w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-        if (lane == 0) sh.red_cnt[warp] = c, sh.scan[warp] = w;
-        __syncthreads();
-        if (tid == 0) {
-            for (uint32_t i = 1; i < SM_THREADS / 32; ++i) c += sh.red_cnt[i], w += sh.scan[i];
-            sh.cnt[turn & 1] = c, sh.sum[turn & 1] = w;
+                for (uint32_t j = 0; j < PER; ++j) {
+                    const uint32_t at = tid + j * SM_THREADS;
+                    me[j] = at < m ? sh.few[at] : Few{0, 0};
+                    uint32_t ranked = 0;
+                    ahead[j] = 0;
+                    if (at < m)
+                        for (uint32_t x = 0; x < m; ++x) {
+                            const Few f = sh.few[x];
+                            if (f.place > me[j].place) ++ranked, ahead[j] += f.weight;
+                        }
+                    in[j] = at < m && ranked < top_k;
+                    sum += in[j] ? me[j].weight : 0;
+                }
+                total = r.block_sum(sum);
+                const u64 most = top_p < 1.0f ? most_of(top_p, total) : total + 1;
+                sum = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < PER; ++j) {
+                    if (in[j] && ahead[j] < most) {
+                        // the likeness again, from the logit that the place holds
+                        const uint32_t key = (uint32_t)(me[j].place >> 32);
+                        const float x = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+                        in[j] = r.likeness(x) >= min_p;
+                    } else {
+                        in[j] = false;
+                    }
+                    const uint32_t at = tid + j * SM_THREADS;
+                    sum += in[j] ? me[j].weight : 0;
+                    if (at < m && !in[j]) sh.few[at].weight = 0;
+                }
+                total = r.block_sum(sum);
+                const u64 draw = draw_of(u, total);
+#pragma unroll
+                for (uint32_t j = 0; j < PER; ++j) {
+                    if (!in[j]) continue;
+                    u64 lower = 0;  // weights of kept tokens with lower ids: larger in the place's lower half
+                    for (uint32_t x = 0; x < m; ++x) {
+                        const Few f = sh.few[x];
+                        if ((uint32_t)f.place > (uint32_t)me[j].place) lower += f.weight;
+                    }
+                    if (lower <= draw && draw < lower + me[j].weight)
+                        give(a, row, (int32_t)(0xFFFFFFFFu - (uint32_t)me[j].place), (float)((double)me[j].weight / (double)total));
+                }
+            }
+            return;  // the others' memory was last touched in front of the last barrier
         }
-        cluster.sync();
-        *number = 0, *sum = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            *number += *cluster.map_shared_rank(&sh.cnt[turn & 1], r);
-            *sum += *cluster.map_shared_rank(&sh.sum[turn & 1], r);
-        }
-        ++turn;  // the other pair next: this one may still be read
-    };
-    uint32_t number;
-    unsigned long long total, from = 0;
-    count(from, &number, &total);
-    if (top_k != 0 && number > top_k) {
-        unsigned long long t = 0;
-        for (int bit = 63; bit >= 0; --bit) {  // the largest place with top_k tokens from it on
-            uint32_t c;
-            unsigned long long w;
-            count(t | 1ull << bit, &c, &w);
-            if (c >= top_k) t |= 1ull << bit;
-        }
-        from = t;
-        count(from, &number, &total);
     }
-    if (top_p < 1.0f && total != 0) {
-        const double p = (double)top_p * (double)total;
-        const unsigned long long most = p >= 1.0 ? (unsigned long long)p : 1ull;
-        unsigned long long t = 0;
-        for (int bit = 63; bit >= 0; --bit) {  // the largest place with at least `most` from it on
-            uint32_t c;
-            unsigned long long w;
-            count(t | 1ull << bit, &c, &w);
-            if (w >= most) t |= 1ull << bit;
-        }
-        from = max(from, t);
-    }
+    if (top_k != 0) from = r.border_place(top_k, 1.0f, 0);
+    if (top_p < 1.0f) from = r.border_place(0, top_p, from);
     // the kept weights of this CTA, warp by warp in order of ids
-    const uint32_t seg = (n + SM_THREADS / 32 - 1) / (SM_THREADS / 32), s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
-    auto kept = [&](uint32_t i) -> unsigned long long {
-        const float e = likeness(s_l[i]);
-        return place(i) >= from && e >= min_p ? weight(e) : 0ull;
+    const uint32_t seg = (n + SM_WARPS - 1) / SM_WARPS, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
+    auto kept = [&](uint32_t x) -> u64 {
+        if (r.bin(s_l[x]) >= SM_BINS || (from != 0 && r.place(x) < from)) return 0;
+        const float e = r.likeness(s_l[x]);
+        return e >= min_p ? Row::weight(e) : 0ull;
     };
-    unsigned long long w = 0;
-    for (uint32_t i = s0 + lane; i < s1; i += 32) w += kept(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+    u64 w = 0;
+    for (uint32_t x = s0 + lane; x < s1; x += 32) w += kept(x);
+    w = warp_sum(w);
     __syncthreads();
-    if (lane == 0) sh.scan[warp] = w;
+    if (lane == 0) sh.scan2[warp] = w;
     __syncthreads();
     if (tid == 0) {
-        unsigned long long all = 0;
-        for (uint32_t i = 0; i < SM_THREADS / 32; ++i) all += sh.scan[i];
-        sh.sum[turn & 1] = all;
+        u64 all = 0;
+        for (uint32_t x = 0; x < SM_WARPS; ++x) all += sh.scan2[x];
+        sh.part = all;
     }
     cluster.sync();
-    unsigned long long before = 0, all = 0;
-    for (uint32_t r = 0; r < ctas; ++r) {
-        const unsigned long long x = *cluster.map_shared_rank(&sh.sum[turn & 1], r);
-        before += r < rank ? x : 0, all += x;
+    u64 ahead = 0;
+    total = 0;
+    for (uint32_t x = 0; x < ctas; ++x) {
+        const u64 v = *cluster.map_shared_rank(&sh.part, x);
+        ahead += x < rank ? v : 0, total += v;
     }
-    const double at = (double)a.uniform[row] * (double)all;
-    unsigned long long r = at >= 1.0 ? (unsigned long long)at : 0ull;
-    r = all != 0 && r >= all ? all - 1 : r;
-    int32_t token = -1;
-    if (all == 0) {
-        if (rank == 0 && tid == 0) {
-            a.token[row] = -1;
-            if (a.prob) a.prob[row] = 0.0f;
-        }
-    } else {
-        for (uint32_t i = 0; i < warp; ++i) before += sh.scan[i];
-        if (before <= r && r < before + w) {  // one warp of one CTA
-            for (uint32_t i = s0; i < s1; i += 32) {
-                const unsigned long long mine = i + lane < s1 ? kept(i + lane) : 0ull;
-                unsigned long long run = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, run, o);
-                    run += lane >= o ? up : 0;
-                }
-                const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + run > r);
-                if (past) {
-                    if (lane == __ffs(past) - 1) {
-                        token = (int32_t)(lo + i + lane);
-                        a.token[row] = token;
-                        if (a.prob) a.prob[row] = (float)((double)mine / (double)all);
-                    }
-                    break;
-                }
-                before += __shfl_sync(0xFFFFFFFFu, run, 31);
+    const u64 draw = draw_of(u, total);
+    for (uint32_t x = 0; x < warp; ++x) ahead += sh.scan2[x];
+    if (ahead <= draw && draw < ahead + w) {  // one warp of one CTA
+        for (uint32_t x = s0; x < s1; x += 32) {
+            const u64 mine = x + lane < s1 ? kept(x + lane) : 0ull;
+            const u64 run = warp_scan(mine, lane);
+            const uint32_t past = __ballot_sync(0xFFFFFFFFu, ahead + run > draw);
+            if (past) {
+                if (lane == __ffs(past) - 1) give(a, row, (int32_t)(lo + x + lane), (float)((double)mine / (double)total));
+                x = s1;
+            } else {
+                ahead += __shfl_sync(0xFFFFFFFFu, run, 31);
             }
         }
     }
-    if (token >= 0 && a.window) {  // the sampled id takes the oldest one's place
-        const int32_t have = a.window_state[2 * row], raw = a.window_state[2 * row + 1];
-        const int32_t next = raw < 0 || raw >= (int32_t)SM_WINDOW ? 0 : raw;
-        a.window[(uint64_t)row * SM_WINDOW + next] = token;
-        a.window_state[2 * row] = min(max(have, 0) + 1, (int32_t)SM_WINDOW);
-        a.window_state[2 * row + 1] = (next + 1) % (int32_t)SM_WINDOW;
-    }
-    if (a.pos && rank == 0 && tid == 0) a.pos[row] += 1;
     cluster.sync();  // shared memory is read from the others until here
 }
 
