@@ -11,7 +11,7 @@
 // A cluster of CTAs takes a row, each a slice of it in shared memory: the logits are read once.  The border of top-k or top-p is
 // found from a histogram of the distance to the maximum (numbers or weights of tokens in 2048 equal bins), and within the bin
 // that holds it by comparing its tokens with one another; a bin with too many of them (equal logits) is halved by place instead.
-// With a top-k of up to 1024 all tokens down to its bin go to one CTA, which does the rest.
+// Where a top-k and the rest of its bin are 2048 tokens at most, they go to one CTA, which does the rest.
 #include <cooperative_groups.h>
 
 #include "serving.cuh"
@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM_WINDOW = 64, SM_BINS = 2048, SM_FEW = 1024;
+constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM_WINDOW = 64, SM_BINS = 2048, SM_FEW = 2048;
 
 using u64 = unsigned long long;
 
@@ -114,6 +114,16 @@ struct Row {
         for (uint32_t w = 0; w < SM_WARPS; ++w) t += sh.scan[w];
         return t;
     }
+    // sum of this thread's and those in front of it
+    __device__ __forceinline__ u64 block_scan(u64 v) const {
+        v = warp_scan(v, lane);
+        __syncthreads();
+        if (lane == 31) sh.scan[warp] = v;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < SM_WARPS; ++w) v += w < warp ? sh.scan[w] : 0;
+        return v;
+    }
     // number and weight of the tokens at places >= t, over the cluster
     __device__ void count(u64 t, uint32_t* number, u64* sum) const {
         uint32_t c = 0;
@@ -199,20 +209,49 @@ struct Row {
         *border = sh.bin, *before = sh.before, *in_bin = sh.number;
         return true;
     }
-    // The tokens of bins first .. last at places >= from, into the few of CTA 0; there are `SM_FEW` at most.
-    __device__ void gather(uint32_t first, uint32_t last, u64 from) const {
+    // The tokens of bins first .. last at places >= from, in CTA 0's list (the number of them returned there): SM_FEW at most.
+    __device__ uint32_t gather(uint32_t first, uint32_t last, u64 from) const {
+        if (tid == 0) sh.n_few = 0;
         cluster.sync();  // the histograms have been read
-        if (rank == 0 && tid == 0) sh.n_few = 0;
-        cluster.sync();
-        uint32_t* counter = cluster.map_shared_rank(&sh.n_few, 0);
-        Few* list = cluster.map_shared_rank(sh.few, 0);
-        for (uint32_t i = tid; i < n; i += SM_THREADS) {
-            const uint32_t b = bin(l[i]);
-            if (b < first || b > last || (from != 0 && place(i) < from)) continue;
-            const uint32_t to = atomicAdd(counter, 1);
-            if (to < SM_FEW) list[to] = Few{place(i), weight(likeness(l[i]))};
+        for (uint32_t i = tid; i < (n + 31) / 32 * 32; i += SM_THREADS) {
+            const uint32_t b = i < n ? bin(l[i]) : SM_BINS;
+            const bool in = b >= first && b <= last && (from == 0 || place(i) >= from);
+            const uint32_t all = __ballot_sync(0xFFFFFFFFu, in);
+            if (all == 0) continue;
+            uint32_t to = 0;
+            if (lane == 0) to = atomicAdd(&sh.n_few, __popc(all));
+            to = __shfl_sync(0xFFFFFFFFu, to, 0) + __popc(all & ((1u << lane) - 1));
+            if (in && to < SM_FEW) sh.few[to] = Few{place(i), weight(likeness(l[i]))};
         }
         cluster.sync();
+        uint32_t m = min(sh.n_few, SM_FEW);
+        if (rank == 0) {
+            for (uint32_t r = 1; r < ctas; ++r) {
+                const uint32_t more = min(at(sh.n_few, r), SM_FEW - m);
+                const Few* list = cluster.map_shared_rank(sh.few, r);
+                for (uint32_t i = tid; i < more; i += SM_THREADS) sh.few[m + i] = list[i];
+                m += more;
+            }
+        }
+        cluster.sync();
+        return m;
+    }
+    // The m tokens of this CTA's list in order of place, the largest first: a bitonic sort; the steps up to 32 apart stay within
+    // a warp's 64 tokens.
+    __device__ void sort(uint32_t m) const {
+        uint32_t size = 64;
+        while (size < m) size *= 2;
+        for (uint32_t i = m + tid; i < size; i += SM_THREADS) sh.few[i] = Few{0, 0};
+        for (uint32_t run = 2; run <= size; run *= 2)
+            for (uint32_t gap = run / 2; gap > 0; gap /= 2) {
+                if (gap >= 32 || run == 2) __syncthreads(); else __syncwarp();
+                for (uint32_t t = tid; t < size / 2; t += SM_THREADS) {
+                    const uint32_t i = 2 * t - (t & (gap - 1)), j = i + gap;
+                    const Few x = sh.few[i], y = sh.few[j];
+                    if ((x.place < y.place) == ((i & run) == 0)) sh.few[i] = y, sh.few[j] = x;
+                }
+            }
+        __syncthreads();
     }
     // The place of the last token that a rule keeps of those at places >= from: the first k, or (top_p < 1) top-p's.
     __device__ u64 border_place(uint32_t k, float top_p, u64 from) const {
@@ -221,18 +260,23 @@ struct Row {
         u64 before, target;
         if (!border_bin(k, top_p, from, &b, &before, &in_bin, &target)) return from;
         if (in_bin <= SM_FEW) {
-            gather(b, b, from);
+            const uint32_t m = gather(b, b, from);
             if (rank == 0) {
-                const uint32_t m = sh.n_few;
-                for (uint32_t i = tid; i < m; i += SM_THREADS) {
-                    const Few me = sh.few[i];
-                    u64 ahead = before;
-                    for (uint32_t j = 0; j < m; ++j) {
-                        const Few f = sh.few[j];
-                        if (f.place > me.place) ahead += by_weight ? f.weight : 1;
-                    }
-                    if (ahead < target && ahead + (by_weight ? me.weight : 1) >= target)
-                        for (uint32_t r = 0; r < ctas; ++r) at(sh.border, r) = me.place;
+                sort(m);
+                constexpr uint32_t PER = SM_FEW / SM_THREADS;
+                u64 w[PER], mine = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < PER; ++j) {
+                    const uint32_t i = tid * PER + j;
+                    w[j] = i >= m ? 0 : by_weight ? sh.few[i].weight : 1;
+                    mine += w[j];
+                }
+                u64 ahead = before + block_scan(mine) - mine;
+#pragma unroll
+                for (uint32_t j = 0; j < PER; ++j) {
+                    if (ahead < target && ahead + w[j] >= target)
+                        for (uint32_t r = 0; r < ctas; ++r) at(sh.border, r) = sh.few[tid * PER + j].place;
+                    ahead += w[j];
                 }
             }
             cluster.sync();
@@ -347,58 +391,46 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
         const bool cut = r.border_bin(top_k, 1.0f, 0, &border, &before, &in_bin, &target);
         // all tokens down to the bin of the last one kept (or all there are)
         if ((cut ? before : 0) + in_bin <= SM_FEW) {
-            r.gather(0, cut ? border : SM_BINS - 1, 0);
+            const uint32_t m = r.gather(0, cut ? border : SM_BINS - 1, 0);
             if (rank == 0) {
-                constexpr uint32_t PER = SM_FEW / SM_THREADS;
-                const uint32_t m = sh.n_few;
-                Few me[PER];
-                u64 ahead[PER];
-                bool in[PER];
-                u64 sum = 0;
+                r.sort(m);
+                constexpr uint32_t PER = SM_FEW / SM_THREADS;  // tokens PER tid .. of the order
+                u64 w[PER], sum = 0;
+                uint32_t id[PER];
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
-                    const uint32_t at = tid + j * SM_THREADS;
-                    me[j] = at < m ? sh.few[at] : Few{0, 0};
-                    uint32_t ranked = 0;
-                    ahead[j] = 0;
-                    if (at < m)
-                        for (uint32_t x = 0; x < m; ++x) {
-                            const Few f = sh.few[x];
-                            if (f.place > me[j].place) ++ranked, ahead[j] += f.weight;
-                        }
-                    in[j] = at < m && ranked < top_k;
-                    sum += in[j] ? me[j].weight : 0;
+                    const uint32_t at = tid * PER + j;
+                    w[j] = at < min(m, top_k) ? sh.few[at].weight : 0;
+                    sum += w[j];
                 }
+                u64 ahead = r.block_scan(sum) - sum;
                 total = r.block_sum(sum);
-                const u64 most = top_p < 1.0f ? most_of(top_p, total) : total + 1;
+                const u64 most = top_p < 1.0f ? most_of(top_p, total) : total;
                 sum = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
-                    if (in[j] && ahead[j] < most) {
-                        // the likeness again, from the logit that the place holds
-                        const uint32_t key = (uint32_t)(me[j].place >> 32);
-                        const float x = __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
-                        in[j] = r.likeness(x) >= min_p;
-                    } else {
-                        in[j] = false;
-                    }
-                    const uint32_t at = tid + j * SM_THREADS;
-                    sum += in[j] ? me[j].weight : 0;
-                    if (at < m && !in[j]) sh.few[at].weight = 0;
+                    const u64 place = w[j] ? sh.few[tid * PER + j].place : 0;
+                    const uint32_t key = (uint32_t)(place >> 32);
+                    id[j] = 0xFFFFFFFFu - (uint32_t)place;
+                    const u64 mine = w[j];
+                    // the likeness again, from the logit that the place holds
+                    if (ahead >= most || (min_p > 0.0f && !(r.likeness(__uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key)) >= min_p)))
+                        w[j] = 0;
+                    ahead += mine, sum += w[j];
                 }
                 total = r.block_sum(sum);
                 const u64 draw = draw_of(u, total);
+                // the first id at which the weights pass the draw: the ids below it weigh at most that
+                uint32_t below = 0;
+                for (uint32_t bit = 1u << (31 - __clz(a.vocab)); bit != 0; bit >>= 1) {
+                    sum = 0;
 #pragma unroll
-                for (uint32_t j = 0; j < PER; ++j) {
-                    if (!in[j]) continue;
-                    u64 lower = 0;  // weights of kept tokens with lower ids: larger in the place's lower half
-                    for (uint32_t x = 0; x < m; ++x) {
-                        const Few f = sh.few[x];
-                        if ((uint32_t)f.place > (uint32_t)me[j].place) lower += f.weight;
-                    }
-                    if (lower <= draw && draw < lower + me[j].weight)
-                        give(a, row, (int32_t)(0xFFFFFFFFu - (uint32_t)me[j].place), (float)((double)me[j].weight / (double)total));
+                    for (uint32_t j = 0; j < PER; ++j) sum += id[j] < (below | bit) ? w[j] : 0;
+                    if (r.block_sum(sum) <= draw) below |= bit;
                 }
+#pragma unroll
+                for (uint32_t j = 0; j < PER; ++j)
+                    if (w[j] && id[j] == below) give(a, row, (int32_t)below, (float)((double)w[j] / (double)total));
             }
             return;  // the others' memory was last touched in front of the last barrier
         }
