@@ -82,8 +82,10 @@ __device__ __forceinline__ u64 most_of(float top_p, u64 total) {
 struct Row {
     cg::cluster_group cluster;
     SampleShared& sh;
-    float* l;  // this CTA's slice
-    uint32_t ctas, rank, lo, n, tid, warp, lane;
+    float* l;         // this CTA's slice, padded with NaN to whole vectors on both sides
+    int32_t lo;       // id of its first place
+    uint32_t n;       // places, a multiple of 4
+    uint32_t ctas, rank, tid, warp, lane;
     float best, temp, cutoff, to_bin;
     bool greedy;
 
@@ -93,7 +95,16 @@ struct Row {
         return !greedy ? expf(__fdiv_rn(__fsub_rn(x, best), temp)) : 0.0f;
     }
     __device__ __forceinline__ static u64 weight(float e) { return (u64)__float2ull_rn(e * 4294967296.0f); }
-    __device__ __forceinline__ u64 place(uint32_t i) const { return (u64)logit_key(l[i]) << 32 | (0xFFFFFFFFu - (lo + i)); }
+    __device__ __forceinline__ u64 place(uint32_t i) const { return (u64)logit_key(l[i]) << 32 | (0xFFFFFFFFu - (uint32_t)(lo + (int32_t)i)); }
+    // f(logit, place) of the whole slice, in no order
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 2
+        for (uint32_t v = tid; v < n / 4; v += SM_THREADS) {
+            const float4 x = reinterpret_cast<const float4*>(l)[v];
+            f(x.x, 4 * v), f(x.y, 4 * v + 1), f(x.z, 4 * v + 2), f(x.w, 4 * v + 3);
+        }
+    }
     // the bin of a logit, SM_BINS for those that weigh nothing: beyond 23 T from the maximum (exp(-23) < 2^-33)
     __device__ __forceinline__ uint32_t bin(float x) const {
         if (x == best) return 0;
@@ -128,9 +139,9 @@ struct Row {
     __device__ void count(u64 t, uint32_t* number, u64* sum) const {
         uint32_t c = 0;
         u64 w = 0;
-        for (uint32_t i = tid; i < n; i += SM_THREADS) {
-            if (bin(l[i]) < SM_BINS && place(i) >= t) ++c, w += weight(likeness(l[i]));
-        }
+        each([&](float x, uint32_t i) {
+            if (bin(x) < SM_BINS && place(i) >= t) ++c, w += weight(likeness(x));
+        });
         const u64 c64 = block_sum(c), w64 = block_sum(w);
         cluster.sync();  // what was there has been read
         if (tid == 0) sh.number = (uint32_t)c64, sh.sum = w64;
@@ -144,17 +155,21 @@ struct Row {
     // where there are fewer than k tokens; in_bin: how many.
     __device__ bool border_bin(uint32_t k, float top_p, u64 from, uint32_t* border, u64* before, uint32_t* in_bin, u64* target_out) const {
         const bool by_weight = top_p < 1.0f;
-        for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) sh.bins.number[i] = sh.bins.low[i] = sh.bins.high[i] = 0;
+        for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) {
+            sh.bins.number[i] = 0;
+            if (by_weight) sh.bins.low[i] = sh.bins.high[i] = 0;
+        }
+        if (tid == 0) sh.n_few = 0;
         __syncthreads();
-        for (uint32_t i = tid; i < n; i += SM_THREADS) {
-            const uint32_t b = bin(l[i]);
-            if (b >= SM_BINS || (from != 0 && place(i) < from)) continue;
+        each([&](float x, uint32_t i) {
+            const uint32_t b = bin(x);
+            if (b >= SM_BINS || (from != 0 && place(i) < from)) return;
             atomicAdd(&sh.bins.number[b], 1);
             if (by_weight) {  // at most 49152 tokens: both halves' sums stay below 2^32
-                const u64 w = weight(likeness(l[i]));
+                const u64 w = weight(likeness(x));
                 atomicAdd(&sh.bins.low[b], (uint32_t)(w & 0xFFFF)), atomicAdd(&sh.bins.high[b], (uint32_t)(w >> 16));
             }
-        }
+        });
         cluster.sync();
         // a run of bins a CTA
         const uint32_t run = SM_BINS / ctas, b0 = rank * run;
@@ -209,20 +224,16 @@ struct Row {
         *border = sh.bin, *before = sh.before, *in_bin = sh.number;
         return true;
     }
-    // The tokens of bins first .. last at places >= from, in CTA 0's list (the number of them returned there): SM_FEW at most.
+    // Behind border_bin: the tokens of bins first .. last at places >= from, in CTA 0's list (their number returned there);
+    // SM_FEW at most.
     __device__ uint32_t gather(uint32_t first, uint32_t last, u64 from) const {
-        if (tid == 0) sh.n_few = 0;
-        cluster.sync();  // the histograms have been read
-        for (uint32_t i = tid; i < (n + 31) / 32 * 32; i += SM_THREADS) {
-            const uint32_t b = i < n ? bin(l[i]) : SM_BINS;
-            const bool in = b >= first && b <= last && (from == 0 || place(i) >= from);
-            const uint32_t all = __ballot_sync(0xFFFFFFFFu, in);
-            if (all == 0) continue;
-            uint32_t to = 0;
-            if (lane == 0) to = atomicAdd(&sh.n_few, __popc(all));
-            to = __shfl_sync(0xFFFFFFFFu, to, 0) + __popc(all & ((1u << lane) - 1));
-            if (in && to < SM_FEW) sh.few[to] = Few{place(i), weight(likeness(l[i]))};
-        }
+        // the histograms have been read in front of the last barrier
+        each([&](float x, uint32_t i) {
+            const uint32_t b = bin(x);
+            if (b < first || b > last || (from != 0 && place(i) < from)) return;
+            const uint32_t to = atomicAdd(&sh.n_few, 1);
+            if (to < SM_FEW) sh.few[to] = Few{place(i), weight(likeness(x))};
+        });
         cluster.sync();
         uint32_t m = min(sh.n_few, SM_FEW);
         if (rank == 0) {
@@ -306,32 +317,45 @@ __device__ __forceinline__ void give(const SampleArgs& a, uint32_t row, int32_t 
     a.window_state[2 * row + 1] = (next + 1) % (int32_t)SM_WINDOW;
 }
 
-__global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
-    extern __shared__ float s_l[];  // this CTA's logits
+__global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
+    extern __shared__ __align__(16) float s_l[];  // this CTA's logits
     __shared__ SampleShared sh;
     pdl_trigger_all();
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.y;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t per = (a.vocab + ctas - 1) / ctas, lo = min(a.vocab, rank * per), n = min(a.vocab, lo + per) - lo;
-    const float* src = a.logits + row * a.stride + lo;
+    // slices end where the row's 16-byte vectors do; a vector that is not the row's throughout is read by its own logits
+    const float* src = a.logits + row * a.stride;
+    const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(src) / 4 % 4), vecs = (shift + a.vocab + 3) / 4;
+    const uint32_t per = (vecs + ctas - 1) / ctas, v0 = min(vecs, rank * per), n = 4 * (min(vecs, v0 + per) - v0);
+    const int32_t lo = (int32_t)(4 * v0) - (int32_t)shift;
+    src += lo;
     float best = -INFINITY, least = INFINITY;
     auto see = [&](float v) {  // NaN is passed over
         best = fmaxf(best, v);
         if (v > -INFINITY) least = fminf(least, v);
     };
-    constexpr uint32_t AHEAD = 8;
-    uint32_t i = tid;
-    for (; i + (AHEAD - 1) * SM_THREADS < n; i += AHEAD * SM_THREADS) {
-        float v[AHEAD];
+    constexpr uint32_t AHEAD = 4;
+    for (uint32_t v = tid; v < n / 4; v += AHEAD * SM_THREADS) {
+        float4 x[AHEAD];
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; ++j) v[j] = __ldg(src + i + j * SM_THREADS);
+        for (uint32_t j = 0; j < AHEAD; ++j) {
+            const uint32_t at = v + j * SM_THREADS;
+            const int32_t id = lo + 4 * (int32_t)at;
+            if (at < n / 4 && id >= 0 && id + 4 <= (int32_t)a.vocab) {
+                x[j] = __ldg(reinterpret_cast<const float4*>(src) + at);
+            } else {
+                float* e = &x[j].x;
 #pragma unroll
-        for (uint32_t j = 0; j < AHEAD; ++j) s_l[i + j * SM_THREADS] = v[j], see(v[j]);
-    }
-    for (; i < n; i += SM_THREADS) {
-        const float v = __ldg(src + i);
-        s_l[i] = v, see(v);
+                for (int k = 0; k < 4; ++k)
+                    e[k] = at < n / 4 && id + k >= 0 && id + k < (int32_t)a.vocab ? __ldg(src + 4 * (int32_t)at + k) : NAN;
+            }
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; ++j) {
+            if (v + j * SM_THREADS < n / 4) reinterpret_cast<float4*>(s_l)[v + j * SM_THREADS] = x[j];
+            see(x[j].x), see(x[j].y), see(x[j].z), see(x[j].w);
+        }
     }
     // the repetition penalty, on the copy: once for every occurrence in the recent window, by the thread of the first one
     const uint32_t held = a.window && a.penalty != 1.0f ? min((uint32_t)max(a.window_state[2 * row], 0), SM_WINDOW) : 0;
@@ -340,7 +364,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
         __syncthreads();
         if (tid < held) {
             const int32_t tok = sh.window[tid];
-            bool first = tok >= (int32_t)lo && tok < (int32_t)(lo + n);
+            bool first = tok >= max(lo, 0) && tok < min(lo + (int32_t)n, (int32_t)a.vocab);
             uint32_t times = 0;
             for (uint32_t j = 0; j < held; ++j)
                 if (sh.window[j] == tok) first &= j >= tid, ++times;
@@ -382,7 +406,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
     const bool greedy = !(temp > 0.0f);
     const uint32_t top_k = greedy ? 1u : a.top_k ? (uint32_t)max(a.top_k[row], 0) : 0u;
     const float cutoff = greedy ? 0.0f : 23.0f * temp;
-    Row r{cluster, sh, s_l, ctas, rank, lo, n, tid, warp, lane, best, temp, cutoff, (float)SM_BINS / fminf(best - least, cutoff), greedy};
+    Row r{cluster, sh, s_l, lo, n, ctas, rank, tid, warp, lane, best, temp, cutoff, (float)SM_BINS / fminf(best - least, cutoff), greedy};
 
     u64 from = 0, total = 0;
     uint32_t border, in_bin;
@@ -470,7 +494,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
             const u64 run = warp_scan(mine, lane);
             const uint32_t past = __ballot_sync(0xFFFFFFFFu, ahead + run > draw);
             if (past) {
-                if (lane == __ffs(past) - 1) give(a, row, (int32_t)(lo + x + lane), (float)((double)mine / (double)total));
+                if (lane == __ffs(past) - 1) give(a, row, lo + (int32_t)(x + lane), (float)((double)mine / (double)total));
                 x = s1;
             } else {
                 ahead += __shfl_sync(0xFFFFFFFFu, run, 31);
@@ -485,9 +509,9 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(SampleArgs a) {
 cudaError_t launch_sample(const SampleArgs& a, uint32_t rows, cudaStream_t s) {
     uint32_t ctas = 1;
     while (ctas < SM_CTAS && a.vocab > ctas * 4096) ctas *= 2;
-    const size_t smem = (size_t)((a.vocab + ctas - 1) / ctas) * 4;
+    const size_t smem = ((a.vocab + 3 + 3) / 4 + ctas - 1) / ctas * 16;  // of a row that begins inside a vector
     static bool configured[MAX_DEVICES] = {};
-    if (cudaError_t e = set_max_smem_once(sample_kernel, SAMPLE_MAX_VOCAB / SM_CTAS * 4, configured); e != cudaSuccess) return e;
+    if (cudaError_t e = set_max_smem_once(sample_kernel, SAMPLE_MAX_VOCAB / SM_CTAS * 4 + 16, configured); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, rows);
     cfg.blockDim = dim3(SM_THREADS);
