@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM_WINDOW = 64, SM_BINS = 2048, SM_FEW = 2048;
+constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM_MOST_CTAS = 16, SM_WINDOW = 64, SM_BINS = 2048, SM_FEW = 2048;
 
 using u64 = unsigned long long;
 
@@ -44,9 +44,8 @@ struct SampleShared {
     };
     float best, least;
     float red[2][SM_WARPS];
-    uint32_t n_few, n_part, bin;
+    uint32_t n_few, bin, number;
     u64 part, border, before, sum, scan[SM_WARPS], scan2[SM_WARPS];
-    uint32_t number, red_number[SM_WARPS];
     int32_t window[SM_WINDOW];
 };
 
@@ -92,9 +91,11 @@ struct Row {
     __device__ __forceinline__ float likeness(float x) const {  // exp((l - max) / T)
         if (!(x > -INFINITY)) return 0.0f;
         if (x == best) return 1.0f;
-        return !greedy ? expf(__fdiv_rn(__fsub_rn(x, best), temp)) : 0.0f;
+        const float d = __fsub_rn(x, best);
+        return !greedy ? expf(temp == 1.0f ? d : __fdiv_rn(d, temp)) : 0.0f;
     }
-    __device__ __forceinline__ static u64 weight(float e) { return (u64)__float2ull_rn(e * 4294967296.0f); }
+    __device__ __forceinline__ static float weight_float(float e) { return rintf(e * 4294967296.0f); }
+    __device__ __forceinline__ static u64 weight(float e) { return (u64)weight_float(e); }
     __device__ __forceinline__ u64 place(uint32_t i) const { return (u64)logit_key(l[i]) << 32 | (0xFFFFFFFFu - (uint32_t)(lo + (int32_t)i)); }
     // f(logit, place) of the whole slice, in no order
     template <class F>
@@ -197,7 +198,7 @@ struct Row {
 #pragma unroll
         for (uint32_t w = 0; w < SM_WARPS; ++w) front += w < warp ? sh.scan[w] : 0, all += sh.scan[w];
         sum += front;
-        if (tid == 0) sh.part = all, sh.n_part = 0xFFFFFFFFu;
+        if (tid == 0) sh.part = all;
         cluster.sync();
         u64 ahead = 0, whole = 0;
         for (uint32_t r = 0; r < ctas; ++r) {
@@ -235,13 +236,15 @@ struct Row {
             if (to < SM_FEW) sh.few[to] = Few{place(i), weight(likeness(x))};
         });
         cluster.sync();
-        uint32_t m = min(sh.n_few, SM_FEW);
+        uint32_t m = 0;
         if (rank == 0) {
-            for (uint32_t r = 1; r < ctas; ++r) {
-                const uint32_t more = min(at(sh.n_few, r), SM_FEW - m);
+            uint32_t mine = lane < ctas ? min(at(sh.n_few, lane), SM_FEW) : 0;
+            const uint32_t upto = warp_scan(mine, lane);
+            m = min(__shfl_sync(0xFFFFFFFFu, upto, 31), SM_FEW);
+            for (uint32_t r = 1 + warp; r < ctas; r += SM_WARPS) {  // a warp a list
+                const uint32_t more = __shfl_sync(0xFFFFFFFFu, mine, r), to = __shfl_sync(0xFFFFFFFFu, upto, r) - more;
                 const Few* list = cluster.map_shared_rank(sh.few, r);
-                for (uint32_t i = tid; i < more; i += SM_THREADS) sh.few[m + i] = list[i];
-                m += more;
+                for (uint32_t i = lane; i < more && to + i < SM_FEW; i += 32) sh.few[to + i] = list[i];
             }
         }
         cluster.sync();
@@ -444,61 +447,75 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
                 }
                 total = r.block_sum(sum);
                 const u64 draw = draw_of(u, total);
-                // the first id at which the weights pass the draw: the ids below it weigh at most that
-                uint32_t below = 0;
-                for (uint32_t bit = 1u << (31 - __clz(a.vocab)); bit != 0; bit >>= 1) {
-                    sum = 0;
+                // the first id at which the kept weights, in order of ids, pass the draw
+                uint32_t kept = 0;
 #pragma unroll
-                    for (uint32_t j = 0; j < PER; ++j) sum += id[j] < (below | bit) ? w[j] : 0;
-                    if (r.block_sum(sum) <= draw) below |= bit;
+                for (uint32_t j = 0; j < PER; ++j) kept += w[j] != 0;
+                kept = (uint32_t)r.block_sum(kept);  // the first ones of the order
+                if (kept <= SM_THREADS / 2) {        // each adds up those below it
+                    if (tid < kept) {
+                        const Few me = sh.few[tid];
+                        u64 below = 0;
+                        for (uint32_t x = 0; x < kept; ++x) {
+                            const Few f = sh.few[x];
+                            below += (uint32_t)f.place > (uint32_t)me.place ? f.weight : 0;
+                        }
+                        if (below <= draw && draw < below + me.weight)
+                            give(a, row, (int32_t)(0xFFFFFFFFu - (uint32_t)me.place), (float)((double)me.weight / (double)total));
+                    }
+                } else {  // bit by bit: the ids below it weigh at most the draw
+                    uint32_t below = 0;
+                    for (uint32_t bit = 1u << (31 - __clz(a.vocab)); bit != 0; bit >>= 1) {
+                        sum = 0;
+#pragma unroll
+                        for (uint32_t j = 0; j < PER; ++j) sum += id[j] < (below | bit) ? w[j] : 0;
+                        if (r.block_sum(sum) <= draw) below |= bit;
+                    }
+#pragma unroll
+                    for (uint32_t j = 0; j < PER; ++j)
+                        if (w[j] && id[j] == below) give(a, row, (int32_t)below, (float)((double)w[j] / (double)total));
                 }
-#pragma unroll
-                for (uint32_t j = 0; j < PER; ++j)
-                    if (w[j] && id[j] == below) give(a, row, (int32_t)below, (float)((double)w[j] / (double)total));
             }
             return;  // the others' memory was last touched in front of the last barrier
         }
     }
     if (top_k != 0) from = r.border_place(top_k, 1.0f, 0);
     if (top_p < 1.0f) from = r.border_place(0, top_p, from);
-    // the kept weights of this CTA, warp by warp in order of ids
+    // the kept weights of this CTA, run by run of ids, a run a warp; as whole numbers in 64-bit floats, exact below 2^53
     const uint32_t seg = (n + SM_WARPS - 1) / SM_WARPS, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
-    auto kept = [&](uint32_t x) -> u64 {
-        if (r.bin(s_l[x]) >= SM_BINS || (from != 0 && r.place(x) < from)) return 0;
+    auto kept = [&](uint32_t x) -> float {
+        if (r.bin(s_l[x]) >= SM_BINS || (from != 0 && r.place(x) < from)) return 0.0f;
         const float e = r.likeness(s_l[x]);
-        return e >= min_p ? Row::weight(e) : 0ull;
+        return e >= min_p ? Row::weight_float(e) : 0.0f;
     };
-    u64 w = 0;
-    for (uint32_t x = s0 + lane; x < s1; x += 32) w += kept(x);
-    w = warp_sum(w);
+    double mine = 0.0;
+#pragma unroll 2
+    for (uint32_t x = s0 + lane; x < s1; x += 32) mine += (double)kept(x);
+    const u64 w = (u64)warp_sum(mine);
     __syncthreads();
     if (lane == 0) sh.scan2[warp] = w;
     __syncthreads();
-    if (tid == 0) {
-        u64 all = 0;
-        for (uint32_t x = 0; x < SM_WARPS; ++x) all += sh.scan2[x];
-        sh.part = all;
-    }
+    u64 all = 0;
+#pragma unroll
+    for (uint32_t x = 0; x < SM_WARPS; ++x) all += sh.scan2[x];
+    if (tid == 0) sh.part = all;
     cluster.sync();
     u64 ahead = 0;
     total = 0;
     for (uint32_t x = 0; x < ctas; ++x) {
-        const u64 v = *cluster.map_shared_rank(&sh.part, x);
+        const u64 v = r.at(sh.part, x);
         ahead += x < rank ? v : 0, total += v;
     }
     const u64 draw = draw_of(u, total);
-    for (uint32_t x = 0; x < warp; ++x) ahead += sh.scan2[x];
-    if (ahead <= draw && draw < ahead + w) {  // one warp of one CTA
-        for (uint32_t x = s0; x < s1; x += 32) {
-            const u64 mine = x + lane < s1 ? kept(x + lane) : 0ull;
-            const u64 run = warp_scan(mine, lane);
-            const uint32_t past = __ballot_sync(0xFFFFFFFFu, ahead + run > draw);
-            if (past) {
-                if (lane == __ffs(past) - 1) give(a, row, lo + (int32_t)(x + lane), (float)((double)mine / (double)total));
-                x = s1;
-            } else {
-                ahead += __shfl_sync(0xFFFFFFFFu, run, 31);
-            }
+    if (ahead <= draw && draw < ahead + all) {  // one CTA: the run that the draw falls into, then its token by all threads
+        uint32_t hit = 0;
+        while (ahead + sh.scan2[hit] <= draw) ahead += sh.scan2[hit++];
+        const uint32_t t0 = min(n, hit * seg), t1 = min(n, t0 + seg);
+        for (uint32_t x = t0; x < t1; x += SM_THREADS) {
+            const u64 me = x + tid < t1 ? (u64)kept(x + tid) : 0ull;
+            const u64 upto = ahead + r.block_scan(me);
+            if (upto > draw && upto - me <= draw) give(a, row, lo + (int32_t)(x + tid), (float)((double)me / (double)total));
+            ahead += r.block_sum(me);
         }
     }
     cluster.sync();  // shared memory is read from the others until here
@@ -507,11 +524,17 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
 }  // namespace
 
 cudaError_t launch_sample(const SampleArgs& a, uint32_t rows, cudaStream_t s) {
+    // 4096 logits a CTA or more, eight CTAs a row; sixteen (beyond what every device promises) while the rows are few
     uint32_t ctas = 1;
-    while (ctas < SM_CTAS && a.vocab > ctas * 4096) ctas *= 2;
+    while (ctas < (rows * SM_MOST_CTAS <= (uint32_t)num_sms() ? SM_MOST_CTAS : SM_CTAS) && a.vocab > ctas * 4096) ctas *= 2;
     const size_t smem = ((a.vocab + 3 + 3) / 4 + ctas - 1) / ctas * 16;  // of a row that begins inside a vector
     static bool configured[MAX_DEVICES] = {};
     if (cudaError_t e = set_max_smem_once(sample_kernel, SAMPLE_MAX_VOCAB / SM_CTAS * 4 + 16, configured); e != cudaSuccess) return e;
+    static bool wide[MAX_DEVICES] = {};
+    if (!wide[current_device()]) {
+        if (cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return e;
+        wide[current_device()] = true;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, rows);
     cfg.blockDim = dim3(SM_THREADS);
