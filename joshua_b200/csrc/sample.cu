@@ -32,19 +32,17 @@ __device__ __forceinline__ uint32_t logit_key(float l) {
     return l > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
 
-struct Few {     // a token among few: its place in the order, its weight
-    u64 place, weight;
-};
 struct SampleShared {
     union {
         struct {
             uint32_t number[SM_BINS], low[SM_BINS], high[SM_BINS];  // tokens, low and high halves of their weights
         } bins;
-        Few few[SM_FEW];
+        u64 few[SM_FEW];  // places of a few tokens; bins.high then is where a bin's tokens go in their order (CTA 0)
     };
     float best, least;
     float red[2][SM_WARPS];
     uint32_t n_few, bin, number;
+    static_assert(SM_FEW * 8 <= SM_BINS * 8, "bins.high lies behind the few");
     u64 part, border, before, sum, scan[SM_WARPS], scan2[SM_WARPS];
     int32_t window[SM_WINDOW];
 };
@@ -97,6 +95,10 @@ struct Row {
     __device__ __forceinline__ static float weight_float(float e) { return rintf(e * 4294967296.0f); }
     __device__ __forceinline__ static u64 weight(float e) { return (u64)weight_float(e); }
     __device__ __forceinline__ u64 place(uint32_t i) const { return (u64)logit_key(l[i]) << 32 | (0xFFFFFFFFu - (uint32_t)(lo + (int32_t)i)); }
+    __device__ __forceinline__ static float logit(u64 place) {
+        const uint32_t key = (uint32_t)(place >> 32);
+        return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
+    }
     // f(logit, place) of the whole slice, in no order
     template <class F>
     __device__ __forceinline__ void each(F f) const {
@@ -152,23 +154,24 @@ struct Row {
     }
 
     // The bin in which the running number of the tokens at places >= from reaches k, or (top_p < 1) their running weight what
-    // top-p keeps; what stands in front of the bin and how many tokens in it.  target: that number or weight.  False
-    // where there are fewer than k tokens; in_bin: how many.
+    // top-p keeps; what stands in front of the bin.  target: that number or weight.  in_bin: by number, how many tokens the bin
+    // holds, and what stands in front of every bin is in CTA 0's bins.high.  False where there are fewer than k tokens; in_bin:
+    // how many.
     __device__ bool border_bin(uint32_t k, float top_p, u64 from, uint32_t* border, u64* before, uint32_t* in_bin, u64* target_out) const {
         const bool by_weight = top_p < 1.0f;
         for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) {
-            sh.bins.number[i] = 0;
-            if (by_weight) sh.bins.low[i] = sh.bins.high[i] = 0;
+            if (by_weight) sh.bins.low[i] = sh.bins.high[i] = 0; else sh.bins.number[i] = 0;
         }
         if (tid == 0) sh.n_few = 0;
         __syncthreads();
         each([&](float x, uint32_t i) {
             const uint32_t b = bin(x);
             if (b >= SM_BINS || (from != 0 && place(i) < from)) return;
-            atomicAdd(&sh.bins.number[b], 1);
             if (by_weight) {  // at most 49152 tokens: both halves' sums stay below 2^32
                 const u64 w = weight(likeness(x));
                 atomicAdd(&sh.bins.low[b], (uint32_t)(w & 0xFFFF)), atomicAdd(&sh.bins.high[b], (uint32_t)(w >> 16));
+            } else {
+                atomicAdd(&sh.bins.number[b], 1);
             }
         });
         cluster.sync();
@@ -176,17 +179,14 @@ struct Row {
         const uint32_t run = SM_BINS / ctas, b0 = rank * run;
         constexpr uint32_t MOST = SM_BINS / SM_THREADS;
         u64 value[MOST], mine = 0;
-        uint32_t number[MOST];
 #pragma unroll
         for (uint32_t j = 0; j < MOST; ++j) {
             const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1, b = tid * per + j;
-            value[j] = 0, number[j] = 0;
+            value[j] = 0;
             if (j < per && b < run) {
-                for (uint32_t r = 0; r < ctas; ++r) {
-                    number[j] += at(sh.bins.number[b0 + b], r);
-                    if (by_weight) value[j] += at(sh.bins.low[b0 + b], r) + ((u64)at(sh.bins.high[b0 + b], r) << 16);
-                }
-                if (!by_weight) value[j] = number[j];
+#pragma unroll 4
+                for (uint32_t r = 0; r < ctas; ++r)
+                    value[j] += by_weight ? at(sh.bins.low[b0 + b], r) + ((u64)at(sh.bins.high[b0 + b], r) << 16) : at(sh.bins.number[b0 + b], r);
             }
             mine += value[j];
         }
@@ -207,62 +207,100 @@ struct Row {
         }
         const u64 target = by_weight ? most_of(top_p, whole) : k;
         *target_out = target;
-        if (whole < target) {  // the same everywhere
-            *in_bin = (uint32_t)whole;
-            cluster.sync();
-            return false;
-        }
         u64 upto = ahead + sum - mine;
+        const bool fewer = whole < target;  // the same everywhere
 #pragma unroll
         for (uint32_t j = 0; j < MOST; ++j) {
             if (upto < target && upto + value[j] >= target) {  // one thread of one CTA
                 const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1;
-                for (uint32_t r = 0; r < ctas; ++r) at(sh.bin, r) = b0 + tid * per + j, at(sh.before, r) = upto, at(sh.number, r) = number[j];
+                for (uint32_t r = 0; r < ctas; ++r) at(sh.bin, r) = b0 + tid * per + j, at(sh.before, r) = upto, at(sh.number, r) = (uint32_t)value[j];
+            }
+            if (!by_weight) {
+                const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1, b = tid * per + j;
+                if (j < per && b < run) at(sh.bins.high[b0 + b], 0) = (uint32_t)upto;
             }
             upto += value[j];
         }
         cluster.sync();
-        *border = sh.bin, *before = sh.before, *in_bin = sh.number;
-        return true;
+        *border = fewer ? SM_BINS - 1 : sh.bin, *before = fewer ? 0 : sh.before, *in_bin = fewer ? (uint32_t)whole : sh.number;
+        return !fewer;
     }
-    // Behind border_bin: the tokens of bins first .. last at places >= from, in CTA 0's list (their number returned there);
-    // SM_FEW at most.
+    // Behind border_bin: the places >= from of bins first .. last in CTA 0's list, and their number in all CTAs; of more than
+    // SM_FEW, nothing else.
     __device__ uint32_t gather(uint32_t first, uint32_t last, u64 from) const {
         // the histograms have been read in front of the last barrier
         each([&](float x, uint32_t i) {
             const uint32_t b = bin(x);
-            if (b < first || b > last || (from != 0 && place(i) < from)) return;
+            if (b < first || b > last) return;
+            const u64 p = place(i);
+            if (p < from) return;
             const uint32_t to = atomicAdd(&sh.n_few, 1);
-            if (to < SM_FEW) sh.few[to] = Few{place(i), weight(likeness(x))};
+            if (to < SM_FEW) sh.few[to] = p;
         });
         cluster.sync();
-        uint32_t m = 0;
-        if (rank == 0) {
-            uint32_t mine = lane < ctas ? min(at(sh.n_few, lane), SM_FEW) : 0;
-            const uint32_t upto = warp_scan(mine, lane);
-            m = min(__shfl_sync(0xFFFFFFFFu, upto, 31), SM_FEW);
+        const uint32_t mine = lane < ctas ? at(sh.n_few, lane) : 0, upto = warp_scan(mine, lane), m = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (rank == 0 && m <= SM_FEW) {
             for (uint32_t r = 1 + warp; r < ctas; r += SM_WARPS) {  // a warp a list
                 const uint32_t more = __shfl_sync(0xFFFFFFFFu, mine, r), to = __shfl_sync(0xFFFFFFFFu, upto, r) - more;
-                const Few* list = cluster.map_shared_rank(sh.few, r);
-                for (uint32_t i = lane; i < more && to + i < SM_FEW; i += 32) sh.few[to + i] = list[i];
+                const u64* list = cluster.map_shared_rank(sh.few, r);
+                for (uint32_t i = lane; i < more; i += 32) sh.few[to + i] = list[i];
             }
         }
         cluster.sync();
         return m;
     }
-    // The m tokens of this CTA's list in order of place, the largest first: a bitonic sort; the steps up to 32 apart stay within
-    // a warp's 64 tokens.
+    static constexpr uint32_t PER = SM_FEW / SM_THREADS, RUN = 256;
+    // The m places of this CTA's list, the largest first.  In bins: each goes behind what bins.high says stands in front of its
+    // bin, then behind the larger ones of the bin.  All of one bin: behind the larger ones.  Where more than RUN have to be
+    // compared with one another: a bitonic sort.
+    __device__ void order(uint32_t m, bool in_bins) const {
+        u64 p[PER];
+        uint32_t b[PER];
+        bool long_run = false;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) {
+            const uint32_t i = tid + j * SM_THREADS;
+            p[j] = i < m ? sh.few[i] : 0, b[j] = i < m ? bin(logit(p[j])) : 0;
+        }
+        __syncthreads();
+        if (in_bins) {
+#pragma unroll
+            for (uint32_t j = 0; j < PER; ++j)
+                if (tid + j * SM_THREADS < m) sh.few[atomicAdd(&sh.bins.high[b[j]], 1)] = p[j];
+            __syncthreads();
+        }
+        uint32_t to[PER];
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) {
+            const uint32_t first = in_bins && b[j] ? sh.bins.high[b[j] - 1] : 0, last = in_bins ? sh.bins.high[b[j]] : m;
+            to[j] = first;
+            if (tid + j * SM_THREADS >= m) continue;
+            long_run |= last - first > RUN;
+            if (last - first <= RUN)
+                for (uint32_t x = first; x < last; ++x) to[j] += sh.few[x] > p[j];
+        }
+        if (__syncthreads_or(long_run)) {
+            sort(m);
+            return;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j)
+            if (tid + j * SM_THREADS < m) sh.few[to[j]] = p[j];
+        __syncthreads();
+    }
+    // The same by a bitonic sort; the steps up to 32 apart stay within a warp's 64 places.
     __device__ void sort(uint32_t m) const {
         uint32_t size = 64;
         while (size < m) size *= 2;
-        for (uint32_t i = m + tid; i < size; i += SM_THREADS) sh.few[i] = Few{0, 0};
+        for (uint32_t i = m + tid; i < size; i += SM_THREADS) sh.few[i] = 0;
         for (uint32_t run = 2; run <= size; run *= 2)
             for (uint32_t gap = run / 2; gap > 0; gap /= 2) {
                 if (gap >= 32 || run == 2) __syncthreads(); else __syncwarp();
                 for (uint32_t t = tid; t < size / 2; t += SM_THREADS) {
                     const uint32_t i = 2 * t - (t & (gap - 1)), j = i + gap;
-                    const Few x = sh.few[i], y = sh.few[j];
-                    if ((x.place < y.place) == ((i & run) == 0)) sh.few[i] = y, sh.few[j] = x;
+                    const u64 x = sh.few[i], y = sh.few[j];
+                    if ((x < y) == ((i & run) == 0)) sh.few[i] = y, sh.few[j] = x;
                 }
             }
         __syncthreads();
@@ -273,23 +311,22 @@ struct Row {
         uint32_t b, in_bin;
         u64 before, target;
         if (!border_bin(k, top_p, from, &b, &before, &in_bin, &target)) return from;
-        if (in_bin <= SM_FEW) {
-            const uint32_t m = gather(b, b, from);
+        const uint32_t m = gather(b, b, from);
+        if (m <= SM_FEW) {
             if (rank == 0) {
-                sort(m);
-                constexpr uint32_t PER = SM_FEW / SM_THREADS;
+                order(m, false);
                 u64 w[PER], mine = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
                     const uint32_t i = tid * PER + j;
-                    w[j] = i >= m ? 0 : by_weight ? sh.few[i].weight : 1;
+                    w[j] = i >= m ? 0 : by_weight ? weight(likeness(logit(sh.few[i]))) : 1;
                     mine += w[j];
                 }
                 u64 ahead = before + block_scan(mine) - mine;
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
                     if (ahead < target && ahead + w[j] >= target)
-                        for (uint32_t r = 0; r < ctas; ++r) at(sh.border, r) = sh.few[tid * PER + j].place;
+                        for (uint32_t r = 0; r < ctas; ++r) at(sh.border, r) = sh.few[tid * PER + j];
                     ahead += w[j];
                 }
             }
@@ -417,17 +454,19 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     if (top_k != 0 && top_k <= SM_FEW) {
         const bool cut = r.border_bin(top_k, 1.0f, 0, &border, &before, &in_bin, &target);
         // all tokens down to the bin of the last one kept (or all there are)
-        if ((cut ? before : 0) + in_bin <= SM_FEW) {
-            const uint32_t m = r.gather(0, cut ? border : SM_BINS - 1, 0);
+        if (before + in_bin <= SM_FEW) {
+            const uint32_t m = r.gather(0, border, 0);
             if (rank == 0) {
-                r.sort(m);
-                constexpr uint32_t PER = SM_FEW / SM_THREADS;  // tokens PER tid .. of the order
+                r.order(m, true);
+                constexpr uint32_t PER = Row::PER;  // tokens PER tid .. of the order
                 u64 w[PER], sum = 0;
                 uint32_t id[PER];
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
                     const uint32_t at = tid * PER + j;
-                    w[j] = at < min(m, top_k) ? sh.few[at].weight : 0;
+                    const u64 place = at < min(m, top_k) ? sh.few[at] : 0;
+                    const float e = place ? r.likeness(Row::logit(place)) : 0.0f;
+                    w[j] = Row::weight(e), id[j] = 0xFFFFFFFFu - (uint32_t)place;
                     sum += w[j];
                 }
                 u64 ahead = r.block_scan(sum) - sum;
@@ -436,13 +475,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
                 sum = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < PER; ++j) {
-                    const u64 place = w[j] ? sh.few[tid * PER + j].place : 0;
-                    const uint32_t key = (uint32_t)(place >> 32);
-                    id[j] = 0xFFFFFFFFu - (uint32_t)place;
                     const u64 mine = w[j];
-                    // the likeness again, from the logit that the place holds
-                    if (ahead >= most || (min_p > 0.0f && !(r.likeness(__uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key)) >= min_p)))
-                        w[j] = 0;
+                    if (ahead >= most || (min_p > 0.0f && mine && !(r.likeness(Row::logit(sh.few[tid * PER + j])) >= min_p))) w[j] = 0;
                     ahead += mine, sum += w[j];
                 }
                 total = r.block_sum(sum);
@@ -453,15 +487,18 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
                 for (uint32_t j = 0; j < PER; ++j) kept += w[j] != 0;
                 kept = (uint32_t)r.block_sum(kept);  // the first ones of the order
                 if (kept <= SM_THREADS / 2) {        // each adds up those below it
+                    u64* weights = reinterpret_cast<u64*>(sh.bins.high);
+#pragma unroll
+                    for (uint32_t j = 0; j < PER; ++j)
+                        if (tid * PER + j < kept) weights[tid * PER + j] = w[j];
+                    __syncthreads();
                     if (tid < kept) {
-                        const Few me = sh.few[tid];
+                        const uint32_t low = (uint32_t)sh.few[tid];  // larger for lower ids
                         u64 below = 0;
-                        for (uint32_t x = 0; x < kept; ++x) {
-                            const Few f = sh.few[x];
-                            below += (uint32_t)f.place > (uint32_t)me.place ? f.weight : 0;
-                        }
-                        if (below <= draw && draw < below + me.weight)
-                            give(a, row, (int32_t)(0xFFFFFFFFu - (uint32_t)me.place), (float)((double)me.weight / (double)total));
+                        for (uint32_t x = 0; x < kept; ++x) below += (uint32_t)sh.few[x] > low ? weights[x] : 0;
+                        const u64 me = weights[tid];
+                        if (below <= draw && draw < below + me)
+                            give(a, row, (int32_t)(0xFFFFFFFFu - low), (float)((double)me / (double)total));
                     }
                 } else {  // bit by bit: the ids below it weigh at most the draw
                     uint32_t below = 0;
