@@ -9,11 +9,15 @@
 //            of the step's largest scale, in two f16 terms (22 bits below the largest).  Accumulators hold a step, not the
 //            sequence: the tensor core adds with truncation, the running output is added round-to-nearest.
 // Up to four query rows stand as four pairs of columns (term, term): one product does both terms.
+#include <cooperative_groups.h>
+
 #include "kv_pages.cuh"
 
 namespace jq {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -24,6 +28,9 @@ __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // read once: no
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
+}
+__device__ __forceinline__ void prefetch_l2(const uint8_t* p, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -419,6 +426,8 @@ struct Attend {
     }
 };
 
+constexpr uint32_t LEAD_MOST = 4;  // partial results of the leading pages
+
 struct PagedArgs {
     KvPages c;
     const float* q;
@@ -436,50 +445,127 @@ struct PagedArgs {
     int32_t* bad_pos;
 };
 
+// The pages of one sequence from page `first` on: ids of 32 at a time, a lane each, and a page's tile of a head requested from
+// memory (into L2) one page ahead.
+template <class T>
+struct Pages {
+    const PagedArgs& a;
+    const int32_t* table;
+    uint32_t kvh, lane, have, end;  // first page whose id is held; page behind the last one wanted
+    int32_t ids;
+    bool lost;  // some id is outside the cache
+
+    __device__ __forceinline__ void fetch(uint32_t from) {
+        const uint32_t p = from + lane;
+        have = from;
+        ids = p < end ? __ldg((p < a.common ? a.c.table : table) + p) : 0;
+    }
+    __device__ __forceinline__ const uint8_t* tile(uint32_t p) {
+        if (p - have >= 32) fetch(p);
+        const int32_t id = __shfl_sync(0xFFFFFFFFu, ids, p - have);
+        const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
+        lost |= !fine;
+        return a.c.pages + ((uint64_t)(fine ? id : 0) * a.c.n_kv + kvh) * T::HEAD;
+    }
+    // the tile, and the next one asked for
+    __device__ __forceinline__ const uint8_t* enter(uint32_t p) {
+        const uint8_t* t = tile(p);
+        if (p + 1 < end) {
+            const uint8_t* next = tile(p + 1);
+            if (lane == 0) prefetch_l2(next, T::HEAD);
+        }
+        return t;
+    }
+};
+
 // Weight of a piece with maximum m under the joint maximum; equal ones are 1 (infinities too)
 __device__ __forceinline__ float piece_weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
 
-__device__ __forceinline__ const float* lead_row(const PagedArgs& a, uint32_t hd, uint32_t i, uint32_t kvh, uint32_t row, const float** m,
-                                                 const float** l) {
-    const uint64_t rows = (uint64_t)a.c.n_seq * a.group, all = a.lead_splits * (uint64_t)a.c.n_kv * rows;
-    const uint64_t at = ((uint64_t)i * a.c.n_kv + kvh) * rows + row;
-    *m = a.lead + all * hd + at, *l = a.lead + all * hd + all + at;
-    return a.lead + at * hd;
-}
+// A row's joined pieces: lane i has dimensions 4 i .. 4 i + 3 (HD 256: also those 128 behind; HD 64: lanes 0 .. 15).
+template <uint32_t HD>
+struct Joined {
+    static constexpr uint32_t N = HD <= 128 ? 1 : HD / 128;
+    float4 x[N];
+    float top, den;
 
-// out = the joined pieces (n of them, `piece(i)` points to [ROWS][HD] sums, maxima, sums) and those of the leading pages, by
-// `threads` threads.  A row of nothing is zero.
-template <uint32_t HD, uint32_t ROWS, class F>
-__device__ __forceinline__ void finish(const PagedArgs& a, uint32_t b, uint32_t head_group, uint32_t n, F piece, uint32_t tid,
-                                       uint32_t threads) {
-    const uint32_t kvh = head_group / a.split, first = head_group % a.split * ROWS, rows = min(ROWS, a.group - first);
-    for (uint32_t i = tid; i < rows * (HD / 4); i += threads) {
-        const uint32_t row = i / (HD / 4), d = i % (HD / 4) * 4, in_batch = b * a.group + first + row;
-        float top = -INFINITY;
-        for (uint32_t j = 0; j < n; ++j) top = fmaxf(top, piece(j)[ROWS * HD + row]);
-        for (uint32_t j = 0; j < a.lead_splits; ++j) {
-            const float *m, *l;
-            lead_row(a, HD, j, kvh, in_batch, &m, &l);
-            top = fmaxf(top, *m);
-        }
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float den = 0.0f;
-        auto add = [&](const float* o, float m, float l) {
-            const float w = piece_weight(m, top);
-            const float4 v = *reinterpret_cast<const float4*>(o + d);
-            x.x = fmaf(w, v.x, x.x), x.y = fmaf(w, v.y, x.y), x.z = fmaf(w, v.z, x.z), x.w = fmaf(w, v.w, x.w);
-            den = fmaf(w, l, den);
-        };
-        for (uint32_t j = 0; j < a.lead_splits; ++j) {
-            const float *m, *l, *o = lead_row(a, HD, j, kvh, in_batch, &m, &l);
-            add(o, *m, *l);
-        }
-        for (uint32_t j = 0; j < n; ++j) add(piece(j) + row * HD, piece(j)[ROWS * HD + row], piece(j)[ROWS * HD + ROWS + row]);
-        const float inv = n + a.lead_splits ? 1.0f / den : 0.0f;
-        *reinterpret_cast<float4*>(a.out + b * a.out_stride + (uint64_t)(kvh * a.group + first + row) * HD + d) =
-            make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i) x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        top = -INFINITY, den = 0.0f;
     }
-}
+    // n more pieces by a warp: piece(i): [ROWS][HD] sums, maxima, sums of exponentials.  OTHERS: other CTAs have just written them.
+    template <uint32_t ROWS, bool OTHERS, class F>
+    __device__ __forceinline__ void add(uint32_t n, F piece, uint32_t row, uint32_t lane) {
+        auto load = [](auto* q) { return OTHERS ? __ldcg(q) : *q; };
+        for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+            const uint32_t cnt = min(32u, n - i0);
+            const float* mine = piece(i0 + min(lane, cnt - 1));
+            const float m = lane < cnt ? load(mine + ROWS * HD + row) : -INFINITY, l = lane < cnt ? load(mine + ROWS * HD + ROWS + row) : 0.0f;
+            float t = fmaxf(top, m);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, o));
+            const float old = piece_weight(top, t), w = lane < cnt ? piece_weight(m, t) : 0.0f;
+            float d = w * l;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, o);
+            den = fmaf(den, old, d), top = t;
+#pragma unroll
+            for (uint32_t k = 0; k < N; ++k) x[k].x *= old, x[k].y *= old, x[k].z *= old, x[k].w *= old;
+#pragma unroll 4
+            for (uint32_t j = 0; j < cnt; ++j) {
+                const float f = __shfl_sync(0xFFFFFFFFu, w, j);
+                const float* from = piece(i0 + j) + row * HD + 4 * lane;
+#pragma unroll
+                for (uint32_t k = 0; k < N; ++k) {
+                    const float4 v = HD >= 128 || lane < HD / 4 ? load(reinterpret_cast<const float4*>(from + 128 * k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    x[k].x = fmaf(f, v.x, x[k].x), x[k].y = fmaf(f, v.y, x[k].y), x[k].z = fmaf(f, v.z, x[k].z), x[k].w = fmaf(f, v.w, x[k].w);
+                }
+            }
+        }
+    }
+    // ... and those of the leading pages (LEAD_MOST at most, all on their way together)
+    __device__ __forceinline__ void add_lead(const PagedArgs& a, uint32_t kvh, uint32_t row, uint32_t lane) {
+        const uint64_t rows = (uint64_t)a.c.n_seq * a.group, stride = a.c.n_kv * rows, all = a.lead_splits * stride, at = kvh * rows + row;
+        float4 v[LEAD_MOST][N];
+        float m[LEAD_MOST], l[LEAD_MOST], t = top;
+#pragma unroll
+        for (uint32_t j = 0; j < LEAD_MOST; ++j) {
+            const bool is = j < a.lead_splits;
+#pragma unroll
+            for (uint32_t k = 0; k < N; ++k)
+                v[j][k] = is && (HD >= 128 || lane < HD / 4) ? *reinterpret_cast<const float4*>(a.lead + (at + j * stride) * HD + 4 * lane + 128 * k)
+                                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            m[j] = is ? a.lead[all * HD + at + j * stride] : -INFINITY, l[j] = is ? a.lead[all * HD + all + at + j * stride] : 0.0f;
+            t = fmaxf(t, m[j]);
+        }
+        const float old = piece_weight(top, t);
+        den *= old, top = t;
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k) x[k].x *= old, x[k].y *= old, x[k].z *= old, x[k].w *= old;
+#pragma unroll
+        for (uint32_t j = 0; j < LEAD_MOST; ++j) {
+            const float f = piece_weight(m[j], t);
+            den = fmaf(f, l[j], den);
+#pragma unroll
+            for (uint32_t k = 0; k < N; ++k) {
+                x[k].x = fmaf(f, v[j][k].x, x[k].x), x[k].y = fmaf(f, v[j][k].y, x[k].y);
+                x[k].z = fmaf(f, v[j][k].z, x[k].z), x[k].w = fmaf(f, v[j][k].w, x[k].w);
+            }
+        }
+    }
+    // the row of the result: nothing where there was nothing
+    __device__ __forceinline__ void finish(const PagedArgs& a, uint32_t b, uint32_t kvh, uint32_t in_group, uint32_t lane) {
+        if (a.lead_splits) add_lead(a, kvh, b * a.group + in_group, lane);
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        float* to = a.out + b * a.out_stride + (uint64_t)(kvh * a.group + in_group) * HD + 4 * lane;
+#pragma unroll
+        for (uint32_t k = 0; k < N; ++k)
+            if (HD >= 128 || lane < HD / 4)
+                *reinterpret_cast<float4*>(to + 128 * k) = make_float4(x[k].x * inv, x[k].y * inv, x[k].z * inv, x[k].w * inv);
+    }
+};
+
+constexpr uint32_t SEG_UNITS = 2;
 
 // Positions of a sequence's own (behind the leading pages), or -1 where its length is out of range.
 __device__ __forceinline__ int32_t own_positions(const PagedArgs& a, uint32_t b) {
@@ -488,25 +574,30 @@ __device__ __forceinline__ int32_t own_positions(const PagedArgs& a, uint32_t b)
     return n == 0 ? 0 : n - (int32_t)(a.done * KV_PAGE);
 }
 
-// The sequences' steps stand in one row: sequence by sequence, head group by head group.  It is cut into equal pieces, one a
-// warp, whatever the lengths; a CTA's warps have neighbouring ones.  Pieces of one segment (sequence, head group) are joined
+// The sequences' work stands in one row of units: sequence by sequence, head group by head group, SEG_UNITS for beginning and
+// ending a segment (its queries, its result), then its steps.  It is cut into equal pieces, one a warp, whatever the lengths; a
+// CTA's warps have neighbouring ones.  Pieces of one segment (sequence, head group) are joined
 // within the CTA, then, where a segment spans CTAs, by the last one of them to arrive, in order.
-template <class T, bool PAIRS, uint32_t WARPS, uint32_t MIN_CTAS>
-__global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(PagedArgs a) {
+template <class T, bool PAIRS, uint32_t WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArgs a) {
     using At = Attend<T, 1, PAIRS>;
     constexpr uint32_t HD = T::HD, ROWS = At::Q::ROWS, PIECE = ROWS * (HD + 2);
     extern __shared__ __align__(16) uint32_t s_mem[];
-    __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_last;
-    uint32_t* s_cum = s_mem;                                                       // [batch + 1] steps in front of a sequence
+    __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_last[2], s_first[2];
+    uint32_t* s_cum = s_mem;                                                       // [batch + 1] units of a head group in front of a sequence
     float* s_piece = reinterpret_cast<float*>(s_mem + ((a.c.n_seq + 4) & ~3u));    // [WARPS][2][PIECE]
     uint32_t* s_q = reinterpret_cast<uint32_t*>(s_piece + WARPS * 2 * PIECE);      // [WARPS] query operands
     pdl_trigger_all();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, batch = a.c.n_seq, groups = a.c.n_kv * a.split;
     if (tid < 2 * WARPS) s_seg[tid] = 0xFFFFFFFFu;
-    // running sum of the sequences' steps, a run of sequences a thread
+    // running sum of the sequences' units, a run of sequences a thread
     const uint32_t per = (batch + WARPS * 32 - 1) / (WARPS * 32), b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
     uint32_t mine = 0;
-    for (uint32_t b = b0; b < b1; ++b) mine += (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
+    auto units_of = [&](uint32_t b) {
+        const uint32_t steps = (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
+        return steps ? steps + SEG_UNITS : 0;
+    };
+    for (uint32_t b = b0; b < b1; ++b) mine += units_of(b);
     uint32_t run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -519,7 +610,7 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(P
     run -= mine;
     for (uint32_t b = b0; b < b1; ++b) {
         s_cum[b] = run;
-        run += (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
+        run += units_of(b);
     }
     if (b1 == batch && (b0 < b1 || tid == 0)) s_cum[batch] = run;
     __syncthreads();
@@ -531,57 +622,69 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(P
     const uint64_t end = me < workers ? (me + 1) * total / workers : 0;
     At w;
     bool first_piece = true;
-    uint32_t b = 0;
-    if (at < end) {  // the last sequence that begins at or before it (and has steps)
+    // a piece of work: steps u0 .. u1 (perhaps none) of the `steps` of a sequence and head group
+    struct Piece {
+        uint32_t b, hg, u0, u1, steps, units;
+    };
+    auto piece_at = [&](uint64_t x, uint32_t b) {  // of the segment that unit x is in; b: at or in front of its sequence
+        while (s_cum[b + 1] == s_cum[b] || (uint64_t)s_cum[b + 1] * groups <= x) ++b;
+        const uint32_t all = s_cum[b + 1] - s_cum[b];
+        const uint64_t in_seq = x - (uint64_t)s_cum[b] * groups;
+        const uint32_t hg = (uint32_t)(in_seq / all), at0 = (uint32_t)(in_seq - (uint64_t)hg * all), at1 = (uint32_t)min((uint64_t)all, at0 + (end - x));
+        auto step = [](uint32_t u) { return u > SEG_UNITS ? u - SEG_UNITS : 0; };
+        return Piece{b, hg, step(at0), step(at1), all - SEG_UNITS, at1 - at0};
+    };
+    constexpr uint32_t PER_PAGE = KV_PAGE / T::POS;
+    Pages<T> pages{a, a.c.table, 0, lane, 0, 0, 0, false};
+    Rows<T> k, v;
+    const uint8_t* tile = nullptr;
+    auto begin = [&](const Piece& p) {  // its first keys on their way
+        pages.table = a.c.table + (uint64_t)p.b * a.c.table_stride, pages.kvh = p.hg / a.split;
+        pages.end = a.done + (p.u1 - 1) / PER_PAGE + 1, pages.lost = false;
+        pages.fetch(a.done + p.u0 / PER_PAGE);
+        tile = pages.enter(a.done + p.u0 / PER_PAGE);
+        k.load(tile, p.u0 % PER_PAGE * T::POS, lane);
+        // and its queries, into L1
+        const uint32_t first = p.hg % a.split * ROWS, lines = min(ROWS, a.group - first) * (HD / 32);
+        const float* q = a.q + p.b * a.q_stride + (uint64_t)(pages.kvh * a.group + first) * HD;
+        for (uint32_t i = lane; i < lines; i += 32) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + 32 * i));
+    };
+    // the next piece with steps, from unit `at` on, which moves behind it
+    auto take = [&](uint32_t b) {
+        Piece p{};
+        while (at < end && p.u0 == p.u1) p = piece_at(at, b), at += p.units, b = p.b;
+        return p;
+    };
+    Piece p{};
+    if (at < end) {  // the last sequence that begins at or in front of it
         uint32_t lo = 0, hi = batch;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
             (uint64_t)s_cum[mid] * groups <= at ? lo = mid : hi = mid;
         }
-        b = lo;
+        p = take(lo);
+        if (p.u0 < p.u1) begin(p);
     }
-    while (at < end) {
-        while (s_cum[b + 1] == s_cum[b] || (uint64_t)s_cum[b + 1] * groups <= at) ++b;
-        const uint32_t steps = s_cum[b + 1] - s_cum[b];
-        const uint64_t in_seq = at - (uint64_t)s_cum[b] * groups;
-        const uint32_t hg = (uint32_t)(in_seq / steps), u0 = (uint32_t)(in_seq % steps);
-        const uint32_t u1 = (uint32_t)min((uint64_t)steps, u0 + (end - at));
-        const uint32_t kvh = hg / a.split, first = hg % a.split * ROWS;
-        const uint32_t own = (uint32_t)own_positions(a, b);
-        // page ids of 32 pages at a time, a lane each
-        constexpr uint32_t PER_PAGE = KV_PAGE / T::POS;
-        const int32_t* table = a.c.table + (uint64_t)b * a.c.table_stride;
-        uint32_t have = u0 / PER_PAGE;
-        int32_t ids = 0;
-        auto fetch_ids = [&] {
-            const uint32_t p = a.done + have + lane;
-            ids = p < a.c.table_stride ? (p < a.common ? a.c.table[p] : table[p]) : -1;
-        };
-        bool lost = false;
-        auto tile_of = [&](uint32_t u) -> const uint8_t* {
-            const uint32_t p = u / PER_PAGE;
-            if (p - have >= 32) have = p, fetch_ids();
-            const int32_t id = __shfl_sync(0xFFFFFFFFu, ids, p - have);
-            const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
-            lost |= !fine;
-            return a.c.pages + ((uint64_t)(fine ? id : 0) * a.c.n_kv + kvh) * T::HEAD;
-        };
-        fetch_ids();
-        const uint8_t* tile = tile_of(u0);
-        Rows<T> k, v;
-        k.load(tile, u0 % PER_PAGE * T::POS, lane);
-        const float* q = a.q + b * a.q_stride + (uint64_t)(kvh * a.group + first) * HD;
+    while (p.u0 < p.u1) {
+        const uint32_t kvh = p.hg / a.split, first = p.hg % a.split * ROWS, own = (uint32_t)own_positions(a, p.b);
+        const float* q = a.q + p.b * a.q_stride + (uint64_t)(kvh * a.group + first) * HD;
         w.load_queries([&](uint32_t i) -> const float* { return first + i < a.group ? q + i * HD : nullptr; }, a.scale, lane,
                        s_q + warp * At::Q::WORDS);
         w.reset();
-        for (uint32_t u = u0; u < u1; ++u) {
+        Piece next{};
+        bool lost = false;
+        for (uint32_t u = p.u0; u < p.u1; ++u) {
             const uint32_t valid = min(own - u * T::POS, T::POS);
             v.load(tile + T::HEAD / 2, u % PER_PAGE * T::POS, lane);
             float s[T::GROUPS][1][2 * At::COLS], alpha[At::MINE];
             w.scores(k, lane, s);
-            if (u + 1 < u1) {
-                tile = tile_of(u + 1);
+            if (u + 1 < p.u1) {
+                if ((u + 1) % PER_PAGE == 0) tile = pages.enter(a.done + (u + 1) / PER_PAGE);
                 k.load(tile, (u + 1) % PER_PAGE * T::POS, lane);
+            } else {
+                lost = pages.lost;
+                next = take(p.b);
+                if (next.u0 < next.u1) begin(next);
             }
             w.softmax(s, valid, lane, alpha);
             w.output(s, v, valid, lane, alpha);
@@ -596,69 +699,89 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(P
         __syncwarp();
         w.store(to, lane);
         __syncwarp();
-        if (u0 == 0 && u1 == steps) {
-            finish<HD, ROWS>(a, b, hg, 1, [&](uint32_t) { return to; }, lane, 32);
+        if (p.u0 == 0 && p.u1 == p.steps) {
+#pragma unroll 2
+            for (uint32_t row = 0; row < min(ROWS, a.group - first); ++row) {
+                Joined<HD> y;
+                y.clear();
+                y.template add<ROWS, false>(1, [&](uint32_t) { return to; }, row, lane);
+                y.finish(a, p.b, kvh, first + row, lane);
+            }
         } else {
-            if (lane == 0) s_seg[slot] = b * groups + hg, s_from[slot] = u0, s_to[slot] = u1;
+            if (lane == 0) s_seg[slot] = p.b * groups + p.hg, s_from[slot] = p.u0, s_to[slot] = p.u1;
             first_piece = false;
         }
-        at += u1 - u0;
+        p = next;
     }
     __syncthreads();
-    // pieces of segments that no warp has whole, in order
-    for (uint32_t i = 0; i < 2 * WARPS;) {
-        const uint32_t seg = s_seg[i];
-        if (seg == 0xFFFFFFFFu) {
-            ++i;
-            continue;
-        }
-        static_assert(WARPS <= 8, "slot numbers in four bits");
-        uint64_t slots = 0;  // of the segment
-        uint32_t n = 0, last = i;
-        for (uint32_t j = i; j < 2 * WARPS; ++j)
-            if (s_seg[j] == seg) slots |= (uint64_t)j << (4 * n), ++n, last = j;
-        const uint32_t sb = seg / groups, hg = seg % groups, steps = s_cum[sb + 1] - s_cum[sb], from = s_from[i], to = s_to[last];
-        auto local = [&](uint32_t j) -> const float* { return s_piece + (uint32_t)(slots >> (4 * j) & 15) * PIECE; };
-        if (from == 0 && to == steps) {
-            finish<HD, ROWS>(a, sb, hg, n, local, tid, WARPS * 32);
-        } else {
-            float* dst = a.part + ((uint64_t)blockIdx.x * 2 + (from == 0)) * PIECE;
-            for (uint32_t x = tid; x < ROWS * (HD / 4); x += WARPS * 32) {
-                const uint32_t row = x / (HD / 4), d = x % (HD / 4) * 4;
-                float top = -INFINITY, den = 0.0f;
-                for (uint32_t j = 0; j < n; ++j) top = fmaxf(top, local(j)[ROWS * HD + row]);
-                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (uint32_t j = 0; j < n; ++j) {
-                    const float* p = local(j);
-                    const float f = piece_weight(p[ROWS * HD + row], top);
-                    const float4 y = *reinterpret_cast<const float4*>(p + row * HD + d);
-                    sum.x = fmaf(f, y.x, sum.x), sum.y = fmaf(f, y.y, sum.y), sum.z = fmaf(f, y.z, sum.z), sum.w = fmaf(f, y.w, sum.w);
-                    den = fmaf(f, p[ROWS * HD + ROWS + row], den);
-                }
-                __stcg(reinterpret_cast<float4*>(dst + row * HD + d), sum);
-                if (d == 0) __stcg(dst + ROWS * HD + row, top), __stcg(dst + ROWS * HD + ROWS + row, den);
+    // Pieces of segments that no warp has whole.  They stand in order, a segment's one after another; a warp joins a row of one.
+    // What the CTA has whole is done; of others (its first and its last at most) the joined pieces go to memory, and the last CTA
+    // to bring some joins them all.
+    static_assert(2 * WARPS <= 32, "a lane a slot");
+    const uint32_t seg_of = lane < 2 * WARPS ? s_seg[lane] : 0xFFFFFFFFu;
+    const uint32_t held = __ballot_sync(0xFFFFFFFFu, seg_of != 0xFFFFFFFFu);
+    // the held slots' numbers in order, one a lane
+    const uint32_t n_held = __popc(held);
+    uint32_t slot_of = 0;
+    for (uint32_t m = held, i = 0; m; m &= m - 1, ++i) slot_of = lane == i ? __ffs(m) - 1 : slot_of;
+    const uint32_t seg = __shfl_sync(0xFFFFFFFFu, seg_of, slot_of);  // of the lane-th held slot
+    const uint32_t before = __shfl_up_sync(0xFFFFFFFFu, seg, 1);
+    const uint32_t starts = __ballot_sync(0xFFFFFFFFu, lane < n_held && (lane == 0 || seg != before));
+    const uint32_t n_seg = __popc(starts);
+    uint32_t open = 0, open_seg[2] = {0, 0};  // 1: a segment that begins in an earlier CTA, 2: one that begins here and goes on
+    for (uint32_t i = 0, m = starts; i < n_seg; ++i, m &= m - 1) {
+        const uint32_t first = __ffs(m) - 1, behind = m & (m - 1) ? __ffs(m & (m - 1)) - 1 : n_held, n = behind - first;
+        const uint32_t sg = __shfl_sync(0xFFFFFFFFu, seg, first), sb = sg / groups, hg = sg % groups, steps = s_cum[sb + 1] - s_cum[sb] - SEG_UNITS;
+        const bool begins = s_from[__shfl_sync(0xFFFFFFFFu, slot_of, first)] == 0;
+        const bool whole = begins && s_to[__shfl_sync(0xFFFFFFFFu, slot_of, behind - 1)] == steps;
+        if (!whole) open |= 1u << begins, open_seg[begins] = sg;
+        for (uint32_t row = (warp + WARPS - i * ROWS % WARPS) % WARPS; row < ROWS; row += WARPS) {  // segments in turn to different warps
+            const uint32_t kvh = hg / a.split, in_group = hg % a.split * ROWS + row;
+            Joined<HD> y;
+            y.clear();
+            y.template add<ROWS, false>(
+                n, [&](uint32_t j) { return (const float*)(s_piece + __shfl_sync(0xFFFFFFFFu, slot_of, first + j) * PIECE); }, row, lane);
+            if (whole) {
+                if (in_group < a.group) y.finish(a, sb, kvh, in_group, lane);
+            } else {
+                float* dst = a.part + ((uint64_t)blockIdx.x * 2 + begins) * PIECE;
+#pragma unroll
+                for (uint32_t k = 0; k < Joined<HD>::N; ++k)
+                    if (HD >= 128 || lane < HD / 4) __stcg(reinterpret_cast<float4*>(dst + row * HD + 4 * lane + 128 * k), y.x[k]);
+                if (lane == 0) __stcg(dst + ROWS * HD + row, y.top), __stcg(dst + ROWS * HD + ROWS + row, y.den);
             }
-            // the CTAs that have a piece of it
-            const uint64_t u_first = (uint64_t)s_cum[sb] * groups + (uint64_t)hg * steps, u_last = u_first + steps - 1;
-            const uint32_t c0 = (uint32_t)(((u_first + 1) * workers - 1) / total / WARPS);
-            const uint32_t c1 = (uint32_t)(((u_last + 1) * workers - 1) / total / WARPS);
+        }
+    }
+    if (open) {  // the same in all threads
+        __threadfence();
+        __syncthreads();
+        auto owners = [&](uint32_t sg, uint32_t* c0) {  // CTAs that have a piece of it, from c0 on
+            const uint32_t sb = sg / groups, units = s_cum[sb + 1] - s_cum[sb];
+            const uint64_t x = (uint64_t)s_cum[sb] * groups + (uint64_t)(sg % groups) * units, x0 = x + SEG_UNITS, x1 = x + units - 1;
+            *c0 = (uint32_t)(((x0 + 1) * workers - 1) / total / WARPS);
+            return (uint32_t)(((x1 + 1) * workers - 1) / total / WARPS) - *c0 + 1;
+        };
+        if (tid < 2) {
+            s_last[tid] = 0;
+            if (open >> tid & 1) {
+                uint32_t c0;
+                const uint32_t sg = open_seg[tid], n = owners(sg, &c0);
+                if (atomicAdd(a.arrived + sg, 1) == n - 1) a.arrived[sg] = 0, s_last[tid] = n, s_first[tid] = c0;
+            }
             __threadfence();
-            __syncthreads();
-            if (tid == 0) {
-                const uint32_t before = atomicAdd(a.arrived + seg, 1);
-                s_last = before == c1 - c0;
-                if (s_last) a.arrived[seg] = 0;
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                const float* part = a.part;
-                finish<HD, ROWS>(a, sb, hg, c1 - c0 + 1,
-                                 [&](uint32_t j) { return part + ((uint64_t)(c0 + j) * 2 + (j == 0)) * PIECE; }, tid, WARPS * 32);
-            }
-            __syncthreads();
         }
-        i = last + 1;  // pieces of a segment follow one another
+        __syncthreads();
+        for (uint32_t i = warp; i < 2 * ROWS; i += WARPS) {
+            const uint32_t which = i / ROWS, row = i % ROWS, n = s_last[which], c0 = s_first[which];
+            if (n == 0) continue;
+            const uint32_t sg = open_seg[which], hg = sg % groups, in_group = hg % a.split * ROWS + row;
+            if (in_group >= a.group) continue;
+            Joined<HD> y;
+            y.clear();
+            y.template add<ROWS, true>(
+                n, [&](uint32_t j) { return (const float*)(a.part + ((uint64_t)(c0 + j) * 2 + (j == 0)) * PIECE); }, row, lane);
+            y.finish(a, sg / groups, hg / a.split, in_group, lane);
+        }
     }
     // sequences without steps of their own
     for (uint32_t sb = blockIdx.x; sb < batch; sb += gridDim.x) {
@@ -668,7 +791,11 @@ __global__ void __launch_bounds__(WARPS * 32, MIN_CTAS) attention_paged_kernel(P
         if (own < 0 || a.len[sb] == 0) {
             for (uint32_t i = tid; i < a.n_q * HD; i += WARPS * 32) a.out[sb * a.out_stride + i] = own < 0 ? NAN : 0.0f;
         } else {
-            for (uint32_t hg = 0; hg < groups; ++hg) finish<HD, ROWS>(a, sb, hg, 0, [&](uint32_t) { return s_piece; }, tid, WARPS * 32);
+            for (uint32_t i = warp; i < a.n_q; i += WARPS) {
+                Joined<HD> y;
+                y.clear();
+                y.finish(a, sb, i / a.group, i % a.group, lane);
+            }
         }
     }
 }
@@ -694,66 +821,70 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_lead_kernel(PagedArgs
         },
         a.scale, lane, s_mem + warp * AREA);
     w.reset();
-    bool lost = false;
-    auto tile_of = [&](uint32_t u) -> const uint8_t* {
-        const int32_t id = __ldg(a.c.table + p0 + u / PER_PAGE);
-        const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
-        lost |= !fine;
-        return a.c.pages + ((uint64_t)(fine ? id : 0) * a.c.n_kv + kvh) * T::HEAD;
-    };
     if (u0 < u1) {
+        Pages<T> pages{a, a.c.table, kvh, lane, 0, p0 + (u1 - 1) / PER_PAGE + 1, 0, false};
+        pages.fetch(p0 + u0 / PER_PAGE);
+        const uint8_t* tile = pages.enter(p0 + u0 / PER_PAGE);
         Rows<T> k, v;
-        const uint8_t* tile = tile_of(u0);
         k.template load<true>(tile, u0 % PER_PAGE * T::POS, lane);
         for (uint32_t u = u0; u < u1; ++u) {
             v.template load<true>(tile + T::HEAD / 2, u % PER_PAGE * T::POS, lane);
             float s[T::GROUPS][NT][2 * At::COLS], alpha[At::MINE];
             w.scores(k, lane, s);
             if (u + 1 < u1) {
-                tile = tile_of(u + 1);
+                if ((u + 1) % PER_PAGE == 0) tile = pages.enter(p0 + (u + 1) / PER_PAGE);
                 k.template load<true>(tile, (u + 1) % PER_PAGE * T::POS, lane);
             }
             w.softmax(s, T::POS, lane, alpha);
             w.output(s, v, T::POS, lane, alpha);
         }
-    }
-    if (lost) {
+        if (pages.lost) {
 #pragma unroll
-        for (uint32_t i = 0; i < At::MINE; ++i) w.sum[i] = NAN;
-        if (lane == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+            for (uint32_t i = 0; i < At::MINE; ++i) w.sum[i] = NAN;
+            if (lane == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+        }
     }
     __syncthreads();  // the query operands have been read
     float* pieces = reinterpret_cast<float*>(s_mem);
     w.store(pieces + warp * AREA, lane);
-    __syncthreads();
-    const uint64_t all = (uint64_t)gridDim.x * a.c.n_kv * rows, base = ((uint64_t)split * a.c.n_kv + kvh) * rows;
-    for (uint32_t i = tid; i < sets * ROWS * (HD / 4); i += WARPS * 32) {
+    // the parts of the CTA's warps and of the cluster's CTAs (page splits of the same rows) are joined, a share of the rows a CTA
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), n = sets * ROWS * (HD / 4);
+    const uint64_t all = (uint64_t)(gridDim.x / ctas) * a.c.n_kv * rows, base = ((uint64_t)(split / ctas) * a.c.n_kv + kvh) * rows;
+    const uint32_t i1 = (rank + 1) * n / ctas;
+    for (uint32_t i = rank * n / ctas + tid; i < i1; i += WARPS * 32) {
         const uint32_t d = i % (HD / 4) * 4, r = i / (HD / 4) % ROWS, st = i / (HD / 4) / ROWS;
         const uint32_t row = (blockIdx.y * sets + st) * ROWS + r;
         if (row >= rows) continue;
         float top = -INFINITY, den = 0.0f;
-        for (uint32_t j = 0; j < parts; ++j) top = fmaxf(top, pieces[(j * sets + st) * AREA + ROWS * HD + r]);
+        for (uint32_t c = 0; c < ctas; ++c)
+            for (uint32_t j = 0; j < parts; ++j) top = fmaxf(top, cluster.map_shared_rank(pieces, c)[(j * sets + st) * AREA + ROWS * HD + r]);
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t j = 0; j < parts; ++j) {
-            const float* p = pieces + (j * sets + st) * AREA;
-            const float f = piece_weight(p[ROWS * HD + r], top);
-            const float4 y = *reinterpret_cast<const float4*>(p + r * HD + d);
-            sum.x = fmaf(f, y.x, sum.x), sum.y = fmaf(f, y.y, sum.y), sum.z = fmaf(f, y.z, sum.z), sum.w = fmaf(f, y.w, sum.w);
-            den = fmaf(f, p[ROWS * HD + ROWS + r], den);
-        }
+#pragma unroll 4
+        for (uint32_t c = 0; c < ctas; ++c)
+            for (uint32_t j = 0; j < parts; ++j) {
+                const float* p = cluster.map_shared_rank(pieces, c) + (j * sets + st) * AREA;
+                const float f = piece_weight(p[ROWS * HD + r], top);
+                const float4 y = *reinterpret_cast<const float4*>(p + r * HD + d);
+                sum.x = fmaf(f, y.x, sum.x), sum.y = fmaf(f, y.y, sum.y), sum.z = fmaf(f, y.z, sum.z), sum.w = fmaf(f, y.w, sum.w);
+                den = fmaf(f, p[ROWS * HD + ROWS + r], den);
+            }
         *reinterpret_cast<float4*>(lead + (base + row) * HD + d) = sum;
         if (d == 0) lead[all * HD + base + row] = top, lead[all * HD + all + base + row] = den;
     }
+    cluster.sync();  // the others have read this CTA's pieces
 }
 
-constexpr uint32_t AP_WARPS = 4, LEAD_WARPS = 8;
-constexpr uint32_t ap_ctas(uint32_t hd) { return hd == 256 ? 2 : 3; }  // a SM, by the registers that the kernel needs
+constexpr uint32_t LEAD_WARPS = 8;
+constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }  // of a CTA, one a SM, by the registers that the kernel needs
 constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
 
 // How a call is cut up: the same for its scratch and its launches.
 struct PagedPlan {
     uint32_t group, split, rows, grid;       // of the kernel over the sequences' own pages
     uint32_t lead, sets, blocks, splits;     // of the leading pages' kernel: pages, row sets of a CTA, row blocks, page splits
+    uint32_t cluster;                        // splits that one cluster joins
     size_t part_at, lead_at, bytes;
 };
 PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t shared) {
@@ -761,18 +892,24 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
     p.group = n_q / n_kv;
     p.rows = p.group <= 4 ? 4 : 8;
     p.split = (p.group + p.rows - 1) / p.rows;
-    p.grid = (uint32_t)num_sms() * ap_ctas(hd);
+    p.grid = (uint32_t)num_sms();
     p.lead = batch > 1 ? shared : 0;
     if (p.lead) {
         const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
         p.sets = 1;
         while (p.sets < LEAD_WARPS && p.sets < tiles) p.sets *= 2;
         p.blocks = (tiles + p.sets - 1) / p.sets;
-        p.splits = std::max(1u, std::min({p.lead, (uint32_t)num_sms() / std::max(1u, p.blocks * n_kv), 32u}));
+        // one wave of one CTA a SM.  Clusters of eight leave SMs of the GPU's groups idle (16 of them took two waves), so eight
+        // only where they are few
+        const uint32_t rows_of = std::max(1u, p.blocks * n_kv), fit = std::max(1u, std::min(p.lead, (uint32_t)num_sms() / rows_of));
+        p.cluster = fit >= 24 && 24 * rows_of <= (uint32_t)num_sms() * 2 / 3 ? 8 : 4;
+        while (p.cluster > fit) p.cluster /= 2;
+        p.splits = std::min(fit, LEAD_MOST * p.cluster);
+        p.splits = p.splits / p.cluster * p.cluster;
     }
     p.part_at = ((size_t)batch * n_kv * p.split * 4 + 255) / 256 * 256;
     p.lead_at = p.part_at + ((size_t)p.grid * 2 * p.rows * (hd + 2) * 4 + 255) / 256 * 256;
-    p.bytes = p.lead_at + (size_t)p.splits * n_q * batch * (hd + 2) * 4;
+    p.bytes = p.lead_at + (p.lead ? (size_t)(p.splits / p.cluster) * n_q * batch * (hd + 2) * 4 : 0);
     return p;
 }
 
@@ -785,11 +922,11 @@ struct LaunchPaged {
     template <class T, bool PAIRS>
     cudaError_t own() const {
         using At = Attend<T, 1, PAIRS>;
-        constexpr uint32_t BYTES = AP_WARPS * (2 * At::Q::ROWS * (T::HD + 2) + At::Q::WORDS) * 4;
-        auto kern = attention_paged_kernel<T, PAIRS, AP_WARPS, ap_ctas(T::HD)>;
+        constexpr uint32_t WARPS = ap_warps(T::HD), BYTES = WARPS * (2 * At::Q::ROWS * (T::HD + 2) + At::Q::WORDS) * 4;
+        auto kern = attention_paged_kernel<T, PAIRS, WARPS>;
         static bool configured[MAX_DEVICES] = {};
         if (cudaError_t e = set_max_smem_once(kern, BYTES + (ATTENTION_MAX_BATCH + 4) * 4, configured); e != cudaSuccess) return e;
-        return launch_pdl(kern, dim3(p.grid), AP_WARPS * 32, BYTES + ((a.c.n_seq + 4) & ~3u) * 4, s, a);
+        return launch_pdl(kern, dim3(p.grid), WARPS * 32, BYTES + ((a.c.n_seq + 4) & ~3u) * 4, s, a);
     }
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
@@ -800,7 +937,19 @@ struct LaunchPaged {
             auto kern = attention_lead_kernel<T, lead_tiles(HD), LEAD_WARPS>;
             static bool configured[MAX_DEVICES] = {};
             if (cudaError_t e = set_max_smem_once(kern, LEAD_WARPS * AREA * 4, configured); e != cudaSuccess) return e;
-            cudaError_t e = launch_pdl(kern, dim3(p.splits, p.blocks, a.c.n_kv), LEAD_WARPS * 32, LEAD_WARPS * AREA * 4, s, a, lead, p.sets);
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(p.splits, p.blocks, a.c.n_kv);
+            cfg.blockDim = dim3(LEAD_WARPS * 32);
+            cfg.dynamicSmemBytes = LEAD_WARPS * AREA * 4;
+            cfg.stream = s;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = p.cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+            attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[1].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, lead, p.sets);
             if (e != cudaSuccess) return e;
         }
         return p.rows == 4 ? own<T, true>() : own<T, false>();
@@ -819,7 +968,7 @@ cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_
     uint8_t* mem = static_cast<uint8_t*>(scratch);
     float* lead = reinterpret_cast<float*>(mem + p.lead_at);
     const PagedArgs a{c, q, q_stride, len, n_q, p.group, p.split, scale, shared, p.lead, out, out_stride,
-                      reinterpret_cast<uint32_t*>(mem), reinterpret_cast<float*>(mem + p.part_at), lead, p.splits, bad_pos};
+                      reinterpret_cast<uint32_t*>(mem), reinterpret_cast<float*>(mem + p.part_at), lead, p.lead ? p.splits / p.cluster : 0, bad_pos};
     cudaError_t e = for_kind(c.kind, c.hd, LaunchPaged{a, p, lead, s});
     return e != cudaSuccess ? e : cudaGetLastError();
 }
