@@ -5,6 +5,8 @@
 //   scores   S^T = K Q^T as m16n8k16 products, keys (codes as they are: whole numbers or halves, exact in f16) the 16-row
 //            operand, query rows the 8 columns, in two f16 terms under a power of two of their row (22 bits).  The accumulator
 //            of a block of 32 dimensions is scaled by the block's factor and added in f32.
+//            Codes of 8 and 4 bits stand in the low bits of a half as they are: a subnormal number, the code plus its bias times
+//            2^-24, which the products take exactly.  The bias times the sum of the query's terms is where their sums begin.
 //   output   O^T = V^T P^T, values the 16-row operand; probabilities times the value's scale of the block, under a power of two
 //            of the step's largest scale, in two f16 terms (22 bits below the largest).  Accumulators hold a step, not the
 //            sequence: the tensor core adds with truncation, the running output is added round-to-nearest.
@@ -36,6 +38,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = A B + (c0, c1) in the columns of this lane
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 // the 8x8 transpose between the accumulator's layout (row = position) and the B operand's (row of lanes = column)
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
@@ -74,8 +82,9 @@ template <uint32_t KIND_, uint32_t HD_>
 struct Step {
     static constexpr uint32_t KIND = KIND_, HD = HD_, NB = HD / 32, BITS = KIND == KV_F16 ? 16 : KIND == KV_Q8_0 ? 8 : 4;
     static constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);  // a head of a page
-    // positions at a time: 16 KB to 4 KB of codes, 16 to 64 registers a lane for keys and as many for values
-    static constexpr uint32_t WANT = 64 * 128 * 4 / (HD * BITS), POS = WANT < 16 ? 16 : WANT > 64 ? 64 : WANT;
+    // positions at a time: 4 KB of keys and of values, 32 registers a lane each (heads of 256 in halves: 64).  Four bits: 2 KB;
+    // 64 positions spill (24 ragged sequences of up to 16384, 32 / 4 heads of 128: 49.1 us, with 32 positions 41.7)
+    static constexpr uint32_t WANT = (KIND == KV_Q4_0 ? 32 : 64) * 128 * 4 / (HD * BITS), POS = WANT < 16 ? 16 : WANT > 64 ? 64 : WANT;
     static constexpr uint32_t GROUPS = POS / 16, VECS = POS * HD * BITS / 8 / 512;
     static constexpr uint32_t SW = KIND == KV_F16 ? 1 : POS / 16;  // words of two scales a block
 };
@@ -116,17 +125,19 @@ struct Rows {
         const float2 f = __half22float2(bits_half2(s[b][i / 2]));
         return i % 2 ? f.y : f.x;
     }
-    // A operand of 16 keys (group a) and 16 dimensions (half h of block b)
+    // A operand of 16 keys (group a) and 16 dimensions (half h of block b); codes with their bias, times 2^-24 (Q4_0: dimensions
+    // 2 and 3 of four times 2^-20)
     __device__ __forceinline__ void key(uint32_t a, uint32_t b, uint32_t h, uint32_t (&r)[4]) const {
         if constexpr (T::KIND == KV_F16) {
             const uint32_t v = (a * T::NB + b) * 2 + h;
             r[0] = word(v, 0), r[1] = word(v, 2), r[2] = word(v, 1), r[3] = word(v, 3);
         } else if constexpr (T::KIND == KV_Q8_0) {
             const uint32_t v = a * T::NB + b, x = word(v, h), y = word(v, 2 + h);
-            r[0] = codes8<0>(x), r[1] = codes8<0>(y), r[2] = codes8<2>(x), r[3] = codes8<2>(y);
+            r[0] = __byte_perm(x, 0, 0x4140), r[1] = __byte_perm(y, 0, 0x4140);
+            r[2] = __byte_perm(x, 0, 0x4342), r[3] = __byte_perm(y, 0, 0x4342);
         } else {
-            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + h);
-            r[0] = codes4<0>(x), r[1] = codes4<2>(x), r[2] = codes4<1>(x), r[3] = codes4<3>(x);
+            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + h), y = x >> 8;
+            r[0] = x & 0x000F000Fu, r[1] = y & 0x000F000Fu, r[2] = x & 0x00F000F0u, r[3] = y & 0x00F000F0u;
         }
     }
     // A operand of 16 dimensions (tile m of block b) and 16 positions (group a)
@@ -149,8 +160,9 @@ struct Rows {
 template <class T, uint32_t NT, bool PAIRS>
 struct Queries {
     static constexpr uint32_t ROWS = PAIRS ? 4 : 8 * NT, MINE = PAIRS ? 1 : 2 * NT;
-    // words of the B operand in shared memory: [tile][block half][term][lane] pairs
-    static constexpr uint32_t WORDS = PAIRS ? 0 : NT * (T::HD / 16) * 2 * 64;
+    // words in shared memory: the B operand, [tile][block half][term][lane] pairs (PAIRS: in registers), and what its sums begin
+    // with, [tile][block][lane % 4] pairs
+    static constexpr uint32_t OPERAND = PAIRS ? 0 : NT * (T::HD / 16) * 2 * 64, WORDS = OPERAND + NT * T::NB * 8;
 };
 
 template <class T, uint32_t NT, bool PAIRS>
@@ -158,7 +170,7 @@ struct Attend {
     using Q = Queries<T, NT, PAIRS>;
     static constexpr uint32_t HD = T::HD, NB = T::NB, GROUPS = T::GROUPS, MINE = Q::MINE, COLS = PAIRS ? 1 : 2;
     uint32_t qf[PAIRS ? 2 * NB : 1][2];  // B operand of the query rows, in registers (PAIRS)
-    const uint32_t* q_shared;            // or in shared memory
+    const uint32_t* q_shared;            // the rest of it
     float rf[MINE];                      // what a row's scores are multiplied by
     float mx[MINE], sum[MINE];           // running maximum; sum of this lane's positions
     float o[NB][2][NT][2 * COLS];        // dimensions 4 (lane / 4) + 2 m + {0, 1} of a block, by column
@@ -200,28 +212,45 @@ struct Attend {
             // a power of two that puts the row's largest value just below 2^15
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
             const float up = __uint_as_float(bits << 23);
-            const float down = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * scale * 1.44269504f;
+            const float down = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * scale *
+                               (T::KIND == KV_F16 ? 1.44269504f : 1.44269504f * 16777216.0f);
 #pragma unroll
-            for (uint32_t b = 0; b < NB; ++b)
+            for (uint32_t b = 0; b < NB; ++b) {
+                float sum = 0.0f;  // of the terms of this lane's column
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
+                    // Q4_0: the codes of dimensions 2 and 3 come times 16
+                    constexpr float OTHER = T::KIND == KV_Q4_0 ? 0.0625f : 1.0f;
                     uint32_t hi[2], lo[2];
                     split2(x[b][4 * h] * up, x[b][4 * h + 1] * up, &hi[0], &lo[0]);
-                    split2(x[b][4 * h + 2] * up, x[b][4 * h + 3] * up, &hi[1], &lo[1]);
+                    split2(x[b][4 * h + 2] * (up * OTHER), x[b][4 * h + 3] * (up * OTHER), &hi[1], &lo[1]);
+                    auto of = [](uint32_t w) {
+                        const float2 f = __half22float2(bits_half2(w));
+                        return f.x + f.y;
+                    };
                     if constexpr (PAIRS) {
                         qf[2 * b + h][0] = n % 2 ? lo[0] : hi[0], qf[2 * b + h][1] = n % 2 ? lo[1] : hi[1];
+                        sum += of(qf[2 * b + h][0]) + of(qf[2 * b + h][1]) * (1.0f / OTHER);
                     } else {
                         uint2* to = reinterpret_cast<uint2*>(shared) + ((t * 2 * NB + 2 * b + h) * 2) * 32 + lane;
                         to[0] = make_uint2(hi[0], hi[1]), to[32] = make_uint2(lo[0], lo[1]);
+                        sum += of(hi[0]) + of(lo[0]) + (of(hi[1]) + of(lo[1])) * (1.0f / OTHER);
                     }
                 }
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                sum *= T::KIND == KV_F16 ? 0.0f : T::KIND == KV_Q8_0 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f;
+                const float b0 = __shfl_sync(0xFFFFFFFFu, sum, 8 * c), b1 = __shfl_sync(0xFFFFFFFFu, sum, 8 * c + 4);
+                if (T::KIND != KV_F16 && n == 0)
+                    *reinterpret_cast<float2*>(shared + Q::OPERAND + ((t * NB + b) * 4 + c) * 2) = make_float2(b0, b1);
+            }
             if constexpr (PAIRS) {
                 rf[0] = __shfl_sync(0xFFFFFFFFu, down, 8 * c);
             } else {
                 rf[2 * t] = __shfl_sync(0xFFFFFFFFu, down, 8 * c), rf[2 * t + 1] = __shfl_sync(0xFFFFFFFFu, down, 8 * c + 4);
             }
         }
-        if constexpr (!PAIRS) __syncwarp();
+        __syncwarp();
     }
 
     // s[group][tile][...]: position lane / 4 (+ 8 in the upper half) by column
@@ -235,6 +264,14 @@ struct Attend {
 #pragma unroll
         for (uint32_t b = 0; b < NB; ++b) {
             uint2 q[2][NT][PAIRS ? 1 : 2];
+            float2 begin[NT];
+#pragma unroll
+            for (uint32_t t = 0; t < NT; ++t) {
+                if constexpr (T::KIND == KV_F16)
+                    begin[t] = make_float2(0.0f, 0.0f);
+                else
+                    begin[t] = *reinterpret_cast<const float2*>(q_shared + Q::OPERAND + ((t * NB + b) * 4 + lane % 4) * 2);
+            }
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
@@ -254,11 +291,11 @@ struct Attend {
                 if constexpr (T::KIND != KV_F16) up = k.scale(b, 2 * a), down = k.scale(b, 2 * a + 1);
 #pragma unroll
                 for (uint32_t t = 0; t < NT; ++t) {
-                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int term = PAIRS ? 0 : 1; term >= 0; --term)
-#pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) mma16816(d, r[h], q[h][t][term].x, q[h][t][term].y);
+                    float d[4];
+                    constexpr int LAST = PAIRS ? 0 : 1;
+                    mma16816(d, r[0], q[0][t][LAST].x, q[0][t][LAST].y, begin[t].x, begin[t].y);
+                    mma16816(d, r[1], q[1][t][LAST].x, q[1][t][LAST].y);
+                    if constexpr (!PAIRS) mma16816(d, r[0], q[0][t][0].x, q[0][t][0].y), mma16816(d, r[1], q[1][t][0].x, q[1][t][0].y);
                     if constexpr (PAIRS) {
                         s[a][t][0] = fmaf(d[0] + d[1], up, s[a][t][0]), s[a][t][1] = fmaf(d[2] + d[3], down, s[a][t][1]);
                     } else {
@@ -378,15 +415,18 @@ struct Attend {
             for (uint32_t m = 0; m < 2; ++m) {
                 float d[NT][4];
 #pragma unroll
-                for (uint32_t t = 0; t < NT; ++t) d[t][0] = d[t][1] = d[t][2] = d[t][3] = 0.0f;
-#pragma unroll
                 for (uint32_t a = 0; a < GROUPS; ++a) {
                     uint32_t r[4];
                     v.value(a, b, m, r);
 #pragma unroll
                     for (uint32_t t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int term = PAIRS ? 0 : 1; term >= 0; --term) mma16816(d[t], r, w.b[a][t][term][0], w.b[a][t][term][1]);
+                        for (int term = PAIRS ? 0 : 1; term >= 0; --term) {
+                            if (a == 0 && term == (PAIRS ? 0 : 1))
+                                mma16816(d[t], r, w.b[a][t][term][0], w.b[a][t][term][1], 0.0f, 0.0f);
+                            else
+                                mma16816(d[t], r, w.b[a][t][term][0], w.b[a][t][term][1]);
+                        }
                 }
 #pragma unroll
                 for (uint32_t t = 0; t < NT; ++t) {
