@@ -7,35 +7,25 @@ namespace jq {
 
 namespace {
 
-// One row of qkv [(n_q + 2 n_kv), HD] per blockIdx.x, a group of min(32, HD / 4) lanes a head, 4 (HD 256: 8) dimensions a lane.
-template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, RopeArgs r, const float* __restrict__ qkv, uint64_t stride,
-                                                        const int32_t* __restrict__ pos, const int32_t* __restrict__ seq, uint32_t n_q,
-                                                        const float* __restrict__ q_norm, const float* __restrict__ k_norm, float eps,
-                                                        float* __restrict__ q_out, int32_t* __restrict__ bad_pos) {
-    constexpr uint32_t LANES = HD / 4 < 32 ? HD / 4 : 32, QUADS = HD / 4 / LANES, HPW = 32 / LANES;
-    constexpr uint32_t CODES = kv_code_bytes(KIND, HD), SCALES = kv_scale_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD);
-    __shared__ __align__(16) float s_head[8 * HPW][HD];
-    pdl_trigger_all();
-    const uint32_t row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / LANES, li = lane % LANES;
-    const uint32_t heads = n_q + 2 * c.n_kv, head = (blockIdx.y * 8 + warp) * HPW + group;
-    const bool live = head < heads;
-    const int32_t p = pos[row];
-    uint8_t* page = page_of(c, seq ? seq[row] : (int32_t)row, p, HEAD);
-    if (page == nullptr || (r.table != nullptr && (uint32_t)p >= r.n_pos)) {  // the same in the whole row
-        if (blockIdx.y == 0 && threadIdx.x == 0 && bad_pos) atomicExch(bad_pos, 1);
-        return;
-    }
+// A group of min(32, HD / 4) lanes has a head of a row, 4 (HD 256: 8) dimensions a lane.
+template <uint32_t HD>
+struct HeadLanes {
+    static constexpr uint32_t LANES = HD / 4 < 32 ? HD / 4 : 32, QUADS = HD / 4 / LANES, PER_WARP = 32 / LANES;
     float x[QUADS][4];
-    const float* src = qkv + row * stride + (uint64_t)head * HD;
+
+    __device__ __forceinline__ static uint32_t dim(uint32_t i) { return 4 * (i * LANES + threadIdx.x % LANES); }
+    __device__ __forceinline__ void load(const float* src, bool live) {
 #pragma unroll
-    for (uint32_t i = 0; i < QUADS; ++i) {
-        const float4 v = live ? *reinterpret_cast<const float4*>(src + 4 * (i * LANES + li)) : make_float4(0, 0, 0, 0);
-        x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+        for (uint32_t i = 0; i < QUADS; ++i) {
+            const float4 v = live ? __ldg(reinterpret_cast<const float4*>(src + dim(i))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+        }
     }
-    const bool is_v = head >= n_q + c.n_kv, is_q = head < n_q;
-    const float* nw = is_q ? q_norm : k_norm;
-    if (nw != nullptr) {
+    __device__ __forceinline__ void store(float* dst) const {
+#pragma unroll
+        for (uint32_t i = 0; i < QUADS; ++i) *reinterpret_cast<float4*>(dst + dim(i)) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+    }
+    __device__ __forceinline__ void norm(const float* w, float eps) {
         float ss = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < QUADS; ++i)
@@ -44,65 +34,203 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, RopeArgs r, c
 #pragma unroll
         for (uint32_t o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
         const float sc = rsqrtf(ss / (float)HD + eps);
-        if (!is_v) {
-#pragma unroll
-            for (uint32_t i = 0; i < QUADS; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[i][e] = x[i][e] * sc * nw[4 * (i * LANES + li) + e];
-        }
-    }
-    if (r.table != nullptr) {  // values pass through shared memory too, and stay as they are
-        float* mine = s_head[warp * HPW + group];
 #pragma unroll
         for (uint32_t i = 0; i < QUADS; ++i)
-            *reinterpret_cast<float4*>(mine + 4 * (i * LANES + li)) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-        __syncwarp();
-        if (!is_v) {
 #pragma unroll
-            for (uint32_t i = 0; i < QUADS; ++i)
+            for (int e = 0; e < 4; ++e) x[i][e] = x[i][e] * sc * w[dim(i) + e];
+    }
+    // to position p; `mine`: HD floats of shared memory of these lanes
+    __device__ __forceinline__ void turn(const RopeArgs& r, uint32_t p, float* mine) {
+        const float2* t = r.table + (uint64_t)p * (r.rot / 2);
+        if (!r.interleaved) {
+            __syncwarp();
+            store(mine);
+            __syncwarp();
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < QUADS; ++i) {
+            const uint32_t d = dim(i);
+            if (r.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    if (d + e < r.rot) {
+                        const float2 cs = __ldg(t + (d + e) / 2);
+                        const float a = x[i][e], b = x[i][e + 1];
+                        x[i][e] = rope_rotate(true, a, b, cs), x[i][e + 1] = rope_rotate(false, b, a, cs);
+                    }
+            } else if (d < r.rot) {
+                const uint32_t half = r.rot / 2;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t d = 4 * (i * LANES + li) + e;
-                    if (d < r.rot)
-                        x[i][e] = rope_rotate(rope_first(r, d), x[i][e], mine[rope_partner(r, d)],
-                                              r.table[(uint64_t)p * (r.rot / 2) + rope_pair(r, d)]);
+                    const uint32_t at = d + e;
+                    if (at < r.rot) {
+                        const bool first = at < half;
+                        x[i][e] = rope_rotate(first, x[i][e], mine[first ? at + half : at - half], __ldg(t + (first ? at : at - half)));
+                    }
                 }
-        }
-    }
-    const uint32_t kvh = is_v ? head - n_q - c.n_kv : head - n_q, in_page = (uint32_t)p % KV_PAGE;
-    uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? CODES + SCALES : 0);
-#pragma unroll
-    for (uint32_t i = 0; i < QUADS; ++i) {
-        const uint32_t d = 4 * (i * LANES + li);
-        const KvQuad q = kv_round<KIND>(x[i]);
-        if (!live) continue;
-        if (is_q) {
-            *reinterpret_cast<float4*>(q_out + ((uint64_t)row * n_q + head) * HD + d) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
-            continue;
-        }
-        if (is_v) {
-            uint8_t* at = part + kv_value_at<KIND, HD>(in_page, d);
-            if constexpr (KIND == KV_F16) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<uint16_t*>(at + (e >> 1) * 512 + (e & 1) * 4) = (uint16_t)q.code[e];
-            } else if constexpr (KIND == KV_Q8_0) {
-#pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) at[(e >> 1) * 8 + (e & 1) * 2] = (uint8_t)q.code[e];
-            } else {
-                at[0] = (uint8_t)(q.code[0] | q.code[1] << 4), at[4] = (uint8_t)(q.code[2] | q.code[3] << 4);
             }
-        } else {
-            uint8_t* at = part + kv_key_at<KIND, HD>(in_page, d);
-            if constexpr (KIND == KV_F16)
-                *reinterpret_cast<uint2*>(at) = make_uint2(q.code[0] | q.code[1] << 16, q.code[2] | q.code[3] << 16);
-            else if constexpr (KIND == KV_Q8_0)
-                *reinterpret_cast<uint32_t*>(at) = q.code[0] | q.code[1] << 8 | q.code[2] << 16 | q.code[3] << 24;
-            else
-                at[0] = (uint8_t)(q.code[0] | q.code[2] << 4), at[2] = (uint8_t)(q.code[1] | q.code[3] << 4);
         }
-        if (KIND != KV_F16 && li % 8 == 0)
-            *reinterpret_cast<uint16_t*>(part + CODES + kv_scale_at<HD>(in_page, d / 32)) = q.scale;
     }
+    // a key's or value's codes as position `pos` of `codes`, its scales as position `in_page` of `scales`; all lanes of the warp,
+    // those with `live` store
+    template <uint32_t KIND>
+    __device__ __forceinline__ void put(uint8_t* codes, uint32_t pos, uint8_t* scales, uint32_t in_page, bool is_v, bool live) const {
+#pragma unroll
+        for (uint32_t i = 0; i < QUADS; ++i) {
+            const uint32_t d = dim(i);
+            const KvQuad q = kv_round<KIND>(x[i]);
+            if (!live) continue;
+            if (is_v) {
+                uint8_t* at = codes + kv_value_at<KIND, HD>(pos, d);
+                if constexpr (KIND == KV_F16) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) *reinterpret_cast<uint16_t*>(at + (e >> 1) * 512 + (e & 1) * 4) = (uint16_t)q.code[e];
+                } else if constexpr (KIND == KV_Q8_0) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) at[(e >> 1) * 8 + (e & 1) * 2] = (uint8_t)q.code[e];
+                } else {
+                    at[0] = (uint8_t)(q.code[0] | q.code[1] << 4), at[4] = (uint8_t)(q.code[2] | q.code[3] << 4);
+                }
+            } else {
+                uint8_t* at = codes + kv_key_at<KIND, HD>(pos, d);
+                if constexpr (KIND == KV_F16)
+                    *reinterpret_cast<uint2*>(at) = make_uint2(q.code[0] | q.code[1] << 16, q.code[2] | q.code[3] << 16);
+                else if constexpr (KIND == KV_Q8_0)
+                    *reinterpret_cast<uint32_t*>(at) = q.code[0] | q.code[1] << 8 | q.code[2] << 16 | q.code[3] << 24;
+                else
+                    at[0] = (uint8_t)(q.code[0] | q.code[2] << 4), at[2] = (uint8_t)(q.code[1] | q.code[3] << 4);
+            }
+            if (KIND != KV_F16 && dim(0) % 32 == 0)
+                *reinterpret_cast<uint16_t*>(scales + kv_scale_at<HD>(in_page, d / 32)) = q.scale;
+        }
+    }
+};
+
+struct AppendArgs {
+    KvPages c;
+    RopeArgs r;
+    const float* qkv;
+    uint64_t stride;
+    const int32_t *pos, *seq;
+    uint32_t rows, n_q;
+    const float *q_norm, *k_norm;
+    float eps;
+    float* q_out;
+    int32_t* bad_pos;
+
+    __device__ __forceinline__ int32_t seq_of(uint32_t row) const { return seq ? seq[row] : (int32_t)row; }
+    // the page of a row's position, NULL if it has no place
+    __device__ __forceinline__ uint8_t* page(uint32_t row, uint32_t head_bytes) const {
+        const int32_t p = pos[row];
+        uint8_t* at = page_of(c, seq_of(row), p, head_bytes);
+        return r.table != nullptr && (uint32_t)p >= r.n_pos ? nullptr : at;
+    }
+};
+
+// A row per blockIdx.x, a head a group of lanes.
+template <uint32_t KIND, uint32_t HD>
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
+    using Lanes = HeadLanes<HD>;
+    constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD);
+    __shared__ __align__(16) float s_head[8 * HPW][HD];
+    pdl_trigger_all();
+    const uint32_t row = blockIdx.x, warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES;
+    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = (blockIdx.y * 8 + warp) * HPW + group;
+    const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
+    uint8_t* page = a.page(row, HEAD);
+    if (page == nullptr) {  // the same in the whole row
+        if (blockIdx.y == 0 && threadIdx.x == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+        return;
+    }
+    Lanes x;
+    x.load(a.qkv + row * a.stride + (uint64_t)head * HD, live);
+    const uint32_t p = (uint32_t)a.pos[row];
+    if (__any_sync(0xFFFFFFFFu, !is_v)) {  // two heads a warp: a value's lanes go along, and stay as they were
+        const Lanes y = x;
+        if (a.q_norm) x.norm(is_q ? a.q_norm : a.k_norm, a.eps);
+        if (a.r.table) x.turn(a.r, p, s_head[warp * HPW + group]);
+        if (is_v) x = y;
+    }
+    const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
+    uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
+    if (live && is_q) x.store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
+    x.template put<KIND>(part, p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
+}
+
+// Which 16 positions a warp of the kernels below takes: rows first + j (j = 0 .. 15) stand at consecutive positions of one
+// sequence in one group of 16 of a page, if they do (`runs`).  Rows are grouped by the first row's position.
+struct RowGroup {
+    uint32_t first_j, rows;  // live ones: j = first_j .. first_j + rows - 1
+    int64_t first;           // row of j = 0 (may be in front of the first row)
+    bool runs;
+};
+__device__ __forceinline__ RowGroup row_group(const int32_t* pos, const int32_t* seq, uint32_t n, uint32_t block) {
+    const uint32_t lane = threadIdx.x & 31;
+    RowGroup g;
+    g.first = (int64_t)block * 16 - (pos[0] & 15);
+    const int64_t row = g.first + (lane & 15);
+    const bool live = row >= 0 && row < n;
+    const int32_t p = live ? pos[row] : 0, s = live ? seq ? seq[row] : (int32_t)row : 0;
+    const uint32_t all = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
+    g.rows = __popc(all), g.first_j = all ? __ffs(all) - 1 : 0;
+    const int32_t p0 = __shfl_sync(0xFFFFFFFFu, p, g.first_j) - (int32_t)g.first_j, s0 = __shfl_sync(0xFFFFFFFFu, s, g.first_j);
+    g.runs = p0 >= 0 && p0 % 16 == 0 && __all_sync(0xFFFFFFFFu, !live || (p == p0 + (int32_t)(lane & 15) && s == s0));
+    return g;
+}
+
+// Many rows: a warp has a head of 16 rows.  Where these are a whole run of 16 positions, the codes are put together in shared
+// memory as they stand in the page and stored from there in whole lines: a position's codes alone are 4 bytes and fewer to a
+// sector of 32.
+template <uint32_t KIND, uint32_t HD>
+__global__ void __launch_bounds__(256) kv_append_rows_kernel(AppendArgs a) {
+    using Lanes = HeadLanes<HD>;
+    constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD), RUN = CODES / 4;
+    constexpr uint32_t AHEAD = HD == 256 ? 2 : 4;  // rows whose loads are on their way together
+    extern __shared__ __align__(16) uint8_t s_mem[];  // [8][HPW][HD] floats, then [8][HPW][RUN] codes
+    pdl_trigger_all();
+    const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES;
+    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = (blockIdx.y * 8 + warp) * HPW + group;
+    float* s_head = reinterpret_cast<float*>(s_mem) + (warp * HPW + group) * HD;
+    uint8_t* s_run = s_mem + 8 * HPW * HD * 4 + (warp * HPW + group) * RUN;
+    if ((blockIdx.y * 8 + warp) * HPW >= heads) return;
+    const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
+    const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
+    const RowGroup g = row_group(a.pos, a.seq, a.rows, blockIdx.x);
+    uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places
+    if (g.runs && g.rows == 16 && a.page((uint32_t)g.first + 15, HEAD)) run = a.page((uint32_t)g.first, HEAD);
+    for (uint32_t j0 = g.first_j; j0 < g.first_j + g.rows; j0 += AHEAD) {
+        Lanes x[AHEAD];
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i)
+            x[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, live && j0 + i < g.first_j + g.rows);
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t row = (uint32_t)(g.first + j0 + i);
+            if (j0 + i >= g.first_j + g.rows) continue;
+            uint8_t* page = run ? run : a.page(row, HEAD);
+            if (page == nullptr) {
+                if (blockIdx.y == 0 && threadIdx.x == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+                continue;
+            }
+            const uint32_t p = (uint32_t)a.pos[row];
+            if (__any_sync(0xFFFFFFFFu, !is_v)) {
+                const Lanes y = x[i];
+                if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
+                if (a.r.table) x[i].turn(a.r, p, s_head);
+                if (is_v) x[i] = y;
+            }
+            if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
+            if (!__any_sync(0xFFFFFFFFu, live && !is_q)) continue;
+            uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
+            x[i].template put<KIND>(run ? s_run : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
+        }
+    }
+    __syncwarp();
+    if (run == nullptr || !live || is_q) return;
+    uint4* to = reinterpret_cast<uint4*>(run + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0) + (uint32_t)a.pos[g.first] % KV_PAGE / 16 * RUN);
+    const uint4* from = reinterpret_cast<const uint4*>(s_run);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x % Lanes::LANES; i < RUN / 16; i += Lanes::LANES) to[i] = from[i];
 }
 
 // A warp a row and kv head, keys and values.
@@ -126,23 +254,155 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvPages c, const int32_t* 
     }
 }
 
+// Sixteen positions of a head's keys or values from the run of memory that holds them: f(position, dimension, four values) for
+// each four that a lane has.
+template <uint32_t KIND, uint32_t HD, bool VALUES, class F>
+__device__ __forceinline__ void read_run(const uint8_t* part, uint32_t in_page, F f) {
+    constexpr uint32_t NB = HD / 32, BITS = KIND == KV_F16 ? 16 : KIND == KV_Q8_0 ? 8 : 4, VECS = 16 * HD * BITS / 8 / 512;
+    const uint32_t lane = threadIdx.x & 31, r = lane / 4, c = lane % 4;
+    const uint4* codes = reinterpret_cast<const uint4*>(part + in_page / 16 * (VECS * 512)) + lane;
+    const uint8_t* scales = part + kv_code_bytes(KIND, HD);
+    auto both = [&](uint32_t pos, uint32_t b) {  // scales of positions pos and pos + 8 of the run
+        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(scales + kv_scale_at<HD>(in_page + pos, b)));
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    };
+    auto half_of = [](uint32_t w, uint32_t i) { return __half2float(__ushort_as_half((unsigned short)(i ? w >> 16 : w & 0xFFFF))); };
+    if constexpr (KIND == KV_F16 && VALUES) {  // two vectors hold four dimensions
+#pragma unroll
+        for (uint32_t b = 0; b < NB; ++b) {
+            const uint4 x = __ldg(codes + 2 * b * 32), y = __ldg(codes + (2 * b + 1) * 32);
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e)
+                    f(8 * h + 2 * c + e, 32 * b + 4 * r,
+                      make_float4(half_of(u[2 * h], e), half_of(u[2 * h + 1], e), half_of(v[2 * h], e), half_of(v[2 * h + 1], e)));
+        }
+        return;
+    }
+#pragma unroll
+    for (uint32_t v = 0; v < VECS; ++v) {
+        const uint4 x = __ldg(codes + v * 32);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        if constexpr (KIND == KV_F16) {
+            const uint32_t d = 32 * (v / 2) + 8 * c + 4 * (v % 2);
+            f(r, d, make_float4(half_of(w[0], 0), half_of(w[0], 1), half_of(w[1], 0), half_of(w[1], 1)));
+            f(r + 8, d, make_float4(half_of(w[2], 0), half_of(w[2], 1), half_of(w[3], 0), half_of(w[3], 1)));
+        } else if constexpr (KIND == KV_Q8_0) {
+            auto at = [&](uint32_t i) { return (float)((int)(w[i / 4] >> (8 * (i % 4)) & 0xFF) - 128); };
+            if constexpr (VALUES) {
+#pragma unroll
+                for (uint32_t e = 0; e < 2; ++e) {
+                    const float2 s = both(2 * c + e, v);
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const float g = h ? s.y : s.x;
+                        f(8 * h + 2 * c + e, 32 * v + 4 * r, make_float4(at(4 * h + e) * g, at(4 * h + 2 + e) * g, at(8 + 4 * h + e) * g, at(10 + 4 * h + e) * g));
+                    }
+                }
+            } else {
+                const float2 s = both(r, v);
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t q = 0; q < 2; ++q) {
+                        const float g = h ? s.y : s.x;
+                        const uint32_t i = 8 * h + 4 * q;
+                        f(r + 8 * h, 32 * v + 8 * c + 4 * q, make_float4(at(i) * g, at(i + 1) * g, at(i + 2) * g, at(i + 3) * g));
+                    }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t o = 0; o < 2; ++o) {  // the two blocks of the vector
+                const uint32_t b = 2 * v + o;
+                auto at = [&](uint32_t i, uint32_t byte, uint32_t high) { return (float)((int)(w[2 * o + i] >> (8 * byte + 4 * high) & 15) - 8); };
+                if constexpr (VALUES) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const float2 s = both(2 * c + e, b);
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const float g = h ? s.y : s.x;
+                            const uint32_t y = 2 * e + h;
+                            f(8 * h + 2 * c + e, 32 * b + 4 * r, make_float4(at(0, y, 0) * g, at(0, y, 1) * g, at(1, y, 0) * g, at(1, y, 1) * g));
+                        }
+                    }
+                } else {
+                    const float2 s = both(r, b);
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                        for (uint32_t q = 0; q < 2; ++q) {
+                            const float g = h ? s.y : s.x;
+                            f(r + 8 * h, 32 * b + 8 * c + 4 * q, make_float4(at(q, h, 0) * g, at(q, 2 + h, 0) * g, at(q, h, 1) * g, at(q, 2 + h, 1) * g));
+                        }
+                }
+            }
+        }
+    }
+}
+
+// Many rows: a warp has the keys or values of a head of 16 rows; where they are consecutive positions, from one run of memory.
+template <uint32_t KIND, uint32_t HD, bool VALUES>
+__device__ __forceinline__ void read_rows(const KvPages& c, const int32_t* pos, const int32_t* seq, uint32_t rows, const RowGroup& g,
+                                          uint32_t head, float* out, uint64_t row_stride, int32_t* bad_pos) {
+    constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);
+    const uint32_t lane = threadIdx.x & 31;
+    float* to = out + g.first * (int64_t)row_stride;
+    if (g.runs) {
+        const uint32_t row = (uint32_t)(g.first + g.first_j);
+        const int32_t p = pos[row];
+        const uint8_t* page = page_of(c, seq ? seq[row] : (int32_t)row, p, HEAD);
+        if (page != nullptr) {
+            const uint8_t* part = page + (uint64_t)head * HEAD + (VALUES ? HEAD / 2 : 0);
+            const uint32_t end = g.first_j + g.rows;
+            read_run<KIND, HD, VALUES>(part, (uint32_t)p % KV_PAGE & ~15u, [&](uint32_t j, uint32_t d, float4 x) {
+                if (j >= g.first_j && j < end) *reinterpret_cast<float4*>(to + j * row_stride + d) = x;
+            });
+            return;
+        }
+    }
+    for (uint32_t j = g.first_j; j < g.first_j + g.rows; ++j) {
+        const uint32_t row = (uint32_t)(g.first + j);
+        const int32_t p = pos[row];
+        const uint8_t* page = page_of(c, seq ? seq[row] : (int32_t)row, p, HEAD);
+        if (page == nullptr && lane == 0 && bad_pos) atomicExch(bad_pos, 1);
+        const uint8_t* part = page + (uint64_t)head * HEAD + (VALUES ? HEAD / 2 : 0);
+        for (uint32_t d = 4 * lane; d < HD; d += 128)
+            *reinterpret_cast<float4*>(to + j * row_stride + d) =
+                page ? kv_load<KIND, HD, VALUES>(part, (uint32_t)p % KV_PAGE, d) : make_float4(NAN, NAN, NAN, NAN);
+    }
+}
+template <uint32_t KIND, uint32_t HD>
+__global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
+                                                           uint32_t rows, float* __restrict__ k, float* __restrict__ v, uint64_t row_stride,
+                                                           uint64_t head_stride, int32_t* __restrict__ bad_pos) {
+    pdl_trigger_all();
+    const uint32_t task = blockIdx.y * 8 + (threadIdx.x >> 5), head = task / 2;
+    if (head >= c.n_kv) return;
+    const RowGroup g = row_group(pos, seq, rows, blockIdx.x);
+    if (g.rows == 0) return;
+    if (task % 2)
+        read_rows<KIND, HD, true>(c, pos, seq, rows, g, head, v + head * head_stride, row_stride, bad_pos);
+    else
+        read_rows<KIND, HD, false>(c, pos, seq, rows, g, head, k + head * head_stride, row_stride, bad_pos);
+}
+
+// From so many rows on, 16 rows a warp: below, a row's latency counts.
+constexpr uint32_t MANY_ROWS = 128;
+
 struct LaunchAppend {
-    const KvPages& c;
-    const RopeArgs& r;
-    const float* qkv;
-    uint64_t stride;
-    const int32_t *pos, *seq;
-    uint32_t rows, n_q;
-    const float *q_norm, *k_norm;
-    float eps;
-    float* q_out;
-    int32_t* bad_pos;
+    const AppendArgs& a;
     cudaStream_t s;
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
-        const uint32_t per_cta = 8 * (HD < 128 ? 2 : 1), heads = n_q + 2 * c.n_kv;
-        return launch_pdl(kv_append_kernel<KIND, HD>, dim3(rows, (heads + per_cta - 1) / per_cta), 256, 0, s, c, r, qkv, stride, pos,
-                          seq, n_q, q_norm, k_norm, eps, q_out, bad_pos);
+        constexpr uint32_t PER_CTA = 8 * HeadLanes<HD>::PER_WARP, BYTES = PER_CTA * (HD * 4 + kv_code_bytes(KIND, HD) / 4);
+        const uint32_t parts = (a.n_q + 2 * a.c.n_kv + PER_CTA - 1) / PER_CTA;
+        if (a.rows < MANY_ROWS) return launch_pdl(kv_append_kernel<KIND, HD>, dim3(a.rows, parts), 256, 0, s, a);
+        static bool configured[MAX_DEVICES] = {};
+        if (cudaError_t e = set_max_smem_once(kv_append_rows_kernel<KIND, HD>, BYTES, configured); e != cudaSuccess) return e;
+        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3((a.rows + 30) / 16, parts), 256, BYTES, s, a);
     }
 };
 struct LaunchRead {
@@ -155,8 +415,11 @@ struct LaunchRead {
     cudaStream_t s;
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
-        return launch_pdl(kv_read_kernel<KIND, HD>, dim3(rows, (c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, k, v, row_stride, head_stride,
-                          bad_pos);
+        if (rows < MANY_ROWS)
+            return launch_pdl(kv_read_kernel<KIND, HD>, dim3(rows, (c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, k, v, row_stride,
+                              head_stride, bad_pos);
+        return launch_pdl(kv_read_rows_kernel<KIND, HD>, dim3((rows + 30) / 16, (2 * c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, rows, k, v,
+                          row_stride, head_stride, bad_pos);
     }
 };
 
@@ -165,7 +428,7 @@ struct LaunchRead {
 cudaError_t launch_kv_append(const KvPages& c, const RopeArgs& r, const float* qkv, uint64_t stride, const int32_t* pos,
                              const int32_t* seq, uint32_t rows, uint32_t n_q, const float* q_norm, const float* k_norm, float eps,
                              float* q_out, int32_t* bad_pos, cudaStream_t s) {
-    cudaError_t e = for_kind(c.kind, c.hd, LaunchAppend{c, r, qkv, stride, pos, seq, rows, n_q, q_norm, k_norm, eps, q_out, bad_pos, s});
+    cudaError_t e = for_kind(c.kind, c.hd, LaunchAppend{AppendArgs{c, r, qkv, stride, pos, seq, rows, n_q, q_norm, k_norm, eps, q_out, bad_pos}, s});
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

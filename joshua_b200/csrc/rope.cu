@@ -18,22 +18,64 @@ __global__ void __launch_bounds__(256) rope_table_kernel(RopeFrequencies f, uint
     }
 }
 
-// A thread takes the four dimensions 4 i .. 4 i + 3 of a head of a row, and reads those of their partners.
+// Eight dimensions a thread and head: four pairs and their table entries, read once for all heads that the thread takes (the
+// row's heads are spread over the threads of a CTA and over blockIdx.y).  Bound by memory: 2048 rows of 40 heads of 128 read and
+// written.
 __global__ void __launch_bounds__(256) rope_kernel(RopeArgs r, const float* __restrict__ x, uint64_t x_stride, const int32_t* __restrict__ pos,
-                                                   uint32_t rows, uint32_t heads, uint32_t hd, float sign, float* __restrict__ out,
-                                                   uint64_t out_stride, int32_t* __restrict__ bad_pos) {
+                                                   uint32_t heads, uint32_t hd, float sign, float* __restrict__ out, uint64_t out_stride,
+                                                   int32_t* __restrict__ bad_pos) {
     pdl_trigger_all();
-    const uint32_t per_row = heads * (hd / 2);
-    const uint64_t n = (uint64_t)rows * per_row;
-    for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < n; t += gridDim.x * 256ull) {
-        const uint32_t row = (uint32_t)(t / per_row), in_row = (uint32_t)(t % per_row), head = in_row / (hd / 2), i = in_row % (hd / 2);
-        const int32_t p = pos[row];
-        if (p < 0 || (uint32_t)p >= r.n_pos) {
-            if (in_row == 0 && bad_pos) atomicExch(bad_pos, 1);
-            continue;
+    const uint32_t row = blockIdx.x, per_head = hd / 8, j = threadIdx.x % per_head;
+    const uint32_t step = blockDim.x / per_head * gridDim.y, h0 = blockIdx.y * (blockDim.x / per_head) + threadIdx.x / per_head;
+    const int32_t p = pos[row];
+    if (p < 0 || (uint32_t)p >= r.n_pos) {
+        if (threadIdx.x == 0 && blockIdx.y == 0 && bad_pos) atomicExch(bad_pos, 1);
+        return;
+    }
+    const bool turns = 8 * j < r.rot;
+    // the two runs of four dimensions: a run and its partners, or neighbours
+    const uint32_t a = turns && !r.interleaved ? 4 * j : 8 * j, b = turns && !r.interleaved ? a + r.rot / 2 : a + 4;
+    float2 cs[4];
+    if (turns) {
+        const float4* t = reinterpret_cast<const float4*>(r.table + (uint64_t)p * (r.rot / 2) + 4 * j);
+        const float4 u = __ldg(t), v = __ldg(t + 1);
+        cs[0] = make_float2(u.x, u.y * sign), cs[1] = make_float2(u.z, u.w * sign);
+        cs[2] = make_float2(v.x, v.y * sign), cs[3] = make_float2(v.z, v.w * sign);
+    }
+    const float* src = x + row * x_stride;
+    float* dst = out + row * out_stride;
+#pragma unroll 4
+    for (uint32_t h = h0; h < heads; h += step) {
+        float4 u = *reinterpret_cast<const float4*>(src + h * hd + a), v = *reinterpret_cast<const float4*>(src + h * hd + b);
+        if (turns) {
+            float* first[4] = {&u.x, &u.y, &u.z, &u.w};
+            float* second[4] = {&v.x, &v.y, &v.z, &v.w};
+            if (r.interleaved) first[1] = &u.z, first[2] = &v.x, first[3] = &v.z, second[0] = &u.y, second[1] = &u.w, second[2] = &v.y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float va = *first[i], vb = *second[i];
+                *first[i] = rope_rotate(true, va, vb, cs[i]), *second[i] = rope_rotate(false, vb, va, cs[i]);
+            }
         }
+        *reinterpret_cast<float4*>(dst + h * hd + a) = u, *reinterpret_cast<float4*>(dst + h * hd + b) = v;
+    }
+}
+
+// The same for heads or rotated parts that are no multiple of 8, two dimensions a thread.
+__global__ void __launch_bounds__(256) rope_pairs_kernel(RopeArgs r, const float* __restrict__ x, uint64_t x_stride,
+                                                         const int32_t* __restrict__ pos, uint32_t heads, uint32_t hd, float sign,
+                                                         float* __restrict__ out, uint64_t out_stride, int32_t* __restrict__ bad_pos) {
+    pdl_trigger_all();
+    const uint32_t row = blockIdx.x, half = r.rot / 2;
+    const int32_t p = pos[row];
+    if (p < 0 || (uint32_t)p >= r.n_pos) {
+        if (threadIdx.x == 0 && bad_pos) atomicExch(bad_pos, 1);
+        return;
+    }
+    for (uint32_t t = threadIdx.x; t < heads * (hd / 2); t += blockDim.x) {
+        const uint32_t head = t / (hd / 2), i = t % (hd / 2);
         // pairs first, then the dimensions behind the rotated ones two by two
-        const uint32_t half = r.rot / 2, a = i >= half ? 2 * i : r.interleaved ? 2 * i : i, b = i >= half || r.interleaved ? a + 1 : a + half;
+        const uint32_t a = i >= half || r.interleaved ? 2 * i : i, b = i >= half || r.interleaved ? a + 1 : a + half;
         const float* src = x + row * x_stride + head * hd;
         float* dst = out + row * out_stride + head * hd;
         float va = src[a], vb = src[b];
@@ -58,9 +100,17 @@ cudaError_t launch_rope_table(const RopeFrequencies& f, uint32_t rot, uint32_t n
 
 cudaError_t launch_rope(const RopeArgs& r, const float* x, uint64_t x_stride, const int32_t* pos, uint32_t rows, uint32_t heads,
                         uint32_t hd, bool inverse, float* out, uint64_t out_stride, int32_t* bad_pos, cudaStream_t s) {
-    const uint64_t n = (uint64_t)rows * heads * (hd / 2);
-    cudaError_t e = launch_pdl(rope_kernel, (unsigned)std::min<uint64_t>((n + 255) / 256, 148 * 16), 256, 0, s, r, x, x_stride, pos, rows,
-                               heads, hd, inverse ? -1.0f : 1.0f, out, out_stride, bad_pos);
+    const float sign = inverse ? -1.0f : 1.0f;
+    cudaError_t e;
+    if (hd % 8 == 0 && r.rot % 8 == 0 && hd <= 2048 && reinterpret_cast<uintptr_t>(r.table) % 16 == 0) {
+        // four heads a thread, fewer where the rows alone do not fill the GPU
+        const uint32_t at_once = std::max(1u, 256 / (hd / 8)), threads = at_once * (hd / 8);
+        const uint32_t most = (heads + at_once - 1) / at_once, few = (most + 3) / 4;
+        const uint32_t parts = std::min(most, std::max(few, (uint32_t)(8 * num_sms()) / rows));
+        e = launch_pdl(rope_kernel, dim3(rows, parts), threads, 0, s, r, x, x_stride, pos, heads, hd, sign, out, out_stride, bad_pos);
+    } else {
+        e = launch_pdl(rope_pairs_kernel, dim3(rows), 256, 0, s, r, x, x_stride, pos, heads, hd, sign, out, out_stride, bad_pos);
+    }
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

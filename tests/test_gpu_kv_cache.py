@@ -65,7 +65,7 @@ def test_append_and_read(kind, hd, n_q, n_kv):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("rows,start", [(1, 0), (1, 63), (15, 1), (16, 16), (17, 47), (64, 0), (65, 63), (200, 30)])
+@pytest.mark.parametrize("rows,start", [(1, 0), (1, 63), (15, 1), (16, 16), (17, 47), (64, 0), (65, 63), (200, 30), (130, 63), (128, 16), (300, 7)])
 def test_prompts_of_all_lengths(kind, rows, start):
     """Runs that begin and end inside pages and groups of 16 leave their neighbours as they were."""
     import torch
@@ -86,15 +86,51 @@ def test_prompts_of_all_lengths(kind, rows, start):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_rows_of_several_sequences(kind, hd):
+    """Hundreds of rows in one call: prompts of three sequences one behind another, then the same rows in another order, and read
+    back in a third; rows without a place among them."""
+    import torch
+
+    n_q, n_kv = 3, 3
+    cache, table = make(kind, n_kv, hd, 3, 4, seed=hd)
+    rng = np.random.RandomState(hd)
+    seq = np.repeat([2, 0, 1], [150, 97, 120])
+    pos = np.concatenate([np.arange(150) + 31, np.arange(97), np.arange(120) + 64])
+    for order in (np.arange(len(pos)), rng.permutation(len(pos))):
+        x = rng.randn(len(pos), (n_q + 2 * n_kv) * hd).astype(np.float32)
+        q = cache.append(torch.from_numpy(x).cuda(), i32(pos[order]), table, n_q=n_q, seq=i32(seq[order]))
+        wq, wk, wv = split(x, n_q, n_kv, hd)
+        assert np.array_equal(q.cpu().numpy().reshape(wq.shape), wq)
+        back = rng.permutation(len(pos))
+        for again in (np.arange(len(pos)), back):
+            k, v = cache.read(i32(pos[order][again]), table, seq=i32(seq[order][again]))
+            assert np.array_equal(k.cpu().numpy(), ref.held(wk, kind)[again].transpose(1, 0, 2))
+            assert np.array_equal(v.cpu().numpy(), ref.held(wv, kind)[again].transpose(1, 0, 2))
+    cache.check_flags()
+    lost = pos.copy()
+    lost[40], lost[200] = -1, 4 * 64
+    x = rng.randn(len(pos), (n_q + 2 * n_kv) * hd).astype(np.float32)
+    out = torch.full((len(pos), n_q * hd), 7.0, device="cuda")
+    cache.append(torch.from_numpy(x).cuda(), i32(lost), table, n_q=n_q, seq=i32(seq), out=out)
+    assert bool((out[[40, 200]] == 7).all()) and int(cache.bad_pos) == 1
+    k, v = cache.read(i32(lost), table, seq=i32(seq))
+    want = ref.held(split(x, n_q, n_kv, hd)[1], kind).transpose(1, 0, 2)
+    want[:, [40, 200]] = np.nan
+    assert np.array_equal(k.cpu().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows", [40, 170])
 @pytest.mark.parametrize("hd,rot,interleaved", [(128, 128, False), (128, 64, True), (64, 64, True), (256, 96, False), (64, 2, False)])
-def test_rotation_on_the_way(kind, hd, rot, interleaved):
+def test_rotation_on_the_way(kind, rows, hd, rot, interleaved):
     import torch
 
     from joshua_b200.rope import Rope, rope_table
 
-    n_q, n_kv, rows = 3, 3, 40
-    rope = Rope(rope_table(500000.0, rot, 700, "cuda"), interleaved=interleaved)
-    cache, table = make(kind, n_kv, hd, 1, 11)
+    n_q, n_kv = 3, 3
+    rope = Rope(rope_table(500000.0, rot, 900, "cuda"), interleaved=interleaved)
+    cache, table = make(kind, n_kv, hd, 1, 13)
     torch.manual_seed(rot)
     x = torch.randn(rows, 9 * hd, device="cuda")
     pos = torch.arange(655, 655 + rows, dtype=torch.int32, device="cuda")
@@ -107,15 +143,15 @@ def test_rotation_on_the_way(kind, hd, rot, interleaved):
     assert np.array_equal(v.cpu().numpy(), ref.held(x[:, 6 * hd:].cpu().numpy().reshape(rows, 3, hd), kind).transpose(1, 0, 2))
 
 
-@pytest.mark.parametrize("hd", [64, 128, 256])
-def test_norms_on_the_way(hd):
+@pytest.mark.parametrize("hd,rows", [(64, 9), (128, 9), (256, 9), (64, 130), (128, 130), (256, 130)])
+def test_norms_on_the_way(hd, rows):
     """The per-head norm in front of the rotation.  Its sum of squares is rounded (hd products and sums, the root, two products:
     under (hd + 8) roundings of 2^-24 in all) and a key then by at most 2^-11 (halves)."""
     import torch
 
     from joshua_b200.rope import Rope, rope_table
 
-    n_q, n_kv, rows = 4, 2, 9
+    n_q, n_kv = 4, 2
     table_np = rope_table(10000.0, hd, 64, "cuda")
     rope = Rope(table_np)
     cache, table = make("f16", n_kv, hd, rows, 1)
