@@ -157,80 +157,84 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
     x.template put<KIND>(part, p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
 }
 
-// Which 16 positions a warp of the kernels below takes: rows first + j (j = 0 .. 15) stand at consecutive positions of one
-// sequence in one group of 16 of a page, if they do (`runs`).  Rows are grouped by the first row's position.
+// The 16 rows that a warp or CTA of the kernels below takes, first + j (j = 0 .. 15): rows are grouped by the first row's position.
 struct RowGroup {
-    uint32_t first_j, rows;  // live ones: j = first_j .. first_j + rows - 1
     int64_t first;           // row of j = 0 (may be in front of the first row)
-    bool runs;
-};
-__device__ __forceinline__ RowGroup row_group(const int32_t* pos, const int32_t* seq, uint32_t n, uint32_t block) {
-    const uint32_t lane = threadIdx.x & 31;
-    RowGroup g;
-    g.first = (int64_t)block * 16 - (pos[0] & 15);
-    const int64_t row = g.first + (lane & 15);
-    const bool live = row >= 0 && row < n;
-    const int32_t p = live ? pos[row] : 0, s = live ? seq ? seq[row] : (int32_t)row : 0;
-    const uint32_t all = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
-    g.rows = __popc(all), g.first_j = all ? __ffs(all) - 1 : 0;
-    const int32_t p0 = __shfl_sync(0xFFFFFFFFu, p, g.first_j) - (int32_t)g.first_j, s0 = __shfl_sync(0xFFFFFFFFu, s, g.first_j);
-    g.runs = p0 >= 0 && p0 % 16 == 0 && __all_sync(0xFFFFFFFFu, !live || (p == p0 + (int32_t)(lane & 15) && s == s0));
-    return g;
-}
+    uint32_t first_j, rows;  // live ones: j = first_j .. first_j + rows - 1
+    bool runs;               // they stand at consecutive positions of one sequence, within a group of 16 of a page
 
-// Many rows: a warp has a head of 16 rows.  Where these are a whole run of 16 positions, the codes are put together in shared
-// memory as they stand in the page and stored from there in whole lines: a position's codes alone are 4 bytes and fewer to a
-// sector of 32.
+    __device__ __forceinline__ RowGroup(const int32_t* pos, uint32_t n, uint32_t block) {
+        first = (int64_t)block * 16 - (pos[0] & 15);
+        first_j = first < 0 ? (uint32_t)-first : 0;
+        rows = (uint32_t)(min((int64_t)n, first + 16) - first) - first_j;
+        if (first + first_j >= n) rows = 0;
+    }
+    __device__ __forceinline__ bool has(uint32_t j) const { return j >= first_j && j < first_j + rows; }
+    __device__ __forceinline__ void look(const int32_t* pos, const int32_t* seq) {  // sets runs
+        const uint32_t j = threadIdx.x & 15;
+        const bool live = has(j);
+        const int32_t p = live ? pos[first + j] : 0, s = live ? seq ? seq[first + j] : (int32_t)(first + j) : 0;
+        const int32_t p0 = __shfl_sync(0xFFFFFFFFu, p, first_j & 15) - (int32_t)first_j, s0 = __shfl_sync(0xFFFFFFFFu, s, first_j & 15);
+        runs = p0 >= 0 && p0 % 16 == 0 && __all_sync(0xFFFFFFFFu, !live || (p == p0 + (int32_t)j && s == s0));
+    }
+};
+
+// Many rows: four warps have a head of 16 rows, four rows each, their loads on their way together.  Where the 16 are a whole run
+// of positions, the codes are put together in shared memory as they stand in the page and stored from there in whole lines: a
+// position's codes alone are 4 bytes and fewer to a sector of 32.
 template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256) kv_append_rows_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, HD == 256 ? 3 : 5) kv_append_rows_kernel(AppendArgs a) {
     using Lanes = HeadLanes<HD>;
     constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD), RUN = CODES / 4;
-    constexpr uint32_t AHEAD = HD == 256 ? 2 : 4;  // rows whose loads are on their way together
-    extern __shared__ __align__(16) uint8_t s_mem[];  // [8][HPW][HD] floats, then [8][HPW][RUN] codes
+    constexpr uint32_t EACH = 4;
+    __shared__ __align__(16) float s_head[8 * HPW][HD];
+    __shared__ __align__(16) uint8_t s_run[2 * HPW][RUN];
     pdl_trigger_all();
-    const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES;
-    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = (blockIdx.y * 8 + warp) * HPW + group;
-    float* s_head = reinterpret_cast<float*>(s_mem) + (warp * HPW + group) * HD;
-    uint8_t* s_run = s_mem + 8 * HPW * HD * 4 + (warp * HPW + group) * RUN;
-    if ((blockIdx.y * 8 + warp) * HPW >= heads) return;
+    const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES, local = (warp & 1) * HPW + group;
+    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = blockIdx.y * 2 * HPW + local;
     const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
     const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
-    const RowGroup g = row_group(a.pos, a.seq, a.rows, blockIdx.x);
-    uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places
+    RowGroup g(a.pos, a.rows, blockIdx.x);
+    const uint32_t j0 = warp / 2 * EACH;
+    Lanes x[EACH];
+#pragma unroll
+    for (uint32_t i = 0; i < EACH; ++i)
+        x[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, live && g.has(j0 + i));
+    g.look(a.pos, a.seq);
+    uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places; the same in the CTA
     if (g.runs && g.rows == 16 && a.page((uint32_t)g.first + 15, HEAD)) run = a.page((uint32_t)g.first, HEAD);
-    for (uint32_t j0 = g.first_j; j0 < g.first_j + g.rows; j0 += AHEAD) {
-        Lanes x[AHEAD];
+    const bool turns = __any_sync(0xFFFFFFFFu, live && !is_v);  // two heads a warp: a value's lanes go along, and stay as they were
 #pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i)
-            x[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, live && j0 + i < g.first_j + g.rows);
-#pragma unroll
-        for (uint32_t i = 0; i < AHEAD; ++i) {
-            const uint32_t row = (uint32_t)(g.first + j0 + i);
-            if (j0 + i >= g.first_j + g.rows) continue;
-            uint8_t* page = run ? run : a.page(row, HEAD);
-            if (page == nullptr) {
-                if (blockIdx.y == 0 && threadIdx.x == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-                continue;
-            }
-            const uint32_t p = (uint32_t)a.pos[row];
-            if (__any_sync(0xFFFFFFFFu, !is_v)) {
-                const Lanes y = x[i];
-                if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
-                if (a.r.table) x[i].turn(a.r, p, s_head);
-                if (is_v) x[i] = y;
-            }
-            if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
-            if (!__any_sync(0xFFFFFFFFu, live && !is_q)) continue;
-            uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
-            x[i].template put<KIND>(run ? s_run : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
+    for (uint32_t i = 0; i < EACH; ++i) {
+        if (!g.has(j0 + i)) continue;
+        const uint32_t row = (uint32_t)(g.first + j0 + i);
+        uint8_t* page = run ? run : a.page(row, HEAD);
+        if (page == nullptr) {
+            if (blockIdx.y == 0 && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+            continue;
         }
+        const uint32_t p = (uint32_t)a.pos[row];
+        if (turns) {
+            const Lanes y = x[i];
+            if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
+            if (a.r.table) x[i].turn(a.r, p, s_head[warp * HPW + group]);
+            if (is_v) x[i] = y;
+        }
+        if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
+        if (!__any_sync(0xFFFFFFFFu, live && !is_q)) continue;
+        uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
+        x[i].template put<KIND>(run ? s_run[local] : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
     }
-    __syncwarp();
-    if (run == nullptr || !live || is_q) return;
-    uint4* to = reinterpret_cast<uint4*>(run + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0) + (uint32_t)a.pos[g.first] % KV_PAGE / 16 * RUN);
-    const uint4* from = reinterpret_cast<const uint4*>(s_run);
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x % Lanes::LANES; i < RUN / 16; i += Lanes::LANES) to[i] = from[i];
+    if (run == nullptr) return;
+    __syncthreads();
+    const uint32_t at = (uint32_t)a.pos[g.first] % KV_PAGE / 16 * RUN;
+    for (uint32_t i = threadIdx.x; i < 2 * HPW * (RUN / 16); i += 256) {
+        const uint32_t h = blockIdx.y * 2 * HPW + i / (RUN / 16), o = i % (RUN / 16) * 16;
+        if (h < a.n_q || h >= heads) continue;
+        const bool v = h >= a.n_q + a.c.n_kv;
+        uint8_t* part = run + (uint64_t)(v ? h - a.n_q - a.c.n_kv : h - a.n_q) * HEAD + (v ? HEAD / 2 : 0);
+        *reinterpret_cast<uint4*>(part + at + o) = *reinterpret_cast<const uint4*>(s_run[i / (RUN / 16)] + o);
+    }
 }
 
 // A warp a row and kv head, keys and values.
@@ -381,8 +385,9 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int3
     pdl_trigger_all();
     const uint32_t task = blockIdx.y * 8 + (threadIdx.x >> 5), head = task / 2;
     if (head >= c.n_kv) return;
-    const RowGroup g = row_group(pos, seq, rows, blockIdx.x);
+    RowGroup g(pos, rows, blockIdx.x);
     if (g.rows == 0) return;
+    g.look(pos, seq);
     if (task % 2)
         read_rows<KIND, HD, true>(c, pos, seq, rows, g, head, v + head * head_stride, row_stride, bad_pos);
     else
@@ -397,12 +402,11 @@ struct LaunchAppend {
     cudaStream_t s;
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
-        constexpr uint32_t PER_CTA = 8 * HeadLanes<HD>::PER_WARP, BYTES = PER_CTA * (HD * 4 + kv_code_bytes(KIND, HD) / 4);
-        const uint32_t parts = (a.n_q + 2 * a.c.n_kv + PER_CTA - 1) / PER_CTA;
-        if (a.rows < MANY_ROWS) return launch_pdl(kv_append_kernel<KIND, HD>, dim3(a.rows, parts), 256, 0, s, a);
-        static bool configured[MAX_DEVICES] = {};
-        if (cudaError_t e = set_max_smem_once(kv_append_rows_kernel<KIND, HD>, BYTES, configured); e != cudaSuccess) return e;
-        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3((a.rows + 30) / 16, parts), 256, BYTES, s, a);
+        constexpr uint32_t HPW = HeadLanes<HD>::PER_WARP;
+        const uint32_t heads = a.n_q + 2 * a.c.n_kv;
+        if (a.rows < MANY_ROWS)
+            return launch_pdl(kv_append_kernel<KIND, HD>, dim3(a.rows, (heads + 8 * HPW - 1) / (8 * HPW)), 256, 0, s, a);
+        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3((a.rows + 30) / 16, (heads + 2 * HPW - 1) / (2 * HPW)), 256, 0, s, a);
     }
 };
 struct LaunchRead {

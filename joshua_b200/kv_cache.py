@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import JoshuaB200Error, check
-from .rope import Rope, rows_arg, stream_of, tensor_arg, vector_arg
+from .rope import Rope, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 PAGE = 64
 TYPES = {"f16": 1, "q4_0": 2, "q8_0": 8}
@@ -34,7 +34,7 @@ class PagedCache:
             raise JoshuaB200Error(_lib.E_INVALID, f"a cache of {n_kv} heads of {head_dim}: head_dim 64, 128 or 256")
         if pages is None:
             pages = torch.empty(n_pages, self.page_bytes, dtype=torch.uint8, device=device)
-        tensor_arg(pages, "pages", torch.uint8)
+        self._index = device_index(pages, "pages", torch.uint8)
         if not pages.is_contiguous() or pages.shape[0] == 0 or pages.numel() != pages.shape[0] * self.page_bytes:
             raise JoshuaB200Error(_lib.E_INVALID, f"pages must be contiguous, [pages, {self.page_bytes}] bytes, not {list(pages.shape)}")
         self.kind, self.n_kv, self.head_dim, self.pages, self.device = kind, n_kv, head_dim, pages, pages.device
@@ -46,52 +46,55 @@ class PagedCache:
         self._scratch: dict = {}
 
     def _table(self, table):
-        tensor_arg(table, "table", torch.int32, self.device)
-        if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-            raise JoshuaB200Error(_lib.E_INVALID, "a page table is [sequences, pages] with contiguous rows")
-        if table.shape[0] > 1 and table.stride(0) != table.shape[1]:
-            raise JoshuaB200Error(_lib.E_INVALID, "the rows of a page table follow one another")
-        return table.data_ptr(), table.shape[0], table.shape[1]
+        if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.get_device() != self._index \
+                or table.dim() != 2 or not table.is_contiguous():
+            raise JoshuaB200Error(_lib.E_INVALID, f"a page table is contiguous int32 [sequences, pages] on {self.device}")
+        return table.data_ptr(), table.size(0), table.size(1)
 
     def append(self, qkv: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, n_q: int, seq: torch.Tensor | None = None,
                rope: Rope | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 0.0,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """Rows [rows, (n_q + 2 n_kv) * head_dim] at positions `pos` of sequences `seq` (None: row i is sequence i): keys and
         values into the cache, the rotated queries [rows, n_q * head_dim] returned."""
-        at, stride, rows = rows_arg(qkv, "qkv", (n_q + 2 * self.n_kv) * self.head_dim, self.device)
+        index, hd, i32, f32 = self._index, self.head_dim, torch.int32, torch.float32
+        at, stride, rows = rows_arg(qkv, "qkv", (n_q + 2 * self.n_kv) * hd, index)
         if out is None:
-            out = torch.empty(rows, n_q * self.head_dim, dtype=torch.float32, device=self.device)
-        elif not out.is_contiguous() or out.shape != (rows, n_q * self.head_dim):
-            raise JoshuaB200Error(_lib.E_INVALID, f"out must be contiguous, [{rows}, {n_q * self.head_dim}]")
-        tensor_arg(out, "out", torch.float32, self.device)
-        if rope is not None and rope.device != self.device:
+            out = _new(rows, n_q * hd, dtype=f32, device=self.device)
+            to = out.data_ptr()
+        else:
+            to = block_arg(out, "out", (rows, n_q * hd), f32, index)
+        if rope is not None and rope._index != index:
             raise JoshuaB200Error(_lib.E_INVALID, "the rope table is on another device")
         pages, n_seq, per = self._table(table)
-        check(self._append(self._ref, rope.ref if rope else None, at, stride, vector_arg(pos, "pos", rows, torch.int32, self.device),
-                           vector_arg(seq, "seq", rows, torch.int32, self.device) if seq is not None else None, pages, n_seq, per,
-                           rows, n_q, vector_arg(q_norm, "q_norm", self.head_dim, torch.float32, self.device) if q_norm is not None else None,
-                           vector_arg(k_norm, "k_norm", self.head_dim, torch.float32, self.device) if k_norm is not None else None,
-                           eps, out.data_ptr(), self._bad, stream_of(qkv)))
+        rc = self._append(self._ref, rope.ref if rope is not None else None, at, stride, vector_arg(pos, "pos", rows, i32, index),
+                          None if seq is None else vector_arg(seq, "seq", rows, i32, index), pages, n_seq, per, rows, n_q,
+                          None if q_norm is None else vector_arg(q_norm, "q_norm", hd, f32, index),
+                          None if k_norm is None else vector_arg(k_norm, "k_norm", hd, f32, index), eps, to, self._bad,
+                          _raw_stream(index))
+        if rc:
+            check(rc)
         return out
 
     def read(self, pos: torch.Tensor, table: torch.Tensor, seq: torch.Tensor | None = None, out=None):
         """(keys, values) f32 [n_kv, rows, head_dim] of positions `pos` of sequences `seq` (None: row i is sequence i), into
         `out` (a pair of such tensors, [n_kv, at least rows, head_dim]) if given."""
-        rows = pos.shape[0]
+        index, hd, n_kv = self._index, self.head_dim, self.n_kv
+        rows = most = pos.size(0) if isinstance(pos, torch.Tensor) and pos.dim() else 0
+        at = vector_arg(pos, "pos", rows, torch.int32, index)
         if out is None:
-            out = torch.empty(2, self.n_kv, rows, self.head_dim, dtype=torch.float32, device=self.device).unbind(0)
-        k, v = out
-        for t in out:
-            tensor_arg(t, "out", torch.float32, self.device)
-            if t.dim() != 3 or t.shape[0] != self.n_kv or t.shape[1] < rows or t.shape[2] != self.head_dim or not t.is_contiguous():
-                raise JoshuaB200Error(_lib.E_INVALID, f"out must be contiguous, [{self.n_kv}, at least {rows}, {self.head_dim}]")
-        if k.shape != v.shape:
-            raise JoshuaB200Error(_lib.E_INVALID, "keys and values go to tensors of one shape")
+            out = _new(2, n_kv, rows, hd, dtype=torch.float32, device=self.device).unbind(0)
+            k_at, v_at = out[0].data_ptr(), out[1].data_ptr()
+        else:
+            most = out[0].size(1) if isinstance(out[0], torch.Tensor) and out[0].dim() == 3 else -1
+            if most < rows:
+                raise JoshuaB200Error(_lib.E_INVALID, f"out must be two tensors [{n_kv}, at least {rows}, {hd}]")
+            k_at, v_at = (block_arg(t, "out", (n_kv, most, hd), torch.float32, index) for t in out)
         pages, n_seq, per = self._table(table)
-        check(self._read(self._ref, vector_arg(pos, "pos", rows, torch.int32, self.device),
-                         vector_arg(seq, "seq", rows, torch.int32, self.device) if seq is not None else None, pages, n_seq, per, rows,
-                         k.data_ptr(), v.data_ptr(), self.head_dim, max(k.shape[1], 1) * self.head_dim, self._bad, stream_of(pos)))
-        return k, v
+        rc = self._read(self._ref, at, None if seq is None else vector_arg(seq, "seq", rows, torch.int32, index), pages, n_seq, per,
+                        rows, k_at, v_at, hd, (most or 1) * hd, self._bad, _raw_stream(index))
+        if rc:
+            check(rc)
+        return out
 
     def scratch(self, batch: int, n_q: int, shared_pages: int = 0) -> torch.Tensor:
         """Zeroed scratch for `attend` of such calls, one stream at a time."""
@@ -102,21 +105,27 @@ class PagedCache:
                out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one query row per sequence, [batch, n_q * head_dim], over its first `lens` positions; the first
         `shared_pages` pages are the same for all.  `scratch`: from `scratch()`; by default one a stream, kept with the cache."""
-        at, stride, batch = rows_arg(q, "q", n_q * self.head_dim, self.device)
+        index, width = self._index, n_q * self.head_dim
+        at, stride, batch = rows_arg(q, "q", width, index)
+        n = batch
         if out is None:
-            out = torch.empty(batch, n_q * self.head_dim, dtype=torch.float32, device=self.device)
-        to, out_stride, n = rows_arg(out, "out", n_q * self.head_dim, self.device)
+            out = _new(batch, width, dtype=torch.float32, device=self.device)
+            to, out_stride = out.data_ptr(), width
+        else:
+            to, out_stride, n = rows_arg(out, "out", width, index)
         pages, n_seq, per = self._table(table)
         if n != batch or n_seq != batch:
             raise JoshuaB200Error(_lib.E_INVALID, f"{batch} query rows, {n} rows of out, {n_seq} of the page table")
-        stream = stream_of(q)
+        stream = _raw_stream(index)
         if scratch is None:
             key = (stream, batch, n_q, shared_pages)
             scratch = self._scratch.get(key)
             if scratch is None:
                 scratch = self._scratch[key] = self.scratch(batch, n_q, shared_pages)
-        check(self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, self.device), pages, batch, per, n_q,
-                           scale, shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream))
+        rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
+                          shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)
+        if rc:
+            check(rc)
         return out
 
     def check_flags(self) -> None:

@@ -15,33 +15,47 @@ from ._lib import JoshuaB200Error, check
 SCALINGS = {None: 0, "none": 0, "linear": 1, "yarn": 2}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+_new, _f32 = torch.empty, torch.float32
 
 
-def stream_of(t: torch.Tensor) -> int:
-    """The current stream of a tensor's device, as the C entries take it."""
-    return _raw_stream(t.device.index)
+def stream_of(index: int) -> int:
+    """The current stream of a device, as the C entries take it."""
+    return _raw_stream(index)
 
 
-def tensor_arg(t, name, dtype, device=None):
-    """Refuses what is no CUDA tensor of `dtype` (on `device`) before its pointer is handed on."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or (device is not None and t.device != device):
-        raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be a {dtype} tensor on the GPU"
-                              + (f" ({device})" if device is not None else ""))
-    return t
+def _refuse(t, name, dtype, index, shape):
+    got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be {shape} of {dtype} on cuda:{index}, not {got}")
 
 
-def rows_arg(t, name, width, device=None):
-    """(pointer, floats between rows, rows) of a two-dimensional f32 tensor whose rows are contiguous."""
-    tensor_arg(t, name, torch.float32, device)
-    if t.dim() != 2 or t.shape[1] != width or (t.stride(1) != 1 and width != 1):
-        raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be [rows, {width}] with contiguous rows, not {list(t.shape)}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else max(t.stride(0), width), t.shape[0]
+def device_index(t, name, dtype) -> int:
+    """The GPU that a tensor of `dtype` is on; refuses all else."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype:
+        raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be a {dtype} tensor on the GPU")
+    return t.get_device()
 
 
-def vector_arg(t, name, n, dtype, device):
-    tensor_arg(t, name, dtype, device)
-    if t.dim() != 1 or t.shape[0] != n or (n > 1 and t.stride(0) != 1):
-        raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be a contiguous vector of {n}, not {list(t.shape)}")
+def rows_arg(t, name, width, index):
+    """(pointer, floats between rows, rows) of a two-dimensional f32 tensor with contiguous rows."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not _f32 or t.get_device() != index or t.dim() != 2 or t.size(1) != width \
+            or (width != 1 and t.stride(1) != 1):
+        _refuse(t, name, _f32, index, f"[rows, {width}] with contiguous rows")
+    rows, stride = t.size(0), t.stride(0)
+    return t.data_ptr(), stride if rows > 1 else max(stride, width), rows
+
+
+def vector_arg(t, name, n, dtype, index):
+    """Pointer of a contiguous vector."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or t.dim() != 1 or t.size(0) != n \
+            or (n > 1 and t.stride(0) != 1):
+        _refuse(t, name, dtype, index, f"a contiguous vector of {n}")
+    return t.data_ptr()
+
+
+def block_arg(t, name, shape, dtype, index):
+    """Pointer of a contiguous tensor of `shape`."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        _refuse(t, name, dtype, index, f"contiguous, {list(shape)},")
     return t.data_ptr()
 
 
@@ -68,8 +82,9 @@ def rope_table(theta: float, rot_dim: int, n_pos: int, device, scaling: str | No
         factors = (ctypes.c_float * len(freq_factors))(*[float(f) for f in freq_factors])
     device = torch.device(device)
     with torch.cuda.device(device):
-        table = torch.empty(max(n_pos, 0), max(rot_dim, 0) // 2, 2, dtype=torch.float32, device=device)
-        check(_lib.lib().jq_rope_table_dev(ctypes.byref(cfg), factors, rot_dim, n_pos, table.data_ptr() or None, stream_of(table)))
+        table = _new(max(n_pos, 0), max(rot_dim, 0) // 2, 2, dtype=_f32, device=device)
+        check(_lib.lib().jq_rope_table_dev(ctypes.byref(cfg), factors, rot_dim, n_pos, table.data_ptr() or None,
+                                           stream_of(torch.cuda.current_device())))
     return table
 
 
@@ -77,7 +92,7 @@ class Rope:
     """A table of `rope_table` and how a head's dimensions pair up."""
 
     def __init__(self, table: torch.Tensor, interleaved: bool = False):
-        tensor_arg(table, "table", torch.float32)
+        self._index = device_index(table, "table", _f32)
         if table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous():
             raise JoshuaB200Error(_lib.E_INVALID, "a rope table is contiguous, [positions, pairs, 2]")
         self.table, self.interleaved, self.device = table, interleaved, table.device
@@ -89,12 +104,17 @@ class Rope:
     def apply(self, x: torch.Tensor, pos: torch.Tensor, heads: int, head_dim: int, inverse: bool = False,
               out: torch.Tensor | None = None) -> torch.Tensor:
         """Rows [rows, heads * head_dim] turned to their positions (`inverse`: back), into `out` (may be `x`)."""
-        at, stride, rows = rows_arg(x, "x", heads * head_dim, self.device)
+        index, width = self._index, heads * head_dim
+        at, stride, rows = rows_arg(x, "x", width, index)
         if out is None:
-            out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        to, out_stride, n = rows_arg(out, "out", heads * head_dim, self.device)
-        if n != rows:
-            raise JoshuaB200Error(_lib.E_INVALID, f"out has {n} rows for {rows}")
-        check(self._entry(self.ref, at, stride, vector_arg(pos, "pos", rows, torch.int32, self.device), rows, heads, head_dim,
-                          inverse, to, out_stride, self._bad, stream_of(x)))
+            out = _new(rows, width, dtype=_f32, device=self.device)
+            to, out_stride = out.data_ptr(), width
+        else:
+            to, out_stride, n = rows_arg(out, "out", width, index)
+            if n != rows:
+                raise JoshuaB200Error(_lib.E_INVALID, f"out has {n} rows for {rows}")
+        rc = self._entry(self.ref, at, stride, vector_arg(pos, "pos", rows, torch.int32, index), rows, heads, head_dim, inverse, to,
+                         out_stride, self._bad, _raw_stream(index))
+        if rc:
+            check(rc)
         return out

@@ -5,7 +5,7 @@ import torch
 
 from . import _lib
 from ._lib import JoshuaB200Error, check
-from .rope import rows_arg, stream_of, tensor_arg, vector_arg
+from .rope import _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 WINDOW = 64
 _entry = None
@@ -22,22 +22,24 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=None, top_k=
     global _entry
     if _entry is None:
         _entry = _lib.lib().jq_sample_dev
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+    f32, i32 = torch.float32, torch.int32
+    index = device_index(logits, "logits", f32)
+    if logits.dim() != 2:
         raise JoshuaB200Error(_lib.E_INVALID, "logits must be [rows, vocab]")
-    at, stride, rows = rows_arg(logits, "logits", logits.shape[1])
-    dev, f32, i32 = logits.device, torch.float32, torch.int32
-
-    def vec(t, name, dtype):
-        return None if t is None else vector_arg(t, name, rows, dtype, dev)
-
-    for t, name, width in ((window, "window", WINDOW), (window_state, "window_state", 2)):
-        if t is not None and (tensor_arg(t, name, i32, dev).shape != (rows, width) or not t.is_contiguous()):
-            raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be contiguous, [{rows}, {width}]")
+    vocab = logits.size(1)
+    at, stride, rows = rows_arg(logits, "logits", vocab, index)
     if token is None:
-        token = torch.empty(rows, dtype=i32, device=dev)
-    prob = torch.empty(rows, dtype=f32, device=dev)
-    check(_entry(at, stride, rows, logits.shape[1], vec(uniform, "uniform", f32), vec(temperature, "temperature", f32),
-                 vec(top_k, "top_k", i32), vec(top_p, "top_p", f32), vec(min_p, "min_p", f32), repetition_penalty,
-                 window.data_ptr() if window is not None else None, window_state.data_ptr() if window_state is not None else None,
-                 vec(token, "token", i32), prob.data_ptr(), vec(pos, "pos", i32), stream_of(logits)))
+        token = _new(rows, dtype=i32, device=logits.device)
+    prob = _new(rows, dtype=f32, device=logits.device)
+    rc = _entry(at, stride, rows, vocab, vector_arg(uniform, "uniform", rows, f32, index),
+                None if temperature is None else vector_arg(temperature, "temperature", rows, f32, index),
+                None if top_k is None else vector_arg(top_k, "top_k", rows, i32, index),
+                None if top_p is None else vector_arg(top_p, "top_p", rows, f32, index),
+                None if min_p is None else vector_arg(min_p, "min_p", rows, f32, index), repetition_penalty,
+                None if window is None else block_arg(window, "window", (rows, WINDOW), i32, index),
+                None if window_state is None else block_arg(window_state, "window_state", (rows, 2), i32, index),
+                vector_arg(token, "token", rows, i32, index), prob.data_ptr(),
+                None if pos is None else vector_arg(pos, "pos", rows, i32, index), _raw_stream(index))
+    if rc:
+        check(rc)
     return token, prob
