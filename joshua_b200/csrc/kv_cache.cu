@@ -41,7 +41,8 @@ struct HeadLanes {
     }
     // to position p; `mine`: HD floats of shared memory of these lanes
     __device__ __forceinline__ void turn(const RopeArgs& r, uint32_t p, float* mine) {
-        const float2* t = r.table + (uint64_t)p * (r.rot / 2);
+        const uint32_t half = r.rot / 2;
+        const float2* t = r.table + (uint64_t)p * half;
         if (!r.interleaved) {
             __syncwarp();
             store(mine);
@@ -50,23 +51,32 @@ struct HeadLanes {
 #pragma unroll
         for (uint32_t i = 0; i < QUADS; ++i) {
             const uint32_t d = dim(i);
-            if (r.interleaved) {
+            if (d >= r.rot) continue;
+            float (&v)[4] = x[i];
+            if (r.vectors) {  // rot a multiple of 8: four dimensions turn together, their table entries are whole vectors
+                if (r.interleaved) {
+                    const float4 cs = __ldg(reinterpret_cast<const float4*>(t + d / 2));
+                    const float y[4] = {v[0], v[1], v[2], v[3]};
+                    v[0] = rope_rotate(true, y[0], y[1], make_float2(cs.x, cs.y)), v[1] = rope_rotate(false, y[1], y[0], make_float2(cs.x, cs.y));
+                    v[2] = rope_rotate(true, y[2], y[3], make_float2(cs.z, cs.w)), v[3] = rope_rotate(false, y[3], y[2], make_float2(cs.z, cs.w));
+                } else {
+                    const bool first = d < half;
+                    const float4* cs = reinterpret_cast<const float4*>(t + (first ? d : d - half));
+                    const float4 c0 = __ldg(cs), c1 = __ldg(cs + 1), y = *reinterpret_cast<const float4*>(mine + (first ? d + half : d - half));
+                    // the second of a pair: a sin + b cos = b cos - a (-sin), rounded alike
+                    const float s = first ? 1.0f : -1.0f;
+                    v[0] = rope_rotate(true, v[0], y.x, make_float2(c0.x, c0.y * s)), v[1] = rope_rotate(true, v[1], y.y, make_float2(c0.z, c0.w * s));
+                    v[2] = rope_rotate(true, v[2], y.z, make_float2(c1.x, c1.y * s)), v[3] = rope_rotate(true, v[3], y.w, make_float2(c1.z, c1.w * s));
+                }
+            } else {
+                const float y[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    if (d + e < r.rot) {
-                        const float2 cs = __ldg(t + (d + e) / 2);
-                        const float a = x[i][e], b = x[i][e + 1];
-                        x[i][e] = rope_rotate(true, a, b, cs), x[i][e + 1] = rope_rotate(false, b, a, cs);
-                    }
-            } else if (d < r.rot) {
-                const uint32_t half = r.rot / 2;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (uint32_t e = 0; e < 4; ++e) {
                     const uint32_t at = d + e;
-                    if (at < r.rot) {
-                        const bool first = at < half;
-                        x[i][e] = rope_rotate(first, x[i][e], mine[first ? at + half : at - half], __ldg(t + (first ? at : at - half)));
-                    }
+                    const bool first = r.interleaved ? e % 2 == 0 : at < half;
+                    if (at >= r.rot) continue;
+                    const float other = r.interleaved ? y[e ^ 1] : mine[first ? at + half : at - half];
+                    v[e] = rope_rotate(first, y[e], other, __ldg(t + (r.interleaved ? at / 2 : first ? at : at - half)));
                 }
             }
         }
@@ -161,7 +171,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
 struct RowGroup {
     int64_t first;           // row of j = 0 (may be in front of the first row)
     uint32_t first_j, rows;  // live ones: j = first_j .. first_j + rows - 1
-    bool runs;               // they stand at consecutive positions of one sequence, within a group of 16 of a page
+    bool runs;               // they stand at consecutive positions of one sequence, within a group of 16 of a page,
+    int32_t p0;              // from p0 on
 
     __device__ __forceinline__ RowGroup(const int32_t* pos, uint32_t n, uint32_t block) {
         first = (int64_t)block * 16 - (pos[0] & 15);
@@ -174,7 +185,8 @@ struct RowGroup {
         const uint32_t j = threadIdx.x & 15;
         const bool live = has(j);
         const int32_t p = live ? pos[first + j] : 0, s = live ? seq ? seq[first + j] : (int32_t)(first + j) : 0;
-        const int32_t p0 = __shfl_sync(0xFFFFFFFFu, p, first_j & 15) - (int32_t)first_j, s0 = __shfl_sync(0xFFFFFFFFu, s, first_j & 15);
+        const int32_t s0 = __shfl_sync(0xFFFFFFFFu, s, first_j & 15);
+        p0 = __shfl_sync(0xFFFFFFFFu, p, first_j & 15) - (int32_t)first_j;
         runs = p0 >= 0 && p0 % 16 == 0 && __all_sync(0xFFFFFFFFu, !live || (p == p0 + (int32_t)j && s == s0));
     }
 };
@@ -213,7 +225,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 3 : 5) kv_append_rows_kernel(
             if (blockIdx.y == 0 && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
             continue;
         }
-        const uint32_t p = (uint32_t)a.pos[row];
+        const uint32_t p = run ? (uint32_t)g.p0 + j0 + i : (uint32_t)a.pos[row];
         if (turns) {
             const Lanes y = x[i];
             if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
@@ -227,7 +239,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 3 : 5) kv_append_rows_kernel(
     }
     if (run == nullptr) return;
     __syncthreads();
-    const uint32_t at = (uint32_t)a.pos[g.first] % KV_PAGE / 16 * RUN;
+    const uint32_t at = (uint32_t)g.p0 % KV_PAGE / 16 * RUN;
     for (uint32_t i = threadIdx.x; i < 2 * HPW * (RUN / 16); i += 256) {
         const uint32_t h = blockIdx.y * 2 * HPW + i / (RUN / 16), o = i % (RUN / 16) * 16;
         if (h < a.n_q || h >= heads) continue;

@@ -102,7 +102,7 @@ cudaError_t launch_rope(const RopeArgs& r, const float* x, uint64_t x_stride, co
                         uint32_t hd, bool inverse, float* out, uint64_t out_stride, int32_t* bad_pos, cudaStream_t s) {
     const float sign = inverse ? -1.0f : 1.0f;
     cudaError_t e;
-    if (hd % 8 == 0 && r.rot % 8 == 0 && hd <= 2048 && reinterpret_cast<uintptr_t>(r.table) % 16 == 0) {
+    if (hd % 8 == 0 && r.vectors) {
         // four heads a thread, fewer where the rows alone do not fill the GPU
         const uint32_t at_once = std::max(1u, 256 / (hd / 8)), threads = at_once * (hd / 8);
         const uint32_t most = (heads + at_once - 1) / at_once, few = (most + 3) / 4;

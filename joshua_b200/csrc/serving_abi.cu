@@ -21,7 +21,8 @@ int32_t check_rope(const char* who, const jq_rope* r, uint32_t head_dim, jq::Rop
     if (r->rot_dim == 0 || r->rot_dim % 2 || r->rot_dim > head_dim)
         return bad(who, "rot_dim " + std::to_string(r->rot_dim) + " must be even, above 0 and at most head_dim " + std::to_string(head_dim));
     if (r->interleaved != 0 && r->interleaved != 1) return bad(who, "interleaved must be 0 or 1");
-    *out = jq::RopeArgs{reinterpret_cast<const float2*>(r->table), r->n_pos, r->rot_dim, (uint32_t)r->interleaved};
+    *out = jq::RopeArgs{reinterpret_cast<const float2*>(r->table), r->n_pos, r->rot_dim, (uint32_t)r->interleaved,
+                        r->rot_dim % 8 == 0 && !unaligned(r->table)};
     return jq::OK;
 }
 
