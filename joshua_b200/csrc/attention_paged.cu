@@ -13,7 +13,7 @@
 // Up to four query rows stand as four pairs of columns (term, term): one product does both terms.
 #include <cooperative_groups.h>
 
-#include "kv_pages.cuh"
+#include "attention_paged.cuh"
 
 namespace jq {
 
@@ -21,11 +21,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {  // read once: not kept in L1
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -51,33 +46,10 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
     return t;
 }
-__device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-__device__ __forceinline__ __half2 bits_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
-// a and b, and what f16 leaves of them
-__device__ __forceinline__ void split2(float a, float b, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    *hi = half2_bits(h), *lo = half2_bits(__floats2half2_rn(a - f.x, b - f.y));
-}
 __device__ __forceinline__ uint32_t split1(float a) {  // (term, term)
     const float h = __half2float(__float2half_rn(a));
     return half2_bits(__floats2half2_rn(h, a - h));
 }
-// bytes b, b + 1 of w (codes + 128) as halves
-template <int B>
-__device__ __forceinline__ uint32_t codes8(uint32_t w) {
-    return half2_bits(__hsub2(bits_half2(__byte_perm(w, 0x64646464u, B == 0 ? 0x4140 : 0x4342)), __float2half2_rn(1152.0f)));
-}
-// four-bit codes + 8 at bits 4 N .. and 16 + 4 N .. as halves
-template <int N>
-__device__ __forceinline__ uint32_t codes4(uint32_t w) {
-    if constexpr (N >= 2) w >>= 8;
-    if constexpr (N % 2 == 0)  // 1024 + n
-        return half2_bits(__hsub2(bits_half2((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(1032.0f)));
-    // 1024 + 16 n
-    return half2_bits(__hfma2(bits_half2((w & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
-}
-
 template <uint32_t KIND_, uint32_t HD_>
 struct Step {
     static constexpr uint32_t KIND = KIND_, HD = HD_, NB = HD / 32, BITS = KIND == KV_F16 ? 16 : KIND == KV_Q8_0 ? 8 : 4;
@@ -466,25 +438,6 @@ struct Attend {
     }
 };
 
-constexpr uint32_t LEAD_MOST = 4;  // partial results of the leading pages
-
-struct PagedArgs {
-    KvPages c;
-    const float* q;
-    uint64_t q_stride;
-    const int32_t* len;
-    uint32_t n_q, group, split;  // query heads; heads a kv head; warps' worth of them (each up to ROWS rows)
-    float scale;
-    uint32_t common, done;  // leading pages named by the first sequence; leading pages that the other kernel takes
-    float* out;
-    uint64_t out_stride;
-    uint32_t* arrived;  // [batch * n_kv * split], zero between calls
-    float* part;        // [grid][2][ROWS (HD + 2)]
-    const float* lead;  // done: [lead_splits][n_kv][batch * group][HD], then their maxima, then their sums
-    uint32_t lead_splits;
-    int32_t* bad_pos;
-};
-
 // The pages of one sequence from page `first` on: ids of 32 at a time, a lane each, and a page's tile of a head requested from
 // memory (into L2) one page ahead.
 template <class T>
@@ -517,9 +470,6 @@ struct Pages {
         return t;
     }
 };
-
-// Weight of a piece with maximum m under the joint maximum; equal ones are 1 (infinities too)
-__device__ __forceinline__ float piece_weight(float m, float top) { return m == top ? 1.0f : ex2(m - top); }
 
 // A row's joined pieces: lane i has dimensions 4 i .. 4 i + 3 (HD 256: also those 128 behind; HD 64: lanes 0 .. 15).
 template <uint32_t HD>
@@ -920,10 +870,13 @@ constexpr uint32_t LEAD_WARPS = 8;
 constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }  // of a CTA, one a SM, by the registers that the kernel needs
 constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
 
+constexpr uint32_t LEAD_TILE_ROWS = 64;
+
 // How a call is cut up: the same for its scratch and its launches.
 struct PagedPlan {
     uint32_t group, split, rows, grid;       // of the kernel over the sequences' own pages
     uint32_t lead, sets, blocks, splits;     // of the leading pages' kernel: pages, row sets of a CTA, row blocks, page splits
+    bool tiles;                              // it is the one of attention_lead.cu
     uint32_t cluster;                        // splits that one cluster joins
     size_t part_at, lead_at, bytes;
 };
@@ -936,9 +889,10 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
     p.lead = batch > 1 ? shared : 0;
     if (p.lead) {
         const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
+        p.tiles = hd <= 128 && rows >= LEAD_TILE_ROWS;
         p.sets = 1;
         while (p.sets < LEAD_WARPS && p.sets < tiles) p.sets *= 2;
-        p.blocks = (tiles + p.sets - 1) / p.sets;
+        p.blocks = p.tiles ? (rows + 127) / 128 : (tiles + p.sets - 1) / p.sets;
         // one wave of one CTA a SM.  Clusters of eight leave SMs of the GPU's groups idle (16 of them took two waves), so eight
         // only where they are few
         const uint32_t rows_of = std::max(1u, p.blocks * n_kv), fit = std::max(1u, std::min(p.lead, (uint32_t)num_sms() / rows_of));
@@ -957,6 +911,7 @@ struct LaunchPaged {
     PagedArgs a;
     const PagedPlan& p;
     float* lead;
+    int* error_flag;
     cudaStream_t s;
 
     template <class T, bool PAIRS>
@@ -971,7 +926,10 @@ struct LaunchPaged {
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
         using T = Step<KIND, HD>;
-        if (p.lead) {
+        if (p.lead && p.tiles) {
+            cudaError_t e = launch_attention_lead_tiles(a, lead, p.splits, p.blocks, p.cluster, error_flag, s);
+            if (e != cudaSuccess) return e;
+        } else if (p.lead) {
             using At = Attend<T, lead_tiles(HD), false>;
             constexpr uint32_t PIECE = At::Q::ROWS * (HD + 2), AREA = PIECE > At::Q::WORDS ? PIECE : At::Q::WORDS;
             auto kern = attention_lead_kernel<T, lead_tiles(HD), LEAD_WARPS>;
@@ -1003,13 +961,14 @@ size_t attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv
 }
 
 cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* len, uint32_t n_q, float scale,
-                                   uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, cudaStream_t s) {
+                                   uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, int* error_flag,
+                                   cudaStream_t s) {
     const PagedPlan p = plan(c.n_seq, n_q, c.n_kv, c.hd, shared);
     uint8_t* mem = static_cast<uint8_t*>(scratch);
     float* lead = reinterpret_cast<float*>(mem + p.lead_at);
     const PagedArgs a{c, q, q_stride, len, n_q, p.group, p.split, scale, shared, p.lead, out, out_stride,
                       reinterpret_cast<uint32_t*>(mem), reinterpret_cast<float*>(mem + p.part_at), lead, p.lead ? p.splits / p.cluster : 0, bad_pos};
-    cudaError_t e = for_kind(c.kind, c.hd, LaunchPaged{a, p, lead, s});
+    cudaError_t e = for_kind(c.kind, c.hd, LaunchPaged{a, p, lead, error_flag, s});
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 

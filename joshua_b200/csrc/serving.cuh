@@ -40,7 +40,8 @@ cudaError_t launch_kv_read(const KvPages& c, const int32_t* pos, const int32_t* 
 constexpr uint32_t ATTENTION_MAX_BATCH = 4096;
 size_t attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t shared);
 cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* len, uint32_t n_q, float scale,
-                                   uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, cudaStream_t s);
+                                   uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, int* error_flag,
+                                   cudaStream_t s);
 
 struct SampleArgs {
     const float* logits;

@@ -175,7 +175,7 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
         return bad(who, "rows of n_q * head_dim floats must not overlap; 16-byte boundaries");
     if (scale == 0.0f) scale = 1.0f / std::sqrt((float)cache->head_dim);
     JQ_CUDA(jq::launch_attention_paged(c, q, q_stride, len, n_q, scale, shared_pages, out, out_stride, scratch, bad_pos_dev,
-                                       static_cast<cudaStream_t>(stream)));
+                                       jq_entry_status_flag(), static_cast<cudaStream_t>(stream)));
     return jq::OK;
 }
 

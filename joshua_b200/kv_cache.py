@@ -49,7 +49,7 @@ class PagedCache:
         if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.get_device() != self._index \
                 or table.dim() != 2 or not table.is_contiguous():
             raise JoshuaB200Error(_lib.E_INVALID, f"a page table is contiguous int32 [sequences, pages] on {self.device}")
-        return table.data_ptr(), table.size(0), table.size(1)
+        return table.data_ptr(), *table.shape
 
     def append(self, qkv: torch.Tensor, pos: torch.Tensor, table: torch.Tensor, n_q: int, seq: torch.Tensor | None = None,
                rope: Rope | None = None, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 0.0,
@@ -82,7 +82,7 @@ class PagedCache:
         rows = most = pos.size(0) if isinstance(pos, torch.Tensor) and pos.dim() else 0
         at = vector_arg(pos, "pos", rows, torch.int32, index)
         if out is None:
-            out = _new(2, n_kv, rows, hd, dtype=torch.float32, device=self.device).unbind(0)
+            out = (_new(n_kv, rows, hd, dtype=torch.float32, device=self.device), _new(n_kv, rows, hd, dtype=torch.float32, device=self.device))
             k_at, v_at = out[0].data_ptr(), out[1].data_ptr()
         else:
             most = out[0].size(1) if isinstance(out[0], torch.Tensor) and out[0].dim() == 3 else -1

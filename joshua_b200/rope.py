@@ -18,11 +18,6 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _new, _f32 = torch.empty, torch.float32
 
 
-def stream_of(index: int) -> int:
-    """The current stream of a device, as the C entries take it."""
-    return _raw_stream(index)
-
-
 def _refuse(t, name, dtype, index, shape):
     got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
     raise JoshuaB200Error(_lib.E_INVALID, f"{name} must be {shape} of {dtype} on cuda:{index}, not {got}")
@@ -37,17 +32,20 @@ def device_index(t, name, dtype) -> int:
 
 def rows_arg(t, name, width, index):
     """(pointer, floats between rows, rows) of a two-dimensional f32 tensor with contiguous rows."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not _f32 or t.get_device() != index or t.dim() != 2 or t.size(1) != width \
-            or (width != 1 and t.stride(1) != 1):
-        _refuse(t, name, _f32, index, f"[rows, {width}] with contiguous rows")
-    rows, stride = t.size(0), t.stride(0)
-    return t.data_ptr(), stride if rows > 1 else max(stride, width), rows
+    if isinstance(t, torch.Tensor) and t.dtype is _f32 and t.get_device() == index and t.dim() == 2:
+        rows, columns = t.shape
+        if columns == width:
+            if t.is_contiguous():
+                return t.data_ptr(), width, rows
+            if width == 1 or t.stride(1) == 1:
+                return t.data_ptr(), t.stride(0) if rows > 1 else width, rows
+    _refuse(t, name, _f32, index, f"[rows, {width}] with contiguous rows")
 
 
 def vector_arg(t, name, n, dtype, index):
     """Pointer of a contiguous vector."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or t.dim() != 1 or t.size(0) != n \
-            or (n > 1 and t.stride(0) != 1):
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or t.dim() != 1 or t.numel() != n \
+            or not t.is_contiguous():
         _refuse(t, name, dtype, index, f"a contiguous vector of {n}")
     return t.data_ptr()
 
@@ -84,7 +82,7 @@ def rope_table(theta: float, rot_dim: int, n_pos: int, device, scaling: str | No
     with torch.cuda.device(device):
         table = _new(max(n_pos, 0), max(rot_dim, 0) // 2, 2, dtype=_f32, device=device)
         check(_lib.lib().jq_rope_table_dev(ctypes.byref(cfg), factors, rot_dim, n_pos, table.data_ptr() or None,
-                                           stream_of(torch.cuda.current_device())))
+                                           _raw_stream(torch.cuda.current_device())))
     return table
 
 
