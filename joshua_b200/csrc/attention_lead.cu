@@ -24,6 +24,8 @@ namespace {
 
 constexpr uint32_t LQ = 128, LK = KV_PAGE;   // query rows and keys of a tile
 constexpr uint32_t L_SOFT = 8, L_CONV = 8;   // warps
+constexpr int UP = 6;                        // probabilities stand times 2^UP ..
+constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
 constexpr uint32_t L_THREADS = (L_SOFT + L_CONV + 4) * 32;  // whole warpgroups: they trade registers
 // Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 80
 // and the softmax threads (64 running outputs, 32 scores, 32 terms) 256 x 144: all of it.
@@ -32,7 +34,7 @@ static_assert(128 * L_REGS_ISSUE + L_CONV * 32 * L_REGS_CONV + L_SOFT * 32 * L_R
 
 // what the warps share beside the tiles
 struct LeadShared {
-    uint16_t ks[4][LK];       // inverse scales of key rows, by tile % 4: powers of two, so their upper halves
+    float ks[4];              // inverse scale of the keys, by tile % 4
     float vs[4][8];           // inverse scales of the values' blocks, by tile % 4
     float row[2][2][LQ];      // row maxima of the two halves
     float stat[2][LQ];        // maxima and sums of the rows
@@ -42,6 +44,40 @@ struct LeadShared {
     uint32_t tmem_slot;
     int abort_flag, lost;     // lost: a page id outside the cache
 };
+
+// two f32 operations in one
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ f32x2 pair(uint32_t a, uint32_t b) { return pair(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 both(f32x2 v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 template <uint32_t KIND, uint32_t HD>
 struct LeadTile {
@@ -155,7 +191,7 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
         constexpr uint32_t DN = HD / 2;  // dimensions of this thread
         float rf;                        // inverse scale of the query row, times log2(e) and the softmax scale
         auto pair_bar = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); };
-        float o[DN];
+        f32x2 o[DN / 2];
         {
             const bool live = at < rows;
             const float4* src = reinterpret_cast<const float4*>(
@@ -164,7 +200,7 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
 #pragma unroll
             for (uint32_t i = 0; i < DN / 4; ++i) {
                 const float4 v = live ? __ldg(src + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                o[4 * i] = v.x, o[4 * i + 1] = v.y, o[4 * i + 2] = v.z, o[4 * i + 3] = v.w;
+                o[2 * i] = pair(v.x, v.y), o[2 * i + 1] = pair(v.z, v.w);
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
             sh.row[1][half][row] = amax;
@@ -178,7 +214,10 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             for (uint32_t c = 0; c < DN / 32; ++c) {
                 uint32_t hi[16], lo[16];
 #pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) split2(o[32 * c + 2 * i] * sc, o[32 * c + 2 * i + 1] * sc, &hi[i], &lo[i]);
+                for (uint32_t i = 0; i < 16; ++i) {
+                    const float2 v = both(o[16 * c + i]);
+                    split2(v.x * sc, v.y * sc, &hi[i], &lo[i]);
+                }
                 tmem_st16(lanes + T::Q_HI + half * (DN / 2) + 16 * c, hi);
                 tmem_st16(lanes + T::Q_LO + half * (DN / 2) + 16 * c, lo);
             }
@@ -188,13 +227,14 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             if (lane == 0) mbar_arrive(&sh.s_free);  // the first scores wait for the query's terms
         }
 #pragma unroll
-        for (uint32_t i = 0; i < DN; ++i) o[i] = 0.0f;
-        float mx = -INFINITY, sum = 0.0f, alpha_prev = 0.0f;  // sum and outputs times 2^14, as the probabilities are
+        for (uint32_t i = 0; i < DN / 2; ++i) o[i] = 0;
+        float mx = -INFINITY, alpha_prev = 0.0f;
+        f32x2 sums = 0;  // sum and outputs times 2^UP, as the probabilities are
         // o = o * alpha + the tile's output
         auto add_tile = [&](uint32_t j, float alpha) {
-            if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {  // while the products run; the maxima settle after a few tiles
+            if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
 #pragma unroll
-                for (uint32_t i = 0; i < DN; ++i) o[i] *= alpha;
+                for (uint32_t i = 0; i < DN / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
             }
             if (!wait_all(&sh.o_full, j & 1)) return;
             tc_fence_after();
@@ -204,59 +244,58 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
                 tmem_ld32(lanes + T::O + half * DN + 32 * c, r);
                 const float f = KIND == KV_F16 ? 1.0f : sh.vs[j & 3][half * (DN / 32) + c];
 #pragma unroll
-                for (uint32_t i = 0; i < 32; ++i) o[32 * c + i] = KIND == KV_F16 ? o[32 * c + i] + __uint_as_float(r[i]) : fmaf(__uint_as_float(r[i]), f, o[32 * c + i]);
+                for (uint32_t i = 0; i < 16; ++i) {
+                    f32x2& x = o[16 * c + i];
+                    x = KIND == KV_F16 ? add2(x, pair(r[2 * i], r[2 * i + 1])) : fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
+                }
             }
         };
         uint32_t j = 0;  // tiles whose barrier this warp has come to
         while (j < n_tiles) {
-            float sc[32];
+            f32x2 sc[16];
             if (!wait_all(&sh.s_full, j & 1)) break;
             tc_fence_after();
             {
                 uint32_t r[32];
                 tmem_ld32(lanes + T::S0 + half * 32, r);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sc[i] = __uint_as_float(r[i]);
+                for (int i = 0; i < 16; ++i) sc[i] = pair(r[2 * i], r[2 * i + 1]);
                 if constexpr (T::HALVES == 2) {
                     tmem_ld32(lanes + T::S0 + 64 + half * 32, r);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sc[i] += __uint_as_float(r[i]);
+                    for (int i = 0; i < 16; ++i) sc[i] = add2(sc[i], pair(r[2 * i], r[2 * i + 1]));
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.s_free);
-            if constexpr (KIND != KV_F16) {
-                const uint4* ks = reinterpret_cast<const uint4*>(&sh.ks[j & 3][half * 32]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 f = ks[i];
-                    const uint32_t w[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        sc[8 * i + 2 * h] *= __uint_as_float(w[h] << 16);
-                        sc[8 * i + 2 * h + 1] *= __uint_as_float(w[h] & 0xFFFF0000u);
-                    }
-                }
-            }
+            const float f = KIND == KV_F16 ? rf : rf * sh.ks[j & 3];
             float cm = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) cm = fmaxf(cm, sc[i]);
+            for (int i = 0; i < 16; ++i) {
+                const float2 v = both(sc[i]);
+                cm = max3(cm, v.x, v.y);
+            }
             sh.row[j & 1][half][row] = cm;
             pair_bar();
-            const float nm = fmaxf(mx, fmaxf(cm, sh.row[j & 1][half ^ 1][row]) * rf);
-            const float alpha = ex2(mx - nm);  // 0 on the first tile (mx = -inf)
-            const float shift = 14.0f - nm;
-            float ps = 0.0f;
+            const float t = fmaxf(cm, sh.row[j & 1][half ^ 1][row]) * f;
+            float alpha = 1.0f;
+            if (t > mx + LAZY) alpha = ex2(mx - t), mx = t;  // 0 on the first tile (mx = -inf)
+            const f32x2 ff = pair(f, f), shift = pair((float)UP - mx, (float)UP - mx);
+            f32x2 ps = 0;
             uint32_t w0[16], w1[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float x = ex2(fmaf(sc[2 * i], rf, shift)), y = ex2(fmaf(sc[2 * i + 1], rf, shift));
-                ps += x + y;
-                split2(x, y, &w0[i], &w1[i]);
+                const float2 y = both(fma2(sc[i], ff, shift));
+                const float p = ex2(y.x), q = ex2(y.y);
+                const f32x2 both_p = pair(p, q);
+                ps = add2(ps, both_p);
+                const __half2 h = __floats2half2_rn(p, q);
+                const float2 g = __half22float2(h);
+                const float2 rest = both(fma2(pair(g.x, g.y), pair(-1.0f, -1.0f), both_p));
+                w0[i] = half2_bits(h), w1[i] = half2_bits(__floats2half2_rn(rest.x, rest.y));
             }
-            sum = sum * alpha + ps;
-            mx = nm;
+            sums = fma2(sums, pair(alpha, alpha), ps);
             if (j++ > 0) add_tile(j - 2, alpha_prev);  // its products have read the probabilities before these
             if (!ok) break;
             alpha_prev = alpha;
@@ -269,6 +308,8 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
         }
         for (; j < n_tiles; ++j) pair_bar();  // the other half of the rows may not have given up
         if (ok && n_tiles) add_tile(n_tiles - 1, alpha_prev);
+        const float2 two = both(sums);
+        const float sum = two.x + two.y;
         sh.row[n_tiles & 1][half][row] = sum;
         pair_bar();
         const float all = sum + sh.row[n_tiles & 1][half ^ 1][row];
@@ -276,10 +317,12 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
         // the rows in the tiles' place, then those of the cluster's CTAs (splits of the same rows) joined, a share of the rows a CTA
         float* stage = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (uint32_t i = 0; i < DN / 4; ++i)
+        for (uint32_t i = 0; i < DN / 4; ++i) {
+            const float2 u = both(o[2 * i]), v = both(o[2 * i + 1]);
             *reinterpret_cast<float4*>(stage + row * T::PITCH + half * DN + 4 * i) =
-                make_float4(o[4 * i] * power(-14), o[4 * i + 1] * power(-14), o[4 * i + 2] * power(-14), o[4 * i + 3] * power(-14));
-        if (half == 0) sh.stat[0][row] = mx, sh.stat[1][row] = bad ? NAN : all * power(-14);
+                make_float4(u.x * power(-UP), u.y * power(-UP), v.x * power(-UP), v.y * power(-UP));
+        }
+        if (half == 0) sh.stat[0][row] = mx, sh.stat[1][row] = bad ? NAN : all * power(-UP);
         __syncwarp();
         cluster_sync_all();
         uint32_t ctas, rank;
@@ -339,22 +382,25 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
                 }
             } else {
                 constexpr uint32_t BLOCKS = KIND == KV_Q8_0 ? 1 : 2;  // of a 16-byte vector
+                uint32_t top = 0x04000400u;  // the page's largest scale
+#pragma unroll
+                for (uint32_t i = 0; i < NB / 2; ++i) {  // 8 bytes a position and block pair
+                    const uint2 v = *reinterpret_cast<const uint2*>(raw + CODES + (i * 32 + lane) * 8);
+                    top = __vmaxu2(top, __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu));
+                }
+                const int e = (int)(__reduce_max_sync(0xFFFFFFFFu, max(top >> 16, top & 0xFFFFu)) >> 10);
+                const float f = power(TOP - e);
+                if (cw == 0 && lane == 0) sh.ks[j & 3] = power(e - TOP);
 #pragma unroll 2
                 for (uint32_t i = cw; i < 4 * NB / BLOCKS; i += L_CONV) {
                     const uint32_t g = i / (NB / BLOCKS), b0 = i % (NB / BLOCKS) * BLOCKS;
                     const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
                     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                    // scales of rows r and r + 8 of the group, by block; their largest exponents
-                    const uint8_t* scales = raw + CODES + (g / 2 * 8 + r) * NB * 8 + g % 2 * 4;
-                    uint32_t top = 0x04000400u;
-#pragma unroll
-                    for (uint32_t b = 0; b < NB; ++b) top = __vmaxu2(top, *reinterpret_cast<const uint32_t*>(scales + b * 8) & 0x7FFF7FFFu);
-                    const int e0 = (int)(top >> 10 & 31), e1 = (int)(top >> 26);
-                    const float f0 = power(TOP - e0), f1 = power(TOP - e1);
+                    const uint8_t* scales = raw + CODES + (g / 2 * 8 + r) * NB * 8 + g % 2 * 4;  // of rows r and r + 8, by block
 #pragma unroll
                     for (uint32_t o = 0; o < BLOCKS; ++o) {
                         const float2 s = __half22float2(bits_half2(*reinterpret_cast<const uint32_t*>(scales + (b0 + o) * 8)));
-                        const __half2 s0 = __float2half2_rn(s.x * f0), s1 = __float2half2_rn(s.y * f1);
+                        const __half2 s0 = __float2half2_rn(s.x * f), s1 = __float2half2_rn(s.y * f);
                         uint32_t hi[2][4], lo[2][4];
                         if constexpr (KIND == KV_Q8_0) {
                             scaled_terms(codes8<0>(w[0]), s0, &hi[0][0], &lo[0][0]), scaled_terms(codes8<2>(w[0]), s0, &hi[0][1], &lo[0][1]);
@@ -372,10 +418,6 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
                         const uint32_t at0 = key_at(st, 16 * g + r, b0 + o), at1 = key_at(st, 16 * g + r + 8, b0 + o);
                         sts_v4(at0, hi[0]), sts_v4(at0 + K_LO, lo[0]);
                         sts_v4(at1, hi[1]), sts_v4(at1 + K_LO, lo[1]);
-                    }
-                    if (b0 == 0 && c == 0) {
-                        sh.ks[j & 3][16 * g + r] = (uint16_t)(__float_as_uint(power(e0 - TOP)) >> 16);
-                        sh.ks[j & 3][16 * g + r + 8] = (uint16_t)(__float_as_uint(power(e1 - TOP)) >> 16);
                     }
                 }
             }

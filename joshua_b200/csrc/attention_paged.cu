@@ -870,7 +870,7 @@ constexpr uint32_t LEAD_WARPS = 8;
 constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }  // of a CTA, one a SM, by the registers that the kernel needs
 constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
 
-constexpr uint32_t LEAD_TILE_ROWS = 64;
+constexpr uint32_t LEAD_TILE_ROWS = 32;
 
 // How a call is cut up: the same for its scratch and its launches.
 struct PagedPlan {
