@@ -330,29 +330,44 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
         asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
         const uint64_t every = (uint64_t)(gridDim.x / ctas) * a.c.n_kv * rows, base = ((uint64_t)(split / ctas) * a.c.n_kv + kvh) * rows;
         const uint32_t stage_at = smem_u32(stage), stat_at = smem_u32(&sh.stat[0][0]), share = LQ / ctas;
-        auto remote = [](uint32_t addr, uint32_t r) {
-            uint32_t x;
-            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(addr), "r"(r));
-            return x;
-        };
+        // the weight of every CTA's part of a row, a thread each, first those of the row's maximum
+        constexpr uint32_t MOST = 8;  // CTAs
+        float* weight = &sh.row[0][0][0];  // [share][ctas]
+        const uint32_t r = rank * share + tid / 2 % share;  // two threads a row, half of the CTAs each
+        if (tid < 2 * share) {
+            float m[MOST / 2], l[MOST / 2], top = -INFINITY, den = 0.0f;
+#pragma unroll
+            for (uint32_t k = 0; k < MOST / 2; ++k) {
+                const uint32_t c = 2 * k + tid % 2;
+                m[k] = c < ctas ? ld_cluster_f32(stat_at + r * 4, c) : -INFINITY, l[k] = c < ctas ? ld_cluster_f32(stat_at + (LQ + r) * 4, c) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < MOST / 2; ++k) top = fmaxf(top, m[k]);
+            top = fmaxf(top, __shfl_xor_sync(__activemask(), top, 1));
+#pragma unroll
+            for (uint32_t k = 0; k < MOST / 2; ++k) {
+                const uint32_t c = 2 * k + tid % 2;
+                const float f = piece_weight(m[k], top);
+                if (c < ctas) weight[tid / 2 * ctas + c] = f, den = fmaf(f, l[k], den);
+            }
+            den += __shfl_xor_sync(__activemask(), den, 1);
+            if (tid % 2 == 0 && row0 + r < rows) lead[every * HD + base + row0 + r] = top, lead[every * HD + every + base + row0 + r] = den;
+        }
+        asm volatile("bar.sync 5, %0;" ::"n"(L_SOFT * 32) : "memory");
+#pragma unroll 2
         for (uint32_t i = tid; i < share * (HD / 4); i += L_SOFT * 32) {
-            const uint32_t r = rank * share + i / (HD / 4), d = i % (HD / 4) * 4;
-            if (row0 + r >= rows) continue;
-            float top = -INFINITY, den = 0.0f;
-            for (uint32_t c = 0; c < ctas; ++c) top = fmaxf(top, ld_cluster_f32(stat_at + r * 4, c));
+            const uint32_t k = i / (HD / 4), d = i % (HD / 4) * 4, at_row = rank * share + k;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
             for (uint32_t c = 0; c < ctas; ++c) {
-                const float f = piece_weight(ld_cluster_f32(stat_at + r * 4, c), top);
+                uint32_t from;
                 float4 y;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                             : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
-                             : "r"(remote(stage_at + (r * T::PITCH + d) * 4, c)));
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(stage_at + (at_row * T::PITCH + d) * 4), "r"(c));
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(from));
+                const float f = weight[k * ctas + c];
                 x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
-                den = fmaf(f, ld_cluster_f32(stat_at + (LQ + r) * 4, c), den);
             }
-            *reinterpret_cast<float4*>(lead + (base + row0 + r) * HD + d) = x;
-            if (d == 0) lead[every * HD + base + row0 + r] = top, lead[every * HD + every + base + row0 + r] = den;
+            if (row0 + at_row < rows) *reinterpret_cast<float4*>(lead + (base + row0 + at_row) * HD + d) = x;
         }
     } else if (warp < L_SOFT + L_CONV) {
         // ── converters ──
