@@ -81,8 +81,7 @@ class LlamaDecoder:
             ly = dict(
                 attn_norm=nv(f"l{l}.attn_norm", h), ffn_norm=nv(f"l{l}.ffn_norm", h),
                 wqkv=q(f"l{l}.wqkv", cfg.qkv_rows, h, s0), wo=q(f"l{l}.wo", h, cfg.q_heads * cfg.head_dim, s0 + 1),
-                k=torch.zeros(batch, cfg.kv_heads, max_ctx, cfg.head_dim, **f32),
-                v=torch.zeros(batch, cfg.kv_heads, max_ctx, cfg.head_dim, **f32))
+                **self._layer_cache())
             if self._has_dense_ffn():
                 ly.update(w_gate=q(f"l{l}.w_gate", cfg.ffn, h, s0 + 2), w_up=q(f"l{l}.w_up", cfg.ffn, h, s0 + 3),
                           w_down=q(f"l{l}.w_down", h, cfg.ffn, s0 + 4))
@@ -111,13 +110,23 @@ class LlamaDecoder:
         self.act = torch.empty(B, cfg.ffn, **f32)
         self.d = torch.empty(B, h, **f32)
         self.logits = torch.empty(B, cfg.vocab, **f32)
-        att_bytes = _lib.lib().jq_attention_scratch_bytes(B, cfg.q_heads, cfg.head_dim, max_ctx)
-        self.att_scratch = torch.empty(att_bytes // 4 + 1, **f32)
-        fused_bytes = _lib.lib().jq_attention_fused_scratch_bytes(B, cfg.q_heads, cfg.kv_heads, cfg.head_dim, max_ctx)
-        self.att_fused_scratch = torch.zeros(fused_bytes // 4 + 1, **f32)   # holds arrival counters: starts at zero
+        self._attention_scratch()
         self.argmax_scratch = torch.empty(_lib.lib().jq_argmax_scratch_bytes(B) // 4 + 1, **f32)
         self.launches_per_step = 5 * cfg.layers + 4   # one sequence; larger batches take other routes
         self.matmuls_per_step = 4 * cfg.layers + 1
+
+    def _layer_cache(self) -> dict:
+        """A layer's keys and values: dense f32 [batch, n_kv, max_ctx, head_dim]."""
+        torch, c = self.torch, self.cfg
+        shape = (self.batch, c.kv_heads, self.max_ctx, c.head_dim)
+        return dict(k=torch.zeros(shape, dtype=torch.float32, device=self.dev), v=torch.zeros(shape, dtype=torch.float32, device=self.dev))
+
+    def _attention_scratch(self) -> None:
+        torch, c, B, f32 = self.torch, self.cfg, self.batch, dict(dtype=self.torch.float32, device=self.dev)
+        att_bytes = _lib.lib().jq_attention_scratch_bytes(B, c.q_heads, c.head_dim, self.max_ctx)
+        self.att_scratch = torch.empty(att_bytes // 4 + 1, **f32)
+        fused_bytes = _lib.lib().jq_attention_fused_scratch_bytes(B, c.q_heads, c.kv_heads, c.head_dim, self.max_ctx)
+        self.att_fused_scratch = torch.zeros(fused_bytes // 4 + 1, **f32)   # holds arrival counters: starts at zero
 
     # ── one token ───────────────────────────────────────────────────────
     def step(self, stream=None) -> None:
@@ -134,18 +143,23 @@ class LlamaDecoder:
         for ly in self.layers:
             check(L.jq_matmul_norm_dev(ly["wqkv"]._h, B, h, c.qkv_rows, P(self.x), P(ly["attn_norm"]), c.eps, None,
                                        P(self.qkv), s))
-            check(L.jq_attention_fused_qknorm_dev(P(self.qkv), P(self.pos), B, c.q_heads, c.kv_heads, c.head_dim,
-                                                  self.max_ctx, c.rope_theta,
-                                                  P(ly["q_norm"]) if self.qk_norm else None,
-                                                  P(ly["k_norm"]) if self.qk_norm else None, c.eps, P(ly["k"]),
-                                                  P(ly["v"]), P(self.attn), P(self.att_fused_scratch),
-                                                  P(self.bad_pos), s))
+            self._attend(ly, s)
             check(L.jq_matmul_norm_dev(ly["wo"]._h, B, c.q_heads * c.head_dim, h, P(self.attn), None, 0.0, P(self.x),
                                        P(self.x), s))
             self._ffn(ly, s)
         check(L.jq_matmul_norm_dev(self.output._h, B, h, c.vocab, P(self.x), P(self.out_norm), c.eps, None,
                                    P(self.logits), s))
         self._sample(s)
+
+    def _attend(self, ly, s) -> None:
+        """self.attn = attention of self.qkv's new rows, which go to the layer's cache."""
+        c, P = self.cfg, lambda t: t.data_ptr()
+        check(_lib.lib().jq_attention_fused_qknorm_dev(P(self.qkv), P(self.pos), self.batch, c.q_heads, c.kv_heads, c.head_dim,
+                                                       self.max_ctx, c.rope_theta,
+                                                       P(ly["q_norm"]) if self.qk_norm else None,
+                                                       P(ly["k_norm"]) if self.qk_norm else None, c.eps, P(ly["k"]),
+                                                       P(ly["v"]), P(self.attn), P(self.att_fused_scratch),
+                                                       P(self.bad_pos), s))
 
     def _has_dense_ffn(self) -> bool:
         return True

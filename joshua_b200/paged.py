@@ -1,0 +1,198 @@
+"""The decoders of this package with their keys and values in pages of few bits, for batches of long sequences.
+
+Sequences take pages from one pool as they grow and give them back when they end; sequences that begin with the same prompt hold
+its full pages in common, and a step reads and multiplies those once for all of them (`share_prompt`).  Rotary positions come
+from a table (any scaling of `rope.rope_table`), the next tokens from `sampling.sample` where a sampling rule is set.
+
+    dec = PagedLlamaDecoder(cfg, device, batch=32, max_ctx=8192, kv_type="q8_0")
+    dec.share_prompt(prompt_ids)                 # or dec.prefill(ids, sequence=i) for each
+    dec.sampling = dict(temperature=..., top_p=...)
+    dec.uniform.uniform_(); dec.step()           # token by token
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import JoshuaB200Error, check
+from .kv_cache import PAGE, PagedCache
+from .llama import LlamaDecoder
+from .moe_decoder import MoeDecoder
+from .rope import Rope, rope_table
+from .sampling import sample
+
+
+class _Paged:
+    def __init__(self, cfg, device, batch: int = 1, max_ctx: int = 640, kv_type: str = "q8_0", n_pages: int | None = None,
+                 rope: Rope | None = None, **more):
+        """`n_pages`: of the pool (default: enough for every sequence to reach max_ctx); `rope`: a table of max_ctx positions
+        (default: the model's theta, unscaled, half layout)."""
+        self.kv_type, self.pages_per_seq = kv_type, -(-max_ctx // PAGE)
+        self.n_pages = batch * self.pages_per_seq if n_pages is None else n_pages
+        super().__init__(cfg, device, batch=batch, max_ctx=max_ctx, **more)
+        self.rope = rope or Rope(rope_table(cfg.rope_theta, cfg.head_dim, max_ctx, self.dev))
+        self.table = torch.zeros(batch, self.pages_per_seq, dtype=torch.int32, device=self.dev)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)
+        self.free = list(range(self.n_pages))[::-1]
+        self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
+        self.held = [0] * batch                   # positions each holds
+        self.shared_pages = 0                     # leading pages that all sequences have in common
+        self.sampling: dict | None = None         # temperature, top_k, top_p, min_p: vectors of `batch`
+        self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)   # numbers in [0, 1) for the next draw
+
+    def _layer_cache(self) -> dict:
+        return dict(cache=PagedCache(self.kv_type, self.cfg.kv_heads, self.cfg.head_dim, n_pages=self.n_pages, device=self.dev))
+
+    def _attention_scratch(self) -> None:
+        """The caches keep their own."""
+
+    # ── pages ───────────────────────────────────────────────────────────
+    def reserve(self, sequence: int, positions: int) -> None:
+        """Pages for the first `positions` positions of a sequence.  A step takes them itself as they fill; reserve them before
+        capturing one in a graph."""
+        if positions > self.max_ctx:
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{positions} positions in a decoder of {self.max_ctx}")
+        mine, want = self.owned[sequence], -(-positions // PAGE)
+        if want <= len(mine):
+            return
+        if want - len(mine) > len(self.free):
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{want - len(mine)} pages wanted, {len(self.free)} of {self.n_pages} are free")
+        new = [self.free.pop() for _ in range(want - len(mine))]
+        self.table[sequence, len(mine):want] = torch.tensor(new, dtype=torch.int32, device=self.dev)
+        mine.extend(new)
+
+    def release(self, sequence: int) -> None:
+        """Ends a sequence: its pages go back (shared ones when the last sequence ends); the next prompt begins at position 0."""
+        for page in self.owned[sequence]:
+            if not any(page in other for i, other in enumerate(self.owned) if i != sequence):
+                self.free.append(page)
+        self.owned[sequence], self.held[sequence] = [], 0
+        self.pos[sequence] = 0
+        self.shared_pages = 0   # not all sequences have them any more
+
+    def reset(self, token: int = 42) -> None:
+        for i in range(self.batch):
+            self.release(i)
+        super().reset(token)
+
+    # ── a prompt ────────────────────────────────────────────────────────
+    def prefill(self, token_ids, sequence: int = 0) -> None:
+        """The prompt's tokens of one sequence in one pass, from where it stands; then self.logits[sequence], its sampled next
+        token (self.token) and position, as `step` leaves them."""
+        self._prompt(token_ids, sequence)
+        self._sample_rows(slice(sequence, sequence + 1))
+
+    def share_prompt(self, token_ids) -> None:
+        """Begins all sequences with one prompt, read once: its full pages are common to all, what is left of it (less than a
+        page) is copied.  Every sequence samples its own next token."""
+        if any(self.held):
+            raise JoshuaB200Error(_lib.E_INVALID, "sequences are under way: reset() first")
+        n = len(token_ids)
+        self._prompt(token_ids, 0)
+        common, rest = self.owned[0][:n // PAGE], self.owned[0][n // PAGE:]
+        for i in range(1, self.batch):
+            self.owned[i] = list(common)
+            self.table[i, :len(common)] = self.table[0, :len(common)]
+            self.reserve(i, n)
+            if n % PAGE:
+                for ly in self.layers:
+                    ly["cache"].pages[self.owned[i][-1]] = ly["cache"].pages[rest[0]]
+            self.held[i] = n
+        self.shared_pages = len(common)
+        self.pos.fill_(n - 1)
+        self.logits.copy_(self.logits[0:1].expand(self.batch, -1).clone())
+        self._sample_rows(slice(0, self.batch))
+
+    def _prompt(self, token_ids, i) -> None:
+        """Logits of the prompt's last token into self.logits[i]; self.pos[i] at that token."""
+        L, c, P = _lib.lib(), self.cfg, lambda t: t.data_ptr()
+        if not hasattr(self, "_layer_index"):   # the routed experts' decoder finds its layers by it
+            self._layer_index = {id(ly): k for k, ly in enumerate(self.layers)}
+        if c.head_dim not in (64, 128):
+            raise JoshuaB200Error(_lib.E_INVALID, "prompts need heads of 64 or 128")
+        s = torch.cuda.current_stream(self.dev).cuda_stream
+        ids = torch.as_tensor(token_ids, dtype=torch.int32).to(self.dev)
+        S, h, start, f32 = int(ids.numel()), c.hidden, self.held[i], dict(dtype=torch.float32, device=self.dev)
+        if S == 0:
+            raise JoshuaB200Error(_lib.E_INVALID, "an empty prompt")
+        self.reserve(i, start + S)
+        end = start + S
+        pos = torch.arange(end, dtype=torch.int32, device=self.dev)
+        seq = torch.full((end,), i, dtype=torch.int32, device=self.dev)
+        first = pos[start:start + 1]
+        x, qkv, att = torch.empty(S, h, **f32), torch.empty(S, c.qkv_rows, **f32), torch.empty(S, c.q_heads * c.head_dim, **f32)
+        dense = torch.empty(2, c.kv_heads, end, c.head_dim, **f32)
+        check(L.jq_embedding_dev(self.embed._h, P(ids), S, c.vocab, h, P(x), P(self.bad), s))
+        for ly in self.layers:
+            check(L.jq_matmul_norm_dev(ly["wqkv"]._h, S, h, c.qkv_rows, P(x), P(ly["attn_norm"]), c.eps, None, P(qkv), s))
+            cache = ly["cache"]
+            q = cache.append(qkv, pos[start:], self.table, n_q=c.q_heads, seq=seq[start:], rope=self.rope,
+                             q_norm=ly["q_norm"] if self.qk_norm else None, k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps)
+            cache.read(pos, self.table, seq=seq, out=(dense[0], dense[1]))   # what the cache holds is what later tokens will see
+            check(L.jq_attention_prefill_dev(P(q), P(dense[0]), P(dense[1]), P(first), S, c.q_heads, c.kv_heads, c.head_dim, end, P(att),
+                                             P(self.bad_pos), s))
+            check(L.jq_matmul_norm_dev(ly["wo"]._h, S, c.q_heads * c.head_dim, h, P(att), None, 0.0, P(x), P(x), s))
+            self._ffn_prefill(ly, x, S, s)
+        last = x[S - 1:S].clone()
+        check(L.jq_matmul_norm_dev(self.output._h, 1, h, c.vocab, P(last), P(self.out_norm), c.eps, None, P(self.logits[i]), s))
+        self.held[i] = end
+        self.pos[i] = end - 1
+
+    # ── a token of every sequence ───────────────────────────────────────
+    def step(self, stream=None) -> None:
+        """One token per sequence, as the dense decoder's step, on the current stream (`stream` is that one's handle or None)."""
+        now = torch.cuda.current_stream(self.dev).cuda_stream
+        if stream is not None and stream != now:
+            raise JoshuaB200Error(_lib.E_INVALID, "a paged decoder's step runs on the current stream")
+        for i in range(self.batch):
+            self.reserve(i, self.held[i] + 1)
+            self.held[i] += 1
+        torch.add(self.pos, 1, out=self.lens)
+        super().step(now)
+
+    def _attend(self, ly, s) -> None:
+        c, cache = self.cfg, ly["cache"]
+        cache.append(self.qkv, self.pos, self.table, n_q=c.q_heads, rope=self.rope, q_norm=ly["q_norm"] if self.qk_norm else None,
+                     k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps, out=self.q)
+        cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, shared_pages=self.shared_pages, out=self.attn)
+
+    def _sample(self, s) -> None:
+        self._sample_rows(slice(0, self.batch))
+
+    def _sample_rows(self, rows) -> None:
+        if self.sampling is None and rows.stop - rows.start == self.batch:
+            super()._sample(torch.cuda.current_stream(self.dev).cuda_stream)
+            return
+        rule = self.sampling or dict(temperature=torch.zeros(self.batch, dtype=torch.float32, device=self.dev))
+        penalised = self.repetition_penalty != 1.0
+        sample(self.logits[rows], self.uniform[rows], **{k: v[rows] for k, v in rule.items()}, repetition_penalty=self.repetition_penalty,
+               window=self.window[rows] if penalised else None, window_state=self.window_state[rows] if penalised else None,
+               pos=self.pos[rows], token=self.token[rows])
+
+    def forward_host(self, token_ids, out_logits=None):
+        if getattr(self, "_host", None) is None:
+            for i in range(self.batch):
+                self.reserve(i, self.max_ctx)
+        held = list(self.held)
+        logits = super().forward_host(token_ids, out_logits)
+        self.held = [n + 1 for n in held]   # the graph's capture walked through step() too
+        return logits
+
+    def check_flags(self) -> None:
+        super().check_flags()
+        for ly in self.layers:
+            ly["cache"].check_flags()
+
+    def cache_bytes(self) -> int:
+        return sum(ly["cache"].pages.numel() for ly in self.layers)
+
+    def step_unfused(self, stream=None) -> None:
+        raise JoshuaB200Error(_lib.E_INVALID, "the separate kernels of the dense cache do not read pages")
+
+
+class PagedLlamaDecoder(_Paged, LlamaDecoder):
+    """`LlamaDecoder` over a paged cache."""
+
+
+class PagedMoeDecoder(_Paged, MoeDecoder):
+    """`MoeDecoder` over a paged cache."""
