@@ -5,8 +5,10 @@
 //   scores   S^T = K Q^T as m16n8k16 products, keys (codes as they are: whole numbers or halves, exact in f16) the 16-row
 //            operand, query rows the 8 columns, in two f16 terms under a power of two of their row (22 bits).  The accumulator
 //            of a block of 32 dimensions is scaled by the block's factor and added in f32.
-//            Codes of 8 and 4 bits stand in the low bits of a half as they are: a subnormal number, the code plus its bias times
-//            2^-24, which the products take exactly.  The bias times the sum of the query's terms is where their sums begin.
+//            Codes of 8 and 4 bits stand in the low bits of a half as they are, 4-bit ones in bits 4 .. 7: a subnormal number, the
+//            code plus its bias times 2^-24 (2^-20), which the products take exactly.  The bias times the sum of the query's terms
+//            is where their sums begin.  (The products are aligned by their exponents before they are added, and a subnormal's
+//            is that of 2^-14: with 4-bit codes in bits 0 .. 3 the result was off by 2.9e-6 of itself, so by 5e-7.)
 //   output   O^T = V^T P^T, values the 16-row operand; probabilities times the value's scale of the block, under a power of two
 //            of the step's largest scale, in two f16 terms (22 bits below the largest).  Accumulators hold a step, not the
 //            sequence: the tensor core adds with truncation, the running output is added round-to-nearest.
@@ -97,8 +99,8 @@ struct Rows {
         const float2 f = __half22float2(bits_half2(s[b][i / 2]));
         return i % 2 ? f.y : f.x;
     }
-    // A operand of 16 keys (group a) and 16 dimensions (half h of block b); codes with their bias, times 2^-24 (Q4_0: dimensions
-    // 2 and 3 of four times 2^-20)
+    // A operand of 16 keys (group a) and 16 dimensions (half h of block b); codes with their bias, times 2^-KEY_SHIFT
+    static constexpr int KEY_SHIFT = T::KIND == KV_Q8_0 ? 24 : T::KIND == KV_Q4_0 ? 20 : 0;
     __device__ __forceinline__ void key(uint32_t a, uint32_t b, uint32_t h, uint32_t (&r)[4]) const {
         if constexpr (T::KIND == KV_F16) {
             const uint32_t v = (a * T::NB + b) * 2 + h;
@@ -108,8 +110,8 @@ struct Rows {
             r[0] = __byte_perm(x, 0, 0x4140), r[1] = __byte_perm(y, 0, 0x4140);
             r[2] = __byte_perm(x, 0, 0x4342), r[3] = __byte_perm(y, 0, 0x4342);
         } else {
-            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + h), y = x >> 8;
-            r[0] = x & 0x000F000Fu, r[1] = y & 0x000F000Fu, r[2] = x & 0x00F000F0u, r[3] = y & 0x00F000F0u;
+            const uint32_t x = word(a * (T::NB / 2) + b / 2, b % 2 * 2 + h);
+            r[0] = x << 4 & 0x00F000F0u, r[1] = x >> 4 & 0x00F000F0u, r[2] = x & 0x00F000F0u, r[3] = x >> 8 & 0x00F000F0u;
         }
     }
     // A operand of 16 dimensions (tile m of block b) and 16 positions (group a)
@@ -185,33 +187,31 @@ struct Attend {
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
             const float up = __uint_as_float(bits << 23);
             const float down = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * scale *
-                               (T::KIND == KV_F16 ? 1.44269504f : 1.44269504f * 16777216.0f);
+                               (1.44269504f * (float)(1 << Rows<T>::KEY_SHIFT));
 #pragma unroll
             for (uint32_t b = 0; b < NB; ++b) {
                 float sum = 0.0f;  // of the terms of this lane's column
 #pragma unroll
                 for (uint32_t h = 0; h < 2; ++h) {
-                    // Q4_0: the codes of dimensions 2 and 3 come times 16
-                    constexpr float OTHER = T::KIND == KV_Q4_0 ? 0.0625f : 1.0f;
                     uint32_t hi[2], lo[2];
                     split2(x[b][4 * h] * up, x[b][4 * h + 1] * up, &hi[0], &lo[0]);
-                    split2(x[b][4 * h + 2] * (up * OTHER), x[b][4 * h + 3] * (up * OTHER), &hi[1], &lo[1]);
+                    split2(x[b][4 * h + 2] * up, x[b][4 * h + 3] * up, &hi[1], &lo[1]);
                     auto of = [](uint32_t w) {
                         const float2 f = __half22float2(bits_half2(w));
                         return f.x + f.y;
                     };
                     if constexpr (PAIRS) {
                         qf[2 * b + h][0] = n % 2 ? lo[0] : hi[0], qf[2 * b + h][1] = n % 2 ? lo[1] : hi[1];
-                        sum += of(qf[2 * b + h][0]) + of(qf[2 * b + h][1]) * (1.0f / OTHER);
+                        sum += of(qf[2 * b + h][0]) + of(qf[2 * b + h][1]);
                     } else {
                         uint2* to = reinterpret_cast<uint2*>(shared) + ((t * 2 * NB + 2 * b + h) * 2) * 32 + lane;
                         to[0] = make_uint2(hi[0], hi[1]), to[32] = make_uint2(lo[0], lo[1]);
-                        sum += of(hi[0]) + of(lo[0]) + (of(hi[1]) + of(lo[1])) * (1.0f / OTHER);
+                        sum += of(hi[0]) + of(lo[0]) + of(hi[1]) + of(lo[1]);
                     }
                 }
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-                sum *= T::KIND == KV_F16 ? 0.0f : T::KIND == KV_Q8_0 ? -128.0f / 16777216.0f : -8.0f / 16777216.0f;
+                sum *= (T::KIND == KV_F16 ? 0.0f : T::KIND == KV_Q8_0 ? -128.0f : -8.0f) / (float)(1 << Rows<T>::KEY_SHIFT);
                 const float b0 = __shfl_sync(0xFFFFFFFFu, sum, 8 * c), b1 = __shfl_sync(0xFFFFFFFFu, sum, 8 * c + 4);
                 if (T::KIND != KV_F16 && n == 0)
                     *reinterpret_cast<float2*>(shared + Q::OPERAND + ((t * NB + b) * 4 + c) * 2) = make_float2(b0, b1);
