@@ -32,6 +32,10 @@ __device__ __forceinline__ uint32_t logit_key(float l) {
     return l > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
 
+struct Token {
+    u64 weight;
+    uint32_t id;
+};
 struct SampleShared {
     union {
         struct {
@@ -39,11 +43,14 @@ struct SampleShared {
         } bins;
         u64 few[SM_FEW];  // places of a few tokens; bins.high then is where a bin's tokens go in their order (CTA 0)
     };
-    float best, least;
+    // written by every CTA of the cluster, into all: a write in front of a barrier costs less than a read behind it
+    float best[SM_MOST_CTAS], least[SM_MOST_CTAS];
+    u64 part[SM_MOST_CTAS];
+    uint32_t few_of[SM_MOST_CTAS];
     float red[2][SM_WARPS];
     uint32_t n_few, bin, number;
     static_assert(SM_FEW * 8 <= SM_BINS * 8, "bins.high lies behind the few");
-    u64 part, border, before, sum, scan[SM_WARPS], scan2[SM_WARPS];
+    u64 border, before, sum, scan[SM_WARPS], scan2[SM_WARPS];
     int32_t window[SM_WINDOW];
 };
 
@@ -149,15 +156,15 @@ struct Row {
         cluster.sync();  // what was there has been read
         if (tid == 0) sh.number = (uint32_t)c64, sh.sum = w64;
         cluster.sync();
-        *number = 0, *sum = 0;
-        for (uint32_t r = 0; r < ctas; ++r) *number += at(sh.number, r), *sum += at(sh.sum, r);
+        *number = warp_sum(lane < ctas ? at(sh.number, lane) : 0u), *sum = warp_sum(lane < ctas ? at(sh.sum, lane) : 0ull);
     }
 
     // The bin in which the running number of the tokens at places >= from reaches k, or (top_p < 1) their running weight what
     // top-p keeps; what stands in front of the bin.  target: that number or weight.  in_bin: by number, how many tokens the bin
     // holds, and what stands in front of every bin is in CTA 0's bins.high.  False where there are fewer than k tokens; in_bin:
     // how many.
-    __device__ bool border_bin(uint32_t k, float top_p, u64 from, uint32_t* border, u64* before, uint32_t* in_bin, u64* target_out) const {
+    // first: no call before, bins.high is zero everywhere.
+    __device__ bool border_bin(bool first, uint32_t k, float top_p, u64 from, uint32_t* border, u64* before, uint32_t* in_bin, u64* target_out) const {
         const bool by_weight = top_p < 1.0f;
         for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) {
             if (by_weight) sh.bins.low[i] = sh.bins.high[i] = 0; else sh.bins.number[i] = 0;
@@ -174,19 +181,33 @@ struct Row {
                 atomicAdd(&sh.bins.number[b], 1);
             }
         });
-        cluster.sync();
-        // a run of bins a CTA
+        // a run of bins a CTA, a bin (of few CTAs: two, or four) a thread
         const uint32_t run = SM_BINS / ctas, b0 = rank * run;
         constexpr uint32_t MOST = SM_BINS / SM_THREADS;
+        const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1;
+        const bool sent = first && !by_weight && ctas > 1;
+        if (sent) {  // numbers to the CTAs that have the bins
+            __syncthreads();
+#pragma unroll
+            for (uint32_t j = 0; j < MOST; ++j) {
+                const uint32_t b = tid + j * SM_THREADS, n_bin = sh.bins.number[b];
+                if (n_bin) atomicAdd(&at(sh.bins.high[b % run], b / run), n_bin);
+            }
+        }
+        cluster.sync();
         u64 value[MOST], mine = 0;
 #pragma unroll
         for (uint32_t j = 0; j < MOST; ++j) {
-            const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1, b = tid * per + j;
+            const uint32_t b = tid * per + j;
             value[j] = 0;
             if (j < per && b < run) {
-#pragma unroll 4
-                for (uint32_t r = 0; r < ctas; ++r)
-                    value[j] += by_weight ? at(sh.bins.low[b0 + b], r) + ((u64)at(sh.bins.high[b0 + b], r) << 16) : at(sh.bins.number[b0 + b], r);
+                if (sent) {
+                    value[j] = sh.bins.high[b];
+                } else {
+#pragma unroll 8
+                    for (uint32_t r = 0; r < ctas; ++r)
+                        value[j] += by_weight ? at(sh.bins.low[b0 + b], r) + ((u64)at(sh.bins.high[b0 + b], r) << 16) : at(sh.bins.number[b0 + b], r);
+                }
             }
             mine += value[j];
         }
@@ -198,27 +219,21 @@ struct Row {
 #pragma unroll
         for (uint32_t w = 0; w < SM_WARPS; ++w) front += w < warp ? sh.scan[w] : 0, all += sh.scan[w];
         sum += front;
-        if (tid == 0) sh.part = all;
+        if (tid < ctas) at(sh.part[rank], tid) = all;
         cluster.sync();
-        u64 ahead = 0, whole = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const u64 x = at(sh.part, r);
-            ahead += r < rank ? x : 0, whole += x;
-        }
+        const u64 part = lane < ctas ? sh.part[lane] : 0;
+        const u64 ahead = warp_sum(lane < rank ? part : 0), whole = warp_sum(part);
         const u64 target = by_weight ? most_of(top_p, whole) : k;
         *target_out = target;
         u64 upto = ahead + sum - mine;
         const bool fewer = whole < target;  // the same everywhere
 #pragma unroll
         for (uint32_t j = 0; j < MOST; ++j) {
+            const uint32_t b = tid * per + j;
             if (upto < target && upto + value[j] >= target) {  // one thread of one CTA
-                const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1;
-                for (uint32_t r = 0; r < ctas; ++r) at(sh.bin, r) = b0 + tid * per + j, at(sh.before, r) = upto, at(sh.number, r) = (uint32_t)value[j];
+                for (uint32_t r = 0; r < ctas; ++r) at(sh.bin, r) = b0 + b, at(sh.before, r) = upto, at(sh.number, r) = (uint32_t)value[j];
             }
-            if (!by_weight) {
-                const uint32_t per = run >= SM_THREADS ? run / SM_THREADS : 1, b = tid * per + j;
-                if (j < per && b < run) at(sh.bins.high[b0 + b], 0) = (uint32_t)upto;
-            }
+            if (!by_weight && j < per && b < run) at(sh.bins.high[b0 + b], 0) = (uint32_t)upto;
             upto += value[j];
         }
         cluster.sync();
@@ -226,25 +241,41 @@ struct Row {
         return !fewer;
     }
     // Behind border_bin: the places >= from of bins first .. last in CTA 0's list, and their number in all CTAs; of more than
-    // SM_FEW, nothing else.
+    // SM_FEW, nothing else.  Every CTA has a share of the list; where one has more than that, the lists are fetched instead and
+    // follow one another (few_of[0]: all of them, the others: 0).
     __device__ uint32_t gather(uint32_t first, uint32_t last, u64 from) const {
-        // the histograms have been read in front of the last barrier
-        each([&](float x, uint32_t i) {
-            const uint32_t b = bin(x);
-            if (b < first || b > last) return;
-            const u64 p = place(i);
-            if (p < from) return;
-            const uint32_t to = atomicAdd(&sh.n_few, 1);
-            if (to < SM_FEW) sh.few[to] = p;
-        });
+        const uint32_t share = SM_FEW / ctas;
+        auto collect = [&] {  // (the histograms have been read in front of the last barrier)
+            each([&](float x, uint32_t i) {
+                const uint32_t b = bin(x);
+                if (b < first || b > last) return;
+                const u64 p = place(i);
+                if (p < from) return;
+                const uint32_t to = atomicAdd(&sh.n_few, 1);
+                if (to < SM_FEW) sh.few[to] = p;
+            });
+            __syncthreads();
+            return sh.n_few;
+        };
+        const uint32_t mine = collect();
+        if (tid < ctas) at(sh.few_of[rank], tid) = mine;
+        if (rank != 0 && mine <= share)
+            for (uint32_t i = tid; i < mine; i += SM_THREADS) at(sh.few[rank * share + i], 0) = sh.few[i];
         cluster.sync();
-        const uint32_t mine = lane < ctas ? at(sh.n_few, lane) : 0, upto = warp_scan(mine, lane), m = __shfl_sync(0xFFFFFFFFu, upto, 31);
-        if (rank == 0 && m <= SM_FEW) {
+        const uint32_t n_of = lane < ctas ? sh.few_of[lane] : 0, upto = warp_scan(n_of, lane), m = __shfl_sync(0xFFFFFFFFu, upto, 31);
+        if (m > SM_FEW || __all_sync(0xFFFFFFFFu, n_of <= share)) return m;  // the same everywhere
+        if (rank == 0) {
+            __syncthreads();
+            if (tid == 0) sh.n_few = 0;
+            __syncthreads();
+            collect();  // others have written over the end of its list
             for (uint32_t r = 1 + warp; r < ctas; r += SM_WARPS) {  // a warp a list
-                const uint32_t more = __shfl_sync(0xFFFFFFFFu, mine, r), to = __shfl_sync(0xFFFFFFFFu, upto, r) - more;
+                const uint32_t more = __shfl_sync(0xFFFFFFFFu, n_of, r), to = __shfl_sync(0xFFFFFFFFu, upto, r) - more;
                 const u64* list = cluster.map_shared_rank(sh.few, r);
                 for (uint32_t i = lane; i < more; i += 32) sh.few[to + i] = list[i];
             }
+            __syncthreads();
+            if (tid < ctas) sh.few_of[tid] = tid == 0 ? m : 0;
         }
         cluster.sync();
         return m;
@@ -254,28 +285,30 @@ struct Row {
     // bin, then behind the larger ones of the bin.  All of one bin: behind the larger ones.  Where more than RUN have to be
     // compared with one another: a bitonic sort.
     __device__ void order(uint32_t m, bool in_bins) const {
-        u64 p[PER];
+        u64 p[PER];  // 0: none
         uint32_t b[PER];
         bool long_run = false;
         __syncthreads();
+        const bool dense = sh.few_of[0] == m;
+        const uint32_t share = SM_FEW / ctas;
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j) {
             const uint32_t i = tid + j * SM_THREADS;
-            p[j] = i < m ? sh.few[i] : 0, b[j] = i < m ? bin(logit(p[j])) : 0;
+            const bool is = dense ? i < m : i % share < sh.few_of[i / share];
+            p[j] = is ? sh.few[i] : 0, b[j] = is ? bin(logit(p[j])) : 0;
         }
+        if (tid == 0) sh.n_few = 0;
         __syncthreads();
-        if (in_bins) {
 #pragma unroll
-            for (uint32_t j = 0; j < PER; ++j)
-                if (tid + j * SM_THREADS < m) sh.few[atomicAdd(&sh.bins.high[b[j]], 1)] = p[j];
-            __syncthreads();
-        }
+        for (uint32_t j = 0; j < PER; ++j)
+            if (p[j]) sh.few[atomicAdd(in_bins ? &sh.bins.high[b[j]] : &sh.n_few, 1)] = p[j];
+        __syncthreads();
         uint32_t to[PER];
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j) {
             const uint32_t first = in_bins && b[j] ? sh.bins.high[b[j] - 1] : 0, last = in_bins ? sh.bins.high[b[j]] : m;
             to[j] = first;
-            if (tid + j * SM_THREADS >= m) continue;
+            if (!p[j]) continue;
             long_run |= last - first > RUN;
             if (last - first <= RUN)
                 for (uint32_t x = first; x < last; ++x) to[j] += sh.few[x] > p[j];
@@ -286,7 +319,7 @@ struct Row {
         }
 #pragma unroll
         for (uint32_t j = 0; j < PER; ++j)
-            if (tid + j * SM_THREADS < m) sh.few[to[j]] = p[j];
+            if (p[j]) sh.few[to[j]] = p[j];
         __syncthreads();
     }
     // The same by a bitonic sort; the steps up to 32 apart stay within a warp's 64 places.
@@ -306,11 +339,11 @@ struct Row {
         __syncthreads();
     }
     // The place of the last token that a rule keeps of those at places >= from: the first k, or (top_p < 1) top-p's.
-    __device__ u64 border_place(uint32_t k, float top_p, u64 from) const {
+    __device__ u64 border_place(bool first, uint32_t k, float top_p, u64 from) const {
         const bool by_weight = top_p < 1.0f;
         uint32_t b, in_bin;
         u64 before, target;
-        if (!border_bin(k, top_p, from, &b, &before, &in_bin, &target)) return from;
+        if (!border_bin(first, k, top_p, from, &b, &before, &in_bin, &target)) return from;
         const uint32_t m = gather(b, b, from);
         if (m <= SM_FEW) {
             if (rank == 0) {
@@ -362,8 +395,15 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     __shared__ SampleShared sh;
     pdl_trigger_all();
     cg::cluster_group cluster = cg::this_cluster();
+    cluster.barrier_arrive();  // others' shared memory may be written once they have begun
     const uint32_t ctas = cluster.num_blocks(), rank = cluster.block_rank(), row = blockIdx.y;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (uint32_t i = tid; i < SM_BINS; i += SM_THREADS) sh.bins.high[i] = 0;
+    // the row's rules, on their way with its logits
+    const float given = a.temperature ? a.temperature[row] : 1.0f, temp = given > 3e38f ? 3e38f : given;  // NaN stays
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
+    const float min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f, u = a.uniform[row];
+    const int32_t wanted_k = a.top_k ? a.top_k[row] : 0;
     // slices end where the row's 16-byte vectors do; a vector that is not the row's throughout is read by its own logits
     const float* src = a.logits + row * a.stride;
     const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(src) / 4 % 4), vecs = (shift + a.vocab + 3) / 4;
@@ -425,26 +465,28 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     }
     if (lane == 0) sh.red[0][warp] = best, sh.red[1][warp] = least;
     __syncthreads();
-    if (tid == 0) {
-        for (uint32_t w = 1; w < SM_WARPS; ++w) best = fmaxf(best, sh.red[0][w]), least = fminf(least, sh.red[1][w]);
-        sh.best = best, sh.least = least;
+    auto reduce = [&](float x, float y) {
+        best = x, least = y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            best = fmaxf(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
+            least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+        }
+    };
+    cluster.barrier_wait();
+    if (warp == 0) {
+        reduce(lane < SM_WARPS ? sh.red[0][lane] : -INFINITY, lane < SM_WARPS ? sh.red[1][lane] : INFINITY);
+        if (lane < ctas) *cluster.map_shared_rank(&sh.best[rank], lane) = best, *cluster.map_shared_rank(&sh.least[rank], lane) = least;
     }
     cluster.sync();
-    best = -INFINITY, least = INFINITY;
-    for (uint32_t r = 0; r < ctas; ++r) {
-        best = fmaxf(best, *cluster.map_shared_rank(&sh.best, r));
-        least = fminf(least, *cluster.map_shared_rank(&sh.least, r));
-    }
+    reduce(lane < ctas ? sh.best[lane] : -INFINITY, lane < ctas ? sh.least[lane] : INFINITY);
     if (!(best > -INFINITY)) {  // nothing to draw: the same in the whole cluster
         if (rank == 0 && tid == 0) give(a, row, -1, 0.0f);
         cluster.sync();
         return;
     }
-    const float given = a.temperature ? a.temperature[row] : 1.0f, temp = given > 3e38f ? 3e38f : given;  // NaN stays
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
-    const float min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f, u = a.uniform[row];
     const bool greedy = !(temp > 0.0f);
-    const uint32_t top_k = greedy ? 1u : a.top_k ? (uint32_t)max(a.top_k[row], 0) : 0u;
+    const uint32_t top_k = greedy ? 1u : (uint32_t)max(wanted_k, 0);
     const float cutoff = greedy ? 0.0f : 23.0f * temp;
     Row r{cluster, sh, s_l, lo, n, ctas, rank, tid, warp, lane, best, temp, cutoff, (float)SM_BINS / fminf(best - least, cutoff), greedy};
 
@@ -452,7 +494,7 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     uint32_t border, in_bin;
     u64 before, target;
     if (top_k != 0 && top_k <= SM_FEW) {
-        const bool cut = r.border_bin(top_k, 1.0f, 0, &border, &before, &in_bin, &target);
+        const bool cut = r.border_bin(true, top_k, 1.0f, 0, &border, &before, &in_bin, &target);
         // all tokens down to the bin of the last one kept (or all there are)
         if (before + in_bin <= SM_FEW) {
             const uint32_t m = r.gather(0, border, 0);
@@ -481,24 +523,36 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
                 }
                 total = r.block_sum(sum);
                 const u64 draw = draw_of(u, total);
-                // the first id at which the kept weights, in order of ids, pass the draw
-                uint32_t kept = 0;
+                // The first id at which the kept weights, in order of ids, pass the draw: among runs of ids (a thread a run), then
+                // among the tokens of the run that it falls into.
+                u64* weight_of = reinterpret_cast<u64*>(sh.bins.high);  // of a run; behind them, a run's tokens
+                Token* tokens = reinterpret_cast<Token*>(weight_of + SM_THREADS);
+                constexpr uint32_t MOST = (sizeof(sh.bins.high) - SM_THREADS * 8) / sizeof(Token);
+                const uint32_t width = (a.vocab + SM_THREADS - 1) / SM_THREADS;
+                weight_of[tid] = 0;
+                if (tid == 0) sh.n_few = 0;
+                __syncthreads();
 #pragma unroll
-                for (uint32_t j = 0; j < PER; ++j) kept += w[j] != 0;
-                kept = (uint32_t)r.block_sum(kept);  // the first ones of the order
-                if (kept <= SM_THREADS / 2) {        // each adds up those below it
-                    u64* weights = reinterpret_cast<u64*>(sh.bins.high);
+                for (uint32_t j = 0; j < PER; ++j)
+                    if (w[j]) atomicAdd(&weight_of[id[j] / width], w[j]);
+                __syncthreads();
+                const u64 upto = r.block_scan(weight_of[tid]);
+                if (upto > draw && upto - weight_of[tid] <= draw) sh.bin = tid, sh.before = upto - weight_of[tid];
+                __syncthreads();
 #pragma unroll
-                    for (uint32_t j = 0; j < PER; ++j)
-                        if (tid * PER + j < kept) weights[tid * PER + j] = w[j];
-                    __syncthreads();
-                    if (tid < kept) {
-                        const uint32_t low = (uint32_t)sh.few[tid];  // larger for lower ids
-                        u64 below = 0;
-                        for (uint32_t x = 0; x < kept; ++x) below += (uint32_t)sh.few[x] > low ? weights[x] : 0;
-                        const u64 me = weights[tid];
-                        if (below <= draw && draw < below + me)
-                            give(a, row, (int32_t)(0xFFFFFFFFu - low), (float)((double)me / (double)total));
+                for (uint32_t j = 0; j < PER; ++j)
+                    if (w[j] && id[j] / width == sh.bin) {
+                        const uint32_t to = atomicAdd(&sh.n_few, 1);
+                        if (to < MOST) tokens[to] = Token{w[j], id[j]};
+                    }
+                __syncthreads();
+                const uint32_t n_run = sh.n_few;
+                if (n_run <= MOST) {
+                    for (uint32_t i = tid; i < n_run; i += SM_THREADS) {
+                        const Token me = tokens[i];
+                        u64 below = sh.before;
+                        for (uint32_t x = 0; x < n_run; ++x) below += tokens[x].id < me.id ? tokens[x].weight : 0;
+                        if (below <= draw && draw < below + me.weight) give(a, row, (int32_t)me.id, (float)((double)me.weight / (double)total));
                     }
                 } else {  // bit by bit: the ids below it weigh at most the draw
                     uint32_t below = 0;
@@ -516,8 +570,8 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
             return;  // the others' memory was last touched in front of the last barrier
         }
     }
-    if (top_k != 0) from = r.border_place(top_k, 1.0f, 0);
-    if (top_p < 1.0f) from = r.border_place(0, top_p, from);
+    if (top_k != 0) from = r.border_place(top_k > SM_FEW, top_k, 1.0f, 0);
+    if (top_p < 1.0f) from = r.border_place(top_k == 0, 0, top_p, from);
     // the kept weights of this CTA, run by run of ids, a run a warp; as whole numbers in 64-bit floats, exact below 2^53
     const uint32_t seg = (n + SM_WARPS - 1) / SM_WARPS, s0 = min(n, warp * seg), s1 = min(n, s0 + seg);
     auto kept = [&](uint32_t x) -> float {
@@ -535,14 +589,11 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
     u64 all = 0;
 #pragma unroll
     for (uint32_t x = 0; x < SM_WARPS; ++x) all += sh.scan2[x];
-    if (tid == 0) sh.part = all;
+    if (tid < ctas) r.at(sh.part[rank], tid) = all;
     cluster.sync();
-    u64 ahead = 0;
-    total = 0;
-    for (uint32_t x = 0; x < ctas; ++x) {
-        const u64 v = r.at(sh.part, x);
-        ahead += x < rank ? v : 0, total += v;
-    }
+    const u64 part = lane < ctas ? sh.part[lane] : 0;
+    u64 ahead = warp_sum(lane < rank ? part : 0);
+    total = warp_sum(part);
     const u64 draw = draw_of(u, total);
     if (ahead <= draw && draw < ahead + all) {  // one CTA: the run that the draw falls into, then its token by all threads
         uint32_t hit = 0;
