@@ -76,7 +76,8 @@ def test_batches(kind, batch, length):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd,n_q,n_kv,batch,shared", [(128, 8, 2, 5, 1), (128, 32, 8, 32, 3), (64, 8, 2, 33, 4), (256, 8, 2, 9, 2),
-                                                      (64, 4, 4, 2, 9), (128, 9, 3, 7, 5), (128, 16, 1, 3, 2), (64, 8, 8, 130, 1)])
+                                                      (64, 4, 4, 2, 9), (128, 9, 3, 7, 5), (128, 16, 1, 3, 2), (64, 8, 8, 130, 1), (128, 32, 8, 100, 9),
+                                                      (64, 16, 2, 9, 40), (128, 8, 1, 33, 33)])
 def test_shared_pages(kind, hd, n_q, n_kv, batch, shared):
     """Sequences behind a common prompt: the same as each by itself, some with nothing of their own, one inactive."""
     import torch

@@ -78,6 +78,28 @@ def test_rules(vocab, kind):
     assert np.all(np.abs(prob - [w[1] for w in want]) <= TOL * np.array([w[1] for w in want]))
 
 
+@pytest.mark.parametrize("vocab,first,count", [(151936, 100, 1500), (151936, 37000, 1100), (30000, 29000, 1000), (151936, 0, 2500)])
+@pytest.mark.parametrize("equal", [False, True])
+def test_candidates_close_together(vocab, first, count, equal):
+    """The likely tokens are neighbours, so one CTA of a row's has nearly all that the rules look at; all alike, or not."""
+    rng = np.random.RandomState(count)
+    l, u, k, p = [], [], [], []
+    for top_k in (900, 1000, 2000, 0):
+        for top_p in (1.0, 0.8):
+            for _ in range(50):
+                row = (rng.randn(vocab) * 0.5 - 12).astype(np.float32)
+                row[first:first + count] = 1.5 if equal else rng.randn(len(row[first:first + count]))
+                draw = np.float32(rng.rand())
+                if decided(row, draw, 1.0, top_k, np.float32(top_p), 0.0):
+                    l.append(row), u.append(draw), k.append(top_k), p.append(np.float32(top_p))
+                    break
+    assert len(l) >= 4
+    token, prob = run(np.stack(l), u, top_k=k, top_p=p)
+    want = [ref.sample(a, b, 1.0, c, d) for a, b, c, d in zip(l, u, k, p)]
+    assert token.tolist() == [w[0] for w in want]
+    assert np.all(np.abs(prob - [w[1] for w in want]) <= TOL * np.array([w[1] for w in want]))
+
+
 @pytest.mark.parametrize("vocab", [3, 5000, 40000])
 def test_each_rule_may_be_absent(vocab):
     rng = np.random.RandomState(1)
