@@ -191,61 +191,75 @@ struct RowGroup {
     }
 };
 
-// Many rows: four warps have a head of 16 rows, four rows each, their loads on their way together.  Where the 16 are a whole run
-// of positions, the codes are put together in shared memory as they stand in the page and stored from there in whole lines: a
-// position's codes alone are 4 bytes and fewer to a sector of 32.
+// Many rows: four warps have a head of 16 rows, four rows each, their loads on their way together, and `turns` heads after one
+// another (the next one's rows are requested before this one's are worked on), so that what is found out about the rows serves
+// all of them.  Where the 16 are a whole run of positions, the codes are put together in shared memory as they stand in the page
+// and stored from there in whole lines: a position's codes alone are 4 bytes and fewer to a sector of 32.
 template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256, HD == 256 ? 3 : 5) kv_append_rows_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, HD == 256 ? 2 : 4) kv_append_rows_kernel(AppendArgs a, uint32_t turns) {
     using Lanes = HeadLanes<HD>;
     constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD), RUN = CODES / 4;
-    constexpr uint32_t EACH = 4;
+    constexpr uint32_t EACH = 4, AT_ONCE = 2 * HPW;  // rows a warp, heads a CTA at a time
     __shared__ __align__(16) float s_head[8 * HPW][HD];
-    __shared__ __align__(16) uint8_t s_run[2 * HPW][RUN];
+    __shared__ __align__(16) uint8_t s_run[AT_ONCE][RUN];
     pdl_trigger_all();
     const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES, local = (warp & 1) * HPW + group;
-    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = blockIdx.y * 2 * HPW + local;
-    const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
-    const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
+    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head0 = blockIdx.y * turns * AT_ONCE;
     RowGroup g(a.pos, a.rows, blockIdx.x);
     const uint32_t j0 = warp / 2 * EACH;
-    Lanes x[EACH];
+    Lanes next[EACH];
+    auto request = [&](uint32_t head) {
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i)
-        x[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, live && g.has(j0 + i));
+        for (uint32_t i = 0; i < EACH; ++i)
+            next[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, head < heads && g.has(j0 + i));
+    };
+    request(head0 + local);
     g.look(a.pos, a.seq);
     uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places; the same in the CTA
     if (g.runs && g.rows == 16 && a.page((uint32_t)g.first + 15, HEAD)) run = a.page((uint32_t)g.first, HEAD);
-    const bool turns = __any_sync(0xFFFFFFFFu, live && !is_v);  // two heads a warp: a value's lanes go along, and stay as they were
+    const uint32_t end = min(heads, head0 + turns * AT_ONCE);
+    for (uint32_t first = head0; first < end; first += AT_ONCE) {
+        const uint32_t head = first + local;
+        const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
+        const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
+        Lanes x[EACH];
 #pragma unroll
-    for (uint32_t i = 0; i < EACH; ++i) {
-        if (!g.has(j0 + i)) continue;
-        const uint32_t row = (uint32_t)(g.first + j0 + i);
-        uint8_t* page = run ? run : a.page(row, HEAD);
-        if (page == nullptr) {
-            if (blockIdx.y == 0 && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-            continue;
+        for (uint32_t i = 0; i < EACH; ++i) x[i] = next[i];
+        if (first + AT_ONCE < end) request(head + AT_ONCE);
+        // two heads a warp: a value's lanes go along, and stay as they were
+        const bool to_turn = __any_sync(0xFFFFFFFFu, live && !is_v), to_keep = __any_sync(0xFFFFFFFFu, live && !is_q);
+#pragma unroll
+        for (uint32_t i = 0; i < EACH; ++i) {
+            if (!g.has(j0 + i)) continue;
+            const uint32_t row = (uint32_t)(g.first + j0 + i);
+            uint8_t* page = run ? run : a.page(row, HEAD);
+            if (page == nullptr) {
+                if (head < HPW && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+                continue;
+            }
+            const uint32_t p = run ? (uint32_t)g.p0 + j0 + i : (uint32_t)a.pos[row];
+            if (to_turn) {
+                const Lanes y = x[i];
+                if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
+                if (a.r.table) x[i].turn(a.r, p, s_head[warp * HPW + group]);
+                if (is_v) x[i] = y;
+            }
+            if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
+            if (!to_keep) continue;
+            uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
+            x[i].template put<KIND>(run ? s_run[local] : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
         }
-        const uint32_t p = run ? (uint32_t)g.p0 + j0 + i : (uint32_t)a.pos[row];
-        if (turns) {
-            const Lanes y = x[i];
-            if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
-            if (a.r.table) x[i].turn(a.r, p, s_head[warp * HPW + group]);
-            if (is_v) x[i] = y;
+        if (run == nullptr || first + AT_ONCE <= a.n_q) continue;  // the same in the CTA
+        __syncthreads();
+        const uint32_t at = (uint32_t)g.p0 % KV_PAGE / 16 * RUN;
+        for (uint32_t i = threadIdx.x; i < AT_ONCE * (RUN / 16); i += 256) {
+            const uint32_t h = first + i / (RUN / 16), o = i % (RUN / 16) * 16;
+            if (h < a.n_q || h >= heads) continue;
+            const bool v = h >= a.n_q + a.c.n_kv;
+            uint8_t* part = run + (uint64_t)(v ? h - a.n_q - a.c.n_kv : h - a.n_q) * HEAD + (v ? HEAD / 2 : 0);
+            *reinterpret_cast<uint4*>(part + at + o) = *reinterpret_cast<const uint4*>(s_run[i / (RUN / 16)] + o);
         }
-        if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
-        if (!__any_sync(0xFFFFFFFFu, live && !is_q)) continue;
-        uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
-        x[i].template put<KIND>(run ? s_run[local] : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
-    }
-    if (run == nullptr) return;
-    __syncthreads();
-    const uint32_t at = (uint32_t)g.p0 % KV_PAGE / 16 * RUN;
-    for (uint32_t i = threadIdx.x; i < 2 * HPW * (RUN / 16); i += 256) {
-        const uint32_t h = blockIdx.y * 2 * HPW + i / (RUN / 16), o = i % (RUN / 16) * 16;
-        if (h < a.n_q || h >= heads) continue;
-        const bool v = h >= a.n_q + a.c.n_kv;
-        uint8_t* part = run + (uint64_t)(v ? h - a.n_q - a.c.n_kv : h - a.n_q) * HEAD + (v ? HEAD / 2 : 0);
-        *reinterpret_cast<uint4*>(part + at + o) = *reinterpret_cast<const uint4*>(s_run[i / (RUN / 16)] + o);
+        __syncthreads();
     }
 }
 
@@ -418,7 +432,11 @@ struct LaunchAppend {
         const uint32_t heads = a.n_q + 2 * a.c.n_kv;
         if (a.rows < MANY_ROWS)
             return launch_pdl(kv_append_kernel<KIND, HD>, dim3(a.rows, (heads + 8 * HPW - 1) / (8 * HPW)), 256, 0, s, a);
-        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3((a.rows + 30) / 16, (heads + 2 * HPW - 1) / (2 * HPW)), 256, 0, s, a);
+        // up to four heads a warp, fewer where that leaves the GPU's SMs with less than four CTAs each
+        const uint32_t blocks = (a.rows + 30) / 16, parts = (heads + 2 * HPW - 1) / (2 * HPW);
+        uint32_t turns = 4;
+        while (turns > 1 && blocks * ((parts + turns - 1) / turns) < 4u * num_sms()) turns /= 2;
+        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3(blocks, (parts + turns - 1) / turns), 256, 0, s, a, turns);
     }
 };
 struct LaunchRead {
