@@ -15,6 +15,7 @@ from ._lib import JoshuaB200Error, check
 from .rope import Rope, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 PAGE = 64
+_capturing = torch.cuda.is_current_stream_capturing
 TYPES = {"f16": 1, "q4_0": 2, "q8_0": 8}
 
 
@@ -104,7 +105,8 @@ class PagedCache:
     def attend(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, scale: float = 0.0, shared_pages: int = 0,
                out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one query row per sequence, [batch, n_q * head_dim], over its first `lens` positions; the first
-        `shared_pages` pages are the same for all.  `scratch`: from `scratch()`; by default one a stream, kept with the cache."""
+        `shared_pages` pages are the same for all.  `scratch`: from `scratch()`; by default one a stream, kept with the cache
+        (while a graph is captured, the graph's own)."""
         index, width = self._index, n_q * self.head_dim
         at, stride, batch = rows_arg(q, "q", width, index)
         n = batch
@@ -118,10 +120,13 @@ class PagedCache:
             raise JoshuaB200Error(_lib.E_INVALID, f"{batch} query rows, {n} rows of out, {n_seq} of the page table")
         stream = _raw_stream(index)
         if scratch is None:
-            key = (stream, batch, n_q, shared_pages)
-            scratch = self._scratch.get(key)
-            if scratch is None:
-                scratch = self._scratch[key] = self.scratch(batch, n_q, shared_pages)
+            if _capturing():  # the graph's own, zeroed by it: it may be replayed beside this stream's next call
+                scratch = self.scratch(batch, n_q, shared_pages)
+            else:
+                key = (stream, batch, n_q, shared_pages)
+                scratch = self._scratch.get(key)
+                if scratch is None:
+                    scratch = self._scratch[key] = self.scratch(batch, n_q, shared_pages)
         rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
                           shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)
         if rc:
