@@ -135,37 +135,11 @@ struct AppendArgs {
         uint8_t* at = page_of(c, seq_of(row), p, head_bytes);
         return r.table != nullptr && (uint32_t)p >= r.n_pos ? nullptr : at;
     }
+    // a key's or value's head in a page
+    __device__ __forceinline__ uint8_t* part(uint8_t* page, uint32_t head, uint32_t head_bytes) const {
+        return head < c.n_kv ? page + (uint64_t)head * head_bytes : page + (uint64_t)(head - c.n_kv) * head_bytes + head_bytes / 2;
+    }
 };
-
-// A row per blockIdx.x, a head a group of lanes.
-template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
-    using Lanes = HeadLanes<HD>;
-    constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD);
-    __shared__ __align__(16) float s_head[8 * HPW][HD];
-    pdl_trigger_all();
-    const uint32_t row = blockIdx.x, warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES;
-    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head = (blockIdx.y * 8 + warp) * HPW + group;
-    const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
-    uint8_t* page = a.page(row, HEAD);
-    if (page == nullptr) {  // the same in the whole row
-        if (blockIdx.y == 0 && threadIdx.x == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-        return;
-    }
-    Lanes x;
-    x.load(a.qkv + row * a.stride + (uint64_t)head * HD, live);
-    const uint32_t p = (uint32_t)a.pos[row];
-    if (__any_sync(0xFFFFFFFFu, !is_v)) {  // two heads a warp: a value's lanes go along, and stay as they were
-        const Lanes y = x;
-        if (a.q_norm) x.norm(is_q ? a.q_norm : a.k_norm, a.eps);
-        if (a.r.table) x.turn(a.r, p, s_head[warp * HPW + group]);
-        if (is_v) x = y;
-    }
-    const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
-    uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
-    if (live && is_q) x.store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
-    x.template put<KIND>(part, p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
-}
 
 // The 16 rows that a warp or CTA of the kernels below takes, first + j (j = 0 .. 15): rows are grouped by the first row's position.
 struct RowGroup {
@@ -191,75 +165,151 @@ struct RowGroup {
     }
 };
 
-// Many rows: four warps have a head of 16 rows, four rows each, their loads on their way together, and `turns` heads after one
-// another (the next one's rows are requested before this one's are worked on), so that what is found out about the rows serves
-// all of them.  Where the 16 are a whole run of positions, the codes are put together in shared memory as they stand in the page
-// and stored from there in whole lines: a position's codes alone are 4 bytes and fewer to a sector of 32.
+// A key's or value's head of a row (keys are heads 0 .. n_kv - 1, values those behind them), its codes to `run` as one of 16
+// positions if that is given.
 template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256, HD == 256 ? 2 : 4) kv_append_rows_kernel(AppendArgs a, uint32_t turns) {
+__device__ __forceinline__ void append_head(const AppendArgs& a, HeadLanes<HD>& x, uint32_t row, uint8_t* page, uint32_t p, uint32_t head,
+                                            float* mine, uint8_t* run = nullptr) {
+    constexpr uint32_t CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD);
+    if (page == nullptr) {  // the same in the warp
+        if (head == 0 && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+        return;
+    }
+    const bool live = head < 2 * a.c.n_kv, is_v = head >= a.c.n_kv;
+    if (__any_sync(0xFFFFFFFFu, !is_v)) {  // two heads a warp: a value's lanes go along, and stay as they were
+        const HeadLanes<HD> y = x;
+        if (a.k_norm) x.norm(a.k_norm, a.eps);
+        if (a.r.table) x.turn(a.r, p, mine);
+        if (is_v) x = y;
+    }
+    uint8_t* part = live ? a.part(page, head, HEAD) : page;
+    x.template put<KIND>(run ? run : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live);
+}
+
+// Queries: a warp has a row and `turns` times as many heads as HD / 8 lanes each leave it, four dimensions and the four that they
+// turn with a lane, so that a pair is one thread's and the row's cosines and sines serve all of its heads.
+template <uint32_t HD>
+__device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t item, uint32_t turns, float* s_warp) {
+    constexpr uint32_t LANES = HD / 8, AT_ONCE = 32 / LANES;
+    const uint32_t chunks = (a.n_q + turns * AT_ONCE - 1) / (turns * AT_ONCE), row = item / chunks;
+    if (row >= a.rows) return;
+    const uint32_t head0 = item % chunks * turns * AT_ONCE, end = min(a.n_q, head0 + turns * AT_ONCE);
+    const float* src = a.qkv + row * a.stride;
+    float* dst = a.q_out + (uint64_t)row * a.n_q * HD;
+    const RopeArgs& r = a.r;
+    if (r.table != nullptr && !r.vectors) {  // pairs that are no whole vectors
+        using Lanes = HeadLanes<HD>;
+        if (a.page(row, 0) == nullptr) return;
+        const uint32_t p = (uint32_t)a.pos[row], group = (threadIdx.x & 31) / Lanes::LANES;
+        for (uint32_t h = head0; h < end; h += Lanes::PER_WARP) {
+            const bool live = h + group < end;
+            Lanes x;
+            x.load(src + (uint64_t)(h + group) * HD, live);
+            if (a.q_norm) x.norm(a.q_norm, a.eps);
+            x.turn(r, p, s_warp + group * HD);
+            if (live) x.store(dst + (uint64_t)(h + group) * HD);
+        }
+        return;
+    }
+    const uint32_t l = (threadIdx.x & 31) % LANES, group = (threadIdx.x & 31) / LANES, half = r.rot / 2;
+    const bool turned = r.table != nullptr && 8 * l < r.rot, split = turned && !r.interleaved;
+    const uint32_t at_u = split ? 4 * l : 8 * l, at_v = split ? half + 4 * l : 8 * l + 4;
+    float4 next_u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), next_v = next_u;
+    auto request = [&](uint32_t head) {
+        if (head >= end) return;
+        next_u = __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_u));
+        next_v = __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_v));
+    };
+    request(head0 + group);
+    if (a.page(row, 0) == nullptr) return;
+    float4 cs0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), cs1 = cs0, wu, wv;
+    if (turned) {
+        const float4* t = reinterpret_cast<const float4*>(r.table + (uint64_t)(uint32_t)a.pos[row] * half + 4 * l);
+        cs0 = __ldg(t), cs1 = __ldg(t + 1);
+    }
+    if (a.q_norm) wu = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_u)), wv = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_v));
+    for (uint32_t h = head0 + group; h < end + group; h += AT_ONCE) {
+        float u[4] = {next_u.x, next_u.y, next_u.z, next_u.w}, v[4] = {next_v.x, next_v.y, next_v.z, next_v.w};
+        request(h + AT_ONCE);
+        if (a.q_norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
+#pragma unroll
+            for (uint32_t o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+            const float sc = rsqrtf(ss / (float)HD + a.eps);
+            u[0] = u[0] * sc * wu.x, u[1] = u[1] * sc * wu.y, u[2] = u[2] * sc * wu.z, u[3] = u[3] * sc * wu.w;
+            v[0] = v[0] * sc * wv.x, v[1] = v[1] * sc * wv.y, v[2] = v[2] * sc * wv.z, v[3] = v[3] * sc * wv.w;
+        }
+        if (turned) {
+            const float2 cs[4] = {make_float2(cs0.x, cs0.y), make_float2(cs0.z, cs0.w), make_float2(cs1.x, cs1.y), make_float2(cs1.z, cs1.w)};
+            auto turn = [](float& x, float& y, float2 by) {
+                const float first = rope_rotate(true, x, y, by);
+                y = rope_rotate(false, y, x, by), x = first;
+            };
+            if (split) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) turn(u[e], v[e], cs[e]);
+            } else {
+                turn(u[0], u[1], cs[0]), turn(u[2], u[3], cs[1]), turn(v[0], v[1], cs[2]), turn(v[2], v[3], cs[3]);
+            }
+        }
+        if (h >= end) continue;
+        *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_u) = make_float4(u[0], u[1], u[2], u[3]);
+        *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_v) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+}
+
+// Keys and values in the first CTAs, queries in the rest.  RUNS: four warps have a key's or value's head of 16 rows, four rows
+// each, their loads on their way together; where the 16 are a whole run of positions, the codes are put together in shared
+// memory as they stand in the page and stored from there in whole lines: a position's codes alone are 4 bytes and fewer to a
+// sector of 32.  Else a warp has one row's.
+template <uint32_t KIND, uint32_t HD, bool RUNS>
+__global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs a, uint32_t kv_blocks, uint32_t turns) {
     using Lanes = HeadLanes<HD>;
     constexpr uint32_t HPW = Lanes::PER_WARP, CODES = kv_code_bytes(KIND, HD), HEAD = kv_head_bytes(KIND, HD), RUN = CODES / 4;
-    constexpr uint32_t EACH = 4, AT_ONCE = 2 * HPW;  // rows a warp, heads a CTA at a time
+    constexpr uint32_t EACH = RUNS ? 4 : 1, AT_ONCE = 2 * HPW;  // rows a warp, heads a CTA of runs
     __shared__ __align__(16) float s_head[8 * HPW][HD];
-    __shared__ __align__(16) uint8_t s_run[AT_ONCE][RUN];
+    __shared__ __align__(16) uint8_t s_run[RUNS ? AT_ONCE : 1][RUNS ? RUN : 16];
     pdl_trigger_all();
-    const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES, local = (warp & 1) * HPW + group;
-    const uint32_t heads = a.n_q + 2 * a.c.n_kv, head0 = blockIdx.y * turns * AT_ONCE;
-    RowGroup g(a.pos, a.rows, blockIdx.x);
-    const uint32_t j0 = warp / 2 * EACH;
-    Lanes next[EACH];
-    auto request = [&](uint32_t head) {
-#pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i)
-            next[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)head * HD, head < heads && g.has(j0 + i));
-    };
-    request(head0 + local);
-    g.look(a.pos, a.seq);
-    uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places; the same in the CTA
-    if (g.runs && g.rows == 16 && a.page((uint32_t)g.first + 15, HEAD)) run = a.page((uint32_t)g.first, HEAD);
-    const uint32_t end = min(heads, head0 + turns * AT_ONCE);
-    for (uint32_t first = head0; first < end; first += AT_ONCE) {
-        const uint32_t head = first + local;
-        const bool live = head < heads, is_q = head < a.n_q, is_v = head >= a.n_q + a.c.n_kv;
-        const uint32_t kvh = is_v ? head - a.n_q - a.c.n_kv : is_q ? 0 : head - a.n_q;
+    const uint32_t warp = threadIdx.x >> 5, group = (threadIdx.x & 31) / Lanes::LANES;
+    if (blockIdx.x >= kv_blocks) {
+        append_queries<HD>(a, (blockIdx.x - kv_blocks) * 8 + warp, turns, s_head[warp * HPW]);
+        return;
+    }
+    const uint32_t heads = 2 * a.c.n_kv;  // keys, then values
+    if constexpr (!RUNS) {
+        const uint32_t parts = (heads + HPW - 1) / HPW, item = blockIdx.x * 8 + warp, row = item / parts;
+        if (row >= a.rows) return;
+        const uint32_t head = item % parts * HPW + group;
+        Lanes x;
+        x.load(a.qkv + row * a.stride + (uint64_t)(a.n_q + head) * HD, head < heads);
+        append_head<KIND, HD>(a, x, row, a.page(row, HEAD), (uint32_t)a.pos[row], head, s_head[warp * HPW + group]);
+    } else {
+        const uint32_t parts = (heads + AT_ONCE - 1) / AT_ONCE, first = blockIdx.x % parts * AT_ONCE, local = (warp & 1) * HPW + group;
+        const uint32_t head = first + local, j0 = warp / 2 * EACH;
+        RowGroup g(a.pos, a.rows, blockIdx.x / parts);
         Lanes x[EACH];
 #pragma unroll
-        for (uint32_t i = 0; i < EACH; ++i) x[i] = next[i];
-        if (first + AT_ONCE < end) request(head + AT_ONCE);
-        // two heads a warp: a value's lanes go along, and stay as they were
-        const bool to_turn = __any_sync(0xFFFFFFFFu, live && !is_v), to_keep = __any_sync(0xFFFFFFFFu, live && !is_q);
+        for (uint32_t i = 0; i < EACH; ++i)
+            x[i].load(a.qkv + (uint64_t)(g.first + j0 + i) * a.stride + (uint64_t)(a.n_q + head) * HD, head < heads && g.has(j0 + i));
+        g.look(a.pos, a.seq);
+        uint8_t* run = nullptr;  // the page of a whole run of 16 that has its places; the same in the CTA
+        if (g.runs && g.rows == 16 && a.page((uint32_t)g.first + 15, HEAD)) run = a.page((uint32_t)g.first, HEAD);
 #pragma unroll
         for (uint32_t i = 0; i < EACH; ++i) {
             if (!g.has(j0 + i)) continue;
             const uint32_t row = (uint32_t)(g.first + j0 + i);
-            uint8_t* page = run ? run : a.page(row, HEAD);
-            if (page == nullptr) {
-                if (head < HPW && threadIdx.x % 32 == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-                continue;
-            }
-            const uint32_t p = run ? (uint32_t)g.p0 + j0 + i : (uint32_t)a.pos[row];
-            if (to_turn) {
-                const Lanes y = x[i];
-                if (a.q_norm) x[i].norm(is_q ? a.q_norm : a.k_norm, a.eps);
-                if (a.r.table) x[i].turn(a.r, p, s_head[warp * HPW + group]);
-                if (is_v) x[i] = y;
-            }
-            if (live && is_q) x[i].store(a.q_out + ((uint64_t)row * a.n_q + head) * HD);
-            if (!to_keep) continue;
-            uint8_t* part = page + (uint64_t)kvh * HEAD + (is_v ? HEAD / 2 : 0);
-            x[i].template put<KIND>(run ? s_run[local] : part, run ? p % 16 : p % KV_PAGE, part + CODES, p % KV_PAGE, is_v, live && !is_q);
+            if (run) append_head<KIND, HD>(a, x[i], row, run, (uint32_t)g.p0 + j0 + i, head, s_head[warp * HPW + group], s_run[local]);
+            else append_head<KIND, HD>(a, x[i], row, a.page(row, HEAD), (uint32_t)a.pos[row], head, s_head[warp * HPW + group]);
         }
-        if (run == nullptr || first + AT_ONCE <= a.n_q) continue;  // the same in the CTA
+        if (run == nullptr) return;
         __syncthreads();
         const uint32_t at = (uint32_t)g.p0 % KV_PAGE / 16 * RUN;
         for (uint32_t i = threadIdx.x; i < AT_ONCE * (RUN / 16); i += 256) {
             const uint32_t h = first + i / (RUN / 16), o = i % (RUN / 16) * 16;
-            if (h < a.n_q || h >= heads) continue;
-            const bool v = h >= a.n_q + a.c.n_kv;
-            uint8_t* part = run + (uint64_t)(v ? h - a.n_q - a.c.n_kv : h - a.n_q) * HEAD + (v ? HEAD / 2 : 0);
-            *reinterpret_cast<uint4*>(part + at + o) = *reinterpret_cast<const uint4*>(s_run[i / (RUN / 16)] + o);
+            if (h < heads) *reinterpret_cast<uint4*>(a.part(run, h, HEAD) + at + o) = *reinterpret_cast<const uint4*>(s_run[i / (RUN / 16)] + o);
         }
-        __syncthreads();
     }
 }
 
@@ -421,7 +471,7 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int3
 }
 
 // From so many rows on, 16 rows a warp: below, a row's latency counts.
-constexpr uint32_t MANY_ROWS = 128;
+constexpr uint32_t MANY_ROWS = 768, QUERY_WARPS = 32;
 
 struct LaunchAppend {
     const AppendArgs& a;
@@ -429,14 +479,18 @@ struct LaunchAppend {
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
         constexpr uint32_t HPW = HeadLanes<HD>::PER_WARP;
-        const uint32_t heads = a.n_q + 2 * a.c.n_kv;
-        if (a.rows < MANY_ROWS)
-            return launch_pdl(kv_append_kernel<KIND, HD>, dim3(a.rows, (heads + 8 * HPW - 1) / (8 * HPW)), 256, 0, s, a);
-        // up to four heads a warp, fewer where that leaves the GPU's SMs with less than four CTAs each
-        const uint32_t blocks = (a.rows + 30) / 16, parts = (heads + 2 * HPW - 1) / (2 * HPW);
-        uint32_t turns = 4;
-        while (turns > 1 && blocks * ((parts + turns - 1) / turns) < 4u * num_sms()) turns /= 2;
-        return launch_pdl(kv_append_rows_kernel<KIND, HD>, dim3(blocks, (parts + turns - 1) / turns), 256, 0, s, a, turns);
+        const uint32_t per_warp = 256 / HD, most = (a.n_q + per_warp - 1) / per_warp;
+        uint32_t turns = 1;
+        while (turns < most && (uint64_t)a.rows * ((most + turns - 1) / turns) > QUERY_WARPS * num_sms()) turns *= 2;
+        const uint32_t q_blocks = (uint32_t)(((uint64_t)a.rows * ((most + turns - 1) / turns) + 7) / 8), heads = 2 * a.c.n_kv;
+        if constexpr (HD < 256) {
+            if (a.seq != nullptr && a.rows >= MANY_ROWS) {
+                const uint32_t kv_blocks = (a.rows + 30) / 16 * ((heads + 2 * HPW - 1) / (2 * HPW));
+                return launch_pdl(kv_append_kernel<KIND, HD, true>, dim3(kv_blocks + q_blocks), 256, 0, s, a, kv_blocks, turns);
+            }
+        }
+        const uint32_t kv_blocks = (uint32_t)(((uint64_t)a.rows * ((heads + HPW - 1) / HPW) + 7) / 8);
+        return launch_pdl(kv_append_kernel<KIND, HD, false>, dim3(kv_blocks + q_blocks), 256, 0, s, a, kv_blocks, turns);
     }
 };
 struct LaunchRead {
@@ -449,11 +503,13 @@ struct LaunchRead {
     cudaStream_t s;
     template <uint32_t KIND, uint32_t HD>
     cudaError_t operator()() const {
-        if (rows < MANY_ROWS)
-            return launch_pdl(kv_read_kernel<KIND, HD>, dim3(rows, (c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, k, v, row_stride,
-                              head_stride, bad_pos);
-        return launch_pdl(kv_read_rows_kernel<KIND, HD>, dim3((rows + 30) / 16, (2 * c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, rows, k, v,
-                          row_stride, head_stride, bad_pos);
+        if constexpr (HD < 256) {
+            if (seq != nullptr && rows >= MANY_ROWS)
+                return launch_pdl(kv_read_rows_kernel<KIND, HD>, dim3((rows + 30) / 16, (2 * c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, rows,
+                                  k, v, row_stride, head_stride, bad_pos);
+        }
+        return launch_pdl(kv_read_kernel<KIND, HD>, dim3(rows, (c.n_kv + 7) / 8), 256, 0, s, c, pos, seq, k, v, row_stride, head_stride,
+                          bad_pos);
     }
 };
 

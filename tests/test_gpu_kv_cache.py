@@ -121,6 +121,51 @@ def test_many_rows_of_several_sequences(kind, hd):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,n_q,n_kv,rot,interleaved", [(64, 5, 5, 64, False), (128, 6, 3, 64, True), (128, 2, 2, 12, False), (256, 2, 1, 256, False)])
+def test_a_thousand_rows(kind, hd, n_q, n_kv, rot, interleaved):
+    """Whole prompts of two sequences in one call, rotated and normed on the way as the same rows a few at a time, in order and out
+    of it; their neighbours stay; rows without a place among them."""
+    import torch
+
+    from joshua_b200.rope import Rope, rope_table
+
+    rope = Rope(rope_table(10000.0, rot, 960, "cuda"), interleaved=interleaved)
+    (cache, table), (other, _) = make(kind, n_kv, hd, 2, 15), make(kind, n_kv, hd, 2, 15)
+    width = (n_q + 2 * n_kv) * hd
+    rng = np.random.RandomState(hd + rot)
+    norm = torch.from_numpy(rng.uniform(0.5, 2.0, hd).astype(np.float32)).cuda()
+    every = i32(list(range(960)) * 2), i32([0] * 960 + [1] * 960)
+    before = torch.from_numpy(rng.randn(1920, width).astype(np.float32)).cuda()
+    for c in (cache, other):
+        c.append(before, every[0], table, n_q=n_q, seq=every[1])
+    seq = np.repeat([1, 0], [603, 411])
+    pos = np.concatenate([np.arange(603) + 47, np.arange(411) + 500])
+    x = torch.from_numpy(rng.randn(len(pos), width).astype(np.float32)).cuda()
+    for order in (np.arange(len(pos)), rng.permutation(len(pos))):
+        kw = dict(n_q=n_q, rope=rope, q_norm=norm, k_norm=norm, eps=1e-5)
+        q = cache.append(x, i32(pos[order]), table, seq=i32(seq[order]), **kw)
+        few = torch.cat([other.append(x[i:i + 100], i32(pos[order][i:i + 100]), table, seq=i32(seq[order][i:i + 100]), **kw)
+                         for i in range(0, len(pos), 100)])
+        assert torch.equal(q, few)
+        read = cache.read(*every[:1], table, seq=every[1])
+        parts = [other.read(every[0][i:i + 100], table, seq=every[1][i:i + 100]) for i in range(0, 1920, 100)]
+        for i in range(2):
+            assert torch.equal(read[i], torch.cat([part[i] for part in parts], 1))
+        _, _, wv = split(x.cpu().numpy(), n_q, n_kv, hd)
+        assert np.array_equal(cache.read(i32(pos[order]), table, seq=i32(seq[order]))[1].cpu().numpy(), ref.held(wv, kind).transpose(1, 0, 2))
+    cache.check_flags()
+    lost = pos.copy()
+    lost[[40, 1000]] = -1, 15 * 64
+    out = torch.full((len(pos), n_q * hd), 7.0, device="cuda")
+    q = cache.append(x, i32(pos), table, seq=i32(seq), **kw)
+    cache.append(x, i32(lost), table, seq=i32(seq), out=out, **kw)
+    q[[40, 1000]] = 7.0
+    assert torch.equal(q, out) and int(cache.bad_pos) == 1
+    k, v = cache.read(i32(lost), table, seq=i32(seq))
+    assert bool(k[:, [40, 1000]].isnan().all()) and int(torch.cat([k, v]).isnan().any(2).sum()) == 4 * n_kv
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("rows", [40, 170])
 @pytest.mark.parametrize("hd,rot,interleaved", [(128, 128, False), (128, 64, True), (64, 64, True), (256, 96, False), (64, 2, False)])
 def test_rotation_on_the_way(kind, rows, hd, rot, interleaved):
