@@ -513,33 +513,37 @@ struct Joined {
             }
         }
     }
-    // ... and those of the leading pages (LEAD_MOST at most, all on their way together)
+    // ... and those of the leading pages, four on their way together
     __device__ __forceinline__ void add_lead(const PagedArgs& a, uint32_t kvh, uint32_t row, uint32_t lane) {
+        constexpr uint32_t AT_ONCE = 4;
         const uint64_t rows = (uint64_t)a.c.n_seq * a.group, stride = a.c.n_kv * rows, all = a.lead_splits * stride, at = kvh * rows + row;
-        float4 v[LEAD_MOST][N];
-        float m[LEAD_MOST], l[LEAD_MOST], t = top;
+        for (uint32_t j0 = 0; j0 < a.lead_splits; j0 += AT_ONCE) {
+            float4 v[AT_ONCE][N];
+            float m[AT_ONCE], l[AT_ONCE], t = top;
 #pragma unroll
-        for (uint32_t j = 0; j < LEAD_MOST; ++j) {
-            const bool is = j < a.lead_splits;
+            for (uint32_t j = 0; j < AT_ONCE; ++j) {
+                const bool is = j0 + j < a.lead_splits;
+                const uint64_t from = at + (j0 + j) * stride;
 #pragma unroll
-            for (uint32_t k = 0; k < N; ++k)
-                v[j][k] = is && (HD >= 128 || lane < HD / 4) ? *reinterpret_cast<const float4*>(a.lead + (at + j * stride) * HD + 4 * lane + 128 * k)
-                                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            m[j] = is ? a.lead[all * HD + at + j * stride] : -INFINITY, l[j] = is ? a.lead[all * HD + all + at + j * stride] : 0.0f;
-            t = fmaxf(t, m[j]);
-        }
-        const float old = piece_weight(top, t);
-        den *= old, top = t;
+                for (uint32_t k = 0; k < N; ++k)
+                    v[j][k] = is && (HD >= 128 || lane < HD / 4) ? *reinterpret_cast<const float4*>(a.lead + from * HD + 4 * lane + 128 * k)
+                                                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                m[j] = is ? a.lead[all * HD + from] : -INFINITY, l[j] = is ? a.lead[all * HD + all + from] : 0.0f;
+                t = fmaxf(t, m[j]);
+            }
+            const float old = piece_weight(top, t);
+            den *= old, top = t;
 #pragma unroll
-        for (uint32_t k = 0; k < N; ++k) x[k].x *= old, x[k].y *= old, x[k].z *= old, x[k].w *= old;
+            for (uint32_t k = 0; k < N; ++k) x[k].x *= old, x[k].y *= old, x[k].z *= old, x[k].w *= old;
 #pragma unroll
-        for (uint32_t j = 0; j < LEAD_MOST; ++j) {
-            const float f = piece_weight(m[j], t);
-            den = fmaf(f, l[j], den);
+            for (uint32_t j = 0; j < AT_ONCE; ++j) {
+                const float f = piece_weight(m[j], t);
+                den = fmaf(f, l[j], den);
 #pragma unroll
-            for (uint32_t k = 0; k < N; ++k) {
-                x[k].x = fmaf(f, v[j][k].x, x[k].x), x[k].y = fmaf(f, v[j][k].y, x[k].y);
-                x[k].z = fmaf(f, v[j][k].z, x[k].z), x[k].w = fmaf(f, v[j][k].w, x[k].w);
+                for (uint32_t k = 0; k < N; ++k) {
+                    x[k].x = fmaf(f, v[j][k].x, x[k].x), x[k].y = fmaf(f, v[j][k].y, x[k].y);
+                    x[k].z = fmaf(f, v[j][k].z, x[k].z), x[k].w = fmaf(f, v[j][k].w, x[k].w);
+                }
             }
         }
     }
@@ -870,7 +874,16 @@ constexpr uint32_t LEAD_WARPS = 8;
 constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }  // of a CTA, one a SM, by the registers that the kernel needs
 constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
 
+// From so many query rows of a kv head on, the leading pages' kernel is the one of attention_lead.cu, whose time does not depend
+// on them up to 128 (32 query heads on 8 of 128, 8-bit, 64 pages, the kernel alone: 16 rows 34.9 us, here 29.8; 32 rows 28.5 and
+// 28.8; 128 rows 34.6 and 49.0; 512 rows 90.4 and 196.9).
 constexpr uint32_t LEAD_TILE_ROWS = 32;
+// Leading pages are taken once for all sequences where that saves so many elements of keys (positions times dimensions, over all
+// passes) that the launch more and its joining, about 8 us, are won back; below, every sequence reads them by itself, most of it
+// from L2.  32 heads on 8 of 128, 8-bit, 64 pages, batch 8: once 23.7 us, by themselves 19.3; batch 12: 24.0 and 24.3; 16: 24.3
+// and 27.6; 32: 26.0 and 43.6.  Batch 128: 4 pages 34.3 and 27.3, 8 pages 35.8 and 35.0.  Heads of 256 (16 on 4, 64 pages): batch
+// 32 54.0 and 48.8, 64 85.8 and 90.4, 128 149 and 169.
+constexpr double LEAD_SAVES = 32e6;
 
 // How a call is cut up: the same for its scratch and its launches.
 struct PagedPlan {
@@ -886,20 +899,20 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
     p.rows = p.group <= 4 ? 4 : 8;
     p.split = (p.group + p.rows - 1) / p.rows;
     p.grid = (uint32_t)num_sms();
-    p.lead = batch > 1 ? shared : 0;
+    const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
+    p.tiles = hd <= 128 && rows >= LEAD_TILE_ROWS;
+    // passes over the leading pages: a sequence's own is the unit, 128 rows of attention_lead.cu take as long as 5, 16 (heads of
+    // 256: 8) rows of attention_lead_kernel as 2.6 (1.56)
+    const double own = (double)batch * p.split, once = p.tiles ? 5.0 * ((rows + 127) / 128) : (hd == 256 ? 1.56 : 2.6) * tiles;
+    p.lead = (own - once) * n_kv * hd * KV_PAGE * shared >= LEAD_SAVES ? shared : 0;
     if (p.lead) {
-        const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
-        p.tiles = hd <= 128 && rows >= LEAD_TILE_ROWS;
-        p.sets = 1;
+        p.sets = 1, p.cluster = 4;
         while (p.sets < LEAD_WARPS && p.sets < tiles) p.sets *= 2;
         p.blocks = p.tiles ? (rows + 127) / 128 : (tiles + p.sets - 1) / p.sets;
-        // one wave of one CTA a SM.  Clusters of eight leave SMs of the GPU's groups idle (16 of them took two waves), so eight
-        // only where they are few
-        const uint32_t rows_of = std::max(1u, p.blocks * n_kv), fit = std::max(1u, std::min(p.lead, (uint32_t)num_sms() / rows_of));
-        p.cluster = fit >= 24 && 24 * rows_of <= (uint32_t)num_sms() * 2 / 3 ? 8 : 4;
+        // one wave of one CTA a SM
+        const uint32_t fit = std::max(1u, std::min(p.lead, (uint32_t)num_sms() / std::max(1u, p.blocks * n_kv)));
         while (p.cluster > fit) p.cluster /= 2;
-        p.splits = std::min(fit, LEAD_MOST * p.cluster);
-        p.splits = p.splits / p.cluster * p.cluster;
+        p.splits = std::min(fit, LEAD_MOST * p.cluster) / p.cluster * p.cluster;
     }
     p.part_at = ((size_t)batch * n_kv * p.split * 4 + 255) / 256 * 256;
     p.lead_at = p.part_at + ((size_t)p.grid * 2 * p.rows * (hd + 2) * 4 + 255) / 256 * 256;

@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t codes4(uint32_t w) {
     return half2_bits(__hfma2(bits_half2((w & 0x00F000F0u) | 0x64006400u), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)));
 }
 
-constexpr uint32_t LEAD_MOST = 4;  // partial results of the leading pages
+constexpr uint32_t LEAD_MOST = 8;  // partial results of the leading pages
 
 struct PagedArgs {
     KvPages c;

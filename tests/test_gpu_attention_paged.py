@@ -74,6 +74,76 @@ def test_batches(kind, batch, length):
     expect(cache.attend(q, i32(lens), table, n_q=n_q), q, kv, n_q, hd)
 
 
+def long_prompt(kind, hd, n_q, n_kv, batch, shared, seed=3, kv=None):
+    """A common prompt of `shared` pages (seven of them, again and again) and up to three pages of each sequence's own."""
+    import torch
+
+    cache, table = make(kind, n_kv, hd, batch, 10, seed=seed)
+    fill(cache, table, [640] * batch, seed=seed, kv=kv)
+    common = table[0, torch.arange(shared, device="cuda") % 7].expand(batch, shared)
+    table = torch.cat([common, table[:, 7:]], 1).contiguous()
+    lens = [shared * 64 + (0, 1, 64, 100, 130, 192)[b % 6] for b in range(batch)]
+    lens[3] = 0
+    return cache, table, lens, queries(batch, n_q, hd, seed + 1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,n_q,n_kv,batch,shared", [
+    (128, 32, 8, 32, 20), (128, 8, 2, 33, 100), (64, 24, 2, 40, 75), (64, 8, 8, 40, 33), (128, 16, 1, 32, 150), (128, 9, 3, 60, 41), (64, 64, 8, 129, 5),
+    (128, 4, 4, 8, 200), (128, 4, 4, 31, 41), (64, 8, 4, 13, 270), (64, 7, 7, 6, 330), (256, 8, 2, 48, 97), (256, 2, 2, 20, 70), (256, 4, 2, 33, 50)])
+def test_long_shared_prompts(kind, hd, n_q, n_kv, batch, shared):
+    """Prompts that are worth a pass of their own: the same as each sequence by itself."""
+    cache, table, lens, q = long_prompt(kind, hd, n_q, n_kv, batch, shared)
+    got = cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared)
+    for b in sorted({0, 2, 3, batch // 2, batch - 1}):
+        kv = tuple(t.cpu().numpy() for t in cache.read(i32(range(lens[b])), table, seq=i32([b] * lens[b])))
+        expect(got[b:b + 1], q[b:b + 1], [kv], n_q, hd)
+    alone = cache.attend(q, i32(lens), table, n_q=n_q)
+    assert float((got - alone).abs().max()) <= 2 * TOL * 6   # values of these inputs are below 6
+    assert bool((got == cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared)).all())
+    cache.check_flags()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,n_q,n_kv,batch,shared", [(128, 32, 8, 32, 20), (64, 24, 2, 40, 75), (128, 4, 4, 8, 200), (256, 2, 2, 20, 70)])
+def test_long_shared_prompts_that_go_wrong(kind, hd, n_q, n_kv, batch, shared):
+    """Lengths below the prompt, NaN and infinities in it, scores that differ by hundreds, queries of zero, shared pages outside
+    the cache."""
+    def kv(b, k, v):
+        k[7].mul_(20.0)
+
+    cache, table, lens, q = long_prompt(kind, hd, n_q, n_kv, batch, shared, kv=kv)
+    q[4] = 0.0
+    lens[5], lens[2] = shared * 64 - 1, -3
+    got = cache.attend(q, i32(lens), table, n_q=n_q, scale=0.25, shared_pages=shared)
+    assert bool(got[[2, 5]].isnan().all()) and bool((got[3] == 0).all()) and int(cache.bad_pos) == 1
+    for b in (0, 4, batch - 1):
+        held = tuple(t.cpu().numpy() for t in cache.read(i32(range(lens[b])), table, seq=i32([b] * lens[b])))
+        expect(got[b:b + 1], q[b:b + 1], [held], n_q, hd, scale=0.25, tol=20 * TOL)
+    cache.bad_pos.zero_()
+    lens[5], lens[2] = shared * 64 + 1, shared * 64
+    bad = queries(1, 3 * n_kv, hd, 9)
+    cache.append(bad, i32([70]), table, n_q=n_kv, seq=i32([0]))
+    fine = cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared)
+    bad[0, n_kv * hd] = np.nan                       # a key of kv head 0, a value of the last one
+    bad[0, 3 * n_kv * hd - 1] = np.inf
+    cache.append(bad, i32([70]), table, n_q=n_kv, seq=i32([0]))
+    got = cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared).reshape(batch, n_q, hd)
+    group = n_q // n_kv
+    held = cache.read(i32([70]), table, seq=i32([0]))
+    live = [b for b in range(batch) if b != 3]
+    assert bool(got[live, :group].isnan().all()) and bool((got[3] == 0).all())
+    lost = held[1][n_kv - 1, 0].isnan()
+    assert bool((got[live][:, n_q - group:].isnan() == lost).all()) and bool(lost.any())
+    if n_kv > 2:
+        assert bool((got[:, group:n_q - group] - fine.reshape(batch, n_q, hd)[:, group:n_q - group]).abs().max() <= 2 * TOL * 6)
+    assert int(cache.bad_pos) == 0
+    for page in (-1, cache.pages.shape[0]):
+        table[:, shared // 2] = page
+        got = cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared)
+        assert bool(got[live].isnan().all()) and bool((got[3] == 0).all()) and int(cache.bad_pos) == 1
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("hd,n_q,n_kv,batch,shared", [(128, 8, 2, 5, 1), (128, 32, 8, 32, 3), (64, 8, 2, 33, 4), (256, 8, 2, 9, 2),
                                                       (64, 4, 4, 2, 9), (128, 9, 3, 7, 5), (128, 16, 1, 3, 2), (64, 8, 8, 130, 1), (128, 32, 8, 100, 9),
