@@ -431,7 +431,7 @@ int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32
 /* Attention of one new token per sequence: out[b, h] = softmax(scale q[b, h] . K[0 .. len[b]) ^T) V, query head h on kv head
  * h / (n_q / n_kv); scale 0: 1 / sqrt(head_dim).  q and out rows are q_stride and out_stride floats apart.  len[b] = 0: zeros.
  *   shared_pages: the first so many pages are the same for the whole batch (a common prompt): read from the first sequence's
- * table entries, once for all.  Every len is then 0 or at least shared_pages * JQ_KV_PAGE.
+ * table entries, and once for all where that is the faster way.  Every len is then 0 or at least shared_pages * JQ_KV_PAGE.
  *   A len outside its range or a page id outside the cache makes the sequence's rows NaN and sets *bad_pos_dev.
  *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, ZEROED once before the first
  * call (it holds arrival counters that the kernels leave at zero); one call at a time. */

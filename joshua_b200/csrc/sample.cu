@@ -612,9 +612,10 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
 }  // namespace
 
 cudaError_t launch_sample(const SampleArgs& a, uint32_t rows, cudaStream_t s) {
-    // 4096 logits a CTA or more, eight CTAs a row; sixteen (beyond what every device promises) while the rows are few
+    // 2048 logits a CTA or more (one row of 32000, top-p: 16.5 us, with 4096 18.5), eight CTAs a row; sixteen (beyond what every
+    // device promises) while the rows are few: one row of 128256 27 us (eight: 36), 64 rows 84 with eight and 139 with sixteen
     uint32_t ctas = 1;
-    while (ctas < (rows * SM_MOST_CTAS <= (uint32_t)num_sms() ? SM_MOST_CTAS : SM_CTAS) && a.vocab > ctas * 4096) ctas *= 2;
+    while (ctas < (rows * SM_MOST_CTAS <= (uint32_t)num_sms() ? SM_MOST_CTAS : SM_CTAS) && a.vocab > ctas * 2048) ctas *= 2;
     const size_t smem = ((a.vocab + 3 + 3) / 4 + ctas - 1) / ctas * 16;  // of a row that begins inside a vector
     static bool configured[MAX_DEVICES] = {};
     if (cudaError_t e = set_max_smem_once(sample_kernel, SAMPLE_MAX_VOCAB / SM_CTAS * 4 + 16, configured); e != cudaSuccess) return e;

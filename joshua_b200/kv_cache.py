@@ -2,7 +2,8 @@
 into it, positions read back, attention of one new token per sequence over it.
 
 The caller owns the page table (int32 [sequences, pages a sequence]): position p of sequence i is in page `table[i, p // 64]`.
-Sequences may share leading pages (a common prompt); `attend(shared_pages=n)` then reads and multiplies them once for the batch.
+Sequences may share leading pages (a common prompt); `attend(shared_pages=n)` then reads and multiplies them once for the batch where
+that is the faster way.
 """
 from __future__ import annotations
 
