@@ -13,6 +13,12 @@
 //            of the step's largest scale, in two f16 terms (22 bits below the largest).  Accumulators hold a step, not the
 //            sequence: the tensor core adds with truncation, the running output is added round-to-nearest.
 // Up to four query rows stand as four pairs of columns (term, term): one product does both terms.
+//
+// Every code is read once and serves all query heads of its kv head.  Long batches are bound by memory: 64 sequences of up to
+// 8192 positions, 32 heads on 8 of 128 in eight bits, 568 MB in 103 us (5.5 TB/s, 84% of a copy), with 48% of the issue slots.
+// Four bits are bound by instructions (24 sequences of up to 16384, 32 heads on 4 of 128, 84 MB: 42 us; 50% of the issue slots by
+// three warps a scheduler, whose chains of product, softmax and product leave the rest), short batches by the chain of one
+// piece (one sequence of 1000: 10 us, of which about 1 the cut, 4 the steps, 5 the joining within and across CTAs).
 #include <cooperative_groups.h>
 
 #include "attention_paged.cuh"
@@ -559,6 +565,8 @@ struct Joined {
     }
 };
 
+// A segment's beginning and end in steps (1 / 2 / 3 / 4: 64 sequences of up to 8192 107.4 / 101.4 / 101.5 / 101.6 us, 512 of up to
+// 200 45.2 / 41.2 / 42.0 / 43.6; its kernel alone).
 constexpr uint32_t SEG_UNITS = 2;
 
 // Positions of a sequence's own (behind the leading pages), or -1 where its length is out of range.
@@ -795,7 +803,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
 }
 
 // The leading pages, once for all sequences: query rows of the batch (of one kv head) are the columns, NT * 8 a warp.  A CTA's
-// warps take `sets` sets of rows and WARPS / sets parts of the CTA's share of the pages.
+// warps take `sets` sets of rows and WARPS / sets parts of the CTA's share of the pages.  Bound by instructions, as the kernel
+// above: a pass of 16 rows takes 2.6 times as long as a sequence's own pass of four over the same positions, and serves more
+// (7 sequences of 32 heads on 8 of 128 in halves, 1024 pages: 101 us, by themselves 299).
 template <class T, uint32_t NT, uint32_t WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) attention_lead_kernel(PagedArgs a, float* __restrict__ lead, uint32_t sets) {
     using At = Attend<T, NT, false>;
@@ -871,8 +881,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_lead_kernel(PagedArgs
 }
 
 constexpr uint32_t LEAD_WARPS = 8;
-constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }  // of a CTA, one a SM, by the registers that the kernel needs
-constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }
+// Warps of a CTA, one a SM, by the registers that a step needs (64 sequences of up to 8192, heads of 128: 10 warps 108.9 us, 12
+// 106.0, 16, which spill, 120.9).
+constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }
+constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }  // columns of a warp / 8, by its registers too
 
 // From so many query rows of a kv head on, the leading pages' kernel is the one of attention_lead.cu, whose time does not depend
 // on them up to 128 (32 query heads on 8 of 128, 8-bit, 64 pages, the kernel alone: 16 rows 34.9 us, here 29.8; 32 rows 28.5 and
@@ -909,7 +921,8 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
         p.sets = 1, p.cluster = 4;
         while (p.sets < LEAD_WARPS && p.sets < tiles) p.sets *= 2;
         p.blocks = p.tiles ? (rows + 127) / 128 : (tiles + p.sets - 1) / p.sets;
-        // one wave of one CTA a SM
+        // one wave of one CTA a SM.  Clusters of four: of eight, SMs of the GPU's groups stay idle, and 16 of them took two waves (16
+        // heads on 4 of 128, batch 32, 256 pages: 54.6 us, 12 of eight 37.2, 32 of four 32.1)
         const uint32_t fit = std::max(1u, std::min(p.lead, (uint32_t)num_sms() / std::max(1u, p.blocks * n_kv)));
         while (p.cluster > fit) p.cluster /= 2;
         p.splits = std::min(fit, LEAD_MOST * p.cluster) / p.cluster * p.cluster;

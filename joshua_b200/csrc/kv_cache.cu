@@ -1,5 +1,10 @@
 // The paged cache: new positions' keys and values rounded into their pages, keys and queries rotated on the way; positions
 // read back as f32 rows.
+//
+// A block of 32 dimensions x becomes codes rint(x / d) under one scale d (kv_round), queries and keys (a cos - b sin, a sin + b
+// cos) before.  Each f32 row is read once, queries written once, codes once: many rows are bound by memory (4096 rows of 32
+// query heads on 8 of 64 in halves, 92 MB in 22.6 us; 1000 rows of 32 on 4 of 128 in four bits, 11.9), few by the chain from a row's
+// position to its page (32 rows 3.2 us, launch included).
 #include "kv_pages.cuh"
 #include "serving.cuh"
 
@@ -470,8 +475,15 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int3
         read_rows<KIND, HD, false>(c, pos, seq, rows, g, head, k + head * head_stride, row_stride, bad_pos);
 }
 
-// From so many rows on, 16 rows a warp: below, a row's latency counts.
-constexpr uint32_t MANY_ROWS = 768, QUERY_WARPS = 32;
+// From so many rows on, runs of 16 positions are put together, where rows may stand in runs (each row another sequence's: never).
+// 1000 rows of a prompt, 32 query heads on 8 of 128, eight bits: 10.8 us, a warp a row 15.3; 4096 rows 46 and 67; 512 rows 9.3 and
+// 9.3; 24 heads on 8 of 64 in halves, 1000 rows 8.3 and 7.8, 4096 rows 16.3 and 24.6.  Reading back, 8 heads of 128: 1000 rows 4.8
+// and 5.3, 512 rows 4.7 and 4.4.  Heads of 256 always a warp a row: a run's registers leave too few warps a SM (4096 rows read
+// 14.1 and 8.6).
+constexpr uint32_t MANY_ROWS = 768;
+// Queries: warps a SM, with one head's worth each, from which on a warp takes more heads of its row (1000 rows, 16 heads of 256:
+// 16 warps 10.4 us, 32 9.4, 64 9.7, 128 11.1).
+constexpr uint32_t QUERY_WARPS = 32;
 
 struct LaunchAppend {
     const AppendArgs& a;
