@@ -568,6 +568,10 @@ struct Joined {
 // A segment's beginning and end in steps (1 / 2 / 3 / 4: 64 sequences of up to 8192 107.4 / 101.4 / 101.5 / 101.6 us, 512 of up to
 // 200 45.2 / 41.2 / 42.0 / 43.6; its kernel alone).
 constexpr uint32_t SEG_UNITS = 2;
+// Where no segment has more than so many units for each warp of a CTA, CTAs take whole segments, and none is joined across CTAs (32
+// heads on 8 of 128, 8-bit, 4 sequences of 500: 9.8 us, cut anywhere 11.0; 512 of up to 200 39.5 and 41.2; one of 300 7.9 and 7.5.
+// With 3 units: 16 sequences of 1000 15.3 us, cut anywhere 13.5).
+constexpr uint32_t WHOLE_UNITS = 2;
 
 // Positions of a sequence's own (behind the leading pages), or -1 where its length is out of range.
 __device__ __forceinline__ int32_t own_positions(const PagedArgs& a, uint32_t b) {
@@ -577,15 +581,15 @@ __device__ __forceinline__ int32_t own_positions(const PagedArgs& a, uint32_t b)
 }
 
 // The sequences' work stands in one row of units: sequence by sequence, head group by head group, SEG_UNITS for beginning and
-// ending a segment (its queries, its result), then its steps.  It is cut into equal pieces, one a warp, whatever the lengths; a
-// CTA's warps have neighbouring ones.  Pieces of one segment (sequence, head group) are joined
-// within the CTA, then, where a segment spans CTAs, by the last one of them to arrive, in order.
+// ending a segment (its queries, its result), then its steps.  It is cut into equal pieces, one a warp, whatever the lengths (short
+// segments: first into CTAs' whole ones); a CTA's warps have neighbouring pieces.  Pieces of one segment (sequence, head group) are
+// joined within the CTA, then, where a segment spans CTAs, by the last one of them to arrive, in order.
 template <class T, bool PAIRS, uint32_t WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArgs a) {
     using At = Attend<T, 1, PAIRS>;
     constexpr uint32_t HD = T::HD, ROWS = At::Q::ROWS, PIECE = ROWS * (HD + 2);
     extern __shared__ __align__(16) uint32_t s_mem[];
-    __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_last[2], s_first[2];
+    __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_most[WARPS], s_last[2], s_first[2];
     uint32_t* s_cum = s_mem;                                                       // [batch + 1] units of a head group in front of a sequence
     float* s_piece = reinterpret_cast<float*>(s_mem + ((a.c.n_seq + 4) & ~3u));    // [WARPS][2][PIECE]
     uint32_t* s_q = reinterpret_cast<uint32_t*>(s_piece + WARPS * 2 * PIECE);      // [WARPS] query operands
@@ -594,21 +598,25 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     if (tid < 2 * WARPS) s_seg[tid] = 0xFFFFFFFFu;
     // running sum of the sequences' units, a run of sequences a thread
     const uint32_t per = (batch + WARPS * 32 - 1) / (WARPS * 32), b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
-    uint32_t mine = 0;
+    uint32_t mine = 0, most = 0;
     auto units_of = [&](uint32_t b) {
         const uint32_t steps = (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
         return steps ? steps + SEG_UNITS : 0;
     };
-    for (uint32_t b = b0; b < b1; ++b) mine += units_of(b);
+    for (uint32_t b = b0; b < b1; ++b) {
+        const uint32_t n = units_of(b);
+        mine += n, most = max(most, n);
+    }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
     uint32_t run = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t up = __shfl_up_sync(0xFFFFFFFFu, run, o);
         run += lane >= o ? up : 0;
     }
-    if (lane == 31) s_scan[warp] = run;
+    if (lane == 31) s_scan[warp] = run, s_most[warp] = most;
     __syncthreads();
-    for (uint32_t w = 0; w < warp; ++w) run += s_scan[w];
+    for (uint32_t w = 0; w < WARPS; ++w) run += w < warp ? s_scan[w] : 0, most = max(most, s_most[w]);
     run -= mine;
     for (uint32_t b = b0; b < b1; ++b) {
         s_cum[b] = run;
@@ -619,9 +627,30 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
 
     const uint64_t total = (uint64_t)s_cum[batch] * groups;
     const uint64_t workers = min((uint64_t)gridDim.x * WARPS, total);
-    const uint64_t me = (uint64_t)blockIdx.x * WARPS + warp;
-    uint64_t at = me < workers ? me * total / workers : 0;
-    const uint64_t end = me < workers ? (me + 1) * total / workers : 0;
+    auto sequence_at = [&](uint64_t x) {  // the last sequence that begins at or in front of unit x: it has units
+        uint32_t lo = 0, hi = batch;
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            (uint64_t)s_cum[mid] * groups <= x ? lo = mid : hi = mid;
+        }
+        return lo;
+    };
+    uint64_t at = 0, end = 0;
+    if (most <= WHOLE_UNITS * WARPS) {  // the same in all CTAs; units fit 32 bits then
+        static_assert((uint64_t)ATTENTION_MAX_BATCH * 4096 * WHOLE_UNITS * WARPS < 0xFFFFFFFFull, "units of 4096 heads a sequence");
+        const uint32_t n = (uint32_t)total, each = n / gridDim.x, more = n % gridDim.x;
+        auto begins = [&](uint32_t cta) {  // the segment that its first unit is in
+            const uint32_t x = cta * each + cta * more / gridDim.x;
+            if (x >= n) return n;
+            const uint32_t b = sequence_at(x), first = s_cum[b] * groups, all = s_cum[b + 1] - s_cum[b];
+            return first + (x - first) / all * all;
+        };
+        const uint32_t c0 = begins(blockIdx.x), units = begins(blockIdx.x + 1) - c0, warps = min(WARPS, units);
+        if (warp < warps) at = c0 + warp * units / warps, end = c0 + (warp + 1) * units / warps;
+    } else {
+        const uint64_t me = (uint64_t)blockIdx.x * WARPS + warp;
+        if (me < workers) at = me * total / workers, end = (me + 1) * total / workers;
+    }
     At w;
     bool first_piece = true;
     // a piece of work: steps u0 .. u1 (perhaps none) of the `steps` of a sequence and head group
@@ -658,13 +687,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
         return p;
     };
     Piece p{};
-    if (at < end) {  // the last sequence that begins at or in front of it
-        uint32_t lo = 0, hi = batch;
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            (uint64_t)s_cum[mid] * groups <= at ? lo = mid : hi = mid;
-        }
-        p = take(lo);
+    if (at < end) {
+        p = take(sequence_at(at));
         if (p.u0 < p.u1) begin(p);
     }
     while (p.u0 < p.u1) {

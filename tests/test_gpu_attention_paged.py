@@ -169,6 +169,20 @@ def test_shared_pages(kind, hd, n_q, n_kv, batch, shared):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,n_q,n_kv", [(64, 8, 1), (128, 4, 4), (128, 16, 2), (128, 9, 1), (256, 8, 2), (256, 6, 1)])
+def test_sequences_that_span_ctas(kind, hd, n_q, n_kv):
+    """Some cut between CTAs, some whole in one, some with nothing; the same answer again from the same scratch."""
+    lens = [3001, 1, 0, 1999, 703, 64, 1600]
+    cache, table = make(kind, n_kv, hd, len(lens), 47, seed=n_q)
+    kv = fill(cache, table, lens, seed=hd)
+    q = queries(len(lens), n_q, hd, 3)
+    got = cache.attend(q, i32(lens), table, n_q=n_q)
+    expect(got, q, kv, n_q, hd)
+    for _ in range(3):
+        assert bool((got == cache.attend(q, i32(lens), table, n_q=n_q)).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_a_long_sequence(kind):
     """Many splits, a batch of very unlike lengths."""
     n_q, n_kv, hd, lens = 8, 2, 64, [30011, 3, 0, 64 * 40, 1]
