@@ -219,49 +219,59 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t ite
     const uint32_t l = (threadIdx.x & 31) % LANES, group = (threadIdx.x & 31) / LANES, half = r.rot / 2;
     const bool turned = r.table != nullptr && 8 * l < r.rot, split = turned && !r.interleaved;
     const uint32_t at_u = split ? 4 * l : 8 * l, at_v = split ? half + 4 * l : 8 * l + 4;
-    float4 next_u = make_float4(0.0f, 0.0f, 0.0f, 0.0f), next_v = next_u;
-    auto request = [&](uint32_t head) {
-        if (head >= end) return;
-        next_u = __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_u));
-        next_v = __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_v));
+    constexpr uint32_t AHEAD = 2;  // heads a lane has on their way
+    float4 next_u[AHEAD], next_v[AHEAD];
+    auto request = [&](uint32_t first) {
+#pragma unroll
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            const uint32_t head = first + i * AT_ONCE + group;
+            const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            next_u[i] = head < end ? __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_u)) : zero;
+            next_v[i] = head < end ? __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_v)) : zero;
+        }
     };
-    request(head0 + group);
+    request(head0);
     if (a.page(row, 0) == nullptr) return;
-    float4 cs0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), cs1 = cs0, wu, wv;
+    float4 cs0 = make_float4(1.0f, 0.0f, 1.0f, 0.0f), cs1 = cs0;
     if (turned) {
         const float4* t = reinterpret_cast<const float4*>(r.table + (uint64_t)(uint32_t)a.pos[row] * half + 4 * l);
         cs0 = __ldg(t), cs1 = __ldg(t + 1);
     }
-    if (a.q_norm) wu = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_u)), wv = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_v));
-    for (uint32_t h = head0 + group; h < end + group; h += AT_ONCE) {
-        float u[4] = {next_u.x, next_u.y, next_u.z, next_u.w}, v[4] = {next_v.x, next_v.y, next_v.z, next_v.w};
-        request(h + AT_ONCE);
-        if (a.q_norm) {
-            float ss = 0.0f;
+    for (uint32_t first = head0; first < end; first += AHEAD * AT_ONCE) {
+        if (first != head0) request(first);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
+        for (uint32_t i = 0; i < AHEAD; ++i) {
+            if (first + i * AT_ONCE >= end) break;  // the same in the warp
+            const uint32_t h = first + i * AT_ONCE + group;
+            float u[4] = {next_u[i].x, next_u[i].y, next_u[i].z, next_u[i].w}, v[4] = {next_v[i].x, next_v[i].y, next_v[i].z, next_v[i].w};
+            if (a.q_norm) {
+                float ss = 0.0f;
 #pragma unroll
-            for (uint32_t o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-            const float sc = rsqrtf(ss / (float)HD + a.eps);
-            u[0] = u[0] * sc * wu.x, u[1] = u[1] * sc * wu.y, u[2] = u[2] * sc * wu.z, u[3] = u[3] * sc * wu.w;
-            v[0] = v[0] * sc * wv.x, v[1] = v[1] * sc * wv.y, v[2] = v[2] * sc * wv.z, v[3] = v[3] * sc * wv.w;
-        }
-        if (turned) {
-            const float2 cs[4] = {make_float2(cs0.x, cs0.y), make_float2(cs0.z, cs0.w), make_float2(cs1.x, cs1.y), make_float2(cs1.z, cs1.w)};
-            auto turn = [](float& x, float& y, float2 by) {
-                const float first = rope_rotate(true, x, y, by);
-                y = rope_rotate(false, y, x, by), x = first;
-            };
-            if (split) {
+                for (int e = 0; e < 4; ++e) ss = fmaf(u[e], u[e], fmaf(v[e], v[e], ss));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) turn(u[e], v[e], cs[e]);
-            } else {
-                turn(u[0], u[1], cs[0]), turn(u[2], u[3], cs[1]), turn(v[0], v[1], cs[2]), turn(v[2], v[3], cs[3]);
+                for (uint32_t o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+                const float4 wu = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_u)), wv = __ldg(reinterpret_cast<const float4*>(a.q_norm + at_v));
+                const float sc = rsqrtf(ss / (float)HD + a.eps);
+                u[0] = u[0] * sc * wu.x, u[1] = u[1] * sc * wu.y, u[2] = u[2] * sc * wu.z, u[3] = u[3] * sc * wu.w;
+                v[0] = v[0] * sc * wv.x, v[1] = v[1] * sc * wv.y, v[2] = v[2] * sc * wv.z, v[3] = v[3] * sc * wv.w;
             }
+            if (turned) {
+                const float2 cs[4] = {make_float2(cs0.x, cs0.y), make_float2(cs0.z, cs0.w), make_float2(cs1.x, cs1.y), make_float2(cs1.z, cs1.w)};
+                auto turn = [](float& x, float& y, float2 by) {
+                    const float first = rope_rotate(true, x, y, by);
+                    y = rope_rotate(false, y, x, by), x = first;
+                };
+                if (split) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) turn(u[e], v[e], cs[e]);
+                } else {
+                    turn(u[0], u[1], cs[0]), turn(u[2], u[3], cs[1]), turn(v[0], v[1], cs[2]), turn(v[2], v[3], cs[3]);
+                }
+            }
+            if (h >= end) continue;
+            *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_u) = make_float4(u[0], u[1], u[2], u[3]);
+            *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_v) = make_float4(v[0], v[1], v[2], v[3]);
         }
-        if (h >= end) continue;
-        *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_u) = make_float4(u[0], u[1], u[2], u[3]);
-        *reinterpret_cast<float4*>(dst + (uint64_t)h * HD + at_v) = make_float4(v[0], v[1], v[2], v[3]);
     }
 }
 
