@@ -3,7 +3,7 @@
 //
 // A block of 32 dimensions x becomes codes rint(x / d) under one scale d (kv_round), queries and keys (a cos - b sin, a sin + b
 // cos) before.  Each f32 row is read once, queries written once, codes once: many rows are bound by memory (4096 rows of 32
-// query heads on 8 of 64 in halves, 92 MB in 22.6 us; 1000 rows of 32 on 4 of 128 in four bits, 11.9), few by the chain from a row's
+// query heads on 8 of 64 in halves, 92 MB in 21.8 us; 1000 rows of 32 on 4 of 128 in four bits, 12.0), few by the chain from a row's
 // position to its page (32 rows 3.2 us, launch included).
 #include "kv_pages.cuh"
 #include "serving.cuh"
@@ -219,7 +219,8 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t ite
     const uint32_t l = (threadIdx.x & 31) % LANES, group = (threadIdx.x & 31) / LANES, half = r.rot / 2;
     const bool turned = r.table != nullptr && 8 * l < r.rot, split = turned && !r.interleaved;
     const uint32_t at_u = split ? 4 * l : 8 * l, at_v = split ? half + 4 * l : 8 * l + 4;
-    constexpr uint32_t AHEAD = 2;  // heads a lane has on their way
+    // heads a lane has on their way (4096 rows of 32 and 2 x 4 heads of 128: one 33.9 us, two 31.7, three 32.2, four, which spill, 32.6)
+    constexpr uint32_t AHEAD = 2;
     float4 next_u[AHEAD], next_v[AHEAD];
     auto request = [&](uint32_t first) {
 #pragma unroll
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int3
 }
 
 // From so many rows on, runs of 16 positions are put together, where rows may stand in runs (each row another sequence's: never).
-// 1000 rows of a prompt, 32 query heads on 8 of 128, eight bits: 10.8 us, a warp a row 15.3; 4096 rows 46 and 67; 512 rows 9.3 and
+// 1000 rows of a prompt, 32 query heads on 8 of 128, eight bits: 10.8 us, a warp a row 15.3; 4096 rows 46 and 67 (44 now); 512 rows 9.3 and
 // 9.3; 24 heads on 8 of 64 in halves, 1000 rows 8.3 and 7.8, 4096 rows 16.3 and 24.6.  Reading back, 8 heads of 128: 1000 rows 4.8
 // and 5.3, 512 rows 4.7 and 4.4.  Heads of 256 always a warp a row: a run's registers leave too few warps a SM (4096 rows read
 // 14.1 and 8.6).
