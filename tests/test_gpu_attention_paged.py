@@ -243,6 +243,31 @@ def test_values_that_are_not_finite_show(kind):
     assert np.nanmax(np.abs(got - want)) <= TOL * 6
 
 
+@pytest.mark.parametrize("shared", [0, 45])
+def test_a_pool_past_32_bits(shared):
+    """Pages from 4 GB on: appended, read and attended, by themselves and as a common prompt."""
+    import torch
+
+    from joshua_b200.kv_cache import PagedCache
+
+    n_q, n_kv, hd, batch, per = 16, 8, 128, 32, 48
+    n_pages = 2**32 // (n_kv * 2 * 64 * (hd + hd // 16)) + batch * per
+    cache = PagedCache("q8_0", n_kv, hd, n_pages=n_pages, device="cuda")
+    assert (n_pages - batch * per + 1) * cache.page_bytes > 2**32
+    table = (n_pages - 1 - torch.randperm(batch * per, device="cuda")).int().reshape(batch, per)
+    if shared:
+        table[:, :shared] = table[0, :shared].clone()
+    lens = [(shared or 40) * 64 + 3 * b for b in range(batch)]
+    kv = fill(cache, table, lens, seed=5)
+    q = queries(batch, n_q, hd, 6)
+    got = cache.attend(q, i32(lens), table, n_q=n_q, shared_pages=shared)
+    for b in (0, 7, batch - 1):
+        held = tuple(t.cpu().numpy() for t in cache.read(i32(range(lens[b])), table, seq=i32([b] * lens[b])))
+        assert shared or all(np.array_equal(x, y) for x, y in zip(held, kv[b]))
+        expect(got[b:b + 1], q[b:b + 1], [held], n_q, hd)
+    cache.check_flags()
+
+
 def test_lengths_and_pages_without_a_place():
     import torch
 
