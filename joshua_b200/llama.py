@@ -286,6 +286,10 @@ class LlamaDecoder:
         return self.weight_bytes + io
 
     # ── the model-level call with host buffers ──────────────────────────
+    def _launches(self, stream) -> None:
+        """What the host call captures: a step's launches."""
+        self.step(stream)
+
     def forward_host(self, token_ids, out_logits=None):
         """`ModelWeights::forward(input_ids, index_pos) -> logits` for one new token per sequence with HOST
         buffers on both sides (the shape of the reference's model call, src/model.rs:362-364): the token ids
@@ -299,11 +303,11 @@ class LlamaDecoder:
             log_pin = torch.empty(self.batch, self.cfg.vocab, dtype=torch.float32).pin_memory()
             with torch.cuda.stream(stream):
                 pos0 = self.pos.clone()
-                self.step(stream.cuda_stream)      # warm-up outside the capture (scratch allocation)
+                self._launches(stream.cuda_stream)   # warm-up outside the capture (scratch allocation)
                 stream.synchronize()
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph, stream=stream):
-                    self.step(stream.cuda_stream)
+                    self._launches(stream.cuda_stream)
                 self.pos.copy_(pos0)
                 stream.synchronize()
             self._host = (stream, tok_pin, log_pin, graph)

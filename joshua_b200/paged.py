@@ -31,7 +31,9 @@ class _Paged:
         self.n_pages = batch * self.pages_per_seq if n_pages is None else n_pages
         super().__init__(cfg, device, batch=batch, max_ctx=max_ctx, **more)
         self.rope = rope or Rope(rope_table(cfg.rope_theta, cfg.head_dim, max_ctx, self.dev))
-        self.table = torch.zeros(batch, self.pages_per_seq, dtype=torch.int32, device=self.dev)
+        # -1: no page.  A row never names a page that its sequence does not hold, so whatever still runs with the row of a sequence
+        # that ended (a graph) raises the caches' flag instead of writing into another sequence's page.
+        self.table = torch.full((batch, self.pages_per_seq), -1, dtype=torch.int32, device=self.dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)
         self.free = list(range(self.n_pages))[::-1]
         self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
@@ -67,6 +69,7 @@ class _Paged:
             if not any(page in other for i, other in enumerate(self.owned) if i != sequence):
                 self.free.append(page)
         self.owned[sequence], self.held[sequence] = [], 0
+        self.table[sequence] = -1
         self.pos[sequence] = 0
         self.shared_pages = 0   # not all sequences have them any more
 
@@ -144,11 +147,18 @@ class _Paged:
         now = torch.cuda.current_stream(self.dev).cuda_stream
         if stream is not None and stream != now:
             raise JoshuaB200Error(_lib.E_INVALID, "a paged decoder's step runs on the current stream")
+        self._advance()
+        self._launches(now)
+
+    def _advance(self) -> None:
+        """Counts one position more of every sequence, with a page for it."""
         for i in range(self.batch):
             self.reserve(i, self.held[i] + 1)
             self.held[i] += 1
+
+    def _launches(self, stream) -> None:
         torch.add(self.pos, 1, out=self.lens)
-        super().step(now)
+        super().step(stream)
 
     def _attend(self, ly, s) -> None:
         c, cache = self.cfg, ly["cache"]
@@ -170,13 +180,15 @@ class _Paged:
                pos=self.pos[rows], token=self.token[rows])
 
     def forward_host(self, token_ids, out_logits=None):
-        if getattr(self, "_host", None) is None:
-            for i in range(self.batch):
-                self.reserve(i, self.max_ctx)
+        token_ids = torch.as_tensor(token_ids, dtype=torch.int32).reshape(self.batch)
         held = list(self.held)
-        logits = super().forward_host(token_ids, out_logits)
-        self.held = [n + 1 for n in held]   # the graph's capture walked through step() too
-        return logits
+        self._advance()
+        self._host_calls = 0   # each sequence's own positions are the limit
+        try:
+            return super().forward_host(token_ids, out_logits)
+        except Exception:
+            self.held = held
+            raise
 
     def check_flags(self) -> None:
         super().check_flags()

@@ -1,0 +1,93 @@
+"""The decoders over pages in the life of a server: sequences that end and begin again, host calls, callers' graphs, refusals.
+
+Every decoder is compared with a twin that reached the same tokens by single steps or prompts of its own, in the same pieces, so that
+the same rows go through the same kernels; page ids differ, and no result depends on them.  What is left are the sums of f32 that a
+batch of another size takes in another order (1e-4 of a logit's size, as in the tests beside these).
+"""
+import numpy as np
+import pytest
+
+from joshua_b200._lib import JoshuaB200Error
+from tests.test_gpu_paged_decoder import ids, make, near
+
+pytestmark = pytest.mark.gpu
+
+
+def whole(dec):
+    """Every page is free or somebody's, none both; rows of the table name their owner's pages and no others."""
+    owned = {p for mine in dec.owned for p in mine}
+    assert sorted(owned | set(dec.free)) == list(range(dec.n_pages)) and not owned & set(dec.free) and len(set(dec.free)) == len(dec.free)
+    for row, mine in zip(dec.table.tolist(), dec.owned):
+        assert row[:len(mine)] == mine and not set(row[len(mine):]) & set(range(dec.n_pages))
+
+
+def host_and_step(dec, twin, rows):
+    """The same tokens by host calls and by steps."""
+    import torch
+
+    for row in rows:
+        got = dec.forward_host(row)
+        twin.token.copy_(torch.tensor(row, dtype=torch.int32))
+        twin.step()
+        near(torch.from_numpy(np.array(got)), twin.logits)
+
+
+def tokens(n, batch, seed):
+    return np.random.RandomState(seed).randint(0, 2048, (n, batch)).tolist()
+
+
+def test_host_calls_behind_a_reset():
+    """The pages of sequences that ended are others' by then."""
+    dec, twin = make(2, max_ctx=256), make(2, max_ctx=256)
+    dec.forward_host([1, 2])
+    dec.reset()
+    for d in (dec, twin):
+        d.prefill(ids(130, 1), sequence=0)
+        d.prefill(ids(10, 2), sequence=1)
+    whole(dec)
+    host_and_step(dec, twin, tokens(60, 2, 3))
+    whole(dec)
+    assert dec.held == [190, 70] and dec.pos.tolist() == [190, 70]
+    dec.check_flags()
+
+
+def test_a_prompt_behind_host_calls():
+    dec, twin = make(2), make(2)
+    dec.forward_host([5, 6])
+    dec.reset()
+    host_and_step(dec, twin, tokens(3, 2, 4))
+    for d in (dec, twin):
+        d.prefill(ids(70, 5), sequence=1)
+    near(dec.logits[1], twin.logits[1])
+    host_and_step(dec, twin, tokens(2, 2, 6))
+    whole(dec)
+
+
+def test_host_calls_to_the_last_position():
+    dec = make(1, max_ctx=66)
+    dec.prefill(ids(65, 1))
+    dec.forward_host([3])
+    assert dec.held == [66]
+    with pytest.raises(JoshuaB200Error):
+        dec.forward_host([4])
+    with pytest.raises(RuntimeError):
+        dec.forward_host([4, 5])       # refused before anything is counted
+    dec.release(0)
+    dec.prefill(ids(3, 1))
+    for _ in range(63):                # the calls before the release do not count
+        dec.forward_host([4])
+    assert dec.held == [66] and dec.pos.tolist() == [66]
+    dec.check_flags()
+
+
+def test_a_released_row_names_no_page():
+    dec = make(3, max_ctx=256)
+    whole(dec)
+    for i in range(3):
+        dec.prefill(ids(100, i), sequence=i)
+    dec.release(1)
+    whole(dec)
+    dec.prefill(ids(130, 7), sequence=1)
+    whole(dec)
+    dec.reset()
+    whole(dec)
