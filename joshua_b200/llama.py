@@ -290,6 +290,20 @@ class LlamaDecoder:
         """What the host call captures: a step's launches."""
         self.step(stream)
 
+    def _capture(self, stream):
+        """A step's launches as a graph; they have run once before, at the positions of the next step."""
+        torch = self.torch
+        with torch.cuda.stream(stream):
+            pos0 = self.pos.clone()
+            self._launches(stream.cuda_stream)   # warm-up outside the capture (scratch allocation)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                self._launches(stream.cuda_stream)
+            self.pos.copy_(pos0)
+            stream.synchronize()
+        return graph
+
     def forward_host(self, token_ids, out_logits=None):
         """`ModelWeights::forward(input_ids, index_pos) -> logits` for one new token per sequence with HOST
         buffers on both sides (the shape of the reference's model call, src/model.rs:362-364): the token ids
@@ -301,16 +315,7 @@ class LlamaDecoder:
             stream = torch.cuda.Stream(self.dev)
             tok_pin = torch.empty(self.batch, dtype=torch.int32).pin_memory()
             log_pin = torch.empty(self.batch, self.cfg.vocab, dtype=torch.float32).pin_memory()
-            with torch.cuda.stream(stream):
-                pos0 = self.pos.clone()
-                self._launches(stream.cuda_stream)   # warm-up outside the capture (scratch allocation)
-                stream.synchronize()
-                graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph, stream=stream):
-                    self._launches(stream.cuda_stream)
-                self.pos.copy_(pos0)
-                stream.synchronize()
-            self._host = (stream, tok_pin, log_pin, graph)
+            self._host = (stream, tok_pin, log_pin, self._capture(stream))
             self._host_calls = int(self.pos.max().item())
         stream, tok_pin, log_pin, graph = self._host
         if self._host_calls >= self.max_ctx:

@@ -179,12 +179,24 @@ class _Paged:
                window=self.window[rows] if penalised else None, window_state=self.window_state[rows] if penalised else None,
                pos=self.pos[rows], token=self.token[rows])
 
+    def _frozen(self):
+        """What a captured step keeps as it was: the host call captures another one when it changes."""
+        return self.shared_pages
+
+    def _capture(self, stream):
+        frozen = self._frozen()
+        graph = super()._capture(stream)
+        self._captured_with = frozen
+        return graph
+
     def forward_host(self, token_ids, out_logits=None):
         token_ids = torch.as_tensor(token_ids, dtype=torch.int32).reshape(self.batch)
         held = list(self.held)
         self._advance()
         self._host_calls = 0   # each sequence's own positions are the limit
         try:
+            if getattr(self, "_host", None) is not None and self._captured_with != self._frozen():
+                self._host = (*self._host[:3], self._capture(self._host[0]))
             return super().forward_host(token_ids, out_logits)
         except Exception:
             self.held = held

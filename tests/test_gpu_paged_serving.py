@@ -91,3 +91,21 @@ def test_a_released_row_names_no_page():
     whole(dec)
     dec.reset()
     whole(dec)
+
+
+def test_host_calls_follow_the_shared_pages():
+    """A common prompt, then prompts of each sequence's own, then a common one of another length."""
+    dec, twin = make(3), make(3)
+    for d in (dec, twin):
+        d.share_prompt(ids(150, 1))
+    host_and_step(dec, twin, tokens(2, 3, 2))
+    for d in (dec, twin):
+        d.reset()
+        for i, n in enumerate((140, 10, 150)):
+            d.prefill(ids(n, 3 + i), sequence=i)
+    host_and_step(dec, twin, tokens(2, 3, 6))
+    for d in (dec, twin):
+        d.reset()
+        d.share_prompt(ids(64, 7))
+    host_and_step(dec, twin, tokens(2, 3, 8))
+    dec.check_flags()
