@@ -294,13 +294,15 @@ class LlamaDecoder:
         """A step's launches as a graph; they have run once before, at the positions of the next step."""
         torch = self.torch
         with torch.cuda.stream(stream):
-            pos0 = self.pos.clone()
+            state = self.pos, self.window, self.window_state
+            before = [t.clone() for t in state]
             self._launches(stream.cuda_stream)   # warm-up outside the capture (scratch allocation)
             stream.synchronize()
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph, stream=stream):
                 self._launches(stream.cuda_stream)
-            self.pos.copy_(pos0)
+            for t, was in zip(state, before):
+                t.copy_(was)
             stream.synchronize()
         return graph
 

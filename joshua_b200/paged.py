@@ -22,6 +22,13 @@ from .rope import Rope, rope_table
 from .sampling import sample
 
 
+def _same(a, b) -> bool:
+    """Equal, tensors being the same one."""
+    if isinstance(a, tuple):
+        return len(a) == len(b) and all(map(_same, a, b))
+    return a is b or not isinstance(a, torch.Tensor) and not isinstance(b, torch.Tensor) and a == b
+
+
 class _Paged:
     def __init__(self, cfg, device, batch: int = 1, max_ctx: int = 640, kv_type: str = "q8_0", n_pages: int | None = None,
                  rope: Rope | None = None, **more):
@@ -181,7 +188,8 @@ class _Paged:
 
     def _frozen(self):
         """What a captured step keeps as it was: the host call captures another one when it changes."""
-        return self.shared_pages
+        rule = self.sampling and tuple(self.sampling.items())   # the tensors themselves: a graph reads them where they are
+        return self.shared_pages, self.repetition_penalty, rule
 
     def _capture(self, stream):
         frozen = self._frozen()
@@ -195,7 +203,7 @@ class _Paged:
         self._advance()
         self._host_calls = 0   # each sequence's own positions are the limit
         try:
-            if getattr(self, "_host", None) is not None and self._captured_with != self._frozen():
+            if getattr(self, "_host", None) is not None and not _same(self._captured_with, self._frozen()):
                 self._host = (*self._host[:3], self._capture(self._host[0]))
             return super().forward_host(token_ids, out_logits)
         except Exception:

@@ -109,3 +109,29 @@ def test_host_calls_follow_the_shared_pages():
         d.share_prompt(ids(64, 7))
     host_and_step(dec, twin, tokens(2, 3, 8))
     dec.check_flags()
+
+
+def test_host_calls_follow_the_sampling_rule():
+    import torch
+
+    dec = make(2)
+    first = dict(top_k=torch.ones(2, dtype=torch.int32, device="cuda"))
+    dec.sampling = first
+    dec.uniform.fill_(0.999)
+    logits = torch.from_numpy(np.array(dec.forward_host([1, 2])))
+    assert dec.token.tolist() == logits.argmax(1).tolist()
+    dec.sampling = dict(temperature=torch.full((2,), 1e4, device="cuda"))    # all ids alike: the draw tells the id
+    dec.forward_host([3, 4])
+    assert all(2048 * 0.998 < t for t in dec.token.tolist())
+    dec.sampling["temperature"] = torch.zeros(2, device="cuda")
+    logits = torch.from_numpy(np.array(dec.forward_host([5, 6])))
+    assert dec.token.tolist() == logits.argmax(1).tolist()
+    dec.sampling, dec.repetition_penalty = None, 1e6
+    best = int(logits[0].argmax())
+    dec.seed_window([best])
+    dec.reset()
+    dec.seed_window(list(range(2047)))       # the last 64 ids of it
+    logits = torch.from_numpy(np.array(dec.forward_host([7, 8])))
+    logits[:, 2047 - 64:2047] /= torch.where(logits[:, 2047 - 64:2047] > 0, 1e6, 1e-6)
+    assert dec.token.tolist() == logits.argmax(1).tolist()
+    assert dec.window_state.tolist() == [[64, 1]] * 2      # one id a call, the capture's own steps leave none
