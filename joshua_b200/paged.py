@@ -59,16 +59,24 @@ class _Paged:
     def reserve(self, sequence: int, positions: int) -> None:
         """Pages for the first `positions` positions of a sequence.  A step takes them itself as they fill; reserve them before
         capturing one in a graph."""
-        if positions > self.max_ctx:
-            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{positions} positions in a decoder of {self.max_ctx}")
-        mine, want = self.owned[sequence], -(-positions // PAGE)
-        if want <= len(mine):
-            return
-        if want - len(mine) > len(self.free):
-            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{want - len(mine)} pages wanted, {len(self.free)} of {self.n_pages} are free")
-        new = [self.free.pop() for _ in range(want - len(mine))]
-        self.table[sequence, len(mine):want] = torch.tensor(new, dtype=torch.int32, device=self.dev)
-        mine.extend(new)
+        self._reserve({sequence: positions})
+
+    def _reserve(self, positions: dict) -> None:
+        """Pages for so many positions of each of these sequences, or for none of them if there are not enough."""
+        wanted = 0
+        for i, n in positions.items():
+            if n > self.max_ctx:
+                raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{n} positions in a decoder of {self.max_ctx}")
+            wanted += max(0, -(-n // PAGE) - len(self.owned[i]))
+        if wanted > len(self.free):
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {len(self.free)} of {self.n_pages} are free")
+        for i, n in positions.items():
+            mine, want = self.owned[i], -(-n // PAGE)
+            if want <= len(mine):
+                continue
+            new = [self.free.pop() for _ in range(want - len(mine))]
+            self.table[i, len(mine):want] = torch.tensor(new, dtype=torch.int32, device=self.dev)
+            mine.extend(new)
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages go back (shared ones when the last sequence ends); the next prompt begins at position 0."""
@@ -158,10 +166,9 @@ class _Paged:
         self._launches(now)
 
     def _advance(self) -> None:
-        """Counts one position more of every sequence, with a page for it."""
-        for i in range(self.batch):
-            self.reserve(i, self.held[i] + 1)
-            self.held[i] += 1
+        """Counts one position more of every sequence, with a page for it; where there is none, nothing."""
+        self._reserve({i: n + 1 for i, n in enumerate(self.held)})
+        self.held = [n + 1 for n in self.held]
 
     def _launches(self, stream) -> None:
         torch.add(self.pos, 1, out=self.lens)

@@ -135,3 +135,27 @@ def test_host_calls_follow_the_sampling_rule():
     logits[:, 2047 - 64:2047] /= torch.where(logits[:, 2047 - 64:2047] > 0, 1e6, 1e-6)
     assert dec.token.tolist() == logits.argmax(1).tolist()
     assert dec.window_state.tolist() == [[64, 1]] * 2      # one id a call, the capture's own steps leave none
+
+
+def test_a_step_that_finds_no_page():
+    """It changes nothing, and can be tried again once pages are back."""
+    prompts = [ids(64, 1), ids(70, 2), ids(64, 3)]
+    dec, twin = make(3, max_ctx=256, n_pages=5), make(3, max_ctx=256)
+    for i, p in enumerate(prompts):
+        dec.prefill(p, sequence=i)
+        twin.prefill(p, sequence=i)
+    for call in (dec.step, lambda: dec.forward_host([1, 2, 3])):
+        with pytest.raises(JoshuaB200Error):
+            call()
+        assert dec.held == [64, 70, 64] and len(dec.free) == 1 and dec.pos.tolist() == dec.held
+        whole(dec)
+    dec.release(1), twin.release(1)
+    dec.token.copy_(twin.token)
+    dec.step(), twin.step()
+    assert dec.held[0] == dec.held[2] == 65
+    dec.release(1)
+    for d in (dec, twin):
+        d.prefill(ids(20, 4), sequence=0)
+    near(dec.logits[0], twin.logits[0])
+    whole(dec)
+    dec.check_flags()
