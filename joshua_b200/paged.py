@@ -8,6 +8,10 @@ from a table (any scaling of `rope.rope_table`), the next tokens from `sampling.
     dec.share_prompt(prompt_ids)                 # or dec.prefill(ids, sequence=i) for each
     dec.sampling = dict(temperature=..., top_p=...)
     dec.uniform.uniform_(); dec.step()           # token by token
+
+A step may be captured in a graph by the caller, its pages reserved before.  The graph keeps the sampling rule's tensors, the penalty
+and the number of shared pages as they were: capture another one when they change.  Replays move `pos` alone; prompts, steps and
+host calls that follow (on the stream of the replays, or behind it) begin where it stands.
 """
 from __future__ import annotations
 
@@ -45,6 +49,7 @@ class _Paged:
         self.free = list(range(self.n_pages))[::-1]
         self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
         self.held = [0] * batch                   # positions each holds
+        self._captured_by_caller = False          # then replays may have moved `pos` past `held`
         self.shared_pages = 0                     # leading pages that all sequences have in common
         self.sampling: dict | None = None         # temperature, top_k, top_p, min_p: vectors of `batch`
         self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)   # numbers in [0, 1) for the next draw
@@ -103,6 +108,7 @@ class _Paged:
     def share_prompt(self, token_ids) -> None:
         """Begins all sequences with one prompt, read once: its full pages are common to all, what is left of it (less than a
         page) is copied.  Every sequence samples its own next token."""
+        self._look()
         if any(self.held):
             raise JoshuaB200Error(_lib.E_INVALID, "sequences are under way: reset() first")
         n = len(token_ids)
@@ -128,6 +134,7 @@ class _Paged:
             self._layer_index = {id(ly): k for k, ly in enumerate(self.layers)}
         if c.head_dim not in (64, 128):
             raise JoshuaB200Error(_lib.E_INVALID, "prompts need heads of 64 or 128")
+        self._look()
         s = torch.cuda.current_stream(self.dev).cuda_stream
         ids = torch.as_tensor(token_ids, dtype=torch.int32).to(self.dev)
         S, h, start, f32 = int(ids.numel()), c.hidden, self.held[i], dict(dtype=torch.float32, device=self.dev)
@@ -167,8 +174,17 @@ class _Paged:
 
     def _advance(self) -> None:
         """Counts one position more of every sequence, with a page for it; where there is none, nothing."""
+        if torch.cuda.is_current_stream_capturing():
+            self._captured_by_caller = True
+            return
+        self._look()
         self._reserve({i: n + 1 for i, n in enumerate(self.held)})
         self.held = [n + 1 for n in self.held]
+
+    def _look(self) -> None:
+        """Positions as replays of a caller's graph left them."""
+        if self._captured_by_caller:
+            self.held = self.pos.tolist()
 
     def _launches(self, stream) -> None:
         torch.add(self.pos, 1, out=self.lens)

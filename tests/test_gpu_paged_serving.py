@@ -159,3 +159,39 @@ def test_a_step_that_finds_no_page():
     near(dec.logits[0], twin.logits[0])
     whole(dec)
     dec.check_flags()
+
+
+def test_a_callers_graph_and_then_a_prompt():
+    """Replays move the positions without the decoder's knowledge: what follows begins where they stand."""
+    import torch
+
+    dec, twin = make(2), make(2)
+    for d in (dec, twin):
+        for i in range(2):
+            d.prefill(ids(60 + i, i), sequence=i)
+            d.reserve(i, 200)
+    torch.cuda.synchronize()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            dec.step()
+        for row in tokens(5, 2, 9):
+            dec.token.copy_(torch.tensor(row, dtype=torch.int32))
+            graph.replay()
+        side.synchronize()
+    for row in tokens(5, 2, 9):
+        twin.token.copy_(torch.tensor(row, dtype=torch.int32))
+        twin.step()
+    near(dec.logits, twin.logits)
+    for d in (dec, twin):
+        d.prefill(ids(30, 5), sequence=1)
+    near(dec.logits[1], twin.logits[1])
+    assert dec.pos.tolist() == twin.pos.tolist() == [65, 96]
+    dec.token.copy_(twin.token)
+    graph.replay(), graph.replay()
+    torch.cuda.synchronize()
+    dec.step()
+    for _ in range(3):
+        twin.step()
+    near(dec.logits, twin.logits, 2e-2)      # tokens of their own now
+    assert dec.pos.tolist() == twin.pos.tolist() and dec.held == twin.held
