@@ -293,6 +293,7 @@ class LlamaDecoder:
     def _capture(self, stream):
         """A step's launches as a graph; they have run once before, at the positions of the next step."""
         torch = self.torch
+        stream.wait_stream(torch.cuda.current_stream(self.dev))
         with torch.cuda.stream(stream):
             state = self.pos, self.window, self.window_state
             before = [t.clone() for t in state]
@@ -323,6 +324,11 @@ class LlamaDecoder:
         if self._host_calls >= self.max_ctx:
             raise _lib.JoshuaB200Error(_lib.E_TOO_LARGE, f"the KV cache holds {self.max_ctx} positions; reset() starts a new sequence")
         self._host_calls += 1
+        # prompts, resets and random numbers of the caller's stream come first (that stream waits for nothing: this call does).  Most
+        # often it is idle: asking takes 3 us, waiting 5.
+        caller = torch.cuda.current_stream(self.dev)
+        if not caller.query():
+            stream.wait_stream(caller)
         tok_pin.copy_(torch.as_tensor(token_ids, dtype=torch.int32).reshape(self.batch))
         with torch.cuda.stream(stream):
             self.token.copy_(tok_pin, non_blocking=True)

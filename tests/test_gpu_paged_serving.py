@@ -195,3 +195,16 @@ def test_a_callers_graph_and_then_a_prompt():
         twin.step()
     near(dec.logits, twin.logits, 2e-2)      # tokens of their own now
     assert dec.pos.tolist() == twin.pos.tolist() and dec.held == twin.held
+
+
+def test_a_host_call_waits_for_the_callers_stream():
+    import torch
+
+    dec = make(2)
+    dec.sampling = dict(temperature=torch.full((2,), 1e4, device="cuda"))    # all ids alike: the draw tells the id
+    dec.uniform.fill_(0.1)
+    dec.forward_host([1, 2])
+    torch.cuda._sleep(100_000_000)     # some 50 ms of work in front of the next numbers
+    dec.uniform.fill_(0.9)
+    dec.forward_host([1, 2])
+    assert all(abs(t - 0.9 * 2048) < 10 for t in dec.token.tolist())
