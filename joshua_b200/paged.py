@@ -200,14 +200,20 @@ class _Paged:
         self._sample_rows(slice(0, self.batch))
 
     def _sample_rows(self, rows) -> None:
-        if self.sampling is None and rows.stop - rows.start == self.batch:
-            super()._sample(torch.cuda.current_stream(self.dev).cuda_stream)
-            return
-        rule = self.sampling or dict(temperature=torch.zeros(self.batch, dtype=torch.float32, device=self.dev))
         penalised = self.repetition_penalty != 1.0
-        sample(self.logits[rows], self.uniform[rows], **{k: v[rows] for k, v in rule.items()}, repetition_penalty=self.repetition_penalty,
-               window=self.window[rows] if penalised else None, window_state=self.window_state[rows] if penalised else None,
-               pos=self.pos[rows], token=self.token[rows])
+        window, state = self.window[rows], self.window_state[rows]
+        if self.sampling is None:   # of equal maxima the last one, however many rows
+            L, P, n = _lib.lib(), lambda t: t[rows].data_ptr(), rows.stop - rows.start
+            s = torch.cuda.current_stream(self.dev).cuda_stream
+            if penalised:
+                check(L.jq_sample_greedy_dev(P(self.logits), n, self.cfg.vocab, self.repetition_penalty, window.data_ptr(), state.data_ptr(),
+                                             P(self.token), P(self.pos), self.argmax_scratch.data_ptr(), s))
+            else:
+                check(L.jq_argmax_dev(P(self.logits), n, self.cfg.vocab, P(self.token), P(self.pos), self.argmax_scratch.data_ptr(), s))
+            return
+        sample(self.logits[rows], self.uniform[rows], **{k: v[rows] for k, v in self.sampling.items()},
+               repetition_penalty=self.repetition_penalty, window=window if penalised else None,
+               window_state=state if penalised else None, pos=self.pos[rows], token=self.token[rows])
 
     def _frozen(self):
         """What a captured step keeps as it was: the host call captures another one when it changes."""

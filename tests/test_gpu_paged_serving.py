@@ -208,3 +208,27 @@ def test_a_host_call_waits_for_the_callers_stream():
     dec.uniform.fill_(0.9)
     dec.forward_host([1, 2])
     assert all(abs(t - 0.9 * 2048) < 10 for t in dec.token.tolist())
+
+
+def test_equal_logits_in_a_prompt_as_in_a_step():
+    """Without a sampling rule the last of equal maxima is taken, for one row of a batch too."""
+    import torch
+
+    from joshua_b200 import synth
+
+    def weights(name, rows, cols, seed):
+        if name != "output":
+            return synth.random_weight_torch(synth.Q8_0, rows, cols, seed, torch.device("cuda", 0))
+        half = synth.random_weight_torch(synth.Q8_0, rows // 2, cols, seed, torch.device("cuda", 0))
+        return torch.cat([half, half])     # every id has a twin 1024 further on
+
+    dec = make(3, weights=weights)
+    dec.prefill(ids(20, 1), sequence=1)
+    assert bool((dec.logits[1, :1024] == dec.logits[1, 1024:]).all())
+    best = int(dec.logits[1, 1024:].argmax()) + 1024
+    assert int(dec.token[1]) == best
+    dec.repetition_penalty = 2.0
+    dec.prefill(ids(20, 2), sequence=2)
+    assert int(dec.token[2]) == int(dec.logits[2, 1024:].argmax()) + 1024 and dec.window_state.tolist() == [[0, 0], [0, 0], [1, 1]]
+    dec.step()
+    assert bool((dec.token >= 1024).all()) and dec.pos.tolist() == [1, 21, 21]
