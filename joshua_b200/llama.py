@@ -218,15 +218,17 @@ class LlamaDecoder:
             check(L.jq_sample_greedy_dev(P(self.logits), B, c.vocab, self.repetition_penalty, P(self.window),
                                          P(self.window_state), P(self.token), P(self.pos), P(self.argmax_scratch), s))
 
-    def seed_window(self, prompt_ids) -> None:
-        """Fills the recent-id window with the tail of the prompt, as the reference's decode loop does
+    def seed_window(self, prompt_ids, sequence: int | None = None) -> None:
+        """Fills the recent-id window (of one sequence, or of all) with the tail of the prompt, as the reference's decode loop does
         (src/engine.rs:1222-1232)."""
         torch = self.torch
         tail = [int(t) for t in prompt_ids][-64:]
-        w = torch.zeros(self.batch, 64, dtype=torch.int32)
-        w[:, :len(tail)] = torch.tensor(tail, dtype=torch.int32)
-        self.window.copy_(w)
-        self.window_state.copy_(torch.tensor([[len(tail), len(tail) % 64]] * self.batch, dtype=torch.int32))
+        first = 0 if sequence is None else range(self.batch)[sequence]
+        rows = slice(0, self.batch) if sequence is None else slice(first, first + 1)
+        w = torch.zeros(64, dtype=torch.int32)
+        w[:len(tail)] = torch.tensor(tail, dtype=torch.int32)
+        self.window[rows].copy_(w.expand(rows.stop - rows.start, -1))
+        self.window_state[rows].copy_(torch.tensor([[len(tail), len(tail) % 64]] * (rows.stop - rows.start), dtype=torch.int32))
 
     def check_flags(self) -> None:
         """Raises if a token id was out of range, a position ran past the KV cache or a wait inside a kernel gave up

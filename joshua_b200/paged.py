@@ -91,6 +91,7 @@ class _Paged:
         self.owned[sequence], self.held[sequence] = [], 0
         self.table[sequence] = -1
         self.pos[sequence] = 0
+        self.window[sequence], self.window_state[sequence] = 0, 0   # the next prompt is another text
         self.shared_pages = 0   # not all sequences have them any more
 
     def reset(self, token: int = 42) -> None:

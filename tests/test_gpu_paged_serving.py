@@ -232,3 +232,28 @@ def test_equal_logits_in_a_prompt_as_in_a_step():
     assert int(dec.token[2]) == int(dec.logits[2, 1024:].argmax()) + 1024 and dec.window_state.tolist() == [[0, 0], [0, 0], [1, 1]]
     dec.step()
     assert bool((dec.token >= 1024).all()) and dec.pos.tolist() == [1, 21, 21]
+
+
+@pytest.mark.parametrize("ruled", [False, True])
+def test_a_slot_that_is_used_again_forgets_its_ids(ruled):
+    import torch
+
+    dec, fresh = make(2), make(2)
+    for d in (dec, fresh):
+        d.repetition_penalty = 1e6
+        if ruled:
+            d.sampling = dict(top_k=torch.ones(2, dtype=torch.int32, device="cuda"))
+    fresh.prefill(ids(40, 1), sequence=0)
+    dec.prefill(ids(10, 2), sequence=1)
+    dec.prefill(ids(40, 1), sequence=0)      # its token goes into the window
+    assert int(dec.token[0]) == int(fresh.token[0])
+    kept = dec.window[1].clone(), dec.window_state[1].clone()
+    dec.release(0)
+    dec.prefill(ids(40, 1), sequence=0)
+    assert int(dec.token[0]) == int(fresh.token[0])
+    assert torch.equal(dec.window[1], kept[0]) and torch.equal(dec.window_state[1], kept[1])
+    dec.release(0)
+    dec.seed_window([int(fresh.token[0])], sequence=0)
+    dec.prefill(ids(40, 1), sequence=0)
+    assert int(dec.token[0]) == int(dec.logits[0].topk(2).indices[1])
+    assert torch.equal(dec.window[1], kept[0]) and torch.equal(dec.window_state[1], kept[1])
