@@ -60,11 +60,16 @@ class _Paged:
     def _attention_scratch(self) -> None:
         """The caches keep their own."""
 
+    def _index(self, sequence: int) -> int:
+        if not 0 <= sequence < self.batch:
+            raise JoshuaB200Error(_lib.E_INVALID, f"sequence {sequence} of {self.batch}")
+        return sequence
+
     # ── pages ───────────────────────────────────────────────────────────
     def reserve(self, sequence: int, positions: int) -> None:
         """Pages for the first `positions` positions of a sequence.  A step takes them itself as they fill; reserve them before
         capturing one in a graph."""
-        self._reserve({sequence: positions})
+        self._reserve({self._index(sequence): positions})
 
     def _reserve(self, positions: dict) -> None:
         """Pages for so many positions of each of these sequences, or for none of them if there are not enough."""
@@ -85,7 +90,7 @@ class _Paged:
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages go back (shared ones when the last sequence ends); the next prompt begins at position 0."""
-        for page in self.owned[sequence]:
+        for page in self.owned[self._index(sequence)]:
             if not any(page in other for i, other in enumerate(self.owned) if i != sequence):
                 self.free.append(page)
         self.owned[sequence], self.held[sequence] = [], 0
@@ -103,7 +108,7 @@ class _Paged:
     def prefill(self, token_ids, sequence: int = 0) -> None:
         """The prompt's tokens of one sequence in one pass, from where it stands; then self.logits[sequence], its sampled next
         token (self.token) and position, as `step` leaves them."""
-        self._prompt(token_ids, sequence)
+        self._prompt(token_ids, self._index(sequence))
         self._sample_rows(slice(sequence, sequence + 1))
 
     def share_prompt(self, token_ids) -> None:

@@ -257,3 +257,14 @@ def test_a_slot_that_is_used_again_forgets_its_ids(ruled):
     dec.prefill(ids(40, 1), sequence=0)
     assert int(dec.token[0]) == int(dec.logits[0].topk(2).indices[1])
     assert torch.equal(dec.window[1], kept[0]) and torch.equal(dec.window_state[1], kept[1])
+
+
+def test_sequences_that_are_not_there():
+    dec = make(2)
+    for i in (-1, 2, -3):
+        for call in (lambda: dec.prefill(ids(5, 1), sequence=i), lambda: dec.reserve(i, 10), lambda: dec.release(i)):
+            with pytest.raises(JoshuaB200Error):
+                call()
+    assert dec.held == [0, 0] and len(dec.free) == dec.n_pages
+    dec.prefill(ids(5, 1), sequence=1)
+    dec.check_flags()
