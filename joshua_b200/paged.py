@@ -117,16 +117,24 @@ class _Paged:
         self._look()
         if any(self.held):
             raise JoshuaB200Error(_lib.E_INVALID, "sequences are under way: reset() first")
-        n = len(token_ids)
+        n, others = len(token_ids), range(1, self.batch)
+        full, pages = n // PAGE, -(-n // PAGE)
+        # what sequences have reserved stays theirs, but for the pages in whose place the common ones stand
+        wanted = max(0, pages - len(self.owned[0])) + sum(max(0, pages - max(full, len(self.owned[i]))) for i in others)
+        back = sum(min(full, len(self.owned[i])) for i in others)
+        if wanted > len(self.free) + back:
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {len(self.free) + back} of {self.n_pages} are free")
         self._prompt(token_ids, 0)
-        common, rest = self.owned[0][:n // PAGE], self.owned[0][n // PAGE:]
-        for i in range(1, self.batch):
-            self.owned[i] = list(common)
-            self.table[i, :len(common)] = self.table[0, :len(common)]
-            self.reserve(i, n)
+        common, rest = self.owned[0][:full], self.owned[0][full:]
+        for i in others:
+            self.free.extend(self.owned[i][:full])
+            self.owned[i] = common + self.owned[i][full:]
+            self.table[i, :full] = self.table[0, :full]
+        self._reserve({i: n for i in others})
+        for i in others:
             if n % PAGE:
                 for ly in self.layers:
-                    ly["cache"].pages[self.owned[i][-1]] = ly["cache"].pages[rest[0]]
+                    ly["cache"].pages[self.owned[i][full]] = ly["cache"].pages[rest[0]]
             self.held[i] = n
         self.shared_pages = len(common)
         self.pos.fill_(n - 1)

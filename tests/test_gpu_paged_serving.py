@@ -268,3 +268,26 @@ def test_sequences_that_are_not_there():
     assert dec.held == [0, 0] and len(dec.free) == dec.n_pages
     dec.prefill(ids(5, 1), sequence=1)
     dec.check_flags()
+
+
+def test_a_common_prompt_keeps_what_was_reserved():
+    dec, plain = make(3, max_ctx=320), make(3, max_ctx=320)
+    dec.reserve(0, 30), dec.reserve(1, 250), dec.reserve(2, 70)
+    for d in (dec, plain):
+        d.share_prompt(ids(150, 1))
+        whole(d)
+    assert [len(mine) for mine in dec.owned] == [3, 4, 3] and len(dec.free) == 15 - 2 - 1 - 2 - 1
+    dec.step(), plain.step()
+    near(dec.logits, plain.logits)
+    dec.reset()
+    assert len(dec.free) == 15
+
+
+def test_a_common_prompt_that_does_not_fit():
+    dec = make(4, max_ctx=320, n_pages=5)       # two common pages and four of the rest
+    with pytest.raises(JoshuaB200Error):
+        dec.share_prompt(ids(150, 1))
+    assert len(dec.free) == 5 and dec.held == [0] * 4 and dec.pos.tolist() == [0] * 4
+    whole(dec)
+    dec.share_prompt(ids(120, 1))               # one and four
+    assert dec.free == [] and dec.shared_pages == 1
