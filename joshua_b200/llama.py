@@ -309,6 +309,9 @@ class LlamaDecoder:
             stream.synchronize()
         return graph
 
+    def _positions_used(self) -> int:
+        return int(self.pos.max().item())
+
     def forward_host(self, token_ids, out_logits=None):
         """`ModelWeights::forward(input_ids, index_pos) -> logits` for one new token per sequence with HOST
         buffers on both sides (the shape of the reference's model call, src/model.rs:362-364): the token ids
@@ -321,7 +324,7 @@ class LlamaDecoder:
             tok_pin = torch.empty(self.batch, dtype=torch.int32).pin_memory()
             log_pin = torch.empty(self.batch, self.cfg.vocab, dtype=torch.float32).pin_memory()
             self._host = (stream, tok_pin, log_pin, self._capture(stream))
-            self._host_calls = int(self.pos.max().item())
+            self._host_calls = self._positions_used()
         stream, tok_pin, log_pin, graph = self._host
         if self._host_calls >= self.max_ctx:
             raise _lib.JoshuaB200Error(_lib.E_TOO_LARGE, f"the KV cache holds {self.max_ctx} positions; reset() starts a new sequence")

@@ -1,6 +1,7 @@
 """The decoders of this package with their keys and values in pages of few bits, for batches of long sequences.
 
-Sequences take pages from one pool as they grow and give them back when they end; sequences that begin with the same prompt hold
+Sequences take pages from one pool as they grow and give them back when they end (`release`); until its next prompt such a sequence
+rests: it takes part in steps with nothing to attend to, and what they leave for it means nothing.  Sequences that begin with the same prompt hold
 its full pages in common, and a step reads and multiplies those once for all of them (`share_prompt`).  Rotary positions come
 from a table (any scaling of `rope.rope_table`), the next tokens from `sampling.sample` where a sampling rule is set.
 
@@ -39,6 +40,8 @@ class _Paged:
         """`n_pages`: of the pool (default: enough for every sequence to reach max_ctx); `rope`: a table of max_ctx positions
         (default: the model's theta, unscaled, half layout)."""
         self.kv_type, self.pages_per_seq = kv_type, -(-max_ctx // PAGE)
+        # resting sequences still bring a row to every append: to a position each of pages behind the pool
+        self._places = min(PAGE, max_ctx)
         self.n_pages = batch * self.pages_per_seq if n_pages is None else n_pages
         super().__init__(cfg, device, batch=batch, max_ctx=max_ctx, **more)
         self.rope = rope or Rope(rope_table(cfg.rope_theta, cfg.head_dim, max_ctx, self.dev))
@@ -46,6 +49,10 @@ class _Paged:
         # that ended (a graph) raises the caches' flag instead of writing into another sequence's page.
         self.table = torch.full((batch, self.pages_per_seq), -1, dtype=torch.int32, device=self.dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)
+        self.resting = [False] * batch
+        self.active = torch.ones(batch, dtype=torch.int32, device=self.dev)       # 0: rests
+        self.idle_pos = torch.zeros(batch, dtype=torch.int32, device=self.dev)    # where a resting sequence's rows go
+        self._seeds: dict[int, list] = {}         # recent ids given to a resting sequence
         self.free = list(range(self.n_pages))[::-1]
         self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
         self.held = [0] * batch                   # positions each holds
@@ -55,7 +62,8 @@ class _Paged:
         self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)   # numbers in [0, 1) for the next draw
 
     def _layer_cache(self) -> dict:
-        return dict(cache=PagedCache(self.kv_type, self.cfg.kv_heads, self.cfg.head_dim, n_pages=self.n_pages, device=self.dev))
+        return dict(cache=PagedCache(self.kv_type, self.cfg.kv_heads, self.cfg.head_dim, n_pages=self.n_pages + -(-self.batch // self._places),
+                                     device=self.dev))
 
     def _attention_scratch(self) -> None:
         """The caches keep their own."""
@@ -89,20 +97,43 @@ class _Paged:
             mine.extend(new)
 
     def release(self, sequence: int) -> None:
-        """Ends a sequence: its pages go back (shared ones when the last sequence ends); the next prompt begins at position 0."""
+        """Ends a sequence: its pages go back (shared ones when the last sequence ends).  It rests until its next prompt, which
+        begins at position 0."""
         for page in self.owned[self._index(sequence)]:
             if not any(page in other for i, other in enumerate(self.owned) if i != sequence):
                 self.free.append(page)
         self.owned[sequence], self.held[sequence] = [], 0
         self.table[sequence] = -1
-        self.pos[sequence] = 0
+        self.table[sequence, 0] = self.n_pages + sequence // self._places
+        self.pos[sequence], self.active[sequence], self.idle_pos[sequence] = 0, 0, sequence % self._places
+        self.resting[sequence] = True
+        self._seeds.pop(sequence, None)
         self.window[sequence], self.window_state[sequence] = 0, 0   # the next prompt is another text
-        self.shared_pages = 0   # not all sequences have them any more
+        if sequence == 0:
+            self.shared_pages = 0   # the kernels find the common pages through the first sequence
+
+    def _wake(self, i: int) -> None:
+        """A sequence that rests, and has its pages, takes part again, from position 0."""
+        if not self.resting[i]:
+            return
+        self.resting[i] = False
+        self.pos[i], self.active[i], self.idle_pos[i] = 0, 1, 0
+        super().seed_window(self._seeds.pop(i, []), i)   # steps have left ids there
+        self.shared_pages = 0       # it has other pages than those who share
 
     def reset(self, token: int = 42) -> None:
+        """All sequences from position 0, none of them resting."""
         for i in range(self.batch):
             self.release(i)
+            self._wake(i)
+        self.table.fill_(-1)
         super().reset(token)
+
+    def seed_window(self, prompt_ids, sequence: int | None = None) -> None:
+        super().seed_window(prompt_ids, sequence)
+        for i in range(self.batch) if sequence is None else [range(self.batch)[sequence]]:
+            if self.resting[i]:
+                self._seeds[i] = [int(t) for t in prompt_ids][-64:]
 
     # ── a prompt ────────────────────────────────────────────────────────
     def prefill(self, token_ids, sequence: int = 0) -> None:
@@ -132,6 +163,7 @@ class _Paged:
             self.table[i, :full] = self.table[0, :full]
         self._reserve({i: n for i in others})
         for i in others:
+            self._wake(i)
             if n % PAGE:
                 for ly in self.layers:
                     ly["cache"].pages[self.owned[i][full]] = ly["cache"].pages[rest[0]]
@@ -155,6 +187,7 @@ class _Paged:
         if S == 0:
             raise JoshuaB200Error(_lib.E_INVALID, "an empty prompt")
         self.reserve(i, start + S)
+        self._wake(i)
         end = start + S
         pos = torch.arange(end, dtype=torch.int32, device=self.dev)
         seq = torch.full((end,), i, dtype=torch.int32, device=self.dev)
@@ -187,21 +220,22 @@ class _Paged:
         self._launches(now)
 
     def _advance(self) -> None:
-        """Counts one position more of every sequence, with a page for it; where there is none, nothing."""
+        """Counts one position more of every sequence that does not rest, with a page for it; where there is none, nothing."""
         if torch.cuda.is_current_stream_capturing():
             self._captured_by_caller = True
             return
         self._look()
-        self._reserve({i: n + 1 for i, n in enumerate(self.held)})
-        self.held = [n + 1 for n in self.held]
+        self._reserve({i: n + 1 for i, n in enumerate(self.held) if not self.resting[i]})
+        self.held = [n + (not rests) for n, rests in zip(self.held, self.resting)]
 
     def _look(self) -> None:
         """Positions as replays of a caller's graph left them."""
         if self._captured_by_caller:
-            self.held = self.pos.tolist()
+            self.held = [0 if rests else n for n, rests in zip(self.pos.tolist(), self.resting)]
 
     def _launches(self, stream) -> None:
-        torch.add(self.pos, 1, out=self.lens)
+        torch.addcmul(self.idle_pos, self.pos, self.active, out=self.pos)   # resting: to its place behind the pool,
+        torch.addcmul(self.active, self.pos, self.active, out=self.lens)    # and no positions to attend to; else pos + 1
         super().step(stream)
 
     def _attend(self, ly, s) -> None:
@@ -228,6 +262,9 @@ class _Paged:
         sample(self.logits[rows], self.uniform[rows], **{k: v[rows] for k, v in self.sampling.items()},
                repetition_penalty=self.repetition_penalty, window=window if penalised else None,
                window_state=state if penalised else None, pos=self.pos[rows], token=self.token[rows])
+
+    def _positions_used(self) -> int:
+        return 0   # each sequence's own are counted by `held`
 
     def _frozen(self):
         """What a captured step keeps as it was: the host call captures another one when it changes."""

@@ -291,3 +291,105 @@ def test_a_common_prompt_that_does_not_fit():
     whole(dec)
     dec.share_prompt(ids(120, 1))               # one and four
     assert dec.free == [] and dec.shared_pages == 1
+
+
+@pytest.mark.parametrize("ruled", [False, True])
+def test_a_sequence_rests(ruled):
+    """From its release to its next prompt a sequence takes no pages and does not hinder the others."""
+    import torch
+
+    dec, twin = make(3, max_ctx=200), make(2, max_ctx=200)
+    for d, at in ((dec, (0, 2)), (twin, (0, 1))):
+        d.repetition_penalty = 1.3
+        if ruled:
+            d.sampling = dict(top_k=torch.ones(d.batch, dtype=torch.int32, device="cuda"))
+        for i, n in zip(at, (100, 30)):
+            d.prefill(ids(n, n), sequence=i)
+    dec.prefill(ids(197, 5), sequence=1)
+    dec.release(1)
+    free = len(dec.free)
+    for row in tokens(70, 2, 1):
+        dec.token.copy_(torch.tensor([row[0], 0, row[1]], dtype=torch.int32))
+        twin.token.copy_(torch.tensor(row, dtype=torch.int32))
+        dec.step(), twin.step()
+    near(dec.logits[::2], twin.logits, 2e-2)
+    assert dec.held == [170, 0, 100] and len(dec.free) == free - 2 and dec.owned[1] == []
+    dec.check_flags()
+    whole(dec)
+    dec.release(0), twin.release(0)
+    for d, i in ((dec, 1), (twin, 0)):                # another prompt in the slot: from position 0 on
+        d.seed_window([1, 2, 3], sequence=i)
+        d.step()                                      # the ids given stay while it rests
+        d.prefill(ids(40, 6), sequence=i)
+    near(dec.logits[1], twin.logits[0])
+    assert dec.held[1] == 40 and int(dec.token[1]) == int(twin.token[0]) and dec.window_state[1].tolist() == [4, 4]
+    assert dec.window[1, :3].tolist() == [1, 2, 3]
+    dec.release(2), dec.release(1)
+    dec.step()                                        # all of them rest
+    assert dec.held == [0, 0, 0] and len(dec.free) == dec.n_pages
+    dec.check_flags()
+
+
+def test_a_graph_and_the_host_call_leave_resting_sequences_alone():
+    import torch
+
+    dec = make(3, max_ctx=130)
+    for i in range(3):
+        dec.prefill(ids(20 + i, i), sequence=i)
+        dec.reserve(i, 130)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        dec.step()
+        with torch.cuda.graph(graph, stream=side):
+            dec.step()
+        side.synchronize()
+    dec.release(1)
+    for _ in range(100):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert dec.pos[[0, 2]].tolist() == [121, 123]
+    dec.check_flags()
+    for _ in range(3):
+        dec.forward_host([1, 2, 3])
+    assert dec.held == [124, 0, 126] and dec.owned[1] == []
+    dec.check_flags()
+    whole(dec)
+
+
+def test_many_resting_sequences():
+    """More of them than a page has positions."""
+    dec = make(70, max_ctx=64)
+    for i in range(1, 70):
+        dec.release(i)
+    dec.prefill(ids(5, 1))
+    dec.step()
+    assert len(dec.free) == 69 and dec.held == [6] + [0] * 69
+    dec.check_flags()
+
+
+def test_a_prompt_stays_common_while_others_end():
+    dec, twin = make(4), make(4)
+    for d in (dec, twin):
+        d.share_prompt(ids(150, 1))
+        d.release(2)
+    assert dec.shared_pages == 2 and len(dec.free) == 20 - 2 - 3
+    twin.shared_pages = 0
+    for row in tokens(2, 4, 3):
+        for d in (dec, twin):
+            d.token.copy_(__import__("torch").tensor(row, dtype=d.token.dtype))
+            d.step()
+    live = [0, 1, 3]
+    near(dec.logits[live], twin.logits[live])
+    for d in (dec, twin):
+        d.prefill(ids(30, 4), sequence=2)
+        d.step()
+    assert dec.shared_pages == 0
+    near(dec.logits, twin.logits, 2e-2)
+    dec.reset()
+    dec.share_prompt(ids(150, 1))
+    dec.release(0)                   # the common pages are found through the first sequence
+    assert dec.shared_pages == 0
+    dec.step()
+    dec.check_flags()
+    whole(dec)
