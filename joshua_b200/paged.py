@@ -145,6 +145,7 @@ class _Paged:
     def share_prompt(self, token_ids) -> None:
         """Begins all sequences with one prompt, read once: its full pages are common to all, what is left of it (less than a
         page) is copied.  Every sequence samples its own next token."""
+        self._can_prompt()
         self._look()
         if any(self.held):
             raise JoshuaB200Error(_lib.E_INVALID, "sequences are under way: reset() first")
@@ -173,13 +174,18 @@ class _Paged:
         self.logits.copy_(self.logits[0:1].expand(self.batch, -1).clone())
         self._sample_rows(slice(0, self.batch))
 
+    def _can_prompt(self) -> None:
+        if self.cfg.head_dim not in (64, 128):
+            raise JoshuaB200Error(_lib.E_INVALID, "prompts need heads of 64 or 128")
+        if getattr(self, "world", 1) > 1:
+            raise JoshuaB200Error(_lib.E_INVALID, "prompts run on one GPU (the exchange windows are sized for decode batches)")
+
     def _prompt(self, token_ids, i) -> None:
         """Logits of the prompt's last token into self.logits[i]; self.pos[i] at that token."""
+        self._can_prompt()
         L, c, P = _lib.lib(), self.cfg, lambda t: t.data_ptr()
         if not hasattr(self, "_layer_index"):   # the routed experts' decoder finds its layers by it
             self._layer_index = {id(ly): k for k, ly in enumerate(self.layers)}
-        if c.head_dim not in (64, 128):
-            raise JoshuaB200Error(_lib.E_INVALID, "prompts need heads of 64 or 128")
         self._look()
         s = torch.cuda.current_stream(self.dev).cuda_stream
         ids = torch.as_tensor(token_ids, dtype=torch.int32).to(self.dev)

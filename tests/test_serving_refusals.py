@@ -154,3 +154,17 @@ def test_an_entry_without_a_context_may_have_no_status_flag(name):
     text = (ROOT / "joshua_b200" / "csrc" / name).read_text()
     stores = [line for line in text.splitlines() if "volatile int*>(error_flag) = 1" in line]
     assert stores and all("&& error_flag)" in line for line in stores)
+
+
+def test_prompts_on_several_ranks():
+    """Refused before a page is taken: the exchange's windows are sized for steps."""
+    from joshua_b200.moe_decoder import MoeDecoderConfig
+    from joshua_b200.paged import PagedMoeDecoder
+
+    dec = object.__new__(PagedMoeDecoder)
+    dec.cfg, dec.world, dec.batch, dec.layers, dec.held = MoeDecoderConfig(), 2, 2, [], [0, 0]
+    dec.free, dec.owned = [1, 0], [[], []]
+    for call in (lambda: dec.prefill([1, 2, 3]), lambda: dec.share_prompt([1, 2, 3])):
+        with pytest.raises(_lib.JoshuaB200Error, match="one GPU"):
+            call()
+    assert dec.free == [1, 0] and dec.owned == [[], []]
