@@ -55,6 +55,7 @@ class _Paged:
         self._seeds: dict[int, list] = {}         # recent ids given to a resting sequence
         self.free = list(range(self.n_pages))[::-1]
         self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
+        self.holders = [0] * self.n_pages         # sequences that have a page
         self.held = [0] * batch                   # positions each holds
         self._captured_by_caller = False          # then replays may have moved `pos` past `held`
         self.shared_pages = 0                     # leading pages that all sequences have in common
@@ -88,20 +89,28 @@ class _Paged:
             wanted += max(0, -(-n // PAGE) - len(self.owned[i]))
         if wanted > len(self.free):
             raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {len(self.free)} of {self.n_pages} are free")
+        places, pages = [], []
         for i, n in positions.items():
-            mine, want = self.owned[i], -(-n // PAGE)
-            if want <= len(mine):
-                continue
-            new = [self.free.pop() for _ in range(want - len(mine))]
-            self.table[i, len(mine):want] = torch.tensor(new, dtype=torch.int32, device=self.dev)
-            mine.extend(new)
+            mine = self.owned[i]
+            while len(mine) < -(-n // PAGE):
+                places.append(i * self.pages_per_seq + len(mine))
+                pages.append(self.free.pop())
+                mine.append(pages[-1])
+                self.holders[pages[-1]] = 1
+        if pages:   # one copy for all of them, from pinned memory: the host waits for nothing
+            new = torch.tensor([places, pages], dtype=torch.int64, pin_memory=True).to(self.dev, non_blocking=True)
+            self.table.view(-1).scatter_(0, new[0], new[1].int())
+
+    def _give_back(self, pages) -> None:
+        for page in pages:
+            self.holders[page] -= 1
+            if self.holders[page] == 0:
+                self.free.append(page)
 
     def release(self, sequence: int) -> None:
         """Ends a sequence: its pages go back (shared ones when the last sequence ends).  It rests until its next prompt, which
         begins at position 0."""
-        for page in self.owned[self._index(sequence)]:
-            if not any(page in other for i, other in enumerate(self.owned) if i != sequence):
-                self.free.append(page)
+        self._give_back(self.owned[self._index(sequence)])
         self.owned[sequence], self.held[sequence] = [], 0
         self.table[sequence] = -1
         self.table[sequence, 0] = self.n_pages + sequence // self._places
@@ -159,7 +168,9 @@ class _Paged:
         self._prompt(token_ids, 0)
         common, rest = self.owned[0][:full], self.owned[0][full:]
         for i in others:
-            self.free.extend(self.owned[i][:full])
+            self._give_back(self.owned[i][:full])
+            for page in common:
+                self.holders[page] += 1
             self.owned[i] = common + self.owned[i][full:]
             self.table[i, :full] = self.table[0, :full]
         self._reserve({i: n for i in others})

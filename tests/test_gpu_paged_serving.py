@@ -393,3 +393,23 @@ def test_a_prompt_stays_common_while_others_end():
     dec.step()
     dec.check_flags()
     whole(dec)
+
+
+def test_taking_pages_waits_for_nothing():
+    import torch
+
+    dec = make(4)
+    for i in range(4):
+        dec.prefill(ids(64, i), sequence=i)
+    dec.step()
+    for i in range(4):
+        dec.release(i)
+        dec.prefill(ids(64, i), sequence=i)
+    torch.cuda.synchronize()
+    torch.cuda._sleep(600_000_000)     # some 300 ms
+    end = torch.cuda.Event()
+    end.record()
+    dec.step()                         # a page of each sequence
+    assert not end.query() and dec.held == [65] * 4 and [len(mine) for mine in dec.owned] == [2] * 4
+    whole(dec)
+    dec.check_flags()
