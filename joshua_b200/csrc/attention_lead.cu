@@ -2,11 +2,12 @@
 // the pages, once for all sequences (attention_paged.cu joins the result with each sequence's own pages).
 //
 // One CTA per (128 query rows, kv head, split of the pages), a page at a time, running maximum and sum in f32.  Queries are two
-// f16 terms under a power of two of their row, keys and values the code times the block's scale, which has 19 bits at most
-// (halves: 11): two f16 terms that hold it exactly (halves: one), keys under a power of two of their position's largest scale,
-// values under one of the page's largest scale of the block of 32 dimensions; probabilities two terms.  A product of two terms
-// each leaves out the smallest of the four.  Accumulators hold 64 dimensions of a score or one page of the output, the running
-// output lives in registers and is added round-to-nearest.
+// f16 terms under a power of two of their row.  Keys and values are the code times the block's scale, 19 bits at most (halves: 11),
+// as two f16 terms (halves: one), keys under a power of two of the page's largest scale, values under one of the page's largest
+// scale of the block of 32 dimensions: exact for scales of at least 2^-21 (four bits: 2^-25) of that largest one; smaller scales are
+// rounded by up to 2^-32 (2^-36) of it.  Probabilities are two terms.  A product of two terms each leaves out the smallest of the
+// four.  Accumulators hold 64 dimensions of a score or one page of the output, the running output lives in registers and is added
+// round-to-nearest.
 //
 // What bounds it is the chain of a tile (scores' product, maximum of the row, exponentials, probabilities' product), not the
 // products: 1.65 us a page with heads of 128 in eight bits, 0.9 with heads of 64 in halves, of which the tensor pipe is busy 19%
@@ -212,10 +213,11 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             sh.row[1][half][row] = amax;
             pair_bar();
             amax = fmaxf(amax, sh.row[1][half ^ 1][row]);
-            // a power of two that puts the row's largest value just below 2^15
+            // a power of two that puts the row's largest value just below 2^15, with the sign of the scale: the row's maximum is
+            // looked for before the scores are multiplied by rf, which must not turn their order round
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
-            const float sc = __uint_as_float(bits << 23);
-            rf = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * (a.scale * 1.44269504f);
+            const float sc = copysignf(__uint_as_float(bits << 23), a.scale);
+            rf = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * (fabsf(a.scale) * 1.44269504f);
 #pragma unroll
             for (uint32_t c = 0; c < DN / 32; ++c) {
                 uint32_t hi[16], lo[16];

@@ -336,3 +336,15 @@ def test_refusals():
         with pytest.raises(JoshuaB200Error):
             bad()
     assert cache.attend(q[:0], n[:0], table[:0], n_q=4).shape == (0, 256)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd,n_q,n_kv,batch,shared", [(128, 32, 8, 32, 20), (64, 24, 2, 40, 75), (128, 4, 4, 8, 200), (256, 2, 2, 20, 70), (64, 8, 2, 3, 1)])
+def test_a_negative_scale(kind, hd, n_q, n_kv, batch, shared):
+    """On every route, with scores of both signs: |scale| and size of the scores as in the tests above."""
+    cache, table, lens, q = long_prompt(kind, hd, n_q, n_kv, max(batch, 4), shared)
+    got = cache.attend(q, i32(lens), table, n_q=n_q, scale=-0.2, shared_pages=shared)
+    for b in (0, 1, 2, len(lens) - 1):
+        held = tuple(t.cpu().numpy() for t in cache.read(i32(range(lens[b])), table, seq=i32([b] * lens[b])))
+        expect(got[b:b + 1], q[b:b + 1], [held], n_q, hd, scale=-0.2, tol=4 * TOL)   # up to 3.2 times the scores of scale 1 / sqrt(hd)
+    cache.check_flags()
