@@ -433,9 +433,11 @@ int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32
  *   shared_pages: the first so many pages are the same for the whole batch (a common prompt): read from the first sequence's
  * table entries, and once for all where that is the faster way.  Every len is then 0 or at least shared_pages * JQ_KV_PAGE.
  *   A len outside its range or a page id outside the cache makes the sequence's rows NaN and sets *bad_pos_dev.
- *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, ZEROED once before the first
- * call (it holds arrival counters that the kernels leave at zero); one call at a time. */
+ *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, its first
+ * JQ_ATTENTION_SCRATCH_ZEROED bytes ZEROED once before the first call (they hold arrival counters that the kernels leave at
+ * zero).  It serves calls of any sizes that it is large enough for, one at a time. */
 #define JQ_ATTENTION_MAX_BATCH 4096u
+#define JQ_ATTENTION_SCRATCH_ZEROED 1024u
 uint64_t jq_attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t head_dim, uint32_t shared_pages);
 int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* len,
                                const int32_t* page_table, uint32_t batch, uint32_t table_stride, uint32_t n_q, float scale,

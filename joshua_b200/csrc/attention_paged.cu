@@ -781,7 +781,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     if (open) {  // the same in all threads
         __threadfence();
         __syncthreads();
-        auto owners = [&](uint32_t sg, uint32_t* c0) {  // CTAs that have a piece of it, from c0 on
+        // CTAs that have a piece of it, from c0 on.  Of the segments whose first step is a CTA's only its last goes on behind it, so c0
+        // tells open segments apart.
+        auto owners = [&](uint32_t sg, uint32_t* c0) {
             const uint32_t sb = sg / groups, units = s_cum[sb + 1] - s_cum[sb];
             const uint64_t x = (uint64_t)s_cum[sb] * groups + (uint64_t)(sg % groups) * units, x0 = x + SEG_UNITS, x1 = x + units - 1;
             *c0 = (uint32_t)(((x0 + 1) * workers - 1) / total / WARPS);
@@ -792,7 +794,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
             if (open >> tid & 1) {
                 uint32_t c0;
                 const uint32_t sg = open_seg[tid], n = owners(sg, &c0);
-                if (atomicAdd(a.arrived + sg, 1) == n - 1) a.arrived[sg] = 0, s_last[tid] = n, s_first[tid] = c0;
+                if (atomicAdd(a.arrived + c0, 1) == n - 1) a.arrived[c0] = 0, s_last[tid] = n, s_first[tid] = c0;
             }
             __threadfence();
         }
@@ -934,7 +936,7 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
     p.group = n_q / n_kv;
     p.rows = p.group <= 4 ? 4 : 8;
     p.split = (p.group + p.rows - 1) / p.rows;
-    p.grid = (uint32_t)num_sms();
+    p.grid = std::min((uint32_t)num_sms(), ATTENTION_MOST_CTAS);
     const uint32_t rows = batch * p.group, tiles = (rows + 8 * lead_tiles(hd) - 1) / (8 * lead_tiles(hd));
     p.tiles = hd <= 128 && rows >= LEAD_TILE_ROWS;
     // passes over the leading pages: a sequence's own is the unit, 128 rows of attention_lead.cu take as long as 5, 16 (heads of
@@ -951,7 +953,8 @@ PagedPlan plan(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_
         while (p.cluster > fit) p.cluster /= 2;
         p.splits = std::min(fit, LEAD_MOST * p.cluster) / p.cluster * p.cluster;
     }
-    p.part_at = ((size_t)batch * n_kv * p.split * 4 + 255) / 256 * 256;
+    // the counters in one place for all calls: what one writes behind them is no other one's counter
+    p.part_at = ATTENTION_MOST_CTAS * 4;
     p.lead_at = p.part_at + ((size_t)p.grid * 2 * p.rows * (hd + 2) * 4 + 255) / 256 * 256;
     p.bytes = p.lead_at + (p.lead ? (size_t)(p.splits / p.cluster) * n_q * batch * (hd + 2) * 4 : 0);
     return p;

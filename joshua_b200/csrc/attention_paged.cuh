@@ -45,7 +45,7 @@ struct PagedArgs {
     uint32_t common, done;  // leading pages named by the first sequence; leading pages that the other kernel takes
     float* out;
     uint64_t out_stride;
-    uint32_t* arrived;  // [batch * n_kv * split], zero between calls
+    uint32_t* arrived;  // a counter a CTA, for the segment that goes on behind it; zero between calls
     float* part;        // [grid][2][ROWS (HD + 2)]
     const float* lead;  // done: [lead_splits][n_kv][batch * group][HD], then their maxima, then their sums
     uint32_t lead_splits;

@@ -37,7 +37,7 @@ cudaError_t launch_kv_append(const KvPages& c, const RopeArgs& r, const float* q
 cudaError_t launch_kv_read(const KvPages& c, const int32_t* pos, const int32_t* seq, uint32_t rows, float* k, float* v,
                            uint64_t row_stride, uint64_t head_stride, int32_t* bad_pos, cudaStream_t s);
 // One query row a sequence and head over positions 0 .. len - 1; the first `shared` pages of sequence 0 are everybody's.
-constexpr uint32_t ATTENTION_MAX_BATCH = 4096;
+constexpr uint32_t ATTENTION_MAX_BATCH = 4096, ATTENTION_MOST_CTAS = 256;  // the scratch begins with a counter a CTA
 size_t attention_paged_scratch_bytes(uint32_t batch, uint32_t n_q, uint32_t n_kv, uint32_t hd, uint32_t shared);
 cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* len, uint32_t n_q, float scale,
                                    uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, int* error_flag,

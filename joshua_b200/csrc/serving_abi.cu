@@ -165,7 +165,7 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
     if (int32_t rc = check_cache(who, cache, page_table, batch, table_stride, &c)) return rc;
     if (int32_t rc = check_heads(who, cache, n_q)) return rc;
     if (!q || !len || !out || !scratch) return bad(who, "NULL buffer");
-    static_assert(JQ_ATTENTION_MAX_BATCH == jq::ATTENTION_MAX_BATCH, "header");
+    static_assert(JQ_ATTENTION_MAX_BATCH == jq::ATTENTION_MAX_BATCH && JQ_ATTENTION_SCRATCH_ZEROED == 4 * jq::ATTENTION_MOST_CTAS, "header");
     if (batch > JQ_ATTENTION_MAX_BATCH) return jq_fail(jq::E_TOO_LARGE, "jq_attention_paged_dev: more than JQ_ATTENTION_MAX_BATCH sequences");
     if ((uint64_t)batch * table_stride > 1u << 28) return bad(who, "a page table of more than 2^28 entries");
     if (shared_pages > table_stride) return bad(who, "more shared pages than a page table row has entries");

@@ -348,3 +348,25 @@ def test_a_negative_scale(kind, hd, n_q, n_kv, batch, shared):
         held = tuple(t.cpu().numpy() for t in cache.read(i32(range(lens[b])), table, seq=i32([b] * lens[b])))
         expect(got[b:b + 1], q[b:b + 1], [held], n_q, hd, scale=-0.2, tol=4 * TOL)   # up to 3.2 times the scores of scale 1 / sqrt(hd)
     cache.check_flags()
+
+
+def test_one_scratch_for_calls_of_all_sizes():
+    """What one call leaves is what the next one needs, whatever their batches, lengths, heads and shared pages."""
+    import torch
+
+    hd, calls = 128, []
+    for kind, n_q, n_kv, batch, length, shared in (("q8_0", 32, 8, 1, 3000, 0), ("q8_0", 32, 8, 100, 1700, 0), ("f16", 32, 8, 5, 900, 0), ("q8_0", 8, 2, 40, 300, 0),
+                                                   ("q4_0", 32, 8, 32, 1500, 20), ("q8_0", 8, 2, 3, 5000, 0), ("q8_0", 32, 8, 32, 1400, 20)):
+        cache, table = make(kind, n_kv, hd, batch, -(-length // 64))
+        if shared:
+            table[:, :shared] = table[0, :shared].clone()
+        lens = [length - b for b in range(batch)]
+        fill(cache, table, lens, seed=batch)
+        q = queries(batch, n_q, hd, batch)
+        n = i32(lens)
+        calls.append((cache, q, n, table, n_q, shared, cache.attend(q, n, table, n_q=n_q, shared_pages=shared)))
+    big = max((c.scratch(q.shape[0], n_q, shared) for c, q, _, _, n_q, shared, _ in calls), key=lambda s: s.numel())
+    for turn in range(3):
+        for c, q, n, table, n_q, shared, want in calls[::-1 if turn % 2 else 1]:
+            got = torch.full_like(want, 7.0)
+            assert torch.equal(c.attend(q, n, table, n_q=n_q, shared_pages=shared, out=got, scratch=big), want)
