@@ -45,7 +45,8 @@ class PagedCache:
         self.bad_pos = torch.zeros(1, dtype=torch.int32, device=pages.device)  # a row or a sequence had no place
         self._bad = self.bad_pos.data_ptr()
         self._append, self._read, self._attend = lib.jq_kv_append_dev, lib.jq_kv_read_dev, lib.jq_attention_paged_dev
-        self._scratch: dict = {}
+        self._scratch: dict = {}   # by stream: one, as large as the largest call so far
+        self._needs: dict = {}     # bytes by call
 
     def _table(self, table):
         if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.get_device() != self._index \
@@ -100,14 +101,22 @@ class PagedCache:
 
     def scratch(self, batch: int, n_q: int, shared_pages: int = 0) -> torch.Tensor:
         """Zeroed scratch for `attend` of such calls, one stream at a time."""
-        n = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages)
-        return torch.zeros(n // 4 + 4, dtype=torch.float32, device=self.device)
+        return torch.zeros(self._scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
+
+    def _scratch_bytes(self, batch: int, n_q: int, shared_pages: int) -> int:
+        key = batch, n_q, shared_pages
+        n = self._needs.get(key)
+        if n is None:
+            if len(self._needs) >= 1024:
+                self._needs.clear()
+            n = self._needs[key] = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages)
+        return n
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, scale: float = 0.0, shared_pages: int = 0,
                out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one query row per sequence, [batch, n_q * head_dim], over its first `lens` positions; the first
-        `shared_pages` pages are the same for all.  `scratch`: from `scratch()`; by default one a stream, kept with the cache
-        (while a graph is captured, the graph's own)."""
+        `shared_pages` pages are the same for all.  `scratch`: from `scratch()`, of this call or a larger one; by default one a
+        stream, kept with the cache (while a graph is captured, the graph's own)."""
         index, width = self._index, n_q * self.head_dim
         at, stride, batch = rows_arg(q, "q", width, index)
         n = batch
@@ -124,10 +133,9 @@ class PagedCache:
             if _capturing():  # the graph's own, zeroed by it: it may be replayed beside this stream's next call
                 scratch = self.scratch(batch, n_q, shared_pages)
             else:
-                key = (stream, batch, n_q, shared_pages)
-                scratch = self._scratch.get(key)
-                if scratch is None:
-                    scratch = self._scratch[key] = self.scratch(batch, n_q, shared_pages)
+                scratch = self._scratch.get(stream)
+                if scratch is None or 4 * scratch.numel() < self._scratch_bytes(batch, n_q, shared_pages):
+                    scratch = self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
         rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
                           shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)
         if rc:

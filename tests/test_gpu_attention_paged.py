@@ -370,3 +370,20 @@ def test_one_scratch_for_calls_of_all_sizes():
         for c, q, n, table, n_q, shared, want in calls[::-1 if turn % 2 else 1]:
             got = torch.full_like(want, 7.0)
             assert torch.equal(c.attend(q, n, table, n_q=n_q, shared_pages=shared, out=got, scratch=big), want)
+
+
+def test_a_cache_keeps_one_scratch_a_stream():
+    import torch
+
+    cache, table = make("q8_0", 8, 128, 32, 24)
+    table[:, :20] = table[0, :20].clone()
+    lens = i32([1400] * 32)
+    fill(cache, table, [1400] * 32, seed=1)
+    q = queries(32, 32, 128, 2)
+    before = cache.attend(q, lens, table, n_q=32)
+    kept = torch.cuda.memory_allocated()
+    for shared in range(21):
+        for batch in (32, 7, 1):
+            cache.attend(q[:batch], lens[:batch], table[:batch], n_q=32, shared_pages=shared, out=torch.empty_like(q[:batch]))
+    assert torch.cuda.memory_allocated() - kept <= 4 * cache.scratch(32, 32, 20).numel()
+    assert torch.equal(before, cache.attend(q, lens, table, n_q=32))
