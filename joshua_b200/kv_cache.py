@@ -16,6 +16,7 @@ from ._lib import JoshuaB200Error, check
 from .rope import Rope, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 PAGE = 64
+SCRATCH_ZEROED = 1024   # bytes at the beginning of a scratch, zero before its first call
 _capturing = torch.cuda.is_current_stream_capturing
 TYPES = {"f16": 1, "q4_0": 2, "q8_0": 8}
 
@@ -101,9 +102,9 @@ class PagedCache:
 
     def scratch(self, batch: int, n_q: int, shared_pages: int = 0) -> torch.Tensor:
         """Zeroed scratch for `attend` of such calls, one stream at a time."""
-        return torch.zeros(self._scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
+        return torch.zeros(self.scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
 
-    def _scratch_bytes(self, batch: int, n_q: int, shared_pages: int) -> int:
+    def scratch_bytes(self, batch: int, n_q: int, shared_pages: int = 0) -> int:
         key = batch, n_q, shared_pages
         n = self._needs.get(key)
         if n is None:
@@ -130,11 +131,12 @@ class PagedCache:
             raise JoshuaB200Error(_lib.E_INVALID, f"{batch} query rows, {n} rows of out, {n_seq} of the page table")
         stream = _raw_stream(index)
         if scratch is None:
-            if _capturing():  # the graph's own, zeroed by it: it may be replayed beside this stream's next call
-                scratch = self.scratch(batch, n_q, shared_pages)
+            if _capturing():  # the graph's own, its counters zeroed by it: it may be replayed beside this stream's next call
+                scratch = _new(self.scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
+                scratch[:SCRATCH_ZEROED // 4].zero_()
             else:
                 scratch = self._scratch.get(stream)
-                if scratch is None or 4 * scratch.numel() < self._scratch_bytes(batch, n_q, shared_pages):
+                if scratch is None or 4 * scratch.numel() < self.scratch_bytes(batch, n_q, shared_pages):
                     scratch = self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
         rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
                           shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)

@@ -1,18 +1,18 @@
 """The decoders of this package with their keys and values in pages of few bits, for batches of long sequences.
 
 Sequences take pages from one pool as they grow and give them back when they end (`release`); until its next prompt such a sequence
-rests: it takes part in steps with nothing to attend to, and what they leave for it means nothing.  Sequences that begin with the same prompt hold
-its full pages in common, and a step reads and multiplies those once for all of them (`share_prompt`).  Rotary positions come
-from a table (any scaling of `rope.rope_table`), the next tokens from `sampling.sample` where a sampling rule is set.
+rests: it takes part in steps with nothing to attend to, and what they leave for it means nothing.  Sequences that begin with the same
+prompt hold its full pages in common, and a step reads and multiplies those once for all of them (`share_prompt`).  Rotary positions
+come from a table (any scaling of `rope.rope_table`), the next tokens from `sampling.sample` where a sampling rule is set.
 
     dec = PagedLlamaDecoder(cfg, device, batch=32, max_ctx=8192, kv_type="q8_0")
     dec.share_prompt(prompt_ids)                 # or dec.prefill(ids, sequence=i) for each
     dec.sampling = dict(temperature=..., top_p=...)
     dec.uniform.uniform_(); dec.step()           # token by token
 
-A step may be captured in a graph by the caller, its pages reserved before.  The graph keeps the sampling rule's tensors, the penalty
-and the number of shared pages as they were: capture another one when they change.  Replays move `pos` alone; prompts, steps and
-host calls that follow (on the stream of the replays, or behind it) begin where it stands.
+A step may be captured in a graph by the caller, its pages reserved and one step run on the stream before.  The graph keeps the
+sampling rule's tensors, the penalty and the number of shared pages as they were: capture another one when they change.  Replays move
+`pos` alone; prompts, steps and host calls that follow (on the stream of the replays, or behind it) begin where it stands.
 """
 from __future__ import annotations
 
@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import JoshuaB200Error, check
-from .kv_cache import PAGE, PagedCache
+from .kv_cache import PAGE, SCRATCH_ZEROED, PagedCache
 from .llama import LlamaDecoder
 from .moe_decoder import MoeDecoder
 from .rope import Rope, rope_table
@@ -40,6 +40,7 @@ class _Paged:
         """`n_pages`: of the pool (default: enough for every sequence to reach max_ctx); `rope`: a table of max_ctx positions
         (default: the model's theta, unscaled, half layout)."""
         self.kv_type, self.pages_per_seq = kv_type, -(-max_ctx // PAGE)
+        self.shared_pages = 0                     # leading pages that all sequences have in common
         # resting sequences still bring a row to every append: to a position each of pages behind the pool
         self._places = min(PAGE, max_ctx)
         self.n_pages = batch * self.pages_per_seq if n_pages is None else n_pages
@@ -58,7 +59,6 @@ class _Paged:
         self.holders = [0] * self.n_pages         # sequences that have a page
         self.held = [0] * batch                   # positions each holds
         self._captured_by_caller = False          # then replays may have moved `pos` past `held`
-        self.shared_pages = 0                     # leading pages that all sequences have in common
         self.sampling: dict | None = None         # temperature, top_k, top_p, min_p: vectors of `batch`
         self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)   # numbers in [0, 1) for the next draw
 
@@ -67,7 +67,12 @@ class _Paged:
                                      device=self.dev))
 
     def _attention_scratch(self) -> None:
-        """The caches keep their own."""
+        """One scratch for the attention of all layers; one that a caller's graph may hold stays until the decoder goes."""
+        c, old = self.cfg, getattr(self, "att_scratch", [])
+        need = self.layers[0]["cache"].scratch_bytes(self.batch, c.q_heads, self.shared_pages)
+        if not old or old[-1].numel() < need:
+            size = max(need, 2 * old[-1].numel() if old else SCRATCH_ZEROED)   # all older ones together are smaller
+            self.att_scratch = [*old, torch.zeros(size, dtype=torch.uint8, device=self.dev)]
 
     def _index(self, sequence: int) -> int:
         if not 0 <= sequence < self.batch:
@@ -181,6 +186,7 @@ class _Paged:
                     ly["cache"].pages[self.owned[i][full]] = ly["cache"].pages[rest[0]]
             self.held[i] = n
         self.shared_pages = len(common)
+        self._attention_scratch()
         self.pos.fill_(n - 1)
         self.logits.copy_(self.logits[0:1].expand(self.batch, -1).clone())
         self._sample_rows(slice(0, self.batch))
@@ -259,7 +265,8 @@ class _Paged:
         c, cache = self.cfg, ly["cache"]
         cache.append(self.qkv, self.pos, self.table, n_q=c.q_heads, rope=self.rope, q_norm=ly["q_norm"] if self.qk_norm else None,
                      k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps, out=self.q)
-        cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, shared_pages=self.shared_pages, out=self.attn)
+        cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, shared_pages=self.shared_pages, out=self.attn,
+                     scratch=self.att_scratch[-1])
 
     def _sample(self, s) -> None:
         self._sample_rows(slice(0, self.batch))

@@ -413,3 +413,39 @@ def test_taking_pages_waits_for_nothing():
     assert not end.query() and dec.held == [65] * 4 and [len(mine) for mine in dec.owned] == [2] * 4
     whole(dec)
     dec.check_flags()
+
+
+def test_one_scratch_for_all_layers():
+    """Growing it leaves a graph of before as it was."""
+    import torch
+
+    dec, twin = make(70, max_ctx=2600), make(70, max_ctx=2600)
+    for d in (dec, twin):
+        for i in range(70):
+            d.prefill(ids(3, i), sequence=i)
+            d.reserve(i, 10)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        dec.step()                  # what a step needs on this stream is there before the capture
+        with torch.cuda.graph(graph, stream=side):
+            dec.step()
+        side.synchronize()
+    small = dec.att_scratch[-1].numel()
+    for d in (dec, twin):
+        d.reset()
+        d.share_prompt(ids(2500, 1))
+    host_and_step(dec, twin, tokens(2, 70, 2))
+    assert dec.att_scratch[-1].numel() > small
+    for d in (dec, twin):
+        d.reset()
+        for i in range(70):
+            d.prefill(ids(3, i), sequence=i)
+            d.reserve(i, 10)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph.replay(), graph.replay()
+        side.synchronize()
+    twin.step(), twin.step()
+    near(dec.logits, twin.logits)
+    dec.check_flags()
