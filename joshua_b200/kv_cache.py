@@ -138,6 +138,11 @@ class PagedCache:
                 scratch = self._scratch.get(stream)
                 if scratch is None or 4 * scratch.numel() < self.scratch_bytes(batch, n_q, shared_pages):
                     scratch = self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
+        else:
+            need = self.scratch_bytes(batch, n_q, shared_pages)
+            if not isinstance(scratch, torch.Tensor) or scratch.get_device() != index or not scratch.is_contiguous() \
+                    or scratch.numel() * scratch.element_size() < max(need, 1) or scratch.data_ptr() % 16:
+                raise JoshuaB200Error(_lib.E_INVALID, f"scratch must be {need} contiguous bytes on {self.device}, from a 16-byte boundary on")
         rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
                           shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)
         if rc:

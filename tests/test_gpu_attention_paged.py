@@ -387,3 +387,19 @@ def test_a_cache_keeps_one_scratch_a_stream():
             cache.attend(q[:batch], lens[:batch], table[:batch], n_q=32, shared_pages=shared, out=torch.empty_like(q[:batch]))
     assert torch.cuda.memory_allocated() - kept <= 4 * cache.scratch(32, 32, 20).numel()
     assert torch.equal(before, cache.attend(q, lens, table, n_q=32))
+
+
+def test_a_scratch_that_will_not_do():
+    import torch
+
+    cache, table = make("q8_0", 8, 128, 32, 24)
+    q, n = queries(32, 32, 128, 0), i32([1] * 32)
+    fill(cache, table, [1] * 32, seed=1)
+    fine = cache.scratch(32, 32, 20)
+    small = cache.scratch(32, 32)
+    assert small.numel() < fine.numel()
+    for bad in (small, fine[:fine.numel() // 2], fine.cpu(), fine[::2], fine[1:], 5, torch.zeros(0, device="cuda")):
+        with pytest.raises(JoshuaB200Error, match="scratch"):
+            cache.attend(q, n, table, n_q=32, shared_pages=20, scratch=bad)
+    whole = torch.zeros(fine.numel() * 4, dtype=torch.uint8, device="cuda")      # of any type
+    assert torch.equal(cache.attend(q, n, table, n_q=32, scratch=whole), cache.attend(q, n, table, n_q=32, scratch=small))
