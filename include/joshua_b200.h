@@ -346,7 +346,8 @@ int32_t jq_sample_greedy_dev(const float* logits, uint64_t rows, uint64_t vocab,
  * `sample_token` (src/engine.rs:2339-2378), with the cache in pages and in
  * fewer bits than the reference keeps it in.  f32 activations, device buffers,
  * a caller stream, no synchronisation, no allocation: all can be captured in a
- * graph.  Rows are 16-byte aligned.
+ * graph.  Rows are 16-byte aligned.  No context: buffers and stream belong to the
+ * calling thread's current device.
  *
  * Rotary positions come from a table of pairs, table[p][i] = m (cos, sin)(p f_i),
  * i < rot_dim / 2, which jq_rope_table_dev builds (in 64 bits, rounded once):

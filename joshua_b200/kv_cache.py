@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from ._lib import JoshuaB200Error, check
-from .rope import Rope, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
+from .rope import Rope, _device, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 PAGE = 64
 SCRATCH_ZEROED = 1024   # bytes at the beginning of a scratch, zero before its first call
@@ -61,6 +61,9 @@ class PagedCache:
         """Rows [rows, (n_q + 2 n_kv) * head_dim] at positions `pos` of sequences `seq` (None: row i is sequence i): keys and
         values into the cache, the rotated queries [rows, n_q * head_dim] returned."""
         index, hd, i32, f32 = self._index, self.head_dim, torch.int32, torch.float32
+        if index != _device():
+            with torch.cuda.device(index):
+                return self.append(qkv, pos, table, n_q, seq, rope, q_norm, k_norm, eps, out)
         at, stride, rows = rows_arg(qkv, "qkv", (n_q + 2 * self.n_kv) * hd, index)
         if out is None:
             out = _new(rows, n_q * hd, dtype=f32, device=self.device)
@@ -83,6 +86,9 @@ class PagedCache:
         """(keys, values) f32 [n_kv, rows, head_dim] of positions `pos` of sequences `seq` (None: row i is sequence i), into
         `out` (a pair of such tensors, [n_kv, at least rows, head_dim]) if given."""
         index, hd, n_kv = self._index, self.head_dim, self.n_kv
+        if index != _device():
+            with torch.cuda.device(index):
+                return self.read(pos, table, seq, out)
         rows = most = pos.size(0) if isinstance(pos, torch.Tensor) and pos.dim() else 0
         at = vector_arg(pos, "pos", rows, torch.int32, index)
         if out is None:
@@ -119,6 +125,9 @@ class PagedCache:
         `shared_pages` pages are the same for all.  `scratch`: from `scratch()`, of this call or a larger one; by default one a
         stream, kept with the cache (while a graph is captured, the graph's own)."""
         index, width = self._index, n_q * self.head_dim
+        if index != _device():
+            with torch.cuda.device(index):
+                return self.attend(q, lens, table, n_q, scale, shared_pages, out, scratch)
         at, stride, batch = rows_arg(q, "q", width, index)
         n = batch
         if out is None:

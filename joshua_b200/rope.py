@@ -15,6 +15,8 @@ from ._lib import JoshuaB200Error, check
 SCALINGS = {None: 0, "none": 0, "linear": 1, "yarn": 2}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
+# the entries launch on the current device, which need not be the tensors'
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
 _new, _f32 = torch.empty, torch.float32
 
 
@@ -103,6 +105,9 @@ class Rope:
               out: torch.Tensor | None = None) -> torch.Tensor:
         """Rows [rows, heads * head_dim] turned to their positions (`inverse`: back), into `out` (may be `x`)."""
         index, width = self._index, heads * head_dim
+        if index != _device():
+            with torch.cuda.device(index):
+                return self.apply(x, pos, heads, head_dim, inverse, out)
         at, stride, rows = rows_arg(x, "x", width, index)
         if out is None:
             out = _new(rows, width, dtype=_f32, device=self.device)

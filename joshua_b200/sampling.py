@@ -5,7 +5,7 @@ import torch
 
 from . import _lib
 from ._lib import JoshuaB200Error, check
-from .rope import _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
+from .rope import _device, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 WINDOW = 64
 _entry = None
@@ -24,6 +24,9 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=None, top_k=
         _entry = _lib.lib().jq_sample_dev
     f32, i32 = torch.float32, torch.int32
     index = device_index(logits, "logits", f32)
+    if index != _device():
+        with torch.cuda.device(index):
+            return sample(logits, uniform, temperature, top_k, top_p, min_p, repetition_penalty, window, window_state, pos, token)
     if logits.dim() != 2:
         raise JoshuaB200Error(_lib.E_INVALID, "logits must be [rows, vocab]")
     vocab = logits.size(1)
