@@ -433,6 +433,10 @@ int32_t jq_kv_read_dev(const jq_kv_cache* cache, const int32_t* pos, const int32
  * h / (n_q / n_kv); scale 0: 1 / sqrt(head_dim).  q and out rows are q_stride and out_stride floats apart.  len[b] = 0: zeros.
  *   shared_pages: the first so many pages are the same for the whole batch (a common prompt): read from the first sequence's
  * table entries, and once for all where that is the faster way.  Every len is then 0 or at least shared_pages * JQ_KV_PAGE.
+ *   Precision: keys and values as the cache holds them; queries as two f16 terms, 22 bits of the row's largest; probabilities times
+ * scales as two f16 terms, 22 bits of the largest of 16 to 64 positions: finer than the cache keeps a key or value, coarser than the
+ * three bf16 terms of jq_attention_prefill_dev.  Pages taken once for the batch: scales below 2^-21 of their page's largest are
+ * rounded, and the products of two small terms left out.  Maxima, sums and results are f32.
  *   A len outside its range or a page id outside the cache makes the sequence's rows NaN and sets *bad_pos_dev.
  *   scratch: jq_attention_paged_scratch_bytes(...) bytes of caller device memory, 16-byte aligned, its first
  * JQ_ATTENTION_SCRATCH_ZEROED bytes ZEROED once before the first call (they hold arrival counters that the kernels leave at

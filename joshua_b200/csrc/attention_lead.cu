@@ -12,8 +12,8 @@
 // What bounds it is the chain of a tile (scores' product, maximum of the row, exponentials, probabilities' product), not the
 // products: 1.65 us a page with heads of 128 in eight bits, 0.9 with heads of 64 in halves, of which the tensor pipe is busy 19%
 // and 28%; the softmax threads have half of an SM's registers, so a second tile cannot run beside the first.  32 sequences, 32
-// heads on 8 of 128, 64 pages: 20 us for 128 CTAs of four pages each, about 10 of them launch, queries and joining; by
-// attention_lead_kernel 55.
+// heads on 8 of 128, 64 pages: 22 us alone and cold for 128 CTAs of four pages each, about 10 of them launch, queries and joining; the
+// whole call with 100 positions of each sequence's own 26 us, with attention_lead_kernel in its place 42.
 //
 // Warps: 0 .. 7 softmax, two threads a query row (32 keys and half of the output dimensions each); 8 .. 15 turn the pages' codes
 // into swizzled K-major tiles, two stages; 16 issues the products; 17 copies the pages.  Tensor memory: the query's terms (the A

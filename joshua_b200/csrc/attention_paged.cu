@@ -912,9 +912,11 @@ constexpr uint32_t LEAD_WARPS = 8;
 constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }
 constexpr uint32_t lead_tiles(uint32_t hd) { return hd == 256 ? 1 : 2; }  // columns of a warp / 8, by its registers too
 
-// From so many query rows of a kv head on, the leading pages' kernel is the one of attention_lead.cu, whose time does not depend
-// on them up to 128 (32 query heads on 8 of 128, 8-bit, 64 pages, the kernel alone: 16 rows 34.9 us, here 29.8; 32 rows 28.5 and
-// 28.8; 128 rows 34.6 and 49.0; 512 rows 90.4 and 196.9).
+// From so many query rows of a kv head on, the leading pages' kernel is the one of attention_lead.cu, whose time hardly depends
+// on them up to 128 (32 query heads on 8 of 128, 8-bit, 64 pages, the whole call with 100 positions of each sequence's own, the pages
+// taken once on either side: 16 rows 22.7 us, by attention_lead_kernel 21.9; 24 rows 22.7 and 23.4; 32 rows 23.2 and 24.4; 64 rows
+// 23.9 and 29.8; 128 rows 26.0 and 42.4; 512 rows 56 and 113.  16 heads on 8, four bits, 200 pages: 16 rows 36.7 and 29.8, 24 rows
+// 37.1 and 36.4, 32 rows 37.4 and 37.5, 48 rows 38.3 and 52.0).
 constexpr uint32_t LEAD_TILE_ROWS = 32;
 // Leading pages are taken once for all sequences where that saves so many elements of keys (positions times dimensions, over all
 // passes) that the launch more and its joining, about 8 us, are won back; below, every sequence reads them by itself, most of it
