@@ -132,15 +132,19 @@ class _Paged:
             return
         self.resting[i] = False
         self.pos[i], self.active[i], self.idle_pos[i] = 0, 1, 0
-        super().seed_window(self._seeds.pop(i, []), i)   # steps have left ids there
+        self.window[i], self.window_state[i] = 0, 0   # steps have left ids there
+        if i in self._seeds:
+            super().seed_window(self._seeds.pop(i), i)
         self.shared_pages = 0       # it has other pages than those who share
 
     def reset(self, token: int = 42) -> None:
         """All sequences from position 0, none of them resting."""
-        for i in range(self.batch):
-            self.release(i)
-            self._wake(i)
-        self.table.fill_(-1)
+        for mine in self.owned:
+            self._give_back(mine)
+        self.owned, self.held, self.resting = [[] for _ in self.owned], [0] * self.batch, [False] * self.batch
+        self._seeds.clear()
+        self.shared_pages = 0
+        self.table.fill_(-1), self.active.fill_(1), self.idle_pos.zero_()
         super().reset(token)
 
     def seed_window(self, prompt_ids, sequence: int | None = None) -> None:
