@@ -47,7 +47,7 @@ class PagedCache:
         self._bad = self.bad_pos.data_ptr()
         self._append, self._read, self._attend = lib.jq_kv_append_dev, lib.jq_kv_read_dev, lib.jq_attention_paged_dev
         self._scratch: dict = {}   # by stream: one, as large as the largest call so far
-        self._needs: dict = {}     # bytes by call
+        self._needs: dict = {}     # bytes by call; by stream and call where the stream's scratch has them
 
     def _table(self, table):
         if not isinstance(table, torch.Tensor) or table.dtype is not torch.int32 or table.get_device() != self._index \
@@ -112,12 +112,21 @@ class PagedCache:
 
     def scratch_bytes(self, batch: int, n_q: int, shared_pages: int = 0) -> int:
         key = batch, n_q, shared_pages
-        n = self._needs.get(key)
-        if n is None:
-            if len(self._needs) >= 1024:
-                self._needs.clear()
-            n = self._needs[key] = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages)
-        return n
+        if key not in self._needs:
+            self._note(key, _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages))
+        return self._needs[key]
+
+    def _grow(self, stream: int, batch: int, n_q: int, shared_pages: int) -> None:
+        """A scratch of the stream for such calls."""
+        need, has = self.scratch_bytes(batch, n_q, shared_pages), self._scratch.get(stream)
+        if has is None or 4 * has.numel() < need:
+            self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
+        self._note((stream, batch, n_q, shared_pages), need)
+
+    def _note(self, key, n: int) -> None:
+        if len(self._needs) >= 1024:
+            self._needs.clear()
+        self._needs[key] = n
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, scale: float = 0.0, shared_pages: int = 0,
                out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
@@ -144,9 +153,9 @@ class PagedCache:
                 scratch = _new(self.scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
                 scratch[:SCRATCH_ZEROED // 4].zero_()
             else:
-                scratch = self._scratch.get(stream)
-                if scratch is None or 4 * scratch.numel() < self.scratch_bytes(batch, n_q, shared_pages):
-                    scratch = self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
+                if (stream, batch, n_q, shared_pages) not in self._needs:
+                    self._grow(stream, batch, n_q, shared_pages)
+                scratch = self._scratch[stream]
         else:
             need = self.scratch_bytes(batch, n_q, shared_pages)
             if not isinstance(scratch, torch.Tensor) or scratch.get_device() != index or not scratch.is_contiguous() \
