@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             float amax = 0.0f;
 #pragma unroll
             for (uint32_t i = 0; i < DN / 4; ++i) {
-                const float4 v = live ? __ldg(src + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float4 v = live ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 o[2 * i] = pair(v.x, v.y), o[2 * i + 1] = pair(v.z, v.w);
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             uint32_t k_sent = 0, v_sent = 0;
             int32_t ids = 0;
             for (uint32_t j = 0; j < n_tiles && ok; ++j) {
-                if (j % 32 == 0) ids = j + lane < n_tiles ? __ldg(a.c.table + p0 + j + lane) : 0;
+                if (j % 32 == 0) ids = j + lane < n_tiles ? a.c.table[p0 + j + lane] : 0;
                 const int32_t id = __shfl_sync(0xFFFFFFFFu, ids, j % 32);
                 const bool fine = id >= 0 && (uint32_t)id < a.c.n_pages;
                 if (!fine && lane == 0) sh.lost = 1;

@@ -457,7 +457,7 @@ struct Pages {
     __device__ __forceinline__ void fetch(uint32_t from) {
         const uint32_t p = from + lane;
         have = from;
-        ids = p < end ? __ldg((p < a.common ? a.c.table : table) + p) : 0;
+        ids = p < end ? (p < a.common ? a.c.table : table)[p] : 0;
     }
     __device__ __forceinline__ const uint8_t* tile(uint32_t p) {
         if (p - have >= 32) fetch(p);

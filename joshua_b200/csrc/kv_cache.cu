@@ -22,7 +22,7 @@ struct HeadLanes {
     __device__ __forceinline__ void load(const float* src, bool live) {
 #pragma unroll
         for (uint32_t i = 0; i < QUADS; ++i) {
-            const float4 v = live ? __ldg(reinterpret_cast<const float4*>(src + dim(i))) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const float4 v = live ? *reinterpret_cast<const float4*>(src + dim(i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
         }
     }
@@ -227,8 +227,8 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t ite
         for (uint32_t i = 0; i < AHEAD; ++i) {
             const uint32_t head = first + i * AT_ONCE + group;
             const float4 zero = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            next_u[i] = head < end ? __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_u)) : zero;
-            next_v[i] = head < end ? __ldg(reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_v)) : zero;
+            next_u[i] = head < end ? *reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_u) : zero;
+            next_v[i] = head < end ? *reinterpret_cast<const float4*>(src + (uint64_t)head * HD + at_v) : zero;
         }
     };
     request(head0);
@@ -331,9 +331,8 @@ __global__ void __launch_bounds__(256, 4) kv_append_kernel(AppendArgs a, uint32_
 
 // A warp a row and kv head, keys and values.
 template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvPages c, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
-                                                      float* __restrict__ k, float* __restrict__ v, uint64_t row_stride,
-                                                      uint64_t head_stride, int32_t* __restrict__ bad_pos) {
+__global__ void __launch_bounds__(256) kv_read_kernel(KvPages c, const int32_t* pos, const int32_t* seq, float* k, float* v, uint64_t row_stride,
+                                                      uint64_t head_stride, int32_t* bad_pos) {
     constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);
     pdl_trigger_all();
     const uint32_t row = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * 8 + (threadIdx.x >> 5);
@@ -471,9 +470,8 @@ __device__ __forceinline__ void read_rows(const KvPages& c, const int32_t* pos, 
     }
 }
 template <uint32_t KIND, uint32_t HD>
-__global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int32_t* __restrict__ pos, const int32_t* __restrict__ seq,
-                                                           uint32_t rows, float* __restrict__ k, float* __restrict__ v, uint64_t row_stride,
-                                                           uint64_t head_stride, int32_t* __restrict__ bad_pos) {
+__global__ void __launch_bounds__(256) kv_read_rows_kernel(KvPages c, const int32_t* pos, const int32_t* seq, uint32_t rows, float* k, float* v,
+                                                           uint64_t row_stride, uint64_t head_stride, int32_t* bad_pos) {
     pdl_trigger_all();
     const uint32_t task = blockIdx.y * 8 + (threadIdx.x >> 5), head = task / 2;
     if (head >= c.n_kv) return;

@@ -20,10 +20,9 @@ __global__ void __launch_bounds__(256) rope_table_kernel(RopeFrequencies f, uint
 
 // Eight dimensions a thread and head: four pairs and their table entries, read once for all heads that the thread takes (the
 // row's heads are spread over the threads of a CTA and over blockIdx.y).  Bound by memory: 2048 rows of 40 heads of 128 read and
-// written in 14.1 us (5.9 TB/s; 10.4 where they are still in L2), one row of 40 heads 1.8.
-__global__ void __launch_bounds__(256) rope_kernel(RopeArgs r, const float* __restrict__ x, uint64_t x_stride, const int32_t* __restrict__ pos,
-                                                   uint32_t heads, uint32_t hd, float sign, float* __restrict__ out, uint64_t out_stride,
-                                                   int32_t* __restrict__ bad_pos) {
+// written in 15.7 us (5.3 TB/s; 9.7 where they are still in L2), one row of 40 heads 1.7.
+__global__ void __launch_bounds__(256) rope_kernel(RopeArgs r, const float* x, uint64_t x_stride, const int32_t* pos, uint32_t heads,
+                                                   uint32_t hd, float sign, float* out, uint64_t out_stride, int32_t* bad_pos) {
     pdl_trigger_all();
     const uint32_t row = blockIdx.x, per_head = hd / 8, j = threadIdx.x % per_head;
     const uint32_t step = blockDim.x / per_head * gridDim.y, h0 = blockIdx.y * (blockDim.x / per_head) + threadIdx.x / per_head;
@@ -44,8 +43,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs r, const float* __re
     }
     const float* src = x + row * x_stride;
     float* dst = out + row * out_stride;
-#pragma unroll 4
-    for (uint32_t h = h0; h < heads; h += step) {
+    for (uint32_t h = h0; h < heads; h += step) {  // out may be x: a thread stores what it alone has loaded
         float4 u = *reinterpret_cast<const float4*>(src + h * hd + a), v = *reinterpret_cast<const float4*>(src + h * hd + b);
         if (turns) {
             float* first[4] = {&u.x, &u.y, &u.z, &u.w};
@@ -62,9 +60,8 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs r, const float* __re
 }
 
 // The same for heads or rotated parts that are no multiple of 8, two dimensions a thread.
-__global__ void __launch_bounds__(256) rope_pairs_kernel(RopeArgs r, const float* __restrict__ x, uint64_t x_stride,
-                                                         const int32_t* __restrict__ pos, uint32_t heads, uint32_t hd, float sign,
-                                                         float* __restrict__ out, uint64_t out_stride, int32_t* __restrict__ bad_pos) {
+__global__ void __launch_bounds__(256) rope_pairs_kernel(RopeArgs r, const float* x, uint64_t x_stride, const int32_t* pos, uint32_t heads,
+                                                         uint32_t hd, float sign, float* out, uint64_t out_stride, int32_t* bad_pos) {
     pdl_trigger_all();
     const uint32_t row = blockIdx.x, half = r.rot / 2;
     const int32_t p = pos[row];
@@ -104,7 +101,7 @@ cudaError_t launch_rope(const RopeArgs& r, const float* x, uint64_t x_stride, co
     cudaError_t e;
     if (hd % 8 == 0 && r.vectors) {
         // four heads a thread, fewer where the rows alone do not fill the GPU (40 heads of 128, from L2: one row 2.3 us with four
-        // heads a thread, 1.6 with one; 2048 rows 10.4 and 11.9)
+        // heads a thread, 1.7 with one; 2048 rows 9.7 and 10.8)
         const uint32_t at_once = std::max(1u, 256 / (hd / 8)), threads = at_once * (hd / 8);
         const uint32_t most = (heads + at_once - 1) / at_once, few = (most + 3) / 4;
         const uint32_t parts = std::min(most, std::max(few, (uint32_t)(8 * num_sms()) / rows));

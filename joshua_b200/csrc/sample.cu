@@ -427,12 +427,12 @@ __global__ void __launch_bounds__(SM_THREADS, 2) sample_kernel(SampleArgs a) {
             const uint32_t at = v + j * SM_THREADS;
             const int32_t id = lo + 4 * (int32_t)at;
             if (at < n / 4 && id >= 0 && id + 4 <= (int32_t)a.vocab) {
-                x[j] = __ldg(reinterpret_cast<const float4*>(src) + at);
+                x[j] = reinterpret_cast<const float4*>(src)[at];
             } else {
                 float* e = &x[j].x;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    e[k] = at < n / 4 && id + k >= 0 && id + k < (int32_t)a.vocab ? __ldg(src + 4 * (int32_t)at + k) : NAN;
+                    e[k] = at < n / 4 && id + k >= 0 && id + k < (int32_t)a.vocab ? src[4 * (int32_t)at + k] : NAN;
             }
         }
 #pragma unroll

@@ -9,7 +9,9 @@
 
 namespace jq {
 
-// The first two statements of a kernel whose predecessor in the stream may still run.
+// The first two statements of a kernel whose predecessor in the stream may still run.  What that one may have written is then read
+// by plain loads: read-only ones (__ldg, or plain ones through const __restrict__) may be moved above the wait, unless their address
+// comes from such a plain load.
 __device__ __forceinline__ void pdl_trigger_all() {
     pdl_trigger();
     pdl_wait();
