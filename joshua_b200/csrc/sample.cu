@@ -30,9 +30,9 @@ constexpr uint32_t SM_THREADS = 512, SM_WARPS = SM_THREADS / 32, SM_CTAS = 8, SM
 
 using u64 = unsigned long long;
 
-// Logits as whole numbers of the same order; NaN and -inf come last, as 0.
+// Logits as whole numbers of the same order, -0 and 0 as one; NaN and -inf come last, as 0.
 __device__ __forceinline__ uint32_t logit_key(float l) {
-    const uint32_t u = __float_as_uint(l);
+    const uint32_t u = __float_as_uint(l + 0.0f);
     return l > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
 }
 

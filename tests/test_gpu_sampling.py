@@ -237,3 +237,14 @@ def test_refusals():
     assert sample(l[:0], u[:0])[0].shape == (0,)
     token, _ = sample(torch.zeros(1, 393216, device="cuda"), torch.full((1,), 0.5, device="cuda"))
     assert int(token) == 196608
+
+
+@pytest.mark.parametrize("vocab", [30, 3000, 151936])
+def test_zeros_of_both_signs_are_equal(vocab):
+    """-0 and 0 are the same logit: the lower id goes first."""
+    l = np.full((5, vocab), -40.0, dtype=np.float32)   # the others weigh nothing
+    l[:, 10], l[:, vocab - 10] = -0.0, 0.0
+    l[4] = 0.0
+    l[4, ::2] = -0.0
+    token, _ = run(l, np.float32([0.5, 0.5, 0.5, 0.999, 0.5]), temperature=[0, 1, 1, 1, 1], top_k=[0, 1, 0, 2, 7], top_p=[1, 1, 0.3, 1, 1])
+    assert token.tolist() == [10, 10, 10, vocab - 10, 3]
