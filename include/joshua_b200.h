@@ -461,7 +461,7 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
  *   temperature <= 0: the maximum, its lowest id.  NULL: 1.
  * The sums are exact, so a row's token does not depend on the batch or the launch.  uniform: in [0, 1).
  * repetition_penalty, window and window_state as for jq_sample_greedy_dev; pos (may be NULL) is advanced by one per row.
- * logits: rows row_stride floats apart, read only; vocab <= JQ_SAMPLE_MAX_VOCAB. */
+ * logits: rows row_stride floats apart, read only; vocab <= JQ_SAMPLE_MAX_VOCAB, rows <= 65535. */
 #define JQ_SAMPLE_MAX_VOCAB 393216u
 int32_t jq_sample_dev(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float* uniform,
                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
