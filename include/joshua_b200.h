@@ -449,6 +449,26 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
                                uint32_t shared_pages, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos_dev,
                                void* stream);
 
+/* Attention of some new tokens of every sequence over its pages, the new ones included (append them first), causal: rows
+ * first[i] .. first[i + 1] - 1 of q (device int32 [batch + 1], ascending; NULL: rows / batch each) are the last positions of sequence
+ * i, which has len[i] with them.  The row at position p sees positions 0 .. p; with a window (0: none) the last `window` of them
+ * and the first `sinks`.  Page table entries of pages that no row of the sequence sees are not followed.  Rows that belong to no
+ * sequence are left as they were; a sequence without rows is not looked at.  len[i] = 0: zeros.
+ *   q, out, scale, scratch, and the precision: as for jq_attention_paged_dev.  A row does not depend on positions that it does not
+ * see, whatever they hold, but for the rounding of scales below 2^-21 (4 bits: 2^-25) of the largest of their page that some row of its
+ * sequence sees.
+ *   A len out of range (negative, above the page table, or fewer than the sequence's rows) or a page id outside the cache that a
+ * row sees makes rows of that sequence NaN (a page: those that see it, and rows near them) and sets *bad_pos_dev; so does a `first` that
+ * descends or passes `rows`, whose sequence stores nothing.
+ *   scratch: jq_attention_chunk_scratch_bytes(...) bytes; one that is large enough serves this entry and jq_attention_paged_dev.
+ * rows <= JQ_ATTENTION_MAX_ROWS, rows * n_q <= 2^27, rows * (4 table_stride + 8) < 2^32. */
+#define JQ_ATTENTION_MAX_ROWS 65536u
+uint64_t jq_attention_chunk_scratch_bytes(uint32_t batch, uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t head_dim);
+int32_t jq_attention_chunk_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* first, const int32_t* len,
+                               const int32_t* page_table, uint32_t batch, uint32_t table_stride, uint32_t rows, uint32_t n_q, float scale,
+                               uint32_t window, uint32_t sinks, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos_dev,
+                               void* stream);
+
 /* One token of every row of logits, drawn with a given random number: `sample_token` at temperature > 0
  * (src/engine.rs:2339-2378) with the usual rules, each row its own (device arrays of `rows`, each may be NULL).
  *   weight of a token: w = rint(2^32 e), e = exp((l - max) / temperature), a whole number; NaN and -inf weigh nothing.

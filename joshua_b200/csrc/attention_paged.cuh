@@ -35,6 +35,14 @@ __device__ __forceinline__ uint32_t codes4(uint32_t w) {
 
 constexpr uint32_t LEAD_MOST = 8;  // partial results of the leading pages
 
+// A call in which a sequence may bring several rows, its last positions, and see a part of its positions.
+struct SpanArgs {
+    const int32_t* first;  // rows first[b] .. first[b + 1] - 1 are sequence b's; NULL: `each` a sequence
+    uint32_t rows, each;
+    uint32_t few;            // sequences of more rows are another kernel's
+    uint32_t window, sinks;  // a row sees its own position, the window - 1 in front of it and the first `sinks`; window 0: all up to its own
+};
+
 struct PagedArgs {
     KvPages c;
     const float* q;
@@ -50,6 +58,31 @@ struct PagedArgs {
     const float* lead;  // done: [lead_splits][n_kv][batch * group][HD], then their maxima, then their sums
     uint32_t lead_splits;
     int32_t* bad_pos;
+    SpanArgs span;
+};
+
+// Rows of sequence b: the first one, how many (none if they are out of range), and its positions.
+struct SequenceRows {
+    uint32_t row, n;
+    int32_t len;  // -1: out of range
+    bool lost;    // its rows are out of range
+};
+__device__ __forceinline__ SequenceRows sequence_rows(const PagedArgs& a, uint32_t b) {
+    SequenceRows s{b * a.span.each, a.span.each, 0, false};
+    if (a.span.first) {
+        const int32_t r0 = a.span.first[b], r1 = a.span.first[b + 1];
+        s.lost = r0 < 0 || r1 < r0 || (uint32_t)r1 > a.span.rows;
+        s.row = s.lost ? 0 : r0, s.n = s.lost ? 0 : r1 - r0;
+    }
+    if (s.n == 0) return s;
+    s.len = a.len[b];
+    if (s.len < 0 || (uint32_t)s.len > a.c.table_stride * KV_PAGE || (s.len > 0 && (uint32_t)s.len < s.n)) s.len = -1;
+    return s;
+}
+// What a row sees: positions below `end`, from `low` on or below `sinks`.
+struct Sight {
+    uint32_t end, low, sinks;
+    __device__ __forceinline__ Sight(const SpanArgs& s, uint32_t pos) : end(pos + 1), low(s.window && end > s.window ? end - s.window : 0), sinks(s.sinks) {}
 };
 
 // Weight of a piece with maximum m under the joint maximum; equal ones are 1 (infinities too)

@@ -45,6 +45,14 @@ cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_
                                    uint32_t shared, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos, int* error_flag,
                                    cudaStream_t s);
 
+// Rows first[i] .. first[i + 1] - 1 (NULL: rows / n_seq each) of q are the last positions of sequence i, which has len[i]; window 0: a
+// row sees all positions up to its own, else that many and the first `sinks`.
+constexpr uint32_t ATTENTION_MAX_ROWS = 65536;
+size_t attention_chunk_scratch_bytes(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd);
+cudaError_t launch_attention_chunk(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* first, const int32_t* len, uint32_t rows,
+                                   uint32_t n_q, float scale, uint32_t window, uint32_t sinks, float* out, uint64_t out_stride,
+                                   void* scratch, int32_t* bad_pos, int* error_flag, cudaStream_t s);
+
 struct SampleArgs {
     const float* logits;
     uint64_t stride;

@@ -179,6 +179,42 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
     return jq::OK;
 }
 
+uint64_t jq_attention_chunk_scratch_bytes(uint32_t batch, uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t head_dim) {
+    if (batch == 0 || batch > JQ_ATTENTION_MAX_BATCH || rows == 0 || rows > JQ_ATTENTION_MAX_ROWS || n_kv == 0 || n_q == 0 || n_q % n_kv)
+        return 0;
+    return jq::attention_chunk_scratch_bytes(rows, n_q, n_kv, head_dim);
+}
+
+int32_t jq_attention_chunk_dev(const jq_kv_cache* cache, const float* q, uint64_t q_stride, const int32_t* first, const int32_t* len,
+                               const int32_t* page_table, uint32_t batch, uint32_t table_stride, uint32_t rows, uint32_t n_q, float scale,
+                               uint32_t window, uint32_t sinks, float* out, uint64_t out_stride, void* scratch, int32_t* bad_pos_dev,
+                               void* stream) {
+    constexpr const char* who = "jq_attention_chunk_dev";
+    if (batch == 0 || rows == 0) return jq::OK;
+    jq::KvPages c;
+    if (int32_t rc = check_cache(who, cache, page_table, batch, table_stride, &c)) return rc;
+    if (int32_t rc = check_heads(who, cache, n_q)) return rc;
+    if (!q || !len || !out || !scratch) return bad(who, "NULL buffer");
+    static_assert(JQ_ATTENTION_MAX_ROWS == jq::ATTENTION_MAX_ROWS, "header");
+    if (batch > JQ_ATTENTION_MAX_BATCH) return jq_fail(jq::E_TOO_LARGE, "jq_attention_chunk_dev: more than JQ_ATTENTION_MAX_BATCH sequences");
+    if (rows > JQ_ATTENTION_MAX_ROWS) return jq_fail(jq::E_TOO_LARGE, "jq_attention_chunk_dev: more than JQ_ATTENTION_MAX_ROWS rows");
+    if (!first && rows % batch) return bad(who, "rows that do not divide into equal parts need `first`");
+    if ((uint64_t)batch * table_stride > 1u << 28) return bad(who, "a page table of more than 2^28 entries");
+    // the kernels count steps of 16 positions, and rows times heads, in 32 bits
+    if ((uint64_t)rows * (4 * (uint64_t)table_stride + 8) > 0xFFFFFFFFull || (uint64_t)rows * n_q > 1u << 27)
+        return jq_fail(jq::E_TOO_LARGE, "jq_attention_chunk_dev: rows times positions, or rows times heads, are too many");
+    if (!std::isfinite(scale)) return bad(who, "the scale must be finite");
+    const uint64_t width = (uint64_t)n_q * cache->head_dim;
+    if (q_stride < width || out_stride < width || q_stride % 4 || out_stride % 4 || unaligned(q, out, scratch))
+        return bad(who, "rows of n_q * head_dim floats must not overlap; 16-byte boundaries");
+    if (scale == 0.0f) scale = 1.0f / std::sqrt((float)cache->head_dim);
+    const uint32_t most = table_stride * JQ_KV_PAGE;
+    if (window >= most) window = 0;
+    JQ_CUDA(jq::launch_attention_chunk(c, q, q_stride, first, len, rows, n_q, scale, window, window ? std::min(sinks, most) : 0, out,
+                                       out_stride, scratch, bad_pos_dev, jq_entry_status_flag(), static_cast<cudaStream_t>(stream)));
+    return jq::OK;
+}
+
 int32_t jq_sample_dev(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const float* uniform,
                       const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                       float repetition_penalty, int32_t* window, int32_t* window_state, int32_t* token, float* prob, int32_t* pos,

@@ -1,9 +1,10 @@
 """A key / value cache in pages of 64 positions, in halves, eight or four bits, and what is done with it: new positions rounded
-into it, positions read back, attention of one new token per sequence over it.
+into it, positions read back, attention of one new token per sequence over it, or of some of each.
 
 The caller owns the page table (int32 [sequences, pages a sequence]): position p of sequence i is in page `table[i, p // 64]`.
 Sequences may share leading pages (a common prompt); `attend(shared_pages=n)` then reads and multiplies them once for the batch where
-that is the faster way.
+that is the faster way.  With a window a token sees the last positions and the first few (sinks) only; table entries of pages that no token of
+a call sees may be anything.
 """
 from __future__ import annotations
 
@@ -46,6 +47,7 @@ class PagedCache:
         self.bad_pos = torch.zeros(1, dtype=torch.int32, device=pages.device)  # a row or a sequence had no place
         self._bad = self.bad_pos.data_ptr()
         self._append, self._read, self._attend = lib.jq_kv_append_dev, lib.jq_kv_read_dev, lib.jq_attention_paged_dev
+        self._chunk = lib.jq_attention_chunk_dev
         self._scratch: dict = {}   # by stream: one, as large as the largest call so far
         self._needs: dict = {}     # bytes by call; by stream and call where the stream's scratch has them
 
@@ -106,22 +108,33 @@ class PagedCache:
             check(rc)
         return out
 
-    def scratch(self, batch: int, n_q: int, shared_pages: int = 0) -> torch.Tensor:
-        """Zeroed scratch for `attend` of such calls, one stream at a time."""
-        return torch.zeros(self.scratch_bytes(batch, n_q, shared_pages) // 4 + 4, dtype=torch.float32, device=self.device)
+    def scratch(self, batch: int, n_q: int, shared_pages: int = 0, rows: int | None = None) -> torch.Tensor:
+        """Zeroed scratch for `attend` of such calls (with `rows`: for `attend_chunk`, or `attend` with a window), one stream at a time."""
+        return torch.zeros(self.scratch_bytes(batch, n_q, shared_pages, rows) // 4 + 4, dtype=torch.float32, device=self.device)
 
-    def scratch_bytes(self, batch: int, n_q: int, shared_pages: int = 0) -> int:
-        key = batch, n_q, shared_pages
+    def scratch_bytes(self, batch: int, n_q: int, shared_pages: int = 0, rows: int | None = None) -> int:
+        key = (batch, n_q, shared_pages) if rows is None else ("rows", batch, n_q, rows)
         if key not in self._needs:
-            self._note(key, _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages))
+            if rows is None:
+                need = _lib.lib().jq_attention_paged_scratch_bytes(batch, n_q, self.n_kv, self.head_dim, shared_pages)
+            else:
+                need = _lib.lib().jq_attention_chunk_scratch_bytes(batch, rows, n_q, self.n_kv, self.head_dim)
+            self._note(key, need)
         return self._needs[key]
 
-    def _grow(self, stream: int, batch: int, n_q: int, shared_pages: int) -> None:
+    def _grow(self, stream: int, batch: int, n_q: int, shared_pages: int, rows: int | None = None) -> None:
         """A scratch of the stream for such calls."""
-        need, has = self.scratch_bytes(batch, n_q, shared_pages), self._scratch.get(stream)
+        need, has = self.scratch_bytes(batch, n_q, shared_pages, rows), self._scratch.get(stream)
         if has is None or 4 * has.numel() < need:
-            self._scratch[stream] = self.scratch(batch, n_q, shared_pages)
-        self._note((stream, batch, n_q, shared_pages), need)
+            self._scratch[stream] = self.scratch(batch, n_q, shared_pages, rows)
+        self._note((stream, batch, n_q, shared_pages) if rows is None else (stream, "rows", batch, n_q, rows), need)
+
+    def _given(self, scratch, need: int) -> torch.Tensor:
+        """A caller's scratch, if it will do."""
+        if not isinstance(scratch, torch.Tensor) or scratch.get_device() != self._index or not scratch.is_contiguous() \
+                or scratch.numel() * scratch.element_size() < max(need, 1) or scratch.data_ptr() % 16:
+            raise JoshuaB200Error(_lib.E_INVALID, f"scratch must be {need} contiguous bytes on {self.device}, from a 16-byte boundary on")
+        return scratch
 
     def _note(self, key, n: int) -> None:
         if len(self._needs) >= 1024:
@@ -129,10 +142,17 @@ class PagedCache:
         self._needs[key] = n
 
     def attend(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, scale: float = 0.0, shared_pages: int = 0,
-               out: torch.Tensor | None = None, scratch: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, scratch: torch.Tensor | None = None, window: int = 0, sinks: int = 0) -> torch.Tensor:
         """Attention of one query row per sequence, [batch, n_q * head_dim], over its first `lens` positions; the first
-        `shared_pages` pages are the same for all.  `scratch`: from `scratch()`, of this call or a larger one; by default one a
-        stream, kept with the cache (while a graph is captured, the graph's own)."""
+        `shared_pages` pages are the same for all.  `window` (0: none): over the last so many of them and the first `sinks`; not with
+        shared pages.  `scratch`: from `scratch()`, of this call or a larger one; by default one a stream, kept with the cache (while a
+        graph is captured, the graph's own)."""
+        if window or sinks:
+            if shared_pages:
+                raise JoshuaB200Error(_lib.E_INVALID, "shared pages go without a window")
+            if isinstance(q, torch.Tensor) and isinstance(lens, torch.Tensor) and q.dim() == 2 and lens.dim() == 1 and q.size(0) != lens.size(0):
+                raise JoshuaB200Error(_lib.E_INVALID, f"{q.size(0)} query rows for {lens.size(0)} sequences")
+            return self.attend_chunk(q, lens, table, n_q, None, scale, window, sinks, out, scratch)
         index, width = self._index, n_q * self.head_dim
         if index != _device():
             with torch.cuda.device(index):
@@ -157,12 +177,50 @@ class PagedCache:
                     self._grow(stream, batch, n_q, shared_pages)
                 scratch = self._scratch[stream]
         else:
-            need = self.scratch_bytes(batch, n_q, shared_pages)
-            if not isinstance(scratch, torch.Tensor) or scratch.get_device() != index or not scratch.is_contiguous() \
-                    or scratch.numel() * scratch.element_size() < max(need, 1) or scratch.data_ptr() % 16:
-                raise JoshuaB200Error(_lib.E_INVALID, f"scratch must be {need} contiguous bytes on {self.device}, from a 16-byte boundary on")
+            self._given(scratch, self.scratch_bytes(batch, n_q, shared_pages))
         rc = self._attend(self._ref, at, stride, vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, n_q, scale,
                           shared_pages, to, out_stride, scratch.data_ptr(), self._bad, stream)
+        if rc:
+            check(rc)
+        return out
+
+    def attend_chunk(self, q: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, n_q: int, first: torch.Tensor | None = None,
+                     scale: float = 0.0, window: int = 0, sinks: int = 0, out: torch.Tensor | None = None,
+                     scratch: torch.Tensor | None = None) -> torch.Tensor:
+        """Attention of some new tokens of every sequence, [rows, n_q * head_dim], whose keys and values are in the cache: rows
+        `first[i]` .. `first[i + 1]` - 1 (int32 [sequences + 1]; None: as many of each) are the last positions of sequence i, which has
+        `lens[i]` with them.  A row sees the positions up to its own; with a `window` (0: none) the last so many and the first
+        `sinks`.  Rows of no sequence are left as they were in `out`.  `scratch`: from `scratch(rows=)`; by default as for `attend`."""
+        index, width = self._index, n_q * self.head_dim
+        if index != _device():
+            with torch.cuda.device(index):
+                return self.attend_chunk(q, lens, table, n_q, first, scale, window, sinks, out, scratch)
+        at, stride, rows = rows_arg(q, "q", width, index)
+        n = rows
+        if out is None:
+            out = _new(rows, width, dtype=torch.float32, device=self.device)
+            to, out_stride = out.data_ptr(), width
+        else:
+            to, out_stride, n = rows_arg(out, "out", width, index)
+        pages, batch, per = self._table(table)
+        if n != rows:
+            raise JoshuaB200Error(_lib.E_INVALID, f"{rows} query rows, {n} rows of out")
+        if not 0 <= window < 2**31 or not 0 <= sinks < 2**31 or sinks and not window:
+            raise JoshuaB200Error(_lib.E_INVALID, f"a window of {window} with {sinks} sinks")
+        stream = _raw_stream(index)
+        if scratch is None:
+            if _capturing():  # the graph's own, as in `attend`
+                scratch = _new(self.scratch_bytes(batch, n_q, 0, rows) // 4 + 4, dtype=torch.float32, device=self.device)
+                scratch[:SCRATCH_ZEROED // 4].zero_()
+            else:
+                if (stream, "rows", batch, n_q, rows) not in self._needs:
+                    self._grow(stream, batch, n_q, 0, rows)
+                scratch = self._scratch[stream]
+        else:
+            self._given(scratch, self.scratch_bytes(batch, n_q, 0, rows))
+        rc = self._chunk(self._ref, at, stride, None if first is None else vector_arg(first, "first", batch + 1, torch.int32, index),
+                         vector_arg(lens, "lens", batch, torch.int32, index), pages, batch, per, rows, n_q, scale, window, sinks, to, out_stride,
+                         scratch.data_ptr(), self._bad, stream)
         if rc:
             check(rc)
         return out
