@@ -488,6 +488,16 @@ int32_t jq_sample_dev(const float* logits, uint64_t row_stride, uint32_t rows, u
                       float repetition_penalty, int32_t* window, int32_t* window_state, int32_t* token, float* prob, int32_t* pos,
                       void* stream);
 
+/* Log probabilities of rows of logits, each row read once: log_prob[i] = l[token[i]] - log sum exp(l), entropy[i] (may be NULL) in
+ * nats, and the `top` (0 .. JQ_LOG_PROBS_MOST) likeliest tokens with theirs, top_token and top_log_prob [rows, top], in order, of equal
+ * logits the lower id first.
+ *   NaN and -inf weigh nothing and are not among the likeliest; +inf counts as the largest finite number.  Where fewer than `top`
+ * tokens weigh anything: id -1, -inf.  A row in which nothing does: -inf, entropy 0.  A token outside the vocabulary: NaN.
+ * logits: rows row_stride floats apart, read only; rows <= 2^24. */
+#define JQ_LOG_PROBS_MOST 32u
+int32_t jq_log_probs_dev(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const int32_t* token, uint32_t top,
+                         float* log_prob, float* entropy, int32_t* top_token, float* top_log_prob, void* stream);
+
 /* ── MoE layer ───────────────────────────────────────────────────────────
  * Replaces `Moe::forward` of the three loaders: routing, per-expert gather,
  * SwiGLU MLP over quantized expert banks, weighted scatter-add, optional

@@ -100,6 +100,7 @@ _SIGNATURES = {
     "jq_attention_paged_dev": (i32, [vp, vp, u64, vp, vp, u32, u32, u32, f32, u32, vp, u64, vp, vp, vp]),
     "jq_attention_chunk_scratch_bytes": (u64, [u32, u32, u32, u32, u32]),
     "jq_attention_chunk_dev": (i32, [vp, vp, u64, vp, vp, vp, u32, u32, u32, u32, f32, u32, u32, vp, u64, vp, vp, vp]),
+    "jq_log_probs_dev": (i32, [vp, u64, u32, u32, vp, u32, vp, vp, vp, vp, vp]),
     "jq_sample_dev": (i32, [vp, u64, u32, u32, vp, vp, vp, vp, vp, f32, vp, vp, vp, vp, vp, vp]),
     "jq_attention_fused_dev": (i32, [vp, vp, u32, u32, u32, u32, u32, f32, vp, vp, vp, vp, vp, vp]),
 }

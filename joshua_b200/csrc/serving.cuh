@@ -69,6 +69,21 @@ struct SampleArgs {
     float* prob;               // NULL: not wanted
     int32_t* pos;              // NULL: no positions to advance
 };
+// Log probability of a token of every row, entropy, the `top` likeliest tokens.
+struct LogProbArgs {
+    const float* logits;
+    uint64_t stride;
+    uint32_t vocab;
+    const int32_t* token;
+    uint32_t top;           // at most LOG_PROBS_MOST
+    float* log_prob;
+    float* entropy;         // NULL: not wanted
+    int32_t* top_token;     // [rows][top]
+    float* top_log_prob;
+};
+constexpr uint32_t LOG_PROBS_MOST = 32;
+cudaError_t launch_log_probs(const LogProbArgs& a, uint32_t rows, cudaStream_t s);
+
 constexpr uint32_t SAMPLE_MAX_VOCAB = 8 * 49152;
 cudaError_t launch_sample(const SampleArgs& a, uint32_t rows, cudaStream_t s);
 

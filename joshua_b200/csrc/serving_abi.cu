@@ -232,4 +232,19 @@ int32_t jq_sample_dev(const float* logits, uint64_t row_stride, uint32_t rows, u
     return jq::OK;
 }
 
+int32_t jq_log_probs_dev(const float* logits, uint64_t row_stride, uint32_t rows, uint32_t vocab, const int32_t* token, uint32_t top,
+                         float* log_prob, float* entropy, int32_t* top_token, float* top_log_prob, void* stream) {
+    constexpr const char* who = "jq_log_probs_dev";
+    static_assert(JQ_LOG_PROBS_MOST == jq::LOG_PROBS_MOST, "header");
+    if (rows == 0) return jq::OK;
+    if (!logits || !token || !log_prob) return bad(who, "NULL buffer");
+    if (vocab == 0 || vocab > 0x7FFFFFFFu || row_stride < vocab) return bad(who, "rows of 1 to 2^31 - 1 logits must not overlap");
+    if (rows > 1u << 24) return jq_fail(jq::E_TOO_LARGE, "jq_log_probs_dev: more than 2^24 rows");
+    if (top > JQ_LOG_PROBS_MOST) return jq_fail(jq::E_TOO_LARGE, "jq_log_probs_dev: more than JQ_LOG_PROBS_MOST tokens of a row");
+    if (top && (!top_token || !top_log_prob)) return bad(who, "NULL buffer of the likeliest tokens");
+    jq::LogProbArgs a{logits, row_stride, vocab, token, top, log_prob, entropy, top_token, top_log_prob};
+    JQ_CUDA(jq::launch_log_probs(a, rows, static_cast<cudaStream_t>(stream)));
+    return jq::OK;
+}
+
 }  // extern "C"

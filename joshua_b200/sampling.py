@@ -1,4 +1,5 @@
-"""Sampling on the device: temperature, top-k, top-p and min-p of every row, drawn with given random numbers."""
+"""Sampling on the device: temperature, top-k, top-p and min-p of every row, drawn with given random numbers; log probabilities of
+tokens, sampled or given."""
 from __future__ import annotations
 
 import torch
@@ -8,7 +9,7 @@ from ._lib import JoshuaB200Error, check
 from .rope import _device, _new, _raw_stream, block_arg, device_index, rows_arg, vector_arg
 
 WINDOW = 64
-_entry = None
+_entry = _scores = None
 
 
 def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=None, top_k=None, top_p=None, min_p=None,
@@ -46,3 +47,30 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=None, top_k=
     if rc:
         check(rc)
     return token, prob
+
+
+def log_probs(logits: torch.Tensor, token: torch.Tensor, top: int = 0):
+    """(log probability of `token`, entropy, ids of the `top` likeliest tokens, their log probabilities) of logits [rows, vocab]: f32
+    [rows], f32 [rows] in nats, int32 and f32 [rows, top].
+
+    `token`: int32 [rows]; one outside the vocabulary gives NaN.  The likeliest come in order, of equal logits the lower id
+    first; where fewer weigh anything (NaN and -inf do not), -1 and -inf."""
+    global _scores
+    if _scores is None:
+        _scores = _lib.lib().jq_log_probs_dev
+    f32, i32 = torch.float32, torch.int32
+    index = device_index(logits, "logits", f32)
+    if index != _device():
+        with torch.cuda.device(index):
+            return log_probs(logits, token, top)
+    if logits.dim() != 2 or not 0 <= top < 2**31:
+        raise JoshuaB200Error(_lib.E_INVALID, "logits must be [rows, vocab], top not negative")
+    vocab, device = logits.size(1), logits.device
+    at, stride, rows = rows_arg(logits, "logits", vocab, index)
+    given = vector_arg(token, "token", rows, i32, index)
+    out = (_new(rows, dtype=f32, device=device), _new(rows, dtype=f32, device=device), _new(rows, top, dtype=i32, device=device),
+           _new(rows, top, dtype=f32, device=device))
+    rc = _scores(at, stride, rows, vocab, given, top, *[t.data_ptr() for t in out], _raw_stream(index))
+    if rc:
+        check(rc)
+    return out
