@@ -2,28 +2,37 @@
 //
 // Rows first[b] .. first[b + 1] - 1 of q are the last positions of sequence b.  Row r at position p: out[r, head, :] =
 // sum_t e_t V_t / sum_t e_t, e_t = exp(scale q . K_t - max), over t <= p with (no window, or p - t < window, or t < sinks).
-// Rows are taken one by one, each as a sequence of its own by attention_paged_kernel (attention_steps.cuh), cut into equal pieces of
-// work whatever the lengths: the codes of its positions are read once a row.
+// Sequences of few rows, and all with heads of 256, are taken row by row, each as a sequence of its own by attention_paged_kernel
+// (attention_steps.cuh), cut into equal pieces of work whatever the lengths: the codes of its positions are read once a row.  The
+// others go to the tiles of attention_chunk_tiles.cu.  Which are which is known on the device alone where `first` tells: both are
+// launched then, and each leaves the other's sequences.
 #include <algorithm>
 
+#include "attention_chunk.cuh"
 #include "attention_steps.cuh"
 
 namespace jq {
 
 namespace {
 
+constexpr uint32_t CHUNK_FEW = 1;
+
 struct ChunkPlan {
     uint32_t group, rows, split, grid;  // query heads a kv head; of a warp; warps' worth of them; CTAs
+    uint32_t few;                       // rows of a sequence that are taken one by one
+    bool tiles;                         // some sequence may have more
     size_t part_at, bytes;
 };
-ChunkPlan plan(uint32_t n_q, uint32_t n_kv, uint32_t hd) {
+ChunkPlan plan(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd) {
     ChunkPlan p{};
     p.group = n_q / n_kv;
     p.rows = p.group <= 4 ? 4 : 8;
     p.split = (p.group + p.rows - 1) / p.rows;
     p.grid = std::min((uint32_t)num_sms(), ATTENTION_MOST_CTAS);
     p.part_at = ATTENTION_MOST_CTAS * 4;
-    p.bytes = p.part_at + (size_t)p.grid * 2 * p.rows * (hd + 2) * 4;
+    p.few = hd <= 128 ? CHUNK_FEW : 0xFFFFFFFFu;
+    p.tiles = rows > p.few;
+    p.bytes = p.part_at + (size_t)p.grid * 2 * (p.tiles ? CHUNK_TILE_ROWS : p.rows) * (hd + 2) * 4;
     return p;
 }
 
@@ -50,16 +59,20 @@ struct LaunchChunk {
 
 }  // namespace
 
-size_t attention_chunk_scratch_bytes(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd) { return plan(n_q, n_kv, hd).bytes; }
+size_t attention_chunk_scratch_bytes(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd) { return plan(rows, n_q, n_kv, hd).bytes; }
 
 cudaError_t launch_attention_chunk(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* first, const int32_t* len, uint32_t rows,
                                    uint32_t n_q, float scale, uint32_t window, uint32_t sinks, float* out, uint64_t out_stride,
                                    void* scratch, int32_t* bad_pos, int* error_flag, cudaStream_t s) {
-    const ChunkPlan p = plan(n_q, c.n_kv, c.hd);
+    const ChunkPlan p = plan(rows, n_q, c.n_kv, c.hd);
     uint8_t* mem = static_cast<uint8_t*>(scratch);
     PagedArgs a{c, q, q_stride, len, n_q, p.group, p.split, scale, 0, 0, out, out_stride,
                 reinterpret_cast<uint32_t*>(mem), reinterpret_cast<float*>(mem + p.part_at), nullptr, 0, bad_pos};
-    a.span = SpanArgs{first, rows, first ? 0 : rows / c.n_seq, 0xFFFFFFFFu, window, sinks};
+    a.span = SpanArgs{first, rows, first ? 0 : rows / c.n_seq, p.few, window, sinks};
+    if (first ? p.tiles : a.span.each > p.few) {
+        cudaError_t e = launch_attention_chunk_tiles(a, p.grid, error_flag, s);
+        if (e != cudaSuccess || !first) return e != cudaSuccess ? e : cudaGetLastError();
+    }
     cudaError_t e = for_kind(c.kind, c.hd, LaunchChunk{a, p, s});
     return e != cudaSuccess ? e : cudaGetLastError();
 }
