@@ -3,17 +3,17 @@
 // A tile is up to 128 query rows: the heads of a kv head of consecutive tokens of a sequence, token by token.  It goes over the pages
 // that some of its tokens sees, a page at a time, running maximum and sum in f32.  Terms as in attention_lead.cu: queries two f16 terms
 // under a power of two of their row; codes times scales as two f16 terms (halves: one) under powers of two of a page's largest scale;
-// probabilities two terms; of a product of two terms each the smallest of the four is left out.  Accumulators hold 64 dimensions of a
-// score or one page of the output; the running output lives in registers.  Scores of positions that a row does not see become nothing
+// probabilities two terms; of a product of two terms each the smallest of the four is left out.  Accumulators hold a score or one page
+// of the output; the running output lives in registers.  Scores of positions that a row does not see become nothing
 // before the maximum, their probabilities zeros; values behind the tile's last position are zeros in the products, and those that are
 // not finite too: they are added at the end, to the rows that see them.
 //
 // The tiles' work stands in one row of units, tile by tile, kv head by kv head, SEG_UNITS for beginning and ending one, then its
 // pages.  It is cut into equal pieces, one a CTA; pieces of a tile that several CTAs have are joined by the last of them to arrive, in order.
 //
-// Warps: 0 .. 15 softmax, four threads a query row (16 keys and a quarter of the output dimensions each); 16 .. 23 first cut the work,
-// then turn the pages' codes into swizzled K-major tiles, two stages; 24 issues the products; 25 copies the pages.  Tensor memory: the
-// query's terms (the A operand of the scores), scores, probabilities (A of the output), output of a page.
+// Warps: 0 .. 3 softmax, a thread a query row; 4 .. 11 first cut the work, then turn the pages' codes into swizzled tiles, two stages; 12
+// issues the products; 13 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
+// (A of the output) of two pages, output of one.
 //
 // Every wait on an mbarrier is bounded.  A warp whose wait ran out waits for none any more, hands nothing on, and goes through the
 // rest of its work so, which brings it to every barrier that others expect it at; the status flag is raised and the rows become NaN.
@@ -27,16 +27,14 @@ namespace jq {
 namespace {
 
 constexpr uint32_t CQ = CHUNK_TILE_ROWS;     // query rows of a tile
-constexpr uint32_t C_SOFT = 16, C_CONV = 8;  // warps
-constexpr uint32_t C_PARTS = C_SOFT / 4;     // threads a row
-constexpr uint32_t C_KEYS = KV_PAGE / C_PARTS;
+constexpr uint32_t C_SOFT = 4, C_CONV = 8;   // warps
 constexpr int UP = 6;                        // probabilities stand times 2^UP ..
 constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
 constexpr uint32_t C_THREADS = (C_SOFT + C_CONV + 4) * 32;  // whole warpgroups: they trade registers
-// Registers a thread: the launch has 896 x 72 = 64512, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 56 and the
-// softmax threads (32 running outputs, 16 scores, 16 terms) 512 x 88.
-constexpr int C_REGS_ISSUE = 32, C_REGS_CONV = 56, C_REGS_SOFT = 88;
-static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT <= C_THREADS * 72, "registers");
+// Registers a thread: the launch has 512 x 128 = 65536, of which the issuer's warpgroup keeps 128 x 64, the converters 256 x 104 and the
+// softmax threads (128 running outputs, 32 scores, 32 terms) 128 x 240.
+constexpr int C_REGS_ISSUE = 64, C_REGS_CONV = 104, C_REGS_SOFT = 240;
+static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT <= C_THREADS * 128, "registers");
 
 constexpr uint32_t SEG_UNITS = 2;   // a tile's beginning and end in pages
 constexpr uint32_t C_PIECES = 96;   // pieces of a CTA at a time
@@ -56,8 +54,7 @@ struct ChunkShared {
     float vs[4][4];           // inverse scales of the values' blocks, by page % 4
     uint8_t odd[4][C_CONV];   // values that are not finite, by page % 4 and converter
     uint8_t lost[8];          // a page id outside the cache, by page % 8
-    float row[2][C_PARTS][CQ];
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full, s_free, p_full, o_full;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], q_full, p_full, o_full;
     uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];  // the raw pages
     uint64_t drained;         // the products of a CTA that gives up
     uint32_t tmem_slot;
@@ -68,6 +65,231 @@ struct ChunkShared {
     ChunkPiece piece[C_PIECES];
 };
 
+template <uint32_t V>
+struct Constant {
+    static constexpr uint32_t value = V;
+};
+
+// The WARPS warps that turn pages into operands: keys K-major (dimensions along a row), values MN-major (the same), so that no lane
+// needs another's codes.  Only the first `valid` positions of a page are anyone's: what stands behind them does not count for the
+// page's scales, and values there, or not finite, become zeros.  Scales are looked over once a page for what is not finite; the path
+// without any has no masks.
+template <uint32_t KIND, uint32_t HD, uint32_t WARPS>
+struct ChunkConverter {
+    using T = PageTile<KIND, HD>;
+    static constexpr uint32_t NB = T::NB, CODES = kv_code_bytes(KIND, HD), K_LO = T::HALVES * T::K_PLANE, V_LO = T::V_PLANE;
+    static constexpr uint32_t BLOCKS = KIND == KV_Q4_0 ? 2 : 1, COLS = NB / BLOCKS, ITEMS = 4 * COLS;  // blocks of a lane's 16 bytes
+    static constexpr int TOP = KIND == KV_Q4_0 ? 26 : 22;  // a scale below 2^(e - 14) times 2^(TOP - e) times a code stays below 2^15
+    static_assert(WARPS % COLS == 0, "a warp has blocks of its own");
+    uint32_t cw, lane, r, c, b0;
+    uint32_t key_to, value_to[2];  // places in a stage: keys of row r, values of positions 2 c and 2 c + 1
+
+    __device__ __forceinline__ ChunkConverter(uint32_t warp, uint32_t lane_)
+        : cw(warp), lane(lane_), r(lane_ / 4), c(lane_ % 4), b0(warp % COLS * BLOCKS) {
+        key_to = b0 / 2 * T::K_PLANE + r * 128 + (((b0 % 2 * 4 + c) ^ r) << 4);
+        for (uint32_t e = 0; e < 2; ++e)
+            value_to[e] = b0 / 2 * (KV_PAGE * 128) + (2 * c + e) * 128 + (((b0 % 2 * 4 + r / 2) ^ (2 * c + e)) << 4) + r % 2 * 8;
+    }
+    // halfwords of positions at and at + 8 that are there; those of finite numbers
+    __device__ __forceinline__ static uint32_t there(uint32_t at, uint32_t valid) {
+        return (at < valid ? 0xFFFFu : 0u) | (at + 8 < valid ? 0xFFFF0000u : 0u);
+    }
+    __device__ __forceinline__ static uint32_t finite(uint32_t w) { return __vcmpltu2(w & 0x7FFF7FFFu, 0x7C007C00u); }
+    // the largest magnitude of scales (four of a position unit in 8 bytes: positions at + 8 k), as bits; first those not finite too
+    template <uint32_t N>
+    __device__ __forceinline__ static uint32_t largest(uint2 (&v)[N], const uint32_t (&at)[N], uint32_t valid, bool* odd) {
+        if (valid < KV_PAGE) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) v[i].x &= there(at[i], valid), v[i].y &= there(at[i] + 16, valid);
+        }
+        auto top_of = [&] {
+            uint32_t t = 0x04000400u;  // not below the smallest normal number
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) t = __vmaxu2(t, __vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu));
+            return __reduce_max_sync(0xFFFFFFFFu, max(t >> 16, t & 0xFFFFu));
+        };
+        uint32_t top = top_of();
+        *odd = top >= 0x7C00u;
+        if (*odd) {
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) v[i].x &= finite(v[i].x), v[i].y &= finite(v[i].y);
+            top = top_of();
+        }
+        return top;
+    }
+    // factors whose product is 2^(TOP - e)
+    struct Up {
+        __half2 a, b;
+        __device__ __forceinline__ explicit Up(int e) {
+            const int n = TOP - e, half = n >> 1;
+            const uint32_t x = (uint32_t)(15 + half) << 10, y = (uint32_t)(15 + n - half) << 10;
+            a = bits_half2(x | x << 16), b = bits_half2(y | y << 16);
+        }
+        __device__ __forceinline__ uint32_t of(uint32_t s) const { return half2_bits(__hmul2(__hmul2(bits_half2(s), a), b)); }
+    };
+    __device__ __forceinline__ static __half2 low(uint32_t s) { return bits_half2(__byte_perm(s, 0, 0x1010)); }
+    __device__ __forceinline__ static __half2 high(uint32_t s) { return bits_half2(__byte_perm(s, 0, 0x3232)); }
+
+    // a page's keys; *inverse: what their products are multiplied by
+    __device__ __forceinline__ void keys(uint32_t stage, const uint8_t* raw, uint32_t valid, float* inverse) const {
+        if constexpr (KIND == KV_F16) {
+#pragma unroll
+            for (uint32_t i = cw; i < ITEMS; i += WARPS) {
+                const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 1024 + lane * 16), y = *reinterpret_cast<const uint4*>(raw + i * 1024 + 512 + lane * 16);
+                const uint32_t to = stage + key_to + i / COLS * 2048;
+                sts_v4(to, {x.x, x.y, y.x, y.y}), sts_v4(to + 1024, {x.z, x.w, y.z, y.w});
+            }
+        } else {
+            constexpr uint32_t N = NB / 2;  // 8-byte units of a lane
+            uint2 v[N];
+            uint32_t at[N];
+#pragma unroll
+            for (uint32_t i = 0; i < N; ++i) {
+                const uint32_t unit = lane * N + i;
+                v[i] = *reinterpret_cast<const uint2*>(raw + CODES + unit * 8), at[i] = unit / NB / 8 * 32 + unit / NB % 8;
+            }
+            bool odd;
+            const int e = (int)(largest(v, at, valid, &odd) >> 10);
+            const Up up(e);
+            if (cw == 0 && lane == 0) *inverse = power(e - TOP);
+#pragma unroll
+            for (uint32_t i = cw; i < ITEMS; i += WARPS) {
+                const uint32_t g = i / COLS, to = stage + key_to + g * 2048;
+                const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                const uint8_t* scales = raw + CODES + (g / 2 * 8 + r) * NB * 8 + g % 2 * 4 + b0 * 8;  // of rows r and r + 8, by block
+#pragma unroll
+                for (uint32_t o = 0; o < BLOCKS; ++o) {
+                    const uint32_t s = up.of(*reinterpret_cast<const uint32_t*>(scales + o * 8));
+                    const __half2 s0 = low(s), s1 = high(s);
+                    uint32_t hi[2][4], lo[2][4];
+                    if constexpr (KIND == KV_Q8_0) {
+#pragma unroll
+                        for (uint32_t q = 0; q < 2; ++q) {
+                            scaled_terms(codes8<0>(w[q]), s0, &hi[0][2 * q], &lo[0][2 * q]), scaled_terms(codes8<2>(w[q]), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
+                            scaled_terms(codes8<0>(w[2 + q]), s1, &hi[1][2 * q], &lo[1][2 * q]);
+                            scaled_terms(codes8<2>(w[2 + q]), s1, &hi[1][2 * q + 1], &lo[1][2 * q + 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t q = 0; q < 2; ++q) {
+                            const uint32_t u = w[2 * o + q];
+                            scaled_terms(codes4<0>(u), s0, &hi[0][2 * q], &lo[0][2 * q]), scaled_terms(codes4<1>(u), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
+                            scaled_terms(codes4<2>(u), s1, &hi[1][2 * q], &lo[1][2 * q]), scaled_terms(codes4<3>(u), s1, &hi[1][2 * q + 1], &lo[1][2 * q + 1]);
+                        }
+                    }
+                    const uint32_t block = to ^ o << 6;  // the second block of a pair stands four 16-byte pieces on, in the swizzle
+                    sts_v4(block, hi[0]), sts_v4(block + K_LO, lo[0]);
+                    sts_v4(block + 1024, hi[1]), sts_v4(block + 1024 + K_LO, lo[1]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ static void sts_v2(uint32_t addr, uint32_t a, uint32_t b) {
+        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+    }
+    // Two dimensions (x = 0, 1) of the position of half h and place e: of a word of Q8_0 codes [x][e], of Q4_0 codes [e][h].
+    template <uint32_t E, uint32_t H>
+    __device__ __forceinline__ static uint32_t value_codes(uint32_t w) {
+        if constexpr (KIND == KV_Q8_0) {
+            return half2_bits(__hsub2(bits_half2(__byte_perm(w, 0x64646464u, E ? 0x4341 : 0x4240)), __float2half2_rn(1152.0f)));
+        } else {  // 1024 + n and 1024 + 16 n
+            constexpr uint32_t BYTE = 2 * E + H;
+            const uint32_t t = __byte_perm(w, 0x64646464u, 0x4040 | BYTE << 8 | BYTE) & 0xFFF0FF0Fu;
+            return half2_bits(__hfma2(bits_half2(t), __halves2half2(__float2half_rn(1.0f), __float2half_rn(0.0625f)),
+                                      __halves2half2(__float2half_rn(-1032.0f), __float2half_rn(-72.0f))));
+        }
+    }
+    // a page's values; inverse: what the products of each block are multiplied by.  True: some value that is there is not finite.
+    __device__ __forceinline__ bool values(uint32_t stage, const uint8_t* raw, uint32_t valid, float* inverse) const {
+        if constexpr (KIND == KV_F16) {
+            bool odd = false;
+#pragma unroll
+            for (uint32_t i = cw; i < ITEMS; i += WARPS) {
+                const uint32_t g = i / COLS;
+                uint32_t w[2][4];
+                __half2 zero = __float2half2_rn(0.0f);
+                if (valid < KV_PAGE) zero = __float2half2_rn(NAN);  // looked at one by one
+#pragma unroll
+                for (uint32_t m = 0; m < 2; ++m) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 1024 + m * 512 + lane * 16);
+                    w[m][0] = x.x, w[m][1] = x.y, w[m][2] = x.z, w[m][3] = x.w;
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) zero = __hfma2(bits_half2(w[m][k]), __float2half2_rn(0.0f), zero);
+                }
+                if (__any_sync(0xFFFFFFFFu, (half2_bits(zero) & 0x7FFF7FFFu) != 0)) {
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; ++k) {  // positions 16 g + 8 (k / 2 % 2) + 2 c and the next
+                        uint32_t& x = w[k / 4][k % 4];
+                        const uint32_t at = 16 * g + k / 2 % 2 * 8 + 2 * c;
+                        x &= (at < valid ? 0xFFFFu : 0u) | (at + 1 < valid ? 0xFFFF0000u : 0u);
+                        const uint32_t fine = finite(x);
+                        odd |= fine != 0xFFFFFFFFu, x &= fine;
+                    }
+                }
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+                    for (uint32_t e = 0; e < 2; ++e) {
+                        const uint32_t order = e ? 0x7632 : 0x5410;
+                        sts_v2(stage + value_to[e] + g * 2048 + h * 1024, __byte_perm(w[0][2 * h], w[0][2 * h + 1], order),
+                               __byte_perm(w[1][2 * h], w[1][2 * h + 1], order));
+                    }
+            }
+            return odd;
+        } else {
+            // lanes 0 .. 15 (and again 16 .. 31) have the block's scales of positions 32 (lane / 8) + lane % 8 + 8 k
+            bool odd[BLOCKS], careful = valid < KV_PAGE;
+            int e[BLOCKS];
+#pragma unroll
+            for (uint32_t o = 0; o < BLOCKS; ++o) {
+                uint2 v[1] = {*reinterpret_cast<const uint2*>(raw + CODES + ((lane & 15) * NB + b0 + o) * 8)};
+                const uint32_t at[1] = {(lane & 15) / 8 * 32 + lane % 8};
+                e[o] = (int)(largest(v, at, valid, &odd[o]) >> 10);
+                if (cw < COLS && lane == 0) inverse[b0 + o] = power(e[o] - TOP);
+                careful |= odd[o];
+            }
+#pragma unroll
+            for (uint32_t i = cw; i < ITEMS; i += WARPS) {
+                const uint32_t g = i / COLS;
+                const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (uint32_t o = 0; o < BLOCKS; ++o) {
+                    const Up up(e[o]);
+                    uint32_t s[2];  // of places e: halves h
+#pragma unroll
+                    for (uint32_t p = 0; p < 2; ++p) {
+                        s[p] = *reinterpret_cast<const uint32_t*>(raw + CODES + ((g / 2 * 8 + 2 * c + p) * NB + b0 + o) * 8 + g % 2 * 4);
+                        if (careful) s[p] &= there(16 * g + 2 * c + p, valid) & finite(s[p]);
+                        s[p] = up.of(s[p]);
+                    }
+                    auto put = [&](auto place, auto half) {
+                        constexpr uint32_t E = decltype(place)::value, H = decltype(half)::value;
+                        const __half2 f = H ? high(s[E]) : low(s[E]);
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (uint32_t m = 0; m < 2; ++m)
+                            scaled_terms(value_codes<E, H>(KIND == KV_Q8_0 ? w[2 * m + H] : w[2 * o + m]), f, &hi[m], &lo[m]);
+                        const uint32_t to = (stage + value_to[E] + g * 2048 + H * 1024) ^ o << 6;
+                        sts_v2(to, hi[0], hi[1]), sts_v2(to + V_LO, lo[0], lo[1]);
+                    };
+                    put(Constant<0>{}, Constant<0>{}), put(Constant<0>{}, Constant<1>{}), put(Constant<1>{}, Constant<0>{}), put(Constant<1>{}, Constant<1>{});
+                }
+            }
+            bool some = odd[0];
+            if constexpr (BLOCKS == 2) some |= odd[1];
+            return some;
+        }
+    }
+};
+
+// Values: 64 dimensions along a row of 128 bytes, keys from row to row; 8 keys 1024 bytes apart, the next 64 dimensions a page of rows on.
+__device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr) {
+    return umma_desc(smem_addr) - ((uint64_t)1 << 16) + ((uint64_t)(KV_PAGE * 128 >> 4) << 16);
+}
+
+
 template <uint32_t KIND, uint32_t HD>
 struct ChunkTile : PageTile<KIND, HD> {
     using P = PageTile<KIND, HD>;
@@ -76,25 +298,10 @@ struct ChunkTile : PageTile<KIND, HD> {
     static constexpr uint32_t SMEM = TILES + 4 * RAW + sizeof(ChunkShared);  // and the tiles in front of every sequence
     static_assert(SMEM + (ATTENTION_MAX_BATCH + 1) * 4 <= 227 * 1024, "shared memory");
     // tensor memory columns
-    static constexpr uint32_t Q_HI = 0, Q_LO = HD / 2, S0 = HD, P0 = S0 + 64 * HALVES, O = P0 + 64;
+    static constexpr uint32_t Q_HI = 0, Q_LO = HD / 2, S0 = HD, P0 = S0 + 2 * KV_PAGE, O = P0 + 2 * KV_PAGE;  // scores and probabilities of two pages
     static_assert(O + HD <= 512, "tensor memory");
 };
 
-// Scores of a row: 16 columns at a, with HALVES = 2 also 16 at b, one wait for both.
-__device__ __forceinline__ void tmem_ld16_pair(uint32_t a, uint32_t b, uint32_t (&x)[16], uint32_t (&y)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%32];\n\t"
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32"
-        "{%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%33];\n\t"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=&r"(x[0]), "=&r"(x[1]), "=&r"(x[2]), "=&r"(x[3]), "=&r"(x[4]), "=&r"(x[5]), "=&r"(x[6]), "=&r"(x[7]), "=&r"(x[8]), "=&r"(x[9]),
-          "=&r"(x[10]), "=&r"(x[11]), "=&r"(x[12]), "=&r"(x[13]), "=&r"(x[14]), "=&r"(x[15]), "=&r"(y[0]), "=&r"(y[1]), "=&r"(y[2]), "=&r"(y[3]),
-          "=&r"(y[4]), "=&r"(y[5]), "=&r"(y[6]), "=&r"(y[7]), "=&r"(y[8]), "=&r"(y[9]), "=&r"(y[10]), "=&r"(y[11]), "=&r"(y[12]), "=&r"(y[13]),
-          "=&r"(y[14]), "=&r"(y[15])
-        : "r"(a), "r"(b)
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -127,7 +334,7 @@ __device__ __forceinline__ SequenceRows tile_rows(const PagedArgs& a, uint32_t b
 template <uint32_t KIND, uint32_t HD>
 __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(PagedArgs a, int* error_flag) {
     using T = ChunkTile<KIND, HD>;
-    constexpr uint32_t HEAD = kv_head_bytes(KIND, HD), DN = HD / C_PARTS;  // dimensions of a softmax thread
+    constexpr uint32_t HEAD = kv_head_bytes(KIND, HD);
     constexpr uint32_t PART = CHUNK_TILE_ROWS * (HD + 2);                  // floats of a part of a tile
     extern __shared__ __align__(1024) uint8_t smem[];  // K and V stages | raw keys, raw values | ChunkShared | s_tiles
     const uint32_t k_base = smem_u32(smem), v_base = k_base + 2 * T::K_STAGE;
@@ -148,9 +355,10 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             mbar_init(&sh.rv_full[i], 1);
             mbar_init(&sh.rk_empty[i], C_CONV);
             mbar_init(&sh.rv_empty[i], C_CONV);
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.s_free[i], C_SOFT);
         }
-        mbar_init(&sh.s_full, 1);
-        mbar_init(&sh.s_free, C_SOFT);
+        mbar_init(&sh.q_full, C_SOFT);
         mbar_init(&sh.p_full, C_SOFT);
         mbar_init(&sh.o_full, 1);
         mbar_init(&sh.drained, 1);
@@ -191,81 +399,117 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             for (uint32_t k = 0; k < sq.n; ++k)
                 for (uint32_t i = tid; i < a.n_q * HD; i += C_SOFT * 32) a.out[(sq.row + k) * a.out_stride + i] = sq.len < 0 ? NAN : 0.0f;
         }
-        // ── softmax: thread = (query row, part) ──
-        const uint32_t quarter = warp & 3, part = warp >> 2, row = quarter * 32 + lane;
-        const uint32_t lanes = tmem + ((quarter * 32) << 16);
-        uint32_t phase = 0, g = 0;  // of the exchange between a row's threads; pages so far
-        auto exchange = [&](float x) -> const float* {  // [part * CQ]: x of the row's threads
-            float* at = &sh.row[phase][0][row];
-            phase ^= 1;
-            at[part * CQ] = x;
-            asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
-            return at;
-        };
-        auto share_max = [&](float x) {
-            const float* v = exchange(x);
-            return fmaxf(fmaxf(v[0], v[CQ]), fmaxf(v[2 * CQ], v[3 * CQ]));
-        };
+        // ── softmax: a thread a query row ──
+        const uint32_t row = tid, lanes = tmem + ((warp * 32) << 16);
+        uint32_t g = 0;   // pages so far
         float rf = 0.0f;  // inverse scale of the query row, times log2(e) and the softmax scale
         // a piece's queries into tensor memory; the scores before have been worked out
         auto query = [&](const ChunkPiece& p) {
             const uint32_t heads = min(a.group, CQ), t = row / heads, h = row % heads;
             const bool live = t < p.tokens && (p.head0 + h) / a.group == p.kvh;
             const float4* src = reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + (live ? t : 0)) * a.q_stride +
-                                                                (uint64_t)(p.head0 + (live ? h : 0)) * HD + part * DN);
+                                                                (uint64_t)(p.head0 + (live ? h : 0)) * HD);
             auto load = [&](uint32_t i) { return live ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
             float amax = 0.0f;
-#pragma unroll
-            for (uint32_t i = 0; i < DN / 4; ++i) {
+#pragma unroll 8
+            for (uint32_t i = 0; i < HD / 4; ++i) {
                 const float4 v = load(i);
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
-            amax = share_max(amax);
             // a power of two that puts the row's largest value just below 2^15, with the sign of the scale: the row's maximum is
             // looked for before the scores are multiplied by rf, which must not turn their order round
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
             const float sc = copysignf(__uint_as_float(bits << 23), a.scale);
             rf = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * (fabsf(a.scale) * 1.44269504f);
-#pragma unroll
-            for (uint32_t c = 0; c < DN / 16; ++c) {
+#pragma unroll 2
+            for (uint32_t c = 0; c < HD / 16; ++c) {
                 uint32_t hi[8], lo[8];
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i) {
                     const float4 v = load(4 * c + i);
                     split2(v.x * sc, v.y * sc, &hi[2 * i], &lo[2 * i]), split2(v.z * sc, v.w * sc, &hi[2 * i + 1], &lo[2 * i + 1]);
                 }
-                tmem_st8(lanes + T::Q_HI + part * (DN / 2) + 8 * c, hi);
-                tmem_st8(lanes + T::Q_LO + part * (DN / 2) + 8 * c, lo);
+                tmem_st8(lanes + T::Q_HI + 8 * c, hi);
+                tmem_st8(lanes + T::Q_LO + 8 * c, lo);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.s_free);  // the first scores wait for the query's terms
+            if (lane == 0) mbar_arrive(&sh.q_full);  // the first scores wait for the query's terms
         };
-        f32x2 o[DN / 2];
+        f32x2 o[HD / 2];
         uint32_t odd_first = 0xFFFFFFFFu, odd_end = 0;
         bool lost = false;
         // o = o * alpha + the page's output; u: its place in the piece's list
         auto add_page = [&](uint32_t j, float alpha, uint32_t u) {
             if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
 #pragma unroll
-                for (uint32_t i = 0; i < DN / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
+                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
             }
-            if (!wait_all(&sh.o_full, j & 1)) return;
+            wait_all(&sh.o_full, j & 1);
             tc_fence_after();
             if (*reinterpret_cast<const uint64_t*>(sh.odd[j & 3]) != 0) odd_first = min(odd_first, u), odd_end = u + 1;
             lost |= sh.lost[j & 7] != 0;
 #pragma unroll
-            for (uint32_t c = 0; c < DN / 16; ++c) {
-                uint32_t r[16];
-                tmem_ld16(lanes + T::O + part * DN + 16 * c, r);
-                const float f = KIND == KV_F16 ? 1.0f : sh.vs[j & 3][(part * DN + 16 * c) / 32];
+            for (uint32_t c = 0; c < HD / 32; ++c) {
+                uint32_t r[32];
+                tmem_ld32(lanes + T::O + 32 * c, r);
+                const float f = KIND == KV_F16 ? 1.0f : sh.vs[j & 3][c];
 #pragma unroll
-                for (uint32_t i = 0; i < 8; ++i) {
-                    f32x2& x = o[8 * c + i];
+                for (uint32_t i = 0; i < 16; ++i) {
+                    f32x2& x = o[16 * c + i];
                     x = KIND == KV_F16 ? add2(x, pair(r[2 * i], r[2 * i + 1])) : fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
                 }
             }
+        };
+        float mx = -INFINITY;
+        f32x2 sums = 0;  // sum and outputs times 2^UP, as the probabilities are
+        // The probabilities of page g into tensor memory; seen (EDGE): the positions that the row sees, a bit each.  Returns what the
+        // sums before are worth under the new maximum.
+        auto page = [&](auto edge, uint32_t seen0, uint32_t seen1) {
+            constexpr bool EDGE = decltype(edge)::value;
+            const uint32_t from = lanes + T::S0 + (g & 1) * KV_PAGE, to = lanes + T::P0 + (g & 1) * KV_PAGE;
+            float cm = -INFINITY;
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c) {
+                uint32_t r[32];
+                tmem_ld32(from + 32 * c, r);
+                const uint32_t seen = c ? seen1 : seen0;
+#pragma unroll
+                for (uint32_t i = 0; i < 32; i += 2) {
+                    const float x = EDGE && !(seen >> i & 1) ? -INFINITY : __uint_as_float(r[i]);
+                    const float y = EDGE && !(seen >> (i + 1) & 1) ? -INFINITY : __uint_as_float(r[i + 1]);
+                    cm = max3(cm, x, y);
+                }
+            }
+            const float f = KIND == KV_F16 ? rf : rf * sh.ks[g & 3], top = cm * f;
+            float alpha = 1.0f;
+            if (top > mx + LAZY) alpha = ex2(mx - top), mx = top;  // 0 on the first page with something to see (mx = -inf)
+            const float base = (float)UP - (mx > -INFINITY ? mx : 0.0f);
+            const f32x2 ff = pair(f, f), shift = pair(base, base);
+            f32x2 ps = 0;
+#pragma unroll
+            for (uint32_t c = 0; c < 2; ++c) {
+                uint32_t r[32], w0[16], w1[16];
+                tmem_ld32(from + 32 * c, r);
+                const uint32_t seen = c ? seen1 : seen0;
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) {
+                    const float2 y = both(fma2(pair(r[2 * i], r[2 * i + 1]), ff, shift));
+                    float x0 = ex2(y.x), x1 = ex2(y.y);
+                    if constexpr (EDGE) x0 = seen >> (2 * i) & 1 ? x0 : 0.0f, x1 = seen >> (2 * i + 1) & 1 ? x1 : 0.0f;
+                    const f32x2 both_p = pair(x0, x1);
+                    ps = add2(ps, both_p);
+                    const __half2 h = __floats2half2_rn(x0, x1);
+                    const float2 hf = __half22float2(h);
+                    const float2 rest = both(fma2(pair(hf.x, hf.y), pair(-1.0f, -1.0f), both_p));
+                    w0[i] = half2_bits(h), w1[i] = half2_bits(__floats2half2_rn(rest.x, rest.y));
+                }
+                tmem_st16(to + 16 * c, w0);
+                tmem_st16(to + 32 + 16 * c, w1);
+            }
+            sums = fma2(sums, pair(alpha, alpha), ps);
+            return alpha;
         };
         meet();
         for (uint32_t turn = 0; turn < sh.batches; ++turn) {
@@ -275,115 +519,64 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 const ChunkPiece& p = sh.piece[k];
                 const uint32_t heads = min(a.group, CQ), t = row / heads, n = p.end - p.first;
                 const Sight see(a.span, p.pos0 + t), last_see(a.span, p.pos0 + p.tokens - 1);
-                const float my_rf = rf;
 #pragma unroll
-                for (uint32_t i = 0; i < DN / 2; ++i) o[i] = 0;
-                float mx = -INFINITY, alpha_prev = 0.0f;
-                f32x2 sums = 0;  // sum and outputs times 2^UP, as the probabilities are
-                odd_first = 0xFFFFFFFFu, odd_end = 0, lost = false;
+                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0;
+                float alpha_prev = 0.0f;
+                mx = -INFINITY, sums = 0, odd_first = 0xFFFFFFFFu, odd_end = 0, lost = false;
                 for (uint32_t j = 0; j < n; ++j, ++g) {
                     const uint32_t u = p.first + j, base = (u < p.sinks ? u : u + p.skip) * KV_PAGE;
-                    f32x2 sc[C_KEYS / 2];
-                    wait_all(&sh.s_full, g & 1);
+                    wait_all(&sh.s_full[g & 1], (g >> 1) & 1);
                     tc_fence_after();
-                    {
-                        uint32_t r[16];
-                        if constexpr (T::HALVES == 2) {
-                            uint32_t r2[16];
-                            tmem_ld16_pair(lanes + T::S0 + part * C_KEYS, lanes + T::S0 + 64 + part * C_KEYS, r, r2);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) sc[i] = add2(pair(r[2 * i], r[2 * i + 1]), pair(r2[2 * i], r2[2 * i + 1]));
-                        } else {
-                            tmem_ld16(lanes + T::S0 + part * C_KEYS, r);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) sc[i] = pair(r[2 * i], r[2 * i + 1]);
-                        }
+                    float alpha;
+                    if (base + KV_PAGE > p.pos0 + 1 || (base < last_see.low && base + KV_PAGE > last_see.sinks)) {
+                        auto seen = [&](uint32_t t0) {  // of 32 positions
+                            auto below = [&](uint32_t x) { return x <= t0 ? 0u : x - t0 >= 32 ? 0xFFFFFFFFu : (1u << (x - t0)) - 1; };
+                            return below(see.end) & (~below(see.low) | below(see.sinks));
+                        };
+                        alpha = page(Constant<1>{}, seen(base), seen(base + 32));
+                    } else {
+                        alpha = page(Constant<0>{}, 0, 0);
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (j + 1 < n && lane == 0) mbar_arrive(&sh.s_free);  // behind the last page: when the next queries are in place
-                    const float f = KIND == KV_F16 ? my_rf : my_rf * sh.ks[g & 3];
-                    // positions of this thread's that the row sees, a bit each
-                    uint32_t seen = 0xFFFFu;
-                    const bool edge = base + KV_PAGE > p.pos0 + 1 || (base < last_see.low && base + KV_PAGE > last_see.sinks);
-                    if (edge) {
-                        const uint32_t t0 = base + part * C_KEYS;
-                        auto below = [&](uint32_t x) { return x <= t0 ? 0u : x - t0 >= C_KEYS ? 0xFFFFu : (1u << (x - t0)) - 1; };
-                        seen = below(see.end) & (~below(see.low) | below(see.sinks));
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float2 v = both(sc[i]);
-                            sc[i] = pair(seen >> (2 * i) & 1 ? v.x : -INFINITY, seen >> (2 * i + 1) & 1 ? v.y : -INFINITY);
-                        }
-                    }
-                    float cm = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float2 v = both(sc[i]);
-                        cm = max3(cm, v.x, v.y);
-                    }
-                    const float top = share_max(cm) * f;
-                    float alpha = 1.0f;
-                    if (top > mx + LAZY) alpha = ex2(mx - top), mx = top;  // 0 on the first page with something to see (mx = -inf)
-                    const float from = (float)UP - (mx > -INFINITY ? mx : 0.0f);
-                    const f32x2 ff = pair(f, f), shift = pair(from, from);
-                    f32x2 ps = 0;
-                    uint32_t w0[8], w1[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float2 y = both(fma2(sc[i], ff, shift));
-                        float x0 = ex2(y.x), x1 = ex2(y.y);
-                        if (edge) x0 = seen >> (2 * i) & 1 ? x0 : 0.0f, x1 = seen >> (2 * i + 1) & 1 ? x1 : 0.0f;
-                        const f32x2 both_p = pair(x0, x1);
-                        ps = add2(ps, both_p);
-                        const __half2 h = __floats2half2_rn(x0, x1);
-                        const float2 hf = __half22float2(h);
-                        const float2 rest = both(fma2(pair(hf.x, hf.y), pair(-1.0f, -1.0f), both_p));
-                        w0[i] = half2_bits(h), w1[i] = half2_bits(__floats2half2_rn(rest.x, rest.y));
-                    }
-                    sums = fma2(sums, pair(alpha, alpha), ps);
-                    if (j > 0) add_page(g - 1, alpha_prev, u - 1);  // its products have read the probabilities before these
+                    if (lane == 0) mbar_arrive(&sh.s_free[g & 1]);
+                    if (j > 0) add_page(g - 1, alpha_prev, u - 1);
                     alpha_prev = alpha;
-                    tmem_st8(lanes + T::P0 + part * 8, w0);
-                    tmem_st8(lanes + T::P0 + 32 + part * 8, w1);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
-                    if (ok && lane == 0) mbar_arrive(&sh.p_full);
+                    if (ok && lane == 0) mbar_arrive(&sh.p_full);  // and the output before has been read
                 }
                 if (k + 1 < pieces) query(sh.piece[k + 1]);
                 add_page(g - 1, alpha_prev, p.end - 1);
                 const float2 two = both(sums);
-                const float* all_sums = exchange(two.x + two.y);
-                float sum = (all_sums[0] + all_sums[CQ]) + (all_sums[2 * CQ] + all_sums[3 * CQ]);
+                float sum = two.x + two.y;
                 if (!ok || lost) sum = NAN;
-                if (lost && row == 0 && part == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+                if (lost && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
                 const bool live = t < p.tokens && (p.head0 + row % heads) / a.group == p.kvh;
                 if (odd_end != 0 && live) {
                     // values that are not finite stood as zeros in the products: they go where a row sees them, and nowhere else
                     for (uint32_t u = odd_first; u < odd_end; ++u) {
-                        const uint32_t page = u < p.sinks ? u : u + p.skip;
-                        const int32_t id = a.c.table[(uint64_t)p.seq * a.c.table_stride + page];
+                        const uint32_t number = u < p.sinks ? u : u + p.skip;
+                        const int32_t id = a.c.table[(uint64_t)p.seq * a.c.table_stride + number];
                         if (id < 0 || (uint32_t)id >= a.c.n_pages) continue;
                         const uint8_t* values = a.c.pages + ((uint64_t)id * a.c.n_kv + p.kvh) * HEAD + HEAD / 2;
                         for (uint32_t i = 0; i < KV_PAGE; ++i) {
-                            const uint32_t at = page * KV_PAGE + i;
+                            const uint32_t at = number * KV_PAGE + i;
                             if (at >= see.end || (at < see.low && at >= see.sinks)) continue;
 #pragma unroll
-                            for (uint32_t d = 0; d < DN; d += 4) {
-                                const float4 v = kv_load<KIND, HD, true>(values, i, part * DN + d);
+                            for (uint32_t d = 0; d < HD; d += 4) {
+                                const float4 v = kv_load<KIND, HD, true>(values, i, d);
                                 auto odd = [](float x) { return fabsf(x) < INFINITY ? 0.0f : x; };
                                 o[d / 2] = add2(o[d / 2], pair(odd(v.x), odd(v.y))), o[d / 2 + 1] = add2(o[d / 2 + 1], pair(odd(v.z), odd(v.w)));
                             }
                         }
                     }
                 }
-                float* to = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row % heads) * HD + part * DN;
+                float* to = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row % heads) * HD;
                 auto store = [&](float den) {
                     if (!live) return;
                     const float inv = 1.0f / den;
 #pragma unroll
-                    for (uint32_t i = 0; i < DN / 4; ++i) {
+                    for (uint32_t i = 0; i < HD / 4; ++i) {
                         const float2 x = both(o[2 * i]), y = both(o[2 * i + 1]);
                         *reinterpret_cast<float4*>(to + 4 * i) = make_float4(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
                     }
@@ -394,11 +587,11 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                     // [HD / 4][CQ] outputs of four dimensions, then maxima, then sums
                     float* mine = a.part + ((uint64_t)blockIdx.x * 2 + (p.first == 0)) * PART;
 #pragma unroll
-                    for (uint32_t i = 0; i < DN / 4; ++i) {
+                    for (uint32_t i = 0; i < HD / 4; ++i) {
                         const float2 x = both(o[2 * i]), y = both(o[2 * i + 1]);
-                        __stcg(reinterpret_cast<float4*>(mine) + (part * (DN / 4) + i) * CQ + row, make_float4(x.x, x.y, y.x, y.y));
+                        __stcg(reinterpret_cast<float4*>(mine) + i * CQ + row, make_float4(x.x, x.y, y.x, y.y));
                     }
-                    if (part == 0) __stcg(mine + HD * CQ + row, mx), __stcg(mine + (HD + 1) * CQ + row, sum);
+                    __stcg(mine + HD * CQ + row, mx), __stcg(mine + (HD + 1) * CQ + row, sum);
                     __threadfence();
                     asm volatile("bar.sync 5, %0;" ::"n"(C_SOFT * 32) : "memory");
                     if (tid == 0) {
@@ -414,14 +607,14 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                         float best = -INFINITY, den = 0.0f;
                         for (uint32_t i = 0; i < p.parts; ++i) best = fmaxf(best, __ldcg(part_of(i) + HD * CQ + row));
 #pragma unroll
-                        for (uint32_t i = 0; i < DN / 2; ++i) o[i] = 0;
+                        for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0;
                         for (uint32_t i = 0; i < p.parts; ++i) {
                             const float* from = part_of(i);
                             const float w = piece_weight(__ldcg(from + HD * CQ + row), best);
                             den = fmaf(w, __ldcg(from + (HD + 1) * CQ + row), den);
 #pragma unroll
-                            for (uint32_t d = 0; d < DN / 4; ++d) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4*>(from) + (part * (DN / 4) + d) * CQ + row);
+                            for (uint32_t d = 0; d < HD / 4; ++d) {
+                                const float4 v = __ldcg(reinterpret_cast<const float4*>(from) + d * CQ + row);
                                 o[2 * d] = fma2(pair(v.x, v.y), pair(w, w), o[2 * d]), o[2 * d + 1] = fma2(pair(v.z, v.w), pair(w, w), o[2 * d + 1]);
                             }
                         }
@@ -507,7 +700,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         });
         asm volatile("bar.sync 7, %0;" ::"n"(C_CONV * 32) : "memory");
         const uint32_t first_seg = sh.first_seg, end_seg = sh.end_seg, batches = end_seg > first_seg ? (end_seg - first_seg + C_PIECES - 1) / C_PIECES : 0;
-        const PageConverter<KIND, HD, C_CONV, true> convert(cw, lane);
+        const ChunkConverter<KIND, HD, C_CONV> convert(cw, lane);
         uint32_t g = 0;
         auto list = [&](uint32_t turn) {
             const uint32_t from = first_seg + turn * C_PIECES, to = min(end_seg, from + C_PIECES);
@@ -566,61 +759,70 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
     } else {
         // ── issuer (one warp issues, one copies, two have nothing to do) ──
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C_REGS_ISSUE));
-        uint32_t g = 0, k_sent = 0, v_sent = 0;
+        uint32_t g = 0, q_phase = 0, k_sent = 0, v_sent = 0;
         meet();
         const uint32_t batches = sh.batches;
         for (uint32_t turn = 0; turn < batches; ++turn) {
             const uint32_t pieces = sh.pieces;
             if (warp == C_SOFT + C_CONV) {
-                constexpr uint32_t idesc_s = umma_idesc_f16(KV_PAGE), idesc_o = umma_idesc_f16(HD);
-                const uint64_t dk = umma_desc(k_base), dv = umma_desc(v_base);
-                auto scores = [&](uint32_t j) {  // one accumulator per 64 dimensions, small products first
-                    // the scores before have been read (the first of a piece: the queries are in place)
-                    wait_all(&sh.s_free, j & 1);
+                constexpr uint32_t idesc_s = umma_idesc_f16(KV_PAGE), idesc_o = umma_idesc_f16(HD) | 1u << 16;  // values MN-major
+                const uint64_t dk = umma_desc(k_base), dv = umma_desc_values(v_base);
+                // scores of page j in one accumulator, small products first; `begins`: of a piece's first, the queries are in place
+                auto scores = [&](uint32_t j, bool begins) {
+                    if (begins) wait_all(&sh.q_full, q_phase), q_phase ^= 1;
+                    wait_all(&sh.s_free[j & 1], ((j >> 1) & 1) ^ 1);
                     if (!wait_all(&sh.k_full[j & 1], (j >> 1) & 1)) return;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint64_t d0 = dk + (uint64_t)(j & 1) * (T::K_STAGE >> 4);
+                        const uint32_t d = tmem + T::S0 + (j & 1) * KV_PAGE;
 #pragma unroll
-                        for (uint32_t h = 0; h < T::HALVES; ++h) {
-                            const uint64_t hi = d0 + h * (T::K_PLANE >> 4), lo = hi + T::HALVES * (T::K_PLANE >> 4);
-                            const uint32_t d = tmem + T::S0 + 64 * h, a_hi = tmem + T::Q_HI + 32 * h, a_lo = tmem + T::Q_LO + 32 * h;
-#pragma unroll
-                            for (uint32_t kk = 0; kk < 4; ++kk) {
-                                umma_f16_ts(d, a_lo + 8 * kk, hi + 2 * kk, idesc_s, kk != 0);
-                                if constexpr (T::TERMS == 2) umma_f16_ts(d, a_hi + 8 * kk, lo + 2 * kk, idesc_s, 1);
-                            }
-#pragma unroll
-                            for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_ts(d, a_hi + 8 * kk, hi + 2 * kk, idesc_s, 1);
+                        for (uint32_t kk = 0; kk < HD / 16; ++kk) {
+                            const uint64_t hi = d0 + kk / 4 * (T::K_PLANE >> 4) + kk % 4 * 2, lo = hi + T::HALVES * (T::K_PLANE >> 4);
+                            umma_f16_ts(d, tmem + T::Q_LO + 8 * kk, hi, idesc_s, kk != 0);
+                            if constexpr (T::TERMS == 2) umma_f16_ts(d, tmem + T::Q_HI + 8 * kk, lo, idesc_s, 1);
                         }
+#pragma unroll
+                        for (uint32_t kk = 0; kk < HD / 16; ++kk)
+                            umma_f16_ts(d, tmem + T::Q_HI + 8 * kk, d0 + kk / 4 * (T::K_PLANE >> 4) + kk % 4 * 2, idesc_s, 1);
                         umma_commit(&sh.k_empty[j & 1]);
-                        umma_commit(&sh.s_full);
+                        umma_commit(&sh.s_full[j & 1]);
                     }
                     __syncwarp();
                 };
                 uint32_t all = 0;
                 for (uint32_t k = 0; k < pieces; ++k) all += sh.piece[k].end - sh.piece[k].first;
-                if (all) scores(g);
+                uint32_t k = 0, left = 0;  // the piece whose scores come next, pages left of it
+                auto next = [&] {
+                    const bool begins = left == 0;
+                    if (begins) left = sh.piece[k].end - sh.piece[k].first, ++k;
+                    --left;
+                    return begins;
+                };
+                if (all) scores(g, next());
                 for (uint32_t j = 0; j < all; ++j, ++g) {
-                    if (j + 1 < all) scores(g + 1);
+                    const bool more = j + 1 < all, begins = more && next();
+                    if (more && !begins) scores(g + 1, false);
                     // the probabilities are in place, the output before has been read
                     wait_all(&sh.v_full[g & 1], (g >> 1) & 1);
-                    if (!wait_all(&sh.p_full, g & 1)) continue;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t hi = dv + (uint64_t)(g & 1) * (T::V_STAGE >> 4), lo = hi + (T::V_PLANE >> 4);
-                        const uint32_t d = tmem + T::O, p_hi = tmem + T::P0, p_lo = p_hi + 32;
+                    if (wait_all(&sh.p_full, g & 1)) {
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint64_t hi = dv + (uint64_t)(g & 1) * (T::V_STAGE >> 4), lo = hi + (T::V_PLANE >> 4);
+                            const uint32_t d = tmem + T::O, p_hi = tmem + T::P0 + (g & 1) * KV_PAGE, p_lo = p_hi + 32;
 #pragma unroll
-                        for (uint32_t kk = 0; kk < 4; ++kk) {
-                            umma_f16_ts(d, p_lo + 8 * kk, hi + 2 * kk, idesc_o, kk != 0);
-                            if constexpr (T::TERMS == 2) umma_f16_ts(d, p_hi + 8 * kk, lo + 2 * kk, idesc_o, 1);
+                            for (uint32_t kk = 0; kk < 4; ++kk) {
+                                umma_f16_ts(d, p_lo + 8 * kk, hi + 128 * kk, idesc_o, kk != 0);
+                                if constexpr (T::TERMS == 2) umma_f16_ts(d, p_hi + 8 * kk, lo + 128 * kk, idesc_o, 1);
+                            }
+#pragma unroll
+                            for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_ts(d, p_hi + 8 * kk, hi + 128 * kk, idesc_o, 1);
+                            umma_commit(&sh.v_empty[g & 1]);
+                            umma_commit(&sh.o_full);
                         }
-#pragma unroll
-                        for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_ts(d, p_hi + 8 * kk, hi + 2 * kk, idesc_o, 1);
-                        umma_commit(&sh.v_empty[g & 1]);
-                        umma_commit(&sh.o_full);
+                        __syncwarp();
                     }
-                    __syncwarp();
+                    if (begins) scores(g + 1, true);  // behind the products of the piece before: its rows bring the next queries
                 }
             } else if (warp == C_SOFT + C_CONV + 1) {
                 // ── loader: a page's keys, or values, of a head are one run of memory; page ids 32 at a time, a lane each ──

@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
     } else if (warp < L_SOFT + L_CONV) {
         // ── converters ──
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L_REGS_CONV));
-        const PageConverter<KIND, HD, L_CONV, false> convert(warp - L_SOFT, lane);
+        const PageConverter<KIND, HD, L_CONV> convert(warp - L_SOFT, lane);
         auto publish = [&](uint64_t* bar) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -319,11 +319,11 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
         for (uint32_t j = 0; j < n_tiles; ++j) {
             const uint32_t st = j & 1, turn = (j >> 1) & 1;
             if (!wait_all(&sh.k_empty[st], turn ^ 1) || !wait_all(&sh.rk_full[st], turn)) break;
-            convert.keys(k_base + st * T::K_STAGE, raw_k + st * T::RAW, LK, &sh.ks[j & 3]);
+            convert.keys(k_base + st * T::K_STAGE, raw_k + st * T::RAW, &sh.ks[j & 3]);
             publish(&sh.k_full[st]);
             if (lane == 0) mbar_arrive(&sh.rk_empty[st]);
             if (!wait_all(&sh.v_empty[st], turn ^ 1) || !wait_all(&sh.rv_full[st], turn)) break;
-            convert.values(v_base + st * T::V_STAGE, raw_v + st * T::RAW, LK, sh.vs[j & 3]);
+            convert.values(v_base + st * T::V_STAGE, raw_v + st * T::RAW, sh.vs[j & 3]);
             publish(&sh.v_full[st]);
             if (lane == 0) mbar_arrive(&sh.rv_empty[st]);
         }

@@ -85,9 +85,8 @@ struct PageTile {
     static_assert(RAW % 16 == 0, "bulk copies");
 };
 
-// The WARPS warps that turn pages into operands.  MASKED: only the first `valid` positions of a page are anyone's; what stands behind
-// them does not count for the page's scales, and values there, or not finite, become zeros.
-template <uint32_t KIND, uint32_t HD, uint32_t WARPS, bool MASKED>
+// The WARPS warps that turn whole pages into operands, both K-major.
+template <uint32_t KIND, uint32_t HD, uint32_t WARPS>
 struct PageConverter {
     using T = PageTile<KIND, HD>;
     static constexpr uint32_t NB = T::NB, CODES = kv_code_bytes(KIND, HD), K_LO = T::HALVES * T::K_PLANE, V_LO = T::V_PLANE;
@@ -101,14 +100,8 @@ struct PageConverter {
     }
     // 16 bytes (8 keys: 8 chunk ..) of a dimension's row of values
     __device__ __forceinline__ static uint32_t value_at(uint32_t stage, uint32_t d, uint32_t chunk) { return stage + d * 128 + ((chunk ^ (d & 7)) << 4); }
-    // halfwords of positions at and at + 8 that are there; halfwords of finite numbers
-    __device__ __forceinline__ static uint32_t there(uint32_t at, uint32_t valid) {
-        return (at < valid ? 0xFFFFu : 0u) | (at + 8 < valid ? 0xFFFF0000u : 0u);
-    }
-    __device__ __forceinline__ static uint32_t finite(uint32_t w) { return __vcmpltu2(w & 0x7FFF7FFFu, 0x7C007C00u); }
-
     // a page's keys; *inverse: what their products are multiplied by
-    __device__ __forceinline__ void keys(uint32_t st, const uint8_t* raw, uint32_t valid, float* inverse) const {
+    __device__ __forceinline__ void keys(uint32_t st, const uint8_t* raw, float* inverse) const {
         if constexpr (KIND == KV_F16) {
 #pragma unroll
             for (uint32_t i = cw; i < 4 * NB; i += WARPS) {
@@ -122,14 +115,7 @@ struct PageConverter {
             uint32_t top = 0x04000400u;  // the page's largest scale
 #pragma unroll
             for (uint32_t i = 0; i < NB / 2; ++i) {  // 8 bytes a position and block pair
-                uint2 v = *reinterpret_cast<const uint2*>(raw + CODES + (i * 32 + lane) * 8);
-                if constexpr (MASKED) {
-                    v.x &= finite(v.x), v.y &= finite(v.y);
-                    if (valid < KV_PAGE) {
-                        const uint32_t unit = (i * 32 + lane) / NB, at = unit / 8 * 32 + unit % 8;
-                        v.x &= there(at, valid), v.y &= there(at + 16, valid);
-                    }
-                }
+                const uint2 v = *reinterpret_cast<const uint2*>(raw + CODES + (i * 32 + lane) * 8);
                 top = __vmaxu2(top, __vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu));
             }
             const int e = (int)(__reduce_max_sync(0xFFFFFFFFu, max(top >> 16, top & 0xFFFFu)) >> 10);
@@ -167,25 +153,14 @@ struct PageConverter {
         }
     }
     // values: keys run along a row of the tile, so four lanes' words are transposed: lane c then has eight keys of two
-    // dimensions (halves: of one).  inverse: what the products of each block are multiplied by.  True (MASKED): some value that
-    // is there is not finite.
-    __device__ __forceinline__ bool values(uint32_t st, const uint8_t* raw, uint32_t valid, float* inverse) const {
-        bool lost = false;
+    // dimensions (halves: of one).  inverse: what the products of each block are multiplied by.
+    __device__ __forceinline__ void values(uint32_t st, const uint8_t* raw, float* inverse) const {
         if constexpr (KIND == KV_F16) {
 #pragma unroll
             for (uint32_t i = cw; i < 8 * NB; i += WARPS) {
                 const uint32_t g = i / (2 * NB), b = i / 2 % NB, m = i % 2;
                 const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
                 uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                if constexpr (MASKED) {
-#pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {  // positions 16 g + 8 (k / 2) + 2 c and the next
-                        const uint32_t at = 16 * g + 8 * (k / 2) + 2 * c;
-                        if (valid < KV_PAGE) w[k] &= (at < valid ? 0xFFFFu : 0u) | (at + 1 < valid ? 0xFFFF0000u : 0u);
-                        const uint32_t fine = finite(w[k]);
-                        lost |= fine != 0xFFFFFFFFu, w[k] &= fine;
-                    }
-                }
                 transpose4(w, c);
                 sts_v4(value_at(st, 32 * b + 4 * r + 2 * m + c % 2, 2 * g + c / 2), w);
             }
@@ -201,13 +176,7 @@ struct PageConverter {
                 __half2 mine[BLOCKS];  // of the group's positions: lane % 8 and that + 8, in the lanes of its 32 positions
 #pragma unroll
                 for (uint32_t o = 0; o < BLOCKS; ++o) {
-                    uint2 s = *reinterpret_cast<const uint2*>(raw + CODES + ((lane & 15) * NB + b0 + o) * 8);
-                    if constexpr (MASKED) {
-                        const uint32_t at = (lane & 15) / 8 * 32 + lane % 8;
-                        if (valid < KV_PAGE) s.x &= there(at, valid), s.y &= there(at + 16, valid);
-                        const uint32_t x = finite(s.x), y = finite(s.y);
-                        lost |= (x & y) != 0xFFFFFFFFu, s.x &= x, s.y &= y;
-                    }
+                    const uint2 s = *reinterpret_cast<const uint2*>(raw + CODES + ((lane & 15) * NB + b0 + o) * 8);
                     const uint32_t t = __vmaxu2(__vmaxu2(s.x & 0x7FFF7FFFu, s.y & 0x7FFF7FFFu), 0x04000400u);
                     const int e = (int)(__reduce_max_sync(0xFFFFFFFFu, max(t >> 16, t & 0xFFFFu)) >> 10);
                     mine[o] = scaled(g % 2 ? s.y : s.x, power(TOP - e));
@@ -257,7 +226,6 @@ struct PageConverter {
                 }
             }
         }
-        return MASKED && lost;
     }
 };
 
