@@ -11,8 +11,8 @@
 // The tiles' work stands in one row of units, tile by tile, kv head by kv head, SEG_UNITS for beginning and ending one, then its
 // pages.  It is cut into equal pieces, one a CTA; pieces of a tile that several CTAs have are joined by the last of them to arrive, in order.
 //
-// Warps: 0 .. 3 softmax, a thread a query row; 4 .. 11 first cut the work, then turn the pages' codes into swizzled tiles, two stages; 12
-// issues the products; 13 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
+// Warps: 0 .. 3 softmax, a thread a query row; 4 .. 7 add up the output, the same; 8 .. 15 first cut the work, then turn the pages' codes
+// into swizzled tiles, two stages; 16 issues the products; 17 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
 // (A of the output) of two pages, output of one.
 //
 // Every wait on an mbarrier is bounded.  A warp whose wait ran out waits for none any more, hands nothing on, and goes through the
@@ -27,14 +27,15 @@ namespace jq {
 namespace {
 
 constexpr uint32_t CQ = CHUNK_TILE_ROWS;     // query rows of a tile
-constexpr uint32_t C_SOFT = 4, C_CONV = 8;   // warps
+constexpr uint32_t C_SOFT = 4, C_SUM = 4, C_CONV = 8;  // warps
+constexpr uint32_t C_FIRST_CONV = C_SOFT + C_SUM, C_ISSUE = C_FIRST_CONV + C_CONV, C_LOAD = C_ISSUE + 1;
 constexpr int UP = 6;                        // probabilities stand times 2^UP ..
 constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
-constexpr uint32_t C_THREADS = (C_SOFT + C_CONV + 4) * 32;  // whole warpgroups: they trade registers
-// Registers a thread: the launch has 512 x 128 = 65536, of which the issuer's warpgroup keeps 128 x 64, the converters 256 x 104 and the
-// softmax threads (128 running outputs, 32 scores, 32 terms) 128 x 240.
-constexpr int C_REGS_ISSUE = 64, C_REGS_CONV = 104, C_REGS_SOFT = 240;
-static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT <= C_THREADS * 128, "registers");
+constexpr uint32_t C_THREADS = (C_ISSUE + 4) * 32;  // whole warpgroups: they trade registers
+// Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 72, the
+// softmax threads (32 scores, 32 terms) 128 x 104, and those that add up the output (128 running sums, 32 new ones) 128 x 200: all of it.
+constexpr int C_REGS_ISSUE = 32, C_REGS_CONV = 72, C_REGS_SOFT = 104, C_REGS_SUM = 200;
+static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT + C_SUM * 32 * C_REGS_SUM <= C_THREADS * 96, "registers");
 
 constexpr uint32_t SEG_UNITS = 2;   // a tile's beginning and end in pages
 constexpr uint32_t C_PIECES = 96;   // pieces of a CTA at a time
@@ -53,8 +54,10 @@ struct ChunkShared {
     float ks[4];              // inverse scale of the keys, by page % 4
     float vs[4][4];           // inverse scales of the values' blocks, by page % 4
     uint8_t odd[4][C_CONV];   // values that are not finite, by page % 4 and converter
-    uint8_t lost[8];          // a page id outside the cache, by page % 8
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], q_full, p_full, o_full;
+    uint8_t lost[16];         // a page id outside the cache, by page % 16
+    float alpha[4][CQ];       // what the sums before are worth under the new maximum, by page % 4
+    float stat[4][2][CQ];     // maxima and sums of a finished piece, by its last page % 4
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], q_full, p_full[2], p_free[2], o_full, o_free;
     uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];  // the raw pages
     uint64_t drained;         // the products of a CTA that gives up
     uint32_t tmem_slot;
@@ -133,7 +136,7 @@ struct ChunkConverter {
     // a page's keys; *inverse: what their products are multiplied by
     __device__ __forceinline__ void keys(uint32_t stage, const uint8_t* raw, uint32_t valid, float* inverse) const {
         if constexpr (KIND == KV_F16) {
-#pragma unroll
+#pragma unroll 1
             for (uint32_t i = cw; i < ITEMS; i += WARPS) {
                 const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 1024 + lane * 16), y = *reinterpret_cast<const uint4*>(raw + i * 1024 + 512 + lane * 16);
                 const uint32_t to = stage + key_to + i / COLS * 2048;
@@ -152,7 +155,7 @@ struct ChunkConverter {
             const int e = (int)(largest(v, at, valid, &odd) >> 10);
             const Up up(e);
             if (cw == 0 && lane == 0) *inverse = power(e - TOP);
-#pragma unroll
+#pragma unroll 1
             for (uint32_t i = cw; i < ITEMS; i += WARPS) {
                 const uint32_t g = i / COLS, to = stage + key_to + g * 2048;
                 const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
@@ -204,7 +207,7 @@ struct ChunkConverter {
     __device__ __forceinline__ bool values(uint32_t stage, const uint8_t* raw, uint32_t valid, float* inverse) const {
         if constexpr (KIND == KV_F16) {
             bool odd = false;
-#pragma unroll
+#pragma unroll 1
             for (uint32_t i = cw; i < ITEMS; i += WARPS) {
                 const uint32_t g = i / COLS;
                 uint32_t w[2][4];
@@ -249,7 +252,7 @@ struct ChunkConverter {
                 if (cw < COLS && lane == 0) inverse[b0 + o] = power(e[o] - TOP);
                 careful |= odd[o];
             }
-#pragma unroll
+#pragma unroll 1
             for (uint32_t i = cw; i < ITEMS; i += WARPS) {
                 const uint32_t g = i / COLS;
                 const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 512 + lane * 16);
@@ -357,15 +360,17 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             mbar_init(&sh.rv_empty[i], C_CONV);
             mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.s_free[i], C_SOFT);
+            mbar_init(&sh.p_full[i], C_SOFT);  // softmax may be a page ahead of the products
+            mbar_init(&sh.p_free[i], 1);
         }
         mbar_init(&sh.q_full, C_SOFT);
-        mbar_init(&sh.p_full, C_SOFT);
         mbar_init(&sh.o_full, 1);
+        mbar_init(&sh.o_free, C_SUM);
         mbar_init(&sh.drained, 1);
         sh.abort_flag = !aligned;
         mbar_fence_init();
     }
-    if (warp == C_SOFT + C_CONV) {
+    if (warp == C_ISSUE) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem_slot)), "r"(512u)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -403,75 +408,65 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         const uint32_t row = tid, lanes = tmem + ((warp * 32) << 16);
         uint32_t g = 0;   // pages so far
         float rf = 0.0f;  // inverse scale of the query row, times log2(e) and the softmax scale
-        // a piece's queries into tensor memory; the scores before have been worked out
-        auto query = [&](const ChunkPiece& p) {
+        // this thread's row of a piece, and whether there is one
+        auto row_of = [&](const ChunkPiece& p, bool* live) {
             const uint32_t heads = min(a.group, CQ), t = row / heads, h = row % heads;
-            const bool live = t < p.tokens && (p.head0 + h) / a.group == p.kvh;
-            const float4* src = reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + (live ? t : 0)) * a.q_stride +
-                                                                (uint64_t)(p.head0 + (live ? h : 0)) * HD);
-            auto load = [&](uint32_t i) { return live ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+            *live = t < p.tokens && (p.head0 + h) / a.group == p.kvh;
+            return reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + (*live ? t : 0)) * a.q_stride + (uint64_t)(p.head0 + (*live ? h : 0)) * HD);
+        };
+        // The largest magnitude of the row, asked for a piece ahead: the row itself then comes from L2.
+        auto largest = [&](const ChunkPiece& p) {
+            bool live;
+            const float4* src = row_of(p, &live);
             float amax = 0.0f;
-#pragma unroll 8
+#pragma unroll 16
             for (uint32_t i = 0; i < HD / 4; ++i) {
-                const float4 v = load(i);
+                const float4 v = src[i];
                 amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
+            return live ? amax : 0.0f;
+        };
+        // a piece's queries into tensor memory; the scores before have been worked out
+        auto query = [&](const ChunkPiece& p, float amax) {
+            bool live;
+            const float4* src = row_of(p, &live);
             // a power of two that puts the row's largest value just below 2^15, with the sign of the scale: the row's maximum is
             // looked for before the scores are multiplied by rf, which must not turn their order round
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
-            const float sc = copysignf(__uint_as_float(bits << 23), a.scale);
+            const float sc = live ? copysignf(__uint_as_float(bits << 23), a.scale) : 0.0f;
             rf = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * (fabsf(a.scale) * 1.44269504f);
-#pragma unroll 2
-            for (uint32_t c = 0; c < HD / 16; ++c) {
-                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) {
-                    const float4 v = load(4 * c + i);
-                    split2(v.x * sc, v.y * sc, &hi[2 * i], &lo[2 * i]), split2(v.z * sc, v.w * sc, &hi[2 * i + 1], &lo[2 * i + 1]);
+            for (uint32_t c = 0; c < HD / 64; ++c) {
+                float4 v[16];
+#pragma unroll
+                for (uint32_t i = 0; i < 16; ++i) v[i] = src[16 * c + i];
+#pragma unroll
+                for (uint32_t i = 0; i < 16; i += 4) {
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) {
+                        const float4 x = v[i + k];
+                        split2(x.x * sc, x.y * sc, &hi[2 * k], &lo[2 * k]), split2(x.z * sc, x.w * sc, &hi[2 * k + 1], &lo[2 * k + 1]);
+                    }
+                    tmem_st8(lanes + T::Q_HI + 32 * c + 2 * i, hi);
+                    tmem_st8(lanes + T::Q_LO + 32 * c + 2 * i, lo);
                 }
-                tmem_st8(lanes + T::Q_HI + 8 * c, hi);
-                tmem_st8(lanes + T::Q_LO + 8 * c, lo);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_full);  // the first scores wait for the query's terms
         };
-        f32x2 o[HD / 2];
-        uint32_t odd_first = 0xFFFFFFFFu, odd_end = 0;
-        bool lost = false;
-        // o = o * alpha + the page's output; u: its place in the piece's list
-        auto add_page = [&](uint32_t j, float alpha, uint32_t u) {
-            if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
-#pragma unroll
-                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
-            }
-            wait_all(&sh.o_full, j & 1);
-            tc_fence_after();
-            if (*reinterpret_cast<const uint64_t*>(sh.odd[j & 3]) != 0) odd_first = min(odd_first, u), odd_end = u + 1;
-            lost |= sh.lost[j & 7] != 0;
-#pragma unroll
-            for (uint32_t c = 0; c < HD / 32; ++c) {
-                uint32_t r[32];
-                tmem_ld32(lanes + T::O + 32 * c, r);
-                const float f = KIND == KV_F16 ? 1.0f : sh.vs[j & 3][c];
-#pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) {
-                    f32x2& x = o[16 * c + i];
-                    x = KIND == KV_F16 ? add2(x, pair(r[2 * i], r[2 * i + 1])) : fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
-                }
-            }
-        };
         float mx = -INFINITY;
         f32x2 sums = 0;  // sum and outputs times 2^UP, as the probabilities are
-        // The probabilities of page g into tensor memory; seen (EDGE): the positions that the row sees, a bit each.  Returns what the
+        // The probabilities of page g into tensor memory, when the products before the last have read theirs; seen (EDGE): the positions that the row sees, a bit each.  Returns what the
         // sums before are worth under the new maximum.
         auto page = [&](auto edge, uint32_t seen0, uint32_t seen1) {
             constexpr bool EDGE = decltype(edge)::value;
             const uint32_t from = lanes + T::S0 + (g & 1) * KV_PAGE, to = lanes + T::P0 + (g & 1) * KV_PAGE;
-            float cm = -INFINITY;
-#pragma unroll
-            for (uint32_t c = 0; c < 2; ++c) {
+            float cms[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+            for (uint32_t c = 0; c < 2; ++c) {  // one copy of the code: what all warps do at a time has to stay in the instruction cache
                 uint32_t r[32];
                 tmem_ld32(from + 32 * c, r);
                 const uint32_t seen = c ? seen1 : seen0;
@@ -479,16 +474,19 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 for (uint32_t i = 0; i < 32; i += 2) {
                     const float x = EDGE && !(seen >> i & 1) ? -INFINITY : __uint_as_float(r[i]);
                     const float y = EDGE && !(seen >> (i + 1) & 1) ? -INFINITY : __uint_as_float(r[i + 1]);
-                    cm = max3(cm, x, y);
+                    cms[i / 2 % 4] = max3(cms[i / 2 % 4], x, y);
                 }
             }
+            const float cm = fmaxf(max3(cms[0], cms[1], cms[2]), cms[3]);
             const float f = KIND == KV_F16 ? rf : rf * sh.ks[g & 3], top = cm * f;
             float alpha = 1.0f;
             if (top > mx + LAZY) alpha = ex2(mx - top), mx = top;  // 0 on the first page with something to see (mx = -inf)
             const float base = (float)UP - (mx > -INFINITY ? mx : 0.0f);
             const f32x2 ff = pair(f, f), shift = pair(base, base);
             f32x2 ps = 0;
-#pragma unroll
+            wait_all(&sh.p_free[g & 1], ((g >> 1) & 1) ^ 1);
+            tc_fence_after();
+#pragma unroll 1
             for (uint32_t c = 0; c < 2; ++c) {
                 uint32_t r[32], w0[16], w1[16];
                 tmem_ld32(from + 32 * c, r);
@@ -514,15 +512,14 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         meet();
         for (uint32_t turn = 0; turn < sh.batches; ++turn) {
             const uint32_t pieces = sh.pieces;
-            if (pieces) query(sh.piece[0]);
+            float amax = pieces ? largest(sh.piece[0]) : 0.0f;
             for (uint32_t k = 0; k < pieces; ++k) {
                 const ChunkPiece& p = sh.piece[k];
-                const uint32_t heads = min(a.group, CQ), t = row / heads, n = p.end - p.first;
-                const Sight see(a.span, p.pos0 + t), last_see(a.span, p.pos0 + p.tokens - 1);
-#pragma unroll
-                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0;
-                float alpha_prev = 0.0f;
-                mx = -INFINITY, sums = 0, odd_first = 0xFFFFFFFFu, odd_end = 0, lost = false;
+                query(p, amax);
+                if (k + 1 < pieces) amax = largest(sh.piece[k + 1]);
+                const uint32_t n = p.end - p.first;
+                const Sight see(a.span, p.pos0 + row / min(a.group, CQ)), last_see(a.span, p.pos0 + p.tokens - 1);
+                mx = -INFINITY, sums = 0;
                 for (uint32_t j = 0; j < n; ++j, ++g) {
                     const uint32_t u = p.first + j, base = (u < p.sinks ? u : u + p.skip) * KV_PAGE;
                     wait_all(&sh.s_full[g & 1], (g >> 1) & 1);
@@ -537,20 +534,74 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                     } else {
                         alpha = page(Constant<0>{}, 0, 0);
                     }
-                    if (lane == 0) mbar_arrive(&sh.s_free[g & 1]);
-                    if (j > 0) add_page(g - 1, alpha_prev, u - 1);
-                    alpha_prev = alpha;
+                    sh.alpha[g & 3][row] = alpha;
+                    if (j + 1 == n) {
+                        const float2 two = both(sums);
+                        sh.stat[g & 3][0][row] = mx, sh.stat[g & 3][1][row] = ok ? two.x + two.y : NAN;
+                    }
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                     tc_fence_before();
                     __syncwarp();
-                    if (ok && lane == 0) mbar_arrive(&sh.p_full);  // and the output before has been read
+                    if (lane == 0) {
+                        mbar_arrive(&sh.s_free[g & 1]);
+                        if (ok) mbar_arrive(&sh.p_full[g & 1]);
+                    }
                 }
-                if (k + 1 < pieces) query(sh.piece[k + 1]);
-                add_page(g - 1, alpha_prev, p.end - 1);
-                const float2 two = both(sums);
-                float sum = two.x + two.y;
+            }
+            meet();
+            meet();
+        }
+    } else if (warp < C_FIRST_CONV) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C_REGS_SUM));
+        // ── the output: a thread a query row ──
+        const uint32_t row = tid - C_SOFT * 32, lanes = tmem + (((warp - C_SOFT) * 32) << 16);
+        uint32_t g = 0;
+        f32x2 o[HD / 2];  // times 2^UP, as the probabilities are
+        meet();
+        for (uint32_t turn = 0; turn < sh.batches; ++turn) {
+            const uint32_t pieces = sh.pieces;
+            for (uint32_t k = 0; k < pieces; ++k) {
+                const ChunkPiece& p = sh.piece[k];
+                const uint32_t heads = min(a.group, CQ), t = row / heads, n = p.end - p.first;
+                uint32_t odd_first = 0xFFFFFFFFu, odd_end = 0;
+                bool lost = false;
+#pragma unroll
+                for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0;
+                for (uint32_t j = 0; j < n; ++j, ++g) {
+                    wait_all(&sh.o_full, g & 1);
+                    tc_fence_after();
+                    const float alpha = sh.alpha[g & 3][row];
+                    if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
+#pragma unroll
+                        for (uint32_t i = 0; i < HD / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
+                    }
+                    if (*reinterpret_cast<const uint64_t*>(sh.odd[g & 3]) != 0) odd_first = min(odd_first, p.first + j), odd_end = p.first + j + 1;
+                    lost |= sh.lost[g & 15] != 0;
+#pragma unroll
+                    for (uint32_t c = 0; c < HD / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(lanes + T::O + 32 * c, r);
+                        const float f = KIND == KV_F16 ? 1.0f : sh.vs[g & 3][c];
+#pragma unroll
+                        for (uint32_t i = 0; i < 16; ++i) {
+                            f32x2& x = o[16 * c + i];
+                            x = KIND == KV_F16 ? add2(x, pair(r[2 * i], r[2 * i + 1])) : fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
+                        }
+                    }
+                    if (j + 1 < n) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.o_free);
+                    }
+                }
+                const float mx = sh.stat[(g - 1) & 3][0][row];
+                float sum = sh.stat[(g - 1) & 3][1][row];
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.o_free);
                 if (!ok || lost) sum = NAN;
-                if (lost && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+                if (lost && row == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+                const Sight see(a.span, p.pos0 + t);
                 const bool live = t < p.tokens && (p.head0 + row % heads) / a.group == p.kvh;
                 if (odd_end != 0 && live) {
                     // values that are not finite stood as zeros in the products: they go where a row sees them, and nowhere else
@@ -592,17 +643,16 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                         __stcg(reinterpret_cast<float4*>(mine) + i * CQ + row, make_float4(x.x, x.y, y.x, y.y));
                     }
                     __stcg(mine + HD * CQ + row, mx), __stcg(mine + (HD + 1) * CQ + row, sum);
-                    __threadfence();
-                    asm volatile("bar.sync 5, %0;" ::"n"(C_SOFT * 32) : "memory");
-                    if (tid == 0) {
+                    asm volatile("bar.sync 5, %0;" ::"n"(C_SUM * 32) : "memory");
+                    if (row == 0) {
+                        __threadfence();  // behind the barrier: for all of the CTA's stores
                         const bool last = atomicAdd(a.arrived + p.owner, 1) == p.parts - 1;
                         if (last) a.arrived[p.owner] = 0;
                         __threadfence();
                         sh.last = last;
                     }
-                    asm volatile("bar.sync 5, %0;" ::"n"(C_SOFT * 32) : "memory");
+                    asm volatile("bar.sync 5, %0;" ::"n"(C_SUM * 32) : "memory");
                     if (sh.last) {
-                        __threadfence();
                         auto part_of = [&](uint32_t i) { return a.part + ((uint64_t)(p.owner + i) * 2 + (i == 0)) * PART; };
                         float best = -INFINITY, den = 0.0f;
                         for (uint32_t i = 0; i < p.parts; ++i) best = fmaxf(best, __ldcg(part_of(i) + HD * CQ + row));
@@ -625,10 +675,10 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             meet();
             meet();
         }
-    } else if (warp < C_SOFT + C_CONV) {
+    } else if (warp < C_ISSUE) {
         // ── converters; first they cut the work ──
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C_REGS_CONV));
-        const uint32_t ct = tid - C_SOFT * 32, cw = warp - C_SOFT;
+        const uint32_t ct = tid - C_FIRST_CONV * 32, cw = warp - C_FIRST_CONV;
         auto scan = [&](uint32_t x, uint32_t which, uint32_t* total) {  // sum of the threads in front
             uint32_t run = x;
 #pragma unroll
@@ -764,7 +814,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         const uint32_t batches = sh.batches;
         for (uint32_t turn = 0; turn < batches; ++turn) {
             const uint32_t pieces = sh.pieces;
-            if (warp == C_SOFT + C_CONV) {
+            if (warp == C_ISSUE) {
                 constexpr uint32_t idesc_s = umma_idesc_f16(KV_PAGE), idesc_o = umma_idesc_f16(HD) | 1u << 16;  // values MN-major
                 const uint64_t dk = umma_desc(k_base), dv = umma_desc_values(v_base);
                 // scores of page j in one accumulator, small products first; `begins`: of a piece's first, the queries are in place
@@ -805,7 +855,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                     if (more && !begins) scores(g + 1, false);
                     // the probabilities are in place, the output before has been read
                     wait_all(&sh.v_full[g & 1], (g >> 1) & 1);
-                    if (wait_all(&sh.p_full, g & 1)) {
+                    wait_all(&sh.o_free, (g & 1) ^ 1);
+                    if (wait_all(&sh.p_full[g & 1], (g >> 1) & 1)) {
                         tc_fence_after();
                         if (elect_one()) {
                             const uint64_t hi = dv + (uint64_t)(g & 1) * (T::V_STAGE >> 4), lo = hi + (T::V_PLANE >> 4);
@@ -818,13 +869,14 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
 #pragma unroll
                             for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_ts(d, p_hi + 8 * kk, hi + 128 * kk, idesc_o, 1);
                             umma_commit(&sh.v_empty[g & 1]);
+                            umma_commit(&sh.p_free[g & 1]);
                             umma_commit(&sh.o_full);
                         }
                         __syncwarp();
                     }
                     if (begins) scores(g + 1, true);  // behind the products of the piece before: its rows bring the next queries
                 }
-            } else if (warp == C_SOFT + C_CONV + 1) {
+            } else if (warp == C_LOAD) {
                 // ── loader: a page's keys, or values, of a head are one run of memory; page ids 32 at a time, a lane each ──
                 for (uint32_t k = 0; k < pieces; ++k) {
                     const ChunkPiece& p = sh.piece[k];
@@ -843,7 +895,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                         if (wait_all(&sh.rk_empty[st], freed)) {
                             ++k_sent;
                             if (lane == 0) {
-                                sh.lost[g & 7] = !fine;
+                                sh.lost[g & 15] = !fine;
                                 mbar_arrive_expect_tx(&sh.rk_full[st], T::RAW);
                                 bulk_g2s(raw_k + st * T::RAW, src, T::RAW, &sh.rk_full[st]);
                             }
@@ -861,12 +913,12 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             meet();
             meet();
         }
-        if (!ok && warp == C_SOFT + C_CONV) {  // products in flight still use tensor memory and the tiles
+        if (!ok && warp == C_ISSUE) {  // products in flight still use tensor memory and the tiles
             if (elect_one()) umma_commit(&sh.drained);
             __syncwarp();
             mbar_wait(&sh.drained, 0);
         }
-        if (!ok && warp == C_SOFT + C_CONV + 1) {  // copies in flight still write to shared memory
+        if (!ok && warp == C_LOAD) {  // copies in flight still write to shared memory
             for (uint32_t back = 1; back <= 2; ++back) {
                 if (k_sent >= back) mbar_wait(&sh.rk_full[(k_sent - back) & 1], ((k_sent - back) >> 1) & 1);
                 if (v_sent >= back) mbar_wait(&sh.rv_full[(v_sent - back) & 1], ((v_sent - back) >> 1) & 1);
@@ -875,7 +927,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
     }
     meet();
     if (tid == 0 && sh.abort_flag && error_flag) *reinterpret_cast<volatile int*>(error_flag) = 1;
-    if (warp == C_SOFT + C_CONV)
+    if (warp == C_ISSUE)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
