@@ -12,7 +12,7 @@
 // pages.  It is cut into equal pieces, one a CTA; pieces of a tile that several CTAs have are joined by the last of them to arrive, in order.
 //
 // Warps: 0 .. 3 softmax, a thread a query row; 4 .. 7 add up the output, the same; 8 .. 15 first cut the work, then turn the pages' codes
-// into swizzled tiles, two stages; 16 issues the products; 17 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
+// into swizzled tiles, two stages (half of them keys, half values); 16 issues the products; 17 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
 // (A of the output) of two pages, output of one.
 //
 // Every wait on an mbarrier is bounded.  A warp whose wait ran out waits for none any more, hands nothing on, and goes through the
@@ -31,14 +31,17 @@ constexpr uint32_t C_SOFT = 4, C_SUM = 4, C_CONV = 8;  // warps
 constexpr uint32_t C_FIRST_CONV = C_SOFT + C_SUM, C_ISSUE = C_FIRST_CONV + C_CONV, C_LOAD = C_ISSUE + 1;
 constexpr int UP = 6;                        // probabilities stand times 2^UP ..
 constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
+constexpr uint32_t C_HALF = C_CONV / 2;                // of the converters: for keys, the others for values
 constexpr uint32_t C_THREADS = (C_ISSUE + 4) * 32;  // whole warpgroups: they trade registers
-// Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 72, the
-// softmax threads (32 scores, 32 terms) 128 x 104, and those that add up the output (128 running sums, 32 new ones) 128 x 200: all of it.
-constexpr int C_REGS_ISSUE = 32, C_REGS_CONV = 72, C_REGS_SOFT = 104, C_REGS_SUM = 200;
+// Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 64, the
+// softmax threads (32 scores, 32 terms) 128 x 112, and those that add up the output (128 running sums, 32 new ones) 128 x 208: all of it.
+// No role may spill in its loop: the tiles leave so little L1 that spills come back from L2 (512 tokens behind 3584: 108 -> 171 us).
+constexpr int C_REGS_ISSUE = 32, C_REGS_CONV = 64, C_REGS_SOFT = 112, C_REGS_SUM = 208;
 static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT + C_SUM * 32 * C_REGS_SUM <= C_THREADS * 96, "registers");
 
 constexpr uint32_t SEG_UNITS = 2;   // a tile's beginning and end in pages
 constexpr uint32_t C_PIECES = 96;   // pieces of a CTA at a time
+constexpr uint32_t C_STAGE = 5;     // 16-byte vectors a row of the stage, one of them empty: no bank conflicts
 
 // Pages first .. end - 1 of the list of pages that a tile sees: those of the sinks, then those from its window's first on.
 struct ChunkPiece {
@@ -52,12 +55,13 @@ struct ChunkPiece {
 // what the warps share beside the tiles
 struct ChunkShared {
     float ks[4];              // inverse scale of the keys, by page % 4
-    float vs[4][4];           // inverse scales of the values' blocks, by page % 4
-    uint8_t odd[4][C_CONV];   // values that are not finite, by page % 4 and converter
+    float vs[4][4];           // inverse scales of the values' blocks, by page % 4 (halves: 1)
+    uint8_t odd[4][C_HALF];   // values that are not finite, by page % 4 and converter
     uint8_t lost[16];         // a page id outside the cache, by page % 16
     float alpha[4][CQ];       // what the sums before are worth under the new maximum, by page % 4
     float stat[4][2][CQ];     // maxima and sums of a finished piece, by its last page % 4
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], q_full, p_full[2], p_free[2], o_full, o_free;
+    // page % 2: what the products wait for (operands in place, the result before read), that they are through
+    uint64_t s_go[2], s_done[2], o_go[2], o_done[2], q_full;
     uint64_t rk_full[2], rk_empty[2], rv_full[2], rv_empty[2];  // the raw pages
     uint64_t drained;         // the products of a CTA that gives up
     uint32_t tmem_slot;
@@ -65,6 +69,7 @@ struct ChunkShared {
     uint32_t last;            // this CTA was the last one to bring its part of a tile
     uint32_t scan[2][C_CONV], first_seg, end_seg;
     uint32_t pieces, batches;  // pieces of this batch; batches
+    float4 stage[2][4][32][C_STAGE];  // of the softmax warps and of the output's: 16 dimensions of 32 rows on their way between lanes
     ChunkPiece piece[C_PIECES];
 };
 
@@ -348,25 +353,20 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, batch = a.c.n_seq;
     const bool aligned = k_base % 1024 == 0;  // the swizzle's period; no static shared memory stands in front
+    if (KIND == KV_F16 && tid < 16) sh.vs[tid / 4][tid % 4] = 1.0f;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], C_CONV);
-            mbar_init(&sh.v_full[i], C_CONV);
-            mbar_init(&sh.k_empty[i], 1);
-            mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.s_go[i], C_HALF + C_SOFT);
+            mbar_init(&sh.s_done[i], 1);
+            mbar_init(&sh.o_go[i], C_HALF + C_SOFT + C_SUM);
+            mbar_init(&sh.o_done[i], 1);
             mbar_init(&sh.rk_full[i], 1);
             mbar_init(&sh.rv_full[i], 1);
-            mbar_init(&sh.rk_empty[i], C_CONV);
-            mbar_init(&sh.rv_empty[i], C_CONV);
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.s_free[i], C_SOFT);
-            mbar_init(&sh.p_full[i], C_SOFT);  // softmax may be a page ahead of the products
-            mbar_init(&sh.p_free[i], 1);
+            mbar_init(&sh.rk_empty[i], C_HALF);
+            mbar_init(&sh.rv_empty[i], C_HALF);
         }
-        mbar_init(&sh.q_full, C_SOFT);
-        mbar_init(&sh.o_full, 1);
-        mbar_init(&sh.o_free, C_SUM);
         mbar_init(&sh.drained, 1);
+        mbar_init(&sh.q_full, C_SOFT);
         sh.abort_flag = !aligned;
         mbar_fence_init();
     }
@@ -408,49 +408,72 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         const uint32_t row = tid, lanes = tmem + ((warp * 32) << 16);
         uint32_t g = 0;   // pages so far
         float rf = 0.0f;  // inverse scale of the query row, times log2(e) and the softmax scale
-        // this thread's row of a piece, and whether there is one
-        auto row_of = [&](const ChunkPiece& p, bool* live) {
-            const uint32_t heads = min(a.group, CQ), t = row / heads, h = row % heads;
-            *live = t < p.tokens && (p.head0 + h) / a.group == p.kvh;
-            return reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + (*live ? t : 0)) * a.q_stride + (uint64_t)(p.head0 + (*live ? h : 0)) * HD);
+        // Rows come 16 dimensions of 8 rows a load, four lanes a row (a row a lane asks the cache for 32 lines a load: 128 rows of 128
+        // took 4 us), and go to their lanes through the stage.
+        const uint32_t heads = min(a.group, CQ);
+        auto rows_of = [&](const ChunkPiece& p, uint32_t i) -> const float4* {  // of row 8 i + lane / 4 of the warp, its lane % 4-th vector
+            const uint32_t r = warp * 32 + 8 * i + lane / 4, t = r / heads, h = r % heads;
+            if (t >= p.tokens || (p.head0 + h) / a.group != p.kvh) return nullptr;
+            return reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + t) * a.q_stride + (uint64_t)(p.head0 + h) * HD) + lane % 4;
         };
-        // The largest magnitude of the row, asked for a piece ahead: the row itself then comes from L2.
+        auto load = [](const float4* from, uint32_t at) { return from ? from[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
+        // The largest magnitude of the thread's row, asked for a piece ahead: the row itself then comes from L2.
         auto largest = [&](const ChunkPiece& p) {
-            bool live;
-            const float4* src = row_of(p, &live);
-            float amax = 0.0f;
-#pragma unroll 16
-            for (uint32_t i = 0; i < HD / 4; ++i) {
-                const float4 v = src[i];
-                amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+            float amax[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float4* from = rows_of(p, i);
+                amax[i] = 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < HD / 16; ++c) {
+                    const float4 v = load(from, 4 * c);
+                    amax[i] = fmaxf(amax[i], fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                }
             }
-            return live ? amax : 0.0f;
+            float mine = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                float x = amax[i];
+                x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
+                x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+                x = __shfl_sync(0xFFFFFFFFu, x, lane % 8 * 4);
+                mine = lane / 8 == i ? x : mine;
+            }
+            return mine;
         };
         // a piece's queries into tensor memory; the scores before have been worked out
         auto query = [&](const ChunkPiece& p, float amax) {
-            bool live;
-            const float4* src = row_of(p, &live);
             // a power of two that puts the row's largest value just below 2^15, with the sign of the scale: the row's maximum is
             // looked for before the scores are multiplied by rf, which must not turn their order round
             const uint32_t e = __float_as_uint(amax) >> 23, bits = e == 255 ? 127u : min(254u, 268u - e);
-            const float sc = live ? copysignf(__uint_as_float(bits << 23), a.scale) : 0.0f;
+            const float sc = copysignf(__uint_as_float(bits << 23), a.scale);
             rf = (bits == 254 ? __uint_as_float(0x00400000u) : __uint_as_float((254u - bits) << 23)) * (fabsf(a.scale) * 1.44269504f);
+            const float4* from[4];
 #pragma unroll
-            for (uint32_t c = 0; c < HD / 64; ++c) {
-                float4 v[16];
+            for (uint32_t i = 0; i < 4; ++i) from[i] = rows_of(p, i);
+            float4 (&stage)[32][C_STAGE] = sh.stage[0][warp];
+            float4 v[4], next[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 16; ++i) v[i] = src[16 * c + i];
+            for (uint32_t i = 0; i < 4; ++i) next[i] = load(from[i], 0);
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD / 16; ++c) {
 #pragma unroll
-                for (uint32_t i = 0; i < 16; i += 4) {
-                    uint32_t hi[8], lo[8];
+                for (uint32_t i = 0; i < 4; ++i) v[i] = next[i];
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {
-                        const float4 x = v[i + k];
-                        split2(x.x * sc, x.y * sc, &hi[2 * k], &lo[2 * k]), split2(x.z * sc, x.w * sc, &hi[2 * k + 1], &lo[2 * k + 1]);
-                    }
-                    tmem_st8(lanes + T::Q_HI + 32 * c + 2 * i, hi);
-                    tmem_st8(lanes + T::Q_LO + 32 * c + 2 * i, lo);
+                for (uint32_t i = 0; i < 4; ++i)
+                    if (c + 1 < HD / 16) next[i] = load(from[i], 4 * (c + 1));
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) stage[8 * i + lane / 4][lane % 4] = v[i];
+                __syncwarp();
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    const float4 x = stage[lane][i];
+                    split2(x.x * sc, x.y * sc, &hi[2 * i], &lo[2 * i]), split2(x.z * sc, x.w * sc, &hi[2 * i + 1], &lo[2 * i + 1]);
                 }
+                __syncwarp();
+                tmem_st8(lanes + T::Q_HI + 8 * c, hi);
+                tmem_st8(lanes + T::Q_LO + 8 * c, lo);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
@@ -484,7 +507,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             const float base = (float)UP - (mx > -INFINITY ? mx : 0.0f);
             const f32x2 ff = pair(f, f), shift = pair(base, base);
             f32x2 ps = 0;
-            wait_all(&sh.p_free[g & 1], ((g >> 1) & 1) ^ 1);
+            wait_all(&sh.o_done[g & 1], ((g >> 1) & 1) ^ 1);
             tc_fence_after();
 #pragma unroll 1
             for (uint32_t c = 0; c < 2; ++c) {
@@ -509,6 +532,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             sums = fma2(sums, pair(alpha, alpha), ps);
             return alpha;
         };
+        if (lane == 0) mbar_arrive(&sh.s_go[0]), mbar_arrive(&sh.s_go[1]);  // nothing to read in front of the first two
         meet();
         for (uint32_t turn = 0; turn < sh.batches; ++turn) {
             const uint32_t pieces = sh.pieces;
@@ -518,11 +542,11 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 query(p, amax);
                 if (k + 1 < pieces) amax = largest(sh.piece[k + 1]);
                 const uint32_t n = p.end - p.first;
-                const Sight see(a.span, p.pos0 + row / min(a.group, CQ)), last_see(a.span, p.pos0 + p.tokens - 1);
+                const Sight see(a.span, p.pos0 + row / heads), last_see(a.span, p.pos0 + p.tokens - 1);
                 mx = -INFINITY, sums = 0;
                 for (uint32_t j = 0; j < n; ++j, ++g) {
                     const uint32_t u = p.first + j, base = (u < p.sinks ? u : u + p.skip) * KV_PAGE;
-                    wait_all(&sh.s_full[g & 1], (g >> 1) & 1);
+                    wait_all(&sh.s_done[g & 1], (g >> 1) & 1);
                     tc_fence_after();
                     float alpha;
                     if (base + KV_PAGE > p.pos0 + 1 || (base < last_see.low && base + KV_PAGE > last_see.sinks)) {
@@ -543,8 +567,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(&sh.s_free[g & 1]);
-                        if (ok) mbar_arrive(&sh.p_full[g & 1]);
+                        mbar_arrive(&sh.s_go[g & 1]);
+                        if (ok) mbar_arrive(&sh.o_go[g & 1]);
                     }
                 }
             }
@@ -557,6 +581,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         const uint32_t row = tid - C_SOFT * 32, lanes = tmem + (((warp - C_SOFT) * 32) << 16);
         uint32_t g = 0;
         f32x2 o[HD / 2];  // times 2^UP, as the probabilities are
+        if (lane == 0) mbar_arrive(&sh.o_go[0]);  // nothing to read in front of the first one
         meet();
         for (uint32_t turn = 0; turn < sh.batches; ++turn) {
             const uint32_t pieces = sh.pieces;
@@ -568,72 +593,97 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
 #pragma unroll
                 for (uint32_t i = 0; i < HD / 2; ++i) o[i] = 0;
                 for (uint32_t j = 0; j < n; ++j, ++g) {
-                    wait_all(&sh.o_full, g & 1);
+                    wait_all(&sh.o_done[g & 1], (g >> 1) & 1);
                     tc_fence_after();
                     const float alpha = sh.alpha[g & 3][row];
                     if (__any_sync(0xFFFFFFFFu, alpha != 1.0f)) {
 #pragma unroll
                         for (uint32_t i = 0; i < HD / 2; ++i) o[i] = mul2(o[i], pair(alpha, alpha));
                     }
-                    if (*reinterpret_cast<const uint64_t*>(sh.odd[g & 3]) != 0) odd_first = min(odd_first, p.first + j), odd_end = p.first + j + 1;
+                    if (*reinterpret_cast<const uint32_t*>(sh.odd[g & 3]) != 0) odd_first = min(odd_first, p.first + j), odd_end = p.first + j + 1;
                     lost |= sh.lost[g & 15] != 0;
 #pragma unroll
                     for (uint32_t c = 0; c < HD / 32; ++c) {
                         uint32_t r[32];
                         tmem_ld32(lanes + T::O + 32 * c, r);
-                        const float f = KIND == KV_F16 ? 1.0f : sh.vs[g & 3][c];
+                        const float f = sh.vs[g & 3][c];
 #pragma unroll
                         for (uint32_t i = 0; i < 16; ++i) {
                             f32x2& x = o[16 * c + i];
-                            x = KIND == KV_F16 ? add2(x, pair(r[2 * i], r[2 * i + 1])) : fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
+                            x = fma2(pair(r[2 * i], r[2 * i + 1]), pair(f, f), x);
                         }
                     }
                     if (j + 1 < n) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.o_free);
+                        if (lane == 0) mbar_arrive(&sh.o_go[(g + 1) & 1]);
                     }
                 }
                 const float mx = sh.stat[(g - 1) & 3][0][row];
                 float sum = sh.stat[(g - 1) & 3][1][row];
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.o_free);
+                if (lane == 0) mbar_arrive(&sh.o_go[g & 1]);
                 if (!ok || lost) sum = NAN;
                 if (lost && row == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
                 const Sight see(a.span, p.pos0 + t);
                 const bool live = t < p.tokens && (p.head0 + row % heads) / a.group == p.kvh;
-                if (odd_end != 0 && live) {
-                    // values that are not finite stood as zeros in the products: they go where a row sees them, and nowhere else
+                // Values that are not finite stood as zeros in the products: they go where a row sees them, and nowhere else; at(d): where
+                // this row's dimension d stands.
+                auto add_odd = [&](auto at) {
+                    if (!live) return;
+#pragma unroll 1
                     for (uint32_t u = odd_first; u < odd_end; ++u) {
                         const uint32_t number = u < p.sinks ? u : u + p.skip;
                         const int32_t id = a.c.table[(uint64_t)p.seq * a.c.table_stride + number];
                         if (id < 0 || (uint32_t)id >= a.c.n_pages) continue;
                         const uint8_t* values = a.c.pages + ((uint64_t)id * a.c.n_kv + p.kvh) * HEAD + HEAD / 2;
+#pragma unroll 1
                         for (uint32_t i = 0; i < KV_PAGE; ++i) {
-                            const uint32_t at = number * KV_PAGE + i;
-                            if (at >= see.end || (at < see.low && at >= see.sinks)) continue;
-#pragma unroll
+                            const uint32_t t = number * KV_PAGE + i;
+                            if (t >= see.end || (t < see.low && t >= see.sinks)) continue;
+#pragma unroll 1
                             for (uint32_t d = 0; d < HD; d += 4) {
                                 const float4 v = kv_load<KIND, HD, true>(values, i, d);
-                                auto odd = [](float x) { return fabsf(x) < INFINITY ? 0.0f : x; };
-                                o[d / 2] = add2(o[d / 2], pair(odd(v.x), odd(v.y))), o[d / 2 + 1] = add2(o[d / 2 + 1], pair(odd(v.z), odd(v.w)));
+                                if (!(fabsf(v.x) < INFINITY)) *at(d) += v.x;
+                                if (!(fabsf(v.y) < INFINITY)) *at(d + 1) += v.y;
+                                if (!(fabsf(v.z) < INFINITY)) *at(d + 2) += v.z;
+                                if (!(fabsf(v.w) < INFINITY)) *at(d + 3) += v.w;
                             }
                         }
                     }
-                }
-                float* to = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row % heads) * HD;
-                auto store = [&](float den) {
-                    if (!live) return;
+                };
+                auto store = [&](float den) {  // through the stage, as the queries came
                     const float inv = 1.0f / den;
+                    float4 (&stage)[32][C_STAGE] = sh.stage[1][warp - C_SOFT];
+                    float4* to[4];
 #pragma unroll
-                    for (uint32_t i = 0; i < HD / 4; ++i) {
-                        const float2 x = both(o[2 * i]), y = both(o[2 * i + 1]);
-                        *reinterpret_cast<float4*>(to + 4 * i) = make_float4(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t r = (warp - C_SOFT) * 32 + 8 * i + lane / 4, tok = r / heads, h = r % heads;
+                        to[i] = tok < p.tokens && (p.head0 + h) / a.group == p.kvh
+                                    ? reinterpret_cast<float4*>(a.out + (uint64_t)(p.row0 + tok) * a.out_stride + (uint64_t)(p.head0 + h) * HD) + lane % 4
+                                    : nullptr;
+                    }
+#pragma unroll
+                    for (uint32_t c = 0; c < HD / 16; ++c) {
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const float2 x = both(o[8 * c + 2 * i]), y = both(o[8 * c + 2 * i + 1]);
+                            stage[lane][i] = make_float4(x.x * inv, x.y * inv, y.x * inv, y.y * inv);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i)
+                            if (to[i]) to[i][4 * c] = stage[8 * i + lane / 4][lane % 4];
+                        __syncwarp();
                     }
                 };
                 if (p.parts == 1) {
                     store(sum);
+                    if (odd_end != 0) {
+                        float* out = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row % heads) * HD;
+                        add_odd([&](uint32_t d) { return out + d; });
+                    }
                 } else {
                     // [HD / 4][CQ] outputs of four dimensions, then maxima, then sums
                     float* mine = a.part + ((uint64_t)blockIdx.x * 2 + (p.first == 0)) * PART;
@@ -643,6 +693,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                         __stcg(reinterpret_cast<float4*>(mine) + i * CQ + row, make_float4(x.x, x.y, y.x, y.y));
                     }
                     __stcg(mine + HD * CQ + row, mx), __stcg(mine + (HD + 1) * CQ + row, sum);
+                    if (odd_end != 0) add_odd([&](uint32_t d) { return mine + (d / 4 * CQ + row) * 4 + d % 4; });
                     asm volatile("bar.sync 5, %0;" ::"n"(C_SUM * 32) : "memory");
                     if (row == 0) {
                         __threadfence();  // behind the barrier: for all of the CTA's stores
@@ -663,9 +714,16 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                             const float w = piece_weight(__ldcg(from + HD * CQ + row), best);
                             den = fmaf(w, __ldcg(from + (HD + 1) * CQ + row), den);
 #pragma unroll
-                            for (uint32_t d = 0; d < HD / 4; ++d) {
-                                const float4 v = __ldcg(reinterpret_cast<const float4*>(from) + d * CQ + row);
-                                o[2 * d] = fma2(pair(v.x, v.y), pair(w, w), o[2 * d]), o[2 * d + 1] = fma2(pair(v.z, v.w), pair(w, w), o[2 * d + 1]);
+                            for (uint32_t d = 0; d < HD / 4; d += 8) {  // eight on their way: more take the loops' registers
+                                float4 v[8];
+#pragma unroll
+                                for (uint32_t k = 0; k < 8; ++k) v[k] = __ldcg(reinterpret_cast<const float4*>(from) + (d + k) * CQ + row);
+#pragma unroll
+                                for (uint32_t k = 0; k < 8; ++k) {
+                                    f32x2 &x = o[2 * (d + k)], &y = o[2 * (d + k) + 1];
+                                    x = fma2(pair(v[k].x, v[k].y), pair(w, w), x), y = fma2(pair(v[k].z, v[k].w), pair(w, w), y);
+                                }
+                                asm volatile("" ::: "memory");
                             }
                         }
                         store(den);
@@ -750,7 +808,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         });
         asm volatile("bar.sync 7, %0;" ::"n"(C_CONV * 32) : "memory");
         const uint32_t first_seg = sh.first_seg, end_seg = sh.end_seg, batches = end_seg > first_seg ? (end_seg - first_seg + C_PIECES - 1) / C_PIECES : 0;
-        const ChunkConverter<KIND, HD, C_CONV> convert(cw, lane);
+        const ChunkConverter<KIND, HD, C_HALF> convert(cw % C_HALF, lane);
         uint32_t g = 0;
         auto list = [&](uint32_t turn) {
             const uint32_t from = first_seg + turn * C_PIECES, to = min(end_seg, from + C_PIECES);
@@ -785,20 +843,21 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 for (uint32_t j = 0; j < n; ++j, ++g) {
                     const uint32_t st = g & 1, half = (g >> 1) & 1, u = p.first + j, base = (u < p.sinks ? u : u + p.skip) * KV_PAGE;
                     const uint32_t valid = min(KV_PAGE, behind - base);
-                    wait_all(&sh.k_empty[st], half ^ 1);
-                    if (wait_all(&sh.rk_full[st], half)) {
+                    if (cw < C_HALF) {
+                        wait_all(&sh.s_done[st], half ^ 1);
+                        if (!wait_all(&sh.rk_full[st], half)) continue;
                         convert.keys(k_base + st * T::K_STAGE, raw_k + st * T::RAW, valid, &sh.ks[g & 3]);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.k_full[st]), mbar_arrive(&sh.rk_empty[st]);
-                    }
-                    wait_all(&sh.v_empty[st], half ^ 1);
-                    if (wait_all(&sh.rv_full[st], half)) {
+                        if (lane == 0) mbar_arrive(&sh.s_go[st]), mbar_arrive(&sh.rk_empty[st]);
+                    } else {
+                        wait_all(&sh.o_done[st], half ^ 1);
+                        if (!wait_all(&sh.rv_full[st], half)) continue;
                         const bool odd = __any_sync(0xFFFFFFFFu, convert.values(v_base + st * T::V_STAGE, raw_v + st * T::RAW, valid, sh.vs[g & 3]));
-                        if (lane == 0) sh.odd[g & 3][cw] = odd;
+                        if (lane == 0) sh.odd[g & 3][cw - C_HALF] = odd;
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.v_full[st]), mbar_arrive(&sh.rv_empty[st]);
+                        if (lane == 0) mbar_arrive(&sh.o_go[st]), mbar_arrive(&sh.rv_empty[st]);
                     }
                 }
             }
@@ -815,13 +874,14 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         for (uint32_t turn = 0; turn < batches; ++turn) {
             const uint32_t pieces = sh.pieces;
             if (warp == C_ISSUE) {
+                // One warp issues both, batch after batch: it waits until its products are taken in, and products of the two in turn
+                // hold each other up (two issuers: 512 tokens behind 3584 201 us).
                 constexpr uint32_t idesc_s = umma_idesc_f16(KV_PAGE), idesc_o = umma_idesc_f16(HD) | 1u << 16;  // values MN-major
                 const uint64_t dk = umma_desc(k_base), dv = umma_desc_values(v_base);
                 // scores of page j in one accumulator, small products first; `begins`: of a piece's first, the queries are in place
                 auto scores = [&](uint32_t j, bool begins) {
                     if (begins) wait_all(&sh.q_full, q_phase), q_phase ^= 1;
-                    wait_all(&sh.s_free[j & 1], ((j >> 1) & 1) ^ 1);
-                    if (!wait_all(&sh.k_full[j & 1], (j >> 1) & 1)) return;
+                    if (!wait_all(&sh.s_go[j & 1], (j >> 1) & 1)) return;
                     tc_fence_after();
                     if (elect_one()) {
                         const uint64_t d0 = dk + (uint64_t)(j & 1) * (T::K_STAGE >> 4);
@@ -835,14 +895,12 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
 #pragma unroll
                         for (uint32_t kk = 0; kk < HD / 16; ++kk)
                             umma_f16_ts(d, tmem + T::Q_HI + 8 * kk, d0 + kk / 4 * (T::K_PLANE >> 4) + kk % 4 * 2, idesc_s, 1);
-                        umma_commit(&sh.k_empty[j & 1]);
-                        umma_commit(&sh.s_full[j & 1]);
+                        umma_commit(&sh.s_done[j & 1]);
                     }
                     __syncwarp();
                 };
-                uint32_t all = 0;
-                for (uint32_t k = 0; k < pieces; ++k) all += sh.piece[k].end - sh.piece[k].first;
-                uint32_t k = 0, left = 0;  // the piece whose scores come next, pages left of it
+                uint32_t all = 0, k = 0, left = 0;  // pages; the piece whose scores come next, pages left of it
+                for (uint32_t i = 0; i < pieces; ++i) all += sh.piece[i].end - sh.piece[i].first;
                 auto next = [&] {
                     const bool begins = left == 0;
                     if (begins) left = sh.piece[k].end - sh.piece[k].first, ++k;
@@ -853,10 +911,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 for (uint32_t j = 0; j < all; ++j, ++g) {
                     const bool more = j + 1 < all, begins = more && next();
                     if (more && !begins) scores(g + 1, false);
-                    // the probabilities are in place, the output before has been read
-                    wait_all(&sh.v_full[g & 1], (g >> 1) & 1);
-                    wait_all(&sh.o_free, (g & 1) ^ 1);
-                    if (wait_all(&sh.p_full[g & 1], (g >> 1) & 1)) {
+                    if (wait_all(&sh.o_go[g & 1], (g >> 1) & 1)) {
                         tc_fence_after();
                         if (elect_one()) {
                             const uint64_t hi = dv + (uint64_t)(g & 1) * (T::V_STAGE >> 4), lo = hi + (T::V_PLANE >> 4);
@@ -868,9 +923,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                             }
 #pragma unroll
                             for (uint32_t kk = 0; kk < 4; ++kk) umma_f16_ts(d, p_hi + 8 * kk, hi + 128 * kk, idesc_o, 1);
-                            umma_commit(&sh.v_empty[g & 1]);
-                            umma_commit(&sh.p_free[g & 1]);
-                            umma_commit(&sh.o_full);
+                            umma_commit(&sh.o_done[g & 1]);
                         }
                         __syncwarp();
                     }
