@@ -15,7 +15,11 @@ namespace jq {
 
 namespace {
 
-constexpr uint32_t CHUNK_FEW = 1;
+// Passes over a sequence's pages, rows times warps' worth of heads, up to which its rows are taken one by one: a tile takes as long as
+// three to four of them (16 sequences of up to 4000 positions, two / three / four rows one by one and eight in tiles: 32 heads on 8 of
+// 128 in eight bits 29 / 45 / 56 and 60 us, in halves 32 / 49 / 73 and 64, 32 heads on 4 27 / 41 / 47 and 41).  Several tokens a pass in
+// attention_paged_kernel, 16 query rows, was no faster than one by one: its products are the bound.
+constexpr uint32_t CHUNK_FEW = 3;
 
 struct ChunkPlan {
     uint32_t group, rows, split, grid;  // query heads a kv head; of a warp; warps' worth of them; CTAs
@@ -30,7 +34,7 @@ ChunkPlan plan(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd) {
     p.split = (p.group + p.rows - 1) / p.rows;
     p.grid = std::min((uint32_t)num_sms(), ATTENTION_MOST_CTAS);
     p.part_at = ATTENTION_MOST_CTAS * 4;
-    p.few = hd <= 128 ? CHUNK_FEW : 0xFFFFFFFFu;
+    p.few = hd <= 128 ? std::max(1u, CHUNK_FEW / p.split) : 0xFFFFFFFFu;
     p.tiles = rows > p.few;
     p.bytes = p.part_at + (size_t)p.grid * 2 * (p.tiles ? CHUNK_TILE_ROWS : p.rows) * (hd + 2) * 4;
     return p;
