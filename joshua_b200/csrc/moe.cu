@@ -3,6 +3,10 @@
 // reference's loaders, which read the ids and weights back to the host on every layer
 // (src/quantized_qwen3_moe.rs:424-520, src/quantized_deepseek2.rs:522-671,
 // src/quantized_deepseek4.rs:1354-1492, src/kimi_k3.rs:256-282).  Nothing here synchronises with the host.
+//
+// These kernels are launched while the one in front still runs, and wait for it in their first statements.  What it may have written
+// is read by plain loads: read-only ones (__ldg, or through const __restrict__) may be moved above the wait.  (With those, a prompt of
+// 33 tokens behind one of 40, 8 experts of 1024 x 256, took its tiles from the lists of the one before in some runs of forty.)
 #include "common.cuh"
 #include "moe_jobs.cuh"
 #include "pipe.cuh"
@@ -16,7 +20,7 @@ namespace {
 // strided pieces in column order and then across the lanes, the same order for every batch size.  Bound by the loads
 // from L1 and L2: with one token a warp five vectors feed 16 multiply-adds a lane, with four eight feed 64.
 template <int TT>
-__global__ void __launch_bounds__(256) moe_logits_kernel(const float* __restrict__ x, const float* __restrict__ router,
+__global__ void __launch_bounds__(256) moe_logits_kernel(const float* x, const float* __restrict__ router,
                                                          uint32_t T, uint32_t E, uint32_t h,
                                                          float* __restrict__ logits) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -39,7 +43,7 @@ __global__ void __launch_bounds__(256) moe_logits_kernel(const float* __restrict
         for (uint32_t j = lane; j < h / 4; j += 32) {
             float4 u[TT];
 #pragma unroll
-            for (int r = 0; r < TT; ++r) u[r] = __ldg(a[r] + j);
+            for (int r = 0; r < TT; ++r) u[r] = a[r][j];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const float4 v = __ldg(b[q] + j);
@@ -73,7 +77,7 @@ constexpr int LG_STAGES = 4, LG_ROWS = 32;
 constexpr size_t LG_SMEM = (size_t)LG_STAGES * LG_ROWS * 512;
 constexpr uint64_t LG_MIN_LOGITS = 6144;
 constexpr size_t LG_SMEM_ALONE = 116 * 1024;  // more than half of an SM's: a CTA has it to itself
-__global__ void __launch_bounds__(128) moe_logits_tile_kernel(const float* __restrict__ x, const float* __restrict__ router,
+__global__ void __launch_bounds__(128) moe_logits_tile_kernel(const float* x, const float* __restrict__ router,
                                                               uint32_t T, uint32_t E, uint32_t h, float* __restrict__ logits) {
     extern __shared__ __align__(16) float4 s_rows[];  // [stage][16 tokens, 16 experts][32]
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -186,8 +190,8 @@ struct RouteSmem {
 
 // One warp per token: scores, selection (bias, group limit), top-k, weights.  Warp `wq` of `nwq` (at most 4)
 // takes tokens first + wq, first + wq + stride, ...
-__device__ __forceinline__ void route_tokens(const float* __restrict__ logits, const MoeRouteParams& rp, uint32_t T,
-                                             const float* __restrict__ bias, const uint32_t* __restrict__ forced_ids,
+__device__ __forceinline__ void route_tokens(const float* logits, const MoeRouteParams& rp, uint32_t T,
+                                             const float* __restrict__ bias, const uint32_t* forced_ids,
                                              uint32_t* __restrict__ ids, float* __restrict__ wts, RouteSmem& sm,
                                              uint32_t first, uint32_t stride, uint32_t wq, uint32_t lane) {
     const uint32_t E = rp.n_expert, K = rp.n_used;
@@ -331,8 +335,8 @@ __device__ __forceinline__ void route_tokens(const float* __restrict__ logits, c
 // for layers without a group limit: no trips through shared memory between the steps, loops of the token's real
 // width.  Same operations in the same order as route_tokens, hence the same ids and weights.
 template <int EPL>
-__device__ __forceinline__ void route_tokens_regs(const float* __restrict__ logits, const MoeRouteParams& rp, uint32_t T,
-                                                  const float* __restrict__ bias, const uint32_t* __restrict__ forced_ids,
+__device__ __forceinline__ void route_tokens_regs(const float* logits, const MoeRouteParams& rp, uint32_t T,
+                                                  const float* __restrict__ bias, const uint32_t* forced_ids,
                                                   uint32_t* __restrict__ ids, float* __restrict__ wts, RouteSmem& sm,
                                                   uint32_t first, uint32_t stride, uint32_t wq, uint32_t lane) {
     const uint32_t E = rp.n_expert, K = rp.n_used;
@@ -435,8 +439,8 @@ __device__ __forceinline__ void route_tokens_regs(const float* __restrict__ logi
 }
 
 // Routing of tokens first + wq, ... by warp wq: the register form where it applies, else the general one.
-__device__ __forceinline__ void route_dispatch(const float* __restrict__ logits, const MoeRouteParams& rp, uint32_t T,
-                                               const float* __restrict__ bias, const uint32_t* __restrict__ forced_ids,
+__device__ __forceinline__ void route_dispatch(const float* logits, const MoeRouteParams& rp, uint32_t T,
+                                               const float* __restrict__ bias, const uint32_t* forced_ids,
                                                uint32_t* __restrict__ ids, float* __restrict__ wts, RouteSmem& sm,
                                                uint32_t first, uint32_t stride, uint32_t wq, uint32_t lane) {
     if (rp.n_group <= 1 && rp.n_expert <= 128)
@@ -447,9 +451,9 @@ __device__ __forceinline__ void route_dispatch(const float* __restrict__ logits,
         route_tokens(logits, rp, T, bias, forced_ids, ids, wts, sm, first, stride, wq, lane);
 }
 
-__global__ void __launch_bounds__(128) moe_route_kernel(const float* __restrict__ logits, MoeRouteParams rp, uint32_t T,
+__global__ void __launch_bounds__(128) moe_route_kernel(const float* logits, MoeRouteParams rp, uint32_t T,
                                                         const float* __restrict__ bias,
-                                                        const uint32_t* __restrict__ forced_ids,
+                                                        const uint32_t* forced_ids,
                                                         uint32_t* __restrict__ ids, float* __restrict__ wts) {
     __shared__ RouteSmem sm;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -469,7 +473,7 @@ struct JobsSliceSmem {
     uint32_t cnt[JOB_SLICES][MAX_EXPERTS];
 };
 
-__device__ __forceinline__ void build_jobs_sliced(const uint32_t* __restrict__ ids, uint32_t T, uint32_t K, uint32_t E,
+__device__ __forceinline__ void build_jobs_sliced(const uint32_t* ids, uint32_t T, uint32_t K, uint32_t E,
                                                   uint32_t rows_per_job, uint32_t* __restrict__ list_token,
                                                   uint32_t* __restrict__ inv, MoeJob* __restrict__ jobs,
                                                   uint32_t* __restrict__ n_jobs, uint32_t* __restrict__ n_list,
@@ -548,7 +552,7 @@ __device__ __forceinline__ void build_jobs_sliced(const uint32_t* __restrict__ i
     }
 }
 
-__global__ void __launch_bounds__(1024) moe_jobs_kernel(const uint32_t* __restrict__ ids, uint32_t T, uint32_t K,
+__global__ void __launch_bounds__(1024) moe_jobs_kernel(const uint32_t* ids, uint32_t T, uint32_t K,
                                                         uint32_t E, uint32_t rows_per_job,
                                                         uint32_t* __restrict__ list_token, uint32_t* __restrict__ inv,
                                                         MoeJob* __restrict__ jobs, uint32_t* __restrict__ n_jobs,
@@ -575,9 +579,9 @@ __global__ void __launch_bounds__(1024) moe_jobs_kernel(const uint32_t* __restri
 // `norm_w` the tokens are RMS-normalised first (every CTA derives 1 / rms of its tokens itself), so the norm
 // kernel in front of the layer disappears.
 __global__ void __launch_bounds__(128) moe_route_fused_kernel(
-    const float* __restrict__ x, const float* __restrict__ norm_w, float eps, const float* __restrict__ router,
+    const float* x, const float* __restrict__ norm_w, float eps, const float* __restrict__ router,
     uint32_t T, uint32_t h, float* __restrict__ logits, MoeRouteParams rp, const float* __restrict__ bias,
-    const uint32_t* __restrict__ forced_ids, uint32_t* __restrict__ ids, float* __restrict__ wts, int do_jobs,
+    const uint32_t* forced_ids, uint32_t* __restrict__ ids, float* __restrict__ wts, int do_jobs,
     uint32_t rows_per_job, uint32_t* __restrict__ list_token, uint32_t* __restrict__ inv, MoeJob* __restrict__ jobs,
     uint32_t* __restrict__ n_jobs, uint32_t* __restrict__ n_list, int* __restrict__ bad_id,
     uint32_t* __restrict__ counter) {
@@ -605,7 +609,7 @@ __global__ void __launch_bounds__(128) moe_route_fused_kernel(
             for (int q = 0; q < 4; ++q) {
                 const uint32_t j = j0 + q * 128;
                 const bool in = j < h / 4;
-                u[q] = in ? __ldg(a + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                u[q] = in ? a[j] : make_float4(0.f, 0.f, 0.f, 0.f);
                 v[q] = in ? __ldg(b + j) : make_float4(0.f, 0.f, 0.f, 0.f);
                 w[q] = (in && norm_w) ? __ldg(g + j) : make_float4(1.f, 1.f, 1.f, 1.f);
             }
@@ -668,8 +672,8 @@ __global__ void __launch_bounds__(128) moe_route_fused_kernel(
 
 // y[t, :] = sum over slots (in slot order) of w[t, s] * out[inv[t*K + s], :]  (+ shared[t, :]) (+ residual[t, :],
 // which may be y itself)
-__global__ void __launch_bounds__(256) moe_combine_kernel(const float* __restrict__ out, const uint32_t* __restrict__ inv,
-                                                          const float* __restrict__ wts, const float* __restrict__ shared,
+__global__ void __launch_bounds__(256) moe_combine_kernel(const float* out, const uint32_t* inv,
+                                                          const float* wts, const float* shared,
                                                           const float* residual, uint32_t T, uint32_t K, uint32_t h,
                                                           float* y) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -735,7 +739,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const float* __restric
 // out = silu(clamp(g)) * clamp(u), element-wise (the dense shared-expert path at batches the grouped kernel
 // does not take)
 // out may be g
-__global__ void __launch_bounds__(256) swiglu_kernel(const float* g, const float* __restrict__ u, uint64_t n, float clamp, float* out) {
+__global__ void __launch_bounds__(256) swiglu_kernel(const float* g, const float* u, uint64_t n, float clamp, float* out) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint64_t i = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x) {
@@ -750,8 +754,8 @@ __global__ void __launch_bounds__(256) swiglu_kernel(const float* g, const float
 
 // xs[pos, :] = x[list_token[pos], :] for the expert-sorted list (pos < *n_list): the activation rows in bucket
 // order, so that an expert's rows are contiguous for a tile GEMM.
-__global__ void __launch_bounds__(256) moe_gather_kernel(const float* __restrict__ x, const uint32_t* __restrict__ list_token,
-                                                         const uint32_t* __restrict__ n_list, uint32_t P, uint32_t h,
+__global__ void __launch_bounds__(256) moe_gather_kernel(const float* x, const uint32_t* list_token,
+                                                         const uint32_t* n_list, uint32_t P, uint32_t h,
                                                          float* __restrict__ xs) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -760,7 +764,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const float* __restrict
     for (uint64_t i = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
         const uint32_t pos = (uint32_t)(i / h4), c = (uint32_t)(i % h4);
         reinterpret_cast<float4*>(xs)[(uint64_t)pos * h4 + c] =
-            __ldg(reinterpret_cast<const float4*>(x) + (uint64_t)list_token[pos] * h4 + c);
+            reinterpret_cast<const float4*>(x)[(uint64_t)list_token[pos] * h4 + c];
     }
 }
 
@@ -770,8 +774,8 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const float* __restrict
 // to `small_jobs` for the grouped decode kernel.  counts = {narrow tiles, wide tiles, rows in the list, small jobs}.
 // Which slot of a list an entry takes depends on timing; the products do not (every entry is computed on its own).
 // One CTA.
-__global__ void __launch_bounds__(1024) moe_tiles_kernel(const MoeJob* __restrict__ jobs, const uint32_t* __restrict__ n_jobs,
-                                                         const uint32_t* __restrict__ n_list, uint32_t E, uint32_t min_rows,
+__global__ void __launch_bounds__(1024) moe_tiles_kernel(const MoeJob* jobs, const uint32_t* n_jobs,
+                                                         const uint32_t* n_list, uint32_t E, uint32_t min_rows,
                                                          GemmTile* __restrict__ narrow, GemmTile* __restrict__ wide,
                                                          MoeJob* __restrict__ small_jobs, uint32_t* __restrict__ counts) {
     __shared__ uint32_t s_row0[MAX_EXPERTS], s_cnt[MAX_EXPERTS], s_n[3];
@@ -810,8 +814,8 @@ __global__ void __launch_bounds__(1024) moe_tiles_kernel(const MoeJob* __restric
 }
 
 // SwiGLU over the first *n_rows rows of [rows, inter] (rows of the expert-sorted list that exist).
-__global__ void __launch_bounds__(256) swiglu_rows_kernel(const float* __restrict__ g, const float* __restrict__ u,
-                                                          const uint32_t* __restrict__ n_rows, uint32_t max_rows, uint32_t inter,
+__global__ void __launch_bounds__(256) swiglu_rows_kernel(const float* g, const float* u,
+                                                          const uint32_t* n_rows, uint32_t max_rows, uint32_t inter,
                                                           float clamp, float* __restrict__ out) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
