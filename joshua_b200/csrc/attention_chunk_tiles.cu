@@ -31,13 +31,22 @@ constexpr uint32_t C_SOFT = 4, C_SUM = 4, C_CONV = 8;  // warps
 constexpr uint32_t C_FIRST_CONV = C_SOFT + C_SUM, C_ISSUE = C_FIRST_CONV + C_CONV, C_LOAD = C_ISSUE + 1;
 constexpr int UP = 6;                        // probabilities stand times 2^UP ..
 constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
+// Scores are multiplied and shifted in one step, exact but for the shift itself: with maxima from here on, whose last bit may be worth
+// more than LAZY leaves, they are rounded as the maximum was and shifted by it first, in a step of their own.
+constexpr float FAR = 0x1p20f;
 constexpr uint32_t C_HALF = C_CONV / 2;                // of the converters: for keys, the others for values
 constexpr uint32_t C_THREADS = (C_ISSUE + 4) * 32;  // whole warpgroups: they trade registers
-// Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the converters 256 x 64, the
-// softmax threads (32 scores, 32 terms) 128 x 112, and those that add up the output (128 running sums, 32 new ones) 128 x 208: all of it.
+// Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the softmax threads (32 scores, 32
+// terms) 128 x 112, the converters 256 x 64 and those that add up the output (128 running sums, 32 new ones) 128 x 208: all of it.  With
+// heads of 64 the latter have half the sums and leave the converters more.
 // No role may spill in its loop: the tiles leave so little L1 that spills come back from L2 (512 tokens behind 3584: 108 -> 171 us).
-constexpr int C_REGS_ISSUE = 32, C_REGS_CONV = 64, C_REGS_SOFT = 112, C_REGS_SUM = 208;
-static_assert(128 * C_REGS_ISSUE + C_CONV * 32 * C_REGS_CONV + C_SOFT * 32 * C_REGS_SOFT + C_SUM * 32 * C_REGS_SUM <= C_THREADS * 96, "registers");
+constexpr int C_REGS_ISSUE = 32, C_REGS_SOFT = 112;
+constexpr int c_regs_conv(uint32_t hd) { return hd == 64 ? 72 : 64; }
+constexpr int c_regs_sum(uint32_t hd) { return hd == 64 ? 192 : 208; }
+constexpr bool c_regs_fit(uint32_t hd) {
+    return 128 * C_REGS_ISSUE + C_CONV * 32 * c_regs_conv(hd) + C_SOFT * 32 * C_REGS_SOFT + C_SUM * 32 * c_regs_sum(hd) <= C_THREADS * 96;
+}
+static_assert(c_regs_fit(64) && c_regs_fit(128), "registers");
 
 constexpr uint32_t SEG_UNITS = 2;   // a tile's beginning and end in pages
 constexpr uint32_t C_PIECES = 96;   // pieces of a CTA at a time
@@ -89,6 +98,7 @@ struct ChunkConverter {
     static constexpr uint32_t BLOCKS = KIND == KV_Q4_0 ? 2 : 1, COLS = NB / BLOCKS, ITEMS = 4 * COLS;  // blocks of a lane's 16 bytes
     static constexpr int TOP = KIND == KV_Q4_0 ? 26 : 22;  // a scale below 2^(e - 14) times 2^(TOP - e) times a code stays below 2^15
     static_assert(WARPS % COLS == 0, "a warp has blocks of its own");
+    static_assert(CODES % 16 == 0 && K_LO % 1024 == 0 && V_LO % 1024 == 0 && TOP / 2 < 15, "vectors of codes, the swizzle's period, Up's factors");
     uint32_t cw, lane, r, c, b0;
     uint32_t key_to, value_to[2];  // places in a stage: keys of row r, values of positions 2 c and 2 c + 1
 
@@ -501,10 +511,23 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 }
             }
             const float cm = fmaxf(max3(cms[0], cms[1], cms[2]), cms[3]);
-            const float f = KIND == KV_F16 ? rf : rf * sh.ks[g & 3], top = cm * f;
-            float alpha = 1.0f;
-            if (top > mx + LAZY) alpha = ex2(mx - top), mx = top;  // 0 on the first page with something to see (mx = -inf)
-            const float base = (float)UP - (mx > -INFINITY ? mx : 0.0f);
+            float f = KIND == KV_F16 ? rf : rf * sh.ks[g & 3], alpha = 1.0f;
+            const float top = __fmul_rn(cm, f);
+            if (top - mx > LAZY) alpha = ex2(mx - top), mx = top;  // 0 on the first page with something to see (mx = -inf)
+            float base = (float)UP - (mx > -INFINITY ? mx : 0.0f);
+            if (__any_sync(0xFFFFFFFFu, fabsf(base) >= FAR)) {
+                const float less = mx > -INFINITY ? mx : 0.0f;
+#pragma unroll 1
+                for (uint32_t c = 0; c < KV_PAGE; c += 8) {
+                    uint32_t r[8];
+                    tmem_ld8(from + c, r);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i) r[i] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(r[i]), f), less));
+                    tmem_st8(from + c, r);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                f = 1.0f, base = (float)UP;
+            }
             const f32x2 ff = pair(f, f), shift = pair(base, base);
             f32x2 ps = 0;
             wait_all(&sh.o_done[g & 1], ((g >> 1) & 1) ^ 1);
@@ -576,7 +599,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             meet();
         }
     } else if (warp < C_FIRST_CONV) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C_REGS_SUM));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(c_regs_sum(HD)));
         // ── the output: a thread a query row ──
         const uint32_t row = tid - C_SOFT * 32, lanes = tmem + (((warp - C_SOFT) * 32) << 16);
         uint32_t g = 0;
@@ -735,7 +758,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         }
     } else if (warp < C_ISSUE) {
         // ── converters; first they cut the work ──
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C_REGS_CONV));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(c_regs_conv(HD)));
         const uint32_t ct = tid - C_FIRST_CONV * 32, cw = warp - C_FIRST_CONV;
         auto scan = [&](uint32_t x, uint32_t which, uint32_t* total) {  // sum of the threads in front
             uint32_t run = x;
@@ -874,8 +897,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         for (uint32_t turn = 0; turn < batches; ++turn) {
             const uint32_t pieces = sh.pieces;
             if (warp == C_ISSUE) {
-                // One warp issues both, batch after batch: it waits until its products are taken in, and products of the two in turn
-                // hold each other up (two issuers: 512 tokens behind 3584 201 us).
+                // one warp issues both, batch after batch
                 constexpr uint32_t idesc_s = umma_idesc_f16(KV_PAGE), idesc_o = umma_idesc_f16(HD) | 1u << 16;  // values MN-major
                 const uint64_t dk = umma_desc(k_base), dv = umma_desc_values(v_base);
                 // scores of page j in one accumulator, small products first; `begins`: of a piece's first, the queries are in place

@@ -344,3 +344,36 @@ def test_refusals():
     with pytest.raises(JoshuaB200Error):
         cache.attend(q[:3], lens, table, n_q=n_q, sinks=5)
     assert cache.attend_chunk(q[:0], lens, table, n_q=n_q, first=first).shape == (0, n_q * hd)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 90])
+@pytest.mark.parametrize("size", [2.0**8, 2.0**14, 2.0**20, 2.0**26])
+def test_scores_far_from_zero(kind, hd, window, size):
+    """Scores of up to many millions: what stands out by more than two scores' rounding takes all (products of 22 bits, sums of 23:
+    2^-20.4 of the magnitudes added up, which are below 4 times the largest score here: 2^-17.4), and every
+    output stays within the values."""
+    n_q, n_kv, counts, lens, sinks = 8, 2, [50, 1, 3, 200], [300, 200, 180, 200], 8 if window else 0
+    cache, table = make(kind, n_kv, hd, 4, 5)
+    held = fill(cache, table, lens, seed=2)
+    q = queries(sum(counts), n_q, hd, 5)
+    scale = size / np.sqrt(hd)
+    got = cache.attend_chunk(q, i32(lens), table, n_q=n_q, first=starts(counts), scale=scale, window=window, sinks=sinks).cpu().numpy()
+    got, x, row, clear = got.reshape(-1, n_q, hd), q.cpu().numpy().astype(np.float64).reshape(-1, n_q, hd), 0, 0
+    for n, length, (k, v) in zip(counts, lens, held):
+        k, v = (np.asarray(t, dtype=np.float64) for t in (k, v))
+        for r in range(n):
+            t = sees(length - n + r, window, sinks)
+            s = np.einsum("hgd,htd->hgt", x[row].reshape(n_kv, -1, hd), k[:, t]) * scale
+            for h in range(n_kv):
+                vv, out, top = v[h][t], got[row].reshape(n_kv, -1, hd)[h], np.abs(s[h]).max()
+                slack = TOL * np.abs(v).max()
+                assert np.isfinite(out).all() and (out >= vv.min(0) - slack).all() and (out <= vv.max(0) + slack).all()
+                for j in range(out.shape[0]):
+                    order = np.argsort(s[h, j])
+                    if len(t) == 1 or s[h, j][order[-1]] - s[h, j][order[-2]] > 2.0**-17 * top + 20:   # e^-20 of the rest
+                        assert np.abs(out[j] - vv[order[-1]]).max() <= slack, (row, h, j)
+                        clear += 1
+            row += 1
+    assert clear > (0 if size < 2.0**10 else sum(counts) * n_q // 2)
