@@ -9,6 +9,10 @@ come from a table (any scaling of `rope.rope_table`), the next tokens from `samp
     dec.share_prompt(prompt_ids)                 # or dec.prefill(ids, sequence=i) for each
     dec.sampling = dict(temperature=..., top_p=...)
     dec.uniform.uniform_(); dec.step()           # token by token
+    dec.extend({0: ids, 3: more}, scores=5)      # several sequences' next tokens in one pass, with their log probabilities
+
+With `attention_window` a token sees that many positions back and the first `attention_sinks`; pages that no later token sees go back to
+the pool as the sequences grow, and long prompts are read in parts.
 
 A step may be captured in a graph by the caller, its pages reserved and one step run on the stream before.  The graph keeps the
 sampling rule's tensors, the penalty and the number of shared pages as they were: capture another one when they change.  Replays move
@@ -24,7 +28,7 @@ from .kv_cache import PAGE, SCRATCH_ZEROED, PagedCache
 from .llama import LlamaDecoder
 from .moe_decoder import MoeDecoder
 from .rope import Rope, rope_table
-from .sampling import sample
+from .sampling import log_probs, sample
 
 
 def _same(a, b) -> bool:
@@ -35,10 +39,18 @@ def _same(a, b) -> bool:
 
 
 class _Paged:
+    attention_window = attention_sinks = 0
+    prompt_rows = 2048    # of a prompt in one pass, where there is a window
+    score_rows = 256      # whose logits are held at a time for their scores
+
     def __init__(self, cfg, device, batch: int = 1, max_ctx: int = 640, kv_type: str = "q8_0", n_pages: int | None = None,
-                 rope: Rope | None = None, **more):
+                 rope: Rope | None = None, attention_window: int = 0, attention_sinks: int = 0, **more):
         """`n_pages`: of the pool (default: enough for every sequence to reach max_ctx); `rope`: a table of max_ctx positions
-        (default: the model's theta, unscaled, half layout)."""
+        (default: the model's theta, unscaled, half layout); `attention_window`: positions that a token sees, its own the last of them
+        (0: all), besides the first `attention_sinks`."""
+        if attention_window < 0 or attention_sinks < 0 or attention_sinks and not attention_window:
+            raise JoshuaB200Error(_lib.E_INVALID, f"a window of {attention_window} with {attention_sinks} sinks")
+        self.attention_window, self.attention_sinks = attention_window, attention_sinks
         self.kv_type, self.pages_per_seq = kv_type, -(-max_ctx // PAGE)
         self.shared_pages = 0                     # leading pages that all sequences have in common
         # resting sequences still bring a row to every append: to a position each of pages behind the pool
@@ -55,7 +67,8 @@ class _Paged:
         self.idle_pos = torch.zeros(batch, dtype=torch.int32, device=self.dev)    # where a resting sequence's rows go
         self._seeds: dict[int, list] = {}         # recent ids given to a resting sequence
         self.free = list(range(self.n_pages))[::-1]
-        self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order
+        self.owned = [[] for _ in range(batch)]   # page ids of each sequence, in order; None: gone back, out of the window
+        self.kept_from = [0] * batch              # pages in front of it (but those of sinks) have gone back
         self.holders = [0] * self.n_pages         # sequences that have a page
         self.held = [0] * batch                   # positions each holds
         self._captured_by_caller = False          # then replays may have moved `pos` past `held`
@@ -69,7 +82,11 @@ class _Paged:
     def _attention_scratch(self) -> None:
         """One scratch for the attention of all layers; one that a caller's graph may hold stays until the decoder goes."""
         c, old = self.cfg, getattr(self, "att_scratch", [])
-        need = self.layers[0]["cache"].scratch_bytes(self.batch, c.q_heads, self.shared_pages)
+        cache = self.layers[0]["cache"]
+        if self.attention_window:
+            need = cache.scratch_bytes(self.batch, c.q_heads, rows=self.batch)
+        else:
+            need = cache.scratch_bytes(self.batch, c.q_heads, self.shared_pages)
         if not old or old[-1].numel() < need:
             size = max(need, 2 * old[-1].numel() if old else SCRATCH_ZEROED)   # all older ones together are smaller
             self.att_scratch = [*old, torch.zeros(size, dtype=torch.uint8, device=self.dev)]
@@ -102,12 +119,33 @@ class _Paged:
                 pages.append(self.free.pop())
                 mine.append(pages[-1])
                 self.holders[pages[-1]] = 1
-        if pages:   # one copy for all of them, from pinned memory: the host waits for nothing
+        self._enter(places, pages)
+
+    def _enter(self, places, pages) -> None:
+        """Page ids into the table: one copy for all of them, from pinned memory: the host waits for nothing."""
+        if pages:
             new = torch.tensor([places, pages], dtype=torch.int64, pin_memory=True).to(self.dev, non_blocking=True)
             self.table.view(-1).scatter_(0, new[0], new[1].int())
 
+    def _trim(self, sequences) -> None:
+        """Gives back the pages that no token from the sequences' next ones on sees."""
+        places, pages = [], []
+        for i in sequences if self.attention_window else ():
+            first = max(self.kept_from[i], -(-self.attention_sinks // PAGE))
+            behind = min((self.held[i] + 1 - self.attention_window) // PAGE, len(self.owned[i]))
+            for k in range(first, behind):
+                if self.owned[i][k] is not None:
+                    places.append(i * self.pages_per_seq + k)
+                    pages.append(self.owned[i][k])
+                    self.owned[i][k] = None
+            self.kept_from[i] = max(first, behind)
+        self._enter(places, [-1] * len(places))
+        self._give_back(pages)
+
     def _give_back(self, pages) -> None:
         for page in pages:
+            if page is None:
+                continue
             self.holders[page] -= 1
             if self.holders[page] == 0:
                 self.free.append(page)
@@ -116,7 +154,7 @@ class _Paged:
         """Ends a sequence: its pages go back (shared ones when the last sequence ends).  It rests until its next prompt, which
         begins at position 0."""
         self._give_back(self.owned[self._index(sequence)])
-        self.owned[sequence], self.held[sequence] = [], 0
+        self.owned[sequence], self.held[sequence], self.kept_from[sequence] = [], 0, 0
         self.table[sequence] = -1
         self.table[sequence, 0] = self.n_pages + sequence // self._places
         self.pos[sequence], self.active[sequence], self.idle_pos[sequence] = 0, 0, sequence % self._places
@@ -142,6 +180,7 @@ class _Paged:
         for mine in self.owned:
             self._give_back(mine)
         self.owned, self.held, self.resting = [[] for _ in self.owned], [0] * self.batch, [False] * self.batch
+        self.kept_from = [0] * self.batch
         self._seeds.clear()
         self.shared_pages = 0
         self.table.fill_(-1), self.active.fill_(1), self.idle_pos.zero_()
@@ -163,7 +202,7 @@ class _Paged:
     def share_prompt(self, token_ids) -> None:
         """Begins all sequences with one prompt, read once: its full pages are common to all, what is left of it (less than a
         page) is copied.  Every sequence samples its own next token."""
-        self._can_prompt()
+        self._can_prompt(dense=not self.attention_window)
         self._look()
         if any(self.held):
             raise JoshuaB200Error(_lib.E_INVALID, "sequences are under way: reset() first")
@@ -171,7 +210,7 @@ class _Paged:
         full, pages = n // PAGE, -(-n // PAGE)
         # what sequences have reserved stays theirs, but for the pages in whose place the common ones stand
         wanted = max(0, pages - len(self.owned[0])) + sum(max(0, pages - max(full, len(self.owned[i]))) for i in others)
-        back = sum(min(full, len(self.owned[i])) for i in others)
+        back = sum(page is not None for i in others for page in self.owned[i][:full])
         if wanted > len(self.free) + back:
             raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {len(self.free) + back} of {self.n_pages} are free")
         self._prompt(token_ids, 0)
@@ -179,8 +218,9 @@ class _Paged:
         for i in others:
             self._give_back(self.owned[i][:full])
             for page in common:
-                self.holders[page] += 1
-            self.owned[i] = common + self.owned[i][full:]
+                if page is not None:
+                    self.holders[page] += 1
+            self.owned[i], self.kept_from[i] = common + self.owned[i][full:], self.kept_from[0]
             self.table[i, :full] = self.table[0, :full]
         self._reserve({i: n for i in others})
         for i in others:
@@ -195,15 +235,95 @@ class _Paged:
         self.logits.copy_(self.logits[0:1].expand(self.batch, -1).clone())
         self._sample_rows(slice(0, self.batch))
 
-    def _can_prompt(self) -> None:
-        if self.cfg.head_dim not in (64, 128):
+    def extend(self, tokens: dict, scores: int | None = None):
+        """The next tokens of several sequences (ids by sequence), each from where it stands, in one pass; then self.logits, the sampled
+        next tokens (self.token) and positions of these sequences, as `prefill` leaves them.
+
+        With `scores` (a number of alternatives, at most 32): by sequence, what `sampling.log_probs` gives for its tokens but the first,
+        each at the position in front of it."""
+        new = {self._index(i): torch.as_tensor(ids, dtype=torch.int32).reshape(-1) for i, ids in sorted(tokens.items())}
+        if not new or any(ids.numel() == 0 for ids in new.values()):
+            raise JoshuaB200Error(_lib.E_INVALID, "nothing to extend, or an empty prompt")
+        if scores is not None and not 0 <= scores <= 32:
+            raise JoshuaB200Error(_lib.E_INVALID, f"{scores} alternatives: 0 to 32")
+        self._can_prompt(dense=False)
+        self._look()
+        self._trim(new)
+        x = self._pass(new)
+        counts = [ids.numel() for ids in new.values()]
+        given = self._scores(x, new, scores) if scores is not None else None
+        ends = torch.tensor(counts).cumsum(0)
+        seqs = torch.tensor(list(new), device=self.dev)
+        last = x[(ends - 1).to(self.dev)].contiguous()
+        self.logits[seqs] = self._head(last)
+        self.pos[seqs] = torch.tensor([self.held[i] - 1 for i in new], dtype=torch.int32, device=self.dev)
+        for i in new:
+            self._sample_rows(slice(i, i + 1))
+        return given
+
+    def _head(self, x):
+        logits = torch.empty(x.size(0), self.cfg.vocab, dtype=torch.float32, device=self.dev)
+        s = torch.cuda.current_stream(self.dev).cuda_stream
+        check(_lib.lib().jq_matmul_norm_dev(self.output._h, x.size(0), self.cfg.hidden, self.cfg.vocab, x.data_ptr(), self.out_norm.data_ptr(),
+                                            self.cfg.eps, None, logits.data_ptr(), s))
+        return logits
+
+    def _scores(self, x, new, top: int) -> dict:
+        """Log probabilities of every sequence's tokens behind its first one, some rows' logits at a time."""
+        out, row = {}, 0
+        for i, ids in new.items():
+            n = ids.numel()
+            ids, parts = ids.to(self.dev), []
+            for a in range(0, n - 1, self.score_rows):
+                b = min(n - 1, a + self.score_rows)
+                parts.append(log_probs(self._head(x[row + a:row + b]), ids[a + 1:b + 1], top=top))
+            if not parts:
+                parts.append(log_probs(self.logits[:0], ids[:0], top=top))
+            out[i] = tuple(torch.cat(p) for p in zip(*parts))
+            row += n
+        return out
+
+    def _pass(self, new: dict):
+        """New ids of some sequences (by sequence, in order) through all layers, over the cache: [rows, hidden]."""
+        L, c, P, i32 = _lib.lib(), self.cfg, lambda t: t.data_ptr(), dict(dtype=torch.int32, device=self.dev)
+        if not hasattr(self, "_layer_index"):   # the routed experts' decoder finds its layers by it
+            self._layer_index = {id(ly): k for k, ly in enumerate(self.layers)}
+        self._reserve({i: self.held[i] + ids.numel() for i, ids in new.items()})
+        for i in new:
+            self._wake(i)
+        counts = [new[i].numel() if i in new else 0 for i in range(self.batch)]
+        S, h, f32 = sum(counts), c.hidden, dict(dtype=torch.float32, device=self.dev)
+        s = torch.cuda.current_stream(self.dev).cuda_stream
+        ids = torch.cat(list(new.values())).to(self.dev)
+        pos = torch.cat([torch.arange(self.held[i], self.held[i] + n) for i, n in enumerate(counts)]).to(**i32)
+        seq = torch.repeat_interleave(torch.arange(self.batch), torch.tensor(counts)).to(**i32)
+        first = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], **i32)
+        lens = torch.tensor([self.held[i] + n for i, n in enumerate(counts)], **i32)
+        x, qkv, att = torch.empty(S, h, **f32), torch.empty(S, c.qkv_rows, **f32), torch.empty(S, c.q_heads * c.head_dim, **f32)
+        check(L.jq_embedding_dev(self.embed._h, P(ids), S, c.vocab, h, P(x), P(self.bad), s))
+        for ly in self.layers:
+            cache = ly["cache"]
+            check(L.jq_matmul_norm_dev(ly["wqkv"]._h, S, h, c.qkv_rows, P(x), P(ly["attn_norm"]), c.eps, None, P(qkv), s))
+            q = cache.append(qkv, pos, self.table, n_q=c.q_heads, seq=seq, rope=self.rope,
+                             q_norm=ly["q_norm"] if self.qk_norm else None, k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps)
+            cache.attend_chunk(q, lens, self.table, n_q=c.q_heads, first=first, window=self.attention_window, sinks=self.attention_sinks, out=att)
+            check(L.jq_matmul_norm_dev(ly["wo"]._h, S, c.q_heads * c.head_dim, h, P(att), None, 0.0, P(x), P(x), s))
+            self._ffn_prefill(ly, x, S, s)
+        for i, n in enumerate(counts):
+            self.held[i] += n
+        return x
+
+    def _can_prompt(self, dense: bool = True) -> None:
+        if dense and self.cfg.head_dim not in (64, 128):
             raise JoshuaB200Error(_lib.E_INVALID, "prompts need heads of 64 or 128")
         if getattr(self, "world", 1) > 1:
             raise JoshuaB200Error(_lib.E_INVALID, "prompts run on one GPU (the exchange windows are sized for decode batches)")
 
     def _prompt(self, token_ids, i) -> None:
         """Logits of the prompt's last token into self.logits[i]; self.pos[i] at that token."""
-        self._can_prompt()
+        self._can_prompt(dense=not self.attention_window)
+        if self.attention_window:
+            return self._prompt_in_parts(token_ids, i)
         L, c, P = _lib.lib(), self.cfg, lambda t: t.data_ptr()
         if not hasattr(self, "_layer_index"):   # the routed experts' decoder finds its layers by it
             self._layer_index = {id(ly): k for k, ly in enumerate(self.layers)}
@@ -237,6 +357,38 @@ class _Paged:
         self.held[i] = end
         self.pos[i] = end - 1
 
+    def _prompt_in_parts(self, token_ids, i) -> None:
+        """The same where there is a window: the dense attention of prompts has none."""
+        ids = torch.as_tensor(token_ids, dtype=torch.int32).reshape(-1)
+        if ids.numel() == 0:
+            raise JoshuaB200Error(_lib.E_INVALID, "an empty prompt")
+        self._look()
+        self._room_for_parts(i, ids.numel())
+        for part in ids.split(self.prompt_rows):
+            self._trim([i])
+            x = self._pass({i: part})
+        self.logits[i] = self._head(x[-1:].clone())[0]
+        self.pos[i] = self.held[i] - 1
+
+    def _room_for_parts(self, i, n: int) -> None:
+        """Raises, before any part is taken, if they do not fit: what each part takes and the window gives back."""
+        if self.held[i] + n > self.max_ctx:
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{self.held[i] + n} positions in a decoder of {self.max_ctx}")
+        mine = [page is not None and self.holders[page] == 1 for page in self.owned[i]]   # whether it goes back to the pool
+        free, held, sinks = len(self.free), self.held[i], -(-self.attention_sinks // PAGE)
+        at = max(self.kept_from[i], sinks)
+        while n:
+            behind = min((held + 1 - self.attention_window) // PAGE, len(mine))
+            if behind > at:
+                free, at = free + sum(mine[at:behind]), behind
+            part = min(n, self.prompt_rows)
+            held, n = held + part, n - part
+            more = max(0, -(-held // PAGE) - len(mine))
+            if more > free:
+                raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{more} pages wanted, {free} of {self.n_pages} are free")
+            free -= more
+            mine += [True] * more
+
     # ── a token of every sequence ───────────────────────────────────────
     def step(self, stream=None) -> None:
         """One token per sequence, as the dense decoder's step, on the current stream (`stream` is that one's handle or None)."""
@@ -252,6 +404,7 @@ class _Paged:
             self._captured_by_caller = True
             return
         self._look()
+        self._trim(i for i in range(self.batch) if not self.resting[i])
         self._reserve({i: n + 1 for i, n in enumerate(self.held) if not self.resting[i]})
         self.held = [n + (not rests) for n, rests in zip(self.held, self.resting)]
 
@@ -269,8 +422,12 @@ class _Paged:
         c, cache = self.cfg, ly["cache"]
         cache.append(self.qkv, self.pos, self.table, n_q=c.q_heads, rope=self.rope, q_norm=ly["q_norm"] if self.qk_norm else None,
                      k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps, out=self.q)
-        cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, shared_pages=self.shared_pages, out=self.attn,
-                     scratch=self.att_scratch[-1])
+        if self.attention_window:
+            cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, out=self.attn, scratch=self.att_scratch[-1],
+                         window=self.attention_window, sinks=self.attention_sinks)
+        else:
+            cache.attend(self.q, self.lens, self.table, n_q=c.q_heads, shared_pages=self.shared_pages, out=self.attn,
+                         scratch=self.att_scratch[-1])
 
     def _sample(self, s) -> None:
         self._sample_rows(slice(0, self.batch))

@@ -2,8 +2,11 @@
 sampler together.
 
     python -m joshua_b200.serve --batch 32 --prompt 2000 --tokens 64 --kv q8_0 [--layers 8] [--yarn 4] [--own-prompts]
+        [--window 1024 --sinks 4] [--logprobs 5]
 
-Prints what the cache takes and the time of a step; with --own-prompts every sequence reads the prompt for itself.
+Prints what the cache takes and the time of a step.  With --own-prompts every sequence reads the prompt for itself (all in one pass); with
+--window a token sees so many positions back, and the first --sinks; with --logprobs every sampled token's log probability comes with
+that many others, and the prompt's own is printed.
 """
 from __future__ import annotations
 
@@ -15,39 +18,50 @@ import torch
 from .llama import LlamaConfig
 from .paged import PagedLlamaDecoder
 from .rope import Rope, rope_table
+from .sampling import log_probs
 
 
-def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float = 1.0, own_prompts: bool = False, cfg=None) -> dict:
+def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float = 1.0, own_prompts: bool = False, cfg=None, window: int = 0,
+        sinks: int = 0, logprobs: int | None = None) -> dict:
     cfg = cfg or LlamaConfig(layers=layers)
     dev = torch.device("cuda", 0)
     max_ctx = prompt + tokens + 1
     scaled = dict(scaling="yarn", factor=yarn, orig_ctx=max(1, int(max_ctx / yarn))) if yarn > 1 else {}
     rope = Rope(rope_table(cfg.rope_theta, cfg.head_dim, max_ctx, dev, **scaled))
-    dec = PagedLlamaDecoder(cfg, dev, batch=batch, max_ctx=max_ctx, kv_type=kv, rope=rope)
+    dec = PagedLlamaDecoder(cfg, dev, batch=batch, max_ctx=max_ctx, kv_type=kv, rope=rope, attention_window=window,
+                            attention_sinks=sinks)
     gen = torch.Generator(device=dev).manual_seed(1)
     ids = torch.randint(0, cfg.vocab, (prompt,), generator=torch.Generator().manual_seed(2)).tolist()
     dec.sampling = dict(temperature=torch.full((batch,), 0.8, device=dev), top_p=torch.full((batch,), 0.95, device=dev),
                         top_k=torch.full((batch,), 100, dtype=torch.int32, device=dev))
     dec.uniform.uniform_(generator=gen)
+    scores = None
     if own_prompts:
-        for i in range(batch):
-            dec.prefill(ids, sequence=i)
+        scores = dec.extend({i: ids for i in range(batch)}, scores=logprobs)
     else:
         dec.share_prompt(ids)
-    for i in range(batch):
-        dec.reserve(i, max_ctx)
-    out, steps = [dec.token.clone()], []
+    if not window:   # steps take a page now and then otherwise, and give one back
+        for i in range(batch):
+            dec.reserve(i, max_ctx)
+
+    def score():
+        return log_probs(dec.logits, dec.token, top=logprobs)[0].clone() if logprobs is not None else None
+
+    out, given, steps = [dec.token.clone()], [score()], []
     for _ in range(tokens - 1):
         dec.uniform.uniform_(generator=gen)
         torch.cuda.synchronize()
         t = time.perf_counter()
         dec.step()
+        given.append(score())
         torch.cuda.synchronize()
         steps.append(time.perf_counter() - t)
         out.append(dec.token.clone())
     dec.check_flags()
     used = dec.n_pages - len(dec.free)
     return {"tokens": torch.stack(out, 1).cpu(), "ms_per_step": 1e3 * sorted(steps)[len(steps) // 2] if steps else 0.0,
+            "log_probs": torch.stack(given, 1).cpu() if logprobs is not None else None,
+            "prompt_log_prob": float(scores[0][0].mean()) if scores else None,
             "pages_used": used, "cache_mib": used * dec.layers[0]["cache"].page_bytes * cfg.layers / 2**20}
 
 
@@ -60,10 +74,16 @@ def main() -> None:
     ap.add_argument("--layers", type=int, default=8)
     ap.add_argument("--yarn", type=float, default=1.0, help="stretch the positions by this factor")
     ap.add_argument("--own-prompts", action="store_true")
+    ap.add_argument("--window", type=int, default=0, help="positions that a token sees (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="first positions that stay visible behind the window")
+    ap.add_argument("--logprobs", type=int, default=None, help="log probabilities of the tokens, with so many others")
     a = ap.parse_args()
-    r = run(a.batch, a.prompt, a.tokens, a.kv, a.layers, a.yarn, a.own_prompts)
+    r = run(a.batch, a.prompt, a.tokens, a.kv, a.layers, a.yarn, a.own_prompts, window=a.window, sinks=a.sinks, logprobs=a.logprobs)
     print(f"{a.batch} sequences behind {a.prompt} tokens, {a.kv} cache: {r['pages_used']} pages, {r['cache_mib']:.0f} MiB; "
           f"{r['ms_per_step']:.2f} ms a step, {1e3 * a.batch / max(r['ms_per_step'], 1e-9):.0f} tokens/s")
+    if r["log_probs"] is not None:
+        print(f"mean log probability of a sampled token {float(r['log_probs'].mean()):.3f}"
+              + (f", of the prompt's {r['prompt_log_prob']:.3f}" if r["prompt_log_prob"] is not None else ""))
 
 
 if __name__ == "__main__":
