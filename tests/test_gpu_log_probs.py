@@ -186,3 +186,20 @@ def test_refusals():
     refused(_lib.E_TOO_LARGE, l, t, top=33), refused(_lib.E_INVALID, l[:, :0], t)
     out = log_probs(l[:0], t[:0], top=3)
     assert [list(o.shape) for o in out] == [[0], [0], [0, 3], [0, 3]]
+
+
+@pytest.mark.parametrize("rows,vocab,pad,top", [(1300, 2047, 3, 3), (1201, 2049, 2, 0), (610, 4098, 1, 32), (150, 40001, 5, 20), (75, 9000, 4, 7), (37, 70003, 0, 32)])
+def test_rows_in_turn(rows, vocab, pad, top):
+    """More rows than are worked on at a time, and rows in several slices, at all distances from a 16-byte boundary."""
+    wide = normal(rows, vocab + pad, 7)
+    check(wide[:, pad:], tokens(rows, vocab, 8), top)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 700])
+def test_rising_rows(rows):
+    """Every value above all before it: each list is cut back again and again."""
+    import torch
+
+    l = torch.linspace(-4, 4, 9001, device="cuda").repeat(rows, 1)
+    l[::2] = l[::2].flip(1)
+    check(l, tokens(rows, 9001, 3), 32)
