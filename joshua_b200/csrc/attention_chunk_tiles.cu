@@ -1,7 +1,7 @@
 // Attention of chunks of new tokens over the quantised cache on the 5th-generation tensor cores.
 //
 // A tile is up to 128 query rows: the heads of a kv head of consecutive tokens of a sequence, token by token.  It goes over the pages
-// that some of its tokens sees, a page at a time, running maximum and sum in f32.  Terms as in attention_lead.cu: queries two f16 terms
+// that some of its tokens see, a page at a time, running maximum and sum in f32.  Terms as in attention_lead.cu: queries two f16 terms
 // under a power of two of their row; codes times scales as two f16 terms (halves: one) under powers of two of a page's largest scale;
 // probabilities two terms; of a product of two terms each the smallest of the four is left out.  Accumulators hold a score or one page
 // of the output; the running output lives in registers.  Scores of positions that a row does not see become nothing
@@ -12,8 +12,15 @@
 // pages.  It is cut into equal pieces, one a CTA; pieces of a tile that several CTAs have are joined by the last of them to arrive, in order.
 //
 // Warps: 0 .. 3 softmax, a thread a query row; 4 .. 7 add up the output, the same; 8 .. 15 first cut the work, then turn the pages' codes
-// into swizzled tiles, two stages (half of them keys, half values); 16 issues the products; 17 copies the pages.  Tensor memory: the query's terms (the A operand of the scores), scores and probabilities
-// (A of the output) of two pages, output of one.
+// into swizzled tiles, two stages (half of them keys, half values); 16 issues the products; 17 copies the pages.  Tensor memory: the
+// query's terms (the A operand of the scores), scores and probabilities (A of the output) of two pages, output of one: scores of a page
+// are under way while the softmax has the one before and the output the one before that.
+//
+// What bounds it: three products of f16 terms a page and tile, 1.14 us at the rate of a library product.  512 tokens behind 3584, 32 heads on
+// 8 of 128, eight bits: 99 us, 59 of them products (the tensor pipe 42% of the time, half of the issue slots, 930 W); 4096 behind 8192
+// 1.74 to 1.78 ms, 1.26 of them (985 W, the power limit: 84% of the rate that a library product has under it); four tokens of 32
+// sequences 116 us, 1.1 us a page, for tiles of 16 rows take the products of 128; four prompts of 500, heads of 64 in halves 48 us, half of
+// it the tiles' beginnings and ends.
 //
 // Every wait on an mbarrier is bounded.  A warp whose wait ran out waits for none any more, hands nothing on, and goes through the
 // rest of its work so, which brings it to every barrier that others expect it at; the status flag is raised and the rows become NaN.
