@@ -454,7 +454,7 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
  * i, which has len[i] with them.  The row at position p sees positions 0 .. p; with a window (0: none) the last `window` of them
  * and the first `sinks`.  Page table entries of pages that no row of the sequence sees are not followed.  Rows that belong to no
  * sequence are left as they were; a sequence without rows is not looked at.  len[i] = 0: zeros.
- *   q, out, scale, scratch, and the precision: as for jq_attention_paged_dev.  A row does not depend on positions that it does not
+ *   q, out, scale, scratch, and the precision: as for jq_attention_paged_dev; q and out must not overlap.  A row does not depend on positions that it does not
  * see, whatever they hold, but for the rounding of scales below 2^-21 (4 bits: 2^-25) of the largest of their page, positions behind
  * the sequence's last left out.
  *   A len out of range (negative, above the page table, or fewer than the sequence's rows) or a page id outside the cache that a

@@ -42,6 +42,14 @@ int32_t check_heads(const char* who, const jq_kv_cache* c, uint32_t n_q) {
     if (n_q != 0 && n_q % c->n_kv == 0 && n_q <= 4096) return jq::OK;
     return bad(who, std::to_string(n_q) + " query heads on " + std::to_string(c->n_kv) + " kv heads");
 }
+// whether rows of `width` floats share any: a's and b's, `rows` of each
+bool rows_meet(const float* a, uint64_t a_stride, const float* b, uint64_t b_stride, uint32_t rows, uint64_t width) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a) / 4, y = reinterpret_cast<uintptr_t>(b) / 4;
+    if (x + (rows - 1) * a_stride + width <= y || y + (rows - 1) * b_stride + width <= x) return false;
+    if (rows == 1 || a_stride != b_stride) return true;  // side by side only as columns of one buffer
+    const uint64_t ahead = x <= y ? (y - x) % a_stride : (a_stride - (x - y) % a_stride) % a_stride;
+    return ahead < width || ahead > a_stride - width;
+}
 
 }  // namespace
 
@@ -207,6 +215,7 @@ int32_t jq_attention_chunk_dev(const jq_kv_cache* cache, const float* q, uint64_
     const uint64_t width = (uint64_t)n_q * cache->head_dim;
     if (q_stride < width || out_stride < width || q_stride % 4 || out_stride % 4 || unaligned(q, out, scratch))
         return bad(who, "rows of n_q * head_dim floats must not overlap; 16-byte boundaries");
+    if (rows_meet(q, q_stride, out, out_stride, rows, width)) return bad(who, "q and out must not overlap");
     if (scale == 0.0f) scale = 1.0f / std::sqrt((float)cache->head_dim);
     const uint32_t most = table_stride * JQ_KV_PAGE;
     if (window >= most) window = 0;

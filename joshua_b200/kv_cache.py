@@ -190,7 +190,7 @@ class PagedCache:
         """Attention of some new tokens of every sequence, [rows, n_q * head_dim], whose keys and values are in the cache: rows
         `first[i]` .. `first[i + 1]` - 1 (int32 [sequences + 1]; None: as many of each) are the last positions of sequence i, which has
         `lens[i]` with them.  A row sees the positions up to its own; with a `window` (0: none) the last so many and the first
-        `sinks`.  Rows of no sequence are left as they were in `out`.  `scratch`: from `scratch(rows=)`; by default as for `attend`."""
+        `sinks`.  Rows of no sequence are left as they were in `out`, which must not overlap `q`.  `scratch`: from `scratch(rows=)`; by default as for `attend`."""
         index, width = self._index, n_q * self.head_dim
         if index != _device():
             with torch.cuda.device(index):

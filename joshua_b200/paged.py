@@ -247,6 +247,9 @@ class _Paged:
         if scores is not None and not 0 <= scores <= 32:
             raise JoshuaB200Error(_lib.E_INVALID, f"{scores} alternatives: 0 to 32")
         self._can_prompt(dense=False)
+        rows = sum(ids.numel() for ids in new.values())
+        if rows > 65536 or rows * self.cfg.q_heads > 2**27 or rows * (4 * self.pages_per_seq + 8) >= 2**32:
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{rows} tokens in one pass")
         self._look()
         self._trim(new)
         x = self._pass(new)

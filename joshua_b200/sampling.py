@@ -63,8 +63,10 @@ def log_probs(logits: torch.Tensor, token: torch.Tensor, top: int = 0):
     if index != _device():
         with torch.cuda.device(index):
             return log_probs(logits, token, top)
-    if logits.dim() != 2 or not 0 <= top < 2**31:
+    if logits.dim() != 2 or top < 0:
         raise JoshuaB200Error(_lib.E_INVALID, "logits must be [rows, vocab], top not negative")
+    if top > 32:
+        raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{top} likeliest tokens of a row: 32 at most")
     vocab, device = logits.size(1), logits.device
     at, stride, rows = rows_arg(logits, "logits", vocab, index)
     given = vector_arg(token, "token", rows, i32, index)

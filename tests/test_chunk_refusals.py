@@ -11,6 +11,9 @@ from tests.test_serving_refusals import A, COMMON, cache, call, refused
 current = test_serving_devices.current
 
 
+B = A + (1 << 20)   # where the results would go: never looked at, as A
+
+
 def test_chunk_scratch():
     f = _lib.lib().jq_attention_chunk_scratch_bytes
     assert f(0, 8, 8, 2, 128) == f(4097, 8, 8, 2, 128) == f(1, 0, 8, 2, 128) == f(1, 65537, 8, 2, 128) == f(1, 8, 8, 0, 128) == f(1, 8, 9, 2, 128) == 0
@@ -19,7 +22,7 @@ def test_chunk_scratch():
 
 
 def test_chunks():
-    ok = dict(cache=cache(), q=A, q_stride=512, first=A, len=A, table=A, n_seq=2, per=3, rows=5, n_q=4, scale=0.0, window=0, sinks=0, out=A,
+    ok = dict(cache=cache(), q=A, q_stride=512, first=A, len=A, table=A, n_seq=2, per=3, rows=5, n_q=4, scale=0.0, window=0, sinks=0, out=B,
               out_stride=512, scratch=A, bad=None, stream=None)
     for nothing in (dict(n_seq=0), dict(rows=0)):
         assert call("jq_attention_chunk_dev", ok, nothing) == _lib.OK
@@ -27,7 +30,9 @@ def test_chunks():
             (dict(n_q=6, cache=cache(n_kv=4)), "query heads"), (dict(q=None), "NULL"), (dict(len=None), "NULL"), (dict(out=None), "NULL"),
             (dict(scratch=None), "NULL"), (dict(first=None), "equal parts"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
             (dict(q_stride=511), "rows"), (dict(out_stride=514), "rows"), (dict(q=A + 4), "boundaries"), (dict(scratch=A + 8), "boundaries"),
-            (dict(n_seq=4096, per=1 << 20), "2^28")]:
+            (dict(n_seq=4096, per=1 << 20), "2^28"), (dict(out=A), "overlap"), (dict(out=A + 4 * 512 * 4), "overlap"), (dict(q=A + 4 * 512 * 5 - 16, out=A), "overlap"),
+            (dict(q_stride=1536, out_stride=1536, out=A + 496 * 4), "overlap"), (dict(q_stride=1536, out_stride=1536, out=A + 1040 * 4), "overlap"),
+            (dict(q_stride=1536, out_stride=1536, q=A + 1024 * 4, out=A + 528 * 4), "overlap"), (dict(q_stride=1536, out=A + 1024 * 4), "overlap")]:
         refused(call("jq_attention_chunk_dev", ok, change), "jq_attention_chunk_dev", word)
     for change, word in ((dict(n_seq=4097), "JQ_ATTENTION_MAX_BATCH"), (dict(rows=65537), "JQ_ATTENTION_MAX_ROWS"),
                          (dict(rows=65536, n_q=4096, q_stride=1 << 20, out_stride=1 << 20), "too many"), (dict(rows=65536, per=1 << 14), "too many")):

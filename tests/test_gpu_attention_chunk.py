@@ -377,3 +377,43 @@ def test_scores_far_from_zero(kind, hd, window, size):
                         clear += 1
             row += 1
     assert clear > (0 if size < 2.0**10 else sum(counts) * n_q // 2)
+
+
+def test_columns_of_one_buffer():
+    """Queries and results beside each other in wider rows; in the same place they are refused."""
+    import torch
+
+    from joshua_b200._lib import JoshuaB200Error
+
+    n_q, n_kv, hd, counts, lens = 8, 2, 64, [20, 1, 5], [100, 64, 65]
+    cache, table = make("q8_0", n_kv, hd, 3, 3)
+    fill(cache, table, lens, seed=1)
+    q = queries(sum(counts), n_q, hd, 4)
+    want = cache.attend_chunk(q, i32(lens), table, n_q=n_q, first=starts(counts))
+    for at, to in ((0, 512), (516, 0), (0, 600)):
+        wide = torch.full((26, 1112), 7.0, device="cuda")
+        wide[:, at:at + 512] = q
+        got = wide[:, to:to + 512]
+        cache.attend_chunk(wide[:, at:at + 512], i32(lens), table, n_q=n_q, first=starts(counts), out=got)
+        assert bool((got == want).all()) and bool((wide[:, at:at + 512] == q).all())
+        beside = torch.ones(1112, dtype=torch.bool)
+        beside[at:at + 512] = beside[to:to + 512] = False
+        assert bool((wide[:, beside.cuda()] == 7.0).all())
+        for step in (0, 256, -256):
+            if 0 <= at + step <= 600:
+                with pytest.raises(JoshuaB200Error):
+                    cache.attend_chunk(wide[:, at:at + 512], i32(lens), table, n_q=n_q, first=starts(counts), out=wide[:, at + step:at + step + 512])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n_q,hd", [(160, 64), (256, 128), (129, 128)])
+def test_many_heads_on_one(kind, n_q, hd):
+    """More query heads on a kv head than a tile has rows; tables that are full to the last position."""
+    counts, lens = [3, 40, 1], [130, 320, 320]
+    cache, table = make(kind, 1, hd, 3, 5)
+    kv = fill(cache, table, lens, seed=3)
+    q = queries(sum(counts), n_q, hd, 4)
+    for window, sinks in ((0, 0), (70, 3)):
+        got = cache.attend_chunk(q, i32(lens), table, n_q=n_q, first=starts(counts), window=window, sinks=sinks)
+        compare(got, q, kv, counts, lens, n_q, hd, window, sinks)
+    cache.check_flags()
