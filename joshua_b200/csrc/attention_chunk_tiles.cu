@@ -309,6 +309,13 @@ struct ChunkConverter {
     }
 };
 
+// Rows of a tile: `heads` (up to 128) places a token.  A division a row and piece took more time than the row's loads.
+struct TileRows {
+    uint32_t heads, inverse;
+    __device__ __forceinline__ explicit TileRows(const PagedArgs& a) : heads(min(a.group, CQ)), inverse((65536 + heads - 1) / heads) {}
+    __device__ __forceinline__ uint32_t token(uint32_t row) const { return row * inverse >> 16; }  // exact: row and heads are below 2^8
+};
+
 // Values: 64 dimensions along a row of 128 bytes, keys from row to row; 8 keys 1024 bytes apart, the next 64 dimensions a page of rows on.
 __device__ __forceinline__ uint64_t umma_desc_values(uint32_t smem_addr) {
     return umma_desc(smem_addr) - ((uint64_t)1 << 16) + ((uint64_t)(KV_PAGE * 128 >> 4) << 16);
@@ -427,10 +434,10 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         float rf = 0.0f;  // inverse scale of the query row, times log2(e) and the softmax scale
         // Rows come 16 dimensions of 8 rows a load, four lanes a row (a row a lane asks the cache for 32 lines a load: 128 rows of 128
         // took 4 us), and go to their lanes through the stage.
-        const uint32_t heads = min(a.group, CQ);
+        const TileRows rows(a);
         auto rows_of = [&](const ChunkPiece& p, uint32_t i) -> const float4* {  // of row 8 i + lane / 4 of the warp, its lane % 4-th vector
-            const uint32_t r = warp * 32 + 8 * i + lane / 4, t = r / heads, h = r % heads;
-            if (t >= p.tokens || (p.head0 + h) / a.group != p.kvh) return nullptr;
+            const uint32_t r = warp * 32 + 8 * i + lane / 4, t = rows.token(r), h = r - t * rows.heads;
+            if (t >= p.tokens || p.head0 + h >= (p.kvh + 1) * a.group) return nullptr;
             return reinterpret_cast<const float4*>(a.q + (uint64_t)(p.row0 + t) * a.q_stride + (uint64_t)(p.head0 + h) * HD) + lane % 4;
         };
         auto load = [](const float4* from, uint32_t at) { return from ? from[at] : make_float4(0.0f, 0.0f, 0.0f, 0.0f); };
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 query(p, amax);
                 if (k + 1 < pieces) amax = largest(sh.piece[k + 1]);
                 const uint32_t n = p.end - p.first;
-                const Sight see(a.span, p.pos0 + row / heads), last_see(a.span, p.pos0 + p.tokens - 1);
+                const Sight see(a.span, p.pos0 + rows.token(row)), last_see(a.span, p.pos0 + p.tokens - 1);
                 mx = -INFINITY, sums = 0;
                 for (uint32_t j = 0; j < n; ++j, ++g) {
                     const uint32_t u = p.first + j, base = (u < p.sinks ? u : u + p.skip) * KV_PAGE;
@@ -617,7 +624,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             const uint32_t pieces = sh.pieces;
             for (uint32_t k = 0; k < pieces; ++k) {
                 const ChunkPiece& p = sh.piece[k];
-                const uint32_t heads = min(a.group, CQ), t = row / heads, n = p.end - p.first;
+                const uint32_t n = p.end - p.first;
                 uint32_t odd_first = 0xFFFFFFFFu, odd_end = 0;
                 bool lost = false;
 #pragma unroll
@@ -649,6 +656,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                         if (lane == 0) mbar_arrive(&sh.o_go[(g + 1) & 1]);
                     }
                 }
+                const TileRows rows(a);  // here: the loop has no register left
+                const uint32_t t = rows.token(row);
                 const float mx = sh.stat[(g - 1) & 3][0][row];
                 float sum = sh.stat[(g - 1) & 3][1][row];
                 tc_fence_before();
@@ -657,7 +666,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 if (!ok || lost) sum = NAN;
                 if (lost && row == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
                 const Sight see(a.span, p.pos0 + t);
-                const bool live = t < p.tokens && (p.head0 + row % heads) / a.group == p.kvh;
+                const bool live = t < p.tokens && p.head0 + row - t * rows.heads < (p.kvh + 1) * a.group;
                 // Values that are not finite stood as zeros in the products: they go where a row sees them, and nowhere else; at(d): where
                 // this row's dimension d stands.
                 auto add_odd = [&](auto at) {
@@ -689,8 +698,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                     float4* to[4];
 #pragma unroll
                     for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t r = (warp - C_SOFT) * 32 + 8 * i + lane / 4, tok = r / heads, h = r % heads;
-                        to[i] = tok < p.tokens && (p.head0 + h) / a.group == p.kvh
+                        const uint32_t r = (warp - C_SOFT) * 32 + 8 * i + lane / 4, tok = rows.token(r), h = r - tok * rows.heads;
+                        to[i] = tok < p.tokens && p.head0 + h < (p.kvh + 1) * a.group
                                     ? reinterpret_cast<float4*>(a.out + (uint64_t)(p.row0 + tok) * a.out_stride + (uint64_t)(p.head0 + h) * HD) + lane % 4
                                     : nullptr;
                     }
@@ -711,7 +720,7 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
                 if (p.parts == 1) {
                     store(sum);
                     if (odd_end != 0) {
-                        float* out = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row % heads) * HD;
+                        float* out = a.out + (uint64_t)(p.row0 + t) * a.out_stride + (uint64_t)(p.head0 + row - t * rows.heads) * HD;
                         add_odd([&](uint32_t d) { return out + d; });
                     }
                 } else {
