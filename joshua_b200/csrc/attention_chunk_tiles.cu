@@ -19,8 +19,8 @@
 // What bounds it: three products of f16 terms a page and tile, 1.14 us at the rate of a library product.  512 tokens behind 3584, 32 heads on
 // 8 of 128, eight bits: 99 us, 59 of them products (the tensor pipe 42% of the time, half of the issue slots, 930 W); 4096 behind 8192
 // 1.74 to 1.78 ms, 1.26 of them (985 W, the power limit: 84% of the rate that a library product has under it); four tokens of 32
-// sequences 116 us, 1.1 us a page, for tiles of 16 rows take the products of 128; four prompts of 500, heads of 64 in halves 48 us, half of
-// it the tiles' beginnings and ends.
+// sequences 116 us, 1.1 us a page, for tiles of 16 rows take the products of 128; four prompts of 500, heads of 64 in halves 45 us, half of
+// it the tiles' beginnings and ends (with divisions for the rows' tokens 47.7).
 //
 // Every wait on an mbarrier is bounded.  A warp whose wait ran out waits for none any more, hands nothing on, and goes through the
 // rest of its work so, which brings it to every barrier that others expect it at; the status flag is raised and the rows become NaN.
@@ -309,7 +309,7 @@ struct ChunkConverter {
     }
 };
 
-// Rows of a tile: `heads` (up to 128) places a token.  A division a row and piece took more time than the row's loads.
+// Rows of a tile: `heads` (up to 128) places a token.
 struct TileRows {
     uint32_t heads, inverse;
     __device__ __forceinline__ explicit TileRows(const PagedArgs& a) : heads(min(a.group, CQ)), inverse((65536 + heads - 1) / heads) {}
