@@ -4,9 +4,9 @@ sampler together.
     python -m joshua_b200.serve --batch 32 --prompt 2000 --tokens 64 --kv q8_0 [--layers 8] [--yarn 4] [--own-prompts]
         [--window 1024 --sinks 4] [--logprobs 5]
 
-Prints what the cache takes and the time of a step.  With --own-prompts every sequence reads the prompt for itself (all in one pass); with
---window a token sees so many positions back, and the first --sinks; with --logprobs every sampled token's log probability comes with
-that many others, and the prompt's own is printed.
+Prints what the cache takes and the time of a step.  With --own-prompts every sequence reads the prompt for itself; with --window a token
+sees so many positions back, and the first --sinks; with --logprobs every sampled token's log probability comes with that many others, and
+prompts of the sequences' own go through the model several at a time, their log probabilities printed.
 """
 from __future__ import annotations
 
@@ -19,6 +19,8 @@ from .llama import LlamaConfig
 from .paged import PagedLlamaDecoder
 from .rope import Rope, rope_table
 from .sampling import log_probs
+
+PASS_ROWS = 16384   # prompt tokens of several sequences in one pass
 
 
 def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float = 1.0, own_prompts: bool = False, cfg=None, window: int = 0,
@@ -35,9 +37,14 @@ def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float 
     dec.sampling = dict(temperature=torch.full((batch,), 0.8, device=dev), top_p=torch.full((batch,), 0.95, device=dev),
                         top_k=torch.full((batch,), 100, dtype=torch.int32, device=dev))
     dec.uniform.uniform_(generator=gen)
-    scores = None
-    if own_prompts:
-        scores = dec.extend({i: ids for i in range(batch)}, scores=logprobs)
+    scores = {}
+    if own_prompts and logprobs is None:
+        for i in range(batch):
+            dec.prefill(ids, sequence=i)
+    elif own_prompts:
+        some = max(1, PASS_ROWS // prompt)
+        for i in range(0, batch, some):
+            scores.update(dec.extend({k: ids for k in range(i, min(batch, i + some))}, scores=logprobs))
     else:
         dec.share_prompt(ids)
     if not window:   # steps take a page now and then otherwise, and give one back
