@@ -417,3 +417,38 @@ def test_many_heads_on_one(kind, n_q, hd):
         got = cache.attend_chunk(q, i32(lens), table, n_q=n_q, first=starts(counts), window=window, sinks=sinks)
         compare(got, q, kv, counts, lens, n_q, hd, window, sinks)
     cache.check_flags()
+
+
+def test_pages_behind_four_gigabytes():
+    import torch
+
+    from joshua_b200.kv_cache import PagedCache
+
+    n_q, n_kv, hd, per, counts, lens = 8, 4, 128, 9, [70, 2, 1], [500, 500, 576]
+    n_pages = 2**32 // (n_kv * 2 * 64 * (hd + hd // 16)) + 3 * per
+    cache = PagedCache("q8_0", n_kv, hd, n_pages=n_pages, device="cuda")
+    assert (n_pages - 3 * per + 1) * cache.page_bytes > 2**32
+    table = torch.arange(n_pages - 3 * per, n_pages, device="cuda").int().flip(0).reshape(3, per).contiguous()
+    kv = fill(cache, table, lens, seed=5)
+    q = queries(sum(counts), n_q, hd, 6)
+    for window, sinks in ((0, 0), (100, 4)):
+        compare(cache.attend_chunk(q, i32(lens), table, n_q=n_q, first=starts(counts), window=window, sinks=sinks), q, kv, counts, lens, n_q, hd, window,
+                sinks)
+    cache.check_flags()
+
+
+def test_wide_rows():
+    """Queries and results whose last rows begin behind 2^32 bytes."""
+    import torch
+
+    n_q, n_kv, hd, counts, lens = 8, 2, 128, [60, 3, 1], [200, 130, 64]
+    cache, table = make("f16", n_kv, hd, 3, 4)
+    kv = fill(cache, table, lens, seed=5)
+    q = queries(sum(counts), n_q, hd, 6)
+    stride = 2**24 + 2**20 + 4
+    far = torch.empty(63 * stride + 2 * 1024, device="cuda")
+    rows = torch.as_strided(far, (64, 1024), (stride, 1))
+    out = torch.as_strided(far, (64, 1024), (stride, 1), 1024)
+    rows.copy_(q)
+    assert cache.attend_chunk(rows, i32(lens), table, n_q=n_q, first=starts(counts), out=out) is out
+    compare(out.contiguous(), q, kv, counts, lens, n_q, hd)

@@ -203,3 +203,21 @@ def test_rising_rows(rows):
     l = torch.linspace(-4, 4, 9001, device="cuda").repeat(rows, 1)
     l[::2] = l[::2].flip(1)
     check(l, tokens(rows, 9001, 3), 32)
+
+
+def test_logits_behind_four_gigabytes():
+    """Rows a long way apart, a plain call on a head's width at the end of them."""
+    import torch
+
+    from joshua_b200.sampling import log_probs
+
+    rows, vocab, stride = 70, 9001, 2**24 + 1
+    far = torch.empty((rows - 1) * stride + vocab, device="cuda")
+    l = torch.as_strided(far, (rows, vocab), (stride, 1))
+    plain_ones = normal(rows, vocab, 4)
+    l.copy_(plain_ones)
+    token = tokens(rows, vocab, 5)
+    got = log_probs(l, token, top=5)
+    check(plain_ones, token, 5)
+    for a, b in zip(got, log_probs(plain_ones, token, top=5)):
+        assert a.shape == b.shape and bool(((a - b).abs() <= (0 if a.dtype == torch.int32 else 2 * TOL)).all())
