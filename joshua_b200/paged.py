@@ -10,6 +10,7 @@ come from a table (any scaling of `rope.rope_table`), the next tokens from `samp
     dec.sampling = dict(temperature=..., top_p=...)
     dec.uniform.uniform_(); dec.step()           # token by token
     dec.extend({0: ids, 3: more}, scores=5)      # several sequences' next tokens in one pass, with their log probabilities
+    dec.rewind(3, positions)                     # without the last of them
 
 With `attention_window` a token sees that many positions back and the first `attention_sinks`; pages that no later token sees go back to
 the pool as the sequences grow, and long prompts are read in parts.
@@ -263,6 +264,24 @@ class _Paged:
         for i in new:
             self._sample_rows(slice(i, i + 1))
         return given
+
+    def rewind(self, sequence: int, positions: int) -> None:
+        """Forgets a sequence's tokens behind its first `positions`, drafts that were not taken: its next ones go there (`extend`, or
+        `step` with self.token[sequence] set).  Not into pages that it has in common with others, nor to where its window has given
+        back what it would see."""
+        self._look()
+        i, n = self._index(sequence), positions
+        if not 0 < n <= self.held[i]:
+            raise JoshuaB200Error(_lib.E_INVALID, f"{n} of {self.held[i]} positions")
+        if n == self.held[i]:
+            return
+        mine, window = self.owned[i], self.attention_window
+        if n < self.shared_pages * PAGE or any(page is not None and self.holders[page] > 1 for page in mine[n // PAGE:]):
+            raise JoshuaB200Error(_lib.E_INVALID, f"{n} positions end in front of pages that sequences share")
+        if window and any(page is None for page in mine[max(0, n + 1 - window) // PAGE:]):
+            raise JoshuaB200Error(_lib.E_INVALID, f"pages in front of position {n} have gone back")
+        self.held[i] = n
+        self.pos[i] = n
 
     def _head(self, x):
         logits = torch.empty(x.size(0), self.cfg.vocab, dtype=torch.float32, device=self.dev)

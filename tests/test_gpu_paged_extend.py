@@ -216,6 +216,52 @@ def test_routed_experts():
     near(a.logits, b.logits, tol=2.0**-6)   # batches of other sizes round differently, and experts in a near tie may change places
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_drafts_that_are_not_taken(window, sinks):
+    a, b = (make(2, "f16", attention_window=window, attention_sinks=sinks) for _ in range(2))
+    for dec in (a, b):
+        dec.extend({0: ids(100, 1), 1: ids(61, 2)})
+    scores = a.extend({0: ids(6, 3), 1: ids(4, 4)}, scores=1)   # the second sequence's pass a page's end
+    assert scores[0][0].shape == (5,) and a.pos.tolist() == [106, 65]
+    a.rewind(0, 102), a.rewind(1, 62)
+    assert a.pos.tolist() == a.held == [102, 62]
+    b.extend({0: ids(6, 3)[:2], 1: ids(4, 4)[:1]})
+    for dec in (a, b):
+        dec.extend({0: ids(3, 5), 1: ids(70, 6)})
+    near(a.logits, b.logits)
+    assert a.pos.tolist() == b.pos.tolist() == [105, 132]
+    a.rewind(0, 104)
+    a.token[0] = ids(3, 5)[2]
+    b.token.copy_(a.token)
+    a.rewind(1, 131), b.rewind(1, 131)
+    a.step()                       # the same token again, by a step
+    b.rewind(0, 104), b.step()
+    near(a.logits, b.logits)
+    a.check_flags(), b.check_flags()
+
+
+def test_where_there_is_no_way_back():
+    dec = make(3)
+    dec.share_prompt(ids(150, 1))                      # two common pages and 22 positions
+    dec.extend({0: ids(5, 2)})
+    dec.rewind(0, 151), dec.rewind(0, 128)
+    for n in (127, 64, 0, -1, 129):                    # 129: no longer held
+        with pytest.raises(JoshuaB200Error):
+            dec.rewind(0, n)
+    with pytest.raises(JoshuaB200Error):
+        dec.rewind(3, 10)
+    win = make(1, attention_window=64, n_pages=4)
+    for part in range(5):
+        win.extend({0: ids(50, part)})
+    win.extend({0: [1]})                               # position 250; what is in front of 187 is gone, page 0 and 1 with it
+    win.rewind(0, 200)
+    with pytest.raises(JoshuaB200Error):
+        win.rewind(0, 150)
+    assert win.held == [200]
+    win.extend({0: ids(9, 9)})
+    win.check_flags(), dec.check_flags()
+
+
 def test_refusals():
     dec = make(2)
     for bad in ({}, {0: []}, {0: [1], 1: []}):
