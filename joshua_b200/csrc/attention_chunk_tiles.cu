@@ -160,7 +160,8 @@ struct ChunkConverter {
         if constexpr (KIND == KV_F16) {
 #pragma unroll 1
             for (uint32_t i = cw; i < ITEMS; i += WARPS) {
-                const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 1024 + lane * 16), y = *reinterpret_cast<const uint4*>(raw + i * 1024 + 512 + lane * 16);
+                const uint4 x = *reinterpret_cast<const uint4*>(raw + i * 1024 + lane * 16);
+                const uint4 y = *reinterpret_cast<const uint4*>(raw + i * 1024 + 512 + lane * 16);
                 const uint32_t to = stage + key_to + i / COLS * 2048;
                 sts_v4(to, {x.x, x.y, y.x, y.y}), sts_v4(to + 1024, {x.z, x.w, y.z, y.w});
             }
@@ -191,7 +192,8 @@ struct ChunkConverter {
                     if constexpr (KIND == KV_Q8_0) {
 #pragma unroll
                         for (uint32_t q = 0; q < 2; ++q) {
-                            scaled_terms(codes8<0>(w[q]), s0, &hi[0][2 * q], &lo[0][2 * q]), scaled_terms(codes8<2>(w[q]), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
+                            scaled_terms(codes8<0>(w[q]), s0, &hi[0][2 * q], &lo[0][2 * q]);
+                            scaled_terms(codes8<2>(w[q]), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
                             scaled_terms(codes8<0>(w[2 + q]), s1, &hi[1][2 * q], &lo[1][2 * q]);
                             scaled_terms(codes8<2>(w[2 + q]), s1, &hi[1][2 * q + 1], &lo[1][2 * q + 1]);
                         }
@@ -199,8 +201,10 @@ struct ChunkConverter {
 #pragma unroll
                         for (uint32_t q = 0; q < 2; ++q) {
                             const uint32_t u = w[2 * o + q];
-                            scaled_terms(codes4<0>(u), s0, &hi[0][2 * q], &lo[0][2 * q]), scaled_terms(codes4<1>(u), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
-                            scaled_terms(codes4<2>(u), s1, &hi[1][2 * q], &lo[1][2 * q]), scaled_terms(codes4<3>(u), s1, &hi[1][2 * q + 1], &lo[1][2 * q + 1]);
+                            scaled_terms(codes4<0>(u), s0, &hi[0][2 * q], &lo[0][2 * q]);
+                            scaled_terms(codes4<1>(u), s0, &hi[0][2 * q + 1], &lo[0][2 * q + 1]);
+                            scaled_terms(codes4<2>(u), s1, &hi[1][2 * q], &lo[1][2 * q]);
+                            scaled_terms(codes4<3>(u), s1, &hi[1][2 * q + 1], &lo[1][2 * q + 1]);
                         }
                     }
                     const uint32_t block = to ^ o << 6;  // the second block of a pair stands four 16-byte pieces on, in the swizzle
@@ -299,7 +303,8 @@ struct ChunkConverter {
                         const uint32_t to = (stage + value_to[E] + g * 2048 + H * 1024) ^ o << 6;
                         sts_v2(to, hi[0], hi[1]), sts_v2(to + V_LO, lo[0], lo[1]);
                     };
-                    put(Constant<0>{}, Constant<0>{}), put(Constant<0>{}, Constant<1>{}), put(Constant<1>{}, Constant<0>{}), put(Constant<1>{}, Constant<1>{});
+                    put(Constant<0>{}, Constant<0>{}), put(Constant<0>{}, Constant<1>{});
+                    put(Constant<1>{}, Constant<0>{}), put(Constant<1>{}, Constant<1>{});
                 }
             }
             bool some = odd[0];
@@ -506,8 +511,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         };
         float mx = -INFINITY;
         f32x2 sums = 0;  // sum and outputs times 2^UP, as the probabilities are
-        // The probabilities of page g into tensor memory, when the products before the last have read theirs; seen (EDGE): the positions that the row sees, a bit each.  Returns what the
-        // sums before are worth under the new maximum.
+        // The probabilities of page g into tensor memory, when the products before the last have read theirs; seen (EDGE): the positions
+        // that the row sees, a bit each.  Returns what the sums before are worth under the new maximum.
         auto page = [&](auto edge, uint32_t seen0, uint32_t seen1) {
             constexpr bool EDGE = decltype(edge)::value;
             const uint32_t from = lanes + T::S0 + (g & 1) * KV_PAGE, to = lanes + T::P0 + (g & 1) * KV_PAGE;
@@ -828,7 +833,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         const uint32_t in_front = scan(mine, 1, &total);
         const uint32_t heads = min(a.group, CQ), blocks = (a.group + CQ - 1) / CQ, segments = a.c.n_kv * blocks;  // of a tile
         const uint64_t units = (uint64_t)total * segments, workers = min((uint64_t)gridDim.x, units);
-        const uint64_t x0 = blockIdx.x < workers ? blockIdx.x * units / workers : 0, x1 = blockIdx.x < workers ? (blockIdx.x + 1) * units / workers : 0;
+        const uint64_t x0 = blockIdx.x < workers ? blockIdx.x * units / workers : 0;
+        const uint64_t x1 = blockIdx.x < workers ? (blockIdx.x + 1) * units / workers : 0;
         auto cta_at = [&](uint64_t x) { return (uint32_t)(((x + 1) * workers - 1) / units); };
         // segments of which [x0, x1) has pages: from the one that x0 is in to the last one of which it has more than the beginning
         uint32_t run = in_front;
@@ -846,7 +852,8 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
             }
         });
         asm volatile("bar.sync 7, %0;" ::"n"(C_CONV * 32) : "memory");
-        const uint32_t first_seg = sh.first_seg, end_seg = sh.end_seg, batches = end_seg > first_seg ? (end_seg - first_seg + C_PIECES - 1) / C_PIECES : 0;
+        const uint32_t first_seg = sh.first_seg, end_seg = sh.end_seg;
+        const uint32_t batches = end_seg > first_seg ? (end_seg - first_seg + C_PIECES - 1) / C_PIECES : 0;
         const ChunkConverter<KIND, HD, C_HALF> convert(cw % C_HALF, lane);
         uint32_t g = 0;
         auto list = [&](uint32_t turn) {

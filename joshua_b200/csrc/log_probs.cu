@@ -309,7 +309,8 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_kernel(LogProbArgs a,
                     if (mask) {
                         const uint32_t i = __ffs(mask) - 1;
                         mask &= mask - 1;
-                        k = key_of(logit_of(reinterpret_cast<const float*>(&sh.ring[slot][i / 4][tid])[i % 4]), at + (i / 4 * LP_THREADS + tid) * 4 + i % 4 - sl.shift);
+                        const float x = reinterpret_cast<const float*>(&sh.ring[slot][i / 4][tid])[i % 4];
+                        k = key_of(logit_of(x), at + (i / 4 * LP_THREADS + tid) * 4 + i % 4 - sl.shift);
                     }
                     const uint32_t in = __ballot_sync(0xFFFFFFFFu, k > border);
                     if (k > border) sh.list[warp][count + __popc(in & ((1u << lane) - 1))] = k;
