@@ -7,7 +7,7 @@
 // accuracy where one token has nearly all of the weight (1 - p = 1e-9 is nothing beside 1 in f32).
 //
 // The likeliest n: keys of (logit, lower id first) as 64-bit numbers.  Keys above a border go on a list of their warp; the border is the
-// n-th largest of the maxima of 32 groups of threads, of the first tile to begin with and of all that came since a few times later, so a
+// n-th largest of the maxima of groups of threads, of the first tile to begin with and of all that came since a few times later, so a
 // list seldom holds more than a few keys.  One that grows all the same is cut back to its n largest.
 //
 // CTAs go from row to row; a cluster of them takes one where rows are few or do not go round evenly, each a slice of it, and rank 0 joins
@@ -34,20 +34,23 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr uint32_t LP_THREADS = 256, LP_WARPS = LP_THREADS / 32, LP_VECS = 2, LP_VALUES = 4 * LP_VECS, LP_TILE = LP_THREADS * LP_VALUES;
-constexpr uint32_t LP_STAGES = 4, LP_GROUP = LP_THREADS / 32, LP_MOST_CTAS = 8;  // tiles on their way; threads of a group; CTAs a row
+constexpr uint32_t LP_STAGES = 4, LP_MOST_CTAS = 8;  // tiles on their way; CTAs a row
 constexpr uint32_t LP_CUT = 48;                      // a warp's list of more is cut back
 constexpr uint32_t LP_CAP = 32 * LP_VALUES + LP_CUT;  // so a tile's keys always fit
 constexpr float LOG2E = 1.44269504f, LEAST = -1000.0f, LARGEST = 3.402823466e38f;
 constexpr uint32_t LP_KEYS = LP_WARPS * LP_CUT;
 static_assert(LOG_PROBS_MOST == 32 && LP_CUT >= LOG_PROBS_MOST && LP_CUT <= 64 && LP_MOST_CTAS * LOG_PROBS_MOST <= LP_KEYS, "lists");
 
+struct Tops {
+    float of32[32], of64[64];
+};
 struct LogProbShared {
     float4 ring[LP_STAGES][LP_VECS][LP_THREADS];
     u64 list[LP_WARPS][LP_CAP];
     alignas(16) u64 keys[LP_KEYS];        // of all lists, those above the border
     u64 best[2][LOG_PROBS_MOST];          // the CTA's, in order, of rows in turn
     u64 joined[LOG_PROBS_MOST];           // the cluster's
-    alignas(16) float group_top[2][32];   // largest ones of groups of threads, in turn
+    alignas(16) Tops tops[2];             // largest ones of groups of threads, in turn
     float4 part[LP_WARPS];                // of the warps: maximum, S without the largest ones' 1, T, number of largest ones
     float4 all[2];                        // of the CTA, of rows in turn
     uint32_t total;                       // of sh.keys
@@ -166,29 +169,41 @@ __device__ __noinline__ float4 join(float4 x) {
         for (int i = 0; i < 3; ++i) r[i] += __shfl_xor_sync(0xFFFFFFFFu, r[i], o);
     return {top, r[0], r[1], r[2]};
 }
-// What groups of threads have seen until now, `most` of a thread: the largest of all, and the n-th largest of the groups'.  All threads.
+// What groups of threads have seen until now, `most` of a thread: the largest of all, and the n-th largest of the groups' for the border.
+// About G log(G / (G - n)) values of the first tile are above that of G groups: 32 groups for up to 24 of them, else 64 (with 32 for all,
+// lists of 32 were cut back again and again: 4 rows of 151818 46 us).  All threads.
 struct Look {
     float best, nth;
 };
-__device__ __noinline__ Look look(float (&tops)[32], float most, uint32_t n) {
+template <uint32_t PER>  // groups a lane
+__device__ __forceinline__ float nth_of(const float* tops, uint32_t n) {
+    const uint32_t lane = threadIdx.x & 31;
+    float g[PER];
+    uint32_t above[PER] = {};
+#pragma unroll
+    for (uint32_t k = 0; k < PER; ++k) g[k] = tops[32 * k + lane];
+#pragma unroll 8
+    for (uint32_t j = 0; j < 32 * PER; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(tops + j);
+#pragma unroll
+        for (uint32_t k = 0; k < PER; ++k) above[k] += x.x > g[k], above[k] += x.y > g[k], above[k] += x.z > g[k], above[k] += x.w > g[k];
+    }
+    float least = INFINITY;
+#pragma unroll
+    for (uint32_t k = 0; k < PER; ++k) least = fminf(least, above[k] < n ? g[k] : INFINITY);
+    return smallest_of(least);
+}
+__device__ __noinline__ Look look(Tops& tops, float most, uint32_t n) {
+    static_assert(LP_THREADS == 256, "8 and 4 threads a group");
     const uint32_t tid = threadIdx.x, lane = tid & 31;
     float g = fminf(most, LARGEST);
-#pragma unroll
-    for (int o = LP_GROUP / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, o));
-    if (lane % LP_GROUP == 0) tops[tid / LP_GROUP] = g;
+    g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, 1));
+    g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, 2));
+    if (lane % 4 == 0) tops.of64[tid / 4] = g;
+    g = fmaxf(g, __shfl_xor_sync(0xFFFFFFFFu, g, 4));
+    if (lane % 8 == 0) tops.of32[tid / 8] = g;
     __syncthreads();
-    g = tops[lane];
-    Look seen{largest_of(g), -INFINITY};
-    if (n) {
-        uint32_t above = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 32; j += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(tops + j);
-            above += x.x > g, above += x.y > g, above += x.z > g, above += x.w > g;
-        }
-        seen.nth = smallest_of(above < n ? g : INFINITY);
-    }
-    return seen;
+    return {largest_of(tops.of32[lane]), n == 0 ? -INFINITY : n <= 24 ? nth_of<1>(tops.of32, n) : nth_of<2>(tops.of64, n)};
 }
 // A warp's list of more than n keys cut back to its n largest; the smallest of them.  The warp.
 __device__ __noinline__ u64 cut_back(u64* list, uint32_t count, uint32_t n) {
@@ -277,7 +292,7 @@ __global__ void __launch_bounds__(LP_THREADS, 4) log_probs_kernel(LogProbArgs a,
         float least = -INFINITY, most = -INFINITY;  // its logit; the thread's largest one
         uint32_t count = 0, next_look = 0;          // of the warp's list; a tile
         auto look_again = [&] {
-            const Look seen = look(sh.group_top[turn ^= 1], most, n);
+            const Look seen = look(sh.tops[turn ^= 1], most, n);
             if (seen.nth > least) border = key_of(seen.nth, 0xFFFFFFFFu), least = seen.nth;
             return seen.best;
         };
