@@ -9,7 +9,8 @@
 // not finite too: they are added at the end, to the rows that see them.
 //
 // The tiles' work stands in one row of units, tile by tile, kv head by kv head, SEG_UNITS for beginning and ending one, then its
-// pages.  It is cut into equal pieces, one a CTA; pieces of a tile that several CTAs have are joined by the last of them to arrive, in order.
+// pages.  It is cut into equal pieces, one a CTA, none smaller than the join of a tile's parts makes worth while; what several CTAs have
+// of a tile is joined by the last of them to arrive, in order.
 //
 // Warps: 0 .. 3 softmax, a thread a query row; 4 .. 7 add up the output, the same; 8 .. 15 first cut the work, then turn the pages' codes
 // into swizzled tiles, two stages (half of them keys, half values); 16 issues the products; 17 copies the pages.  Tensor memory: the
@@ -56,6 +57,9 @@ constexpr bool c_regs_fit(uint32_t hd) {
 static_assert(c_regs_fit(64) && c_regs_fit(128), "registers");
 
 constexpr uint32_t SEG_UNITS = 2;   // a tile's beginning and end in pages
+// What joining a part takes the last CTA, in pages (16 tokens, 8 heads on one of 128: 8000 positions cut over all CTAs 148 us, with 0.7 / 1 /
+// 1.5 / 3 here 46.6 / 46.9 / 50.5 / 55.1; 32 on 8, 1000 positions 41.2 and 32.0 / 31.6 / 33.9 / 36.1; 16000 62.0 and 64.6 / 67.8 / 65.3 / 69.8).
+constexpr float JOIN_UNITS = 1.0f;
 constexpr uint32_t C_PIECES = 96;   // pieces of a CTA at a time
 constexpr uint32_t C_STAGE = 5;     // 16-byte vectors a row of the stage, one of them empty: no bank conflicts
 
@@ -832,7 +836,10 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         each_tile([&](uint32_t, uint32_t, const SequenceRows&, uint32_t, uint32_t, const TilePages& pages) { mine += pages.n + SEG_UNITS; });
         const uint32_t in_front = scan(mine, 1, &total);
         const uint32_t heads = min(a.group, CQ), blocks = (a.group + CQ - 1) / CQ, segments = a.c.n_kv * blocks;  // of a tile
-        const uint64_t units = (uint64_t)total * segments, workers = min((uint64_t)gridDim.x, units);
+        const uint64_t units = (uint64_t)total * segments;
+        // of a tile of n units, pieces of sqrt(JOIN_UNITS n) end first: smaller ones wait for the join
+        const uint32_t least = max(1u, (uint32_t)sqrtf(JOIN_UNITS * (float)total / (float)max(n_tiles, 1u)));
+        const uint64_t workers = units >= (uint64_t)gridDim.x * least ? gridDim.x : ((uint32_t)units + least - 1) / least;
         const uint64_t x0 = blockIdx.x < workers ? blockIdx.x * units / workers : 0;
         const uint64_t x1 = blockIdx.x < workers ? (blockIdx.x + 1) * units / workers : 0;
         auto cta_at = [&](uint64_t x) { return (uint32_t)(((x + 1) * workers - 1) / units); };
