@@ -459,7 +459,8 @@ int32_t jq_attention_paged_dev(const jq_kv_cache* cache, const float* q, uint64_
  * the sequence's last left out.
  *   A len out of range (negative, above the page table, or fewer than the sequence's rows) or a page id outside the cache that a
  * row sees makes rows of that sequence NaN (a page: those that see it, and rows near them) and sets *bad_pos_dev; so does a `first` that
- * descends or passes `rows`, whose sequence stores nothing.
+ * descends or passes `rows`, whose sequence stores nothing.  One that goes up and down, so that the sequences' rows together pass the
+ * limits below, is refused whole: *bad_pos_dev is set and nothing is stored.
  *   scratch: jq_attention_chunk_scratch_bytes(...) bytes; one that is large enough serves this entry and jq_attention_paged_dev.
  * rows <= JQ_ATTENTION_MAX_ROWS, rows * n_q <= 2^27, rows * (4 table_stride + 8) < 2^32. */
 #define JQ_ATTENTION_MAX_ROWS 65536u

@@ -365,11 +365,10 @@ struct TilePages {
         sinks = min((uint32_t)(((uint64_t)see.sinks + KV_PAGE - 1) / KV_PAGE), low), skip = low - sinks, n = end - skip;
     }
 };
-// sequences of this kernel: its rows, or none
-__device__ __forceinline__ SequenceRows tile_rows(const PagedArgs& a, uint32_t b) {
-    SequenceRows s = sequence_rows(a, b);
-    if (s.n <= a.span.few || s.len <= 0) s.n = 0;
-    return s;
+// rows of a sequence that this kernel takes
+__device__ __forceinline__ uint32_t tile_rows(const PagedArgs& a, uint32_t b) {
+    const SequenceRows s = sequence_rows(a, b);
+    return s.n <= a.span.few || s.len <= 0 ? 0 : s.n;
 }
 
 template <uint32_t KIND, uint32_t HD>
@@ -430,10 +429,11 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
     if (warp < C_SOFT) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C_REGS_SOFT));
         // rows of sequences without positions, or with ones out of range
+        const bool fit = rows_fit(a, lane);
         for (uint32_t b = blockIdx.x; b < batch; b += gridDim.x) {
             const SequenceRows sq = sequence_rows(a, b);
-            if ((sq.lost || sq.len < 0) && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-            if (sq.n <= a.span.few || sq.len > 0) continue;
+            if ((!fit || sq.lost || sq.len < 0) && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+            if (!fit || sq.n <= a.span.few || sq.len > 0) continue;
             for (uint32_t k = 0; k < sq.n; ++k)
                 for (uint32_t i = tid; i < a.n_q * HD; i += C_SOFT * 32) a.out[(sq.row + k) * a.out_stride + i] = sq.len < 0 ? NAN : 0.0f;
         }
@@ -804,9 +804,11 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         {
             const uint32_t per = (batch + C_CONV * 32 - 1) / (C_CONV * 32), b0 = min(batch, ct * per), b1 = min(batch, b0 + per);
             uint32_t mine = 0;
-            for (uint32_t b = b0; b < b1; ++b) mine += ChunkTiles(a, tile_rows(a, b).n).tiles;
+            const bool fit = rows_fit(a, lane);  // if not, nobody has tiles
+            auto tiles_of = [&](uint32_t b) { return fit ? ChunkTiles(a, tile_rows(a, b)).tiles : 0; };
+            for (uint32_t b = b0; b < b1; ++b) mine += tiles_of(b);
             uint32_t run = scan(mine, 0, &n_tiles);
-            for (uint32_t b = b0; b < b1; ++b) s_tiles[b] = run, run += ChunkTiles(a, tile_rows(a, b).n).tiles;
+            for (uint32_t b = b0; b < b1; ++b) s_tiles[b] = run, run += tiles_of(b);
             if (ct == 0) s_tiles[batch] = n_tiles, sh.first_seg = 0, sh.end_seg = 0;
             asm volatile("bar.sync 7, %0;" ::"n"(C_CONV * 32) : "memory");
         }

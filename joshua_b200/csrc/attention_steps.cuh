@@ -559,8 +559,6 @@ struct Joined {
     }
 };
 
-constexpr uint64_t SPAN_MOST_SEGMENTS = 1u << 27;  // rows of a call times query heads
-
 // Warps of a CTA, one a SM, by the registers that a step needs (64 sequences of up to 8192, heads of 128: 10 warps 108.9 us, 12
 // 106.0, 16, which spill, 120.9).
 constexpr uint32_t ap_warps(uint32_t hd) { return hd == 256 ? 8 : 12; }
@@ -624,11 +622,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     // running sum of the sequences' units, a run of sequences a thread
     const uint32_t per = (batch + WARPS * 32 - 1) / (WARPS * 32), b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
     uint32_t mine = 0, most = 0;
+    bool fit = true;
+    if constexpr (SPAN) fit = rows_fit(a, lane);
     auto units_of = [&](uint32_t b) {
         uint32_t steps, rows = 1;
         if constexpr (SPAN) {
             const SequenceRows sq = sequence_rows(a, b);
-            steps = sq.n <= a.span.few ? steps_a_row<T>(a, sq) : 0, rows = sq.n;
+            steps = fit && sq.n <= a.span.few ? steps_a_row<T>(a, sq) : 0, rows = sq.n;
             most = max(most, steps ? steps + SEG_UNITS : 0);
         } else {
             steps = (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
@@ -910,8 +910,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
         for (uint32_t sb = blockIdx.x; sb < batch; sb += gridDim.x) {
             if (s_cum[sb + 1] != s_cum[sb]) continue;
             const SequenceRows sq = sequence_rows(a, sb);
-            if ((sq.lost || sq.len < 0) && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
-            if (sq.n > a.span.few || sq.len > 0) continue;
+            if ((!fit || sq.lost || sq.len < 0) && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
+            if (!fit || sq.n > a.span.few || sq.len > 0) continue;
             for (uint32_t k = 0; k < sq.n; ++k)
                 for (uint32_t i = tid; i < a.n_q * HD; i += WARPS * 32) a.out[(sq.row + k) * a.out_stride + i] = sq.len < 0 ? NAN : 0.0f;
         }

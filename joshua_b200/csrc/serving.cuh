@@ -48,6 +48,11 @@ cudaError_t launch_attention_paged(const KvPages& c, const float* q, uint64_t q_
 // Rows first[i] .. first[i + 1] - 1 (NULL: rows / n_seq each) of q are the last positions of sequence i, which has len[i]; window 0: a
 // row sees all positions up to its own, else that many and the first `sinks`.
 constexpr uint32_t ATTENTION_MAX_ROWS = 65536;
+// The kernels count steps of 16 positions (and a little for each row), and rows times heads, in 32 bits.
+constexpr uint64_t SPAN_MOST_SEGMENTS = 1u << 27;  // rows of a call times query heads
+__host__ __device__ constexpr bool span_rows_fit(uint64_t rows, uint32_t table_stride, uint32_t n_q) {
+    return rows * (4 * (uint64_t)table_stride + 8) <= 0xFFFFFFFFull && rows * n_q <= SPAN_MOST_SEGMENTS;
+}
 size_t attention_chunk_scratch_bytes(uint32_t rows, uint32_t n_q, uint32_t n_kv, uint32_t hd);
 cudaError_t launch_attention_chunk(const KvPages& c, const float* q, uint64_t q_stride, const int32_t* first, const int32_t* len, uint32_t rows,
                                    uint32_t n_q, float scale, uint32_t window, uint32_t sinks, float* out, uint64_t out_stride,

@@ -208,8 +208,7 @@ int32_t jq_attention_chunk_dev(const jq_kv_cache* cache, const float* q, uint64_
     if (rows > JQ_ATTENTION_MAX_ROWS) return jq_fail(jq::E_TOO_LARGE, "jq_attention_chunk_dev: more than JQ_ATTENTION_MAX_ROWS rows");
     if (!first && rows % batch) return bad(who, "rows that do not divide into equal parts need `first`");
     if ((uint64_t)batch * table_stride > 1u << 28) return bad(who, "a page table of more than 2^28 entries");
-    // the kernels count steps of 16 positions, and rows times heads, in 32 bits
-    if ((uint64_t)rows * (4 * (uint64_t)table_stride + 8) > 0xFFFFFFFFull || (uint64_t)rows * n_q > 1u << 27)
+    if (!jq::span_rows_fit(rows, table_stride, n_q))
         return jq_fail(jq::E_TOO_LARGE, "jq_attention_chunk_dev: rows times positions, or rows times heads, are too many");
     if (!std::isfinite(scale)) return bad(who, "the scale must be finite");
     const uint64_t width = (uint64_t)n_q * cache->head_dim;
