@@ -10,7 +10,7 @@ come from a table (any scaling of `rope.rope_table`), the next tokens from `samp
     dec.sampling = dict(temperature=..., top_p=...)
     dec.uniform.uniform_(); dec.step()           # token by token
     dec.extend({0: ids, 3: more}, scores=5)      # several sequences' next tokens in one pass, with their log probabilities
-    dec.rewind(3, positions)                     # without the last of them
+    dec.rewind(3, positions)                     # without the last of them (or with all: under a penalty they become recent ids)
 
 With `attention_window` a token sees that many positions back and the first `attention_sinks`; pages that no later token sees go back to
 the pool as the sequences grow, and long prompts are read in parts.
@@ -20,6 +20,8 @@ sampling rule's tensors, the penalty and the number of shared pages as they were
 `pos` alone; prompts, steps and host calls that follow (on the stream of the replays, or behind it) begin where it stands.
 """
 from __future__ import annotations
+
+from dataclasses import dataclass, field
 
 import torch
 
@@ -37,6 +39,25 @@ def _same(a, b) -> bool:
     if isinstance(a, tuple):
         return len(a) == len(b) and all(map(_same, a, b))
     return a is b or not isinstance(a, torch.Tensor) and not isinstance(b, torch.Tensor) and a == b
+
+
+def _by_age(window, state) -> list:
+    """A row of recent ids from the oldest to the latest."""
+    ids, (count, at) = window.tolist(), state.tolist()
+    count = min(count, 64)
+    return [ids[(at - count + k) % 64] for k in range(count)]
+
+
+@dataclass
+class _Given:
+    """Ids that a sequence was given at positions start .. end - 1, and its recent ids (the repetition penalty's) in front of them."""
+    start: int
+    end: int
+    ids: torch.Tensor | None   # None: a prompt's, which are not among the recent ids
+    recent: tuple | list       # rows of `window` and `window_state`; a list once they were looked at
+    drawn: bool                # the latest of them was drawn for `start`
+    holes: list = field(default_factory=list)   # ranges of positions whose ids are not among them: prompts, tokens set by hand
+    entered: bool = False      # `ids` came in behind them
 
 
 class _Paged:
@@ -72,6 +93,8 @@ class _Paged:
         self.kept_from = [0] * batch              # pages in front of it (but those of sinks) have gone back
         self.holders = [0] * self.n_pages         # sequences that have a page
         self.held = [0] * batch                   # positions each holds
+        self._given: dict[int, _Given] = {}       # what it was given last, under a repetition penalty
+        self._drawn = [False] * batch             # its latest recent id was drawn for its next position
         self._captured_by_caller = False          # then replays may have moved `pos` past `held`
         self.sampling: dict | None = None         # temperature, top_k, top_p, min_p: vectors of `batch`
         self.uniform = torch.zeros(batch, dtype=torch.float32, device=self.dev)   # numbers in [0, 1) for the next draw
@@ -161,6 +184,7 @@ class _Paged:
         self.pos[sequence], self.active[sequence], self.idle_pos[sequence] = 0, 0, sequence % self._places
         self.resting[sequence] = True
         self._seeds.pop(sequence, None)
+        self._forget_given(sequence)
         self.window[sequence], self.window_state[sequence] = 0, 0   # the next prompt is another text
         if sequence == 0:
             self.shared_pages = 0   # the kernels find the common pages through the first sequence
@@ -170,6 +194,7 @@ class _Paged:
         if not self.resting[i]:
             return
         self.resting[i] = False
+        self._forget_given(i)
         self.pos[i], self.active[i], self.idle_pos[i] = 0, 1, 0
         self.window[i], self.window_state[i] = 0, 0   # steps have left ids there
         if i in self._seeds:
@@ -183,6 +208,7 @@ class _Paged:
         self.owned, self.held, self.resting = [[] for _ in self.owned], [0] * self.batch, [False] * self.batch
         self.kept_from = [0] * self.batch
         self._seeds.clear()
+        self._given, self._drawn = {}, [False] * self.batch
         self.shared_pages = 0
         self.table.fill_(-1), self.active.fill_(1), self.idle_pos.zero_()
         super().reset(token)
@@ -190,6 +216,7 @@ class _Paged:
     def seed_window(self, prompt_ids, sequence: int | None = None) -> None:
         super().seed_window(prompt_ids, sequence)
         for i in range(self.batch) if sequence is None else [range(self.batch)[sequence]]:
+            self._forget_given(i)
             if self.resting[i]:
                 self._seeds[i] = [int(t) for t in prompt_ids][-64:]
 
@@ -197,7 +224,7 @@ class _Paged:
     def prefill(self, token_ids, sequence: int = 0) -> None:
         """The prompt's tokens of one sequence in one pass, from where it stands; then self.logits[sequence], its sampled next
         token (self.token) and position, as `step` leaves them."""
-        self._prompt(token_ids, self._index(sequence))
+        self._note_given({sequence: self._prompt(token_ids, self._index(sequence))})
         self._sample_rows(slice(sequence, sequence + 1))
 
     def share_prompt(self, token_ids) -> None:
@@ -234,6 +261,7 @@ class _Paged:
         self._attention_scratch()
         self.pos.fill_(n - 1)
         self.logits.copy_(self.logits[0:1].expand(self.batch, -1).clone())
+        self._note_given({i: n for i in range(self.batch)})
         self._sample_rows(slice(0, self.batch))
 
     def extend(self, tokens: dict, scores: int | None = None):
@@ -241,7 +269,10 @@ class _Paged:
         next tokens (self.token) and positions of these sequences, as `prefill` leaves them.
 
         With `scores` (a number of alternatives, at most 32): by sequence, what `sampling.log_probs` gives for its tokens but the first,
-        each at the position in front of it."""
+        each at the position in front of it.
+
+        The repetition penalty's recent ids take what is sampled, as with `prefill`: a prompt's are the caller's to enter (`seed_window`), drafts
+        come in with `rewind`, which says how many of them stay."""
         new = {self._index(i): torch.as_tensor(ids, dtype=torch.int32).reshape(-1) for i, ids in sorted(tokens.items())}
         if not new or any(ids.numel() == 0 for ids in new.values()):
             raise JoshuaB200Error(_lib.E_INVALID, "nothing to extend, or an empty prompt")
@@ -261,27 +292,101 @@ class _Paged:
         last = x[(ends - 1).to(self.dev)].contiguous()
         self.logits[seqs] = self._head(last)
         self.pos[seqs] = torch.tensor([self.held[i] - 1 for i in new], dtype=torch.int32, device=self.dev)
+        self._note_given({i: ids.numel() for i, ids in new.items()}, new)
         for i in new:
             self._sample_rows(slice(i, i + 1))
         return given
 
-    def rewind(self, sequence: int, positions: int) -> None:
+    def rewind(self, sequence: int, positions: int, token: int | None = None) -> None:
         """Forgets a sequence's tokens behind its first `positions`, drafts that were not taken: its next ones go there (`extend`, or
-        `step` with self.token[sequence] set).  Not into pages that it has in common with others, nor to where its window has given
-        back what it would see."""
+        `step`, which reads self.token[sequence]; `token` is written there).  Not into pages that it has in common with others, nor to where
+        its window has given back what it would see.
+
+        Under a repetition penalty the recent ids become those of the text that is left: of the drafts of the last `extend` the ones in
+        front of `positions` (all of them, where that is where the sequence stands) come in, in the place of what was drawn there; what was
+        drawn behind them goes out, and `token` comes in.  Where the way back leads to the first of the last ids given or beyond, or over
+        more than 64 steps, what newer ids had pushed out is not brought back."""
         self._look()
         i, n = self._index(sequence), positions
         if not 0 < n <= self.held[i]:
             raise JoshuaB200Error(_lib.E_INVALID, f"{n} of {self.held[i]} positions")
-        if n == self.held[i]:
-            return
+        if token is not None and not 0 <= token < self.cfg.vocab:
+            raise JoshuaB200Error(_lib.E_INVALID, f"token {token} of {self.cfg.vocab}")
         mine, window = self.owned[i], self.attention_window
-        if n < self.shared_pages * PAGE or any(page is not None and self.holders[page] > 1 for page in mine[n // PAGE:]):
-            raise JoshuaB200Error(_lib.E_INVALID, f"{n} positions end in front of pages that sequences share")
-        if window and any(page is None for page in mine[max(0, n + 1 - window) // PAGE:]):
-            raise JoshuaB200Error(_lib.E_INVALID, f"pages in front of position {n} have gone back")
+        if n < self.held[i]:
+            if n < self.shared_pages * PAGE or any(page is not None and self.holders[page] > 1 for page in mine[n // PAGE:]):
+                raise JoshuaB200Error(_lib.E_INVALID, f"{n} positions end in front of pages that sequences share")
+            if window and any(page is None for page in mine[max(0, n + 1 - window) // PAGE:]):
+                raise JoshuaB200Error(_lib.E_INVALID, f"pages in front of position {n} have gone back")
+        self._rewind_recent(i, n, token)
+        if token is not None:
+            self.token[i] = token
         self.held[i] = n
         self.pos[i] = n
+
+    # ── the repetition penalty's recent ids ─────────────────────────────
+    def _forget_given(self, i: int) -> None:
+        self._given.pop(i, None)
+        self._drawn[i] = False
+
+    def _note_given(self, counts: dict, ids: dict | None = None) -> None:
+        """Keeps the recent ids of sequences as they are in front of what is drawn next; counts: of the ids that each was given, `ids`
+        (None, or at position 0: a prompt)."""
+        penalised, rows = self.repetition_penalty != 1.0, list(counts)
+        window, state = (t[torch.tensor(rows, device=self.dev)] for t in (self.window, self.window_state)) if penalised else (None, None)
+        for k, (i, n) in enumerate(counts.items()):
+            before = self._given.pop(i, None)
+            if penalised:
+                start, end, drawn = self.held[i] - n, self.held[i], self._drawn[i]
+                text = ids[i].clone() if ids and start else None
+                holes = [range(r.start, min(r.stop, start)) for r in before.holes if r.start < start] if before else []
+                if before and before.ids is not None and not before.entered:
+                    holes.append(range(before.start + before.drawn, before.end))
+                if text is None:
+                    holes.append(range(start + drawn, end))
+                self._given[i] = _Given(start, end, text, (window[k], state[k]), drawn, holes)
+            self._drawn[i] = penalised
+
+    def _rewind_recent(self, i: int, n: int, token: int | None) -> None:
+        given, held = self._given.get(i), self.held[i]
+        if self.repetition_penalty == 1.0:
+            return self._forget_given(i)
+        if n == held and token is None and (given is None or given.ids is None):
+            return
+        if given is not None and not isinstance(given.recent, list):
+            given.recent = _by_age(*given.recent)
+        if given is not None and given.start < min(n, given.end) and given.ids is None and given.drawn:   # a prompt stands where it was drawn
+            given.recent, given.drawn = given.recent[:-1], False
+            given.holes = [*given.holes, range(given.start, given.start + 1)]
+        recent = self._recent(i, n, token is None) + ([] if token is None else [token])
+        super().seed_window(recent, i)
+        if given is not None:
+            given.entered = True
+        self._drawn[i] = token is not None or n == held and self._drawn[i]
+        if given is None or n < given.start:
+            given = self._given[i] = _Given(n, n, None, recent[-64:], token is not None, given.holes if given else [])
+        elif n < given.end:
+            given.end, given.ids = n, None if given.ids is None else given.ids[:n - given.start]
+        if n < held or token is not None:
+            given.holes = [range(r.start, min(r.stop, n)) for r in given.holes if r.start < n] + [range(n, n + 1)] * (token is None)
+
+    def _recent(self, i: int, n: int, whole: bool) -> list:
+        """Recent ids of a sequence's first n positions, and what was drawn for the next one if it stands there (and `whole`)."""
+        now, given, held, drawn = _by_age(self.window[i], self.window_state[i]), self._given.get(i), self.held[i], self._drawn[i]
+        if given is not None and n < given.start:
+            now, held, drawn = given.recent, given.start, given.drawn
+        holes = given.holes if given else []
+        if given is None or n < given.start:   # those of positions n .. held go out
+            gone = sum(not any(p in r for r in holes) for p in range(n, held)) + drawn
+            return now[:max(0, len(now) - gone)]
+        recent = given.recent[:-1] if given.drawn else given.recent
+        if given.ids is not None:
+            recent = recent + given.ids[:n - given.start].tolist()
+        since = [p for p in range(given.end, held + drawn) if not any(p in r for r in holes)]   # positions of the ids drawn since
+        kept = sum(p < n or whole and p == n == held for p in since)
+        if kept:
+            recent = now[:len(now) - len(since) + kept] if len(since) > len(now) else recent + now[len(now) - len(since):][:kept]
+        return recent[-64:]
 
     def _head(self, x):
         logits = torch.empty(x.size(0), self.cfg.vocab, dtype=torch.float32, device=self.dev)
@@ -341,8 +446,8 @@ class _Paged:
         if getattr(self, "world", 1) > 1:
             raise JoshuaB200Error(_lib.E_INVALID, "prompts run on one GPU (the exchange windows are sized for decode batches)")
 
-    def _prompt(self, token_ids, i) -> None:
-        """Logits of the prompt's last token into self.logits[i]; self.pos[i] at that token."""
+    def _prompt(self, token_ids, i) -> int:
+        """Logits of the prompt's last token into self.logits[i]; self.pos[i] at that token.  How many there were."""
         self._can_prompt(dense=not self.attention_window)
         if self.attention_window:
             return self._prompt_in_parts(token_ids, i)
@@ -378,8 +483,9 @@ class _Paged:
         check(L.jq_matmul_norm_dev(self.output._h, 1, h, c.vocab, P(last), P(self.out_norm), c.eps, None, P(self.logits[i]), s))
         self.held[i] = end
         self.pos[i] = end - 1
+        return S
 
-    def _prompt_in_parts(self, token_ids, i) -> None:
+    def _prompt_in_parts(self, token_ids, i) -> int:
         """The same where there is a window: the dense attention of prompts has none."""
         ids = torch.as_tensor(token_ids, dtype=torch.int32).reshape(-1)
         if ids.numel() == 0:
@@ -391,6 +497,7 @@ class _Paged:
             x = self._pass({i: part})
         self.logits[i] = self._head(x[-1:].clone())[0]
         self.pos[i] = self.held[i] - 1
+        return ids.numel()
 
     def _room_for_parts(self, i, n: int) -> None:
         """Raises, before any part is taken, if they do not fit: what each part takes and the window gives back."""
@@ -429,11 +536,13 @@ class _Paged:
         self._trim(i for i in range(self.batch) if not self.resting[i])
         self._reserve({i: n + 1 for i, n in enumerate(self.held) if not self.resting[i]})
         self.held = [n + (not rests) for n, rests in zip(self.held, self.resting)]
+        self._drawn = [self.repetition_penalty != 1.0 if not rests else drawn for drawn, rests in zip(self._drawn, self.resting)]
 
     def _look(self) -> None:
         """Positions as replays of a caller's graph left them."""
         if self._captured_by_caller:
-            self.held = [0 if rests else n for n, rests in zip(self.pos.tolist(), self.resting)]
+            was, self.held = self.held, [0 if rests else n for n, rests in zip(self.pos.tolist(), self.resting)]
+            self._drawn = [self.repetition_penalty != 1.0 if n != old else drawn for n, old, drawn in zip(self.held, was, self._drawn)]
 
     def _launches(self, stream) -> None:
         torch.addcmul(self.idle_pos, self.pos, self.active, out=self.pos)   # resting: to its place behind the pool,
