@@ -163,28 +163,22 @@ __device__ __forceinline__ void quantize_unit_values(const float (&v)[8], uint32
 }
 
 
-// The unit's values come from memory.  COHERENT: x may have been written by another CTA of this same launch
-// (the persistent chain): read it from L2.  With `nw` (the unit's 256 RMS-norm weights) the values split are
-// x * rs * nw, i.e. the normalised row.
-template <bool COHERENT = false>
-__device__ __forceinline__ void load_unit_values(const float* __restrict__ xu, uint32_t lane, float (&v)[8]) {
+// A unit's values (the kernel in front may have written them), or its RMS-norm weights, from memory.
+template <bool WEIGHTS = false>
+__device__ __forceinline__ void load_unit_values(const float* xu, uint32_t lane, float (&v)[8]) {
     const float4* src = reinterpret_cast<const float4*>(xu + lane * 8);
-    float4 lo4 = COHERENT ? __ldcg(src) : __ldg(src), hi4 = COHERENT ? __ldcg(src + 1) : __ldg(src + 1);
+    float4 lo4 = WEIGHTS ? __ldg(src) : ld_behind(src), hi4 = WEIGHTS ? __ldg(src + 1) : ld_behind(src + 1);
     v[0] = lo4.x, v[1] = lo4.y, v[2] = lo4.z, v[3] = lo4.w, v[4] = hi4.x, v[5] = hi4.y, v[6] = hi4.z, v[7] = hi4.w;
 }
 
-template <bool COHERENT = false>
-__device__ __forceinline__ void quantize_unit_warp(const float* __restrict__ xu, uint32_t lane, uint32_t type,
-                                                   int8_t* planes, float2* meta, float* sum16,
-                                                   const float* __restrict__ nw = nullptr, float rs = 1.0f) {
-    float v[8];
-    load_unit_values<COHERENT>(xu, lane, v);
-    if (nw) {
-        float g[8];
-        load_unit_values<false>(nw, lane, g);
+// The values of a normalised row, x * rs * nw.
+__device__ __forceinline__ void quantize_unit_warp(const float* xu, uint32_t lane, uint32_t type, int8_t* planes, float2* meta,
+                                                   float* sum16, const float* nw, float rs) {
+    float v[8], g[8];
+    load_unit_values(xu, lane, v);
+    load_unit_values<true>(nw, lane, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * g[j];
-    }
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * rs * g[j];
     quantize_unit_values(v, lane, type, planes, meta, sum16);
 }
 
@@ -192,9 +186,8 @@ __device__ __forceinline__ void quantize_unit_warp(const float* __restrict__ xu,
 // (w = 0 .. NW-1) that meet on named barrier 1.  Loads are requested in batches before any is used, so the
 // prologue costs about one trip to L2 instead of one per unit.  With `norm_w` every row is RMS-normalised
 // first (1 / rms from the units' sums of squares, added in unit order).  s_tmp: NW * GEMV_MMA_MAX_M floats.
-template <bool COHERENT, int NW>
-__device__ __forceinline__ void split_activations(const float* __restrict__ x, uint32_t rows, uint32_t k,
-                                                  const float* __restrict__ norm_w, float eps, uint32_t type,
+template <int NW>
+__device__ __forceinline__ void split_activations(const float* x, uint32_t rows, uint32_t k, const float* norm_w, float eps, uint32_t type,
                                                   uint8_t* s_act, int w, uint32_t lane, float* s_tmp) {
     const uint32_t units_per_row = k / 256, total = rows * units_per_row;
     const uint64_t groups = (uint64_t)rows * (k / 32);
@@ -206,7 +199,7 @@ __device__ __forceinline__ void split_activations(const float* __restrict__ x, u
             float v[4][8];
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (u0 + r * NW < total) load_unit_values<COHERENT>(x + (uint64_t)(u0 + r * NW) * 256, lane, v[r]);
+                if (u0 + r * NW < total) load_unit_values(x + (uint64_t)(u0 + r * NW) * 256, lane, v[r]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const uint32_t u = u0 + r * NW;
@@ -220,8 +213,8 @@ __device__ __forceinline__ void split_activations(const float* __restrict__ x, u
         for (int r = 0; r < 2; ++r) {
             const uint32_t u = w + r * NW;
             if (u < total) {
-                load_unit_values<COHERENT>(x + (uint64_t)u * 256, lane, v[r]);
-                load_unit_values<false>(norm_w + (u % units_per_row) * 256, lane, g[r]);
+                load_unit_values(x + (uint64_t)u * 256, lane, v[r]);
+                load_unit_values<true>(norm_w + (u % units_per_row) * 256, lane, g[r]);
             }
         }
 #pragma unroll
@@ -257,7 +250,7 @@ __device__ __forceinline__ void split_activations(const float* __restrict__ x, u
             const float4* xr = reinterpret_cast<const float4*>(x + (uint64_t)r * k);
             float ss = 0.0f;
             for (uint32_t i = w * 32 + lane; i < k / 4; i += NW * 32) {
-                float4 q = COHERENT ? __ldcg(xr + i) : __ldg(xr + i);
+                float4 q = ld_behind(xr + i);
                 ss = fmaf(q.x, q.x, fmaf(q.y, q.y, fmaf(q.z, q.z, fmaf(q.w, q.w, ss))));
             }
 #pragma unroll
@@ -271,8 +264,8 @@ __device__ __forceinline__ void split_activations(const float* __restrict__ x, u
             const float rs = rsqrtf(tot / (float)k + eps);
             for (uint32_t uc = w; uc < units_per_row; uc += NW) {
                 const uint32_t u = r * units_per_row + uc;
-                quantize_unit_warp<COHERENT>(x + (uint64_t)u * 256, lane, type, planes + (uint64_t)u * 768, meta + u * 8,
-                                             sum16 + u * 16, norm_w + uc * 256, rs);
+                quantize_unit_warp(x + (uint64_t)u * 256, lane, type, planes + (uint64_t)u * 768, meta + u * 8,
+                                   sum16 + u * 16, norm_w + uc * 256, rs);
             }
         }
         (void)s_rs;
@@ -280,7 +273,7 @@ __device__ __forceinline__ void split_activations(const float* __restrict__ x, u
     asm volatile("bar.sync 1, %0;" ::"r"(NW * 32) : "memory");
 }
 
-__global__ void __launch_bounds__(256) quantize_acts_kernel(const float* __restrict__ x, uint64_t m, uint64_t k,
+__global__ void __launch_bounds__(256) quantize_acts_kernel(const float* x, uint64_t m, uint64_t k,
                                                             uint32_t type, int8_t* __restrict__ planes,
                                                             float2* __restrict__ meta, float* __restrict__ sum16) {
     // one block per 256-value unit, one thread per value; warp = 32-value group
@@ -365,14 +358,6 @@ struct Traits<T_Q6_K> {
     static constexpr uint32_t UNIT_BYTES = 210, CHUNK_UNITS = 16;
 };
 
-// Activation data is read from shared memory when the kernel staged it there (ACT == 1) and from global
-// memory through the read-only path otherwise.
-template <int ACT, class T>
-__device__ __forceinline__ T ld_act(const T* p) {
-    if (ACT) return *p;
-    return __ldg(p);
-}
-
 // Per-lane roles, fixed for the kernel's lifetime.
 //
 // One MMA has 8 activation columns.  A slot is three columns (hi, mid, lo planes of one batch row for one
@@ -417,7 +402,7 @@ struct Roles {
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             uint32_t pos = row0 + min((uint32_t)b, cnt - 1);
-            brow[b] = act_rows ? __ldg(act_rows + pos) : pos;
+            brow[b] = act_rows ? act_rows[pos] : pos;
         }
         // register arrays must only be indexed by compile-time constants: pick with selects
 #pragma unroll
@@ -441,7 +426,7 @@ struct Roles {
 // g+8 in shared memory; U is the unit's index along k (its first 32-group is 8U).
 //   colacc[h][j][r]  running sum of held column j, row r (0: g, 1: g+8), pass h
 //   minacc[b][r]     running sum of the minima terms of batch row b
-template <uint32_t TYPE, int MB, int NH, int ACT>
+template <uint32_t TYPE, int MB, int NH>
 __device__ __forceinline__ void process_unit(const uint8_t* u0, const uint8_t* u1, uint32_t U, const ActPlanes& act,
                                              const Roles<MB, NH>& ro, const uint2* s_grid, const uint2* s_mask,
                                              float colacc[NH][2][2], float minacc[MB * NH][2]) {
@@ -466,10 +451,10 @@ __device__ __forceinline__ void process_unit(const uint8_t* u0, const uint8_t* u
             if (!ro.sup_live) {
                 bsup[h] = make_uint2(0u, 0u);
             } else if (k16) {
-                bsup[h].x = ld_act<ACT>(reinterpret_cast<const uint32_t*>(src + off16 - 4 * ro.t));
+                bsup[h].x = *reinterpret_cast<const uint32_t*>(src + off16 - 4 * ro.t);
                 bsup[h].y = 0u;
             } else {
-                bsup[h] = ld_act<ACT>(reinterpret_cast<const uint2*>(src));
+                bsup[h] = *reinterpret_cast<const uint2*>(src);
             }
         }
     };
@@ -515,7 +500,7 @@ __device__ __forceinline__ void process_unit(const uint8_t* u0, const uint8_t* u
             for (int j = 0; j < 2; ++j) {
                 // activation scale of the batch row this column belongs to (one per 256-value unit)
                 uint32_t row = ro.col_row[h][j];
-                float sa = ld_act<ACT>(&act.meta[(uint64_t)row * act.n_groups + G0].x) * ro.col_w[j];
+                float sa = act.meta[(uint64_t)row * act.n_groups + G0].x * ro.col_w[j];
                 float v0 = INT_SCALE ? (float)isum[h][j][0] : fsum[h][j][0];
                 float v1 = INT_SCALE ? (float)isum[h][j][1] : fsum[h][j][1];
                 colacc[h][j][0] = fmaf(f0 * sa, v0, colacc[h][j][0]);
@@ -573,7 +558,7 @@ __device__ __forceinline__ void process_unit(const uint8_t* u0, const uint8_t* u
             float m0 = (float)((mw0 >> sh) & 0xFF) * dm0, m1 = (float)((mw1 >> sh) & 0xFF) * dm1;
 #pragma unroll
             for (int b = 0; b < MB * NH; ++b) {
-                float sx = ld_act<ACT>(&act.meta[(uint64_t)ro.brow[b] * act.n_groups + G0 + 2 * ro.t + e].y);
+                float sx = act.meta[(uint64_t)ro.brow[b] * act.n_groups + G0 + 2 * ro.t + e].y;
                 minacc[b][0] = fmaf(m0, sx, minacc[b][0]);
                 minacc[b][1] = fmaf(m1, sx, minacc[b][1]);
             }
@@ -745,7 +730,7 @@ __device__ __forceinline__ void process_unit(const uint8_t* u0, const uint8_t* u
             float m0 = (float)(u0[j16] >> 4) * dm0, m1 = (float)(u1[j16] >> 4) * dm1;
 #pragma unroll
             for (int b = 0; b < MB * NH; ++b) {
-                float sx = ld_act<ACT>(act.sum16 + ((uint64_t)ro.brow[b] * act.n_groups + G0) * 2 + j16);
+                float sx = act.sum16[((uint64_t)ro.brow[b] * act.n_groups + G0) * 2 + j16];
                 minacc[b][0] = fmaf(m0, sx, minacc[b][0]);
                 minacc[b][1] = fmaf(m1, sx, minacc[b][1]);
             }
@@ -908,10 +893,10 @@ __global__ void __launch_bounds__((NCW + 2) * 32, 1) gemv_mma_kernel(const __gri
         // Consumers and the reducer split the activations into planes in shared memory while the producer
         // fills the ring.
         __shared__ float s_tmp[(NCW + 1) * GEMV_MMA_MAX_M];
-        split_activations<false, NCW + 1>(ga.x, ga.x_rows, (uint32_t)k, ga.norm_w, ga.norm_eps,
+        split_activations<NCW + 1>(ga.x, ga.x_rows, (uint32_t)k, ga.norm_w, ga.norm_eps,
                                           TYPE, s_act, warp - 1, lane, s_tmp);
     }
-    const uint32_t n_jobs = grouped ? __ldg(ga.n_jobs) : 1u;
+    const uint32_t n_jobs = grouped ? ld_behind(ga.n_jobs) : 1u;
     const uint32_t n_tiles = n_jobs * tiles_per_expert;
     // tile -> (job, row tile); the job gives the expert (weight offset) and the activation rows
     auto job_of = [&](uint32_t tile, uint32_t* rt) -> MoeJob {
@@ -1007,7 +992,7 @@ __global__ void __launch_bounds__((NCW + 2) * 32, 1) gemv_mma_kernel(const __gri
                     for (uint32_t u = cw; u < cnt; u += NCW) {
                         const uint8_t* u0 = st + ro.g * plan.row_stride + sh0 + u * Tr::UNIT_BYTES;
                         const uint8_t* u1 = st + (ro.g + 8) * plan.row_stride + sh1 + u * Tr::UNIT_BYTES;
-                        process_unit<TYPE, MB, NH, ACT>(u0, u1, u_lo + u, a, ro, s_grid, s_mask, colacc, minacc);
+                        process_unit<TYPE, MB, NH>(u0, u1, u_lo + u, a, ro, s_grid, s_mask, colacc, minacc);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[s]);
@@ -1149,10 +1134,10 @@ __global__ void __launch_bounds__((16 + 2) * 32, 1) gemv_narrow_kernel(const __g
     pdl_wait();  // the job list comes from the kernel before this one
     if (ACT && warp != 0) {
         __shared__ float s_tmp[(NCW + 1) * GEMV_MMA_MAX_M];
-        split_activations<false, NCW + 1>(ga.x, ga.x_rows, (uint32_t)k, ga.norm_w, ga.norm_eps, TYPE, s_act, warp - 1,
+        split_activations<NCW + 1>(ga.x, ga.x_rows, (uint32_t)k, ga.norm_w, ga.norm_eps, TYPE, s_act, warp - 1,
                                           lane, s_tmp);
     }
-    const uint32_t n_st = __ldg(ga.n_jobs) * st_per_expert;
+    const uint32_t n_st = ld_behind(ga.n_jobs) * st_per_expert;
     const uint32_t rb16 = (uint32_t)(row_bytes & 15), eb16 = (uint32_t)(ga.expert_bytes & 15);
     auto shift_of = [&](uint32_t sub, uint32_t e, uint32_t row) -> uint32_t {
         return ((uint32_t)(reinterpret_cast<uintptr_t>(ga.w[sub]) & 15) + e * eb16 + row * rb16) & 15;
@@ -1236,7 +1221,7 @@ __global__ void __launch_bounds__((16 + 2) * 32, 1) gemv_narrow_kernel(const __g
                     const uint8_t* sp = ring + s * stage_bytes + ti * ROWS * plan.row_stride;
                     const uint8_t* u0 = sp + ro.g * plan.row_stride + sh0 + u * Tr::UNIT_BYTES;
                     const uint8_t* u1 = sp + (ro.g + 8) * plan.row_stride + sh1 + u * Tr::UNIT_BYTES;
-                    process_unit<TYPE, MB, NH, ACT>(u0, u1, u, a, ro, s_grid, s_mask, colacc, minacc);
+                    process_unit<TYPE, MB, NH>(u0, u1, u, a, ro, s_grid, s_mask, colacc, minacc);
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[s]);

@@ -1,0 +1,31 @@
+"""The linears, the decoders' own kernels and the exchange read what the kernel in front may have written by plain loads, as the serving and
+routing kernels do (tests/test_serving_loads.py, tests/test_moe_loads.py): read-only ones may be moved above the wait for it.  Read
+from the sources, since whether a compiler moves a load cannot be told from results."""
+import re
+
+import pytest
+
+from tests.conftest import ROOT
+
+# by file: what may be read so all the same, weights and tables that no kernel of a step writes (pointers; in __ldg)
+FILES = {
+    "gemv_mma.cu": (set(), {"src", "src + 1"}),   # of load_unit_values<WEIGHTS>
+}
+
+
+def source(name):
+    return re.sub(r"//[^\n]*", "", (ROOT / "joshua_b200" / "csrc" / name).read_text())
+
+
+@pytest.mark.parametrize("name", FILES)
+def test_what_may_be_on_its_way_is_read_by_plain_loads(name):
+    text, (pointers, loads) = source(name), FILES[name]
+    assert set(re.findall(r"\bconst\b[^,;(){}]*\*\s*__restrict__ (\w+)", text)) <= pointers
+    assert {m for m in re.findall(r"__ldg\(((?:[^()]|\([^()]*\))*)\)", text)} <= loads
+    assert "ld.global.nc" not in text
+
+
+def test_the_activations_of_the_linears():
+    text = source("gemv_mma.cu")
+    assert len(re.findall(r"WEIGHTS \? __ldg\(src(?: \+ 1)?\) : ld_behind\(src(?: \+ 1)?\)", text)) == 2
+    assert set(re.findall(r"load_unit_values<true>\((\w+)", text)) == {"norm_w", "nw"}
