@@ -580,8 +580,8 @@ __device__ __forceinline__ void convert64(uint32_t u, uint32_t g, const RowWin& 
 // up: as a call it cost the kernel seven per cent where it never ran (Q4_K 28672 x 4096, 8 rows 53.5 us instead of 50.4).
 template <uint32_t TYPE, int NB, class Add>
 __device__ __forceinline__ void add_lost(const uint8_t* row, uint32_t win0, uint32_t n_chunks, uint32_t S0, uint32_t S1, uint64_t k,
-                                      const __half* __restrict__ x_hi, const __half* __restrict__ x_lo,
-                                      const float* __restrict__ rel, uint64_t m_rows, uint64_t tok0, uint32_t n_tok, Add add) {
+                                      const __half* x_hi, const __half* x_lo, const float* rel, uint64_t m_rows, uint64_t tok0,
+                                      uint32_t n_tok, Add add) {
 #pragma unroll 1
     for (uint32_t c = win0; c < win0 + n_chunks; ++c) {
         const uint8_t* win = row + (uint64_t)c * HT<TYPE>::UNIT;
@@ -632,21 +632,16 @@ __device__ __forceinline__ void convert_minima(uint32_t u, const RowWin& rw, uin
     }
 }
 
-// Loads of what a kernel in front wrote, for places directly behind pdl_wait: read-only loads (__ldg, or plain ones through
-// __restrict__) may be moved above the wait, volatile ones stay.  (The sign of a row's scale, read too early: in one call out
-// of eight of 200 rows x 14336 columns a window with a scale of its own, where the call before had none, counted some 500 times.)
+// What the kernels in front wrote is read by plain or volatile loads (pipe.cuh: ld_behind).  (The sign of a row's scale, read too early by
+// a read-only one: in one call out of eight of 200 rows x 14336 columns a window with a scale of its own, where the call before had
+// none, counted some 500 times.)  This one comes from L2.
 __device__ __forceinline__ float ld_behind_wait(const float* p) {
     float v;
     asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
     return v;
 }
-// The same for the list of expert tiles, which every CTA of an SM reads: kept in L1 (the lists of two launches that could overlap are
+// The list of expert tiles, which every CTA of an SM reads: kept in L1 (the lists of two launches that could overlap are
 // one layer's, and equal).  Through L2 the routed-expert model's prompt of 1000 tokens took 36.7 ms instead of 35.7.
-__device__ __forceinline__ uint32_t ld_list(const uint32_t* p) {
-    uint32_t v;
-    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint4 ld_list(const GemmTile* p) {
     uint4 v;
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
@@ -658,9 +653,9 @@ template <uint32_t TYPE, int N_TILE, uint32_t VEC>
 __global__ void __launch_bounds__(H_THREADS, 1)
     gemm_f16_kernel(const uint8_t* __restrict__ w_a, uint64_t n, uint64_t k, const __grid_constant__ CUtensorMap map_hi,
                     const __grid_constant__ CUtensorMap map_lo, const __grid_constant__ CUtensorMap map_sums,
-                    const float* __restrict__ inv, const float* __restrict__ rel, const __half* __restrict__ x_hi,
-                    const __half* __restrict__ x_lo, uint64_t m_rows, float* dst_a, const float* residual, int* __restrict__ error_flag,
-                    const GemmTile* __restrict__ tiles, const uint32_t* __restrict__ n_tiles, uint64_t expert_bytes,
+                    const float* inv, const float* rel, const __half* x_hi,
+                    const __half* x_lo, uint64_t m_rows, float* dst_a, const float* residual, int* __restrict__ error_flag,
+                    const GemmTile* tiles, const uint32_t* n_tiles, uint64_t expert_bytes,
                     const uint8_t* __restrict__ w_b, float* dst_b, uint32_t split) {
     using T = HT<TYPE>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -680,6 +675,7 @@ __global__ void __launch_bounds__(H_THREADS, 1)
     __shared__ uint64_t scales_known;  // wide tiles: scaled_groups, by converter group, whether some token has windows with own scales
     __shared__ uint32_t scaled_groups, tmem_base_slot;
     __shared__ int abort_flag, lost_flag;
+    __shared__ float s_inv[N_TILE];  // of the tokens, for the join
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_trigger();
@@ -692,7 +688,7 @@ __global__ void __launch_bounds__(H_THREADS, 1)
     float* dst = bank ? dst_b : dst_a;
     if (tiles != nullptr) {
         pdl_wait();
-        if (blockIdx.y >= ld_list(n_tiles)) return;
+        if (blockIdx.y >= ld_behind(n_tiles)) return;
         const uint4 t = ld_list(tiles + blockIdx.y);  // expert, row0, cnt
         w += (uint64_t)t.x * expert_bytes;
         tok0 = t.y;
@@ -905,6 +901,8 @@ __global__ void __launch_bounds__(H_THREADS, 1)
         if (scaled) rescale(n_chunks);
         if (!ok) abort_flag = 1;
         pdl_wait();  // dst and the rows' scales belong to the kernels before this one
+        const bool joins = (S::FINE || split > 1) && tid < N_TILE;  // a token a thread: loads in the join would be waited for one by one
+        const float scale = joins && tok0 + tid < m ? ld_behind_wait(inv + tok0 + tid) : 0.0f;
         // The ring and the staged bytes are idle once every converter is here: the last read-back waited for this CTA's
         // last products.
         asm volatile("bar.sync 1, %0;" ::"n"(H_CONV * 32) : "memory");
@@ -916,7 +914,7 @@ __global__ void __launch_bounds__(H_THREADS, 1)
                 for (int c = 0; c < MY_COLS; ++c) {
                     const uint64_t tok = tok0 + g * MY_COLS + c;
                     if (tok < m) {
-                        const float v = sums[c] * fabsf(__ldg(inv + tok));
+                        const float v = sums[c] * fabsf(inv[tok]);
                         dst[tok * n + out_row] = residual ? residual[tok * n + out_row] + v : v;
                     }
                 }
@@ -926,6 +924,7 @@ __global__ void __launch_bounds__(H_THREADS, 1)
             // of their own steps)
 #pragma unroll
             for (int c = 0; c < MY_COLS; ++c) red[(g * MY_COLS + c) * HM + q * 32 + lane] = sums[c];
+            if (joins) s_inv[tid] = fabsf(scale);
         }
         if constexpr (T::LOSES) {
             if (lost_flag && ok && first_tok < m) {  // each thread adds to what it has just stored
@@ -935,7 +934,9 @@ __global__ void __launch_bounds__(H_THREADS, 1)
                                           if (S::FINE || split > 1)
                                               red[(g * MY_COLS + t) * HM + q * 32 + lane] += v;
                                           else if (out_row < n)
-                                              dst[(first_tok + t) * n + out_row] += v * fabsf(__ldg(inv + first_tok + t));
+                                              // (not a plain load: although it never runs, the compiler made the whole kernel slower for
+                                              // it, Q4_K 4096 x 14336, 333 rows 121 -> 130 us)
+                                              dst[(first_tok + t) * n + out_row] += v * fabsf(ld_behind_wait(inv + first_tok + t));
                                       });
             }
         }
@@ -1095,7 +1096,7 @@ __global__ void __launch_bounds__(H_THREADS, 1)
                         const uint32_t addr = red + ((p * N_TILE + t) * HM + row) * 4;
                         v += split > 1 ? ld_cluster_f32(addr, r) : __uint_as_float(s32(addr));
                     }
-                v *= fabsf(__ldg(inv + tok));
+                v *= s_inv[t];
                 dst[at] = residual ? residual[at] + v : v;
             }
         }

@@ -237,10 +237,12 @@ __device__ __forceinline__ void f16_unit(const uint8_t* u0, const uint8_t* u1, c
 }
 
 // The two 16-byte pieces of a unit that lane l splits: they are what lane t = l % 4 of a quad multiplies in group l / 4.
-template <uint32_t TYPE>
+// xu: activations, which the kernel in front may have written, or the norm's weights.
+template <uint32_t TYPE, bool WEIGHTS = false>
 __device__ __forceinline__ void load_run(const float* xu, uint32_t lane, float (&v)[8]) {
     const uint32_t o0 = TYPE == T_MXFP4 ? (lane >> 2) * 32 + (lane & 3) * 4 : lane * 8, o1 = o0 + (TYPE == T_MXFP4 ? 16 : 4);
-    const float4 a = __ldg(reinterpret_cast<const float4*>(xu + o0)), b = __ldg(reinterpret_cast<const float4*>(xu + o1));
+    const float4 *p = reinterpret_cast<const float4*>(xu + o0), *q = reinterpret_cast<const float4*>(xu + o1);
+    const float4 a = WEIGHTS ? __ldg(p) : ld_behind(p), b = WEIGHTS ? __ldg(q) : ld_behind(q);
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
@@ -500,7 +502,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_f16_kernel(const __grid_const
         }
         for (uint32_t u = pu; u < U; u += NCW > U ? U : NCW) {
             float w[8];
-            if (ga.norm_w != nullptr) load_run<TYPE>(ga.norm_w + (uint64_t)(unit0 + u) * 256, lane, w);
+            if (ga.norm_w != nullptr) load_run<TYPE, true>(ga.norm_w + (uint64_t)(unit0 + u) * 256, lane, w);
             for (uint32_t r0 = pr; r0 < p_rows; r0 += 4 * pn) {
                 float v[4][8];
 #pragma unroll

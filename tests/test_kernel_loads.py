@@ -10,6 +10,8 @@ from tests.conftest import ROOT
 # by file: what may be read so all the same, weights and tables that no kernel of a step writes (pointers; in __ldg)
 FILES = {
     "gemv_mma.cu": (set(), {"src", "src + 1"}),   # of load_unit_values<WEIGHTS>
+    "gemv_f16.cu": (set(), {"p", "q"}),           # of load_run<WEIGHTS>
+    "gemm_f16.cu": ({"w_a", "w_b", "norm_w"}, {"nr + i", "nr + at"}),
 }
 
 
@@ -29,3 +31,7 @@ def test_the_activations_of_the_linears():
     text = source("gemv_mma.cu")
     assert len(re.findall(r"WEIGHTS \? __ldg\(src(?: \+ 1)?\) : ld_behind\(src(?: \+ 1)?\)", text)) == 2
     assert set(re.findall(r"load_unit_values<true>\((\w+)", text)) == {"norm_w", "nw"}
+    text = source("gemv_f16.cu")
+    assert len(re.findall(r"WEIGHTS \? __ldg\((\w)\) : ld_behind\(\1\)", text)) == 2
+    assert set(re.findall(r"load_run<TYPE, true>\(([\w.]+)", text)) == {"ga.norm_w"}
+    assert re.search(r"float4\* nr = reinterpret_cast<const float4\*>\(norm_w\)", source("gemm_f16.cu"))
