@@ -132,8 +132,7 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint32_t (&v)[
 
 template <uint32_t HD>
 __global__ void __launch_bounds__(A_THREADS, 1)
-    attention_prefill_kernel(const float* __restrict__ q, const float* __restrict__ cache_k, const float* __restrict__ cache_v,
-                             const int32_t* __restrict__ pos, uint32_t seq, uint32_t nq, uint32_t nkv, uint32_t max_ctx,
+    attention_prefill_kernel(const float* q, const float* cache_k, const float* cache_v, const int32_t* pos, uint32_t seq, uint32_t nq, uint32_t nkv, uint32_t max_ctx,
                              float* __restrict__ out, int32_t* __restrict__ bad_pos, int* __restrict__ error_flag) {
     using T = AttTile<HD>;
     extern __shared__ __align__(1024) uint8_t smem[];  // K and V stages | raw rows | AttShared
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(A_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem_slot;
-    pdl_wait();
+    pdl_wait();  // q, the cache and the position are read by plain loads: read-only ones may be moved above it
     // heads run fastest, the last queries first: they see the most keys, and a long CTA in the last wave leaves the
     // other SMs waiting
     const uint32_t head = blockIdx.x, kvh = head / (nq / nkv), s0 = (gridDim.y - 1 - blockIdx.y) * AQ;
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(A_THREADS, 1)
                 float amax = 0.0f;
 #pragma unroll
                 for (uint32_t i = 0; i < DN / 4; ++i) {
-                    const float4 v = sr < seq ? __ldg(src + i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    const float4 v = sr < seq ? src[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     o[4 * i] = v.x, o[4 * i + 1] = v.y, o[4 * i + 2] = v.z, o[4 * i + 3] = v.w;
                     amax = fmaxf(amax, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
                 }
@@ -335,7 +334,7 @@ __global__ void __launch_bounds__(A_THREADS, 1)
                 for (uint32_t t = sh.odd_first * AK; t < min(sh.odd_end * AK, visible) && sr < seq; ++t)
 #pragma unroll
                     for (uint32_t i = 0; i < DN; ++i) {
-                        const float v = __ldg(V + (uint64_t)t * HD + i);
+                        const float v = V[(uint64_t)t * HD + i];
                         if (!(fabsf(v) < INFINITY)) o[i] += v;
                     }
             }

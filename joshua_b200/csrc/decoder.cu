@@ -14,6 +14,8 @@ namespace jq {
 
 namespace {
 
+// What the kernel in front may have written is read by plain loads behind this: read-only ones (__ldg, or plain ones through const
+// __restrict__) may be moved above it.
 __device__ __forceinline__ void pdl_wait_() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float block_sum(float v, float* red) {
@@ -31,7 +33,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 // out[r, :] = rmsnorm(x[r, :] (+ res[r, :])) * w;  when res != NULL the sum is also written to sum_out
 // (the new residual stream).  One CTA of 1024 threads per row; each thread keeps its float4 pieces in
 // registers between the two passes (rows up to 16384 wide; wider rows re-read).
-__global__ void __launch_bounds__(1024) rmsnorm_kernel(const float* __restrict__ x, const float* __restrict__ res,
+__global__ void __launch_bounds__(1024) rmsnorm_kernel(const float* x, const float* res,
                                                        const float* __restrict__ w, float eps, uint32_t h,
                                                        float* __restrict__ sum_out, float* __restrict__ out,
                                                        uint32_t x_stride) {
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(const float* __restrict__
 // Rotary embedding (rotate-half pairing: element i pairs with i + hd/2) of the q and k parts of a fused
 // qkv row, then k and v are appended to the cache at position pos[b].
 //   qkv [B, (nq + 2*nkv) * hd];  q_out [B, nq*hd];  cache_k / cache_v [B, nkv, max_ctx, hd]
-__global__ void __launch_bounds__(128) rope_append_kernel(const float* __restrict__ qkv, const int32_t* __restrict__ pos,
+__global__ void __launch_bounds__(128) rope_append_kernel(const float* qkv, const int32_t* pos,
                                                           uint32_t nq, uint32_t nkv, uint32_t hd, uint32_t max_ctx,
                                                           float theta, float* __restrict__ q_out,
                                                           float* __restrict__ cache_k, float* __restrict__ cache_v,
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(128) rope_append_kernel(const float* __restric
 // above: same results.  Bound by L2: qkv was just written there, q and the cache rows are read next.
 // 512 tokens of 32 + 2 x 8 heads of 128: 20.5 -> 12.4 us, 2048: 41.9 -> 24.6 (with some 6 us of an empty launch).
 template <int PER>
-__global__ void __launch_bounds__(256) rope_append_rows_kernel(const float* __restrict__ qkv, const int32_t* __restrict__ pos,
+__global__ void __launch_bounds__(256) rope_append_rows_kernel(const float* qkv, const int32_t* pos,
                                                                uint32_t nq, uint32_t nkv, uint32_t max_ctx, float theta,
                                                                float* __restrict__ q_out, float* __restrict__ cache_k,
                                                                float* __restrict__ cache_v, int32_t* __restrict__ bad_pos,
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(256) rope_append_rows_kernel(const float* __re
         const float* src = qkv + ((uint64_t)b * heads + head) * HD + lane;
         float v[PER];
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = __ldg(src + 32 * j);
+        for (int j = 0; j < PER; ++j) v[j] = src[32 * j];
         if (head >= nq + nkv) {
             float* dst = cache_v + (((uint64_t)cb * nkv + (head - nq - nkv)) * max_ctx + p) * HD + lane;
 #pragma unroll
@@ -231,9 +233,8 @@ __global__ void __launch_bounds__(256) rope_append_rows_kernel(const float* __re
 constexpr uint32_t ATT_CHUNK = 64;
 
 // part[b, head, chunk, 0..hd-1] = sum_t exp(s_t - m) V[t, :];  part[.., hd] = m;  part[.., hd+1] = sum_t exp(s_t - m)
-__global__ void __launch_bounds__(128) attention_partial_kernel(const float* __restrict__ q, const float* __restrict__ cache_k,
-                                                                const float* __restrict__ cache_v,
-                                                                const int32_t* __restrict__ pos, uint32_t nq, uint32_t nkv,
+__global__ void __launch_bounds__(128) attention_partial_kernel(const float* q, const float* cache_k, const float* cache_v,
+                                                                const int32_t* pos, uint32_t nq, uint32_t nkv,
                                                                 uint32_t hd, uint32_t max_ctx, uint32_t n_chunks,
                                                                 float* __restrict__ part, int32_t* __restrict__ bad_pos,
                                                                 uint32_t dv, float scale) {
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(128) attention_partial_kernel(const float* __r
     }
 }
 
-__global__ void __launch_bounds__(128) attention_merge_kernel(const float* __restrict__ part, uint32_t hd, uint32_t n_chunks,
+__global__ void __launch_bounds__(128) attention_merge_kernel(const float* part, uint32_t hd, uint32_t n_chunks,
                                                               float* __restrict__ out) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     pdl_wait_();
@@ -337,8 +338,7 @@ __global__ void __launch_bounds__(ATT_FUSED_THREADS, HD > 128 || LOAD == ATT_ALL
 }
 
 // y = a + b
-__global__ void __launch_bounds__(256) add_kernel(const float* __restrict__ a, const float* __restrict__ b, uint64_t n,
-                                                  float* __restrict__ y) {
+__global__ void __launch_bounds__(256) add_kernel(const float* a, const float* b, uint64_t n, float* y) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     pdl_wait_();
     for (uint64_t i = blockIdx.x * (uint64_t)blockDim.x + threadIdx.x; i < n; i += (uint64_t)gridDim.x * blockDim.x)
@@ -384,8 +384,8 @@ constexpr uint32_t SAMPLE_WINDOW = 64;
 
 __global__ void __launch_bounds__(256) argmax_slices_kernel(float* __restrict__ logits, uint32_t vocab,
                                                             float* __restrict__ part_v, uint32_t* __restrict__ part_i,
-                                                            float penalty, const int32_t* __restrict__ window,
-                                                            const int32_t* __restrict__ win_state) {
+                                                            float penalty, const int32_t* window,
+                                                            const int32_t* win_state) {
     __shared__ float sv[8];
     __shared__ uint32_t si[8];
     __shared__ int32_t s_win[SAMPLE_WINDOW];
@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(256) argmax_slices_kernel(float* __restrict__ 
     }
 }
 
-__global__ void __launch_bounds__(64) argmax_final_kernel(const float* __restrict__ part_v, const uint32_t* __restrict__ part_i,
+__global__ void __launch_bounds__(64) argmax_final_kernel(const float* part_v, const uint32_t* part_i,
                                                           int32_t* __restrict__ token, int32_t* __restrict__ pos,
                                                           int32_t* __restrict__ window, int32_t* __restrict__ win_state) {
     __shared__ float sv[2];
@@ -511,8 +511,8 @@ size_t attention_scratch_bytes(uint32_t batch, uint32_t nq, uint32_t hd, uint32_
 // k_pe, then K[pos] = [k_nope of the head | k_pe] and V[pos] = v of the head appended to the per-head caches.
 //   q [B, nh * (nope + rope)] in place;  comp [B, comp_stride], k_pe = comp[kv_lora ..];  kv [B, nh * (nope + vd)];
 //   cache_k [B, nh, max_ctx, nope + rope];  cache_v [B, nh, max_ctx, vd].
-__global__ void __launch_bounds__(128) mla_assemble_kernel(float* __restrict__ q, const float* __restrict__ comp,
-                                                           const float* __restrict__ kv, const int32_t* __restrict__ pos,
+__global__ void __launch_bounds__(128) mla_assemble_kernel(float* __restrict__ q, const float* comp,
+                                                           const float* kv, const int32_t* pos,
                                                            uint32_t nh, uint32_t nope, uint32_t rope, uint32_t vd,
                                                            uint32_t kv_lora, uint32_t max_ctx,
                                                            const float* __restrict__ inv_freq, float mscale,

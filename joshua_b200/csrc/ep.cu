@@ -104,9 +104,9 @@ __device__ bool publish(uint32_t* done, const Window& win, uint64_t flag_off, ui
 
 // grid = P + world CTAs.  CTA p < P stores pair p's activation row and local expert id into its owner's
 // window; CTA P + d marks the unused slots of my block on rank d.  pair_slot[p] = owner * cap + slot.
-__global__ void __launch_bounds__(256) ep_dispatch_kernel(Window win, Layout l, uint32_t me, const float* __restrict__ x,
+__global__ void __launch_bounds__(256) ep_dispatch_kernel(Window win, Layout l, uint32_t me, const float* x,
                                                           const float* __restrict__ norm_w, float eps,
-                                                          const uint32_t* __restrict__ ids, uint32_t T, uint32_t K,
+                                                          const uint32_t* ids, uint32_t T, uint32_t K,
                                                           uint32_t* __restrict__ pair_slot, uint32_t* __restrict__ epoch,
                                                           uint32_t* __restrict__ done, uint32_t polls, int* status) {
     __shared__ uint32_t s_red[8];
@@ -188,11 +188,11 @@ __global__ void __launch_bounds__(256) ep_dispatch_kernel(Window win, Layout l, 
 // after every owner's return of this epoch has arrived.  The return CTAs wait for nothing and come first in the
 // grid, so the combine CTAs' (bounded) wait never keeps them from running, whatever the grid's size.
 __global__ void __launch_bounds__(256) ep_return_combine_kernel(Window win, Layout l, uint32_t me, uint32_t n_rows,
-                                                                const float* __restrict__ out_list,
-                                                                const uint32_t* __restrict__ inv,
-                                                                const uint32_t* __restrict__ pair_slot,
-                                                                const float* __restrict__ wts, uint32_t T, uint32_t K,
-                                                                const uint32_t* __restrict__ epoch, uint32_t* __restrict__ done,
+                                                                const float* out_list,
+                                                                const uint32_t* inv,
+                                                                const uint32_t* pair_slot,
+                                                                const float* wts, uint32_t T, uint32_t K,
+                                                                const uint32_t* epoch, uint32_t* __restrict__ done,
                                                                 const float* residual, float* y, uint32_t polls, int* status) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x < n_rows) {

@@ -20,7 +20,7 @@ struct JobsSmem {
 
 // Body of the job builder for the `nthreads` threads of one CTA (tid = 0 .. nthreads - 1, whole warps).
 template <class Sync>
-__device__ __forceinline__ void build_jobs(const uint32_t* __restrict__ ids, uint32_t T, uint32_t K, uint32_t E,
+__device__ __forceinline__ void build_jobs(const uint32_t* ids, uint32_t T, uint32_t K, uint32_t E,
                                            uint32_t rows_per_job, uint32_t* __restrict__ list_token,
                                            uint32_t* __restrict__ inv, MoeJob* __restrict__ jobs,
                                            uint32_t* __restrict__ n_jobs, uint32_t* __restrict__ n_list,
@@ -91,7 +91,7 @@ struct JobsSmallSmem {
 };
 
 template <class Sync>
-__device__ __forceinline__ void build_jobs_small(const uint32_t* __restrict__ ids, uint32_t T, uint32_t K, uint32_t E,
+__device__ __forceinline__ void build_jobs_small(const uint32_t* ids, uint32_t T, uint32_t K, uint32_t E,
                                                  uint32_t rows_per_job, uint32_t* __restrict__ list_token,
                                                  uint32_t* __restrict__ inv, MoeJob* __restrict__ jobs,
                                                  uint32_t* __restrict__ n_jobs, uint32_t* __restrict__ n_list,
