@@ -237,10 +237,14 @@ class _Paged:
         n, others = len(token_ids), range(1, self.batch)
         full, pages = n // PAGE, -(-n // PAGE)
         # what sequences have reserved stays theirs, but for the pages in whose place the common ones stand
-        wanted = max(0, pages - len(self.owned[0])) + sum(max(0, pages - max(full, len(self.owned[i]))) for i in others)
-        back = sum(page is not None for i in others for page in self.owned[i][:full])
-        if wanted > len(self.free) + back:
-            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {len(self.free) + back} of {self.n_pages} are free")
+        wanted, free = sum(max(0, pages - max(full, len(self.owned[i]))) for i in others), len(self.free)
+        if self.attention_window:   # pages go back while the prompt is read
+            free = self._room_for_parts(0, n)
+        else:
+            wanted += max(0, pages - len(self.owned[0]))
+        free += sum(page is not None for i in others for page in self.owned[i][:full])
+        if wanted > free:
+            raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{wanted} pages wanted, {free} of {self.n_pages} are free")
         self._prompt(token_ids, 0)
         common, rest = self.owned[0][:full], self.owned[0][full:]
         for i in others:
@@ -499,8 +503,9 @@ class _Paged:
         self.pos[i] = self.held[i] - 1
         return ids.numel()
 
-    def _room_for_parts(self, i, n: int) -> None:
-        """Raises, before any part is taken, if they do not fit: what each part takes and the window gives back."""
+    def _room_for_parts(self, i, n: int) -> int:
+        """Pages that are free behind all parts: what each takes and the window gives back.  Raises, before any is taken, if one does not
+        fit."""
         if self.held[i] + n > self.max_ctx:
             raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{self.held[i] + n} positions in a decoder of {self.max_ctx}")
         mine = [page is not None and self.holders[page] == 1 for page in self.owned[i]]   # whether it goes back to the pool
@@ -517,6 +522,7 @@ class _Paged:
                 raise JoshuaB200Error(_lib.E_TOO_LARGE, f"{more} pages wanted, {free} of {self.n_pages} are free")
             free -= more
             mine += [True] * more
+        return free
 
     # ── a token of every sequence ───────────────────────────────────────
     def step(self, stream=None) -> None:

@@ -1,0 +1,55 @@
+"""Prompts behind attention windows whose pages go back while they are read."""
+import pytest
+
+from joshua_b200._lib import JoshuaB200Error
+from tests.test_gpu_paged_decoder import ids, make
+from tests.test_gpu_paged_extend import near
+
+pytestmark = pytest.mark.gpu
+
+
+def windowed(batch, n_pages=None):
+    dec = make(batch, max_ctx=2000, n_pages=n_pages, attention_window=100, attention_sinks=4)
+    dec.prompt_rows = 120
+    return dec
+
+
+@pytest.mark.parametrize("n,pages", [(1500, 8), (1536, 6), (30, 3)])   # ends within a page, at a page's end, in the first one
+def test_a_long_shared_prompt_through_a_small_pool(n, pages):
+    small, wide = windowed(3, pages), windowed(3)
+    for dec in (small, wide):
+        dec.share_prompt(ids(n, 3))
+        assert dec.held == [n] * 3
+    near(small.logits, wide.logits)
+    for _ in range(2):
+        wide.token.copy_(small.token)
+        if n == 1500:
+            small.step(), wide.step()
+            near(small.logits, wide.logits)
+    for i in range(3):
+        small.release(i)
+    assert sorted(small.free) == list(range(pages))
+    small.check_flags(), wide.check_flags()
+
+
+def test_one_that_does_not_fit_is_refused_whole():
+    dec = windowed(3, 6)
+    for bad in (1500, 1996, 2001):    # one page too few for the others' ends; past max_ctx
+        free, table = list(dec.free), dec.table.clone()
+        with pytest.raises(JoshuaB200Error):
+            dec.share_prompt(ids(bad, 3))
+        assert dec.held == [0] * 3 and dec.free == free and bool((dec.table == table).all()) and dec.owned == [[], [], []]
+    dec.share_prompt(ids(1472, 3))    # a page's end: nothing is copied
+    assert dec.held == [1472] * 3
+    dec.check_flags()
+
+
+def test_reserved_pages_go_back_for_the_common_ones():
+    dec = windowed(3, 9)
+    dec.reserve(1, 128), dec.reserve(2, 64)
+    dec.share_prompt(ids(1472, 3))
+    assert dec.held == [1472] * 3 and dec.owned[1] == dec.owned[2] == dec.owned[0]
+    for i in range(3):
+        dec.release(i)
+    assert sorted(dec.free) == list(range(9))
+    dec.check_flags()
