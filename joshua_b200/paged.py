@@ -103,12 +103,13 @@ class _Paged:
         return dict(cache=PagedCache(self.kv_type, self.cfg.kv_heads, self.cfg.head_dim, n_pages=self.n_pages + -(-self.batch // self._places),
                                      device=self.dev))
 
-    def _attention_scratch(self) -> None:
-        """One scratch for the attention of all layers; one that a caller's graph may hold stays until the decoder goes."""
+    def _attention_scratch(self, rows: int | None = None) -> None:
+        """One scratch for the attention of all layers, of steps and of passes of so many `rows`; one that a caller's graph may hold stays
+        until the decoder goes."""
         c, old = self.cfg, getattr(self, "att_scratch", [])
         cache = self.layers[0]["cache"]
-        if self.attention_window:
-            need = cache.scratch_bytes(self.batch, c.q_heads, rows=self.batch)
+        if rows or self.attention_window:
+            need = cache.scratch_bytes(self.batch, c.q_heads, rows=rows or self.batch)
         else:
             need = cache.scratch_bytes(self.batch, c.q_heads, self.shared_pages)
         if not old or old[-1].numel() < need:
@@ -431,13 +432,15 @@ class _Paged:
         first = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], **i32)
         lens = torch.tensor([self.held[i] + n for i, n in enumerate(counts)], **i32)
         x, qkv, att = torch.empty(S, h, **f32), torch.empty(S, c.qkv_rows, **f32), torch.empty(S, c.q_heads * c.head_dim, **f32)
+        self._attention_scratch(S)
         check(L.jq_embedding_dev(self.embed._h, P(ids), S, c.vocab, h, P(x), P(self.bad), s))
         for ly in self.layers:
             cache = ly["cache"]
             check(L.jq_matmul_norm_dev(ly["wqkv"]._h, S, h, c.qkv_rows, P(x), P(ly["attn_norm"]), c.eps, None, P(qkv), s))
             q = cache.append(qkv, pos, self.table, n_q=c.q_heads, seq=seq, rope=self.rope,
                              q_norm=ly["q_norm"] if self.qk_norm else None, k_norm=ly["k_norm"] if self.qk_norm else None, eps=c.eps)
-            cache.attend_chunk(q, lens, self.table, n_q=c.q_heads, first=first, window=self.attention_window, sinks=self.attention_sinks, out=att)
+            cache.attend_chunk(q, lens, self.table, n_q=c.q_heads, first=first, window=self.attention_window, sinks=self.attention_sinks, out=att,
+                               scratch=self.att_scratch[-1])
             check(L.jq_matmul_norm_dev(ly["wo"]._h, S, c.q_heads * c.head_dim, h, P(att), None, 0.0, P(x), P(x), s))
             self._ffn_prefill(ly, x, S, s)
         for i, n in enumerate(counts):

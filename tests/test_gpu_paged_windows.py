@@ -53,3 +53,19 @@ def test_reserved_pages_go_back_for_the_common_ones():
         dec.release(i)
     assert sorted(dec.free) == list(range(9))
     dec.check_flags()
+
+
+@pytest.mark.parametrize("window", [0, 100])
+def test_one_scratch_for_all_layers_of_a_pass(window):
+    import torch
+
+    from tests.test_gpu_paged_decoder import config
+
+    dec = make(2, cfg=config(layers=6), attention_window=window)
+    need = dec.layers[0]["cache"].scratch_bytes(2, 8, rows=200)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    dec.extend({0: ids(150, 1), 1: ids(50, 2)}), dec.prefill(ids(90, 3)), dec.step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - before < 2 * need   # 20 MB; of every layer's own, six times that
+    dec.check_flags()
