@@ -39,9 +39,6 @@ constexpr uint32_t C_SOFT = 4, C_SUM = 4, C_CONV = 8;  // warps
 constexpr uint32_t C_FIRST_CONV = C_SOFT + C_SUM, C_ISSUE = C_FIRST_CONV + C_CONV, C_LOAD = C_ISSUE + 1;
 constexpr int UP = 6;                        // probabilities stand times 2^UP ..
 constexpr float LAZY = 8.0f;                 // .. and are up to 2^LAZY: below 2^15
-// Scores are multiplied and shifted in one step, exact but for the shift itself: with maxima from here on, whose last bit may be worth
-// more than LAZY leaves, they are rounded as the maximum was and shifted by it first, in a step of their own.
-constexpr float FAR = 0x1p20f;
 constexpr uint32_t C_HALF = C_CONV / 2;                // of the converters: for keys, the others for values
 constexpr uint32_t C_THREADS = (C_ISSUE + 4) * 32;  // whole warpgroups: they trade registers
 // Registers a thread: the launch has 640 x 96 = 61440, of which the issuer's warpgroup keeps 128 x 32, the softmax threads (32 scores, 32

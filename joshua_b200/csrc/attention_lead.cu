@@ -216,10 +216,19 @@ __global__ void __launch_bounds__(L_THREADS, 1) attention_lead_tiles_kernel(Page
             }
             sh.row[j & 1][half][row] = cm;
             pair_bar();
-            const float t = fmaxf(cm, sh.row[j & 1][half ^ 1][row]) * f;
+            const float t = __fmul_rn(fmaxf(cm, sh.row[j & 1][half ^ 1][row]), f);
             float alpha = 1.0f;
-            if (t > mx + LAZY) alpha = ex2(mx - t), mx = t;  // 0 on the first tile (mx = -inf)
-            const f32x2 ff = pair(f, f), shift = pair((float)UP - mx, (float)UP - mx);
+            if (fabsf(mx) < FAR ? t > mx + LAZY : t - mx > LAZY) alpha = ex2(mx - t), mx = t;  // 0 on the first tile (mx = -inf)
+            float by = f, base = (float)UP - mx;
+            if (__any_sync(0xFFFFFFFFu, fabsf(mx) >= FAR)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 v = both(sc[i]);
+                    sc[i] = pair(__fsub_rn(__fmul_rn(v.x, f), mx), __fsub_rn(__fmul_rn(v.y, f), mx));
+                }
+                by = 1.0f, base = (float)UP;
+            }
+            const f32x2 ff = pair(by, by), shift = pair(base, base);
             f32x2 ps = 0;
             uint32_t w0[16], w1[16];
 #pragma unroll

@@ -10,6 +10,11 @@ namespace jq {
 
 namespace {
 
+// Scores are multiplied and shifted by their maximum in one step, exact but for the shift itself: with maxima from here on, whose last bit
+// may be worth more than the probabilities' terms have room for, they are rounded as the maximum was and shifted by it first, in a step
+// of their own.
+constexpr float FAR = 0x1p20f;
+
 __device__ __forceinline__ void sts_v4(uint32_t addr, const uint32_t (&v)[4]) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
