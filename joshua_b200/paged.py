@@ -281,6 +281,8 @@ class _Paged:
         new = {self._index(i): torch.as_tensor(ids, dtype=torch.int32).reshape(-1) for i, ids in sorted(tokens.items())}
         if not new or any(ids.numel() == 0 for ids in new.values()):
             raise JoshuaB200Error(_lib.E_INVALID, "nothing to extend, or an empty prompt")
+        if len({ids.device for ids in new.values()}) > 1:
+            new = {i: ids.to(self.dev) for i, ids in new.items()}
         if scores is not None and not 0 <= scores <= 32:
             raise JoshuaB200Error(_lib.E_INVALID, f"{scores} alternatives: 0 to 32")
         self._can_prompt(dense=False)

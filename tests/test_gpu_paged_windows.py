@@ -69,3 +69,14 @@ def test_one_scratch_for_all_layers_of_a_pass(window):
     torch.cuda.synchronize()
     assert torch.cuda.memory_allocated() - before < 2 * need   # 20 MB; of every layer's own, six times that
     dec.check_flags()
+
+
+def test_ids_from_the_host_and_the_device():
+    import torch
+
+    a, b = make(3), make(3)
+    prompts = {0: ids(70, 1), 1: ids(5, 2), 2: ids(33, 3)}
+    want = a.extend(prompts, scores=2)
+    got = b.extend({0: torch.tensor(prompts[0], device="cuda"), 1: prompts[1], 2: torch.tensor(prompts[2])}, scores=2)
+    assert bool((a.logits == b.logits).all()) and a.held == b.held == [70, 5, 33]
+    assert all(bool((x == y).all()) for i in want for x, y in zip(want[i], got[i]))
