@@ -80,3 +80,18 @@ def test_ids_from_the_host_and_the_device():
     got = b.extend({0: torch.tensor(prompts[0], device="cuda"), 1: prompts[1], 2: torch.tensor(prompts[2])}, scores=2)
     assert bool((a.logits == b.logits).all()) and a.held == b.held == [70, 5, 33]
     assert all(bool((x == y).all()) for i in want for x, y in zip(want[i], got[i]))
+
+
+def test_the_serving_command_gives_pages_back():
+    """The pages that a run behind a window holds at its end: those of the sinks and of the window, fewer than without one."""
+    from joshua_b200.llama import LlamaConfig
+    from joshua_b200.serve import run
+
+    cfg = LlamaConfig(layers=2, hidden=1024, q_heads=8, kv_heads=2, head_dim=128, ffn=2048, vocab=2048)
+    more = dict(batch=3, prompt=500, tokens=200, kv="q8_0", layers=2, cfg=cfg)
+    plain = run(**more)
+    assert plain["pages_used"] == 7 + 3 * 4        # 448 positions in common, reserved up to 701
+    for window, sinks in ((64, 2), (130, 0)):
+        used = run(**more, window=window, sinks=sinks)["pages_used"]
+        # a step has made room for itself before it takes its page
+        assert used <= 3 * (-(-sinks // 64) + (window - 1) // 64 + 2) < plain["pages_used"]
