@@ -23,6 +23,24 @@ from .sampling import log_probs
 PASS_ROWS = 16384   # prompt tokens of several sequences in one pass
 
 
+def score_prompts(dec, ids: list, alternatives: int) -> dict:
+    """Reads one prompt into every sequence, several at a time, one longer than PASS_ROWS in parts; by sequence, what `sampling.log_probs`
+    gives for its tokens but the first."""
+    scores: dict = {}
+    some = max(1, PASS_ROWS // len(ids))
+    for i in range(0, dec.batch, some):
+        sequences = range(i, min(dec.batch, i + some))
+        for at in range(0, len(ids), PASS_ROWS):
+            part = ids[at:at + PASS_ROWS]
+            if at:   # its first token, by the logits that the part before it has left
+                first = torch.tensor(part[:1], dtype=torch.int32, device=dec.dev)
+                for k in sequences:
+                    scores[k].append(log_probs(dec.logits[k:k + 1], first, top=alternatives))
+            for k, got in dec.extend({k: part for k in sequences}, scores=alternatives).items():
+                scores.setdefault(k, []).append(got)
+    return {k: tuple(torch.cat(t) for t in zip(*parts)) for k, parts in scores.items()}
+
+
 def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float = 1.0, own_prompts: bool = False, cfg=None, window: int = 0,
         sinks: int = 0, logprobs: int | None = None) -> dict:
     cfg = cfg or LlamaConfig(layers=layers)
@@ -42,9 +60,7 @@ def run(batch: int, prompt: int, tokens: int, kv: str, layers: int, yarn: float 
         for i in range(batch):
             dec.prefill(ids, sequence=i)
     elif own_prompts:
-        some = max(1, PASS_ROWS // prompt)
-        for i in range(0, batch, some):
-            scores.update(dec.extend({k: ids for k in range(i, min(batch, i + some))}, scores=logprobs))
+        scores = score_prompts(dec, ids, logprobs)
     else:
         dec.share_prompt(ids)
     if not window:   # steps take a page now and then otherwise, and give one back

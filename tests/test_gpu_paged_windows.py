@@ -95,3 +95,23 @@ def test_the_serving_command_gives_pages_back():
         used = run(**more, window=window, sinks=sinks)["pages_used"]
         # a step has made room for itself before it takes its page
         assert used <= 3 * (-(-sinks // 64) + (window - 1) // 64 + 2) < plain["pages_used"]
+
+
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("rows", [150, 64, 40, 7])
+def test_scores_of_a_prompt_in_parts(monkeypatch, window, rows):
+    """The serving command's prompts that are longer than a pass: what is scored does not depend on the parts, but for the rounding of
+    passes of other row counts (tests/test_gpu_paged_extend.py derives 2^-6 of a logit's size where the cache was filled otherwise): log
+    probabilities are off by twice that."""
+    from joshua_b200 import serve
+
+    once, parts = (make(3, attention_window=window) for _ in range(2))
+    prompt = ids(150, 1)
+    want = serve.score_prompts(once, prompt, 2)
+    monkeypatch.setattr(serve, "PASS_ROWS", rows)
+    got = serve.score_prompts(parts, prompt, 2)
+    assert parts.held == once.held == [150] * 3 and sorted(got) == [0, 1, 2]
+    spread = 2 * 2.0**-6 * float(once.logits.abs().max())
+    for i in range(3):
+        assert [list(t.shape) for t in got[i]] == [[149], [149], [149, 2], [149, 2]]
+        assert float((got[i][0] - want[i][0]).abs().max()) <= spread and float((got[i][3] - want[i][3]).abs().max()) <= spread
