@@ -85,6 +85,7 @@ struct ChunkShared {
     int abort_flag;
     uint32_t last;            // this CTA was the last one to bring its part of a tile
     uint32_t scan[2][C_CONV], first_seg, end_seg;
+    uint32_t named[C_SOFT], named_too[C_CONV];  // rows of all sequences, by warp: of the softmax, of the converters
     uint32_t pieces, batches;  // pieces of this batch; batches
     float4 stage[2][4][32][C_STAGE];  // of the softmax warps and of the output's: 16 dimensions of 32 rows on their way between lanes
     ChunkPiece piece[C_PIECES];
@@ -363,10 +364,7 @@ struct TilePages {
     }
 };
 // rows of a sequence that this kernel takes
-__device__ __forceinline__ uint32_t tile_rows(const PagedArgs& a, uint32_t b) {
-    const SequenceRows s = sequence_rows(a, b);
-    return s.n <= a.span.few || s.len <= 0 ? 0 : s.n;
-}
+__device__ __forceinline__ uint32_t tile_rows(const PagedArgs& a, const SequenceRows& s) { return s.n <= a.span.few || s.len <= 0 ? 0 : s.n; }
 
 template <uint32_t KIND, uint32_t HD>
 __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(PagedArgs a, int* error_flag) {
@@ -426,7 +424,14 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
     if (warp < C_SOFT) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C_REGS_SOFT));
         // rows of sequences without positions, or with ones out of range
-        const bool fit = rows_fit(a, lane);
+        uint32_t named = 0;
+        for (uint32_t b = tid; b < batch; b += C_SOFT * 32) named += sequence_rows(a, b).n;
+        named = __reduce_add_sync(0xFFFFFFFFu, named);
+        if (lane == 0) sh.named[warp] = named;
+        asm volatile("bar.sync 4, %0;" ::"n"(C_SOFT * 32) : "memory");
+        named = 0;
+        for (uint32_t w = 0; w < C_SOFT; ++w) named += sh.named[w];
+        const bool fit = rows_fit(a, named);
         for (uint32_t b = blockIdx.x; b < batch; b += gridDim.x) {
             const SequenceRows sq = sequence_rows(a, b);
             if ((!fit || sq.lost || sq.len < 0) && tid == 0 && a.bad_pos) atomicExch(a.bad_pos, 1);
@@ -800,12 +805,19 @@ __global__ void __launch_bounds__(C_THREADS, 1) attention_chunk_tiles_kernel(Pag
         uint32_t n_tiles = 0, total = 0;
         {
             const uint32_t per = (batch + C_CONV * 32 - 1) / (C_CONV * 32), b0 = min(batch, ct * per), b1 = min(batch, b0 + per);
-            uint32_t mine = 0;
-            const bool fit = rows_fit(a, lane);  // if not, nobody has tiles
-            auto tiles_of = [&](uint32_t b) { return fit ? ChunkTiles(a, tile_rows(a, b)).tiles : 0; };
-            for (uint32_t b = b0; b < b1; ++b) mine += tiles_of(b);
+            uint32_t mine = 0, named = 0;
+            for (uint32_t b = b0; b < b1; ++b) {
+                const SequenceRows s = sequence_rows(a, b);
+                named += s.n, mine += ChunkTiles(a, tile_rows(a, s)).tiles;
+            }
+            named = __reduce_add_sync(0xFFFFFFFFu, named);
+            if (lane == 0) sh.named_too[cw] = named;
             uint32_t run = scan(mine, 0, &n_tiles);
-            for (uint32_t b = b0; b < b1; ++b) s_tiles[b] = run, run += tiles_of(b);
+            named = 0;
+            for (uint32_t w = 0; w < C_CONV; ++w) named += sh.named_too[w];
+            const bool fit = rows_fit(a, named);
+            if (!fit) run = n_tiles = 0;  // nobody has tiles
+            for (uint32_t b = b0; b < b1; ++b) s_tiles[b] = run, run += fit ? ChunkTiles(a, tile_rows(a, sequence_rows(a, b))).tiles : 0;
             if (ct == 0) s_tiles[batch] = n_tiles, sh.first_seg = 0, sh.end_seg = 0;
             asm volatile("bar.sync 7, %0;" ::"n"(C_CONV * 32) : "memory");
         }

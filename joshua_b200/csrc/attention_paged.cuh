@@ -80,17 +80,9 @@ __device__ __forceinline__ SequenceRows sequence_rows(const PagedArgs& a, uint32
     return s;
 }
 // Whether the sequences' rows together are as few as the host allows a call, so that sums of their steps and tiles hold in 32 bits: a
-// `first` that goes up and down names rows many times.  A warp, all of it.
-__device__ __forceinline__ bool rows_fit(const PagedArgs& a, uint32_t lane) {
-    if (!a.span.first) return true;
-    uint32_t n = 0;
-#pragma unroll 4
-    for (uint32_t b = lane; b < a.c.n_seq; b += 32) {
-        const int32_t r0 = a.span.first[b], r1 = a.span.first[b + 1];
-        n += r0 < 0 || r1 < r0 || (uint32_t)r1 > a.span.rows ? 0 : r1 - r0;
-    }
-    n = __reduce_add_sync(0xFFFFFFFFu, n);
-    return span_rows_fit(n, a.c.table_stride, a.n_q);
+// `first` that goes up and down names rows many times.  named: `sequence_rows(..).n` of all, summed up.
+__device__ __forceinline__ bool rows_fit(const PagedArgs& a, uint32_t named) {
+    return !a.span.first || span_rows_fit(named, a.c.table_stride, a.n_q);
 }
 // What a row sees: positions below `end`, from `low` on or below `sinks`.
 struct Sight {

@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     constexpr uint32_t HD = T::HD, ROWS = At::Q::ROWS, PIECE = ROWS * (HD + 2);
     extern __shared__ __align__(16) uint32_t s_mem[];
     __shared__ uint32_t s_seg[2 * WARPS], s_from[2 * WARPS], s_to[2 * WARPS], s_scan[WARPS], s_most[WARPS], s_last[2], s_first[2];
-    __shared__ uint32_t s_seq[SPAN ? 2 * WARPS : 1];
+    __shared__ uint32_t s_seq[SPAN ? 2 * WARPS : 1], s_named[SPAN ? WARPS : 1];
     uint32_t* s_cum = s_mem;                                                       // [batch + 1] units of a head group in front of a sequence
     float* s_piece = reinterpret_cast<float*>(s_mem + ((a.c.n_seq + 4) & ~3u));    // [WARPS][2][PIECE]
     uint32_t* s_q = reinterpret_cast<uint32_t*>(s_piece + WARPS * 2 * PIECE);      // [WARPS] query operands
@@ -621,15 +621,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     if (tid < 2 * WARPS) s_seg[tid] = 0xFFFFFFFFu;
     // running sum of the sequences' units, a run of sequences a thread
     const uint32_t per = (batch + WARPS * 32 - 1) / (WARPS * 32), b0 = min(batch, tid * per), b1 = min(batch, b0 + per);
-    uint32_t mine = 0, most = 0;
+    uint32_t mine = 0, most = 0, named = 0;
     bool fit = true;
-    if constexpr (SPAN) fit = rows_fit(a, lane);
     auto units_of = [&](uint32_t b) {
         uint32_t steps, rows = 1;
         if constexpr (SPAN) {
             const SequenceRows sq = sequence_rows(a, b);
             steps = fit && sq.n <= a.span.few ? steps_a_row<T>(a, sq) : 0, rows = sq.n;
-            most = max(most, steps ? steps + SEG_UNITS : 0);
+            most = max(most, steps ? steps + SEG_UNITS : 0), named += sq.n;
         } else {
             steps = (uint32_t)(max(own_positions(a, b), 0) + T::POS - 1) / T::POS;
         }
@@ -648,9 +647,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
         run += lane >= o ? up : 0;
     }
     if (lane == 31) s_scan[warp] = run, s_most[warp] = most;
+    if constexpr (SPAN) {
+        named = __reduce_add_sync(0xFFFFFFFFu, named);
+        if (lane == 0) s_named[warp] = named;
+    }
     __syncthreads();
     for (uint32_t w = 0; w < WARPS; ++w) run += w < warp ? s_scan[w] : 0, most = max(most, s_most[w]);
     run -= mine;
+    auto all_fit = [&] {
+        uint32_t n = 0;
+        for (uint32_t w = 0; w < WARPS; ++w) n += SPAN ? s_named[w] : 0;
+        return rows_fit(a, n);
+    };
+    if constexpr (SPAN) {
+        fit = all_fit();
+        if (!fit) run = 0, most = 0;  // nobody has units
+    }
     for (uint32_t b = b0; b < b1; ++b) {
         s_cum[b] = run;
         run += units_of(b);
@@ -907,6 +919,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_paged_kernel(PagedArg
     }
     if constexpr (SPAN) {
         // sequences without positions, or with ones out of range
+        const bool fit = all_fit();  // again: the loops above have no register left
         for (uint32_t sb = blockIdx.x; sb < batch; sb += gridDim.x) {
             if (s_cum[sb + 1] != s_cum[sb]) continue;
             const SequenceRows sq = sequence_rows(a, sb);
