@@ -3,9 +3,10 @@
 // Rows first[b] .. first[b + 1] - 1 of q are the last positions of sequence b.  Row r at position p: out[r, head, :] =
 // sum_t e_t V_t / sum_t e_t, e_t = exp(scale q . K_t - max), over t <= p with (no window, or p - t < window, or t < sinks).
 // Sequences of few rows, and all with heads of 256, are taken row by row, each as a sequence of its own by attention_paged_kernel
-// (attention_steps.cuh), cut into equal pieces of work whatever the lengths: the codes of its positions are read once a row.  The
+// (attention_steps.cuh), cut into equal pieces of work whatever the lengths: the codes of its positions are read once a row.  (So a prompt
+// with heads of 256 takes as long as its rows: 2000 behind 2000, 16 heads on 4 in eight bits, 2.27 ms; 8 on 2 in halves 0.97.)  The
 // others go to the tiles of attention_chunk_tiles.cu.  Which are which is known on the device alone where `first` tells: both are
-// launched then, and each leaves the other's sequences.
+// launched then, one after the other, and each leaves the other's sequences (four tokens of 32 sequences: 122 us, with `first` 137).
 #include <algorithm>
 
 #include "attention_chunk.cuh"

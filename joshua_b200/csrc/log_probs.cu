@@ -16,8 +16,9 @@
 // in between, they learn at barriers: results do not depend on who comes first.
 //
 // Many rows are bounded by the one read of the logits (1000 rows of 128256: 84 us, 6.1 TB/s; blocks of 512 threads, two an SM, 99 us:
-// their barriers stop more of an SM at a time), few rows by the steps from the launch to the end of a row (1 of 128256, 5 likeliest: 9.8 us,
-// of which the tiles take half; 64 of 151936: 11.5 us, with the 20 likeliest 20.8 us).
+// their barriers stop more of an SM at a time; four blocks an SM leave 64 registers a thread, with which 8 bytes spill), few rows by the
+// steps from the launch to the end of a row (1 of 128256, 5 likeliest: 9.8 us, of which the tiles take half; 64 of 151936: 11.5 us, with
+// the 20 likeliest 20.8 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
